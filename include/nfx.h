@@ -345,6 +345,76 @@ int nfx_fp8_e4m3_fake_quant_host(const float* x, float scale, float* y, int64_t 
  * (0 expected).  Synchronous. */
 int nfx_fp8_e4m3_selfcheck(unsigned long long* mismatches);
 
+/* ---- A pre-norm FP8 linear layer: layer norm, block quantiser, block-scaled product --
+ * Operators of one transformer layer, forward and backward, for callers that hold their
+ * tensors on the GPU.  No counterpart in the reference (its LayerNorm and Linear exist
+ * inside TokenMixer::Forward only, cpp/src/fno.cpp:1418-1438, and its 8-bit forms are
+ * per tensor or per channel).  All pointers are DEVICE pointers on the current device,
+ * except where NULL is allowed; calls are asynchronous on `stream`, allocate nothing and
+ * keep nothing between calls.  Matrices are row-major with a row stride in elements
+ * ("ld..."); a matrix of one row has no use for it.  Refused arguments give
+ * NFX_INVALID_ARG and a message in nfx_last_error(). */
+enum { NFX_F32 = 0, NFX_BF16 = 1, NFX_F16 = 2 };
+
+/* Layer norm over the last dimension of x (rows, d):
+ *   y = (x - mean) rstd gamma + beta,  rstd = 1 / sqrt(var + eps), var the biased variance.
+ * y has x's type; gamma and beta (d,) have param_type, NULL: ones and zeros.  mean and rstd
+ * (rows,) are written where not NULL (the backward pass reads them).  Statistics in fp32. */
+int nfx_layer_norm(const void* x, int x_type, int64_t ldx, const void* gamma, const void* beta, int param_type,
+                   int64_t rows, int64_t d, float eps, void* y, int64_t ldy, float* mean, float* rstd,
+                   void* stream);
+
+/* The same layer norm with y in FP8, as nfx_fp8_quantise with tile = 0 would make it from an
+ * fp32 y: codes (rows, d), scales (rows, ceil(d / 128)) at r * scale_row_stride + b *
+ * scale_block_stride. */
+int nfx_layer_norm_fp8(const void* x, int x_type, int64_t ldx, const void* gamma, const void* beta,
+                       int param_type, int64_t rows, int64_t d, float eps, uint8_t* codes, int64_t ld_codes,
+                       float* scales, int64_t scale_row_stride, int64_t scale_block_stride, float* mean,
+                       float* rstd, void* stream);
+
+/* Gradient of nfx_layer_norm: with a = gamma dy and xh = (x - mean) rstd,
+ *   dx = rstd (a - mean(a) - xh mean(a xh)),  dgamma = sum over rows of dy xh,
+ *   dbeta = sum over rows of dy.
+ * dy and dx have x's type; dgamma and dbeta (d,) have param_type, either may be NULL.  The
+ * workspace (16-byte aligned, nfx_layer_norm_backward_workspace bytes; may be NULL when
+ * dgamma and dbeta are) holds partial sums that are joined in a fixed order, so results do
+ * not change from run to run.  dx may be dy or x (the same pointer and stride). */
+int64_t nfx_layer_norm_backward_workspace(int64_t rows, int64_t d);
+int nfx_layer_norm_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, int x_type,
+                            const float* mean, const float* rstd, const void* gamma, int param_type,
+                            int64_t rows, int64_t d, void* dx, int64_t lddx, void* dgamma, void* dbeta,
+                            void* workspace, int64_t workspace_bytes, void* stream);
+
+/* FP8 E4M3 codes of x (rows, cols) with one fp32 scale per group: tile = 0, groups of 128
+ * along a row (scales (rows, ceil(cols / 128))); tile = 1, tiles of 128 x 128 (scales
+ * (ceil(rows / 128), ceil(cols / 128))).  A group's scale is max |x| / 448 over its finite
+ * elements (at least 2^-126) and a code is E4M3(x * (1 / scale)) by the encoder of
+ * nfx_fp8_e4m3_to_bits (infinities give +-448, NaN gives 0x7F).  With codes_t not NULL the
+ * codes of the transpose (cols, rows) are written as well, from the same read of x: with tile
+ * = 0 its groups run along the rows of x, with tile = 1 it has the same codes.  col_sums
+ * (cols,), allowed with tile = 0, receives the sums of x's columns; it needs a 16-byte
+ * aligned workspace of nfx_fp8_quantise_workspace bytes. */
+int64_t nfx_fp8_quantise_workspace(int64_t rows, int64_t cols);
+int nfx_fp8_quantise(const void* x, int x_type, int64_t ldx, int64_t rows, int64_t cols, int tile,
+                     uint8_t* codes, int64_t ld_codes, float* scales, int64_t scale_row_stride,
+                     int64_t scale_block_stride, uint8_t* codes_t, int64_t ld_codes_t, float* scales_t,
+                     int64_t scale_t_row_stride, int64_t scale_t_block_stride, float* col_sums, void* workspace,
+                     int64_t workspace_bytes, void* stream);
+
+/* C = act(A B^T + bias) for FP8 E4M3 operands in the quantiser's form, A (M, K) and B (N, K):
+ *   C[m, n] = act(sum_b sa[m, b] sb[n, b] sum_{k in block b} A[m, k] B[n, k] + bias[n])
+ * over blocks of 128 along K; with a_tile (b_tile) the scales are per 128 rows.  Each block's
+ * sum is formed by the tensor cores, the sum over blocks in fp32.  The product of two scales
+ * that meet must be finite in fp32.  The rows of A and B start on 16-byte boundaries (base
+ * and row stride); any M, N, K >= 0.  bias (N,) of bias_type or NULL; act 0 none, 1 GELU
+ * (tanh form), 2 ReLU; C of c_type.  The gradients of a linear layer are products of the same
+ * kind: dX = dY W is (dY, W^T) with the tiles' transposed codes, dW = dY^T X is (dY^T, X^T). */
+int nfx_fp8_gemm(const uint8_t* A, int64_t lda, const float* scale_a, int64_t scale_a_row_stride,
+                 int64_t scale_a_block_stride, int a_tile, const uint8_t* B, int64_t ldb, const float* scale_b,
+                 int64_t scale_b_row_stride, int64_t scale_b_block_stride, int b_tile, int64_t M, int64_t N,
+                 int64_t K, const void* bias, int bias_type, int act, void* C, int c_type, int64_t ldc,
+                 void* stream);
+
 /* Read and clear the device error word of the current device (bit flags of waits
  * that timed out inside kernels).  Synchronises the device. */
 int nfx_device_errors(unsigned* flags_out);

@@ -31,6 +31,27 @@ lib.nfx_load_neuroir.argtypes = [C.c_char_p, C.c_char_p, C.c_int, C.POINTER(C.c_
 lib.nfx_device_errors.restype = C.c_int
 lib.nfx_device_errors.argtypes = [C.POINTER(C.c_uint)]
 
+_i64 = C.c_int64
+lib.nfx_layer_norm.restype = C.c_int
+lib.nfx_layer_norm.argtypes = [_vp, C.c_int, _i64, _vp, _vp, C.c_int, _i64, _i64, C.c_float, _vp, _i64, _vp,
+                               _vp, _vp]
+lib.nfx_layer_norm_fp8.restype = C.c_int
+lib.nfx_layer_norm_fp8.argtypes = [_vp, C.c_int, _i64, _vp, _vp, C.c_int, _i64, _i64, C.c_float, _vp, _i64,
+                                   _vp, _i64, _i64, _vp, _vp, _vp]
+lib.nfx_layer_norm_backward_workspace.restype = _i64
+lib.nfx_layer_norm_backward_workspace.argtypes = [_i64, _i64]
+lib.nfx_layer_norm_backward.restype = C.c_int
+lib.nfx_layer_norm_backward.argtypes = [_vp, _i64, _vp, _i64, C.c_int, _vp, _vp, _vp, C.c_int, _i64, _i64, _vp,
+                                        _i64, _vp, _vp, _vp, _i64, _vp]
+lib.nfx_fp8_quantise_workspace.restype = _i64
+lib.nfx_fp8_quantise_workspace.argtypes = [_i64, _i64]
+lib.nfx_fp8_quantise.restype = C.c_int
+lib.nfx_fp8_quantise.argtypes = [_vp, C.c_int, _i64, _i64, _i64, C.c_int, _vp, _i64, _vp, _i64, _i64, _vp, _i64,
+                                 _vp, _i64, _i64, _vp, _vp, _i64, _vp]
+lib.nfx_fp8_gemm.restype = C.c_int
+lib.nfx_fp8_gemm.argtypes = [_vp, _i64, _vp, _i64, _i64, C.c_int, _vp, _i64, _vp, _i64, _i64, C.c_int, _i64,
+                             _i64, _i64, _vp, C.c_int, C.c_int, _vp, C.c_int, _i64, _vp]
+
 if hasattr(lib, "nfx_runtime_create"):
     lib.nfx_runtime_create.restype = C.c_int
     lib.nfx_runtime_create.argtypes = [C.c_char_p, C.c_int, C.POINTER(_vp)]

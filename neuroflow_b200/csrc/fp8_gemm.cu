@@ -1,0 +1,317 @@
+// fp8_gemm.cu -- product of two FP8 E4M3 matrices with an fp32 scale for each block of 128
+// along K, on tcgen05 (kind::f8f6f4).
+//
+//   C[m, n] = act( sum_b sa[m, b] sb[n, b] ( sum_{k in block b} A[m, k] B[n, k] ) + bias[n] )
+//
+// sa and sb are per row, or per 128 rows (tiles).  The tensor core sums one block of 128 (four
+// K = 32 instructions) into a TMEM stage; the epilogue warps read that stage, multiply it by
+// the block's scales and add it to fp32 accumulators in registers, so the sum over the blocks is
+// fp32 and no product of scales is rounded to fewer bits.
+//
+// Structure (persistent, one CTA per SM, 128 x NT tiles):
+//   warps 0 ..      promotion and epilogue: NT / 128 groups of four warps, a warp owning the 32
+//                   TMEM lanes 32 * (warp % 4) .. and 128 columns
+//   then 1 warp     TMA producer (ring of kStages stages: 128 x 128 of A, NT x 128 of B)
+//   then 1 warp     TMEM owner and MMA issuer
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "block_ops.h"
+#include "nfx_internal.h"
+#include "numerics.cuh"
+#include "sm100.cuh"
+
+namespace nfx {
+namespace {
+
+constexpr int kBM = 128;
+constexpr int kBK = kGroup;
+
+template <int NT>
+struct GemmCfg {
+    static constexpr int kEpiWarps = 4 * (NT / 128);
+    static constexpr int kThreads = 32 * (kEpiWarps + 2);
+    static constexpr int kABytes = kBM * kBK;
+    static constexpr int kBBytes = NT * kBK;
+    static constexpr int kStageBytes = kABytes + kBBytes;
+    static constexpr int kStages = NT == 256 ? 4 : 6;
+    static constexpr int kAccStages = 512 / NT;
+    static constexpr int kOffScale = kStages * kStageBytes;  // per-column scales: 2 x 128 floats a warp
+    static constexpr int kOffBars = kOffScale + kEpiWarps * 2 * 128 * 4;
+    static constexpr int kSmemBytes = kOffBars + 8 * (2 * kStages + 2 * kAccStages) + 16 + 1024;
+    static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
+};
+
+__device__ __forceinline__ void tmem_ld16_wait(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]),
+                   "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]),
+                   "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+}
+
+// GELU as z * sigmoid(2u) (the tanh form's identity), the exponential by ex2.approx.
+__device__ __forceinline__ float gelu_sig(float z) {
+    const float c2 = -2.0f * 0.7978845608028654f * 1.4426950408889634f;
+    const float inner = fmaf(z, (0.044715f * z) * z, z);
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(c2 * inner));
+    return __fdividef(z, 1.0f + e);
+}
+__device__ __forceinline__ float gemm_act(float z, int act) {
+    return act == 1 ? gelu_sig(z) : (act == 2 ? relu_ref(z) : z);
+}
+
+// Tile t of a grid of tm x tn tiles: bands of 16 row tiles, row tiles fastest inside a band, so
+// that the tiles in flight share operand rows in L2.
+__device__ __forceinline__ void tile_at(int t, int tm, int tn, int& m, int& n) {
+    const int band = 16 * tn, b = t / band, rem = t % band;
+    const int h = min(16, tm - b * 16);
+    m = b * 16 + rem % h;
+    n = rem / h;
+}
+
+// COL: 0 the columns of a 128-column group share a scale (B in tiles), 1 one scale per column
+template <int NT, int COL>
+__global__ void __launch_bounds__(GemmCfg<NT>::kThreads, 1)
+fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                const Fp8GemmArgs p) {
+    using C = GemmCfg<NT>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kOffBars);
+    uint64_t* empty = full + C::kStages;
+    uint64_t* accFull = empty + C::kStages;
+    uint64_t* accEmpty = accFull + C::kAccStages;
+    uint32_t* sTmem = reinterpret_cast<uint32_t*>(accEmpty + C::kAccStages);
+    volatile int* sAbort = reinterpret_cast<volatile int*>(sTmem + 1);
+
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const int tm = (p.M + kBM - 1) / kBM, tn = (p.N + NT - 1) / NT;
+    const int tiles = tm * tn;
+    const int KB = (p.K + kBK - 1) / kBK;
+    const uint64_t budget = p.wait_ns ? p.wait_ns : kWaitNs;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::kStages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int s = 0; s < C::kAccStages; ++s) {
+            mbar_init(&accFull[s], 1);
+            mbar_init(&accEmpty[s], C::kEpiWarps);
+        }
+        *sAbort = 0;
+        fence_mbar_init();
+    }
+    if (warp == C::kEpiWarps + 1) tmem_alloc(sTmem, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *sTmem;
+
+    if (warp == C::kEpiWarps) {
+        // ---------------- TMA producer
+        if (elect_one()) {
+            int it = 0;
+            bool ok = true;
+            for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+                int mt, nt;
+                tile_at(t, tm, tn, mt, nt);
+                for (int kb = 0; kb < KB; ++kb, ++it) {
+                    const int s = it % C::kStages;
+                    const uint32_t ph = (it / C::kStages) & 1;
+                    if (!mbar_wait_backoff(&empty[s], ph ^ 1, sAbort, 128, 32, budget)) {
+                        *sAbort = 1;
+                        atomicOr(p.err, kErrWaitSlotFree);
+                        ok = false;
+                        break;
+                    }
+                    mbar_arrive_expect_tx(&full[s], C::kStageBytes);
+                    uint8_t* st = smem + s * C::kStageBytes;
+                    tma_load_2d(st, &tmA, &full[s], kb * kBK, mt * kBM);
+                    tma_load_2d(st + C::kABytes, &tmB, &full[s], kb * kBK, nt * NT);
+                }
+            }
+            // every load that was issued lands before the CTA exits
+            for (int j = it > C::kStages ? it - C::kStages : 0; j < it; ++j)
+                if (!mbar_wait_drain(&full[j % C::kStages], (j / C::kStages) & 1)) {
+                    atomicOr(p.err, kErrWaitDrain);
+                    break;
+                }
+        }
+        __syncwarp();
+    } else if (warp == C::kEpiWarps + 1) {
+        // ---------------- MMA issuer
+        if (elect_one()) {
+            int it = 0;
+            bool ok = true;
+            for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+                for (int kb = 0; kb < KB; ++kb, ++it) {
+                    const int s = it % C::kStages, a = it % C::kAccStages;
+                    if (!mbar_wait(&accEmpty[a], ((it / C::kAccStages) & 1) ^ 1, sAbort, budget)) {
+                        *sAbort = 1;
+                        atomicOr(p.err, kErrWaitAccFree);
+                        ok = false;
+                        break;
+                    }
+                    if (!mbar_wait(&full[s], (it / C::kStages) & 1, sAbort, budget)) {
+                        *sAbort = 1;
+                        atomicOr(p.err, kErrWaitTmaFull);
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t ab = smem_u32(smem + s * C::kStageBytes), bb = ab + C::kABytes;
+#pragma unroll
+                    for (int k = 0; k < kBK / 32; ++k)
+                        mma_f8(tmem_base + a * NT, umma_desc(ab + 32 * k, 128), umma_desc(bb + 32 * k, 128),
+                               idesc_e4m3(NT), k > 0 ? 1u : 0u);
+                    mma_commit(&empty[s]);
+                    mma_commit(&accFull[a]);
+                }
+            }
+            // the last commit completes before TMEM is released
+            if (it > 0 && !mbar_wait_drain(&accFull[(it - 1) % C::kAccStages], ((it - 1) / C::kAccStages) & 1))
+                atomicOr(p.err, kErrWaitDrain);
+        }
+        __syncwarp();
+    } else {
+        // ---------------- promotion and epilogue
+        const int quad = warp & 3, grp = warp >> 2;
+        float* myScale = reinterpret_cast<float*>(smem + C::kOffScale) + warp * 256;
+        int it = 0;
+        bool ok = true;
+        for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+            int mt, nt;
+            tile_at(t, tm, tn, mt, nt);
+            const int m = mt * kBM + quad * 32 + lane;
+            const int n0 = nt * NT + grp * 128;
+            const int mc = min(m, p.M - 1);
+            const float* sa = p.sa + static_cast<int64_t>(p.a_tile ? mc / 128 : mc) * p.sars;
+            const float* sb = p.sb + static_cast<int64_t>(min(n0, p.N - 1) / 128) * p.sbrs;
+            float2 acc[64];
+#pragma unroll
+            for (int j = 0; j < 64; ++j) acc[j] = make_float2(0.0f, 0.0f);
+            float sc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            auto load_scales = [&](int kb, float& a) {
+                a = 0.0f;
+                if (kb >= KB) return;
+                a = __ldg(sa + kb * p.sabs);
+                if constexpr (COL == 0) {
+                    a *= __ldg(sb + kb * p.sbbs);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int n = n0 + j * 32 + lane;
+                        sc[j] = n < p.N ? __ldg(p.sb + static_cast<int64_t>(n) * p.sbrs + kb * p.sbbs) : 0.0f;
+                    }
+                }
+            };
+            float s_next;
+            load_scales(0, s_next);
+            for (int kb = 0; kb < KB; ++kb, ++it) {
+                const float s = s_next;
+                const float* cs = myScale + (kb & 1) * 128;
+                if constexpr (COL == 1) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) myScale[(kb & 1) * 128 + j * 32 + lane] = sc[j];
+                    __syncwarp();
+                }
+                load_scales(kb + 1, s_next);
+                const int a = it % C::kAccStages;
+                if (!mbar_wait(&accFull[a], (it / C::kAccStages) & 1, sAbort, budget)) {
+                    *sAbort = 1;
+                    atomicOr(p.err, kErrWaitAccFull);
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t tb = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + a * NT + grp * 128;
+                uint32_t r0[16], r1[16];
+                auto add = [&](const uint32_t (&r)[16], int c) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float2 d = make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
+                        float2 f = make_float2(s, s);
+                        if constexpr (COL == 1)
+                            f = mul2_rn(f, *reinterpret_cast<const float2*>(cs + c * 16 + 2 * j));
+                        acc[c * 8 + j] = fma2_rn(d, f, acc[c * 8 + j]);
+                    }
+                };
+                tmem_ld16(tb, r0);
+#pragma unroll
+                for (int c = 0; c < 8; c += 2) {
+                    tmem_ld16_wait(r0);
+                    tmem_ld16(tb + (c + 1) * 16, r1);
+                    add(r0, c);
+                    tmem_ld16_wait(r1);
+                    if (c + 2 < 8) {
+                        tmem_ld16(tb + (c + 2) * 16, r0);
+                    } else {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&accEmpty[a]);
+                    }
+                    add(r1, c + 1);
+                }
+            }
+            if (!ok) break;
+            if (m < p.M) {
+                const int64_t row = static_cast<int64_t>(m) * p.ldc;
+#pragma unroll
+                for (int j = 0; j < 64; ++j) {
+                    const int n = n0 + 2 * j;
+                    float v0 = acc[j].x, v1 = acc[j].y;
+                    if (n < p.N) {
+                        if (p.bias) v0 += load_any(p.bias, p.btype, n);
+                        store_any(p.C, p.ctype, row + n, gemm_act(v0, p.act));
+                    }
+                    if (n + 1 < p.N) {
+                        if (p.bias) v1 += load_any(p.bias, p.btype, n + 1);
+                        store_any(p.C, p.ctype, row + n + 1, gemm_act(v1, p.act));
+                    }
+                }
+            }
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == C::kEpiWarps + 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, 512);
+    }
+}
+
+template <int NT>
+cudaError_t launch(const Fp8GemmArgs& p, cudaStream_t stream) {
+    using C = GemmCfg<NT>;
+    CUtensorMap tmA{}, tmB{};
+    if (p.K > 0 &&
+        (!encode_2d(&tmA, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.A, p.K, p.M, p.lda, kBK, kBM, 128) ||
+         !encode_2d(&tmB, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.B, p.K, p.N, p.ldb, kBK, NT, 128)))
+        return cudaErrorInvalidValue;
+    auto kern = p.b_tile ? fp8_gemm_kernel<NT, 0> : fp8_gemm_kernel<NT, 1>;
+    cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), C::kSmemBytes);
+    if (e != cudaSuccess) return e;
+    const int64_t tiles = static_cast<int64_t>((p.M + kBM - 1) / kBM) * ((p.N + NT - 1) / NT);
+    const int sms = device_sm_count();
+    kern<<<static_cast<int>(tiles < sms ? tiles : sms), C::kThreads, C::kSmemBytes, stream>>>(tmA, tmB, p);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t fp8_gemm_launch(const Fp8GemmArgs& p_in, cudaStream_t stream) {
+    Fp8GemmArgs p = p_in;
+    p.wait_ns = debug_wait_budget_ns();
+    const int64_t wide = static_cast<int64_t>((p.M + 127) / 128) * ((p.N + 255) / 256);
+    return wide >= device_sm_count() ? launch<256>(p, stream) : launch<128>(p, stream);
+}
+
+}  // namespace nfx

@@ -98,6 +98,7 @@ struct Fp8GemmArgs {
     void* C;
     int ctype;
     int64_t ldc;
+    int tma_c;  // set by the launcher: C's rows allow TMA stores
     int M, N, K;
     unsigned* err;
     unsigned long long wait_ns;

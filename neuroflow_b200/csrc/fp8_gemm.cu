@@ -10,9 +10,13 @@
 //
 // Structure (persistent, one CTA per SM, 128 x NT tiles):
 //   warps 0 ..      promotion and epilogue: NT / 128 groups of four warps, a warp owning the 32
-//                   TMEM lanes 32 * (warp % 4) .. and 128 columns
-//   then 1 warp     TMA producer (ring of kStages stages: 128 x 128 of A, NT x 128 of B)
-//   then 1 warp     TMEM owner and MMA issuer
+//                   TMEM lanes 32 * (warp % 4) .. and 128 columns; the result leaves through a
+//                   swizzled 4 KB staging buffer per warp (TMA stores of 32 rows x 128 bytes, or
+//                   coalesced element stores where C's rows are not 16-byte aligned)
+//   then 4 warps    TMA producer (ring of kStages stages: 128 x 128 of A, NT x 128 of B), TMEM
+//                   owner and MMA issuer, two idle
+// With NT = 256 the accumulators take 128 registers of each epilogue thread: the last four warps
+// give registers up to them (setmaxnreg; 8 x 32 x 208 + 4 x 32 x 88 = 12 x 32 x 168 at launch).
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -28,18 +32,20 @@ namespace {
 
 constexpr int kBM = 128;
 constexpr int kBK = kGroup;
+constexpr int kOutBytes = 32 * 128;  // one staging buffer
 
 template <int NT>
 struct GemmCfg {
     static constexpr int kEpiWarps = 4 * (NT / 128);
-    static constexpr int kThreads = 32 * (kEpiWarps + 2);
+    static constexpr int kThreads = 32 * (kEpiWarps + 4);
     static constexpr int kABytes = kBM * kBK;
     static constexpr int kBBytes = NT * kBK;
     static constexpr int kStageBytes = kABytes + kBBytes;
     static constexpr int kStages = NT == 256 ? 4 : 6;
     static constexpr int kAccStages = 512 / NT;
-    static constexpr int kOffScale = kStages * kStageBytes;  // per-column scales: 2 x 128 floats a warp
-    static constexpr int kOffBars = kOffScale + kEpiWarps * 2 * 128 * 4;
+    // per epilogue warp: two sets of 128 column scales during a tile, the staging buffer after it
+    static constexpr int kOffOut = kStages * kStageBytes;
+    static constexpr int kOffBars = kOffOut + kEpiWarps * kOutBytes;
     static constexpr int kSmemBytes = kOffBars + 8 * (2 * kStages + 2 * kAccStages) + 16 + 1024;
     static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
 };
@@ -61,8 +67,101 @@ __device__ __forceinline__ float gelu_sig(float z) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(c2 * inner));
     return __fdividef(z, 1.0f + e);
 }
-__device__ __forceinline__ float gemm_act(float z, int act) {
-    return act == 1 ? gelu_sig(z) : (act == 2 ? relu_ref(z) : z);
+
+template <int R>
+__device__ __forceinline__ void reg_inc() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R));
+}
+template <int R>
+__device__ __forceinline__ void reg_dec() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R));
+}
+
+// Adds the bias (128 floats in shared memory) to one row's accumulators and applies the activation.
+__device__ __forceinline__ void finish_row(float2 (&acc)[64], const float* bias, int act) {
+    if (bias) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+            const float4 v = *reinterpret_cast<const float4*>(bias + 4 * j);
+            acc[2 * j].x += v.x, acc[2 * j].y += v.y;
+            acc[2 * j + 1].x += v.z, acc[2 * j + 1].y += v.w;
+        }
+    }
+    if (act == 1) {
+#pragma unroll
+        for (int j = 0; j < 64; ++j) acc[j] = make_float2(gelu_sig(acc[j].x), gelu_sig(acc[j].y));
+    } else if (act == 2) {
+#pragma unroll
+        for (int j = 0; j < 64; ++j) acc[j] = make_float2(relu_ref(acc[j].x), relu_ref(acc[j].y));
+    }
+}
+
+// Columns c0 .. of a row as the bytes of one staging chunk (16 bytes).
+template <int CT>
+__device__ __forceinline__ uint4 pack_chunk(const float2 (&acc)[64], int j) {
+    uint4 v;
+    if constexpr (CT == kF32) {
+        v = make_uint4(__float_as_uint(acc[2 * j].x), __float_as_uint(acc[2 * j].y),
+                       __float_as_uint(acc[2 * j + 1].x), __float_as_uint(acc[2 * j + 1].y));
+    } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 a = acc[4 * j + i];
+            if constexpr (CT == kBF16) {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(a.x, a.y);
+                w[i] = *reinterpret_cast<const uint32_t*>(&h);
+            } else {
+                const __half2 h = __floats2half2_rn(a.x, a.y);
+                w[i] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+        }
+        v = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    return v;
+}
+
+// A warp's 32 rows x 128 columns at (m0, n0) to C through its staging buffer `buf`, in boxes of 32
+// rows x 128 bytes (the lane holds row m0 + lane).
+template <int CT>
+__device__ __forceinline__ void store_rows(const float2 (&acc)[64], const Fp8GemmArgs& p, const CUtensorMap* tmC,
+                                           uint8_t* buf, int m0, int n0, int lane) {
+    constexpr int kEl = CT == kF32 ? 4 : 2;
+    constexpr int kCols = 128 / kEl;  // columns of a box
+#pragma unroll
+    for (int b = 0; b < 128 / kCols; ++b) {
+        const int n = n0 + b * kCols;
+        if (n >= p.N) break;
+        if (p.tma_c) {  // the previous box has been read
+            if (lane == 0) tma_store_wait_read<0>();
+            __syncwarp();
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<uint4*>(buf + swz_offset(lane * 128 + j * 16, 128)) = pack_chunk<CT>(acc, b * 8 + j);
+        // a TMA store clips its box at 16 bytes, not at the element: a last box whose row ends inside 16
+        // bytes goes out by elements
+        if (p.tma_c && (n + kCols <= p.N || p.N * kEl % 16 == 0)) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                tma_store_2d(tmC, buf, n, m0);
+                tma_store_commit();
+            }
+        } else {
+            __syncwarp();
+            const int rows = min(32, p.M - m0), cols = min(kCols, p.N - n);
+            for (int r = 0; r < rows; ++r) {
+                uint8_t* dst = static_cast<uint8_t*>(p.C) + (static_cast<int64_t>(m0 + r) * p.ldc + n) * kEl;
+                for (int c = lane; c < cols; c += 32) {
+                    const uint8_t* src = buf + swz_offset(r * 128 + c * kEl, 128);
+                    if constexpr (kEl == 4) *reinterpret_cast<uint32_t*>(dst + c * 4) = *reinterpret_cast<const uint32_t*>(src);
+                    else *reinterpret_cast<uint16_t*>(dst + c * 2) = *reinterpret_cast<const uint16_t*>(src);
+                }
+            }
+            __syncwarp();
+        }
+    }
 }
 
 // Tile t of a grid of tm x tn tiles: bands of 16 row tiles, row tiles fastest inside a band, so
@@ -75,10 +174,10 @@ __device__ __forceinline__ void tile_at(int t, int tm, int tn, int& m, int& n) {
 }
 
 // COL: 0 the columns of a 128-column group share a scale (B in tiles), 1 one scale per column
-template <int NT, int COL>
+template <int NT, int COL, int CT>
 __global__ void __launch_bounds__(GemmCfg<NT>::kThreads, 1)
 fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                const Fp8GemmArgs p) {
+                const __grid_constant__ CUtensorMap tmC, const Fp8GemmArgs p) {
     using C = GemmCfg<NT>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -114,6 +213,10 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     tc_fence_after();
     const uint32_t tmem_base = *sTmem;
 
+    // the register split stands inside the roles' branches: where they met again, the compiler would
+    // have to assume the smaller count
+    if (warp >= C::kEpiWarps) {
+        if constexpr (NT == 256) reg_dec<88>();
     if (warp == C::kEpiWarps) {
         // ---------------- TMA producer
         if (elect_one()) {
@@ -180,10 +283,13 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                 atomicOr(p.err, kErrWaitDrain);
         }
         __syncwarp();
+    }
     } else {
         // ---------------- promotion and epilogue
+        if constexpr (NT == 256) reg_inc<208>();
         const int quad = warp & 3, grp = warp >> 2;
-        float* myScale = reinterpret_cast<float*>(smem + C::kOffScale) + warp * 256;
+        uint8_t* myOut = smem + C::kOffOut + warp * kOutBytes;
+        float* myScale = reinterpret_cast<float*>(myOut);
         int it = 0;
         bool ok = true;
         for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
@@ -198,6 +304,12 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
 #pragma unroll
             for (int j = 0; j < 64; ++j) acc[j] = make_float2(0.0f, 0.0f);
             float sc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            float bias[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (p.bias) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (n0 + j * 32 + lane < p.N) bias[j] = load_any(p.bias, p.btype, n0 + j * 32 + lane);
+            }
             auto load_scales = [&](int kb, float& a) {
                 a = 0.0f;
                 if (kb >= KB) return;
@@ -214,6 +326,10 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             };
             float s_next;
             load_scales(0, s_next);
+            if (COL == 1 && p.tma_c) {  // the last tile's box has been read
+                if (lane == 0) tma_store_wait_read<0>();
+                __syncwarp();
+            }
             for (int kb = 0; kb < KB; ++kb, ++it) {
                 const float s = s_next;
                 const float* cs = myScale + (kb & 1) * 128;
@@ -261,23 +377,20 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                 }
             }
             if (!ok) break;
-            if (m < p.M) {
-                const int64_t row = static_cast<int64_t>(m) * p.ldc;
+            if (p.bias) {
+                if (p.tma_c && lane == 0) tma_store_wait_read<0>();
+                __syncwarp();
 #pragma unroll
-                for (int j = 0; j < 64; ++j) {
-                    const int n = n0 + 2 * j;
-                    float v0 = acc[j].x, v1 = acc[j].y;
-                    if (n < p.N) {
-                        if (p.bias) v0 += load_any(p.bias, p.btype, n);
-                        store_any(p.C, p.ctype, row + n, gemm_act(v0, p.act));
-                    }
-                    if (n + 1 < p.N) {
-                        if (p.bias) v1 += load_any(p.bias, p.btype, n + 1);
-                        store_any(p.C, p.ctype, row + n + 1, gemm_act(v1, p.act));
-                    }
-                }
+                for (int j = 0; j < 4; ++j) myScale[j * 32 + lane] = bias[j];
+                __syncwarp();
             }
+            finish_row(acc, p.bias ? myScale : nullptr, p.act);
+            __syncwarp();  // every lane has read the scales and the bias
+            const int m0 = mt * kBM + quad * 32;
+            if (m0 < p.M) store_rows<CT>(acc, p, &tmC, myOut, m0, n0, lane);
         }
+        if (lane == 0) tma_store_wait_all<0>();
+        __syncwarp();
     }
 
     tc_fence_before();
@@ -288,7 +401,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     }
 }
 
-template <int NT>
+template <int NT, int CT>
 cudaError_t launch(const Fp8GemmArgs& p, cudaStream_t stream) {
     using C = GemmCfg<NT>;
     CUtensorMap tmA{}, tmB{};
@@ -296,13 +409,26 @@ cudaError_t launch(const Fp8GemmArgs& p, cudaStream_t stream) {
         (!encode_2d(&tmA, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.A, p.K, p.M, p.lda, kBK, kBM, 128) ||
          !encode_2d(&tmB, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.B, p.K, p.N, p.ldb, kBK, NT, 128)))
         return cudaErrorInvalidValue;
-    auto kern = p.b_tile ? fp8_gemm_kernel<NT, 0> : fp8_gemm_kernel<NT, 1>;
+    CUtensorMap tmC{};
+    constexpr int kEl = CT == kF32 ? 4 : 2;
+    if (p.tma_c && !encode_2d(&tmC, CT == kF32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                    : CT == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                  : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                              p.C, p.N, p.M, p.ldc * kEl, 128 / kEl, 32, 128))
+        return cudaErrorInvalidValue;
+    auto kern = p.b_tile ? fp8_gemm_kernel<NT, 0, CT> : fp8_gemm_kernel<NT, 1, CT>;
     cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), C::kSmemBytes);
     if (e != cudaSuccess) return e;
     const int64_t tiles = static_cast<int64_t>((p.M + kBM - 1) / kBM) * ((p.N + NT - 1) / NT);
     const int sms = device_sm_count();
-    kern<<<static_cast<int>(tiles < sms ? tiles : sms), C::kThreads, C::kSmemBytes, stream>>>(tmA, tmB, p);
+    kern<<<static_cast<int>(tiles < sms ? tiles : sms), C::kThreads, C::kSmemBytes, stream>>>(tmA, tmB, tmC, p);
     return cudaGetLastError();
+}
+
+template <int CT>
+cudaError_t dispatch(const Fp8GemmArgs& p, cudaStream_t stream) {
+    const int64_t wide = static_cast<int64_t>((p.M + 127) / 128) * ((p.N + 255) / 256);
+    return wide >= device_sm_count() ? launch<256, CT>(p, stream) : launch<128, CT>(p, stream);
 }
 
 }  // namespace
@@ -310,8 +436,11 @@ cudaError_t launch(const Fp8GemmArgs& p, cudaStream_t stream) {
 cudaError_t fp8_gemm_launch(const Fp8GemmArgs& p_in, cudaStream_t stream) {
     Fp8GemmArgs p = p_in;
     p.wait_ns = debug_wait_budget_ns();
-    const int64_t wide = static_cast<int64_t>((p.M + 127) / 128) * ((p.N + 255) / 256);
-    return wide >= device_sm_count() ? launch<256>(p, stream) : launch<128>(p, stream);
+    // a TMA store needs 16-byte aligned rows; a result of one row has no row stride
+    if (p.M == 1) p.ldc = (static_cast<int64_t>(p.N) + 15) / 16 * 16;
+    p.tma_c = reinterpret_cast<uintptr_t>(p.C) % 16 == 0 && p.ldc * type_bytes(p.ctype) % 16 == 0;
+    if (p.ctype == kF32) return dispatch<kF32>(p, stream);
+    return p.ctype == kBF16 ? dispatch<kBF16>(p, stream) : dispatch<kF16>(p, stream);
 }
 
 }  // namespace nfx

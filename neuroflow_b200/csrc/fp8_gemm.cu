@@ -173,7 +173,29 @@ __device__ __forceinline__ void tile_at(int t, int tm, int tn, int& m, int& n) {
     n = rem / h;
 }
 
-// COL: 0 the columns of a 128-column group share a scale (B in tiles), 1 one scale per column
+// A warp's finished accumulators (rows m0 + lane, columns n0 ..) to C, through its staging buffer.
+template <int CT>
+__device__ __forceinline__ void epilogue(float2 (&acc)[64], const Fp8GemmArgs& p, const CUtensorMap* tmC,
+                                         uint8_t* buf, int m0, int n0, int lane) {
+    float* sb = reinterpret_cast<float*>(buf);
+    if (p.bias) {
+        float b[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int n = n0 + j * 32 + lane;
+            b[j] = n < p.N ? load_any(p.bias, p.btype, n) : 0.0f;
+        }
+        if (p.tma_c && lane == 0) tma_store_wait_read<0>();
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sb[j * 32 + lane] = b[j];
+        __syncwarp();
+    }
+    finish_row(acc, p.bias ? sb : nullptr, p.act);
+    __syncwarp();  // every lane has read the bias
+    if (m0 < p.M) store_rows<CT>(acc, p, tmC, buf, m0, n0, lane);
+}
+
 template <int NT, int COL, int CT>
 __global__ void __launch_bounds__(GemmCfg<NT>::kThreads, 1)
 fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
@@ -304,12 +326,6 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
 #pragma unroll
             for (int j = 0; j < 64; ++j) acc[j] = make_float2(0.0f, 0.0f);
             float sc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            float bias[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (p.bias) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (n0 + j * 32 + lane < p.N) bias[j] = load_any(p.bias, p.btype, n0 + j * 32 + lane);
-            }
             auto load_scales = [&](int kb, float& a) {
                 a = 0.0f;
                 if (kb >= KB) return;
@@ -377,17 +393,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                 }
             }
             if (!ok) break;
-            if (p.bias) {
-                if (p.tma_c && lane == 0) tma_store_wait_read<0>();
-                __syncwarp();
-#pragma unroll
-                for (int j = 0; j < 4; ++j) myScale[j * 32 + lane] = bias[j];
-                __syncwarp();
-            }
-            finish_row(acc, p.bias ? myScale : nullptr, p.act);
-            __syncwarp();  // every lane has read the scales and the bias
-            const int m0 = mt * kBM + quad * 32;
-            if (m0 < p.M) store_rows<CT>(acc, p, &tmC, myOut, m0, n0, lane);
+            __syncwarp();  // every lane has read the column scales
+            epilogue<CT>(acc, p, &tmC, myOut, mt * kBM + quad * 32, n0, lane);
         }
         if (lane == 0) tma_store_wait_all<0>();
         __syncwarp();
@@ -401,6 +408,300 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     }
 }
 
+// COL: 0 the columns of a 128-column group share a scale (B in tiles), 1 one scale per column
+//
+// One tile is 256 x 256, computed by a pair of CTAs with cta_group::2 MMAs: CTA r holds rows
+// 128 r .. of the tile's A and of its B (so each operand byte is fetched once per pair, 64 KB for
+// 128 x 256 x 256 products instead of 96 KB by two CTAs alone), and rows 128 r .. of the result in
+// its TMEM.  Warps of each CTA:
+//   0-7    promotion and epilogue     8   TMA producer        9   TMEM owner; CTA 0's issues the MMAs
+//   10     scale producer (cp.async into a ring, several blocks ahead: a scale that is fetched in
+//          the promotion loop itself costs an L2 latency per block)
+// Barriers: full (CTA 0's, both CTAs' bytes), empty and accFull (both CTAs', by commit), accEmpty (CTA
+// 0's, arrivals from the epilogue warps of both), sFull and sEmpty (each CTA's own scales).
+constexpr int kPairThreads = 384;
+constexpr int kPairEpi = 8;
+
+template <int COL>
+struct PairCfg {
+    static constexpr int kStages = 5;
+    static constexpr int kStageBytes = 2 * 128 * kBK;
+    static constexpr int kScaleStages = 8;
+    static constexpr int kScaleBytes = (128 + (COL ? 256 : 4)) * 4;
+    static constexpr int kOffOut = kStages * kStageBytes;
+    static constexpr int kOffScale = kOffOut + kPairEpi * kOutBytes;
+    static constexpr int kOffBars = kOffScale + kScaleStages * kScaleBytes;
+    static constexpr int kSmemBytes = kOffBars + 8 * (2 * kStages + 2 * 2 + 2 * kScaleStages) + 16 + 1024;
+    static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
+};
+
+template <int COL, int CT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                     const __grid_constant__ CUtensorMap tmC, const Fp8GemmArgs p) {
+    using C = PairCfg<COL>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kOffBars);
+    uint64_t* empty = full + C::kStages;
+    uint64_t* accFull = empty + C::kStages;
+    uint64_t* accEmpty = accFull + 2;
+    uint64_t* sFull = accEmpty + 2;
+    uint64_t* sEmpty = sFull + C::kScaleStages;
+    uint32_t* sTmem = reinterpret_cast<uint32_t*>(sEmpty + C::kScaleStages);
+    volatile int* sAbort = reinterpret_cast<volatile int*>(sTmem + 1);
+
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    const int tm = (p.M + 255) / 256, tn = (p.N + 255) / 256;
+    const int tiles = tm * tn;
+    const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
+    const int KB = (p.K + kBK - 1) / kBK;
+    const uint64_t budget = p.wait_ns ? p.wait_ns : kWaitNs;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::kStages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&accFull[s], 1);
+            mbar_init(&accEmpty[s], 2 * kPairEpi);
+        }
+        for (int s = 0; s < C::kScaleStages; ++s) {
+            mbar_init(&sFull[s], 32);
+            mbar_init(&sEmpty[s], kPairEpi);
+        }
+        *sAbort = 0;
+        fence_mbar_init();
+    }
+    if (warp == kPairEpi + 1) tmem_alloc_pair(sTmem, 512);
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();  // both CTAs' barriers are ready
+    tc_fence_after();
+    const uint32_t tmem_base = *sTmem;
+
+    // the register split stands inside the roles' branches: where they met again, the compiler would
+    // have to assume the smaller count
+    if (warp >= kPairEpi) {
+        reg_dec<88>();
+        if (warp == kPairEpi) {
+            // ---------------- TMA producer
+            if (elect_one()) {
+                int it = 0;
+                bool ok = true;
+                for (int t = first; ok && t < tiles; t += step) {
+                    int mt, nt;
+                    tile_at(t, tm, tn, mt, nt);
+                    for (int kb = 0; kb < KB; ++kb, ++it) {
+                        const int s = it % C::kStages;
+                        if (!mbar_wait_backoff(&empty[s], ((it / C::kStages) & 1) ^ 1, sAbort, 128, 32, budget)) {
+                            *sAbort = 1;
+                            atomicOr(p.err, kErrWaitSlotFree);
+                            ok = false;
+                            break;
+                        }
+                        if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * C::kStageBytes);
+                        const uint32_t bar = map_rank(smem_u32(&full[s]), 0);
+                        uint8_t* st = smem + s * C::kStageBytes;
+                        tma_load_2d_pair(st, &tmA, bar, kb * kBK, mt * 256 + rank * 128);
+                        tma_load_2d_pair(st + 128 * kBK, &tmB, bar, kb * kBK, nt * 256 + rank * 128);
+                    }
+                }
+                // every load that was issued has landed and been read before the CTA exits
+                for (int j = it > C::kStages ? it - C::kStages : 0; j < it; ++j)
+                    if (!mbar_wait_drain(&empty[j % C::kStages], (j / C::kStages) & 1)) {
+                        atomicOr(p.err, kErrWaitDrain);
+                        break;
+                    }
+            }
+            __syncwarp();
+        } else if (warp == kPairEpi + 1) {
+            // ---------------- MMA issuer
+            if (rank == 0 && elect_one()) {
+                int it = 0;
+                bool ok = true;
+                for (int t = first; ok && t < tiles; t += step) {
+                    for (int kb = 0; kb < KB; ++kb, ++it) {
+                        const int s = it % C::kStages, a = it & 1;
+                        if (!mbar_wait(&accEmpty[a], ((it >> 1) & 1) ^ 1, sAbort, budget)) {
+                            *sAbort = 1;
+                            atomicOr(p.err, kErrWaitAccFree);
+                            ok = false;
+                            break;
+                        }
+                        if (!mbar_wait(&full[s], (it / C::kStages) & 1, sAbort, budget)) {
+                            *sAbort = 1;
+                            atomicOr(p.err, kErrWaitTmaFull);
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint32_t ab = smem_u32(smem + s * C::kStageBytes), bb = ab + 128 * kBK;
+#pragma unroll
+                        for (int k = 0; k < kBK / 32; ++k)
+                            mma_f8_pair(tmem_base + a * 256, umma_desc(ab + 32 * k, 128), umma_desc(bb + 32 * k, 128),
+                                        idesc_e4m3_pair(256), k > 0 ? 1u : 0u);
+                        mma_commit_pair(&empty[s]);
+                        mma_commit_pair(&accFull[a]);
+                    }
+                }
+                // the last commit completes before TMEM is released
+                if (it > 0 && !mbar_wait_drain(&accFull[(it - 1) & 1], ((it - 1) >> 1) & 1))
+                    atomicOr(p.err, kErrWaitDrain);
+            }
+            __syncwarp();
+        } else if (warp == kPairEpi + 2) {
+            // ---------------- scale producer
+            int it = 0;
+            bool ok = true;
+            for (int t = first; ok && t < tiles; t += step) {
+                int mt, nt;
+                tile_at(t, tm, tn, mt, nt);
+                const int m0 = mt * 256 + rank * 128, n0 = nt * 256;
+                const float* src[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int m = min(m0 + j * 32 + lane, p.M - 1);
+                    src[j] = p.sa + static_cast<int64_t>(p.a_tile ? m / 128 : m) * p.sars;
+                }
+                for (int kb = 0; kb < KB; ++kb, ++it) {
+                    const int s = it % C::kScaleStages;
+                    if (!mbar_wait(&sEmpty[s], ((it / C::kScaleStages) & 1) ^ 1, sAbort, budget)) {
+                        *sAbort = 1;
+                        atomicOr(p.err, kErrWaitSlotFree);
+                        ok = false;
+                        break;
+                    }
+                    float* dst = reinterpret_cast<float*>(smem + C::kOffScale + s * C::kScaleBytes);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) cp_async4(dst + j * 32 + lane, src[j] + kb * p.sabs, true);
+                    if constexpr (COL == 1) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const int n = n0 + j * 32 + lane;
+                            cp_async4(dst + 128 + j * 32 + lane,
+                                      p.sb + static_cast<int64_t>(min(n, p.N - 1)) * p.sbrs + kb * p.sbbs, n < p.N);
+                        }
+                    } else if (lane < 2) {
+                        const int g = min(n0 + lane * 128, p.N - 1) / 128;
+                        cp_async4(dst + 128 + lane, p.sb + static_cast<int64_t>(g) * p.sbrs + kb * p.sbbs, true);
+                    }
+                    cp_async_arrive(&sFull[s]);
+                }
+            }
+            cp_async_wait_all();
+        }
+    } else {
+        // ---------------- promotion and epilogue
+        reg_inc<208>();
+        const int quad = warp & 3, grp = warp >> 2;
+        uint8_t* myOut = smem + C::kOffOut + warp * kOutBytes;
+        const uint32_t accEmpty0 = map_rank(smem_u32(accEmpty), 0);
+        int it = 0;
+        bool ok = true;
+        for (int t = first; ok && t < tiles; t += step) {
+            int mt, nt;
+            tile_at(t, tm, tn, mt, nt);
+            const int m0 = mt * 256 + rank * 128 + quad * 32;
+            const int n0 = nt * 256 + grp * 128;
+            float2 acc[64];
+#pragma unroll
+            for (int j = 0; j < 64; ++j) acc[j] = make_float2(0.0f, 0.0f);
+            for (int kb = 0; kb < KB; ++kb, ++it) {
+                const int a = it & 1, ss = it % C::kScaleStages;
+                const float* sc = reinterpret_cast<const float*>(smem + C::kOffScale + ss * C::kScaleBytes);
+                if (!mbar_wait(&sFull[ss], (it / C::kScaleStages) & 1, sAbort, budget) ||
+                    !mbar_wait(&accFull[a], (it >> 1) & 1, sAbort, budget)) {
+                    *sAbort = 1;
+                    atomicOr(p.err, kErrWaitAccFull);
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                float s = sc[quad * 32 + lane];
+                if constexpr (COL == 0) s *= sc[128 + grp];
+                const uint32_t tb = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + a * 256 + grp * 128;
+                uint32_t r0[16], r1[16];
+                auto add = [&](const uint32_t (&r)[16], int c) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        float2 f0 = make_float2(s, s), f1 = f0;
+                        if constexpr (COL == 1) {
+                            const float4 cs = *reinterpret_cast<const float4*>(sc + 128 + grp * 128 + c * 16 + 4 * j);
+                            f0 = mul2_rn(f0, make_float2(cs.x, cs.y));
+                            f1 = mul2_rn(f1, make_float2(cs.z, cs.w));
+                        }
+                        acc[c * 8 + 2 * j] = fma2_rn(make_float2(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1])),
+                                                     f0, acc[c * 8 + 2 * j]);
+                        acc[c * 8 + 2 * j + 1] = fma2_rn(
+                            make_float2(__uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3])), f1, acc[c * 8 + 2 * j + 1]);
+                    }
+                };
+                tmem_ld16(tb, r0);
+#pragma unroll
+                for (int c = 0; c < 8; c += 2) {
+                    tmem_ld16_wait(r0);
+                    tmem_ld16(tb + (c + 1) * 16, r1);
+                    add(r0, c);
+                    tmem_ld16_wait(r1);
+                    if (c + 2 < 8) {
+                        tmem_ld16(tb + (c + 2) * 16, r0);
+                    } else {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_cluster(accEmpty0 + a * 8);
+                    }
+                    add(r1, c + 1);
+                }
+                __syncwarp();  // every lane has read the block's scales
+                if (lane == 0) mbar_arrive(&sEmpty[ss]);
+            }
+            if (!ok) break;
+            epilogue<CT>(acc, p, &tmC, myOut, m0, n0, lane);
+        }
+        if (lane == 0) tma_store_wait_all<0>();
+        __syncwarp();
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();  // neither CTA leaves while the other may still reach its shared memory
+    if (warp == kPairEpi + 1) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem_base, 512);
+    }
+}
+
+template <int CT>
+bool c_map(CUtensorMap* tmC, const Fp8GemmArgs& p) {
+    constexpr int kEl = CT == kF32 ? 4 : 2;
+    return !p.tma_c || encode_2d(tmC, CT == kF32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                      : CT == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                    : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                                 p.C, p.N, p.M, p.ldc * kEl, 128 / kEl, 32, 128);
+}
+
+template <int CT>
+cudaError_t launch_pair(const Fp8GemmArgs& p, cudaStream_t stream) {
+    CUtensorMap tmA{}, tmB{}, tmC{};
+    if (p.K > 0 &&
+        (!encode_2d(&tmA, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.A, p.K, p.M, p.lda, kBK, 128, 128) ||
+         !encode_2d(&tmB, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.B, p.K, p.N, p.ldb, kBK, 128, 128)))
+        return cudaErrorInvalidValue;
+    if (!c_map<CT>(&tmC, p)) return cudaErrorInvalidValue;
+    auto kern = p.b_tile ? fp8_gemm_pair_kernel<0, CT> : fp8_gemm_pair_kernel<1, CT>;
+    const int smem = p.b_tile ? PairCfg<0>::kSmemBytes : PairCfg<1>::kSmemBytes;
+    cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), smem);
+    if (e != cudaSuccess) return e;
+    const int64_t tiles = static_cast<int64_t>((p.M + 255) / 256) * ((p.N + 255) / 256);
+    const int pairs = device_sm_count() / 2;
+    kern<<<2 * static_cast<int>(tiles < pairs ? tiles : pairs), kPairThreads, smem, stream>>>(tmA, tmB, tmC, p);
+    return cudaGetLastError();
+}
+
 template <int NT, int CT>
 cudaError_t launch(const Fp8GemmArgs& p, cudaStream_t stream) {
     using C = GemmCfg<NT>;
@@ -410,12 +711,7 @@ cudaError_t launch(const Fp8GemmArgs& p, cudaStream_t stream) {
          !encode_2d(&tmB, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.B, p.K, p.N, p.ldb, kBK, NT, 128)))
         return cudaErrorInvalidValue;
     CUtensorMap tmC{};
-    constexpr int kEl = CT == kF32 ? 4 : 2;
-    if (p.tma_c && !encode_2d(&tmC, CT == kF32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
-                                    : CT == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
-                                                  : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-                              p.C, p.N, p.M, p.ldc * kEl, 128 / kEl, 32, 128))
-        return cudaErrorInvalidValue;
+    if (!c_map<CT>(&tmC, p)) return cudaErrorInvalidValue;
     auto kern = p.b_tile ? fp8_gemm_kernel<NT, 0, CT> : fp8_gemm_kernel<NT, 1, CT>;
     cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), C::kSmemBytes);
     if (e != cudaSuccess) return e;
@@ -427,8 +723,8 @@ cudaError_t launch(const Fp8GemmArgs& p, cudaStream_t stream) {
 
 template <int CT>
 cudaError_t dispatch(const Fp8GemmArgs& p, cudaStream_t stream) {
-    const int64_t wide = static_cast<int64_t>((p.M + 127) / 128) * ((p.N + 255) / 256);
-    return wide >= device_sm_count() ? launch<256, CT>(p, stream) : launch<128, CT>(p, stream);
+    const int64_t wide = static_cast<int64_t>((p.M + 255) / 256) * ((p.N + 255) / 256);
+    return 2 * wide >= device_sm_count() ? launch_pair<CT>(p, stream) : launch<128, CT>(p, stream);
 }
 
 }  // namespace

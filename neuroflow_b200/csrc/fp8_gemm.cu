@@ -59,15 +59,19 @@ __device__ __forceinline__ void tmem_ld16_wait(uint32_t (&r)[16]) {
                  : "memory");
 }
 
-// GELU as z * sigmoid(2u) (the tanh form's identity), the exponential by ex2.approx.
-__device__ __forceinline__ float gelu_sig(float z) {
+// GELU as z * sigmoid(2u) (the tanh form's identity), the exponential by ex2.approx.  Two values
+// share a reciprocal, 1 / a = b / (a b) (the special-function unit bounds this epilogue); the
+// exponents are held under 2^60 so that the product stays finite, where z 2^-60 stands for a result
+// that is smaller still.
+__device__ __forceinline__ float2 gelu_sig2(float2 z) {
     const float c2 = -2.0f * 0.7978845608028654f * 1.4426950408889634f;
-    const float inner = fmaf(z, (0.044715f * z) * z, z);
-    float e;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(c2 * inner));
-    return __fdividef(z, 1.0f + e);
+    float2 e;
+    const float ux = c2 * fmaf(z.x, (0.044715f * z.x) * z.x, z.x), uy = c2 * fmaf(z.y, (0.044715f * z.y) * z.y, z.y);
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(fminf(ux, 60.0f)));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(fminf(uy, 60.0f)));
+    const float a = 1.0f + e.x, b = 1.0f + e.y, r = __fdividef(1.0f, a * b);
+    return make_float2(z.x * (r * b), z.y * (r * a));
 }
-
 template <int R>
 __device__ __forceinline__ void reg_inc() {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R));
@@ -77,11 +81,12 @@ __device__ __forceinline__ void reg_dec() {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R));
 }
 
-// Adds the bias (128 floats in shared memory) to one row's accumulators and applies the activation.
-__device__ __forceinline__ void finish_row(float2 (&acc)[64], const float* bias, int act) {
+// Adds the bias (2 NP floats in shared memory) to one row's accumulators and applies the activation.
+template <int NP>
+__device__ __forceinline__ void finish_row(float2 (&acc)[NP], const float* bias, int act) {
     if (bias) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
+        for (int j = 0; j < NP / 2; ++j) {
             const float4 v = *reinterpret_cast<const float4*>(bias + 4 * j);
             acc[2 * j].x += v.x, acc[2 * j].y += v.y;
             acc[2 * j + 1].x += v.z, acc[2 * j + 1].y += v.w;
@@ -89,16 +94,16 @@ __device__ __forceinline__ void finish_row(float2 (&acc)[64], const float* bias,
     }
     if (act == 1) {
 #pragma unroll
-        for (int j = 0; j < 64; ++j) acc[j] = make_float2(gelu_sig(acc[j].x), gelu_sig(acc[j].y));
+        for (int j = 0; j < NP; ++j) acc[j] = gelu_sig2(acc[j]);
     } else if (act == 2) {
 #pragma unroll
-        for (int j = 0; j < 64; ++j) acc[j] = make_float2(relu_ref(acc[j].x), relu_ref(acc[j].y));
+        for (int j = 0; j < NP; ++j) acc[j] = make_float2(relu_ref(acc[j].x), relu_ref(acc[j].y));
     }
 }
 
 // Columns c0 .. of a row as the bytes of one staging chunk (16 bytes).
-template <int CT>
-__device__ __forceinline__ uint4 pack_chunk(const float2 (&acc)[64], int j) {
+template <int CT, int NP>
+__device__ __forceinline__ uint4 pack_chunk(const float2 (&acc)[NP], int j) {
     uint4 v;
     if constexpr (CT == kF32) {
         v = make_uint4(__float_as_uint(acc[2 * j].x), __float_as_uint(acc[2 * j].y),
@@ -121,15 +126,15 @@ __device__ __forceinline__ uint4 pack_chunk(const float2 (&acc)[64], int j) {
     return v;
 }
 
-// A warp's 32 rows x 128 columns at (m0, n0) to C through its staging buffer `buf`, in boxes of 32
+// A warp's 32 rows x 2 NP columns at (m0, n0) to C through its staging buffer `buf`, in boxes of 32
 // rows x 128 bytes (the lane holds row m0 + lane).
-template <int CT>
-__device__ __forceinline__ void store_rows(const float2 (&acc)[64], const Fp8GemmArgs& p, const CUtensorMap* tmC,
+template <int CT, int NP>
+__device__ __forceinline__ void store_rows(const float2 (&acc)[NP], const Fp8GemmArgs& p, const CUtensorMap* tmC,
                                            uint8_t* buf, int m0, int n0, int lane) {
     constexpr int kEl = CT == kF32 ? 4 : 2;
     constexpr int kCols = 128 / kEl;  // columns of a box
 #pragma unroll
-    for (int b = 0; b < 128 / kCols; ++b) {
+    for (int b = 0; b < 2 * NP / kCols; ++b) {
         const int n = n0 + b * kCols;
         if (n >= p.N) break;
         if (p.tma_c) {  // the previous box has been read
@@ -138,7 +143,7 @@ __device__ __forceinline__ void store_rows(const float2 (&acc)[64], const Fp8Gem
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            *reinterpret_cast<uint4*>(buf + swz_offset(lane * 128 + j * 16, 128)) = pack_chunk<CT>(acc, b * 8 + j);
+            *reinterpret_cast<uint4*>(buf + swz_offset(lane * 128 + j * 16, 128)) = pack_chunk<CT, NP>(acc, b * 8 + j);
         // a TMA store clips its box at 16 bytes, not at the element: a last box whose row ends inside 16
         // bytes goes out by elements
         if (p.tma_c && (n + kCols <= p.N || p.N * kEl % 16 == 0)) {
@@ -173,27 +178,47 @@ __device__ __forceinline__ void tile_at(int t, int tm, int tn, int& m, int& n) {
     n = rem / h;
 }
 
+// W columns of this warp's TMEM lanes, complete on return.  Load and wait are one statement: a wait
+// that names the registers of earlier loads as its operands makes the compiler copy them, which cost
+// more than the overlap of the loads gained.
+__device__ __forceinline__ void tmem_read(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_read(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+}
+
 // A warp's finished accumulators (rows m0 + lane, columns n0 ..) to C, through its staging buffer.
-template <int CT>
-__device__ __forceinline__ void epilogue(float2 (&acc)[64], const Fp8GemmArgs& p, const CUtensorMap* tmC,
+template <int CT, int NP>
+__device__ __forceinline__ void epilogue(float2 (&acc)[NP], const Fp8GemmArgs& p, const CUtensorMap* tmC,
                                          uint8_t* buf, int m0, int n0, int lane) {
     float* sb = reinterpret_cast<float*>(buf);
     if (p.bias) {
-        float b[4];
+        float b[NP / 16];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < NP / 16; ++j) {
             const int n = n0 + j * 32 + lane;
             b[j] = n < p.N ? load_any(p.bias, p.btype, n) : 0.0f;
         }
         if (p.tma_c && lane == 0) tma_store_wait_read<0>();
         __syncwarp();
 #pragma unroll
-        for (int j = 0; j < 4; ++j) sb[j * 32 + lane] = b[j];
+        for (int j = 0; j < NP / 16; ++j) sb[j * 32 + lane] = b[j];
         __syncwarp();
     }
-    finish_row(acc, p.bias ? sb : nullptr, p.act);
+    finish_row<NP>(acc, p.bias ? sb : nullptr, p.act);
     __syncwarp();  // every lane has read the bias
-    if (m0 < p.M) store_rows<CT>(acc, p, tmC, buf, m0, n0, lane);
+    if (m0 < p.M) store_rows<CT, NP>(acc, p, tmC, buf, m0, n0, lane);
 }
 
 template <int NT, int COL, int CT>
@@ -394,7 +419,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             }
             if (!ok) break;
             __syncwarp();  // every lane has read the column scales
-            epilogue<CT>(acc, p, &tmC, myOut, mt * kBM + quad * 32, n0, lane);
+            epilogue<CT, 64>(acc, p, &tmC, myOut, mt * kBM + quad * 32, n0, lane);
         }
         if (lane == 0) tma_store_wait_all<0>();
         __syncwarp();
@@ -411,27 +436,37 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
 // COL: 0 the columns of a 128-column group share a scale (B in tiles), 1 one scale per column
 //
 // One tile is 256 x 256, computed by a pair of CTAs with cta_group::2 MMAs: CTA r holds rows
-// 128 r .. of the tile's A and of its B (so each operand byte is fetched once per pair, 64 KB for
-// 128 x 256 x 256 products instead of 96 KB by two CTAs alone), and rows 128 r .. of the result in
-// its TMEM.  Warps of each CTA:
-//   0-7    promotion and epilogue     8   TMA producer        9   TMEM owner; CTA 0's issues the MMAs
-//   10     scale producer (cp.async into a ring, several blocks ahead: a scale that is fetched in
+// 128 r .. of the tile's A and half the rows of its B (so each operand byte is fetched once per pair,
+// 64 KB for 128 x 256 x 256 products instead of 96 KB by two CTAs alone), and rows 128 r .. of the
+// result in its TMEM.  The tile's two column halves are separate MMAs (N = 128) with two TMEM stages
+// each, so a half's accumulators are handed over after 256 cycles and not after 512: the time from
+// an MMA's end to the reuse of its stage (barriers, TMEM reads) is what has to be covered.
+// Warps of each CTA:
+//   0-15   promotion and epilogue, 32 rows x 64 columns each    16  TMA producer
+//   17     TMEM owner; CTA 0's issues the MMAs
+//   18     scale producer (cp.async into a ring, several blocks ahead: a scale that is fetched in
 //          the promotion loop itself costs an L2 latency per block)
+// Sixteen promoting warps and not eight: a warp's loop is a chain of barrier, TMEM read and sums, and
+// four of them on a scheduler cover each other's latencies.  Their registers (64 accumulators, 32 on the
+// way from TMEM) are given up by the other four warps: 16 x 32 x 112 + 4 x 32 x 32 = 20 x 32 x 96.
 // Barriers: full (CTA 0's, both CTAs' bytes), empty and accFull (both CTAs', by commit), accEmpty (CTA
 // 0's, arrivals from the epilogue warps of both), sFull and sEmpty (each CTA's own scales).
-constexpr int kPairThreads = 384;
-constexpr int kPairEpi = 8;
+constexpr int kPairThreads = 640;
+constexpr int kPairEpi = 16;
 
 template <int COL>
 struct PairCfg {
-    static constexpr int kStages = 5;
+    static constexpr int kStages = 4;
+    // columns of one TMEM read: 8192 x 16384 x 4096 takes 525 us with 32 and 583 with 16 where the
+    // columns share a scale, 798 and 713 where the column scales take registers too
+    static constexpr int kRead = COL ? 16 : 32;
     static constexpr int kStageBytes = 2 * 128 * kBK;
     static constexpr int kScaleStages = 8;
     static constexpr int kScaleBytes = (128 + (COL ? 256 : 4)) * 4;
     static constexpr int kOffOut = kStages * kStageBytes;
     static constexpr int kOffScale = kOffOut + kPairEpi * kOutBytes;
     static constexpr int kOffBars = kOffScale + kScaleStages * kScaleBytes;
-    static constexpr int kSmemBytes = kOffBars + 8 * (2 * kStages + 2 * 2 + 2 * kScaleStages) + 16 + 1024;
+    static constexpr int kSmemBytes = kOffBars + 8 * (2 * kStages + 2 * 4 + 2 * kScaleStages) + 16 + 1024;
     static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
 };
 
@@ -445,8 +480,8 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kOffBars);
     uint64_t* empty = full + C::kStages;
     uint64_t* accFull = empty + C::kStages;
-    uint64_t* accEmpty = accFull + 2;
-    uint64_t* sFull = accEmpty + 2;
+    uint64_t* accEmpty = accFull + 4;
+    uint64_t* sFull = accEmpty + 4;
     uint64_t* sEmpty = sFull + C::kScaleStages;
     uint32_t* sTmem = reinterpret_cast<uint32_t*>(sEmpty + C::kScaleStages);
     volatile int* sAbort = reinterpret_cast<volatile int*>(sTmem + 1);
@@ -465,9 +500,9 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
         }
-        for (int s = 0; s < 2; ++s) {
+        for (int s = 0; s < 4; ++s) {  // stage * 2 + column half
             mbar_init(&accFull[s], 1);
-            mbar_init(&accEmpty[s], 2 * kPairEpi);
+            mbar_init(&accEmpty[s], kPairEpi);
         }
         for (int s = 0; s < C::kScaleStages; ++s) {
             mbar_init(&sFull[s], 32);
@@ -486,7 +521,7 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
     // the register split stands inside the roles' branches: where they met again, the compiler would
     // have to assume the smaller count
     if (warp >= kPairEpi) {
-        reg_dec<88>();
+        reg_dec<32>();
         if (warp == kPairEpi) {
             // ---------------- TMA producer
             if (elect_one()) {
@@ -507,7 +542,9 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
                         const uint32_t bar = map_rank(smem_u32(&full[s]), 0);
                         uint8_t* st = smem + s * C::kStageBytes;
                         tma_load_2d_pair(st, &tmA, bar, kb * kBK, mt * 256 + rank * 128);
-                        tma_load_2d_pair(st + 128 * kBK, &tmB, bar, kb * kBK, nt * 256 + rank * 128);
+                        // 64 rows of each column half: the half's other 64 are the other CTA's
+                        tma_load_2d_pair(st + 128 * kBK, &tmB, bar, kb * kBK, nt * 256 + rank * 64);
+                        tma_load_2d_pair(st + 192 * kBK, &tmB, bar, kb * kBK, nt * 256 + 128 + rank * 64);
                     }
                 }
                 // every load that was issued has landed and been read before the CTA exits
@@ -521,35 +558,43 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
         } else if (warp == kPairEpi + 1) {
             // ---------------- MMA issuer
             if (rank == 0 && elect_one()) {
-                int it = 0;
+                int it = 0, issued = -1;
+                uint32_t parity = 0;
                 bool ok = true;
                 for (int t = first; ok && t < tiles; t += step) {
                     for (int kb = 0; kb < KB; ++kb, ++it) {
-                        const int s = it % C::kStages, a = it & 1;
-                        if (!mbar_wait(&accEmpty[a], ((it >> 1) & 1) ^ 1, sAbort, budget)) {
-                            *sAbort = 1;
-                            atomicOr(p.err, kErrWaitAccFree);
-                            ok = false;
-                            break;
-                        }
+                        const int s = it % C::kStages, a = (it & 1) * 2;
                         if (!mbar_wait(&full[s], (it / C::kStages) & 1, sAbort, budget)) {
                             *sAbort = 1;
                             atomicOr(p.err, kErrWaitTmaFull);
                             ok = false;
                             break;
                         }
-                        tc_fence_after();
                         const uint32_t ab = smem_u32(smem + s * C::kStageBytes), bb = ab + 128 * kBK;
 #pragma unroll
-                        for (int k = 0; k < kBK / 32; ++k)
-                            mma_f8_pair(tmem_base + a * 256, umma_desc(ab + 32 * k, 128), umma_desc(bb + 32 * k, 128),
-                                        idesc_e4m3_pair(256), k > 0 ? 1u : 0u);
-                        mma_commit_pair(&empty[s]);
-                        mma_commit_pair(&accFull[a]);
+                        for (int h = 0; h < 2; ++h) {
+                            if (ok && !mbar_wait(&accEmpty[a + h], ((it >> 1) & 1) ^ 1, sAbort, budget)) {
+                                *sAbort = 1;
+                                atomicOr(p.err, kErrWaitAccFree);
+                                ok = false;
+                            }
+                            if (!ok) break;
+                            tc_fence_after();
+#pragma unroll
+                            for (int k = 0; k < kBK / 32; ++k)
+                                mma_f8_pair(tmem_base + (a + h) * 128, umma_desc(ab + 32 * k, 128),
+                                            umma_desc(bb + h * 64 * kBK + 32 * k, 128), idesc_e4m3_pair(128),
+                                            k > 0 ? 1u : 0u);
+                            if (h == 1) mma_commit_pair(&empty[s]);
+                            mma_commit_pair(&accFull[a + h]);
+                            issued = a + h;
+                            parity = (it >> 1) & 1;
+                        }
+                        if (!ok) break;
                     }
                 }
                 // the last commit completes before TMEM is released
-                if (it > 0 && !mbar_wait_drain(&accFull[(it - 1) & 1], ((it - 1) >> 1) & 1))
+                if (issued >= 0 && !mbar_wait_drain(&accFull[issued], parity))
                     atomicOr(p.err, kErrWaitDrain);
             }
             __syncwarp();
@@ -569,7 +614,7 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
                 }
                 for (int kb = 0; kb < KB; ++kb, ++it) {
                     const int s = it % C::kScaleStages;
-                    if (!mbar_wait(&sEmpty[s], ((it / C::kScaleStages) & 1) ^ 1, sAbort, budget)) {
+                    if (!mbar_wait_backoff(&sEmpty[s], ((it / C::kScaleStages) & 1) ^ 1, sAbort, 128, 32, budget)) {
                         *sAbort = 1;
                         atomicOr(p.err, kErrWaitSlotFree);
                         ok = false;
@@ -596,22 +641,18 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
         }
     } else {
         // ---------------- promotion and epilogue
-        reg_inc<208>();
-        const int quad = warp & 3, grp = warp >> 2;
-        uint8_t* myOut = smem + C::kOffOut + warp * kOutBytes;
+        reg_inc<112>();
+        constexpr int W = C::kRead;
+        const int quad = warp & 3, part = warp >> 2, half = part >> 1;
         const uint32_t accEmpty0 = map_rank(smem_u32(accEmpty), 0);
         int it = 0;
         bool ok = true;
         for (int t = first; ok && t < tiles; t += step) {
-            int mt, nt;
-            tile_at(t, tm, tn, mt, nt);
-            const int m0 = mt * 256 + rank * 128 + quad * 32;
-            const int n0 = nt * 256 + grp * 128;
-            float2 acc[64];
+            float2 acc[32];
 #pragma unroll
-            for (int j = 0; j < 64; ++j) acc[j] = make_float2(0.0f, 0.0f);
+            for (int j = 0; j < 32; ++j) acc[j] = make_float2(0.0f, 0.0f);
             for (int kb = 0; kb < KB; ++kb, ++it) {
-                const int a = it & 1, ss = it % C::kScaleStages;
+                const int a = (it & 1) * 2 + half, ss = it % C::kScaleStages;
                 const float* sc = reinterpret_cast<const float*>(smem + C::kOffScale + ss * C::kScaleBytes);
                 if (!mbar_wait(&sFull[ss], (it / C::kScaleStages) & 1, sAbort, budget) ||
                     !mbar_wait(&accFull[a], (it >> 1) & 1, sAbort, budget)) {
@@ -622,45 +663,41 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
                 }
                 tc_fence_after();
                 float s = sc[quad * 32 + lane];
-                if constexpr (COL == 0) s *= sc[128 + grp];
-                const uint32_t tb = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + a * 256 + grp * 128;
-                uint32_t r0[16], r1[16];
-                auto add = [&](const uint32_t (&r)[16], int c) {
+                if constexpr (COL == 0) s *= sc[128 + half];
+                const uint32_t tb =
+                    tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + a * 128 + (part & 1) * 64;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        float2 f0 = make_float2(s, s), f1 = f0;
-                        if constexpr (COL == 1) {
-                            const float4 cs = *reinterpret_cast<const float4*>(sc + 128 + grp * 128 + c * 16 + 4 * j);
-                            f0 = mul2_rn(f0, make_float2(cs.x, cs.y));
-                            f1 = mul2_rn(f1, make_float2(cs.z, cs.w));
-                        }
-                        acc[c * 8 + 2 * j] = fma2_rn(make_float2(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1])),
-                                                     f0, acc[c * 8 + 2 * j]);
-                        acc[c * 8 + 2 * j + 1] = fma2_rn(
-                            make_float2(__uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3])), f1, acc[c * 8 + 2 * j + 1]);
-                    }
-                };
-                tmem_ld16(tb, r0);
-#pragma unroll
-                for (int c = 0; c < 8; c += 2) {
-                    tmem_ld16_wait(r0);
-                    tmem_ld16(tb + (c + 1) * 16, r1);
-                    add(r0, c);
-                    tmem_ld16_wait(r1);
-                    if (c + 2 < 8) {
-                        tmem_ld16(tb + (c + 2) * 16, r0);
-                    } else {
+                for (int c = 0; c < 64 / W; ++c) {
+                    uint32_t r[W];
+                    tmem_read(tb + c * W, r);
+                    if (c == 64 / W - 1) {
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) mbar_arrive_cluster(accEmpty0 + a * 8);
                     }
-                    add(r1, c + 1);
+#pragma unroll
+                    for (int j = 0; j < W / 4; ++j) {
+                        float2 f0 = make_float2(s, s), f1 = f0;
+                        if constexpr (COL == 1) {
+                            const float4 cs = *reinterpret_cast<const float4*>(sc + 128 + part * 64 + c * W + 4 * j);
+                            f0 = mul2_rn(f0, make_float2(cs.x, cs.y));
+                            f1 = mul2_rn(f1, make_float2(cs.z, cs.w));
+                        }
+                        float2& a0 = acc[c * (W / 2) + 2 * j];
+                        float2& a1 = acc[c * (W / 2) + 2 * j + 1];
+                        a0 = fma2_rn(make_float2(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1])), f0, a0);
+                        a1 = fma2_rn(make_float2(__uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3])), f1, a1);
+                    }
                 }
                 __syncwarp();  // every lane has read the block's scales
                 if (lane == 0) mbar_arrive(&sEmpty[ss]);
             }
             if (!ok) break;
-            epilogue<CT>(acc, p, &tmC, myOut, m0, n0, lane);
+            // (the tile's place is found only now: registers are short in the loop above)
+            int mt, nt;
+            tile_at(t, tm, tn, mt, nt);
+            epilogue<CT, 32>(acc, p, &tmC, smem + C::kOffOut + warp * kOutBytes, mt * 256 + rank * 128 + quad * 32,
+                             nt * 256 + part * 64, lane);
         }
         if (lane == 0) tma_store_wait_all<0>();
         __syncwarp();
@@ -689,7 +726,7 @@ cudaError_t launch_pair(const Fp8GemmArgs& p, cudaStream_t stream) {
     CUtensorMap tmA{}, tmB{}, tmC{};
     if (p.K > 0 &&
         (!encode_2d(&tmA, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.A, p.K, p.M, p.lda, kBK, 128, 128) ||
-         !encode_2d(&tmB, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.B, p.K, p.N, p.ldb, kBK, 128, 128)))
+         !encode_2d(&tmB, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.B, p.K, p.N, p.ldb, kBK, 64, 128)))
         return cudaErrorInvalidValue;
     if (!c_map<CT>(&tmC, p)) return cudaErrorInvalidValue;
     auto kern = p.b_tile ? fp8_gemm_pair_kernel<0, CT> : fp8_gemm_pair_kernel<1, CT>;

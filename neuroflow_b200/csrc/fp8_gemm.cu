@@ -8,15 +8,16 @@
 // the block's scales and add it to fp32 accumulators in registers, so the sum over the blocks is
 // fp32 and no product of scales is rounded to fewer bits.
 //
-// Structure (persistent, one CTA per SM, 128 x NT tiles):
-//   warps 0 ..      promotion and epilogue: NT / 128 groups of four warps, a warp owning the 32
-//                   TMEM lanes 32 * (warp % 4) .. and 128 columns; the result leaves through a
-//                   swizzled 4 KB staging buffer per warp (TMA stores of 32 rows x 128 bytes, or
-//                   coalesced element stores where C's rows are not 16-byte aligned)
-//   then 4 warps    TMA producer (ring of kStages stages: 128 x 128 of A, NT x 128 of B), TMEM
-//                   owner and MMA issuer, two idle
-// With NT = 256 the accumulators take 128 registers of each epilogue thread: the last four warps
-// give registers up to them (setmaxnreg; 8 x 32 x 208 + 4 x 32 x 88 = 12 x 32 x 168 at launch).
+// Two kernels: pairs of CTAs on 256 x 256 tiles for large results, and a narrow one, with K split
+// over a cluster, for few rows of A or few tiles; dispatch() below chooses.  Both are
+// warp-specialised: a TMA producer, an MMA issuer, a scale producer, and the promoting warps.
+//
+// Measured (one B200; HBM 6,457 GB/s, FP8 taken as twice the measured bf16 rate, 3,276 TFLOP/s):
+//   8192x16384x4096 to bf16   524 us, 2,100 TFLOP/s, at the 1,000 W power cap (1.5 GHz); 573 us with
+//                             bias and GELU.  A block of K takes 824 cycles where its MMAs take 512:
+//                             without the sums 670, without TMEM reads too 650 (barrier hand-over)
+//   4096x4096x8192 to fp32    about 195 us with column scales (a second multiply per element)
+//   1x4096x4096               6.4 us, of which 4.9 are the start and the join (1x1024x1024 takes that)
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -30,34 +31,8 @@
 namespace nfx {
 namespace {
 
-constexpr int kBM = 128;
 constexpr int kBK = kGroup;
 constexpr int kOutBytes = 32 * 128;  // one staging buffer
-
-template <int NT>
-struct GemmCfg {
-    static constexpr int kEpiWarps = 4 * (NT / 128);
-    static constexpr int kThreads = 32 * (kEpiWarps + 4);
-    static constexpr int kABytes = kBM * kBK;
-    static constexpr int kBBytes = NT * kBK;
-    static constexpr int kStageBytes = kABytes + kBBytes;
-    static constexpr int kStages = NT == 256 ? 4 : 6;
-    static constexpr int kAccStages = 512 / NT;
-    // per epilogue warp: two sets of 128 column scales during a tile, the staging buffer after it
-    static constexpr int kOffOut = kStages * kStageBytes;
-    static constexpr int kOffBars = kOffOut + kEpiWarps * kOutBytes;
-    static constexpr int kSmemBytes = kOffBars + 8 * (2 * kStages + 2 * kAccStages) + 16 + 1024;
-    static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
-};
-
-__device__ __forceinline__ void tmem_ld16_wait(uint32_t (&r)[16]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]),
-                   "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]),
-                   "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
-                 :
-                 : "memory");
-}
 
 // GELU as z * sigmoid(2u) (the tanh form's identity), the exponential by ex2.approx.  Two values
 // share a reciprocal, 1 / a = b / (a b) (the special-function unit bounds this epilogue); the
@@ -101,6 +76,16 @@ __device__ __forceinline__ void finish_row(float2 (&acc)[NP], const float* bias,
     }
 }
 
+template <int CT>
+__device__ __forceinline__ uint32_t pack_half(float2 a) {
+    if constexpr (CT == kBF16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a.x, a.y);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+        const __half2 h = __floats2half2_rn(a.x, a.y);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+}
 // Columns c0 .. of a row as the bytes of one staging chunk (16 bytes).
 template <int CT, int NP>
 __device__ __forceinline__ uint4 pack_chunk(const float2 (&acc)[NP], int j) {
@@ -111,16 +96,7 @@ __device__ __forceinline__ uint4 pack_chunk(const float2 (&acc)[NP], int j) {
     } else {
         uint32_t w[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 a = acc[4 * j + i];
-            if constexpr (CT == kBF16) {
-                const __nv_bfloat162 h = __floats2bfloat162_rn(a.x, a.y);
-                w[i] = *reinterpret_cast<const uint32_t*>(&h);
-            } else {
-                const __half2 h = __floats2half2_rn(a.x, a.y);
-                w[i] = *reinterpret_cast<const uint32_t*>(&h);
-            }
-        }
+        for (int i = 0; i < 4; ++i) w[i] = pack_half<CT>(acc[4 * j + i]);
         v = make_uint4(w[0], w[1], w[2], w[3]);
     }
     return v;
@@ -219,218 +195,6 @@ __device__ __forceinline__ void epilogue(float2 (&acc)[NP], const Fp8GemmArgs& p
     finish_row<NP>(acc, p.bias ? sb : nullptr, p.act);
     __syncwarp();  // every lane has read the bias
     if (m0 < p.M) store_rows<CT, NP>(acc, p, tmC, buf, m0, n0, lane);
-}
-
-template <int NT, int COL, int CT>
-__global__ void __launch_bounds__(GemmCfg<NT>::kThreads, 1)
-fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                const __grid_constant__ CUtensorMap tmC, const Fp8GemmArgs p) {
-    using C = GemmCfg<NT>;
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kOffBars);
-    uint64_t* empty = full + C::kStages;
-    uint64_t* accFull = empty + C::kStages;
-    uint64_t* accEmpty = accFull + C::kAccStages;
-    uint32_t* sTmem = reinterpret_cast<uint32_t*>(accEmpty + C::kAccStages);
-    volatile int* sAbort = reinterpret_cast<volatile int*>(sTmem + 1);
-
-    const int warp = threadIdx.x >> 5;
-    const int lane = threadIdx.x & 31;
-    const int tm = (p.M + kBM - 1) / kBM, tn = (p.N + NT - 1) / NT;
-    const int tiles = tm * tn;
-    const int KB = (p.K + kBK - 1) / kBK;
-    const uint64_t budget = p.wait_ns ? p.wait_ns : kWaitNs;
-
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < C::kStages; ++s) {
-            mbar_init(&full[s], 1);
-            mbar_init(&empty[s], 1);
-        }
-        for (int s = 0; s < C::kAccStages; ++s) {
-            mbar_init(&accFull[s], 1);
-            mbar_init(&accEmpty[s], C::kEpiWarps);
-        }
-        *sAbort = 0;
-        fence_mbar_init();
-    }
-    if (warp == C::kEpiWarps + 1) tmem_alloc(sTmem, 512);
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem_base = *sTmem;
-
-    // the register split stands inside the roles' branches: where they met again, the compiler would
-    // have to assume the smaller count
-    if (warp >= C::kEpiWarps) {
-        if constexpr (NT == 256) reg_dec<88>();
-    if (warp == C::kEpiWarps) {
-        // ---------------- TMA producer
-        if (elect_one()) {
-            int it = 0;
-            bool ok = true;
-            for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
-                int mt, nt;
-                tile_at(t, tm, tn, mt, nt);
-                for (int kb = 0; kb < KB; ++kb, ++it) {
-                    const int s = it % C::kStages;
-                    const uint32_t ph = (it / C::kStages) & 1;
-                    if (!mbar_wait_backoff(&empty[s], ph ^ 1, sAbort, 128, 32, budget)) {
-                        *sAbort = 1;
-                        atomicOr(p.err, kErrWaitSlotFree);
-                        ok = false;
-                        break;
-                    }
-                    mbar_arrive_expect_tx(&full[s], C::kStageBytes);
-                    uint8_t* st = smem + s * C::kStageBytes;
-                    tma_load_2d(st, &tmA, &full[s], kb * kBK, mt * kBM);
-                    tma_load_2d(st + C::kABytes, &tmB, &full[s], kb * kBK, nt * NT);
-                }
-            }
-            // every load that was issued lands before the CTA exits
-            for (int j = it > C::kStages ? it - C::kStages : 0; j < it; ++j)
-                if (!mbar_wait_drain(&full[j % C::kStages], (j / C::kStages) & 1)) {
-                    atomicOr(p.err, kErrWaitDrain);
-                    break;
-                }
-        }
-        __syncwarp();
-    } else if (warp == C::kEpiWarps + 1) {
-        // ---------------- MMA issuer
-        if (elect_one()) {
-            int it = 0;
-            bool ok = true;
-            for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
-                for (int kb = 0; kb < KB; ++kb, ++it) {
-                    const int s = it % C::kStages, a = it % C::kAccStages;
-                    if (!mbar_wait(&accEmpty[a], ((it / C::kAccStages) & 1) ^ 1, sAbort, budget)) {
-                        *sAbort = 1;
-                        atomicOr(p.err, kErrWaitAccFree);
-                        ok = false;
-                        break;
-                    }
-                    if (!mbar_wait(&full[s], (it / C::kStages) & 1, sAbort, budget)) {
-                        *sAbort = 1;
-                        atomicOr(p.err, kErrWaitTmaFull);
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
-                    const uint32_t ab = smem_u32(smem + s * C::kStageBytes), bb = ab + C::kABytes;
-#pragma unroll
-                    for (int k = 0; k < kBK / 32; ++k)
-                        mma_f8(tmem_base + a * NT, umma_desc(ab + 32 * k, 128), umma_desc(bb + 32 * k, 128),
-                               idesc_e4m3(NT), k > 0 ? 1u : 0u);
-                    mma_commit(&empty[s]);
-                    mma_commit(&accFull[a]);
-                }
-            }
-            // the last commit completes before TMEM is released
-            if (it > 0 && !mbar_wait_drain(&accFull[(it - 1) % C::kAccStages], ((it - 1) / C::kAccStages) & 1))
-                atomicOr(p.err, kErrWaitDrain);
-        }
-        __syncwarp();
-    }
-    } else {
-        // ---------------- promotion and epilogue
-        if constexpr (NT == 256) reg_inc<208>();
-        const int quad = warp & 3, grp = warp >> 2;
-        uint8_t* myOut = smem + C::kOffOut + warp * kOutBytes;
-        float* myScale = reinterpret_cast<float*>(myOut);
-        int it = 0;
-        bool ok = true;
-        for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
-            int mt, nt;
-            tile_at(t, tm, tn, mt, nt);
-            const int m = mt * kBM + quad * 32 + lane;
-            const int n0 = nt * NT + grp * 128;
-            const int mc = min(m, p.M - 1);
-            const float* sa = p.sa + static_cast<int64_t>(p.a_tile ? mc / 128 : mc) * p.sars;
-            const float* sb = p.sb + static_cast<int64_t>(min(n0, p.N - 1) / 128) * p.sbrs;
-            float2 acc[64];
-#pragma unroll
-            for (int j = 0; j < 64; ++j) acc[j] = make_float2(0.0f, 0.0f);
-            float sc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            auto load_scales = [&](int kb, float& a) {
-                a = 0.0f;
-                if (kb >= KB) return;
-                a = __ldg(sa + kb * p.sabs);
-                if constexpr (COL == 0) {
-                    a *= __ldg(sb + kb * p.sbbs);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int n = n0 + j * 32 + lane;
-                        sc[j] = n < p.N ? __ldg(p.sb + static_cast<int64_t>(n) * p.sbrs + kb * p.sbbs) : 0.0f;
-                    }
-                }
-            };
-            float s_next;
-            load_scales(0, s_next);
-            if (COL == 1 && p.tma_c) {  // the last tile's box has been read
-                if (lane == 0) tma_store_wait_read<0>();
-                __syncwarp();
-            }
-            for (int kb = 0; kb < KB; ++kb, ++it) {
-                const float s = s_next;
-                const float* cs = myScale + (kb & 1) * 128;
-                if constexpr (COL == 1) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) myScale[(kb & 1) * 128 + j * 32 + lane] = sc[j];
-                    __syncwarp();
-                }
-                load_scales(kb + 1, s_next);
-                const int a = it % C::kAccStages;
-                if (!mbar_wait(&accFull[a], (it / C::kAccStages) & 1, sAbort, budget)) {
-                    *sAbort = 1;
-                    atomicOr(p.err, kErrWaitAccFull);
-                    ok = false;
-                    break;
-                }
-                tc_fence_after();
-                const uint32_t tb = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + a * NT + grp * 128;
-                uint32_t r0[16], r1[16];
-                auto add = [&](const uint32_t (&r)[16], int c) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const float2 d = make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
-                        float2 f = make_float2(s, s);
-                        if constexpr (COL == 1)
-                            f = mul2_rn(f, *reinterpret_cast<const float2*>(cs + c * 16 + 2 * j));
-                        acc[c * 8 + j] = fma2_rn(d, f, acc[c * 8 + j]);
-                    }
-                };
-                tmem_ld16(tb, r0);
-#pragma unroll
-                for (int c = 0; c < 8; c += 2) {
-                    tmem_ld16_wait(r0);
-                    tmem_ld16(tb + (c + 1) * 16, r1);
-                    add(r0, c);
-                    tmem_ld16_wait(r1);
-                    if (c + 2 < 8) {
-                        tmem_ld16(tb + (c + 2) * 16, r0);
-                    } else {
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&accEmpty[a]);
-                    }
-                    add(r1, c + 1);
-                }
-            }
-            if (!ok) break;
-            __syncwarp();  // every lane has read the column scales
-            epilogue<CT, 64>(acc, p, &tmC, myOut, mt * kBM + quad * 32, n0, lane);
-        }
-        if (lane == 0) tma_store_wait_all<0>();
-        __syncwarp();
-    }
-
-    tc_fence_before();
-    __syncthreads();
-    if (warp == C::kEpiWarps + 1) {
-        tc_fence_after();
-        tmem_dealloc(tmem_base, 512);
-    }
 }
 
 // COL: 0 the columns of a 128-column group share a scale (B in tiles), 1 one scale per column
@@ -739,29 +503,335 @@ cudaError_t launch_pair(const Fp8GemmArgs& p, cudaStream_t stream) {
     return cudaGetLastError();
 }
 
-template <int NT, int CT>
-cudaError_t launch(const Fp8GemmArgs& p, cudaStream_t stream) {
-    using C = GemmCfg<NT>;
-    CUtensorMap tmA{}, tmB{};
-    if (p.K > 0 &&
-        (!encode_2d(&tmA, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.A, p.K, p.M, p.lda, kBK, kBM, 128) ||
-         !encode_2d(&tmB, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.B, p.K, p.N, p.ldb, kBK, NT, 128)))
-        return cudaErrorInvalidValue;
-    CUtensorMap tmC{};
-    if (!c_map<CT>(&tmC, p)) return cudaErrorInvalidValue;
-    auto kern = p.b_tile ? fp8_gemm_kernel<NT, 0, CT> : fp8_gemm_kernel<NT, 1, CT>;
-    cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), C::kSmemBytes);
-    if (e != cudaSuccess) return e;
-    const int64_t tiles = static_cast<int64_t>((p.M + kBM - 1) / kBM) * ((p.N + NT - 1) / NT);
-    const int sms = device_sm_count();
-    kern<<<static_cast<int>(tiles < sms ? tiles : sms), C::kThreads, C::kSmemBytes, stream>>>(tmA, tmB, tmC, p);
-    return cudaGetLastError();
+// The narrow kernel, for few rows of A (a token to a few hundred): rows of B (weights) on the 128 lanes
+// of the MMA and NT rows of A as its columns, so that a product with few rows does not pad them to
+// 128, and K split over the CTAs of a cluster so that all SMs read weights.  Each CTA sums its share of
+// the blocks, puts the partial tile into its shared memory, and after a cluster barrier every CTA adds
+// the partials of its columns in the order of the ranks (deterministic; no atomics, no workspace),
+// applies bias and activation and stores.  Two CTAs per SM up to NT = 64.  Warps: four of promotion for
+// each 32 columns (a warp reads 32 x 32 accumulators a block), then one TMA producer, one TMEM owner and
+// MMA issuer, one scale producer.
+template <int NT>
+struct NarrowCfg {
+    static constexpr int kPart = NT < 32 ? NT : 32;  // columns of a promoting warp
+    static constexpr int kEpi = 4 * (NT / kPart);
+    static constexpr int kThreads = 32 * (kEpi + 4);
+    static constexpr int kPerSm = NT > 64 ? 1 : 2;
+    static constexpr int kABytes = 128 * kBK;
+    static constexpr int kStageBytes = kABytes + NT * kBK;
+    static constexpr int kStages = (NT > 64 ? 163840 : 98304) / kStageBytes;
+    static constexpr int kAcc = 4;
+    static constexpr int kTmem = NT * kAcc;
+    static constexpr int kScaleStages = 8;
+    static constexpr int kScaleBytes = (128 + NT) * 4;
+    static constexpr int kOffScale = kStages * kStageBytes;
+    static constexpr int kOffBars = kOffScale + kScaleStages * kScaleBytes;
+    static constexpr int kSmemBytes = kOffBars + 8 * (2 * kStages + 2 * kAcc + 2 * kScaleStages) + 16 + 1024;
+    static_assert(kPerSm * (kSmemBytes + 1024) <= 228 * 1024, "CTAs per SM");
+    static_assert(128 * NT * 4 <= kStages * kStageBytes, "the partial tile takes the place of the stages");
+};
+
+__device__ __forceinline__ float4 ld_cluster4(uint32_t cluster_addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(cluster_addr)
+                 : "memory");
+    return v;
 }
 
+template <int NT, int CT>
+__global__ void __launch_bounds__(NarrowCfg<NT>::kThreads, NarrowCfg<NT>::kPerSm)
+fp8_gemm_narrow_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
+                       const Fp8GemmArgs p, const int split) {
+    using C = NarrowCfg<NT>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kOffBars);
+    uint64_t* empty = full + C::kStages;
+    uint64_t* accFull = empty + C::kStages;
+    uint64_t* accEmpty = accFull + C::kAcc;
+    uint64_t* sFull = accEmpty + C::kAcc;
+    uint64_t* sEmpty = sFull + C::kScaleStages;
+    uint32_t* sTmem = reinterpret_cast<uint32_t*>(sEmpty + C::kScaleStages);
+    volatile int* sAbort = reinterpret_cast<volatile int*>(sTmem + 1);
+
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const int rank = blockIdx.x % split, tile = blockIdx.x / split;  // a cluster is `split` blocks in a row
+    const int tx = (p.M + NT - 1) / NT;
+    const int n0 = tile / tx * 128, m0 = tile % tx * NT;
+    const int KB = (p.K + kBK - 1) / kBK;
+    const int kb0 = static_cast<int>(static_cast<int64_t>(KB) * rank / split);
+    const int count = static_cast<int>(static_cast<int64_t>(KB) * (rank + 1) / split) - kb0;
+    const uint64_t budget = p.wait_ns ? p.wait_ns : kWaitNs;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::kStages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int s = 0; s < C::kAcc; ++s) {
+            mbar_init(&accFull[s], 1);
+            mbar_init(&accEmpty[s], C::kEpi);
+        }
+        for (int s = 0; s < C::kScaleStages; ++s) {
+            mbar_init(&sFull[s], 32);
+            mbar_init(&sEmpty[s], C::kEpi);
+        }
+        *sAbort = 0;
+        fence_mbar_init();
+    }
+    if (warp == C::kEpi + 1) tmem_alloc(sTmem, C::kTmem);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *sTmem;
+    float* part = reinterpret_cast<float*>(smem);  // (NT, 128) partial sums, after the last block
+
+    if (warp == C::kEpi) {
+        // ---------------- TMA producer
+        if (elect_one()) {
+            int it = 0;
+            for (; it < count; ++it) {
+                const int s = it % C::kStages;
+                if (!mbar_wait(&empty[s], ((it / C::kStages) & 1) ^ 1, sAbort, budget)) {
+                    *sAbort = 1;
+                    atomicOr(p.err, kErrWaitSlotFree);
+                    break;
+                }
+                mbar_arrive_expect_tx(&full[s], C::kStageBytes);
+                uint8_t* st = smem + s * C::kStageBytes;
+                tma_load_2d(st, &tmW, &full[s], (kb0 + it) * kBK, n0);
+                tma_load_2d(st + C::kABytes, &tmX, &full[s], (kb0 + it) * kBK, m0);
+            }
+            // every load that was issued lands before the CTA exits
+            for (int j = it > C::kStages ? it - C::kStages : 0; j < it; ++j)
+                if (!mbar_wait_drain(&full[j % C::kStages], (j / C::kStages) & 1)) {
+                    atomicOr(p.err, kErrWaitDrain);
+                    break;
+                }
+        }
+        __syncwarp();
+    } else if (warp == C::kEpi + 1) {
+        // ---------------- MMA issuer
+        if (elect_one()) {
+            int it = 0;
+            for (; it < count; ++it) {
+                const int s = it % C::kStages, a = it % C::kAcc;
+                const bool free = mbar_wait(&accEmpty[a], ((it / C::kAcc) & 1) ^ 1, sAbort, budget);
+                if (!free || !mbar_wait(&full[s], (it / C::kStages) & 1, sAbort, budget)) {
+                    *sAbort = 1;
+                    atomicOr(p.err, free ? kErrWaitTmaFull : kErrWaitAccFree);
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t ab = smem_u32(smem + s * C::kStageBytes), bb = ab + C::kABytes;
+#pragma unroll
+                for (int k = 0; k < kBK / 32; ++k)
+                    mma_f8(tmem_base + a * NT, umma_desc(ab + 32 * k, 128), umma_desc(bb + 32 * k, 128), idesc_e4m3(NT),
+                           k > 0 ? 1u : 0u);
+                mma_commit(&empty[s]);
+                mma_commit(&accFull[a]);
+            }
+            // the last commit completes before TMEM is released
+            if (it > 0 && !mbar_wait_drain(&accFull[(it - 1) % C::kAcc], ((it - 1) / C::kAcc) & 1))
+                atomicOr(p.err, kErrWaitDrain);
+        }
+        __syncwarp();
+    } else if (warp == C::kEpi + 2) {
+        // ---------------- scale producer
+        const float* src[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int n = min(n0 + j * 32 + lane, p.N - 1);
+            src[j] = p.sb + static_cast<int64_t>(p.b_tile ? n / 128 : n) * p.sbrs;
+        }
+        for (int it = 0; it < count; ++it) {
+            const int s = it % C::kScaleStages, kb = kb0 + it;
+            if (!mbar_wait_backoff(&sEmpty[s], ((it / C::kScaleStages) & 1) ^ 1, sAbort, 128, 32, budget)) {
+                *sAbort = 1;
+                atomicOr(p.err, kErrWaitSlotFree);
+                break;
+            }
+            float* dst = reinterpret_cast<float*>(smem + C::kOffScale + s * C::kScaleBytes);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) cp_async4(dst + j * 32 + lane, src[j] + kb * p.sbbs, true);
+#pragma unroll
+            for (int j = 0; j < NT; j += 32) {
+                const int m = m0 + j + lane;
+                if (j + lane < NT)
+                    cp_async4(dst + 128 + j + lane,
+                              p.sa + static_cast<int64_t>(min(m, p.M - 1) / (p.a_tile ? 128 : 1)) * p.sars + kb * p.sabs,
+                              m < p.M);
+            }
+            cp_async_arrive(&sFull[s]);
+        }
+        cp_async_wait_all();
+    } else if (warp < C::kEpi) {
+        // ---------------- promotion
+        constexpr int W = C::kPart;
+        const int quad = warp & 3, col0 = (warp >> 2) * W;
+        float2 acc[W / 2];
+#pragma unroll
+        for (int j = 0; j < W / 2; ++j) acc[j] = make_float2(0.0f, 0.0f);
+        bool ok = true;
+        for (int it = 0; it < count; ++it) {
+            const int a = it % C::kAcc, ss = it % C::kScaleStages;
+            const float* sc = reinterpret_cast<const float*>(smem + C::kOffScale + ss * C::kScaleBytes);
+            if (!mbar_wait(&sFull[ss], (it / C::kScaleStages) & 1, sAbort, budget) ||
+                !mbar_wait(&accFull[a], (it / C::kAcc) & 1, sAbort, budget)) {
+                *sAbort = 1;
+                atomicOr(p.err, kErrWaitAccFull);
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            const float s = sc[quad * 32 + lane];
+            uint32_t r[W];
+            tmem_read(tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + a * NT + col0, r);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&accEmpty[a]);
+#pragma unroll
+            for (int j = 0; j < W / 4; ++j) {
+                const float4 cs = *reinterpret_cast<const float4*>(sc + 128 + col0 + 4 * j);
+                const float2 f0 = mul2_rn(make_float2(s, s), make_float2(cs.x, cs.y));
+                const float2 f1 = mul2_rn(make_float2(s, s), make_float2(cs.z, cs.w));
+                acc[2 * j] = fma2_rn(make_float2(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1])), f0, acc[2 * j]);
+                acc[2 * j + 1] =
+                    fma2_rn(make_float2(__uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3])), f1, acc[2 * j + 1]);
+            }
+            __syncwarp();  // every lane has read the block's scales
+            if (lane == 0) mbar_arrive(&sEmpty[ss]);
+        }
+        // the last block's MMAs have read every stage: the partial tile goes in their place
+        if (ok) {
+#pragma unroll
+            for (int j = 0; j < W / 2; ++j) {
+                part[(col0 + 2 * j) * 128 + quad * 32 + lane] = acc[j].x;
+                part[(col0 + 2 * j + 1) * 128 + quad * 32 + lane] = acc[j].y;
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (split > 1) cluster_sync();  // the partial tiles of all ranks are there
+
+    // ---------------- join: this CTA's columns (rows of C), a warp per column, four rows of B a lane
+    const bool failed = *sAbort != 0;
+    const int cols = (NT + split - 1) / split;
+    constexpr int kEl = CT == kF32 ? 4 : 2;
+    const bool vec = reinterpret_cast<uintptr_t>(p.C) % (4 * kEl) == 0 && p.ldc % 4 == 0;
+    for (int c = rank * cols + warp; c < min(NT, (rank + 1) * cols) && !failed; c += C::kThreads / 32) {
+        const int m = m0 + c, n = n0 + lane * 4;
+        if (m >= p.M || n >= p.N) continue;
+        float4 v;
+        if (split == 1) {
+            v = *reinterpret_cast<const float4*>(part + c * 128 + lane * 4);
+        } else {
+            const uint32_t at = smem_u32(part + c * 128 + lane * 4);
+            v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            float4 w[8];
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+                if (r < split) w[r] = ld_cluster4(map_rank(at, r));
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+                if (r < split) v.x += w[r].x, v.y += w[r].y, v.z += w[r].z, v.w += w[r].w;
+        }
+        float o[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (p.bias && n + i < p.N) o[i] += load_any(p.bias, p.btype, n + i);
+        if (p.act == 1) {
+            const float2 g0 = gelu_sig2(make_float2(o[0], o[1])), g1 = gelu_sig2(make_float2(o[2], o[3]));
+            o[0] = g0.x, o[1] = g0.y, o[2] = g1.x, o[3] = g1.y;
+        } else if (p.act == 2) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = relu_ref(o[i]);
+        }
+        const int64_t at = static_cast<int64_t>(m) * p.ldc + n;
+        if (vec && n + 4 <= p.N) {
+            if constexpr (CT == kF32) {
+                *reinterpret_cast<float4*>(static_cast<float*>(p.C) + at) = make_float4(o[0], o[1], o[2], o[3]);
+            } else {
+                const float2 pr[2] = {make_float2(o[0], o[1]), make_float2(o[2], o[3])};
+                uint2 w;
+                w.x = pack_half<CT>(pr[0]);
+                w.y = pack_half<CT>(pr[1]);
+                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.C) + at) = w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (n + i < p.N) store_any(p.C, CT, at + i, o[i]);
+        }
+    }
+
+    if (warp == C::kEpi + 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, C::kTmem);
+    }
+    if (split > 1) cluster_sync();  // no CTA leaves while another may still read its partial tile
+}
+
+template <int NT, int CT>
+cudaError_t launch_narrow(const Fp8GemmArgs& p, int split, cudaStream_t stream) {
+    using C = NarrowCfg<NT>;
+    CUtensorMap tmW{}, tmX{};
+    if (p.K > 0 &&
+        (!encode_2d(&tmW, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.B, p.K, p.N, p.ldb, kBK, 128, 128) ||
+         !encode_2d(&tmX, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.A, p.K, p.M, p.lda, kBK, NT, 128)))
+        return cudaErrorInvalidValue;
+    auto kern = fp8_gemm_narrow_kernel<NT, CT>;
+    cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), C::kSmemBytes);
+    if (e != cudaSuccess) return e;
+    const int64_t tiles = static_cast<int64_t>((p.N + 127) / 128) * ((p.M + NT - 1) / NT);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(tiles * split));
+    cfg.blockDim = dim3(C::kThreads);
+    cfg.dynamicSmemBytes = C::kSmemBytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = static_cast<unsigned>(split);
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, tmW, tmX, p, split);
+}
+
+// Which kernel, and how it is cut.  Both need about half a microsecond a block of K and CTA (pair: 256 x
+// 256 per two SMs, narrow: 128 x NT per CTA), so the time goes by rounds of CTAs times blocks: in blocks,
+//   pair    rounds * (KB + 5) + 10       (a tile's epilogue is worth 5 blocks, the start 10)
+//   narrow  rounds * (KB / split + 5) + 5
+// e.g. 512x4096x4096: narrow 19.6 us, pair 21.2; 1000x4096x1024: 16.8 and 10.5; 1024x1024x16384: 34.6
+// and 63; 2048x2048x2048 only the pair fits one round (14.7 us).
+// NT is the smallest width that holds M (at most 128), narrower still while even the largest split leaves
+// half the SMs without a CTA (64x1024x1024: 6.7 us with NT = 64, 5.5 with 16).  The split doubles while all
+// CTAs fit one round and each keeps two blocks or more (1x4096x4096: 10.7, 8.1, 6.4 us with 1, 2, 4; 7.7
+// with 8, which takes two rounds).
 template <int CT>
 cudaError_t dispatch(const Fp8GemmArgs& p, cudaStream_t stream) {
-    const int64_t wide = static_cast<int64_t>((p.M + 255) / 256) * ((p.N + 255) / 256);
-    return 2 * wide >= device_sm_count() ? launch_pair<CT>(p, stream) : launch<128, CT>(p, stream);
+    const int64_t sms = device_sm_count(), KB = (p.K + kBK - 1) / kBK;
+    const int64_t tn = (static_cast<int64_t>(p.N) + 127) / 128;
+    const auto tiles = [&](int nt) { return tn * ((static_cast<int64_t>(p.M) + nt - 1) / nt); };
+    const auto rounds = [](int64_t n, int64_t at_once) { return (n + at_once - 1) / at_once; };
+    int nt = p.M <= 16 ? 16 : (p.M <= 32 ? 32 : (p.M <= 64 ? 64 : 128));
+    int most = 1;
+    while (most < 8 && most * 4 <= KB) most *= 2;
+    while (nt > 16 && tiles(nt) * most * 2 <= sms) nt /= 2;
+    int split = 1;
+    while (split < most && tiles(nt) * split * 2 <= sms) split *= 2;
+    const int64_t wide = ((static_cast<int64_t>(p.M) + 255) / 256) * ((static_cast<int64_t>(p.N) + 255) / 256);
+    const int64_t pair = rounds(wide, sms / 2) * (KB + 5) + 10;
+    const int64_t narrow = rounds(tiles(nt) * split, nt > 64 ? sms : 2 * sms) * ((KB + split - 1) / split + 5) + 5;
+    if (nt == 128 && pair < narrow) return launch_pair<CT>(p, stream);
+    if (nt == 16) return launch_narrow<16, CT>(p, split, stream);
+    if (nt == 32) return launch_narrow<32, CT>(p, split, stream);
+    if (nt == 64) return launch_narrow<64, CT>(p, split, stream);
+    return launch_narrow<128, CT>(p, split, stream);
 }
 
 }  // namespace

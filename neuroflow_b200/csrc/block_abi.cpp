@@ -176,7 +176,7 @@ int nfx_fp8_quantise(const void* x, int x_type, int64_t ldx, int64_t rows, int64
         if (col_sums && cols > 0)
             return launched(fn, nfx::column_reduce_launch(static_cast<float*>(workspace),
                                                           static_cast<int>(up(rows, nfx::kGroup)), cols, col_sums,
-                                                          NFX_F32, st));
+                                                          nullptr, NFX_F32, st));
         return NFX_OK;
     });
 }

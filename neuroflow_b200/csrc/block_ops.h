@@ -66,8 +66,9 @@ struct NormGradArgs {
 int layer_norm_parts(int64_t rows, int64_t d);
 cudaError_t layer_norm_backward_launch(const NormGradArgs& a, int xtype, cudaStream_t s);
 
-// out[i] = sum_p part[p * n + i] in the order of p (out of type otype)
-cudaError_t column_reduce_launch(const float* part, int parts, int64_t n, void* out, int otype,
+// out0[i] = sum over p < parts of part[p * n + i], always in the same order (out of type otype); out1
+// the same of the next parts * n numbers.  Either may be nullptr.
+cudaError_t column_reduce_launch(const float* part, int parts, int64_t n, void* out0, void* out1, int otype,
                                  cudaStream_t s);
 
 struct QuantArgs {

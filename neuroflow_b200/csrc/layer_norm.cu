@@ -29,7 +29,7 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
     return t;
 }
 
-// Any width, alignment and stride: one block per row, the row read three times (from L2
+// Wider than the row kernels below hold: one block per row, the row read three times (from L2
 // after the first).
 template <typename T>
 __global__ void __launch_bounds__(kAnyThreads) norm_any_kernel(NormArgs a) {
@@ -116,34 +116,453 @@ __global__ void __launch_bounds__(kAnyThreads) norm_grad_any_kernel(NormGradArgs
     }
 }
 
-// 32 columns per block, 8 threads per column over the partial sums, joined in a fixed order.
-__global__ void __launch_bounds__(256) column_reduce_kernel(const float* __restrict__ part, int parts,
-                                                            int64_t n, void* out, int otype) {
-    __shared__ float red[8][33];
+// 32 columns per block, 32 threads per column over the partial sums, joined in a fixed order.  Block
+// row y handles the y-th set of partial sums and its output.
+__global__ void __launch_bounds__(1024) column_reduce_kernel(const float* __restrict__ part, int parts, int64_t n,
+                                                             void* out0, void* out1, int otype) {
+    __shared__ float red[32][33];
     const int c = threadIdx.x & 31, t = threadIdx.x >> 5;
     const int64_t i = static_cast<int64_t>(blockIdx.x) * 32 + c;
+    void* out = blockIdx.y ? out1 : out0;
+    if (!out) return;
+    part += static_cast<int64_t>(blockIdx.y) * parts * n;
     float s = 0.0f;
-    if (i < n)
-        for (int p = t; p < parts; p += 8) s += part[p * n + i];
+    if (i < n) {
+#pragma unroll 4
+        for (int p = t; p < parts; p += 32) s += __ldg(part + p * n + i);
+    }
     red[t][c] = s;
     __syncthreads();
-    if (t == 0 && i < n) {
+    s = warp_sum(red[c][t]);  // the warp's column is t, its lanes the 32 sums
+    if (c == 0 && static_cast<int64_t>(blockIdx.x) * 32 + t < n)
+        store_any(out, otype, static_cast<int64_t>(blockIdx.x) * 32 + t, s);
+}
+
+// ---------------------------------------------------------------------------
+// The row in registers: read once, both statistics and the output from it.  TPR threads per row, each
+// holding VPT packs of VE elements (16 bytes, or one element where rows are not 16-byte aligned).  A
+// warp's packs are contiguous -- pack j of lane l of warp w is (w * VPT + j) * 32 + l of the row -- so
+// the 128 elements of an FP8 group lie in one warp: half a warp's pack (16-bit types), one pack (fp32)
+// or four (VE = 1), and its maximum is a few shuffles.
+// ---------------------------------------------------------------------------
+template <typename T, int VE>
+struct Pack {
+    T v[VE];
+};
+template <typename T, int VE>
+__device__ __forceinline__ void load_pack(const T* p, float (&o)[VE]) {
+    if constexpr (VE == 1) {
+        o[0] = to_f32(__ldg(p));
+    } else {
+        const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+        const Pack<T, VE> k = *reinterpret_cast<const Pack<T, VE>*>(&u);
 #pragma unroll
-        for (int k = 1; k < 8; ++k) s += red[k][c];
-        store_any(out, otype, i, s);
+        for (int i = 0; i < VE; ++i) o[i] = to_f32(k.v[i]);
     }
+}
+template <typename T, int VE>
+__device__ __forceinline__ void store_pack(T* p, const float (&o)[VE]) {
+    if constexpr (VE == 1) {
+        *p = from_f32<T>(o[0]);
+    } else {
+        Pack<T, VE> k;
+#pragma unroll
+        for (int i = 0; i < VE; ++i) k.v[i] = from_f32<T>(o[i]);
+        *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(&k);
+    }
+}
+// VE parameters (of x's type or fp32) from element i; `vec` when they are 16-byte aligned.
+template <typename T, int VE>
+__device__ __forceinline__ void load_params(const void* p, int type, bool vec, int i, float none, float (&o)[VE]) {
+    if (!p) {
+#pragma unroll
+        for (int k = 0; k < VE; ++k) o[k] = none;
+    } else if (VE > 1 && vec && type == kF32) {
+#pragma unroll
+        for (int k = 0; k < VE; k += 4) {
+            const float4 f = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + i + k));
+            o[k] = f.x, o[k + 1] = f.y, o[k + 2] = f.z, o[k + 3] = f.w;
+        }
+    } else if (VE == 8 && vec) {
+        const uint4 u = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i));
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int k = 0; k < VE; k += 2) {
+            float2 f;
+            if (type == kBF16) f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[k / 2]));
+            else f = __half22float2(*reinterpret_cast<const __half2*>(&w[k / 2]));
+            o[k] = f.x, o[k + 1] = f.y;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < VE; ++k) o[k] = load_any(p, type, i + k);
+    }
+}
+
+// Sum over the TPR threads of a row, the same bits in each of them.
+template <int TPR>
+__device__ __forceinline__ float row_sum(float v, float* red) {
+#pragma unroll
+    for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    if constexpr (TPR > 32) {
+        __syncthreads();  // the previous sum has been read
+        if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+        __syncthreads();
+        v = red[0];
+#pragma unroll
+        for (int w = 1; w < TPR / 32; ++w) v += red[w];
+    }
+    return v;
+}
+
+// FP8 codes of a lane's VPT packs (values v, columns col0(j) ..): groups of 128 within the warp.
+template <int VE, int VPT, int TPR>
+__device__ __forceinline__ void store_codes(const float (&v)[VPT][VE], const Fp8Out& q, int64_t r, int d, bool live,
+                                            int first_pack, int lane, bool wide) {
+    constexpr int kPerGroup = VE == 1 ? 4 : 1;                             // packs of a lane in one group
+    constexpr int kLanes = VE == 1 ? 32 : (kGroup / VE < TPR ? kGroup / VE : TPR);  // lanes of one group
+#pragma unroll
+    for (int j = 0; j < VPT; j += kPerGroup) {
+        float am = 0.0f;
+#pragma unroll
+        for (int h = 0; h < kPerGroup; ++h)
+#pragma unroll
+            for (int i = 0; i < VE; ++i) am = fmaxf(am, finite_abs(v[j + h][i]));
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o >>= 1) am = fmaxf(am, __shfl_xor_sync(0xFFFFFFFFu, am, o));
+        const float sc = group_scale(am), inv = __frcp_rn(sc);
+        const int c0 = (first_pack + j * 32) * VE;  // this lane's first column
+        if (live && c0 < d && (VE == 1 ? lane == 0 : lane % kLanes == 0)) q.scales[r * q.srs + (c0 / kGroup) * q.sbs] = sc;
+#pragma unroll
+        for (int h = 0; h < kPerGroup; ++h) {
+            const int c = c0 + h * 32 * VE;
+            if (!live || c >= d) continue;
+            uint8_t* dst = q.codes + r * q.ld + c;
+            uint32_t b[VE];
+#pragma unroll
+            for (int i = 0; i < VE; ++i) b[i] = e4m3_code(v[j + h][i], inv);
+            if (VE == 8 && wide) {
+                uint2 w;
+                w.x = b[0] | b[1 % VE] << 8 | b[2 % VE] << 16 | b[3 % VE] << 24;
+                w.y = b[4 % VE] | b[5 % VE] << 8 | b[6 % VE] << 16 | b[7 % VE] << 24;
+                *reinterpret_cast<uint2*>(dst) = w;
+            } else if (VE == 4 && wide) {
+                *reinterpret_cast<uint32_t*>(dst) = b[0] | b[1 % VE] << 8 | b[2 % VE] << 16 | b[3 % VE] << 24;
+            } else {
+#pragma unroll
+                for (int i = 0; i < VE; ++i) dst[i] = static_cast<uint8_t>(b[i]);
+            }
+        }
+    }
+}
+
+constexpr int row_block(int tpr) { return tpr > 128 ? tpr : 128; }
+
+template <typename T, int VE, int VPT, int TPR, bool FP8>
+__global__ void __launch_bounds__(row_block(TPR)) norm_row_kernel(NormArgs a, bool pvec, bool wide) {
+    __shared__ float red[TPR > 32 ? TPR / 32 : 1];
+    constexpr int kRows = row_block(TPR) / TPR;
+    const int lane = threadIdx.x & 31, sub = threadIdx.x % TPR;
+    const int64_t r = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / TPR;
+    const bool live = r < a.rows;
+    // pack j of this thread is first + j * 32 (a row of fewer than 32 threads has one pack a thread)
+    const int first = TPR < 32 ? sub : (sub >> 5) * VPT * 32 + lane;
+    const T* x = static_cast<const T*>(a.x) + r * a.ldx;
+    const float fd = static_cast<float>(a.d);
+    float v[VPT][VE], s = 0.0f;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+        const int c = (first + j * 32) * VE;
+#pragma unroll
+        for (int i = 0; i < VE; ++i) v[j][i] = 0.0f;
+        if (live && c < a.d) load_pack<T, VE>(x + c, v[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < VPT; ++j)
+#pragma unroll
+        for (int i = 0; i < VE; ++i) s += v[j][i];
+    const float mu = __fdiv_rn(row_sum<TPR>(s, red), fd);
+    s = 0.0f;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+        const bool in = (first + j * 32) * VE < a.d;
+#pragma unroll
+        for (int i = 0; i < VE; ++i) {
+            v[j][i] = in ? v[j][i] - mu : 0.0f;
+            s = fmaf(v[j][i], v[j][i], s);
+        }
+    }
+    const float rs = __frsqrt_rn(__fdiv_rn(row_sum<TPR>(s, red), fd) + a.eps);
+    if (live && sub == 0) {
+        if (a.mean) a.mean[r] = mu;
+        if (a.rstd) a.rstd[r] = rs;
+    }
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+        const int c = (first + j * 32) * VE;
+        if (c >= a.d) continue;
+        float g[VE], b[VE];
+        load_params<T, VE>(a.gamma, a.ptype, pvec, c, 1.0f, g);
+        load_params<T, VE>(a.beta, a.ptype, pvec, c, 0.0f, b);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) v[j][i] = fmaf(v[j][i] * rs, g[i], b[i]);
+        if constexpr (!FP8) {
+            if (live) store_pack<T, VE>(static_cast<T*>(a.y) + r * a.ldy + c, v[j]);
+        }
+    }
+    if constexpr (FP8) store_codes<VE, VPT, TPR>(v, a.q, r, a.d, live, first, lane, wide);
+}
+
+template <typename T, int VE, int VPT, int TPR>
+cudaError_t norm_row(const NormArgs& a, bool pvec, cudaStream_t s) {
+    constexpr int kRows = row_block(TPR) / TPR;
+    const int64_t grid = (a.rows + kRows - 1) / kRows;
+    if (grid > 0x7FFFFFFF) return cudaErrorInvalidValue;
+    if (a.y) {
+        norm_row_kernel<T, VE, VPT, TPR, false><<<static_cast<unsigned>(grid), row_block(TPR), 0, s>>>(a, pvec, false);
+    } else {
+        const bool wide = reinterpret_cast<uintptr_t>(a.q.codes) % 8 == 0 && (a.rows == 1 || a.q.ld % 8 == 0);
+        norm_row_kernel<T, VE, VPT, TPR, true><<<static_cast<unsigned>(grid), row_block(TPR), 0, s>>>(a, pvec, wide);
+    }
+    return cudaGetLastError();
+}
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+// Threads and packs per row by the width: the fewest threads that leave a thread 32 elements at most.
+template <typename T, int VE>
+cudaError_t norm_width(const NormArgs& a, bool pvec, cudaStream_t s) {
+    constexpr int kV = 32 / VE;  // packs of 32 elements
+    if constexpr (VE > 1) {
+        if (a.d <= 16 * VE) return norm_row<T, VE, 1, 16>(a, pvec, s);
+        if (a.d <= 32 * VE) return norm_row<T, VE, 1, 32>(a, pvec, s);
+        if (a.d <= 64 * VE) return norm_row<T, VE, 2, 32>(a, pvec, s);
+    } else {
+        if (a.d <= 128) return norm_row<T, VE, 4, 32>(a, pvec, s);
+        if (a.d <= 256) return norm_row<T, VE, 8, 32>(a, pvec, s);
+    }
+    if (a.d <= 512) return norm_row<T, VE, kV / 2, 32>(a, pvec, s);
+    if (a.d <= 1024) return norm_row<T, VE, kV, 32>(a, pvec, s);
+    if (a.d <= 2048) return norm_row<T, VE, kV / 2, 128>(a, pvec, s);
+    if (a.d <= 4096) return norm_row<T, VE, kV, 128>(a, pvec, s);
+    if (a.d <= 8192) return norm_row<T, VE, kV, 256>(a, pvec, s);
+    return norm_row<T, VE, kV, 512>(a, pvec, s);
 }
 
 template <typename T>
 cudaError_t norm_t(const NormArgs& a, cudaStream_t s) {
+    constexpr int VE = 16 / sizeof(T);
+    if (a.d <= 16384 && a.rows <= 0x7FFFFFFF) {
+        const bool pvec = aligned16(a.gamma) && aligned16(a.beta) && (a.ptype == kF32 || VE == 8);
+        const bool rows16 = aligned16(a.x) && (a.rows == 1 || a.ldx % VE == 0) &&
+                            (!a.y || (aligned16(a.y) && (a.rows == 1 || a.ldy % VE == 0)));
+        if (rows16 && a.d % VE == 0) return norm_width<T, VE>(a, pvec, s);
+        return norm_width<T, 1>(a, false, s);
+    }
     const int64_t cap = 8ll * device_sm_count();
     norm_any_kernel<T><<<static_cast<int>(a.rows < cap ? a.rows : cap), kAnyThreads, 0, s>>>(a);
     return cudaGetLastError();
 }
 
+// ---------------------------------------------------------------------------
+// Backward with a row of x and dy in registers: TPR threads per row, 16 elements each, both row sums in
+// one reduction.  Blocks walk over the rows; a thread's columns are the same in every row, so the
+// parameter gradients are sums in its registers (in shared memory where a block of 1,024 threads
+// leaves 64 registers a thread), written once per block.  The next row's loads are issued before this
+// row's sums are joined.
+// ---------------------------------------------------------------------------
+template <typename T, int VE>
+struct Raw {
+    uint4 u;
+    __device__ __forceinline__ void load(const T* p) { u = __ldg(reinterpret_cast<const uint4*>(p)); }
+    __device__ __forceinline__ void get(float (&o)[VE]) const {
+        const Pack<T, VE> k = *reinterpret_cast<const Pack<T, VE>*>(&u);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) o[i] = to_f32(k.v[i]);
+    }
+    __device__ __forceinline__ void zero() { u = make_uint4(0, 0, 0, 0); }
+};
+template <typename T>
+struct Raw<T, 1> {
+    T u;
+    __device__ __forceinline__ void load(const T* p) { u = *p; }
+    __device__ __forceinline__ void get(float (&o)[1]) const { o[0] = to_f32(u); }
+    __device__ __forceinline__ void zero() { u = from_f32<T>(0.0f); }
+};
+
+// Sums of (a, b) over the TPR threads of a row; `buf` alternates between calls, so that one barrier
+// separates a call's reads from the next but one's writes.
+template <int TPR>
+__device__ __forceinline__ float2 row_sum2(float a, float b, float2 (*red)[32], int buf) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        a += __shfl_xor_sync(0xFFFFFFFFu, a, o);
+        b += __shfl_xor_sync(0xFFFFFFFFu, b, o);
+    }
+    if constexpr (TPR > 32) {
+        const int w = threadIdx.x >> 5, w0 = w / (TPR / 32) * (TPR / 32);
+        if ((threadIdx.x & 31) == 0) red[buf][w] = make_float2(a, b);
+        __syncthreads();
+        float2 t = red[buf][w0];
+#pragma unroll
+        for (int k = 1; k < TPR / 32; ++k) {
+            const float2 u = red[buf][w0 + k];
+            t.x += u.x, t.y += u.y;
+        }
+        return t;
+    }
+    return make_float2(a, b);
+}
+
+constexpr int grad_block(int tpr) { return tpr > 256 ? tpr : 256; }
+
+template <typename T, int VE, int TPR>
+__global__ void __launch_bounds__(grad_block(TPR), TPR > 256 ? 1 : 2)
+norm_grad_row_kernel(NormGradArgs a, bool pvec) {
+    constexpr int VPT = 16 / VE, kThreads = grad_block(TPR), kRows = kThreads / TPR;
+    constexpr bool kShared = TPR == 1024;
+    __shared__ float2 red[2][32];
+    extern __shared__ float sums[];  // 2 x d: the block's sums, joined at the end (kShared: all along)
+    const int lane = threadIdx.x & 31, sub = threadIdx.x % TPR, group = threadIdx.x / TPR;
+    const int first = (sub >> 5) * VPT * 32 + lane;
+    const float fd = static_cast<float>(a.d);
+    float gam[VPT][VE], pg[VPT][VE], pb[VPT][VE];
+    Raw<T, VE> rx[VPT], rg[VPT];
+    float mu_next = 0.0f, rs_next = 0.0f;
+    auto fetch = [&](int64_t r) {
+        if (r < a.rows) mu_next = __ldg(a.mean + r), rs_next = __ldg(a.rstd + r);
+        const T* x = static_cast<const T*>(a.x) + r * a.ldx;
+        const T* dy = static_cast<const T*>(a.dy) + r * a.lddy;
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            const int c = (first + j * 32) * VE;
+            if (r < a.rows && c < a.d) rx[j].load(x + c), rg[j].load(dy + c);
+            else rx[j].zero(), rg[j].zero();
+        }
+    };
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+        const int c = (first + j * 32) * VE;
+#pragma unroll
+        for (int i = 0; i < VE; ++i) pg[j][i] = pb[j][i] = gam[j][i] = 0.0f;
+        if (!kShared && c < a.d) load_params<T, VE>(a.gamma, a.ptype, pvec, c, 1.0f, gam[j]);
+        if (kShared && a.part && c < a.d)
+#pragma unroll
+            for (int i = 0; i < VE; ++i) sums[c + i] = sums[a.d + c + i] = 0.0f;
+    }
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
+    int buf = 0;
+    fetch(static_cast<int64_t>(blockIdx.x) * kRows + group);
+    for (int64_t base = static_cast<int64_t>(blockIdx.x) * kRows; base < a.rows; base += step, buf ^= 1) {
+        const int64_t r = base + group;
+        const bool live = r < a.rows;
+        const float mu = mu_next, rs = rs_next;
+        float xh[VPT][VE], g[VPT][VE];
+        float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            rx[j].get(xh[j]);
+            rg[j].get(g[j]);
+            const int c = (first + j * 32) * VE;
+            float w[VE];
+#pragma unroll
+            for (int i = 0; i < VE; ++i) w[i] = gam[j][i];
+            if (kShared && c < a.d) load_params<T, VE>(a.gamma, a.ptype, pvec, c, 1.0f, w);
+#pragma unroll
+            for (int i = 0; i < VE; ++i) {
+                xh[j][i] = (xh[j][i] - mu) * rs;
+                const float ga = g[j][i] * w[i];
+                s1 += ga;
+                s2 = fmaf(ga, xh[j][i], s2);
+                if constexpr (!kShared) {
+                    pg[j][i] = fmaf(g[j][i], xh[j][i], pg[j][i]);
+                    pb[j][i] += g[j][i];
+                }
+            }
+            if (kShared && a.part && c < a.d) {
+#pragma unroll
+                for (int i = 0; i < VE; ++i) {
+                    sums[c + i] = fmaf(g[j][i], xh[j][i], sums[c + i]);
+                    sums[a.d + c + i] += g[j][i];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < VE; ++i) g[j][i] *= w[i];
+        }
+        fetch(r + step);
+        const float2 t = row_sum2<TPR>(s1, s2, red, buf);
+        const float m1 = __fdiv_rn(t.x, fd), m2 = __fdiv_rn(t.y, fd);
+        T* dx = static_cast<T*>(a.dx) + r * a.lddx;
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            const int c = (first + j * 32) * VE;
+            if (!live || c >= a.d) continue;
+            float o[VE];
+#pragma unroll
+            for (int i = 0; i < VE; ++i) o[i] = rs * (g[j][i] - m1 - xh[j][i] * m2);
+            store_pack<T, VE>(dx + c, o);
+        }
+    }
+    if (!a.part) return;
+    // the block's row groups join their sums, one after the other
+    if constexpr (!kShared) {
+        for (int k = 0; k < kRows; ++k) {
+            __syncthreads();
+            if (group == k) {
+#pragma unroll
+                for (int j = 0; j < VPT; ++j) {
+                    const int c = (first + j * 32) * VE;
+                    if (c >= a.d) continue;
+#pragma unroll
+                    for (int i = 0; i < VE; ++i) {
+                        sums[c + i] = k ? sums[c + i] + pg[j][i] : pg[j][i];
+                        sums[a.d + c + i] = k ? sums[a.d + c + i] + pb[j][i] : pb[j][i];
+                    }
+                }
+            }
+        }
+    }
+    __syncthreads();
+    float* out_g = a.part + static_cast<int64_t>(blockIdx.x) * a.d;
+    float* out_b = a.part + (static_cast<int64_t>(a.parts) + blockIdx.x) * a.d;
+    for (int i = threadIdx.x; i < a.d; i += kThreads) {
+        out_g[i] = sums[i];
+        out_b[i] = sums[a.d + i];
+    }
+}
+
+template <typename T, int VE, int TPR>
+cudaError_t norm_grad_row(const NormGradArgs& a, bool pvec, cudaStream_t s) {
+    auto kern = norm_grad_row_kernel<T, VE, TPR>;
+    const int smem = a.part ? 2 * a.d * 4 : 0;
+    cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), smem);
+    if (e != cudaSuccess) return e;
+    kern<<<a.parts, grad_block(TPR), smem, s>>>(a, pvec);
+    return cudaGetLastError();
+}
+
+template <typename T, int VE>
+cudaError_t norm_grad_width(const NormGradArgs& a, bool pvec, cudaStream_t s) {
+    if (a.d <= 512) return norm_grad_row<T, VE, 32>(a, pvec, s);
+    if (a.d <= 1024) return norm_grad_row<T, VE, 64>(a, pvec, s);
+    if (a.d <= 2048) return norm_grad_row<T, VE, 128>(a, pvec, s);
+    if (a.d <= 4096) return norm_grad_row<T, VE, 256>(a, pvec, s);
+    if (a.d <= 8192) return norm_grad_row<T, VE, 512>(a, pvec, s);
+    return norm_grad_row<T, VE, 1024>(a, pvec, s);
+}
+
 template <typename T>
 cudaError_t norm_grad_t(const NormGradArgs& a, cudaStream_t s) {
-    if (a.rows > 0) norm_grad_any_kernel<T><<<a.parts, kAnyThreads, 0, s>>>(a);
+    if (a.rows == 0) return cudaSuccess;
+    if (a.d <= 16384) {
+        constexpr int VE = 16 / sizeof(T);
+        const bool pvec = aligned16(a.gamma) && (a.ptype == kF32 || VE == 8);
+        const bool rows16 = aligned16(a.x) && aligned16(a.dy) && aligned16(a.dx) &&
+                            (a.rows == 1 || (a.ldx % VE == 0 && a.lddy % VE == 0 && a.lddx % VE == 0));
+        if (rows16 && a.d % VE == 0) return norm_grad_width<T, VE>(a, pvec, s);
+        return norm_grad_width<T, 1>(a, false, s);
+    }
+    norm_grad_any_kernel<T><<<a.parts, kAnyThreads, 0, s>>>(a);
     return cudaGetLastError();
 }
 
@@ -155,14 +574,17 @@ cudaError_t layer_norm_launch(const NormArgs& a, int xtype, cudaStream_t s) {
     return norm_t<__half>(a, s);
 }
 
-int layer_norm_parts(int64_t rows, int64_t) {
-    const int64_t cap = 2ll * device_sm_count();
+// Blocks of the backward kernels, each with its own partial sums: enough to fill the SMs at the
+// kernels' occupancy, few enough that the partial sums stay small against the rows.
+int layer_norm_parts(int64_t rows, int64_t d) {
+    const int64_t cap = (d <= 4096 ? 2ll : 1ll) * device_sm_count();
     return static_cast<int>(rows < cap ? rows : cap);
 }
 
-cudaError_t column_reduce_launch(const float* part, int parts, int64_t n, void* out, int otype,
+cudaError_t column_reduce_launch(const float* part, int parts, int64_t n, void* out0, void* out1, int otype,
                                  cudaStream_t s) {
-    column_reduce_kernel<<<static_cast<unsigned>((n + 31) / 32), 256, 0, s>>>(part, parts, n, out, otype);
+    const dim3 grid(static_cast<unsigned>((n + 31) / 32), out1 ? 2 : 1);
+    column_reduce_kernel<<<grid, 1024, 0, s>>>(part, parts, n, out0, out1, otype);
     return cudaGetLastError();
 }
 
@@ -170,9 +592,8 @@ cudaError_t layer_norm_backward_launch(const NormGradArgs& a, int xtype, cudaStr
     cudaError_t e = xtype == kF32    ? norm_grad_t<float>(a, s)
                     : xtype == kBF16 ? norm_grad_t<__nv_bfloat16>(a, s)
                                      : norm_grad_t<__half>(a, s);
-    if (e == cudaSuccess && a.dgamma) e = column_reduce_launch(a.part, a.parts, a.d, a.dgamma, a.ptype, s);
-    if (e == cudaSuccess && a.dbeta)
-        e = column_reduce_launch(a.part + static_cast<int64_t>(a.parts) * a.d, a.parts, a.d, a.dbeta, a.ptype, s);
+    if (e == cudaSuccess && (a.dgamma || a.dbeta))
+        e = column_reduce_launch(a.part, a.parts, a.d, a.dgamma, a.dbeta, a.ptype, s);
     return e;
 }
 

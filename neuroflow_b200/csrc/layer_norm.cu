@@ -12,6 +12,7 @@
 #include "block_ops.h"
 #include "nfx_internal.h"
 #include "numerics.cuh"
+#include "row_pack.cuh"
 
 namespace nfx {
 namespace {
@@ -145,32 +146,6 @@ __global__ void __launch_bounds__(1024) column_reduce_kernel(const float* __rest
 // the 128 elements of an FP8 group lie in one warp: half a warp's pack (16-bit types), one pack (fp32)
 // or four (VE = 1), and its maximum is a few shuffles.
 // ---------------------------------------------------------------------------
-template <typename T, int VE>
-struct Pack {
-    T v[VE];
-};
-template <typename T, int VE>
-__device__ __forceinline__ void load_pack(const T* p, float (&o)[VE]) {
-    if constexpr (VE == 1) {
-        o[0] = to_f32(__ldg(p));
-    } else {
-        const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
-        const Pack<T, VE> k = *reinterpret_cast<const Pack<T, VE>*>(&u);
-#pragma unroll
-        for (int i = 0; i < VE; ++i) o[i] = to_f32(k.v[i]);
-    }
-}
-template <typename T, int VE>
-__device__ __forceinline__ void store_pack(T* p, const float (&o)[VE]) {
-    if constexpr (VE == 1) {
-        *p = from_f32<T>(o[0]);
-    } else {
-        Pack<T, VE> k;
-#pragma unroll
-        for (int i = 0; i < VE; ++i) k.v[i] = from_f32<T>(o[i]);
-        *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(&k);
-    }
-}
 // VE parameters (of x's type or fp32) from element i; `vec` when they are 16-byte aligned.
 template <typename T, int VE>
 __device__ __forceinline__ void load_params(const void* p, int type, bool vec, int i, float none, float (&o)[VE]) {
@@ -213,47 +188,6 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
         for (int w = 1; w < TPR / 32; ++w) v += red[w];
     }
     return v;
-}
-
-// FP8 codes of a lane's VPT packs (values v, columns col0(j) ..): groups of 128 within the warp.
-template <int VE, int VPT, int TPR>
-__device__ __forceinline__ void store_codes(const float (&v)[VPT][VE], const Fp8Out& q, int64_t r, int d, bool live,
-                                            int first_pack, int lane, bool wide) {
-    constexpr int kPerGroup = VE == 1 ? 4 : 1;                             // packs of a lane in one group
-    constexpr int kLanes = VE == 1 ? 32 : (kGroup / VE < TPR ? kGroup / VE : TPR);  // lanes of one group
-#pragma unroll
-    for (int j = 0; j < VPT; j += kPerGroup) {
-        float am = 0.0f;
-#pragma unroll
-        for (int h = 0; h < kPerGroup; ++h)
-#pragma unroll
-            for (int i = 0; i < VE; ++i) am = fmaxf(am, finite_abs(v[j + h][i]));
-#pragma unroll
-        for (int o = kLanes / 2; o > 0; o >>= 1) am = fmaxf(am, __shfl_xor_sync(0xFFFFFFFFu, am, o));
-        const float sc = group_scale(am), inv = __frcp_rn(sc);
-        const int c0 = (first_pack + j * 32) * VE;  // this lane's first column
-        if (live && c0 < d && (VE == 1 ? lane == 0 : lane % kLanes == 0)) q.scales[r * q.srs + (c0 / kGroup) * q.sbs] = sc;
-#pragma unroll
-        for (int h = 0; h < kPerGroup; ++h) {
-            const int c = c0 + h * 32 * VE;
-            if (!live || c >= d) continue;
-            uint8_t* dst = q.codes + r * q.ld + c;
-            uint32_t b[VE];
-#pragma unroll
-            for (int i = 0; i < VE; ++i) b[i] = e4m3_code(v[j + h][i], inv);
-            if (VE == 8 && wide) {
-                uint2 w;
-                w.x = b[0] | b[1 % VE] << 8 | b[2 % VE] << 16 | b[3 % VE] << 24;
-                w.y = b[4 % VE] | b[5 % VE] << 8 | b[6 % VE] << 16 | b[7 % VE] << 24;
-                *reinterpret_cast<uint2*>(dst) = w;
-            } else if (VE == 4 && wide) {
-                *reinterpret_cast<uint32_t*>(dst) = b[0] | b[1 % VE] << 8 | b[2 % VE] << 16 | b[3 % VE] << 24;
-            } else {
-#pragma unroll
-                for (int i = 0; i < VE; ++i) dst[i] = static_cast<uint8_t>(b[i]);
-            }
-        }
-    }
 }
 
 constexpr int row_block(int tpr) { return tpr > 128 ? tpr : 128; }
@@ -326,8 +260,6 @@ cudaError_t norm_row(const NormArgs& a, bool pvec, cudaStream_t s) {
     }
     return cudaGetLastError();
 }
-
-bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 // Threads and packs per row by the width: the fewest threads that leave a thread 32 elements at most.
 template <typename T, int VE>

@@ -40,7 +40,7 @@ __global__ void e4m3_fake_quant_kernel(const float* __restrict__ x, float scale,
 
 // Every fp32 bit pattern through the hardware-conversion encoder (which saturates by
 // itself) and, clamped as e4m3_code clamps, through the reference one, and through the
-// executors' inner fake-quant against the reference round trip; every code through
+// four-value encoder, and through the executors' inner fake-quant against the reference round trip; every code through
 // both decoders (bit patterns).
 __global__ void e4m3_selfcheck_kernel(unsigned long long* bad) {
     unsigned long long n = 0;
@@ -49,6 +49,10 @@ __global__ void e4m3_selfcheck_kernel(unsigned long long* bad) {
         const float v = __uint_as_float(static_cast<uint32_t>(i));
         const float xs = v > 448.0f ? 448.0f : (v < -448.0f ? -448.0f : v);
         if (nfx::e4m3_encode_fast(v) != nfx::e4m3_encode_ref(xs)) ++n;
+        // four at a time, in each of the places beside other values
+        const uint32_t want = nfx::e4m3_encode_ref(xs);
+        if (nfx::e4m3_encode4(v, -1.0f, v, 0.0f) != (want | 0xB800u | want << 16)) ++n;
+        if (nfx::e4m3_encode4(2.0f, v, 448.0f, v) != (0x40u | want << 8 | 0x7E0000u | want << 24)) ++n;
         // the executors' inner fake-quant: the reference value, any NaN for a NaN
         const float fq = nfx::fp8_fake_quant_inner(v, 1.0f, 1.0f);
         const float fr = nfx::e4m3_decode_ref(nfx::e4m3_encode_ref(xs));

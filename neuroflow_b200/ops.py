@@ -107,38 +107,45 @@ def _p(t):
     return None if t is None else t.data_ptr()
 
 
-class _On:
-    """The device of `t` and the stream of a call: allocations inside belong to that stream."""
+def _elsewhere(t, stream):
+    """Whether a call on `t` needs another device or stream made current first (see _on)."""
+    return stream is not None or t.device.index != torch.cuda.current_device()
 
-    def __init__(self, t, stream):
-        self.stack = None
-        if t.device.index != torch.cuda.current_device() or stream is not None:
-            self.stack = contextlib.ExitStack()
-            self.stack.enter_context(torch.cuda.device(t.device))
-            if stream is not None:
-                if not isinstance(stream, torch.cuda.Stream):
-                    stream = torch.cuda.ExternalStream(int(stream), device=t.device)
-                self.stack.enter_context(torch.cuda.stream(stream))
 
-    def __enter__(self):
-        return torch.cuda.current_stream().cuda_stream
+@contextlib.contextmanager
+def _on(t, stream):
+    """The device of `t` and the stream of a call made current, so that what the call allocates
+    belongs to that stream."""
+    with torch.cuda.device(t.device):
+        if stream is None:
+            yield
+            return
+        if not isinstance(stream, torch.cuda.Stream):
+            stream = torch.cuda.ExternalStream(int(stream), device=t.device)
+        with torch.cuda.stream(stream):
+            yield
 
-    def __exit__(self, *exc):
-        if self.stack is not None:
-            self.stack.close()
-        return False
+
+def _stream(t):
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
 def _codes(rows, cols, device):
     """An empty code matrix whose rows start on 16-byte boundaries."""
-    pitch = _up(max(cols, 1), 16)
-    return torch.empty((rows, pitch), dtype=torch.uint8, device=device).view(E4M3)[:, :cols]
+    pitch = _up(cols, 16) or 16
+    c = torch.empty((rows, pitch), dtype=E4M3, device=device)
+    return c if pitch == cols else c[:, :cols]
 
 
 def _scales(rows, cols, device):
     """Empty scales (rows, ceil(cols / 128)) with the block index outermost, the order in which
     the product reads them."""
-    return torch.empty((_up(cols, GROUP) // GROUP, rows), dtype=torch.float32, device=device).t()
+    return torch.empty_strided((rows, -(-cols // GROUP)), (1, rows), dtype=torch.float32, device=device)
+
+
+def _row_stats(x, rows):
+    """Two empty fp32 vectors (mean, rstd), one element for each row of x."""
+    return x.new_empty((2, rows) if x.dim() == 2 else (2, *x.shape[:-1]), dtype=torch.float32).unbind(0)
 
 
 def _norm_args(fn, x, gamma, beta):
@@ -160,16 +167,23 @@ def layer_norm(x, gamma=None, beta=None, eps=1e-5, out=None, stats=False, stream
     row, which layer_norm_backward takes: (y, mean, rstd)."""
     fn = "layer_norm"
     x2, xt, g, b, pt = _norm_args(fn, x, gamma, beta)
+    if _elsewhere(x, stream):
+        with _on(x, stream):
+            return layer_norm(x, gamma, beta, eps, out, stats)
     rows, d = x2.shape
-    with _On(x, stream) as s:
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
-        if out is not None and (y.shape != x.shape or y.dtype != x.dtype or y.device != x.device):
+    if out is None:
+        y = y2 = torch.empty_like(x, memory_format=torch.contiguous_format)
+        ldy = d
+    else:
+        y = out
+        if y.shape != x.shape or y.dtype != x.dtype or y.device != x.device:
             _refuse(fn, "out must have x's shape, type and device")
         y2 = _rows(fn, "out", y)
-        mean, rstd = torch.empty((2, rows), dtype=torch.float32, device=x.device) if stats else (None, None)
-        _nfx.check(_lib.nfx_layer_norm(_p(x2), xt, x2.stride(0), _p(g), _p(b), pt, rows, d, eps, _p(y2), y2.stride(0),
-                                       _p(mean), _p(rstd), s))
-    return (y, mean.view(x.shape[:-1]), rstd.view(x.shape[:-1])) if stats else y
+        ldy = y2.stride(0)
+    mean, rstd = _row_stats(x, rows) if stats else (None, None)
+    _nfx.check(_lib.nfx_layer_norm(x2.data_ptr(), xt, x2.stride(0), _p(g), _p(b), pt, rows, d, eps, y2.data_ptr(), ldy,
+                                   _p(mean), _p(rstd), _stream(x)))
+    return (y, mean, rstd) if stats else y
 
 
 def layer_norm_fp8(x, gamma=None, beta=None, eps=1e-5, stats=False, stream=None):
@@ -177,14 +191,16 @@ def layer_norm_fp8(x, gamma=None, beta=None, eps=1e-5, stats=False, stream=None)
     makes of an fp32 y, which is never written.  With `stats`: (blocks, mean, rstd)."""
     fn = "layer_norm_fp8"
     x2, xt, g, b, pt = _norm_args(fn, x, gamma, beta)
+    if _elsewhere(x, stream):
+        with _on(x, stream):
+            return layer_norm_fp8(x, gamma, beta, eps, stats)
     rows, d = x2.shape
-    with _On(x, stream) as s:
-        q = Fp8Blocks(_codes(rows, d, x.device), _scales(rows, d, x.device))
-        mean, rstd = torch.empty((2, rows), dtype=torch.float32, device=x.device) if stats else (None, None)
-        _nfx.check(_lib.nfx_layer_norm_fp8(_p(x2), xt, x2.stride(0), _p(g), _p(b), pt, rows, d, eps, _p(q.codes),
-                                           q.codes.stride(0), _p(q.scales), q.scales.stride(0), q.scales.stride(1),
-                                           _p(mean), _p(rstd), s))
-    return (q, mean.view(x.shape[:-1]), rstd.view(x.shape[:-1])) if stats else q
+    codes, scales = _codes(rows, d, x.device), _scales(rows, d, x.device)
+    mean, rstd = _row_stats(x, rows) if stats else (None, None)
+    _nfx.check(_lib.nfx_layer_norm_fp8(x2.data_ptr(), xt, x2.stride(0), _p(g), _p(b), pt, rows, d, eps, codes.data_ptr(),
+                                       codes.stride(0), scales.data_ptr(), 1, rows, _p(mean), _p(rstd), _stream(x)))
+    q = Fp8Blocks(codes, scales)
+    return (q, mean, rstd) if stats else q
 
 
 def layer_norm_backward(dy, x, mean, rstd, gamma=None, param_grads=True, stream=None):
@@ -201,16 +217,19 @@ def layer_norm_backward(dy, x, mean, rstd, gamma=None, param_grads=True, stream=
         if _type(fn, name, t) != 0 or t.numel() != rows or not t.is_contiguous():
             _refuse(fn, f"{name} must be a contiguous float32 tensor of {rows}")
     _same_device(fn, x, dy=dy, mean=mean, rstd=rstd)
-    with _On(x, stream) as s:
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        dg = db = ws = None
-        n = 0
-        if param_grads:
-            dg, db = torch.empty((2, d), dtype=torch.float32 if g is None else g.dtype, device=x.device)
-            n = _lib.nfx_layer_norm_backward_workspace(rows, d)
-            ws = torch.empty(n, dtype=torch.uint8, device=x.device)
-        _nfx.check(_lib.nfx_layer_norm_backward(_p(dy2), dy2.stride(0), _p(x2), x2.stride(0), xt, _p(mean), _p(rstd),
-                                                _p(g), pt, rows, d, _p(dx), d, _p(dg), _p(db), _p(ws), n, s))
+    if _elsewhere(x, stream):
+        with _on(x, stream):
+            return layer_norm_backward(dy, x, mean, rstd, gamma, param_grads)
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format)
+    dg = db = ws = None
+    n = 0
+    if param_grads:
+        dg, db = torch.empty((2, d), dtype=torch.float32 if g is None else g.dtype, device=x.device).unbind(0)
+        n = _lib.nfx_layer_norm_backward_workspace(rows, d)
+        ws = torch.empty(n, dtype=torch.uint8, device=x.device)
+    _nfx.check(_lib.nfx_layer_norm_backward(dy2.data_ptr(), dy2.stride(0), x2.data_ptr(), x2.stride(0), xt, mean.data_ptr(),
+                                            rstd.data_ptr(), _p(g), pt, rows, d, dx.data_ptr(), d, _p(dg), _p(db), _p(ws),
+                                            n, _stream(x)))
     return dx, dg, db
 
 
@@ -226,18 +245,28 @@ def fp8_quantise(x, tile=False, transposed=False, col_sums=False, stream=None):
     rows, cols = x2.shape
     if tile and col_sums:
         _refuse(fn, "column sums are made with groups of 1 x 128 only")
-    srows, scols = (_up(rows, GROUP) // GROUP, _up(cols, GROUP) // GROUP) if tile else (rows, cols)
-    with _On(x, stream) as s:
-        q = Fp8Blocks(_codes(rows, cols, x.device), _scales(srows, cols, x.device), tile)
-        qt = Fp8Blocks(_codes(cols, rows, x.device), _scales(scols, rows, x.device), tile) if transposed else None
-        sums = torch.empty(cols, dtype=torch.float32, device=x.device) if col_sums else None
-        n = _lib.nfx_fp8_quantise_workspace(rows, cols) if col_sums else 0
-        ws = torch.empty(n, dtype=torch.uint8, device=x.device) if col_sums else None
-        t = (_p(qt.codes), qt.codes.stride(0), _p(qt.scales), *qt.scales.stride()) if transposed else (None, 0, None, 0, 0)
-        _nfx.check(_lib.nfx_fp8_quantise(_p(x2), xt, x2.stride(0), rows, cols, int(tile), _p(q.codes), q.codes.stride(0),
-                                         _p(q.scales), *q.scales.stride(), *t, _p(sums), _p(ws), n, s))
-    out = (q,) + ((qt,) if transposed else ()) + ((sums,) if col_sums else ())
-    return out if len(out) > 1 else q
+    if _elsewhere(x, stream):
+        with _on(x, stream):
+            return fp8_quantise(x, tile, transposed, col_sums)
+    dev = x.device
+    srows, scols = (-(-rows // GROUP), -(-cols // GROUP)) if tile else (rows, cols)
+    codes, scales = _codes(rows, cols, dev), _scales(srows, cols, dev)
+    q = Fp8Blocks(codes, scales, tile)
+    t = (None, 0, None, 0, 0)
+    if transposed:
+        ct, st = _codes(cols, rows, dev), _scales(scols, rows, dev)
+        t = (ct.data_ptr(), ct.stride(0), st.data_ptr(), 1, scols)
+    sums = ws = None
+    n = 0
+    if col_sums:
+        sums = torch.empty(cols, dtype=torch.float32, device=dev)
+        n = _lib.nfx_fp8_quantise_workspace(rows, cols)
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    _nfx.check(_lib.nfx_fp8_quantise(x2.data_ptr(), xt, x2.stride(0), rows, cols, int(tile), codes.data_ptr(),
+                                     codes.stride(0), scales.data_ptr(), 1, srows, *t, _p(sums), _p(ws), n, _stream(x)))
+    if not (transposed or col_sums):
+        return q
+    return (q,) + ((Fp8Blocks(ct, st, tile),) if transposed else ()) + ((sums,) if col_sums else ())
 
 
 def _operand(fn, name, q):
@@ -262,19 +291,27 @@ def fp8_gemm(a, b, bias=None, act=0, out_dtype=torch.bfloat16, out=None, stream=
     (m, k), (n, kb) = _operand(fn, "a", a), _operand(fn, "b", b)
     if k != kb:
         _refuse(fn, f"a has {k} columns and b {kb}")
+    ac, bc, sa, sb = a.codes, b.codes, a.scales, b.scales
     bias = _vector(fn, "bias", bias, n)
-    _same_device(fn, a.codes, b=b.codes, bias=bias, out=out)
+    _same_device(fn, ac, b=bc, bias=bias, out=out)
     if out is None and out_dtype not in _TYPES:
         _refuse(fn, f"out_dtype must be float32, bfloat16 or float16, not {out_dtype}")
-    with _On(a.codes, stream) as s:
-        c = torch.empty((m, n), dtype=out_dtype, device=a.codes.device) if out is None else out
-        if out is not None and (_type(fn, "out", c) is None or c.shape != (m, n)):
+    if _elsewhere(ac, stream):
+        with _on(ac, stream):
+            return fp8_gemm(a, b, bias, act, out_dtype, out)
+    if out is None:
+        c = torch.empty((m, n), dtype=out_dtype, device=ac.device)
+        ct, ldc = _TYPES[out_dtype], n
+    else:
+        c = out
+        ct = _type(fn, "out", c)
+        if c.shape != (m, n):
             _refuse(fn, f"out must be ({m}, {n})")
-        c2 = _rows(fn, "out", c)
-        _nfx.check(_lib.nfx_fp8_gemm(_p(a.codes), a.codes.stride(0), _p(a.scales), *a.scales.stride(), int(a.tile),
-                                     _p(b.codes), b.codes.stride(0), _p(b.scales), *b.scales.stride(), int(b.tile),
-                                     m, n, k, _p(bias), 0 if bias is None else _TYPES[bias.dtype], int(act), _p(c2),
-                                     _TYPES[c.dtype], c2.stride(0), s))
+        ldc = _rows(fn, "out", c).stride(0)
+    _nfx.check(_lib.nfx_fp8_gemm(ac.data_ptr(), ac.stride(0), sa.data_ptr(), sa.stride(0), sa.stride(1), int(a.tile),
+                                 bc.data_ptr(), bc.stride(0), sb.data_ptr(), sb.stride(0), sb.stride(1), int(b.tile), m, n, k,
+                                 _p(bias), 0 if bias is None else _TYPES[bias.dtype], int(act), c.data_ptr(), ct, ldc,
+                                 _stream(ac)))
     return c
 
 

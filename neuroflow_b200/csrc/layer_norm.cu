@@ -168,6 +168,9 @@ __device__ __forceinline__ void load_params(const void* p, int type, bool vec, i
             else f = __half22float2(*reinterpret_cast<const __half2*>(&w[k / 2]));
             o[k] = f.x, o[k + 1] = f.y;
         }
+    } else if (type == kF32) {
+#pragma unroll
+        for (int k = 0; k < VE; ++k) o[k] = __ldg(static_cast<const float*>(p) + i + k);
     } else {
 #pragma unroll
         for (int k = 0; k < VE; ++k) o[k] = load_any(p, type, i + k);
@@ -203,13 +206,20 @@ __global__ void __launch_bounds__(row_block(TPR)) norm_row_kernel(NormArgs a, bo
     const int first = TPR < 32 ? sub : (sub >> 5) * VPT * 32 + lane;
     const T* x = static_cast<const T*>(a.x) + r * a.ldx;
     const float fd = static_cast<float>(a.d);
+    // (the warps whose packs all lie inside the row need no test per pack)
+    const bool full = live && TPR >= 32 && (first - lane + VPT * 32) * VE <= a.d;
     float v[VPT][VE], s = 0.0f;
+    if (full) {
 #pragma unroll
-    for (int j = 0; j < VPT; ++j) {
-        const int c = (first + j * 32) * VE;
+        for (int j = 0; j < VPT; ++j) load_pack<T, VE>(x + (first + j * 32) * VE, v[j]);
+    } else {
 #pragma unroll
-        for (int i = 0; i < VE; ++i) v[j][i] = 0.0f;
-        if (live && c < a.d) load_pack<T, VE>(x + c, v[j]);
+        for (int j = 0; j < VPT; ++j) {
+            const int c = (first + j * 32) * VE;
+#pragma unroll
+            for (int i = 0; i < VE; ++i) v[j][i] = 0.0f;
+            if (live && c < a.d) load_pack<T, VE>(x + c, v[j]);
+        }
     }
 #pragma unroll
     for (int j = 0; j < VPT; ++j)
@@ -219,11 +229,12 @@ __global__ void __launch_bounds__(row_block(TPR)) norm_row_kernel(NormArgs a, bo
     s = 0.0f;
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
-        const bool in = (first + j * 32) * VE < a.d;
+        if (full || (first + j * 32) * VE < a.d) {
 #pragma unroll
-        for (int i = 0; i < VE; ++i) {
-            v[j][i] = in ? v[j][i] - mu : 0.0f;
-            s = fmaf(v[j][i], v[j][i], s);
+            for (int i = 0; i < VE; ++i) {
+                v[j][i] -= mu;
+                s = fmaf(v[j][i], v[j][i], s);
+            }
         }
     }
     const float rs = __frsqrt_rn(__fdiv_rn(row_sum<TPR>(s, red), fd) + a.eps);
@@ -231,10 +242,8 @@ __global__ void __launch_bounds__(row_block(TPR)) norm_row_kernel(NormArgs a, bo
         if (a.mean) a.mean[r] = mu;
         if (a.rstd) a.rstd[r] = rs;
     }
-#pragma unroll
-    for (int j = 0; j < VPT; ++j) {
+    auto finish = [&](int j) {
         const int c = (first + j * 32) * VE;
-        if (c >= a.d) continue;
         float g[VE], b[VE];
         load_params<T, VE>(a.gamma, a.ptype, pvec, c, 1.0f, g);
         load_params<T, VE>(a.beta, a.ptype, pvec, c, 0.0f, b);
@@ -243,6 +252,14 @@ __global__ void __launch_bounds__(row_block(TPR)) norm_row_kernel(NormArgs a, bo
         if constexpr (!FP8) {
             if (live) store_pack<T, VE>(static_cast<T*>(a.y) + r * a.ldy + c, v[j]);
         }
+    };
+    if (full) {
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) finish(j);
+    } else {
+#pragma unroll
+        for (int j = 0; j < VPT; ++j)
+            if ((first + j * 32) * VE < a.d) finish(j);
     }
     if constexpr (FP8) store_codes<VE, VPT, TPR>(v, a.q, r, a.d, live, first, lane, wide);
 }
@@ -297,7 +314,7 @@ cudaError_t norm_t(const NormArgs& a, cudaStream_t s) {
 }
 
 // ---------------------------------------------------------------------------
-// Backward with a row of x and dy in registers: TPR threads per row, 16 elements each, both row sums in
+// Backward with a row of x and dy in registers: TPR threads per row, VPT packs each, both row sums in
 // one reduction.  Blocks walk over the rows; a thread's columns are the same in every row, so the
 // parameter gradients are sums in its registers (in shared memory where a block of 1,024 threads
 // leaves 64 registers a thread), written once per block.  The next row's loads are issued before this
@@ -348,10 +365,10 @@ __device__ __forceinline__ float2 row_sum2(float a, float b, float2 (*red)[32], 
 
 constexpr int grad_block(int tpr) { return tpr > 256 ? tpr : 256; }
 
-template <typename T, int VE, int TPR>
-__global__ void __launch_bounds__(grad_block(TPR), TPR > 256 ? 1 : 2)
+template <typename T, int VE, int VPT, int TPR>
+__global__ void __launch_bounds__(grad_block(TPR), TPR > 256 ? 1 : (VE * VPT > 8 ? 2 : 4))
 norm_grad_row_kernel(NormGradArgs a, bool pvec) {
-    constexpr int VPT = 16 / VE, kThreads = grad_block(TPR), kRows = kThreads / TPR;
+    constexpr int kThreads = grad_block(TPR), kRows = kThreads / TPR;
     constexpr bool kShared = TPR == 1024;
     __shared__ float2 red[2][32];
     extern __shared__ float sums[];  // 2 x d: the block's sums, joined at the end (kShared: all along)
@@ -361,15 +378,21 @@ norm_grad_row_kernel(NormGradArgs a, bool pvec) {
     float gam[VPT][VE], pg[VPT][VE], pb[VPT][VE];
     Raw<T, VE> rx[VPT], rg[VPT];
     float mu_next = 0.0f, rs_next = 0.0f;
+    const bool full = (first - lane + VPT * 32) * VE <= a.d;
     auto fetch = [&](int64_t r) {
-        if (r < a.rows) mu_next = __ldg(a.mean + r), rs_next = __ldg(a.rstd + r);
-        const T* x = static_cast<const T*>(a.x) + r * a.ldx;
-        const T* dy = static_cast<const T*>(a.dy) + r * a.lddy;
+        const T* x = static_cast<const T*>(a.x) + r * a.ldx + first * VE;
+        const T* dy = static_cast<const T*>(a.dy) + r * a.lddy + first * VE;
+        if (r < a.rows && full) {
+            mu_next = __ldg(a.mean + r), rs_next = __ldg(a.rstd + r);
 #pragma unroll
-        for (int j = 0; j < VPT; ++j) {
-            const int c = (first + j * 32) * VE;
-            if (r < a.rows && c < a.d) rx[j].load(x + c), rg[j].load(dy + c);
-            else rx[j].zero(), rg[j].zero();
+            for (int j = 0; j < VPT; ++j) rx[j].load(x + j * 32 * VE), rg[j].load(dy + j * 32 * VE);
+        } else {
+            if (r < a.rows) mu_next = __ldg(a.mean + r), rs_next = __ldg(a.rstd + r);
+#pragma unroll
+            for (int j = 0; j < VPT; ++j) {
+                if (r < a.rows && (first + j * 32) * VE < a.d) rx[j].load(x + j * 32 * VE), rg[j].load(dy + j * 32 * VE);
+                else rx[j].zero(), rg[j].zero();
+            }
         }
     };
 #pragma unroll
@@ -424,15 +447,20 @@ norm_grad_row_kernel(NormGradArgs a, bool pvec) {
         fetch(r + step);
         const float2 t = row_sum2<TPR>(s1, s2, red, buf);
         const float m1 = __fdiv_rn(t.x, fd), m2 = __fdiv_rn(t.y, fd);
-        T* dx = static_cast<T*>(a.dx) + r * a.lddx;
-#pragma unroll
-        for (int j = 0; j < VPT; ++j) {
-            const int c = (first + j * 32) * VE;
-            if (!live || c >= a.d) continue;
+        T* dx = static_cast<T*>(a.dx) + r * a.lddx + first * VE;
+        auto put = [&](int j) {
             float o[VE];
 #pragma unroll
             for (int i = 0; i < VE; ++i) o[i] = rs * (g[j][i] - m1 - xh[j][i] * m2);
-            store_pack<T, VE>(dx + c, o);
+            store_pack<T, VE>(dx + j * 32 * VE, o);
+        };
+        if (live && full) {
+#pragma unroll
+            for (int j = 0; j < VPT; ++j) put(j);
+        } else if (live) {
+#pragma unroll
+            for (int j = 0; j < VPT; ++j)
+                if ((first + j * 32) * VE < a.d) put(j);
         }
     }
     if (!a.part) return;
@@ -463,9 +491,9 @@ norm_grad_row_kernel(NormGradArgs a, bool pvec) {
     }
 }
 
-template <typename T, int VE, int TPR>
+template <typename T, int VE, int VPT, int TPR>
 cudaError_t norm_grad_row(const NormGradArgs& a, bool pvec, cudaStream_t s) {
-    auto kern = norm_grad_row_kernel<T, VE, TPR>;
+    auto kern = norm_grad_row_kernel<T, VE, VPT, TPR>;
     const int smem = a.part ? 2 * a.d * 4 : 0;
     cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), smem);
     if (e != cudaSuccess) return e;
@@ -473,14 +501,16 @@ cudaError_t norm_grad_row(const NormGradArgs& a, bool pvec, cudaStream_t s) {
     return cudaGetLastError();
 }
 
+// Eight elements a thread up to 1,024 columns (four blocks an SM), sixteen above (two; one over 4,096).
 template <typename T, int VE>
 cudaError_t norm_grad_width(const NormGradArgs& a, bool pvec, cudaStream_t s) {
-    if (a.d <= 512) return norm_grad_row<T, VE, 32>(a, pvec, s);
-    if (a.d <= 1024) return norm_grad_row<T, VE, 64>(a, pvec, s);
-    if (a.d <= 2048) return norm_grad_row<T, VE, 128>(a, pvec, s);
-    if (a.d <= 4096) return norm_grad_row<T, VE, 256>(a, pvec, s);
-    if (a.d <= 8192) return norm_grad_row<T, VE, 512>(a, pvec, s);
-    return norm_grad_row<T, VE, 1024>(a, pvec, s);
+    if (a.d <= 256) return norm_grad_row<T, VE, 8 / VE, 32>(a, pvec, s);
+    if (a.d <= 512) return norm_grad_row<T, VE, 8 / VE, 64>(a, pvec, s);
+    if (a.d <= 1024) return norm_grad_row<T, VE, 8 / VE, 128>(a, pvec, s);
+    if (a.d <= 2048) return norm_grad_row<T, VE, 16 / VE, 128>(a, pvec, s);
+    if (a.d <= 4096) return norm_grad_row<T, VE, 16 / VE, 256>(a, pvec, s);
+    if (a.d <= 8192) return norm_grad_row<T, VE, 16 / VE, 512>(a, pvec, s);
+    return norm_grad_row<T, VE, 16 / VE, 1024>(a, pvec, s);
 }
 
 template <typename T>
@@ -509,8 +539,10 @@ cudaError_t layer_norm_launch(const NormArgs& a, int xtype, cudaStream_t s) {
 // Blocks of the backward kernels, each with its own partial sums: enough to fill the SMs at the
 // kernels' occupancy, few enough that the partial sums stay small against the rows.
 int layer_norm_parts(int64_t rows, int64_t d) {
-    const int64_t cap = (d <= 4096 ? 2ll : 1ll) * device_sm_count();
-    return static_cast<int>(rows < cap ? rows : cap);
+    const int64_t per_block = d <= 256 ? 8 : (d <= 512 ? 4 : (d <= 2048 ? 2 : 1));  // rows at a time
+    const int64_t cap = (d <= 1024 ? 4ll : (d <= 4096 ? 2ll : 1ll)) * device_sm_count();
+    const int64_t want = (rows + per_block - 1) / per_block;
+    return static_cast<int>(want < cap ? want : cap);
 }
 
 cudaError_t column_reduce_launch(const float* part, int parts, int64_t n, void* out0, void* out1, int otype,

@@ -37,40 +37,60 @@ __device__ __forceinline__ void store_pack(T* p, const float (&o)[VE]) {
 }
 // FP8 codes of a lane's VPT packs (values v, zero beyond column d): pack j holds columns (first_pack +
 // 32 j) VE .., so a group of 128 lies in one warp.  A group's maximum is taken over all its elements
-// first and again over the finite ones where it is infinite (a NaN is no maximum anyway).  `wide`:
+// first and again over the finite ones where it is infinite (a NaN is no maximum anyway).  The
+// division and the reciprocal of a scale are done by one lane per group, all groups at once.  `wide`:
 // code rows start on 8-byte boundaries.
 template <int VE, int VPT, int TPR>
 __device__ __forceinline__ void store_codes(const float (&v)[VPT][VE], const Fp8Out& q, int64_t r, int64_t d, bool live,
                                             int64_t first_pack, int lane, bool wide) {
-    constexpr int kPerGroup = VE == 1 ? 4 : 1;                                      // packs of a lane in one group
+    constexpr int kPer = VE == 1 ? 4 : 1;                                           // packs of a lane in one group
     constexpr int kLanes = VE == 1 ? 32 : (kGroup / VE < TPR ? kGroup / VE : TPR);  // lanes of one group
+    constexpr int kGroups = VPT / kPer;
+    static_assert(kGroups <= kLanes, "a lane for each group");
+    float am[kGroups];
+    auto maxima = [&](bool finite) {
 #pragma unroll
-    for (int j = 0; j < VPT; j += kPerGroup) {
-        float am = 0.0f;
+        for (int j = 0; j < kGroups; ++j) {
+            am[j] = 0.0f;
 #pragma unroll
-        for (int h = 0; h < kPerGroup; ++h)
+            for (int h = 0; h < kPer; ++h)
 #pragma unroll
-            for (int i = 0; i < VE; ++i) am = fmaxf(am, fabsf(v[j + h][i]));
+                for (int i = 0; i < VE; ++i)
+                    am[j] = fmaxf(am[j], finite ? finite_abs(v[j * kPer + h][i]) : fabsf(v[j * kPer + h][i]));
 #pragma unroll
-        for (int o = kLanes / 2; o > 0; o >>= 1) am = fmaxf(am, __shfl_xor_sync(0xFFFFFFFFu, am, o));
-        if (__any_sync(0xFFFFFFFFu, !(am <= 3.402823466e38f))) {
-            am = 0.0f;
-#pragma unroll
-            for (int h = 0; h < kPerGroup; ++h)
-#pragma unroll
-                for (int i = 0; i < VE; ++i) am = fmaxf(am, finite_abs(v[j + h][i]));
-#pragma unroll
-            for (int o = kLanes / 2; o > 0; o >>= 1) am = fmaxf(am, __shfl_xor_sync(0xFFFFFFFFu, am, o));
+            for (int o = kLanes / 2; o > 0; o >>= 1) am[j] = fmaxf(am[j], __shfl_xor_sync(0xFFFFFFFFu, am[j], o));
         }
-        const float sc = group_scale(am), inv = __frcp_rn(sc);
-        const int64_t c0 = (first_pack + j * 32) * VE;  // this lane's first column
-        if (live && c0 < d && (VE == 1 ? lane == 0 : lane % kLanes == 0)) q.scales[r * q.srs + (c0 / kGroup) * q.sbs] = sc;
+    };
+    maxima(false);
+    float mine = am[0], top = am[0];
+    const int at = lane % kLanes;
+#pragma unroll
+    for (int j = 1; j < kGroups; ++j) top = fmaxf(top, am[j]);
+    if (__any_sync(0xFFFFFFFFu, !(top <= 3.402823466e38f))) {
+        maxima(true);
+        mine = am[0];
+    }
+#pragma unroll
+    for (int j = 1; j < kGroups; ++j) mine = at == j ? am[j] : mine;
+    const float sc = group_scale(mine), inv_mine = __frcp_rn(sc);
+    // the first column of group `at` of this lane's row
+    const int64_t c_at = (first_pack - at + static_cast<int64_t>(at) * kPer * 32) * VE;
+    if (live && at < kGroups && c_at < d) q.scales[r * q.srs + (c_at / kGroup) * q.sbs] = sc;
+#pragma unroll
+    for (int j = 0; j < kGroups; ++j) {
+        const float inv = __shfl_sync(0xFFFFFFFFu, inv_mine, j, kLanes);
+        const int64_t c0 = (first_pack + j * kPer * 32) * VE;  // this lane's first column
         uint8_t* dst = q.codes + r * q.ld + c0;
         if constexpr (VE == 1) {
-            const uint32_t w = e4m3_encode4(v[j][0] * inv, v[j + 1][0] * inv, v[j + 2][0] * inv, v[j + 3][0] * inv);
+            const uint32_t w = e4m3_encode4(v[4 * j][0] * inv, v[4 * j + 1][0] * inv, v[4 * j + 2][0] * inv, v[4 * j + 3][0] * inv);
+            if (live && c0 - lane + kGroup <= d) {
 #pragma unroll
-            for (int h = 0; h < 4; ++h)
-                if (live && c0 + h * 32 < d) dst[h * 32] = static_cast<uint8_t>(w >> (8 * h));
+                for (int h = 0; h < 4; ++h) dst[h * 32] = static_cast<uint8_t>(w >> (8 * h));
+            } else {
+#pragma unroll
+                for (int h = 0; h < 4; ++h)
+                    if (live && c0 + h * 32 < d) dst[h * 32] = static_cast<uint8_t>(w >> (8 * h));
+            }
         } else {
             uint32_t w[VE / 4];
 #pragma unroll

@@ -9,6 +9,7 @@
 #include "nfx_internal.h"
 #include "numerics.cuh"
 #include "row_pack.cuh"
+#include "sm100.cuh"
 
 namespace nfx {
 namespace {
@@ -35,120 +36,145 @@ __global__ void __launch_bounds__(128) quant_rows_kernel(QuantArgs a, int64_t ch
     store_codes<VE, VPT, TPR>(v, a.q, r, a.cols, live, first, lane, wide);
 }
 
-// One block per 128 x 128 tile.  A thread holds 8 rows x 8 columns in registers: lane % 16 counts the
-// columns' eights, 2 * warp + lane / 16 the rows'.  A row's maximum is 8 values and four shuffles, a
-// column's 8 values, a shuffle and eight partial results in shared memory.  The transposed codes go
-// through shared memory (16 KB, 8-byte slots XOR-ed with the column's eight, so that neither side has
-// more conflicts than its width) and leave as 128-byte rows.  The tile is read once from HBM and its
-// bytes are the bound; `VEC`: rows of x start on 16-byte boundaries.
+// 128 x 128 tiles, one at a time per block.  A thread holds 8 rows x 8
+// columns in registers: lane % 16 counts the columns' eights, 2 * warp + lane / 16 the rows'.  A row's
+// maximum is 8 values and four shuffles, a column's 8 values, a shuffle and eight partial results in
+// shared memory; scales and reciprocals are made by one thread per row and per column.  The
+// transposed codes go through shared memory (16 KB, 8-byte slots XOR-ed with the column's eight, so that
+// neither side has more conflicts than its width) and leave as 128-byte rows.  The tile's bytes are the
+// bound; what keeps them coming for 16-bit types (kAhead) is that the blocks walk over the tiles and a
+// thread copies its part of the next one into shared memory (cp.async, its own slots, so no barrier)
+// while it works on this one: 16384x4096 bf16 both ways with sums 85 us, 147 with a block per tile.  An
+// fp32 tile is twice the bytes for the same work, and there a block per tile is faster (131072x128 to
+// tiles: 17 us, 28 walking).  `VEC`: rows of x start on 16-byte boundaries.
 constexpr int kTileThreads = 256;
 
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kTileThreads, 2) quant_tile_kernel(QuantArgs a, bool wide, bool wide_t) {
+constexpr bool kAhead = VEC && sizeof(T) == 2;
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kTileThreads, 2) quant_tile_kernel(QuantArgs a, int tiles, int cblocks, bool wide,
+                                                                     bool wide_t) {
+    extern __shared__ __align__(16) uint8_t next[];  // the next tile: slot n of thread t at (n * 256 + t) * 16
     __shared__ __align__(16) uint8_t tileT[kGroup * kGroup];
-    __shared__ float cmax[8][kGroup], csum[8][kGroup], rscale[kGroup], cinv[kGroup];
+    __shared__ __align__(16) float cmax[8][kGroup], csum[8][kGroup], rmax[kGroup], rinv[kGroup], cinv[kGroup];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int cc = lane & 15, rr = warp * 2 + (lane >> 4);  // this thread's eights
-    const int64_t cblocks = (a.cols + kGroup - 1) / kGroup;
-    const int64_t br = blockIdx.x / cblocks, bc = blockIdx.x % cblocks;
-    const int64_t r0 = br * kGroup + rr * 8, c0 = bc * kGroup + cc * 8;
-    constexpr int VE = 16 / sizeof(T);
-    float v[8][8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const T* x = static_cast<const T*>(a.x) + (r0 + i) * a.ldx + c0;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[i][k] = 0.0f;
-        if (r0 + i >= a.rows) continue;
-        if (VEC && c0 + 8 <= a.cols) {
-#pragma unroll
-            for (int k = 0; k < 8; k += VE) {
-                float o[VE];
-                load_pack<T, VE>(x + k, o);
-#pragma unroll
-                for (int e = 0; e < VE; ++e) v[i][k + e] = o[e];
-            }
-        } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (c0 + k < a.cols) v[i][k] = to_f32(x[k]);
-        }
-    }
-    // largest magnitudes and sums; `finite` is the second look, when a maximum is infinite
-    float rm[8], cm[8];
-    auto maxima = [&](bool finite) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) rm[i] = cm[i] = 0.0f;
+    constexpr int VE = 16 / sizeof(T), kPacks = 8 / VE;
+    const bool cols_too = a.qt.codes || a.part;
+    constexpr bool kWalk = kAhead<T, VEC>;
+
+    auto ahead = [&](int t) {
+        const int64_t r0 = static_cast<int64_t>(t / cblocks) * kGroup + rr * 8, c0 = static_cast<int64_t>(t % cblocks) * kGroup + cc * 8;
+        const T* x = static_cast<const T*>(a.x) + r0 * a.ldx + c0;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const float m = finite ? finite_abs(v[i][k]) : fabsf(v[i][k]);
-                rm[i] = fmaxf(rm[i], m);
-                cm[k] = fmaxf(cm[k], m);
+            for (int k = 0; k < kPacks; ++k) {
+                const int64_t left = r0 + i < a.rows ? a.cols - c0 - k * VE : 0;
+                const int n = left >= VE ? 16 : (left > 0 ? static_cast<int>(left * sizeof(T)) : 0);
+                cp_async16(next + ((i * kPacks + k) * kTileThreads + threadIdx.x) * 16, n ? x + i * a.ldx + k * VE : a.x, n);
             }
     };
-    maxima(false);
-    float top = 0.0f;
+    if (kWalk) ahead(blockIdx.x);
+
+    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+        const int64_t br = tile / cblocks, bc = tile % cblocks;
+        const int64_t r0 = br * kGroup + rr * 8, c0 = bc * kGroup + cc * 8;
+        float v[8][8];
+        if constexpr (kWalk) {
+            cp_async_wait_all();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = fmaxf(top, rm[i]);
-    if (!(top <= 3.402823466e38f)) maxima(true);
-    if (a.tile) {
-        top = 0.0f;
+            for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmaxf(top, rm[i]);
-        top = warp_max(top);
-        if (lane == 0) cmax[warp][0] = top;
-        __syncthreads();
+                for (int k = 0; k < kPacks; ++k) {
+                    const Pack<T, VE> p =
+                        *reinterpret_cast<const Pack<T, VE>*>(next + ((i * kPacks + k) * kTileThreads + threadIdx.x) * 16);
 #pragma unroll
-        for (int w = 0; w < 8; ++w) top = fmaxf(top, cmax[w][0]);
-    } else {
+                    for (int e = 0; e < VE; ++e) v[i][k * VE + e] = to_f32(p.v[e]);
+                }
+        } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+            for (int i = 0; i < 8; ++i) {
+                const T* x = static_cast<const T*>(a.x) + (r0 + i) * a.ldx + c0;
+                if (VEC && r0 + i < a.rows && c0 + 8 <= a.cols) {
 #pragma unroll
-            for (int o = 8; o > 0; o >>= 1) rm[i] = fmaxf(rm[i], __shfl_xor_sync(0xFFFFFFFFu, rm[i], o));
-        if (a.qt.codes || a.part) {
+                    for (int k = 0; k < kPacks; ++k) {
+                        float o[VE];
+                        load_pack<T, VE>(x + k * VE, o);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                float s = 0.0f;
+                        for (int e = 0; e < VE; ++e) v[i][k * VE + e] = o[e];
+                    }
+                } else {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) s += v[i][k];
-                s += __shfl_xor_sync(0xFFFFFFFFu, s, 16);
-                cm[k] = fmaxf(cm[k], __shfl_xor_sync(0xFFFFFFFFu, cm[k], 16));
-                if (lane < 16) {
-                    cmax[warp][cc * 8 + k] = cm[k];
-                    csum[warp][cc * 8 + k] = s;
+                    for (int k = 0; k < 8; ++k) v[i][k] = r0 + i < a.rows && c0 + k < a.cols ? to_f32(x[k]) : 0.0f;
                 }
             }
         }
-    }
-    // codes along the rows
-    const float tscale = group_scale(top), tinv = __frcp_rn(tscale);
+        // largest magnitudes; `finite` is the second look, when a maximum is infinite
+        float rm[8], cm[8], top = 0.0f;
+        auto maxima = [&](bool finite) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float sc = a.tile ? tscale : group_scale(rm[i]), inv = a.tile ? tinv : __frcp_rn(sc);
-        if (!a.tile && cc == 0) rscale[rr * 8 + i] = sc;
-        const uint32_t w0 = e4m3_encode4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
-        const uint32_t w1 = e4m3_encode4(v[i][4] * inv, v[i][5] * inv, v[i][6] * inv, v[i][7] * inv);
-        if (r0 + i >= a.rows || c0 >= a.cols) continue;
-        uint8_t* dst = a.q.codes + (r0 + i) * a.q.ld + c0;
-        if (wide && c0 + 8 <= a.cols) {
-            *reinterpret_cast<uint2*>(dst) = make_uint2(w0, w1);
+            for (int i = 0; i < 8; ++i) rm[i] = cm[i] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const float m = finite ? finite_abs(v[i][k]) : fabsf(v[i][k]);
+                    rm[i] = fmaxf(rm[i], m);
+                    cm[k] = fmaxf(cm[k], m);
+                }
+            top = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = fmaxf(top, rm[i]);
+        };
+        maxima(false);
+        if (!(top <= 3.402823466e38f)) maxima(true);
+        if (a.tile) {
+            top = warp_max(top);
+            if (lane == 0) rmax[warp] = top;
         } else {
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (c0 + k < a.cols) dst[k] = static_cast<uint8_t>((k < 4 ? w0 : w1) >> (8 * (k & 3)));
+            for (int i = 0; i < 8; ++i) {
+#pragma unroll
+                for (int o = 8; o > 0; o >>= 1) rm[i] = fmaxf(rm[i], __shfl_xor_sync(0xFFFFFFFFu, rm[i], o));
+                if (cc == i) rmax[rr * 8 + i] = rm[i];
+            }
+            if (cols_too) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    float s = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) s += v[i][k];
+                    s += __shfl_xor_sync(0xFFFFFFFFu, s, 16);
+                    cm[k] = fmaxf(cm[k], __shfl_xor_sync(0xFFFFFFFFu, cm[k], 16));
+                    if (lane < 16) {
+                        cmax[warp][cc * 8 + k] = cm[k];
+                        csum[warp][cc * 8 + k] = s;
+                    }
+                }
+            }
         }
-    }
-    if (a.tile && threadIdx.x == 0) {
-        a.q.scales[br * a.q.srs + bc * a.q.sbs] = tscale;
-        if (a.qt.codes) a.qt.scales[bc * a.qt.srs + br * a.qt.sbs] = tscale;
-    }
-    __syncthreads();
-    if (!a.tile && threadIdx.x < kGroup) {
-        const int t = threadIdx.x;
-        if (br * kGroup + t < a.rows) a.q.scales[(br * kGroup + t) * a.q.srs + bc * a.q.sbs] = rscale[t];
-        if (a.qt.codes || a.part) {
+        __syncthreads();
+        // this tile's values are in registers: the slots are free for the next one
+        if (kWalk && tile + gridDim.x < tiles) ahead(tile + gridDim.x);
+        float tinv = 0.0f;
+        if (a.tile) {
+#pragma unroll
+            for (int w = 0; w < 8; ++w) top = fmaxf(top, rmax[w]);
+            const float sc = group_scale(top);
+            tinv = __frcp_rn(sc);
+            if (threadIdx.x == 0) {
+                a.q.scales[br * a.q.srs + bc * a.q.sbs] = sc;
+                if (a.qt.codes) a.qt.scales[bc * a.qt.srs + br * a.qt.sbs] = sc;
+            }
+        } else if (threadIdx.x < kGroup) {
+            const int t = threadIdx.x;
+            const float sc = group_scale(rmax[t]);
+            rinv[t] = __frcp_rn(sc);
+            if (br * kGroup + t < a.rows) a.q.scales[(br * kGroup + t) * a.q.srs + bc * a.q.sbs] = sc;
+        } else if (cols_too) {
+            const int t = threadIdx.x - kGroup;
             float m = 0.0f, s = 0.0f;
 #pragma unroll
             for (int w = 0; w < 8; ++w) {
@@ -162,36 +188,66 @@ __global__ void __launch_bounds__(kTileThreads, 2) quant_tile_kernel(QuantArgs a
                 if (a.qt.codes) a.qt.scales[(bc * kGroup + t) * a.qt.srs + br * a.qt.sbs] = sc;
             }
         }
-    }
-    if (!a.qt.codes) return;
-    if (!a.tile) __syncthreads();
-    // codes along the columns
+        __syncthreads();
+        // codes along the rows
+        const bool inside = wide && c0 + 8 <= a.cols && r0 + 8 <= a.rows;
+        uint8_t* row = a.q.codes + r0 * a.q.ld + c0;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        const float inv = a.tile ? tinv : cinv[cc * 8 + k];
-        const uint32_t w0 = e4m3_encode4(v[0][k] * inv, v[1][k] * inv, v[2][k] * inv, v[3][k] * inv);
-        const uint32_t w1 = e4m3_encode4(v[4][k] * inv, v[5][k] * inv, v[6][k] * inv, v[7][k] * inv);
-        *reinterpret_cast<uint2*>(tileT + (cc * 8 + k) * kGroup + (rr ^ cc) * 8) = make_uint2(w0, w1);
-    }
-    __syncthreads();
+        for (int i = 0; i < 8; ++i) {
+            const float inv = a.tile ? tinv : rinv[rr * 8 + i];
+            const uint32_t w0 = e4m3_encode4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
+            const uint32_t w1 = e4m3_encode4(v[i][4] * inv, v[i][5] * inv, v[i][6] * inv, v[i][7] * inv);
+            if (inside) {
+                *reinterpret_cast<uint2*>(row + i * a.q.ld) = make_uint2(w0, w1);
+            } else if (r0 + i < a.rows) {
 #pragma unroll
-    for (int n = 0; n < kGroup * 8 / kTileThreads; ++n) {
-        const int t = n * kTileThreads + threadIdx.x, col = t >> 3, half = t & 7;  // 16 rows of one column
-        const int e = col >> 3;
-        uint4 w = *reinterpret_cast<const uint4*>(tileT + col * kGroup + ((2 * half) ^ (e & 14)) * 8);
-        if (e & 1) w = make_uint4(w.z, w.w, w.x, w.y);
-        const int64_t c = bc * kGroup + col, r = br * kGroup + half * 16;
-        if (c >= a.cols || r >= a.rows) continue;
-        uint8_t* dst = a.qt.codes + c * a.qt.ld + r;
-        if (wide_t && r + 16 <= a.rows) {
-            *reinterpret_cast<uint4*>(dst) = w;
-        } else {
-            const uint32_t b[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-            for (int k = 0; k < 16; ++k)
-                if (r + k < a.rows) dst[k] = static_cast<uint8_t>(b[k >> 2] >> (8 * (k & 3)));
+                for (int k = 0; k < 8; ++k)
+                    if (c0 + k < a.cols) row[i * a.q.ld + k] = static_cast<uint8_t>((k < 4 ? w0 : w1) >> (8 * (k & 3)));
+            }
         }
+        if (!a.qt.codes) continue;
+        // codes along the columns
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float inv = a.tile ? tinv : cinv[cc * 8 + k];
+            const uint32_t w0 = e4m3_encode4(v[0][k] * inv, v[1][k] * inv, v[2][k] * inv, v[3][k] * inv);
+            const uint32_t w1 = e4m3_encode4(v[4][k] * inv, v[5][k] * inv, v[6][k] * inv, v[7][k] * inv);
+            *reinterpret_cast<uint2*>(tileT + (cc * 8 + k) * kGroup + (rr ^ cc) * 8) = make_uint2(w0, w1);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < kGroup * 8 / kTileThreads; ++n) {
+            const int t = n * kTileThreads + threadIdx.x, col = t >> 3, part = t & 7;  // 16 rows of one column
+            const int e = col >> 3;
+            uint4 w = *reinterpret_cast<const uint4*>(tileT + col * kGroup + ((2 * part) ^ (e & 14)) * 8);
+            if (e & 1) w = make_uint4(w.z, w.w, w.x, w.y);
+            const int64_t c = bc * kGroup + col, r = br * kGroup + part * 16;
+            if (c >= a.cols || r >= a.rows) continue;
+            uint8_t* dst = a.qt.codes + c * a.qt.ld + r;
+            if (wide_t && r + 16 <= a.rows) {
+                *reinterpret_cast<uint4*>(dst) = w;
+            } else {
+                const uint32_t b[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int k = 0; k < 16; ++k)
+                    if (r + k < a.rows) dst[k] = static_cast<uint8_t>(b[k >> 2] >> (8 * (k & 3)));
+            }
+        }
+        // (the next tile's maxima are written before its first barrier, its transposed codes after it)
     }
+}
+
+template <typename T, bool VEC>
+cudaError_t quant_tile(const QuantArgs& a, bool wide, bool wide_t, cudaStream_t s) {
+    const int64_t cblocks = (a.cols + kGroup - 1) / kGroup, tiles = (a.rows + kGroup - 1) / kGroup * cblocks;
+    auto kern = quant_tile_kernel<T, VEC>;
+    const int smem = kAhead<T, VEC> ? kGroup * kGroup * static_cast<int>(sizeof(T)) : 0;
+    cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), smem);
+    if (e != cudaSuccess) return e;
+    const int64_t cap = kAhead<T, VEC> ? 2ll * device_sm_count() : tiles;
+    kern<<<static_cast<unsigned>(tiles < cap ? tiles : cap), kTileThreads, smem, s>>>(
+        a, static_cast<int>(tiles), static_cast<int>(cblocks), wide, wide_t);
+    return cudaGetLastError();
 }
 
 bool code_rows(const Fp8Out& q, int64_t rows, int64_t bytes) {
@@ -218,11 +274,8 @@ cudaError_t quant_t(const QuantArgs& a, cudaStream_t s) {
         if (a.cols <= 32 * VE) return quant_rows<T, VE, 1, 32>(a, s);
         return quant_rows<T, VE, 2, 32>(a, s);
     }
-    const int64_t tiles = (a.rows + kGroup - 1) / kGroup * ((a.cols + kGroup - 1) / kGroup);
     const bool wide = code_rows(a.q, a.rows, 8), wide_t = code_rows(a.qt, a.cols, 16);
-    if (rows16) quant_tile_kernel<T, true><<<static_cast<unsigned>(tiles), kTileThreads, 0, s>>>(a, wide, wide_t);
-    else quant_tile_kernel<T, false><<<static_cast<unsigned>(tiles), kTileThreads, 0, s>>>(a, wide, wide_t);
-    return cudaGetLastError();
+    return rows16 ? quant_tile<T, true>(a, wide, wide_t, s) : quant_tile<T, false>(a, wide, wide_t, s);
 }
 
 }  // namespace

@@ -19,6 +19,13 @@ namespace {
 
 constexpr int kAnyThreads = 256;
 
+// s / d with d's reciprocal at hand: the product, and one correction by the exact remainder (Markstein's
+// step), which gives back a constant row's value exactly.
+__device__ __forceinline__ float mean_of(float s, float fd, float inv_d) {
+    const float q = s * inv_d;
+    return fmaf(fmaf(-q, fd, s), inv_d, q);
+}
+
 // Sum of v over the block, the same value in every thread.  `red` holds one float per warp.
 __device__ __forceinline__ float block_sum(float v, float* red) {
     v = warp_sum(v);
@@ -183,12 +190,13 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
 #pragma unroll
     for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
     if constexpr (TPR > 32) {
+        const int w = threadIdx.x >> 5, w0 = w / (TPR / 32) * (TPR / 32);  // the row's first warp
         __syncthreads();  // the previous sum has been read
-        if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+        if ((threadIdx.x & 31) == 0) red[w] = v;
         __syncthreads();
-        v = red[0];
+        v = red[w0];
 #pragma unroll
-        for (int w = 1; w < TPR / 32; ++w) v += red[w];
+        for (int k = 1; k < TPR / 32; ++k) v += red[w0 + k];
     }
     return v;
 }
@@ -197,7 +205,7 @@ constexpr int row_block(int tpr) { return tpr > 128 ? tpr : 128; }
 
 template <typename T, int VE, int VPT, int TPR, bool FP8>
 __global__ void __launch_bounds__(row_block(TPR)) norm_row_kernel(NormArgs a, bool pvec, bool wide) {
-    __shared__ float red[TPR > 32 ? TPR / 32 : 1];
+    __shared__ float red[row_block(TPR) / 32];
     constexpr int kRows = row_block(TPR) / TPR;
     const int lane = threadIdx.x & 31, sub = threadIdx.x % TPR;
     const int64_t r = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / TPR;
@@ -225,7 +233,8 @@ __global__ void __launch_bounds__(row_block(TPR)) norm_row_kernel(NormArgs a, bo
     for (int j = 0; j < VPT; ++j)
 #pragma unroll
         for (int i = 0; i < VE; ++i) s += v[j][i];
-    const float mu = __fdiv_rn(row_sum<TPR>(s, red), fd);
+    const float inv_d = __frcp_rn(fd);
+    const float mu = mean_of(row_sum<TPR>(s, red), fd, inv_d);
     s = 0.0f;
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
@@ -237,7 +246,7 @@ __global__ void __launch_bounds__(row_block(TPR)) norm_row_kernel(NormArgs a, bo
             }
         }
     }
-    const float rs = __frsqrt_rn(__fdiv_rn(row_sum<TPR>(s, red), fd) + a.eps);
+    const float rs = __frsqrt_rn(fmaf(row_sum<TPR>(s, red), inv_d, a.eps));
     if (live && sub == 0) {
         if (a.mean) a.mean[r] = mu;
         if (a.rstd) a.rstd[r] = rs;
@@ -278,24 +287,32 @@ cudaError_t norm_row(const NormArgs& a, bool pvec, cudaStream_t s) {
     return cudaGetLastError();
 }
 
-// Threads and packs per row by the width: the fewest threads that leave a thread 32 elements at most.
+// Threads and packs per row by the width: the fewest threads that leave a thread 32 elements at most, and
+// with single-element packs 8 up to 4,096 columns (more loads to a row than a warp should queue:
+// 5003x771 fp32 takes 19 us with 32).
 template <typename T, int VE>
 cudaError_t norm_width(const NormArgs& a, bool pvec, cudaStream_t s) {
-    constexpr int kV = 32 / VE;  // packs of 32 elements
     if constexpr (VE > 1) {
+        constexpr int kV = 32 / VE;  // packs of 32 elements
         if (a.d <= 16 * VE) return norm_row<T, VE, 1, 16>(a, pvec, s);
         if (a.d <= 32 * VE) return norm_row<T, VE, 1, 32>(a, pvec, s);
         if (a.d <= 64 * VE) return norm_row<T, VE, 2, 32>(a, pvec, s);
+        if (a.d <= 512) return norm_row<T, VE, kV / 2, 32>(a, pvec, s);
+        if (a.d <= 1024) return norm_row<T, VE, kV, 32>(a, pvec, s);
+        if (a.d <= 2048) return norm_row<T, VE, kV / 2, 128>(a, pvec, s);
+        if (a.d <= 4096) return norm_row<T, VE, kV, 128>(a, pvec, s);
+        if (a.d <= 8192) return norm_row<T, VE, kV, 256>(a, pvec, s);
+        return norm_row<T, VE, kV, 512>(a, pvec, s);
     } else {
         if (a.d <= 128) return norm_row<T, VE, 4, 32>(a, pvec, s);
         if (a.d <= 256) return norm_row<T, VE, 8, 32>(a, pvec, s);
+        if (a.d <= 512) return norm_row<T, VE, 8, 64>(a, pvec, s);
+        if (a.d <= 1024) return norm_row<T, VE, 8, 128>(a, pvec, s);
+        if (a.d <= 2048) return norm_row<T, VE, 8, 256>(a, pvec, s);
+        if (a.d <= 4096) return norm_row<T, VE, 8, 512>(a, pvec, s);
+        if (a.d <= 8192) return norm_row<T, VE, 16, 512>(a, pvec, s);
+        return norm_row<T, VE, 32, 512>(a, pvec, s);
     }
-    if (a.d <= 512) return norm_row<T, VE, kV / 2, 32>(a, pvec, s);
-    if (a.d <= 1024) return norm_row<T, VE, kV, 32>(a, pvec, s);
-    if (a.d <= 2048) return norm_row<T, VE, kV / 2, 128>(a, pvec, s);
-    if (a.d <= 4096) return norm_row<T, VE, kV, 128>(a, pvec, s);
-    if (a.d <= 8192) return norm_row<T, VE, kV, 256>(a, pvec, s);
-    return norm_row<T, VE, kV, 512>(a, pvec, s);
 }
 
 template <typename T>
@@ -374,7 +391,7 @@ norm_grad_row_kernel(NormGradArgs a, bool pvec) {
     extern __shared__ float sums[];  // 2 x d: the block's sums, joined at the end (kShared: all along)
     const int lane = threadIdx.x & 31, sub = threadIdx.x % TPR, group = threadIdx.x / TPR;
     const int first = (sub >> 5) * VPT * 32 + lane;
-    const float fd = static_cast<float>(a.d);
+    const float inv_d = __frcp_rn(static_cast<float>(a.d));
     float gam[VPT][VE], pg[VPT][VE], pb[VPT][VE];
     Raw<T, VE> rx[VPT], rg[VPT];
     float mu_next = 0.0f, rs_next = 0.0f;
@@ -407,10 +424,11 @@ norm_grad_row_kernel(NormGradArgs a, bool pvec) {
     }
     const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
     int buf = 0;
-    fetch(static_cast<int64_t>(blockIdx.x) * kRows + group);
+    if (!kShared) fetch(static_cast<int64_t>(blockIdx.x) * kRows + group);
     for (int64_t base = static_cast<int64_t>(blockIdx.x) * kRows; base < a.rows; base += step, buf ^= 1) {
         const int64_t r = base + group;
         const bool live = r < a.rows;
+        if (kShared) fetch(r);
         const float mu = mu_next, rs = rs_next;
         float xh[VPT][VE], g[VPT][VE];
         float s1 = 0.0f, s2 = 0.0f;
@@ -444,9 +462,9 @@ norm_grad_row_kernel(NormGradArgs a, bool pvec) {
 #pragma unroll
             for (int i = 0; i < VE; ++i) g[j][i] *= w[i];
         }
-        fetch(r + step);
+        if (!kShared) fetch(r + step);
         const float2 t = row_sum2<TPR>(s1, s2, red, buf);
-        const float m1 = __fdiv_rn(t.x, fd), m2 = __fdiv_rn(t.y, fd);
+        const float m1 = t.x * inv_d, m2 = t.y * inv_d;
         T* dx = static_cast<T*>(a.dx) + r * a.lddx + first * VE;
         auto put = [&](int j) {
             float o[VE];
@@ -504,6 +522,9 @@ cudaError_t norm_grad_row(const NormGradArgs& a, bool pvec, cudaStream_t s) {
 // Eight elements a thread up to 1,024 columns (four blocks an SM), sixteen above (two; one over 4,096).
 template <typename T, int VE>
 cudaError_t norm_grad_width(const NormGradArgs& a, bool pvec, cudaStream_t s) {
+    if constexpr (VE == 4) {
+        if (a.d <= 128) return norm_grad_row<T, VE, 1, 32>(a, pvec, s);
+    }
     if (a.d <= 256) return norm_grad_row<T, VE, 8 / VE, 32>(a, pvec, s);
     if (a.d <= 512) return norm_grad_row<T, VE, 8 / VE, 64>(a, pvec, s);
     if (a.d <= 1024) return norm_grad_row<T, VE, 8 / VE, 128>(a, pvec, s);

@@ -430,6 +430,10 @@ __device__ __forceinline__ void cp_async4(void* dst, const void* src, bool valid
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(valid ? 4 : 0)
                  : "memory");
 }
+// 16 bytes of which the first `bytes` are copied and the rest are zeros.
+__device__ __forceinline__ void cp_async16(void* dst, const void* src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
+}
 // This thread's arrival on `bar` (one of its expected count) once its cp.asyncs so far are complete.
 __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");

@@ -8,7 +8,9 @@
 //
 // All statistics and sums are fp32; the variance is the mean of the centred squares (a
 // second sweep), not E[x^2] - mu^2, which cancels when |mu| is large against the spread.
-// Outputs are rounded once.
+// That sweep also sums the centred values themselves: their mean is the rounding error of mu,
+// and taking it out leaves y within two or three roundings of the formula (it decides how many
+// FP8 codes fall on the other side of a rounding boundary).  Outputs are rounded once.
 #include "block_ops.h"
 #include "nfx_internal.h"
 #include "numerics.cuh"
@@ -184,28 +186,34 @@ __device__ __forceinline__ void load_params(const void* p, int type, bool vec, i
     }
 }
 
-// Sum over the TPR threads of a row, the same bits in each of them.
+// Sums of (a, b) over the TPR threads of a row, the same bits in each of them.
 template <int TPR>
-__device__ __forceinline__ float row_sum(float v, float* red) {
+__device__ __forceinline__ float2 row_sums(float a, float b, float2* red) {
 #pragma unroll
-    for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1) {
+        a += __shfl_xor_sync(0xFFFFFFFFu, a, o);
+        b += __shfl_xor_sync(0xFFFFFFFFu, b, o);
+    }
+    float2 t = make_float2(a, b);
     if constexpr (TPR > 32) {
         const int w = threadIdx.x >> 5, w0 = w / (TPR / 32) * (TPR / 32);  // the row's first warp
-        __syncthreads();  // the previous sum has been read
-        if ((threadIdx.x & 31) == 0) red[w] = v;
+        if ((threadIdx.x & 31) == 0) red[w] = t;
         __syncthreads();
-        v = red[w0];
+        t = red[w0];
 #pragma unroll
-        for (int k = 1; k < TPR / 32; ++k) v += red[w0 + k];
+        for (int k = 1; k < TPR / 32; ++k) {
+            const float2 u = red[w0 + k];
+            t.x += u.x, t.y += u.y;
+        }
     }
-    return v;
+    return t;
 }
 
 constexpr int row_block(int tpr) { return tpr > 128 ? tpr : 128; }
 
 template <typename T, int VE, int VPT, int TPR, bool FP8>
 __global__ void __launch_bounds__(row_block(TPR)) norm_row_kernel(NormArgs a, bool pvec, bool wide) {
-    __shared__ float red[row_block(TPR) / 32];
+    __shared__ float2 red[2][row_block(TPR) / 32];
     constexpr int kRows = row_block(TPR) / TPR;
     const int lane = threadIdx.x & 31, sub = threadIdx.x % TPR;
     const int64_t r = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / TPR;
@@ -234,19 +242,24 @@ __global__ void __launch_bounds__(row_block(TPR)) norm_row_kernel(NormArgs a, bo
 #pragma unroll
         for (int i = 0; i < VE; ++i) s += v[j][i];
     const float inv_d = __frcp_rn(fd);
-    const float mu = mean_of(row_sum<TPR>(s, red), fd, inv_d);
+    const float mu0 = mean_of(row_sums<TPR>(s, 0.0f, red[0]).x, fd, inv_d);
     s = 0.0f;
+    float s1 = 0.0f;
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
         if (full || (first + j * 32) * VE < a.d) {
 #pragma unroll
             for (int i = 0; i < VE; ++i) {
-                v[j][i] -= mu;
+                v[j][i] -= mu0;
+                s1 += v[j][i];
                 s = fmaf(v[j][i], v[j][i], s);
             }
         }
     }
-    const float rs = __frsqrt_rn(fmaf(row_sum<TPR>(s, red), inv_d, a.eps));
+    // the centred values' own mean is what the first sum's rounding left over
+    const float2 t = row_sums<TPR>(s1, s, red[1]);
+    const float rest = t.x * inv_d, mu = mu0 + rest;
+    const float rs = __frsqrt_rn(fmaf(-rest, rest, t.y * inv_d) + a.eps);
     if (live && sub == 0) {
         if (a.mean) a.mean[r] = mu;
         if (a.rstd) a.rstd[r] = rs;
@@ -257,7 +270,7 @@ __global__ void __launch_bounds__(row_block(TPR)) norm_row_kernel(NormArgs a, bo
         load_params<T, VE>(a.gamma, a.ptype, pvec, c, 1.0f, g);
         load_params<T, VE>(a.beta, a.ptype, pvec, c, 0.0f, b);
 #pragma unroll
-        for (int i = 0; i < VE; ++i) v[j][i] = fmaf(v[j][i] * rs, g[i], b[i]);
+        for (int i = 0; i < VE; ++i) v[j][i] = fmaf((v[j][i] - rest) * rs, g[i], b[i]);
         if constexpr (!FP8) {
             if (live) store_pack<T, VE>(static_cast<T*>(a.y) + r * a.ldy + c, v[j]);
         }

@@ -13,8 +13,8 @@
 // warp-specialised: a TMA producer, an MMA issuer, a scale producer, and the promoting warps.
 //
 // Measured (one B200; HBM 6,457 GB/s, FP8 taken as twice the measured bf16 rate, 3,276 TFLOP/s):
-//   8192x16384x4096 to bf16   524 us, 2,100 TFLOP/s, at the 1,000 W power cap (1.5 GHz); 573 us with
-//                             bias and GELU.  A block of K takes 824 cycles where its MMAs take 512:
+//   8192x16384x4096 to bf16   507 us, 2,170 TFLOP/s, at the 1,000 W power cap (1.5 GHz); 553 us with
+//                             bias and GELU.  A block of K takes 745 cycles where its MMAs take 512:
 //                             without the sums 670, without TMEM reads too 650 (barrier hand-over)
 //   4096x4096x8192 to fp32    about 195 us with column scales (a second multiply per element)
 //   1x4096x4096               6.4 us, of which 4.9 are the start and the join (1x1024x1024 takes that)
@@ -221,7 +221,7 @@ constexpr int kPairEpi = 16;
 template <int COL>
 struct PairCfg {
     static constexpr int kStages = 4;
-    // columns of one TMEM read: 8192 x 16384 x 4096 takes 525 us with 32 and 583 with 16 where the
+    // columns of one TMEM read: 8192 x 16384 x 4096 took 525 us with 32 and 583 with 16 where the
     // columns share a scale, 798 and 713 where the column scales take registers too
     static constexpr int kRead = COL ? 16 : 32;
     static constexpr int kStageBytes = 2 * 128 * kBK;
@@ -230,7 +230,7 @@ struct PairCfg {
     static constexpr int kOffOut = kStages * kStageBytes;
     static constexpr int kOffScale = kOffOut + kPairEpi * kOutBytes;
     static constexpr int kOffBars = kOffScale + kScaleStages * kScaleBytes;
-    static constexpr int kSmemBytes = kOffBars + 8 * (2 * kStages + 2 * 4 + 2 * kScaleStages) + 16 + 1024;
+    static constexpr int kSmemBytes = kOffBars + 8 * (2 * kStages + 2 * 4 + 2 * kScaleStages) + 16 + 64 + 1024;
     static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
 };
 
@@ -250,7 +250,7 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
     uint32_t* sTmem = reinterpret_cast<uint32_t*>(sEmpty + C::kScaleStages);
     volatile int* sAbort = reinterpret_cast<volatile int*>(sTmem + 1);
 
-    const int warp = threadIdx.x >> 5;
+    const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0);  // (known to be the same in all lanes)
     const int lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank();
     const int tm = (p.M + 255) / 256, tn = (p.N + 255) / 256;
@@ -296,7 +296,7 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
                     tile_at(t, tm, tn, mt, nt);
                     for (int kb = 0; kb < KB; ++kb, ++it) {
                         const int s = it % C::kStages;
-                        if (!mbar_wait_backoff(&empty[s], ((it / C::kStages) & 1) ^ 1, sAbort, 128, 32, budget)) {
+                        if (!mbar_wait(&empty[s], ((it / C::kStages) & 1) ^ 1, sAbort, budget)) {
                             *sAbort = 1;
                             atomicOr(p.err, kErrWaitSlotFree);
                             ok = false;
@@ -407,43 +407,53 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
         // ---------------- promotion and epilogue
         reg_inc<112>();
         constexpr int W = C::kRead;
-        const int quad = warp & 3, part = warp >> 2, half = part >> 1;
-        const uint32_t accEmpty0 = map_rank(smem_u32(accEmpty), 0);
+        // registers are short in the loop over the blocks (64 accumulators and the columns on their way from
+        // TMEM leave about sixteen): the tile's number waits in shared memory, its place is found when
+        // it is needed, and the addresses are one number each
+        volatile int* my_tile = reinterpret_cast<volatile int*>(sTmem + 4 + warp);
+        const uint32_t accEmpty0 = map_rank(smem_u32(accEmpty), 0) + (warp >> 3) * 8;
+        const uint32_t tmem0 =
+            tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16) + (warp >> 3) * 128 + ((warp >> 2) & 1) * 64;
+        const int row = (warp & 3) * 32 + lane;
         int it = 0;
         bool ok = true;
-        for (int t = first; ok && t < tiles; t += step) {
+        if (lane == 0) *my_tile = first;
+        __syncwarp();
+        while (ok && *my_tile < tiles) {
             float2 acc[32];
 #pragma unroll
             for (int j = 0; j < 32; ++j) acc[j] = make_float2(0.0f, 0.0f);
-            for (int kb = 0; kb < KB; ++kb, ++it) {
-                const int a = (it & 1) * 2 + half, ss = it % C::kScaleStages;
+            for (int left = KB; left > 0; --left, ++it) {
+                const int par = it & 1, ss = it % C::kScaleStages;
                 const float* sc = reinterpret_cast<const float*>(smem + C::kOffScale + ss * C::kScaleBytes);
                 if (!mbar_wait(&sFull[ss], (it / C::kScaleStages) & 1, sAbort, budget) ||
-                    !mbar_wait(&accFull[a], (it >> 1) & 1, sAbort, budget)) {
+                    !mbar_wait(&accFull[par * 2 + (warp >> 3)], (it >> 1) & 1, sAbort, budget)) {
                     *sAbort = 1;
                     atomicOr(p.err, kErrWaitAccFull);
                     ok = false;
                     break;
                 }
                 tc_fence_after();
-                float s = sc[quad * 32 + lane];
-                if constexpr (COL == 0) s *= sc[128 + half];
-                const uint32_t tb =
-                    tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + a * 128 + (part & 1) * 64;
+                float s = sc[row];
+                if constexpr (COL == 0) {
+                    s *= sc[128 + (warp >> 3)];
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sEmpty[ss]);
+                }
 #pragma unroll
                 for (int c = 0; c < 64 / W; ++c) {
                     uint32_t r[W];
-                    tmem_read(tb + c * W, r);
+                    tmem_read(tmem0 + par * 256 + c * W, r);
                     if (c == 64 / W - 1) {
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive_cluster(accEmpty0 + a * 8);
+                        if (lane == 0) mbar_arrive_cluster(accEmpty0 + par * 16);
                     }
 #pragma unroll
                     for (int j = 0; j < W / 4; ++j) {
                         float2 f0 = make_float2(s, s), f1 = f0;
                         if constexpr (COL == 1) {
-                            const float4 cs = *reinterpret_cast<const float4*>(sc + 128 + part * 64 + c * W + 4 * j);
+                            const float4 cs = *reinterpret_cast<const float4*>(sc + 128 + (warp >> 2) * 64 + c * W + 4 * j);
                             f0 = mul2_rn(f0, make_float2(cs.x, cs.y));
                             f1 = mul2_rn(f1, make_float2(cs.z, cs.w));
                         }
@@ -453,15 +463,19 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
                         a1 = fma2_rn(make_float2(__uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3])), f1, a1);
                     }
                 }
-                __syncwarp();  // every lane has read the block's scales
-                if (lane == 0) mbar_arrive(&sEmpty[ss]);
+                if constexpr (COL == 1) {
+                    __syncwarp();  // every lane has read the block's scales
+                    if (lane == 0) mbar_arrive(&sEmpty[ss]);
+                }
             }
             if (!ok) break;
-            // (the tile's place is found only now: registers are short in the loop above)
             int mt, nt;
+            const int t = *my_tile;
             tile_at(t, tm, tn, mt, nt);
-            epilogue<CT, 32>(acc, p, &tmC, smem + C::kOffOut + warp * kOutBytes, mt * 256 + rank * 128 + quad * 32,
-                             nt * 256 + part * 64, lane);
+            epilogue<CT, 32>(acc, p, &tmC, smem + C::kOffOut + warp * kOutBytes, mt * 256 + rank * 128 + (warp & 3) * 32,
+                             nt * 256 + (warp >> 2) * 64, lane);
+            if (lane == 0) *my_tile = t + step;
+            __syncwarp();
         }
         if (lane == 0) tma_store_wait_all<0>();
         __syncwarp();
@@ -556,7 +570,7 @@ fp8_gemm_narrow_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_con
     uint32_t* sTmem = reinterpret_cast<uint32_t*>(sEmpty + C::kScaleStages);
     volatile int* sAbort = reinterpret_cast<volatile int*>(sTmem + 1);
 
-    const int warp = threadIdx.x >> 5;
+    const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0);  // (known to be the same in all lanes)
     const int lane = threadIdx.x & 31;
     const int rank = blockIdx.x % split, tile = blockIdx.x / split;  // a cluster is `split` blocks in a row
     const int tx = (p.M + NT - 1) / NT;

@@ -195,8 +195,8 @@ __global__ void __launch_bounds__(kTileThreads, 2) quant_tile_kernel(QuantArgs a
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const float inv = a.tile ? tinv : rinv[rr * 8 + i];
-            const uint32_t w0 = e4m3_encode4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
-            const uint32_t w1 = e4m3_encode4(v[i][4] * inv, v[i][5] * inv, v[i][6] * inv, v[i][7] * inv);
+            const uint32_t w0 = scaled_codes(v[i][0], v[i][1], v[i][2], v[i][3], inv);
+            const uint32_t w1 = scaled_codes(v[i][4], v[i][5], v[i][6], v[i][7], inv);
             if (inside) {
                 *reinterpret_cast<uint2*>(row + i * a.q.ld) = make_uint2(w0, w1);
             } else if (r0 + i < a.rows) {
@@ -210,8 +210,8 @@ __global__ void __launch_bounds__(kTileThreads, 2) quant_tile_kernel(QuantArgs a
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             const float inv = a.tile ? tinv : cinv[cc * 8 + k];
-            const uint32_t w0 = e4m3_encode4(v[0][k] * inv, v[1][k] * inv, v[2][k] * inv, v[3][k] * inv);
-            const uint32_t w1 = e4m3_encode4(v[4][k] * inv, v[5][k] * inv, v[6][k] * inv, v[7][k] * inv);
+            const uint32_t w0 = scaled_codes(v[0][k], v[1][k], v[2][k], v[3][k], inv);
+            const uint32_t w1 = scaled_codes(v[4][k], v[5][k], v[6][k], v[7][k], inv);
             *reinterpret_cast<uint2*>(tileT + (cc * 8 + k) * kGroup + (rr ^ cc) * 8) = make_uint2(w0, w1);
         }
         __syncthreads();

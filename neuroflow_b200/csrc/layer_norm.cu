@@ -225,6 +225,8 @@ __global__ void __launch_bounds__(row_block(TPR)) norm_row_kernel(NormArgs a, bo
     // (the warps whose packs all lie inside the row need no test per pack)
     const bool full = live && TPR >= 32 && (first - lane + VPT * 32) * VE <= a.d;
     float v[VPT][VE], s = 0.0f;
+    constexpr int N = VPT * VE;
+    float* f = &v[0][0];  // the same numbers as one array (indices are constants after unrolling)
     if (full) {
 #pragma unroll
         for (int j = 0; j < VPT; ++j) load_pack<T, VE>(x + (first + j * 32) * VE, v[j]);
@@ -237,29 +239,44 @@ __global__ void __launch_bounds__(row_block(TPR)) norm_row_kernel(NormArgs a, bo
             if (live && c < a.d) load_pack<T, VE>(x + c, v[j]);
         }
     }
+    // two elements to an instruction (f32x2): with 16-bit rows, instructions and not bytes are the bound
+    float2 p2 = make_float2(f[0], f[1]);
 #pragma unroll
-    for (int j = 0; j < VPT; ++j)
-#pragma unroll
-        for (int i = 0; i < VE; ++i) s += v[j][i];
+    for (int k = 2; k < N; k += 2) p2 = add2_rn(p2, make_float2(f[k], f[k + 1]));
+    s = p2.x + p2.y;
     const float inv_d = __frcp_rn(fd);
     const float mu0 = mean_of(row_sums<TPR>(s, 0.0f, red[0]).x, fd, inv_d);
-    s = 0.0f;
     float s1 = 0.0f;
+    s = 0.0f;
+    if (full) {
+        const float2 m2 = make_float2(-mu0, -mu0);
+        float2 q1 = make_float2(0.0f, 0.0f), q2 = q1;
 #pragma unroll
-    for (int j = 0; j < VPT; ++j) {
-        if (full || (first + j * 32) * VE < a.d) {
+        for (int k = 0; k < N; k += 2) {
+            const float2 c = add2_rn(make_float2(f[k], f[k + 1]), m2);
+            f[k] = c.x, f[k + 1] = c.y;
+            q1 = add2_rn(q1, c);
+            q2 = fma2_rn(c, c, q2);
+        }
+        s1 = q1.x + q1.y;
+        s = q2.x + q2.y;
+    } else {
 #pragma unroll
-            for (int i = 0; i < VE; ++i) {
-                v[j][i] -= mu0;
-                s1 += v[j][i];
-                s = fmaf(v[j][i], v[j][i], s);
+        for (int j = 0; j < VPT; ++j) {
+            if ((first + j * 32) * VE < a.d) {
+#pragma unroll
+                for (int i = 0; i < VE; ++i) {
+                    v[j][i] -= mu0;
+                    s1 += v[j][i];
+                    s = fmaf(v[j][i], v[j][i], s);
+                }
             }
         }
     }
     // the centred values' own mean is what the first sum's rounding left over
     const float2 t = row_sums<TPR>(s1, s, red[1]);
     const float rest = t.x * inv_d, mu = mu0 + rest;
-    const float rs = __frsqrt_rn(fmaf(-rest, rest, t.y * inv_d) + a.eps);
+    const float rs = __frsqrt_rn(fmaf(-rest, rest, t.y * inv_d) + a.eps), off = -rest * rs;
     if (live && sub == 0) {
         if (a.mean) a.mean[r] = mu;
         if (a.rstd) a.rstd[r] = rs;
@@ -269,8 +286,16 @@ __global__ void __launch_bounds__(row_block(TPR)) norm_row_kernel(NormArgs a, bo
         float g[VE], b[VE];
         load_params<T, VE>(a.gamma, a.ptype, pvec, c, 1.0f, g);
         load_params<T, VE>(a.beta, a.ptype, pvec, c, 0.0f, b);
+        if constexpr (VE == 1) {
+            v[j][0] = fmaf(fmaf(v[j][0], rs, off), g[0], b[0]);
+        } else {
 #pragma unroll
-        for (int i = 0; i < VE; ++i) v[j][i] = fmaf((v[j][i] - rest) * rs, g[i], b[i]);
+            for (int i = 0; i < VE; i += 2) {
+                const float2 xh = fma2_rn(make_float2(v[j][i], v[j][i + 1]), make_float2(rs, rs), make_float2(off, off));
+                const float2 y = fma2_rn(xh, make_float2(g[i], g[i + 1]), make_float2(b[i], b[i + 1]));
+                v[j][i] = y.x, v[j][i + 1] = y.y;
+            }
+        }
         if constexpr (!FP8) {
             if (live) store_pack<T, VE>(static_cast<T*>(a.y) + r * a.ldy + c, v[j]);
         }

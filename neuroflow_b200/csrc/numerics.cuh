@@ -91,6 +91,14 @@ __device__ __forceinline__ float2 fma2_rn(float2 a, float2 b, float2 c) {
     return r;
 }
 
+__device__ __forceinline__ float2 add2_rn(float2 a, float2 b) {
+    float2 r;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+        "add.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+
 // fake-quant round trip: (q - zp) * s.
 __device__ __forceinline__ float fake_quant(float v, float s, float zp) {
     return __fmul_rn(__fsub_rn(fq_code(v, s, zp), zp), s);

@@ -2,6 +2,8 @@
 // elements), and their FP8 form: shared by the layer norm and the quantiser.
 #pragma once
 
+#include <type_traits>
+
 #include "block_ops.h"
 #include "numerics.cuh"
 
@@ -13,15 +15,20 @@ template <typename T, int VE>
 struct Pack {
     T v[VE];
 };
+// the VE numbers of 16 bytes
+template <typename T, int VE>
+__device__ __forceinline__ void unpack(uint4 u, float (&o)[VE]) {
+    const Pack<T, VE> k = *reinterpret_cast<const Pack<T, VE>*>(&u);
+#pragma unroll
+    for (int i = 0; i < VE; ++i) o[i] = to_f32(k.v[i]);
+}
 template <typename T, int VE>
 __device__ __forceinline__ void load_pack(const T* p, float (&o)[VE]) {
     if constexpr (VE == 1) {
         o[0] = to_f32(__ldg(p));
     } else {
         const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
-        const Pack<T, VE> k = *reinterpret_cast<const Pack<T, VE>*>(&u);
-#pragma unroll
-        for (int i = 0; i < VE; ++i) o[i] = to_f32(k.v[i]);
+        unpack<T, VE>(u, o);
     }
 }
 template <typename T, int VE>
@@ -29,12 +36,28 @@ __device__ __forceinline__ void store_pack(T* p, const float (&o)[VE]) {
     if constexpr (VE == 1) {
         *p = from_f32<T>(o[0]);
     } else {
-        Pack<T, VE> k;
+        uint32_t w[4];
 #pragma unroll
-        for (int i = 0; i < VE; ++i) k.v[i] = from_f32<T>(o[i]);
-        *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(&k);
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (VE == 4) {
+                w[i] = __float_as_uint(o[i]);
+            } else if constexpr (sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value) {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(o[2 * i], o[2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t*>(&h);
+            } else {
+                const __half2 h = __floats2half2_rn(o[2 * i], o[2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+        }
+        *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
     }
 }
+// The codes of four values times `inv` (two products to an instruction, each rounded by itself).
+__device__ __forceinline__ uint32_t scaled_codes(float a, float b, float c, float d, float inv) {
+    const float2 p = mul2_rn(make_float2(a, b), make_float2(inv, inv)), q = mul2_rn(make_float2(c, d), make_float2(inv, inv));
+    return e4m3_encode4(p.x, p.y, q.x, q.y);
+}
+
 // FP8 codes of a lane's VPT packs (values v, zero beyond column d): pack j holds columns (first_pack +
 // 32 j) VE .., so a group of 128 lies in one warp.  A group's maximum is taken over all its elements
 // first and again over the finite ones where it is infinite (a NaN is no maximum anyway).  The
@@ -82,7 +105,7 @@ __device__ __forceinline__ void store_codes(const float (&v)[VPT][VE], const Fp8
         const int64_t c0 = (first_pack + j * kPer * 32) * VE;  // this lane's first column
         uint8_t* dst = q.codes + r * q.ld + c0;
         if constexpr (VE == 1) {
-            const uint32_t w = e4m3_encode4(v[4 * j][0] * inv, v[4 * j + 1][0] * inv, v[4 * j + 2][0] * inv, v[4 * j + 3][0] * inv);
+            const uint32_t w = scaled_codes(v[4 * j][0], v[4 * j + 1][0], v[4 * j + 2][0], v[4 * j + 3][0], inv);
             if (live && c0 - lane + kGroup <= d) {
 #pragma unroll
                 for (int h = 0; h < 4; ++h) dst[h * 32] = static_cast<uint8_t>(w >> (8 * h));
@@ -95,7 +118,7 @@ __device__ __forceinline__ void store_codes(const float (&v)[VPT][VE], const Fp8
             uint32_t w[VE / 4];
 #pragma unroll
             for (int i = 0; i < VE / 4; ++i)
-                w[i] = e4m3_encode4(v[j][4 * i] * inv, v[j][4 * i + 1] * inv, v[j][4 * i + 2] * inv, v[j][4 * i + 3] * inv);
+                w[i] = scaled_codes(v[j][4 * i], v[j][4 * i + 1], v[j][4 * i + 2], v[j][4 * i + 3], inv);
             if (!live || c0 >= d) continue;
             if (wide) {
                 if constexpr (VE == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);

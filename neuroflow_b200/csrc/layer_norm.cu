@@ -11,6 +11,8 @@
 // That sweep also sums the centred values themselves: their mean is the rounding error of mu,
 // and taking it out leaves y within two or three roundings of the formula (it decides how many
 // FP8 codes fall on the other side of a rounding boundary).  Outputs are rounded once.
+#include <atomic>
+
 #include "block_ops.h"
 #include "nfx_internal.h"
 #include "numerics.cuh"
@@ -209,120 +211,165 @@ __device__ __forceinline__ float2 row_sums(float a, float b, float2* red) {
     return t;
 }
 
+// A pack as it was read.
+template <typename T, int VE>
+struct Raw {
+    uint4 u;
+    __device__ __forceinline__ void load(const T* p) { u = __ldg(reinterpret_cast<const uint4*>(p)); }
+    __device__ __forceinline__ void get(float (&o)[VE]) const {
+        unpack<T, VE>(u, o);
+    }
+    __device__ __forceinline__ void zero() { u = make_uint4(0, 0, 0, 0); }
+};
+template <typename T>
+struct Raw<T, 1> {
+    T u;
+    __device__ __forceinline__ void load(const T* p) { u = *p; }
+    __device__ __forceinline__ void get(float (&o)[1]) const { o[0] = to_f32(u); }
+    __device__ __forceinline__ void zero() { u = from_f32<T>(0.0f); }
+};
+
 constexpr int row_block(int tpr) { return tpr > 128 ? tpr : 128; }
+// Rows of one or two packs a thread are too short to cover their own latency: resident blocks walk over
+// them and fetch a row ahead (131072x128 fp32: 27.0 us, 30.6 with a block for each four rows).  Longer rows
+// are faster with a block each (16384x4096 bf16 to FP8: 65 us, 72 walking).
+constexpr bool walks(int vpt, int tpr) { return tpr <= 32 && vpt <= 2; }
 
 template <typename T, int VE, int VPT, int TPR, bool FP8>
-__global__ void __launch_bounds__(row_block(TPR)) norm_row_kernel(NormArgs a, bool pvec, bool wide) {
+__global__ void __launch_bounds__(row_block(TPR), TPR >= 512 ? 2 : 1) norm_row_kernel(NormArgs a, bool pvec, bool wide) {
     __shared__ float2 red[2][row_block(TPR) / 32];
-    constexpr int kRows = row_block(TPR) / TPR;
+    constexpr int kRows = row_block(TPR) / TPR, N = VPT * VE;
+    constexpr bool kWalk = walks(VPT, TPR);
     const int lane = threadIdx.x & 31, sub = threadIdx.x % TPR;
-    const int64_t r = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / TPR;
-    const bool live = r < a.rows;
     // pack j of this thread is first + j * 32 (a row of fewer than 32 threads has one pack a thread)
     const int first = TPR < 32 ? sub : (sub >> 5) * VPT * 32 + lane;
-    const T* x = static_cast<const T*>(a.x) + r * a.ldx;
-    const float fd = static_cast<float>(a.d);
+    const float fd = static_cast<float>(a.d), inv_d = __frcp_rn(fd);
     // (the warps whose packs all lie inside the row need no test per pack)
-    const bool full = live && TPR >= 32 && (first - lane + VPT * 32) * VE <= a.d;
-    float v[VPT][VE], s = 0.0f;
-    constexpr int N = VPT * VE;
-    float* f = &v[0][0];  // the same numbers as one array (indices are constants after unrolling)
-    if (full) {
+    const bool full = TPR >= 32 && (first - lane + VPT * 32) * VE <= a.d;
+    Raw<T, VE> rx[VPT];
+    auto fetch = [&](int64_t r) {
+        const T* x = static_cast<const T*>(a.x) + r * a.ldx + first * VE;
+        if (full && r < a.rows) {
 #pragma unroll
-        for (int j = 0; j < VPT; ++j) load_pack<T, VE>(x + (first + j * 32) * VE, v[j]);
-    } else {
+            for (int j = 0; j < VPT; ++j) rx[j].load(x + j * 32 * VE);
+        } else {
 #pragma unroll
-        for (int j = 0; j < VPT; ++j) {
-            const int c = (first + j * 32) * VE;
-#pragma unroll
-            for (int i = 0; i < VE; ++i) v[j][i] = 0.0f;
-            if (live && c < a.d) load_pack<T, VE>(x + c, v[j]);
+            for (int j = 0; j < VPT; ++j) {
+                if (r < a.rows && (first + j * 32) * VE < a.d) rx[j].load(x + j * 32 * VE);
+                else rx[j].zero();
+            }
         }
-    }
-    // two elements to an instruction (f32x2): with 16-bit rows, instructions and not bytes are the bound
-    float2 p2 = make_float2(f[0], f[1]);
+    };
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
+    fetch(static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / TPR);
+    for (int64_t base = static_cast<int64_t>(blockIdx.x) * kRows; base < a.rows; base += step) {
+        const int64_t r = base + threadIdx.x / TPR;
+        const bool live = r < a.rows;
+        float v[VPT][VE], s;
+        float* f = &v[0][0];  // the same numbers as one array (indices are constants after unrolling)
 #pragma unroll
-    for (int k = 2; k < N; k += 2) p2 = add2_rn(p2, make_float2(f[k], f[k + 1]));
-    s = p2.x + p2.y;
-    const float inv_d = __frcp_rn(fd);
-    const float mu0 = mean_of(row_sums<TPR>(s, 0.0f, red[0]).x, fd, inv_d);
-    float s1 = 0.0f;
-    s = 0.0f;
-    if (full) {
-        const float2 m2 = make_float2(-mu0, -mu0);
-        float2 q1 = make_float2(0.0f, 0.0f), q2 = q1;
+        for (int j = 0; j < VPT; ++j) rx[j].get(v[j]);
+        if constexpr (kWalk) fetch(r + step);  // the next row comes while this one is worked on
+        // two elements to an instruction (f32x2): with 16-bit rows, instructions and not bytes are the bound
+        float2 p2 = make_float2(f[0], f[1]);
 #pragma unroll
-        for (int k = 0; k < N; k += 2) {
-            const float2 c = add2_rn(make_float2(f[k], f[k + 1]), m2);
-            f[k] = c.x, f[k + 1] = c.y;
-            q1 = add2_rn(q1, c);
-            q2 = fma2_rn(c, c, q2);
-        }
-        s1 = q1.x + q1.y;
-        s = q2.x + q2.y;
-    } else {
+        for (int k = 2; k < N; k += 2) p2 = add2_rn(p2, make_float2(f[k], f[k + 1]));
+        s = p2.x + p2.y;
+        const float mu0 = mean_of(row_sums<TPR>(s, 0.0f, red[0]).x, fd, inv_d);
+        float s1 = 0.0f;
+        s = 0.0f;
+        if (full) {
+            const float2 m2 = make_float2(-mu0, -mu0);
+            float2 q1 = make_float2(0.0f, 0.0f), q2 = q1;
 #pragma unroll
-        for (int j = 0; j < VPT; ++j) {
-            if ((first + j * 32) * VE < a.d) {
+            for (int k = 0; k < N; k += 2) {
+                const float2 c = add2_rn(make_float2(f[k], f[k + 1]), m2);
+                f[k] = c.x, f[k + 1] = c.y;
+                q1 = add2_rn(q1, c);
+                q2 = fma2_rn(c, c, q2);
+            }
+            s1 = q1.x + q1.y;
+            s = q2.x + q2.y;
+        } else {
 #pragma unroll
-                for (int i = 0; i < VE; ++i) {
-                    v[j][i] -= mu0;
-                    s1 += v[j][i];
-                    s = fmaf(v[j][i], v[j][i], s);
+            for (int j = 0; j < VPT; ++j) {
+                if ((first + j * 32) * VE < a.d) {
+#pragma unroll
+                    for (int i = 0; i < VE; ++i) {
+                        v[j][i] -= mu0;
+                        s1 += v[j][i];
+                        s = fmaf(v[j][i], v[j][i], s);
+                    }
                 }
             }
         }
-    }
-    // the centred values' own mean is what the first sum's rounding left over
-    const float2 t = row_sums<TPR>(s1, s, red[1]);
-    const float rest = t.x * inv_d, mu = mu0 + rest;
-    const float rs = __frsqrt_rn(fmaf(-rest, rest, t.y * inv_d) + a.eps), off = -rest * rs;
-    if (live && sub == 0) {
-        if (a.mean) a.mean[r] = mu;
-        if (a.rstd) a.rstd[r] = rs;
-    }
-    auto finish = [&](int j) {
-        const int c = (first + j * 32) * VE;
-        float g[VE], b[VE];
-        load_params<T, VE>(a.gamma, a.ptype, pvec, c, 1.0f, g);
-        load_params<T, VE>(a.beta, a.ptype, pvec, c, 0.0f, b);
-        if constexpr (VE == 1) {
-            v[j][0] = fmaf(fmaf(v[j][0], rs, off), g[0], b[0]);
+        // the centred values' own mean is what the first sum's rounding left over
+        const float2 t = row_sums<TPR>(s1, s, red[1]);
+        const float rest = t.x * inv_d, mu = mu0 + rest;
+        const float rs = __frsqrt_rn(fmaf(-rest, rest, t.y * inv_d) + a.eps), off = -rest * rs;
+        if (live && sub == 0) {
+            if (a.mean) a.mean[r] = mu;
+            if (a.rstd) a.rstd[r] = rs;
+        }
+        auto finish = [&](int j) {
+            const int c = (first + j * 32) * VE;
+            float g[VE], b[VE];
+            load_params<T, VE>(a.gamma, a.ptype, pvec, c, 1.0f, g);
+            load_params<T, VE>(a.beta, a.ptype, pvec, c, 0.0f, b);
+            if constexpr (VE == 1) {
+                v[j][0] = fmaf(fmaf(v[j][0], rs, off), g[0], b[0]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < VE; i += 2) {
+                    const float2 xh = fma2_rn(make_float2(v[j][i], v[j][i + 1]), make_float2(rs, rs), make_float2(off, off));
+                    const float2 y = fma2_rn(xh, make_float2(g[i], g[i + 1]), make_float2(b[i], b[i + 1]));
+                    v[j][i] = y.x, v[j][i + 1] = y.y;
+                }
+            }
+            if constexpr (!FP8) {
+                if (live) store_pack<T, VE>(static_cast<T*>(a.y) + r * a.ldy + c, v[j]);
+            }
+        };
+        if (full) {
+#pragma unroll
+            for (int j = 0; j < VPT; ++j) finish(j);
         } else {
 #pragma unroll
-            for (int i = 0; i < VE; i += 2) {
-                const float2 xh = fma2_rn(make_float2(v[j][i], v[j][i + 1]), make_float2(rs, rs), make_float2(off, off));
-                const float2 y = fma2_rn(xh, make_float2(g[i], g[i + 1]), make_float2(b[i], b[i + 1]));
-                v[j][i] = y.x, v[j][i + 1] = y.y;
-            }
+            for (int j = 0; j < VPT; ++j)
+                if ((first + j * 32) * VE < a.d) finish(j);
         }
-        if constexpr (!FP8) {
-            if (live) store_pack<T, VE>(static_cast<T*>(a.y) + r * a.ldy + c, v[j]);
-        }
-    };
-    if (full) {
-#pragma unroll
-        for (int j = 0; j < VPT; ++j) finish(j);
-    } else {
-#pragma unroll
-        for (int j = 0; j < VPT; ++j)
-            if ((first + j * 32) * VE < a.d) finish(j);
+        if constexpr (FP8) store_codes<VE, VPT, TPR>(v, a.q, r, a.d, live, first, lane, wide);
+        if constexpr (!kWalk) break;
     }
-    if constexpr (FP8) store_codes<VE, VPT, TPR>(v, a.q, r, a.d, live, first, lane, wide);
+}
+
+template <typename T, int VE, int VPT, int TPR, bool FP8>
+cudaError_t norm_row_go(const NormArgs& a, bool pvec, bool wide, cudaStream_t s) {
+    constexpr int kThreads = row_block(TPR), kRows = kThreads / TPR;
+    auto kern = norm_row_kernel<T, VE, VPT, TPR, FP8>;
+    const int64_t want = (a.rows + kRows - 1) / kRows;
+    int64_t grid = want;
+    if constexpr (walks(VPT, TPR)) {
+        static std::atomic<int> known[64];  // asked for once per kernel and device
+        const int d = current_device() & 63;
+        int most = known[d].load(std::memory_order_relaxed);
+        if (most == 0) {
+            if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&most, kern, kThreads, 0) != cudaSuccess || most < 1) most = 1;
+            most *= device_sm_count();
+            known[d].store(most, std::memory_order_relaxed);
+        }
+        grid = want < most ? want : most;
+    }
+    if (grid > 0x7FFFFFFF) return cudaErrorInvalidValue;
+    kern<<<static_cast<unsigned>(grid), kThreads, 0, s>>>(a, pvec, wide);
+    return cudaGetLastError();
 }
 
 template <typename T, int VE, int VPT, int TPR>
 cudaError_t norm_row(const NormArgs& a, bool pvec, cudaStream_t s) {
-    constexpr int kRows = row_block(TPR) / TPR;
-    const int64_t grid = (a.rows + kRows - 1) / kRows;
-    if (grid > 0x7FFFFFFF) return cudaErrorInvalidValue;
-    if (a.y) {
-        norm_row_kernel<T, VE, VPT, TPR, false><<<static_cast<unsigned>(grid), row_block(TPR), 0, s>>>(a, pvec, false);
-    } else {
-        const bool wide = reinterpret_cast<uintptr_t>(a.q.codes) % 8 == 0 && (a.rows == 1 || a.q.ld % 8 == 0);
-        norm_row_kernel<T, VE, VPT, TPR, true><<<static_cast<unsigned>(grid), row_block(TPR), 0, s>>>(a, pvec, wide);
-    }
-    return cudaGetLastError();
+    if (a.y) return norm_row_go<T, VE, VPT, TPR, false>(a, pvec, false, s);
+    const bool wide = reinterpret_cast<uintptr_t>(a.q.codes) % 8 == 0 && (a.rows == 1 || a.q.ld % 8 == 0);
+    return norm_row_go<T, VE, VPT, TPR, true>(a, pvec, wide, s);
 }
 
 // Threads and packs per row by the width: the fewest threads that leave a thread 32 elements at most, and
@@ -375,25 +422,6 @@ cudaError_t norm_t(const NormArgs& a, cudaStream_t s) {
 // leaves 64 registers a thread), written once per block.  The next row's loads are issued before this
 // row's sums are joined.
 // ---------------------------------------------------------------------------
-template <typename T, int VE>
-struct Raw {
-    uint4 u;
-    __device__ __forceinline__ void load(const T* p) { u = __ldg(reinterpret_cast<const uint4*>(p)); }
-    __device__ __forceinline__ void get(float (&o)[VE]) const {
-        const Pack<T, VE> k = *reinterpret_cast<const Pack<T, VE>*>(&u);
-#pragma unroll
-        for (int i = 0; i < VE; ++i) o[i] = to_f32(k.v[i]);
-    }
-    __device__ __forceinline__ void zero() { u = make_uint4(0, 0, 0, 0); }
-};
-template <typename T>
-struct Raw<T, 1> {
-    T u;
-    __device__ __forceinline__ void load(const T* p) { u = *p; }
-    __device__ __forceinline__ void get(float (&o)[1]) const { o[0] = to_f32(u); }
-    __device__ __forceinline__ void zero() { u = from_f32<T>(0.0f); }
-};
-
 // Sums of (a, b) over the TPR threads of a row; `buf` alternates between calls, so that one barrier
 // separates a call's reads from the next but one's writes.
 template <int TPR>

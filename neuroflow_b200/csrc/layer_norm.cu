@@ -17,6 +17,7 @@
 #include "nfx_internal.h"
 #include "numerics.cuh"
 #include "row_pack.cuh"
+#include "sm100.cuh"
 
 namespace nfx {
 namespace {
@@ -128,20 +129,27 @@ __global__ void __launch_bounds__(kAnyThreads) norm_grad_any_kernel(NormGradArgs
     }
 }
 
-// 32 columns per block, 32 threads per column over the partial sums, joined in a fixed order.  Block
-// row y handles the y-th set of partial sums and its output.
-__global__ void __launch_bounds__(1024) column_reduce_kernel(const float* __restrict__ part, int parts, int64_t n,
-                                                             void* out0, void* out1, int otype) {
+// 32 columns per block, 32 threads per column over the partial sums (eight loads in flight), joined in a
+// fixed order.  Block row y handles the y-th set of partial sums and its output.  Launched with
+// programmatic serialization: it waits for the kernel before it by itself.
+__global__ void __launch_bounds__(1024) column_reduce_kernel(const float* part, int parts, int64_t n, void* out0, void* out1,
+                                                             int otype) {
     __shared__ float red[32][33];
     const int c = threadIdx.x & 31, t = threadIdx.x >> 5;
     const int64_t i = static_cast<int64_t>(blockIdx.x) * 32 + c;
     void* out = blockIdx.y ? out1 : out0;
     if (!out) return;
+    grid_dep_wait();
     part += static_cast<int64_t>(blockIdx.y) * parts * n;
     float s = 0.0f;
     if (i < n) {
-#pragma unroll 4
-        for (int p = t; p < parts; p += 32) s += __ldg(part + p * n + i);
+        for (int p = t; p < parts; p += 256) {
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = p + 32 * k < parts ? part[static_cast<int64_t>(p + 32 * k) * n + i] : 0.0f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) s += v[k];
+        }
     }
     red[t][c] = s;
     __syncthreads();
@@ -454,7 +462,10 @@ norm_grad_row_kernel(NormGradArgs a, bool pvec) {
     constexpr int kThreads = grad_block(TPR), kRows = kThreads / TPR;
     constexpr bool kShared = TPR == 1024;
     __shared__ float2 red[2][32];
-    extern __shared__ float sums[];  // 2 x d: the block's sums, joined at the end (kShared: all along)
+    // The block's sums: number e of a row's thread t at e * TPR + t (no bank conflicts), E of dgamma, then E
+    // of dbeta; used at the end to join the row groups, with kShared all along.
+    extern __shared__ float sums[];
+    constexpr int E = VPT * VE;
     const int lane = threadIdx.x & 31, sub = threadIdx.x % TPR, group = threadIdx.x / TPR;
     const int first = (sub >> 5) * VPT * 32 + lane;
     const float inv_d = __frcp_rn(static_cast<float>(a.d));
@@ -484,9 +495,10 @@ norm_grad_row_kernel(NormGradArgs a, bool pvec) {
 #pragma unroll
         for (int i = 0; i < VE; ++i) pg[j][i] = pb[j][i] = gam[j][i] = 0.0f;
         if (!kShared && c < a.d) load_params<T, VE>(a.gamma, a.ptype, pvec, c, 1.0f, gam[j]);
-        if (kShared && a.part && c < a.d)
+        if (kShared && a.part) {
 #pragma unroll
-            for (int i = 0; i < VE; ++i) sums[c + i] = sums[a.d + c + i] = 0.0f;
+            for (int i = 0; i < VE; ++i) sums[(j * VE + i) * TPR + sub] = sums[(E + j * VE + i) * TPR + sub] = 0.0f;
+        }
     }
     const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
     int buf = 0;
@@ -518,11 +530,13 @@ norm_grad_row_kernel(NormGradArgs a, bool pvec) {
                     pb[j][i] += g[j][i];
                 }
             }
-            if (kShared && a.part && c < a.d) {
+            if (kShared && a.part) {
 #pragma unroll
                 for (int i = 0; i < VE; ++i) {
-                    sums[c + i] = fmaf(g[j][i], xh[j][i], sums[c + i]);
-                    sums[a.d + c + i] += g[j][i];
+                    float& sg = sums[(j * VE + i) * TPR + sub];
+                    float& sb = sums[(E + j * VE + i) * TPR + sub];
+                    sg = fmaf(g[j][i], xh[j][i], sg);
+                    sb += g[j][i];
                 }
             }
 #pragma unroll
@@ -548,37 +562,58 @@ norm_grad_row_kernel(NormGradArgs a, bool pvec) {
         }
     }
     if (!a.part) return;
+    grid_dep_launch();  // the kernel that joins the blocks' sums may be placed
     // the block's row groups join their sums, one after the other
     if constexpr (!kShared) {
-        for (int k = 0; k < kRows; ++k) {
-            __syncthreads();
+        for (int k = 1; k < kRows; ++k) {
             if (group == k) {
 #pragma unroll
-                for (int j = 0; j < VPT; ++j) {
-                    const int c = (first + j * 32) * VE;
-                    if (c >= a.d) continue;
-#pragma unroll
-                    for (int i = 0; i < VE; ++i) {
-                        sums[c + i] = k ? sums[c + i] + pg[j][i] : pg[j][i];
-                        sums[a.d + c + i] = k ? sums[a.d + c + i] + pb[j][i] : pb[j][i];
-                    }
+                for (int e = 0; e < E; ++e) {
+                    sums[e * TPR + sub] = pg[e / VE][e % VE];
+                    sums[(E + e) * TPR + sub] = pb[e / VE][e % VE];
                 }
             }
+            __syncthreads();
+            if (group == 0) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    pg[e / VE][e % VE] += sums[e * TPR + sub];
+                    pb[e / VE][e % VE] += sums[(E + e) * TPR + sub];
+                }
+            }
+            __syncthreads();
+        }
+        if (group != 0) return;
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            pg[e / VE][e % VE] = sums[e * TPR + sub];
+            pb[e / VE][e % VE] = sums[(E + e) * TPR + sub];
         }
     }
-    __syncthreads();
     float* out_g = a.part + static_cast<int64_t>(blockIdx.x) * a.d;
     float* out_b = a.part + (static_cast<int64_t>(a.parts) + blockIdx.x) * a.d;
-    for (int i = threadIdx.x; i < a.d; i += kThreads) {
-        out_g[i] = sums[i];
-        out_b[i] = sums[a.d + i];
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+        const int c = (first + j * 32) * VE;
+        if (c >= a.d) continue;
+        if constexpr (VE == 1) {
+            out_g[c] = pg[j][0];
+            out_b[c] = pb[j][0];
+        } else {  // (d is a multiple of VE, the workspace 16-byte aligned)
+#pragma unroll
+            for (int i = 0; i < VE; i += 4) {
+                *reinterpret_cast<float4*>(out_g + c + i) = make_float4(pg[j][i], pg[j][i + 1], pg[j][i + 2], pg[j][i + 3]);
+                *reinterpret_cast<float4*>(out_b + c + i) = make_float4(pb[j][i], pb[j][i + 1], pb[j][i + 2], pb[j][i + 3]);
+            }
+        }
     }
 }
 
 template <typename T, int VE, int VPT, int TPR>
 cudaError_t norm_grad_row(const NormGradArgs& a, bool pvec, cudaStream_t s) {
     auto kern = norm_grad_row_kernel<T, VE, VPT, TPR>;
-    const int smem = a.part ? 2 * a.d * 4 : 0;
+    const int smem = a.part && (TPR == 1024 || grad_block(TPR) > TPR) ? 2 * VPT * VE * TPR * 4 : 0;
     cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), smem);
     if (e != cudaSuccess) return e;
     kern<<<a.parts, grad_block(TPR), smem, s>>>(a, pvec);
@@ -634,9 +669,16 @@ int layer_norm_parts(int64_t rows, int64_t d) {
 
 cudaError_t column_reduce_launch(const float* part, int parts, int64_t n, void* out0, void* out1, int otype,
                                  cudaStream_t s) {
-    const dim3 grid(static_cast<unsigned>((n + 31) / 32), out1 ? 2 : 1);
-    column_reduce_kernel<<<grid, 1024, 0, s>>>(part, parts, n, out0, out1, otype);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>((n + 31) / 32), out1 ? 2 : 1);
+    cfg.blockDim = dim3(1024);
+    cfg.stream = s;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, column_reduce_kernel, part, parts, n, out0, out1, otype);
 }
 
 cudaError_t layer_norm_backward_launch(const NormGradArgs& a, int xtype, cudaStream_t s) {

@@ -4,7 +4,8 @@
 
 Compiles neuroflow_b200/csrc/*.cu and *.cpp with nvcc for sm_100a only
 (-gencode arch=compute_100a,code=sm_100a), objects under _build/, and links
-neuroflow_b200/libnfx.so and the nflow_infer command-line front-end next to it.  The CUDA runtime is linked statically so the library does
+neuroflow_b200/libnfx.so, the nflow_infer command-line front-end and the torch front-end
+_nfx_torch.so of neuroflow_b200.ops next to it.  The CUDA runtime is linked statically so the library does
 not depend on which libcudart the host process (e.g. torch) loaded.
 """
 from __future__ import annotations
@@ -65,7 +66,34 @@ def build(verbose: bool = False) -> str:
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
     _build_cli()
+    _build_torch()
     return LIB
+
+
+TORCH_SRC = os.path.join(PKG, "torch_ext", "nfx_torch.cpp")
+TORCH_EXT = os.path.join(PKG, "_nfx_torch.so")
+
+
+def _build_torch() -> None:
+    """The compiled torch front-end of neuroflow_b200.ops (a Python module next to libnfx.so), with the
+    headers and libraries of the installed torch."""
+    hdr = os.path.join(ROOT, "include", "nfx.h")
+    if os.path.exists(TORCH_EXT) and os.path.getmtime(TORCH_EXT) >= max(os.path.getmtime(TORCH_SRC), os.path.getmtime(hdr)):
+        return
+    import sysconfig
+
+    import torch
+    inc = os.path.join(os.path.dirname(torch.__file__), "include")
+    cuda = os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include")
+    cmd = ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-DTORCH_EXTENSION_NAME=_nfx_torch",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I" + os.path.join(ROOT, "include"),
+           "-isystem", inc, "-isystem", os.path.join(inc, "torch", "csrc", "api", "include"), "-isystem", cuda,
+           "-isystem", sysconfig.get_paths()["include"], TORCH_SRC, "-o", TORCH_EXT, "-L" + PKG, "-lnfx",
+           "-L" + os.path.join(os.path.dirname(torch.__file__), "lib"), "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu",
+           "-ltorch_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"torch front-end build failed:\n{r.stdout}\n{r.stderr}")
 
 
 CLI_SRC = os.path.join(PKG, "cli", "nflow_infer.cpp")

@@ -392,14 +392,14 @@ int nfx_layer_norm_backward(const void* dy, int64_t lddy, const void* x, int64_t
  * nfx_fp8_e4m3_to_bits (infinities give +-448, NaN gives 0x7F).  With codes_t not NULL the
  * codes of the transpose (cols, rows) are written as well, from the same read of x: with tile
  * = 0 its groups run along the rows of x, with tile = 1 it has the same codes.  col_sums
- * (cols,), allowed with tile = 0, receives the sums of x's columns; it needs a 16-byte
- * aligned workspace of nfx_fp8_quantise_workspace bytes. */
+ * (cols,) of sums_type, allowed with tile = 0, receives the sums of x's columns (formed in
+ * fp32); it needs a 16-byte aligned workspace of nfx_fp8_quantise_workspace bytes. */
 int64_t nfx_fp8_quantise_workspace(int64_t rows, int64_t cols);
 int nfx_fp8_quantise(const void* x, int x_type, int64_t ldx, int64_t rows, int64_t cols, int tile,
                      uint8_t* codes, int64_t ld_codes, float* scales, int64_t scale_row_stride,
                      int64_t scale_block_stride, uint8_t* codes_t, int64_t ld_codes_t, float* scales_t,
-                     int64_t scale_t_row_stride, int64_t scale_t_block_stride, float* col_sums, void* workspace,
-                     int64_t workspace_bytes, void* stream);
+                     int64_t scale_t_row_stride, int64_t scale_t_block_stride, void* col_sums, int sums_type,
+                     void* workspace, int64_t workspace_bytes, void* stream);
 
 /* C = act(A B^T + bias) for FP8 E4M3 operands in the quantiser's form, A (M, K) and B (N, K):
  *   C[m, n] = act(sum_b sa[m, b] sb[n, b] sum_{k in block b} A[m, k] B[n, k] + bias[n])

@@ -47,7 +47,7 @@ lib.nfx_fp8_quantise_workspace.restype = _i64
 lib.nfx_fp8_quantise_workspace.argtypes = [_i64, _i64]
 lib.nfx_fp8_quantise.restype = C.c_int
 lib.nfx_fp8_quantise.argtypes = [_vp, C.c_int, _i64, _i64, _i64, C.c_int, _vp, _i64, _vp, _i64, _i64, _vp, _i64,
-                                 _vp, _i64, _i64, _vp, _vp, _i64, _vp]
+                                 _vp, _i64, _i64, _vp, C.c_int, _vp, _i64, _vp]
 lib.nfx_fp8_gemm.restype = C.c_int
 lib.nfx_fp8_gemm.argtypes = [_vp, _i64, _vp, _i64, _i64, C.c_int, _vp, _i64, _vp, _i64, _i64, C.c_int, _i64,
                              _i64, _i64, _vp, C.c_int, C.c_int, _vp, C.c_int, _i64, _vp]

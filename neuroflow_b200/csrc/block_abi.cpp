@@ -144,11 +144,12 @@ int64_t nfx_fp8_quantise_workspace(int64_t rows, int64_t cols) {
 int nfx_fp8_quantise(const void* x, int x_type, int64_t ldx, int64_t rows, int64_t cols, int tile,
                      uint8_t* codes, int64_t ld_codes, float* scales, int64_t scale_row_stride,
                      int64_t scale_block_stride, uint8_t* codes_t, int64_t ld_codes_t, float* scales_t,
-                     int64_t scale_t_row_stride, int64_t scale_t_block_stride, float* col_sums, void* workspace,
-                     int64_t workspace_bytes, void* stream) {
+                     int64_t scale_t_row_stride, int64_t scale_t_block_stride, void* col_sums, int sums_type,
+                     void* workspace, int64_t workspace_bytes, void* stream) {
     const char* fn = "nfx_fp8_quantise";
     return guarded(fn, [&]() -> int {
         if (!type_ok(x_type)) return bad(fn, "x_type must be NFX_F32, NFX_BF16 or NFX_F16");
+        if (!type_ok(sums_type)) return bad(fn, "sums_type must be NFX_F32, NFX_BF16 or NFX_F16");
         if (rows < 0 || cols < 0) return bad(fn, "rows and cols must be >= 0");
         if (rows > kIntMax || cols > kIntMax) return bad(fn, "rows and cols must be below 2^31");
         if (tile != 0 && tile != 1) return bad(fn, "tile must be 0 or 1");
@@ -158,7 +159,8 @@ int nfx_fp8_quantise(const void* x, int x_type, int64_t ldx, int64_t rows, int64
             if (!x || !codes || !scales || (codes_t && !scales_t)) return bad(fn, "null pointer");
             if ((rows > 1 && (ldx < cols || ld_codes < cols)) || (codes_t && cols > 1 && ld_codes_t < rows))
                 return bad(fn, "a row stride is smaller than its row");
-            if (!elements_aligned(x, x_type) || !aligned(scales, 4) || !aligned(scales_t, 4) || !aligned(col_sums, 4))
+            if (!elements_aligned(x, x_type) || !aligned(scales, 4) || !aligned(scales_t, 4) ||
+                !elements_aligned(col_sums, sums_type))
                 return bad(fn, "a pointer is not aligned to its element");
             if (up(rows, nfx::kGroup) * up(cols, nfx::kGroup) > kIntMax) return bad(fn, "too many blocks");
             if (col_sums) {
@@ -176,7 +178,7 @@ int nfx_fp8_quantise(const void* x, int x_type, int64_t ldx, int64_t rows, int64
         if (col_sums && cols > 0)
             return launched(fn, nfx::column_reduce_launch(static_cast<float*>(workspace),
                                                           static_cast<int>(up(rows, nfx::kGroup)), cols, col_sums,
-                                                          nullptr, NFX_F32, st));
+                                                          nullptr, sums_type, st));
         return NFX_OK;
     });
 }

@@ -124,56 +124,10 @@ def fp8_gemm(a, b, bias=None, act=0, out_dtype=torch.bfloat16, out=None, stream=
     return _ext.fp8_gemm(*a, *b, bias, act, out_dtype, out)
 
 
-# ---- autograd -------------------------------------------------------------------------------
-class _LayerNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, gamma, beta, eps):
-        y, mean, rstd = layer_norm(x, gamma, beta, eps, stats=True)
-        ctx.save_for_backward(x, gamma, mean, rstd)
-        ctx.beta = None if beta is None else beta.dtype
-        return y
-
-    @staticmethod
-    def backward(ctx, dy):
-        x, gamma, mean, rstd = ctx.saved_tensors
-        params = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
-        dx, dg, db = layer_norm_backward(dy.contiguous(), x, mean, rstd, gamma, param_grads=params)
-        return (dx, dg if ctx.needs_input_grad[1] else None,
-                db.to(ctx.beta) if ctx.needs_input_grad[2] else None, None)
-
-
+# ---- under autograd -------------------------------------------------------------------------
 def layer_norm_autograd(x, gamma=None, beta=None, eps=1e-5):
     """layer_norm as a differentiable function of x, gamma and beta."""
-    return _LayerNorm.apply(x, gamma, beta, eps)
-
-
-class _Fp8Linear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, w, b):
-        need_dx, need_dw = ctx.needs_input_grad[:2]
-        xq, xt = fp8_quantise(x, transposed=True) if need_dw else (fp8_quantise(x), None)
-        wq, wt = fp8_quantise(w, tile=True, transposed=True) if need_dx else (fp8_quantise(w, tile=True), None)
-        ctx.saved = (xt, wt)
-        ctx.like = (x.shape, x.dtype, w.dtype, None if b is None else b.dtype)
-        return fp8_gemm(xq, wq, bias=b, out_dtype=x.dtype).view(*x.shape[:-1], w.shape[0])
-
-    @staticmethod
-    def backward(ctx, dy):
-        (xt, wt), (shape, xdt, wdt, bdt) = ctx.saved, ctx.like
-        need_dx, need_dw, need_db = ctx.needs_input_grad
-        dy = dy.reshape(-1, dy.shape[-1]).contiguous()
-        dx = dw = db = None
-        # one read of dy makes the operands of both products and the bias gradient
-        got = fp8_quantise(dy, transposed=need_dw, col_sums=need_db)
-        got = list(got) if need_dw or need_db else [got]
-        dq = got.pop(0)
-        if need_dw:
-            dw = fp8_gemm(got.pop(0), xt, out_dtype=wdt)
-        if need_db:
-            db = got.pop(0).to(bdt)
-        if need_dx:
-            dx = fp8_gemm(dq, wt, out_dtype=xdt).view(shape)
-        return dx, dw, db
+    return _ext.layer_norm_autograd(x, gamma, beta, eps)
 
 
 def fp8_linear(x, weight, bias=None):
@@ -181,8 +135,4 @@ def fp8_linear(x, weight, bias=None):
     128 along K, weight (N, K) in 128 x 128 tiles; the gradient dy in groups along N for dx and, with x,
     in groups along the tokens for the weight gradient.  Gradients pass through the rounding to FP8
     unchanged; they come in the types of x, weight and bias, the output in x's."""
-    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
-        _refuse("fp8_linear", f"weight must be (N, {x.shape[-1] if x.dim() else '?'})")
-    if bias is not None and bias.shape != weight.shape[:1]:
-        _refuse("fp8_linear", f"bias must be a vector of {weight.shape[0]}")
-    return _Fp8Linear.apply(x, weight, bias)
+    return _ext.fp8_linear(x, weight, bias)

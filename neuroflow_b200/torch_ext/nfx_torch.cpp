@@ -9,6 +9,7 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <optional>
@@ -25,6 +26,7 @@ namespace {
 constexpr int64_t kGroup = 128;
 
 [[noreturn]] void raise(int code, const std::string& msg) {
+    py::gil_scoped_acquire gil;  // (a backward pass runs without it)
     py::object cls = py::module_::import("neuroflow_b200._nfx").attr("NfxError");
     py::object err = cls(code, msg);
     PyErr_SetObject(cls.ptr(), err.ptr());
@@ -106,7 +108,6 @@ struct Fp8 {
     }
     uint8_t* data() const { return static_cast<uint8_t*>(codes.data_ptr()); }
     float* scale() const { return static_cast<float*>(scales.data_ptr()); }
-    py::tuple both() const { return py::make_tuple(codes, scales); }
 };
 
 struct Norm {
@@ -133,7 +134,10 @@ std::pair<Tensor, Tensor> stats_of(const Tensor& x) {
 }
 float* ptr(const Tensor& t) { return t.defined() ? static_cast<float*>(t.data_ptr()) : nullptr; }
 
-py::object layer_norm(const Tensor& x, const OptTensor& gamma, const OptTensor& beta, double eps, const OptTensor& out, bool stats) {
+struct NormOut {
+    Tensor y, mean, rstd;
+};
+NormOut layer_norm(const Tensor& x, const OptTensor& gamma, const OptTensor& beta, double eps, const OptTensor& out, bool stats) {
     const char* fn = "layer_norm";
     const Norm n = norm_of(fn, x, gamma, beta);
     c10::cuda::CUDAGuard guard(x.device());
@@ -151,8 +155,7 @@ py::object layer_norm(const Tensor& x, const OptTensor& gamma, const OptTensor& 
     if (stats) st = stats_of(x);
     check(nfx_layer_norm(x.const_data_ptr(), n.xt, n.x.ld, n.g, n.b, n.pt, n.x.rows, n.x.cols, static_cast<float>(eps),
                          y.data_ptr(), ldy, ptr(st.first), ptr(st.second), stream_of(x)));
-    if (!stats) return py::cast(y);
-    return py::make_tuple(y, st.first, st.second);
+    return {y, st.first, st.second};
 }
 
 py::object layer_norm_fp8(const Tensor& x, const OptTensor& gamma, const OptTensor& beta, double eps, bool stats) {
@@ -163,11 +166,14 @@ py::object layer_norm_fp8(const Tensor& x, const OptTensor& gamma, const OptTens
     if (stats) st = stats_of(x);
     check(nfx_layer_norm_fp8(x.const_data_ptr(), n.xt, n.x.ld, n.g, n.b, n.pt, n.x.rows, n.x.cols, static_cast<float>(eps),
                              q.data(), q.ld, q.scale(), 1, q.srows, ptr(st.first), ptr(st.second), stream_of(x)));
-    if (!stats) return q.both();
+    if (!stats) return py::make_tuple(q.codes, q.scales);
     return py::make_tuple(q.codes, q.scales, st.first, st.second);
 }
 
-py::tuple layer_norm_backward(const Tensor& dy, const Tensor& x, const Tensor& mean, const Tensor& rstd, const OptTensor& gamma,
+struct NormGrad {
+    Tensor dx, dgamma, dbeta;
+};
+NormGrad layer_norm_backward(const Tensor& dy, const Tensor& x, const Tensor& mean, const Tensor& rstd, const OptTensor& gamma,
                               bool param_grads) {
     const char* fn = "layer_norm_backward";
     const Norm n = norm_of(fn, x, gamma, std::nullopt);
@@ -195,11 +201,15 @@ py::tuple layer_norm_backward(const Tensor& dy, const Tensor& x, const Tensor& m
                                   static_cast<const float*>(mean.const_data_ptr()), static_cast<const float*>(rstd.const_data_ptr()),
                                   n.g, n.pt, n.x.rows, d, dx.data_ptr(), d, param_grads ? dg.data_ptr() : nullptr,
                                   param_grads ? db.data_ptr() : nullptr, param_grads ? ws.data_ptr() : nullptr, bytes, stream_of(x)));
-    if (!param_grads) return py::make_tuple(dx, py::none(), py::none());
-    return py::make_tuple(dx, dg, db);
+    return {dx, dg, db};
 }
 
-py::tuple fp8_quantise(const Tensor& x, bool tile, bool transposed, bool col_sums) {
+struct Quantised {
+    Fp8 q;
+    std::optional<Fp8> qt;
+    Tensor sums;
+};
+Quantised fp8_quantise(const Tensor& x, bool tile, bool transposed, bool col_sums, at::ScalarType sums_type = at::kFloat) {
     const char* fn = "fp8_quantise";
     const int xt = type_of(fn, "x", x);
     const Rows r = rows_of(fn, "x", x);
@@ -211,14 +221,15 @@ py::tuple fp8_quantise(const Tensor& x, bool tile, bool transposed, bool col_sum
     Tensor sums, ws;
     int64_t bytes = 0;
     if (col_sums) {
-        sums = empty({r.cols}, at::kFloat, x);
+        sums = empty({r.cols}, sums_type, x);
         bytes = nfx_fp8_quantise_workspace(r.rows, r.cols);
         ws = empty({bytes}, at::kByte, x);
     }
     check(nfx_fp8_quantise(x.const_data_ptr(), xt, r.ld, r.rows, r.cols, tile, q.data(), q.ld, q.scale(), 1, q.srows,
-                           qt ? qt->data() : nullptr, qt ? qt->ld : 0, qt ? qt->scale() : nullptr, 1, qt ? qt->srows : 0, ptr(sums),
-                           col_sums ? ws.data_ptr() : nullptr, bytes, stream_of(x)));
-    return py::make_tuple(q.codes, q.scales, qt ? py::object(qt->both()) : py::none(), col_sums ? py::cast(sums) : py::none());
+                           qt ? qt->data() : nullptr, qt ? qt->ld : 0, qt ? qt->scale() : nullptr, 1, qt ? qt->srows : 0,
+                           col_sums ? sums.data_ptr() : nullptr, type_of(sums_type), col_sums ? ws.data_ptr() : nullptr, bytes,
+                           stream_of(x)));
+    return {q, qt, sums};
 }
 
 struct Operand {
@@ -266,12 +277,101 @@ Tensor fp8_gemm(const Tensor& ac, const Tensor& as, bool a_tile, const Tensor& b
     return c;
 }
 
+// ---- autograd -----------------------------------------------------------------------------------
+OptTensor defined(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
+
+struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
+    static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const OptTensor& gamma, const OptTensor& beta,
+                          double eps) {
+        const NormOut n = layer_norm(x, gamma, beta, eps, std::nullopt, true);
+        ctx->save_for_backward({x, gamma ? *gamma : Tensor(), n.mean, n.rstd});
+        ctx->saved_data["params"] = (gamma && gamma->requires_grad()) || (beta && beta->requires_grad());
+        ctx->saved_data["beta"] = beta ? static_cast<int64_t>(beta->scalar_type()) : static_cast<int64_t>(-1);
+        return n.y;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list dy) {
+        const auto saved = ctx->get_saved_variables();
+        const NormGrad g = layer_norm_backward(dy[0].contiguous(), saved[0], saved[2], saved[3], defined(saved[1]),
+                                               ctx->saved_data["params"].toBool());
+        const int64_t bt = ctx->saved_data["beta"].toInt();
+        Tensor db = g.dbeta;
+        if (db.defined() && bt >= 0) db = db.to(static_cast<at::ScalarType>(bt));
+        return {g.dx, saved[1].defined() ? g.dgamma : Tensor(), bt >= 0 ? db : Tensor(), Tensor()};
+    }
+};
+
+// y = Q(x) Q(W)^T + b; dx = Q(dy) Q(W^T)^T, dW = Q(dy^T) Q(x^T)^T, db = sums of dy's columns.  The transposed
+// operands of the backward products are made with the forward ones, from the same reads.
+struct Fp8LinearFn : torch::autograd::Function<Fp8LinearFn> {
+    static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptTensor& b) {
+        const bool dx = x.requires_grad(), dw = w.requires_grad(), db = b && b->requires_grad();
+        const Quantised xq = fp8_quantise(x, false, dw, false), wq = fp8_quantise(w, true, dx, false);
+        const Tensor none;
+        ctx->save_for_backward({dw ? xq.qt->codes : none, dw ? xq.qt->scales : none, dx ? wq.qt->codes : none,
+                                dx ? wq.qt->scales : none});
+        ctx->saved_data["db"] = db;
+        ctx->saved_data["x"] = x.sizes().vec();
+        ctx->saved_data["types"] = std::vector<int64_t>{static_cast<int64_t>(x.scalar_type()), static_cast<int64_t>(w.scalar_type()),
+                                                        b ? static_cast<int64_t>(b->scalar_type()) : 0};
+        auto sizes = x.sizes().vec();
+        sizes.back() = w.size(0);
+        return fp8_gemm(xq.q.codes, xq.q.scales, false, wq.q.codes, wq.q.scales, true, b, 0, x.scalar_type(), std::nullopt).view(sizes);
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        const auto types = ctx->saved_data["types"].toIntVector();
+        const bool need_dw = saved[0].defined(), need_dx = saved[2].defined(), need_db = ctx->saved_data["db"].toBool();
+        const Tensor dy = grads[0].contiguous();
+        // one read of dy makes the operands of both products and the bias gradient
+        const Quantised q = fp8_quantise(dy, false, need_dw, need_db,
+                                         need_db ? static_cast<at::ScalarType>(types[2]) : at::kFloat);
+        Tensor dx, dw;
+        if (need_dw)
+            dw = fp8_gemm(q.qt->codes, q.qt->scales, false, saved[0], saved[1], false, std::nullopt, 0,
+                          static_cast<at::ScalarType>(types[1]), std::nullopt);
+        if (need_dx)
+            dx = fp8_gemm(q.q.codes, q.q.scales, false, saved[2], saved[3], true, std::nullopt, 0,
+                          static_cast<at::ScalarType>(types[0]), std::nullopt).view(ctx->saved_data["x"].toIntVector());
+        return {dx, dw, q.sums};
+    }
+};
+
+Tensor fp8_linear(const Tensor& x, const Tensor& w, const OptTensor& b) {
+    const char* fn = "fp8_linear";
+    type_of(fn, "x", x);
+    type_of(fn, "weight", w);
+    if (w.dim() != 2 || x.dim() < 1 || x.size(-1) != w.size(1))
+        refuse(fn, "weight must be (N, " + (x.dim() ? std::to_string(x.size(-1)) : std::string("?")) + ")");
+    same_device(fn, x, "weight", w);
+    int t = 0;
+    vector_of(fn, "bias", b, w.size(0), x, &t);
+    return Fp8LinearFn::apply(x, w, b);
+}
+
+py::object or_none(const Tensor& t) { return t.defined() ? py::cast(t) : py::none(); }
+
 }  // namespace
 
 PYBIND11_MODULE(_nfx_torch, m) {
-    m.def("layer_norm", &layer_norm);
+    m.def("layer_norm", [](const Tensor& x, const OptTensor& g, const OptTensor& b, double eps, const OptTensor& out, bool stats) {
+        const NormOut n = layer_norm(x, g, b, eps, out, stats);
+        return stats ? py::object(py::make_tuple(n.y, n.mean, n.rstd)) : py::cast(n.y);
+    });
     m.def("layer_norm_fp8", &layer_norm_fp8);
-    m.def("layer_norm_backward", &layer_norm_backward);
-    m.def("fp8_quantise", &fp8_quantise);
+    m.def("layer_norm_backward", [](const Tensor& dy, const Tensor& x, const Tensor& mean, const Tensor& rstd, const OptTensor& g,
+                                    bool params) {
+        const NormGrad n = layer_norm_backward(dy, x, mean, rstd, g, params);
+        return py::make_tuple(n.dx, or_none(n.dgamma), or_none(n.dbeta));
+    });
+    m.def("fp8_quantise", [](const Tensor& x, bool tile, bool transposed, bool col_sums) {
+        const Quantised q = fp8_quantise(x, tile, transposed, col_sums);
+        return py::make_tuple(q.q.codes, q.q.scales, q.qt ? py::object(py::make_tuple(q.qt->codes, q.qt->scales)) : py::none(),
+                              or_none(q.sums));
+    });
     m.def("fp8_gemm", &fp8_gemm);
+    m.def("fp8_linear", &fp8_linear);
+    m.def("layer_norm_autograd", [](const Tensor& x, const OptTensor& g, const OptTensor& b, double eps) {
+        norm_of("layer_norm_autograd", x, g, b);
+        return LayerNormFn::apply(x, g, b, eps);
+    });
 }

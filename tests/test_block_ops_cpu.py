@@ -51,9 +51,10 @@ def test_layer_norm_backward_refusals():
 
 
 def test_quantise_refusals():
-    f = lambda x=P, xt=1, ld=130, rows=4, cols=130, tile=0, codes=P, ldc=144, scales=P, ct=None, ldt=16, st=None, sums=None, ws=None, n=0: \
-        L.nfx_fp8_quantise(x, xt, ld, rows, cols, tile, codes, ldc, scales, 1, 4, ct, ldt, st, 1, 130, sums, ws, n, None)
+    f = lambda x=P, xt=1, ld=130, rows=4, cols=130, tile=0, codes=P, ldc=144, scales=P, ct=None, ldt=16, st=None, sums=None, sumt=0, ws=None, n=0: \
+        L.nfx_fp8_quantise(x, xt, ld, rows, cols, tile, codes, ldc, scales, 1, 4, ct, ldt, st, 1, 130, sums, sumt, ws, n, None)
     _bad(f(xt=9), "x_type")
+    _bad(f(sumt=4), "sums_type")
     _bad(f(rows=-1), "rows")
     _bad(f(cols=1 << 31), "2^31")
     _bad(f(tile=2), "tile")

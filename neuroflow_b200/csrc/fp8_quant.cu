@@ -67,13 +67,21 @@ __global__ void __launch_bounds__(kTileThreads, 2) quant_tile_kernel(QuantArgs a
     auto ahead = [&](int t) {
         const int64_t r0 = static_cast<int64_t>(t / cblocks) * kGroup + rr * 8, c0 = static_cast<int64_t>(t % cblocks) * kGroup + cc * 8;
         const T* x = static_cast<const T*>(a.x) + r0 * a.ldx + c0;
+        uint8_t* slot = next + threadIdx.x * 16;
+        if (r0 + 8 <= a.rows && c0 + 8 <= a.cols) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i, x += a.ldx)
+#pragma unroll
+                for (int k = 0; k < kPacks; ++k) cp_async16(slot + (i * kPacks + k) * kTileThreads * 16, x + k * VE, 16);
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < 8; ++i)
 #pragma unroll
             for (int k = 0; k < kPacks; ++k) {
                 const int64_t left = r0 + i < a.rows ? a.cols - c0 - k * VE : 0;
                 const int n = left >= VE ? 16 : (left > 0 ? static_cast<int>(left * sizeof(T)) : 0);
-                cp_async16(next + ((i * kPacks + k) * kTileThreads + threadIdx.x) * 16, n ? x + i * a.ldx + k * VE : a.x, n);
+                cp_async16(slot + (i * kPacks + k) * kTileThreads * 16, n ? x + i * a.ldx + k * VE : a.x, n);
             }
     };
     if (kWalk) ahead(blockIdx.x);
@@ -192,28 +200,40 @@ __global__ void __launch_bounds__(kTileThreads, 2) quant_tile_kernel(QuantArgs a
         // codes along the rows
         const bool inside = wide && c0 + 8 <= a.cols && r0 + 8 <= a.rows;
         uint8_t* row = a.q.codes + r0 * a.q.ld + c0;
+        uint32_t odd = 0;
+        auto along_rows = [&](auto mend) {
+            constexpr bool kMend = decltype(mend)::value;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float inv = a.tile ? tinv : rinv[rr * 8 + i];
-            const uint32_t w0 = scaled_codes(v[i][0], v[i][1], v[i][2], v[i][3], inv);
-            const uint32_t w1 = scaled_codes(v[i][4], v[i][5], v[i][6], v[i][7], inv);
-            if (inside) {
-                *reinterpret_cast<uint2*>(row + i * a.q.ld) = make_uint2(w0, w1);
-            } else if (r0 + i < a.rows) {
+            for (int i = 0; i < 8; ++i) {
+                const float inv = a.tile ? tinv : rinv[rr * 8 + i];
+                const uint32_t w0 = scaled_codes<kMend>(v[i][0], v[i][1], v[i][2], v[i][3], inv, odd);
+                const uint32_t w1 = scaled_codes<kMend>(v[i][4], v[i][5], v[i][6], v[i][7], inv, odd);
+                if (inside) {
+                    *reinterpret_cast<uint2*>(row + i * a.q.ld) = make_uint2(w0, w1);
+                } else if (r0 + i < a.rows) {
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    if (c0 + k < a.cols) row[i * a.q.ld + k] = static_cast<uint8_t>((k < 4 ? w0 : w1) >> (8 * (k & 3)));
+                    for (int k = 0; k < 8; ++k)
+                        if (c0 + k < a.cols) row[i * a.q.ld + k] = static_cast<uint8_t>((k < 4 ? w0 : w1) >> (8 * (k & 3)));
+                }
             }
-        }
+        };
+        along_rows(std::false_type{});
+        if (odd) along_rows(std::true_type{});  // (rare; the same bytes again, put right)
         if (!a.qt.codes) continue;
         // codes along the columns
+        odd = 0;
+        auto along_columns = [&](auto mend) {
+            constexpr bool kMend = decltype(mend)::value;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const float inv = a.tile ? tinv : cinv[cc * 8 + k];
-            const uint32_t w0 = scaled_codes(v[0][k], v[1][k], v[2][k], v[3][k], inv);
-            const uint32_t w1 = scaled_codes(v[4][k], v[5][k], v[6][k], v[7][k], inv);
-            *reinterpret_cast<uint2*>(tileT + (cc * 8 + k) * kGroup + (rr ^ cc) * 8) = make_uint2(w0, w1);
-        }
+            for (int k = 0; k < 8; ++k) {
+                const float inv = a.tile ? tinv : cinv[cc * 8 + k];
+                const uint32_t w0 = scaled_codes<kMend>(v[0][k], v[1][k], v[2][k], v[3][k], inv, odd);
+                const uint32_t w1 = scaled_codes<kMend>(v[4][k], v[5][k], v[6][k], v[7][k], inv, odd);
+                *reinterpret_cast<uint2*>(tileT + (cc * 8 + k) * kGroup + (rr ^ cc) * 8) = make_uint2(w0, w1);
+            }
+        };
+        along_columns(std::false_type{});
+        if (odd) along_columns(std::true_type{});
         __syncthreads();
 #pragma unroll
         for (int n = 0; n < kGroup * 8 / kTileThreads; ++n) {

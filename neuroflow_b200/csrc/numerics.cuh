@@ -212,10 +212,12 @@ __device__ __forceinline__ uint32_t e4m3_encode_fast(float v) {
 #endif
 }
 
-// e4m3_encode_fast of four values as the bytes of a word, by two paired conversions.  The conversion
-// differs from the reference encoder only in results of magnitude 8 (see above; it gives 0x7F for every
-// NaN), which are found with a test for a zero byte and are rare: they take the second look.
-__device__ __forceinline__ uint32_t e4m3_encode4(float v0, float v1, float v2, float v3) {
+// Four values as the bytes of a word by two paired conversions.  The conversion gives e4m3_encode_fast's
+// codes (0x7F for every NaN) save where that has the reference's code 7 and the conversion the smallest
+// normal, code 8: `odd` collects a bit for every word with a code of magnitude 8, whatever its value
+// (a test for a zero byte), and e4m3_mend4 puts such a word right.  They are rare, so callers convert
+// everything first and look at `odd` once.
+__device__ __forceinline__ uint32_t e4m3_convert4(float v0, float v1, float v2, float v3, uint32_t& odd) {
 #ifdef __CUDA_ARCH__
     uint32_t w;
     asm("{\n\t.reg .b16 lo, hi;\n\t"
@@ -224,16 +226,24 @@ __device__ __forceinline__ uint32_t e4m3_encode4(float v0, float v1, float v2, f
         : "=r"(w)
         : "f"(v0), "f"(v1), "f"(v2), "f"(v3));
     const uint32_t t = (w & 0x7F7F7F7Fu) ^ 0x08080808u;
-    if ((t - 0x01010101u) & ~t & 0x80808080u) {
-        const float v[4] = {v0, v1, v2, v3};
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (((w >> (8 * i)) & 0x7Fu) == 8u && fabsf(v[i]) < 0.015625f) w -= 1u << (8 * i);
-    }
+    odd |= (t - 0x01010101u) & ~t & 0x80808080u;
     return w;
 #else
+    (void)odd;
     return e4m3_encode_ref(v0) | e4m3_encode_ref(v1) << 8 | e4m3_encode_ref(v2) << 16 | e4m3_encode_ref(v3) << 24;
 #endif
+}
+__device__ __forceinline__ uint32_t e4m3_mend4(uint32_t w, float v0, float v1, float v2, float v3) {
+    w -= (w & 0x7Fu) == 8u && fabsf(v0) < 0.015625f ? 1u : 0u;
+    w -= (w & 0x7F00u) == 0x800u && fabsf(v1) < 0.015625f ? 0x100u : 0u;
+    w -= (w & 0x7F0000u) == 0x80000u && fabsf(v2) < 0.015625f ? 0x10000u : 0u;
+    w -= (w & 0x7F000000u) == 0x8000000u && fabsf(v3) < 0.015625f ? 0x1000000u : 0u;
+    return w;
+}
+__device__ __forceinline__ uint32_t e4m3_encode4(float v0, float v1, float v2, float v3) {
+    uint32_t odd = 0;
+    const uint32_t w = e4m3_convert4(v0, v1, v2, v3, odd);
+    return odd ? e4m3_mend4(w, v0, v1, v2, v3) : w;
 }
 
 // e4m3_decode_ref by the hardware conversion (E4M3 -> f16 is exact, f16 -> f32 too);

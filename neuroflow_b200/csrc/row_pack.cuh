@@ -52,10 +52,13 @@ __device__ __forceinline__ void store_pack(T* p, const float (&o)[VE]) {
         *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
     }
 }
-// The codes of four values times `inv` (two products to an instruction, each rounded by itself).
-__device__ __forceinline__ uint32_t scaled_codes(float a, float b, float c, float d, float inv) {
+// The codes of four values times `inv` (two products to an instruction, each rounded by itself): plain
+// conversions that note in `odd` where they may differ from the encoder, or, with MEND, its codes.
+template <bool MEND>
+__device__ __forceinline__ uint32_t scaled_codes(float a, float b, float c, float d, float inv, uint32_t& odd) {
     const float2 p = mul2_rn(make_float2(a, b), make_float2(inv, inv)), q = mul2_rn(make_float2(c, d), make_float2(inv, inv));
-    return e4m3_encode4(p.x, p.y, q.x, q.y);
+    const uint32_t w = e4m3_convert4(p.x, p.y, q.x, q.y, odd);
+    return MEND ? e4m3_mend4(w, p.x, p.y, q.x, q.y) : w;
 }
 
 // FP8 codes of a lane's VPT packs (values v, zero beyond column d): pack j holds columns (first_pack +
@@ -99,36 +102,42 @@ __device__ __forceinline__ void store_codes(const float (&v)[VPT][VE], const Fp8
     // the first column of group `at` of this lane's row
     const int64_t c_at = (first_pack - at + static_cast<int64_t>(at) * kPer * 32) * VE;
     if (live && at < kGroups && c_at < d) q.scales[r * q.srs + (c_at / kGroup) * q.sbs] = sc;
+    uint32_t odd = 0;
+    auto write = [&](auto mend) {
+        constexpr bool kMend = decltype(mend)::value;
 #pragma unroll
-    for (int j = 0; j < kGroups; ++j) {
-        const float inv = __shfl_sync(0xFFFFFFFFu, inv_mine, j, kLanes);
-        const int64_t c0 = (first_pack + j * kPer * 32) * VE;  // this lane's first column
-        uint8_t* dst = q.codes + r * q.ld + c0;
-        if constexpr (VE == 1) {
-            const uint32_t w = scaled_codes(v[4 * j][0], v[4 * j + 1][0], v[4 * j + 2][0], v[4 * j + 3][0], inv);
-            if (live && c0 - lane + kGroup <= d) {
+        for (int j = 0; j < kGroups; ++j) {
+            const float inv = __shfl_sync(0xFFFFFFFFu, inv_mine, j, kLanes);
+            const int64_t c0 = (first_pack + j * kPer * 32) * VE;  // this lane's first column
+            uint8_t* dst = q.codes + r * q.ld + c0;
+            if constexpr (VE == 1) {
+                const uint32_t w = scaled_codes<kMend>(v[4 * j][0], v[4 * j + 1][0], v[4 * j + 2][0], v[4 * j + 3][0], inv, odd);
+                if (live && c0 - lane + kGroup <= d) {
 #pragma unroll
-                for (int h = 0; h < 4; ++h) dst[h * 32] = static_cast<uint8_t>(w >> (8 * h));
+                    for (int h = 0; h < 4; ++h) dst[h * 32] = static_cast<uint8_t>(w >> (8 * h));
+                } else {
+#pragma unroll
+                    for (int h = 0; h < 4; ++h)
+                        if (live && c0 + h * 32 < d) dst[h * 32] = static_cast<uint8_t>(w >> (8 * h));
+                }
             } else {
+                uint32_t w[VE / 4];
 #pragma unroll
-                for (int h = 0; h < 4; ++h)
-                    if (live && c0 + h * 32 < d) dst[h * 32] = static_cast<uint8_t>(w >> (8 * h));
-            }
-        } else {
-            uint32_t w[VE / 4];
+                for (int i = 0; i < VE / 4; ++i)
+                    w[i] = scaled_codes<kMend>(v[j][4 * i], v[j][4 * i + 1], v[j][4 * i + 2], v[j][4 * i + 3], inv, odd);
+                if (!live || c0 >= d) continue;
+                if (wide) {
+                    if constexpr (VE == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+                    else *reinterpret_cast<uint32_t*>(dst) = w[0];
+                } else {
 #pragma unroll
-            for (int i = 0; i < VE / 4; ++i)
-                w[i] = scaled_codes(v[j][4 * i], v[j][4 * i + 1], v[j][4 * i + 2], v[j][4 * i + 3], inv);
-            if (!live || c0 >= d) continue;
-            if (wide) {
-                if constexpr (VE == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
-                else *reinterpret_cast<uint32_t*>(dst) = w[0];
-            } else {
-#pragma unroll
-                for (int i = 0; i < VE; ++i) dst[i] = static_cast<uint8_t>(w[i / 4] >> (8 * (i % 4)));
+                    for (int i = 0; i < VE; ++i) dst[i] = static_cast<uint8_t>(w[i / 4] >> (8 * (i % 4)));
+                }
             }
         }
-    }
+    };
+    write(std::false_type{});
+    if (__any_sync(0xFFFFFFFFu, odd != 0)) write(std::true_type{});  // (rare; the same bytes again, put right)
 }
 
 }  // namespace nfx

@@ -522,18 +522,20 @@ cudaError_t launch_pair(const Fp8GemmArgs& p, cudaStream_t stream) {
 // 128, and K split over the CTAs of a cluster so that all SMs read weights.  Each CTA sums its share of
 // the blocks, puts the partial tile into its shared memory, and after a cluster barrier every CTA adds
 // the partials of its columns in the order of the ranks (deterministic; no atomics, no workspace),
-// applies bias and activation and stores.  Two CTAs per SM up to NT = 64.  Warps: four of promotion for
+// applies bias and activation and stores.  Up to NT = 64 two CTAs fit an SM; a grid that has no more CTAs
+// than SMs takes the memory of both for its own ring instead (DEEP: 64x4096x16384 18.5 -> 15.5 us, the
+// latency of a copy over the stages in flight is what a block of K waits for).  Warps: four of promotion for
 // each 32 columns (a warp reads 32 x 32 accumulators a block), then one TMA producer, one TMEM owner and
 // MMA issuer, one scale producer.
-template <int NT>
+template <int NT, bool DEEP>
 struct NarrowCfg {
     static constexpr int kPart = NT < 32 ? NT : 32;  // columns of a promoting warp
     static constexpr int kEpi = 4 * (NT / kPart);
     static constexpr int kThreads = 32 * (kEpi + 4);
-    static constexpr int kPerSm = NT > 64 ? 1 : 2;
+    static constexpr int kPerSm = DEEP || NT > 64 ? 1 : 2;
     static constexpr int kABytes = 128 * kBK;
     static constexpr int kStageBytes = kABytes + NT * kBK;
-    static constexpr int kStages = (NT > 64 ? 163840 : 98304) / kStageBytes;
+    static constexpr int kStages = (NT > 64 ? 163840 : (DEEP ? 184320 : 98304)) / kStageBytes;
     static constexpr int kAcc = 4;
     static constexpr int kTmem = NT * kAcc;
     static constexpr int kScaleStages = 8;
@@ -554,11 +556,11 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t cluster_addr) {
     return v;
 }
 
-template <int NT, int CT>
-__global__ void __launch_bounds__(NarrowCfg<NT>::kThreads, NarrowCfg<NT>::kPerSm)
+template <int NT, int CT, bool DEEP>
+__global__ void __launch_bounds__(NarrowCfg<NT, DEEP>::kThreads, NarrowCfg<NT, DEEP>::kPerSm)
 fp8_gemm_narrow_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                        const Fp8GemmArgs p, const int split) {
-    using C = NarrowCfg<NT>;
+    using C = NarrowCfg<NT, DEEP>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kOffBars);
@@ -790,15 +792,15 @@ fp8_gemm_narrow_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_con
     if (split > 1) cluster_sync();  // no CTA leaves while another may still read its partial tile
 }
 
-template <int NT, int CT>
+template <int NT, int CT, bool DEEP>
 cudaError_t launch_narrow(const Fp8GemmArgs& p, int split, cudaStream_t stream) {
-    using C = NarrowCfg<NT>;
+    using C = NarrowCfg<NT, DEEP>;
     CUtensorMap tmW{}, tmX{};
     if (p.K > 0 &&
         (!encode_2d(&tmW, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.B, p.K, p.N, p.ldb, kBK, 128, 128) ||
          !encode_2d(&tmX, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.A, p.K, p.M, p.lda, kBK, NT, 128)))
         return cudaErrorInvalidValue;
-    auto kern = fp8_gemm_narrow_kernel<NT, CT>;
+    auto kern = fp8_gemm_narrow_kernel<NT, CT, DEEP>;
     cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), C::kSmemBytes);
     if (e != cudaSuccess) return e;
     const int64_t tiles = static_cast<int64_t>((p.N + 127) / 128) * ((p.M + NT - 1) / NT);
@@ -842,10 +844,11 @@ cudaError_t dispatch(const Fp8GemmArgs& p, cudaStream_t stream) {
     const int64_t pair = rounds(wide, sms / 2) * (KB + 5) + 10;
     const int64_t narrow = rounds(tiles(nt) * split, nt > 64 ? sms : 2 * sms) * ((KB + split - 1) / split + 5) + 5;
     if (nt == 128 && pair < narrow) return launch_pair<CT>(p, stream);
-    if (nt == 16) return launch_narrow<16, CT>(p, split, stream);
-    if (nt == 32) return launch_narrow<32, CT>(p, split, stream);
-    if (nt == 64) return launch_narrow<64, CT>(p, split, stream);
-    return launch_narrow<128, CT>(p, split, stream);
+    const bool deep = tiles(nt) * split <= sms;
+    if (nt == 16) return deep ? launch_narrow<16, CT, true>(p, split, stream) : launch_narrow<16, CT, false>(p, split, stream);
+    if (nt == 32) return deep ? launch_narrow<32, CT, true>(p, split, stream) : launch_narrow<32, CT, false>(p, split, stream);
+    if (nt == 64) return deep ? launch_narrow<64, CT, true>(p, split, stream) : launch_narrow<64, CT, false>(p, split, stream);
+    return launch_narrow<128, CT, true>(p, split, stream);
 }
 
 }  // namespace

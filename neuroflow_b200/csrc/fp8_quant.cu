@@ -289,7 +289,9 @@ cudaError_t quant_t(const QuantArgs& a, cudaStream_t s) {
     constexpr int VE = 16 / sizeof(T);
     const bool rows16 = aligned16(a.x) && (a.rows == 1 || a.ldx % VE == 0);
     if (!a.tile && !a.qt.codes && !a.part) {
-        if (!rows16 || a.cols % VE) return quant_rows<T, 1, 8, 32>(a, s);
+        if (!rows16 || a.cols % VE)
+            return aligned_rows(a.x, a.rows, a.ldx, sizeof(T), 2 * sizeof(T)) && a.cols % 2 == 0 ? quant_rows<T, 2, 4, 32>(a, s)
+                                                                                             : quant_rows<T, 1, 8, 32>(a, s);
         if (a.cols <= 16 * VE) return quant_rows<T, VE, 1, 16>(a, s);
         if (a.cols <= 32 * VE) return quant_rows<T, VE, 1, 32>(a, s);
         return quant_rows<T, VE, 2, 32>(a, s);

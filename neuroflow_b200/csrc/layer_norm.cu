@@ -171,7 +171,7 @@ __device__ __forceinline__ void load_params(const void* p, int type, bool vec, i
     if (!p) {
 #pragma unroll
         for (int k = 0; k < VE; ++k) o[k] = none;
-    } else if (VE > 1 && vec && type == kF32) {
+    } else if (VE > 2 && vec && type == kF32) {
 #pragma unroll
         for (int k = 0; k < VE; k += 4) {
             const float4 f = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + i + k));
@@ -222,19 +222,10 @@ __device__ __forceinline__ float2 row_sums(float a, float b, float2* red) {
 // A pack as it was read.
 template <typename T, int VE>
 struct Raw {
-    uint4 u;
-    __device__ __forceinline__ void load(const T* p) { u = __ldg(reinterpret_cast<const uint4*>(p)); }
-    __device__ __forceinline__ void get(float (&o)[VE]) const {
-        unpack<T, VE>(u, o);
-    }
-    __device__ __forceinline__ void zero() { u = make_uint4(0, 0, 0, 0); }
-};
-template <typename T>
-struct Raw<T, 1> {
-    T u;
-    __device__ __forceinline__ void load(const T* p) { u = *p; }
-    __device__ __forceinline__ void get(float (&o)[1]) const { o[0] = to_f32(u); }
-    __device__ __forceinline__ void zero() { u = from_f32<T>(0.0f); }
+    word_t<T, VE> u;
+    __device__ __forceinline__ void load(const T* p) { u = __ldg(reinterpret_cast<const word_t<T, VE>*>(p)); }
+    __device__ __forceinline__ void get(float (&o)[VE]) const { unpack<T, VE>(u, o); }
+    __device__ __forceinline__ void zero() { u = word_t<T, VE>{}; }
 };
 
 constexpr int row_block(int tpr) { return tpr > 128 ? tpr : 128; }
@@ -381,11 +372,11 @@ cudaError_t norm_row(const NormArgs& a, bool pvec, cudaStream_t s) {
 }
 
 // Threads and packs per row by the width: the fewest threads that leave a thread 32 elements at most, and
-// with single-element packs 8 up to 4,096 columns (more loads to a row than a warp should queue:
+// with packs of one or two elements 8 up to 4,096 columns (more loads to a row than a warp should queue:
 // 5003x771 fp32 takes 19 us with 32).
 template <typename T, int VE>
 cudaError_t norm_width(const NormArgs& a, bool pvec, cudaStream_t s) {
-    if constexpr (VE > 1) {
+    if constexpr (VE > 2) {
         constexpr int kV = 32 / VE;  // packs of 32 elements
         if (a.d <= 16 * VE) return norm_row<T, VE, 1, 16>(a, pvec, s);
         if (a.d <= 32 * VE) return norm_row<T, VE, 1, 32>(a, pvec, s);
@@ -397,14 +388,15 @@ cudaError_t norm_width(const NormArgs& a, bool pvec, cudaStream_t s) {
         if (a.d <= 8192) return norm_row<T, VE, kV, 256>(a, pvec, s);
         return norm_row<T, VE, kV, 512>(a, pvec, s);
     } else {
-        if (a.d <= 128) return norm_row<T, VE, 4, 32>(a, pvec, s);
-        if (a.d <= 256) return norm_row<T, VE, 8, 32>(a, pvec, s);
-        if (a.d <= 512) return norm_row<T, VE, 8, 64>(a, pvec, s);
-        if (a.d <= 1024) return norm_row<T, VE, 8, 128>(a, pvec, s);
-        if (a.d <= 2048) return norm_row<T, VE, 8, 256>(a, pvec, s);
-        if (a.d <= 4096) return norm_row<T, VE, 8, 512>(a, pvec, s);
-        if (a.d <= 8192) return norm_row<T, VE, 16, 512>(a, pvec, s);
-        return norm_row<T, VE, 32, 512>(a, pvec, s);
+        constexpr int k8 = 8 / VE;  // packs of eight elements
+        if (a.d <= 128) return norm_row<T, VE, k8 / 2, 32>(a, pvec, s);
+        if (a.d <= 256) return norm_row<T, VE, k8, 32>(a, pvec, s);
+        if (a.d <= 512) return norm_row<T, VE, k8, 64>(a, pvec, s);
+        if (a.d <= 1024) return norm_row<T, VE, k8, 128>(a, pvec, s);
+        if (a.d <= 2048) return norm_row<T, VE, k8, 256>(a, pvec, s);
+        if (a.d <= 4096) return norm_row<T, VE, k8, 512>(a, pvec, s);
+        if (a.d <= 8192) return norm_row<T, VE, 2 * k8, 512>(a, pvec, s);
+        return norm_row<T, VE, 4 * k8, 512>(a, pvec, s);
     }
 }
 
@@ -413,9 +405,12 @@ cudaError_t norm_t(const NormArgs& a, cudaStream_t s) {
     constexpr int VE = 16 / sizeof(T);
     if (a.d <= 16384 && a.rows <= 0x7FFFFFFF) {
         const bool pvec = aligned16(a.gamma) && aligned16(a.beta) && (a.ptype == kF32 || VE == 8);
-        const bool rows16 = aligned16(a.x) && (a.rows == 1 || a.ldx % VE == 0) &&
-                            (!a.y || (aligned16(a.y) && (a.rows == 1 || a.ldy % VE == 0)));
-        if (rows16 && a.d % VE == 0) return norm_width<T, VE>(a, pvec, s);
+        const auto rows_on = [&](int64_t bytes) {
+            return aligned_rows(a.x, a.rows, a.ldx, sizeof(T), bytes) && (!a.y || aligned_rows(a.y, a.rows, a.ldy, sizeof(T), bytes)) &&
+                   a.d * static_cast<int64_t>(sizeof(T)) % bytes == 0;
+        };
+        if (rows_on(16)) return norm_width<T, VE>(a, pvec, s);
+        if (rows_on(2 * sizeof(T))) return norm_width<T, 2>(a, false, s);
         return norm_width<T, 1>(a, false, s);
     }
     const int64_t cap = 8ll * device_sm_count();
@@ -597,9 +592,12 @@ norm_grad_row_kernel(NormGradArgs a, bool pvec) {
     for (int j = 0; j < VPT; ++j) {
         const int c = (first + j * 32) * VE;
         if (c >= a.d) continue;
-        if constexpr (VE == 1) {
-            out_g[c] = pg[j][0];
-            out_b[c] = pb[j][0];
+        if constexpr (VE <= 2) {
+#pragma unroll
+            for (int i = 0; i < VE; ++i) {
+                out_g[c + i] = pg[j][i];
+                out_b[c + i] = pb[j][i];
+            }
         } else {  // (d is a multiple of VE, the workspace 16-byte aligned)
 #pragma unroll
             for (int i = 0; i < VE; i += 4) {
@@ -641,9 +639,12 @@ cudaError_t norm_grad_t(const NormGradArgs& a, cudaStream_t s) {
     if (a.d <= 16384) {
         constexpr int VE = 16 / sizeof(T);
         const bool pvec = aligned16(a.gamma) && (a.ptype == kF32 || VE == 8);
-        const bool rows16 = aligned16(a.x) && aligned16(a.dy) && aligned16(a.dx) &&
-                            (a.rows == 1 || (a.ldx % VE == 0 && a.lddy % VE == 0 && a.lddx % VE == 0));
-        if (rows16 && a.d % VE == 0) return norm_grad_width<T, VE>(a, pvec, s);
+        const auto rows_on = [&](int64_t bytes) {
+            return aligned_rows(a.x, a.rows, a.ldx, sizeof(T), bytes) && aligned_rows(a.dy, a.rows, a.lddy, sizeof(T), bytes) &&
+                   aligned_rows(a.dx, a.rows, a.lddx, sizeof(T), bytes) && a.d * static_cast<int64_t>(sizeof(T)) % bytes == 0;
+        };
+        if (rows_on(16)) return norm_grad_width<T, VE>(a, pvec, s);
+        if (rows_on(2 * sizeof(T))) return norm_grad_width<T, 2>(a, false, s);
         return norm_grad_width<T, 1>(a, false, s);
     }
     norm_grad_any_kernel<T><<<a.parts, kAnyThreads, 0, s>>>(a);

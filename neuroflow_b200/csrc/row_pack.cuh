@@ -1,5 +1,6 @@
-// row_pack.cuh -- rows of a matrix in the registers of a warp, by packs of 16 bytes (or single
-// elements), and their FP8 form: shared by the layer norm and the quantiser.
+// row_pack.cuh -- rows of a matrix in the registers of a warp, by packs of 16 bytes (pairs of elements or
+// single ones where rows are not aligned to more), and their FP8 form: shared by the layer norm and the
+// quantiser.
 #pragma once
 
 #include <type_traits>
@@ -11,45 +12,60 @@ namespace nfx {
 
 inline bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
+inline bool aligned_rows(const void* p, int64_t rows, int64_t ld, int64_t el, int64_t bytes) {
+    return reinterpret_cast<uintptr_t>(p) % bytes == 0 && (rows == 1 || ld * el % bytes == 0);
+}
+
 template <typename T, int VE>
 struct Pack {
     T v[VE];
 };
-// the VE numbers of 16 bytes
+template <int BYTES>
+struct Word;
+template <>
+struct Word<2> { using type = uint16_t; };
+template <>
+struct Word<4> { using type = uint32_t; };
+template <>
+struct Word<8> { using type = uint2; };
+template <>
+struct Word<16> { using type = uint4; };
 template <typename T, int VE>
-__device__ __forceinline__ void unpack(uint4 u, float (&o)[VE]) {
+using word_t = typename Word<static_cast<int>(sizeof(T)) * VE>::type;
+
+// the VE numbers of a pack
+template <typename T, int VE>
+__device__ __forceinline__ void unpack(word_t<T, VE> u, float (&o)[VE]) {
     const Pack<T, VE> k = *reinterpret_cast<const Pack<T, VE>*>(&u);
 #pragma unroll
     for (int i = 0; i < VE; ++i) o[i] = to_f32(k.v[i]);
 }
 template <typename T, int VE>
 __device__ __forceinline__ void load_pack(const T* p, float (&o)[VE]) {
-    if constexpr (VE == 1) {
-        o[0] = to_f32(__ldg(p));
+    unpack<T, VE>(__ldg(reinterpret_cast<const word_t<T, VE>*>(p)), o);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
     } else {
-        const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
-        unpack<T, VE>(u, o);
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
     }
 }
 template <typename T, int VE>
 __device__ __forceinline__ void store_pack(T* p, const float (&o)[VE]) {
     if constexpr (VE == 1) {
         *p = from_f32<T>(o[0]);
+    } else if constexpr (sizeof(T) == 4) {
+        if constexpr (VE == 2) *reinterpret_cast<float2*>(p) = make_float2(o[0], o[1]);
+        else *reinterpret_cast<float4*>(p) = make_float4(o[0], o[1], o[2], o[3]);
+    } else if constexpr (VE == 2) {
+        *reinterpret_cast<uint32_t*>(p) = pack2<T>(o[0], o[1]);
     } else {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if constexpr (VE == 4) {
-                w[i] = __float_as_uint(o[i]);
-            } else if constexpr (sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value) {
-                const __nv_bfloat162 h = __floats2bfloat162_rn(o[2 * i], o[2 * i + 1]);
-                w[i] = *reinterpret_cast<const uint32_t*>(&h);
-            } else {
-                const __half2 h = __floats2half2_rn(o[2 * i], o[2 * i + 1]);
-                w[i] = *reinterpret_cast<const uint32_t*>(&h);
-            }
-        }
-        *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+        *reinterpret_cast<uint4*>(p) =
+            make_uint4(pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3]), pack2<T>(o[4], o[5]), pack2<T>(o[6], o[7]));
     }
 }
 // The codes of four values times `inv` (two products to an instruction, each rounded by itself): plain
@@ -69,8 +85,8 @@ __device__ __forceinline__ uint32_t scaled_codes(float a, float b, float c, floa
 template <int VE, int VPT, int TPR>
 __device__ __forceinline__ void store_codes(const float (&v)[VPT][VE], const Fp8Out& q, int64_t r, int64_t d, bool live,
                                             int64_t first_pack, int lane, bool wide) {
-    constexpr int kPer = VE == 1 ? 4 : 1;                                           // packs of a lane in one group
-    constexpr int kLanes = VE == 1 ? 32 : (kGroup / VE < TPR ? kGroup / VE : TPR);  // lanes of one group
+    constexpr int kPer = VE <= 2 ? 4 / VE : 1;                                      // packs of a lane in one group
+    constexpr int kLanes = VE <= 2 ? 32 : (kGroup / VE < TPR ? kGroup / VE : TPR);  // lanes of one group
     constexpr int kGroups = VPT / kPer;
     static_assert(kGroups <= kLanes, "a lane for each group");
     float am[kGroups];
@@ -119,6 +135,18 @@ __device__ __forceinline__ void store_codes(const float (&v)[VPT][VE], const Fp8
 #pragma unroll
                     for (int h = 0; h < 4; ++h)
                         if (live && c0 + h * 32 < d) dst[h * 32] = static_cast<uint8_t>(w >> (8 * h));
+                }
+            } else if constexpr (VE == 2) {
+                const uint32_t w = scaled_codes<kMend>(v[2 * j][0], v[2 * j][1], v[2 * j + 1][0], v[2 * j + 1][1], inv, odd);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (!live || c0 + h * 64 >= d) continue;
+                    if (wide) {
+                        *reinterpret_cast<uint16_t*>(dst + h * 64) = static_cast<uint16_t>(w >> (16 * h));
+                    } else {
+                        dst[h * 64] = static_cast<uint8_t>(w >> (16 * h));
+                        dst[h * 64 + 1] = static_cast<uint8_t>(w >> (16 * h + 8));
+                    }
                 }
             } else {
                 uint32_t w[VE / 4];

@@ -96,7 +96,7 @@ def _same(q, x, tile):
     assert q.tile == tile and (q.codes.shape[0] < 2 or q.codes.stride(0) % 16 == 0)
 
 
-SHAPES = [(1, 1), (1, 128), (2, 127), (3, 129), (127, 16), (128, 128), (129, 257), (260, 384), (5, 4096), (513, 1000), (300, 7)]
+SHAPES = [(1, 1), (33, 130), (7, 1002), (1, 128), (2, 127), (3, 129), (127, 16), (128, 128), (129, 257), (260, 384), (5, 4096), (513, 1000), (300, 7)]
 
 
 @gpu

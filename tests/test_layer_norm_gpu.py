@@ -48,7 +48,8 @@ def _y_tol(x, g, b, r, xh, dtype):
     return t + ULP[dtype] * (y.abs() + t) + tiny
 
 
-WIDTHS = [1, 2, 3, 31, 64, 127, 128, 129, 256, 511, 771, 1024, 1032, 2048, 4096, 5000, 8192, 16384, 20001]
+WIDTHS = [1, 2, 3, 31, 64, 66, 127, 128, 129, 256, 511, 514, 771, 1024, 1030, 1032, 2048, 2050, 4096, 4098, 5000, 8192, 9998,
+          16384, 20001]
 
 
 @pytest.mark.parametrize("dtype,ptype", [("float32", "float32"), ("bfloat16", "bfloat16"),
@@ -230,7 +231,7 @@ def test_autograd_and_in_place_gradient():
     assert torch.equal(x.grad, dx) and torch.equal(g.grad, dg) and torch.equal(b.grad, db)
 
 
-@pytest.mark.parametrize("d", [64, 100, 128, 129, 771, 1024, 2048, 5000, 16384, 20001])
+@pytest.mark.parametrize("d", [64, 66, 100, 128, 129, 130, 771, 1024, 1030, 2048, 4098, 5000, 9998, 16384, 20001])
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
 def test_fp8_form(d, dtype):
     """Scales to the layer norm's own tolerance; codes as those of the 64-bit y, save where y / scale

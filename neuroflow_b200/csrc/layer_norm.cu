@@ -229,16 +229,18 @@ struct Raw {
 };
 
 constexpr int row_block(int tpr) { return tpr > 128 ? tpr : 128; }
-// Rows of one or two packs a thread are too short to cover their own latency: resident blocks walk over
-// them and fetch a row ahead (131072x128 fp32: 27.0 us, 30.6 with a block for each four rows).  Longer rows
-// are faster with a block each (16384x4096 bf16 to FP8: 65 us, 72 walking).
-constexpr bool walks(int vpt, int tpr) { return tpr <= 32 && vpt <= 2; }
+// With at most 16 elements a thread, resident blocks walk over the rows: the parameters stay in registers
+// (read again for every row, fp32 parameters are twice the bytes of a bf16 row from L1: without any
+// parameters 8191x2048 took 10.4 us against 15.9) and the next row is fetched ahead.  8191x2048 bf16 15.9
+// -> 13.2 us, 65536x512 31.9 -> 26.5, 131072x128 fp32 30.6 -> 26.9.  Wider rows keep 32 elements a thread and a
+// block each (4096x8192 bf16: 34 us, 39 walking).
+constexpr bool walks(int n, int tpr) { return n <= 16 && tpr <= 512; }
 
 template <typename T, int VE, int VPT, int TPR, bool FP8>
 __global__ void __launch_bounds__(row_block(TPR), TPR >= 512 ? 2 : 1) norm_row_kernel(NormArgs a, bool pvec, bool wide) {
     __shared__ float2 red[2][row_block(TPR) / 32];
     constexpr int kRows = row_block(TPR) / TPR, N = VPT * VE;
-    constexpr bool kWalk = walks(VPT, TPR);
+    constexpr bool kWalk = walks(N, TPR);
     const int lane = threadIdx.x & 31, sub = threadIdx.x % TPR;
     // pack j of this thread is first + j * 32 (a row of fewer than 32 threads has one pack a thread)
     const int first = TPR < 32 ? sub : (sub >> 5) * VPT * 32 + lane;
@@ -261,6 +263,21 @@ __global__ void __launch_bounds__(row_block(TPR), TPR >= 512 ? 2 : 1) norm_row_k
     };
     const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
     fetch(static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / TPR);
+    // walking, a thread's columns are the same in every row: their parameters stay in registers
+    constexpr int kHeld = kWalk ? VPT : 1;
+    float gam[kHeld][VE], bet[kHeld][VE];
+    if constexpr (kWalk) {
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            const int c = (first + j * 32) * VE;
+#pragma unroll
+            for (int i = 0; i < VE; ++i) gam[j][i] = bet[j][i] = 0.0f;
+            if (full || c < a.d) {
+                load_params<T, VE>(a.gamma, a.ptype, pvec, c, 1.0f, gam[j]);
+                load_params<T, VE>(a.beta, a.ptype, pvec, c, 0.0f, bet[j]);
+            }
+        }
+    }
     for (int64_t base = static_cast<int64_t>(blockIdx.x) * kRows; base < a.rows; base += step) {
         const int64_t r = base + threadIdx.x / TPR;
         const bool live = r < a.rows;
@@ -313,8 +330,13 @@ __global__ void __launch_bounds__(row_block(TPR), TPR >= 512 ? 2 : 1) norm_row_k
         auto finish = [&](int j) {
             const int c = (first + j * 32) * VE;
             float g[VE], b[VE];
-            load_params<T, VE>(a.gamma, a.ptype, pvec, c, 1.0f, g);
-            load_params<T, VE>(a.beta, a.ptype, pvec, c, 0.0f, b);
+            if constexpr (kWalk) {
+#pragma unroll
+                for (int i = 0; i < VE; ++i) g[i] = gam[j][i], b[i] = bet[j][i];
+            } else {
+                load_params<T, VE>(a.gamma, a.ptype, pvec, c, 1.0f, g);
+                load_params<T, VE>(a.beta, a.ptype, pvec, c, 0.0f, b);
+            }
             if constexpr (VE == 1) {
                 v[j][0] = fmaf(fmaf(v[j][0], rs, off), g[0], b[0]);
             } else {
@@ -348,7 +370,7 @@ cudaError_t norm_row_go(const NormArgs& a, bool pvec, bool wide, cudaStream_t s)
     auto kern = norm_row_kernel<T, VE, VPT, TPR, FP8>;
     const int64_t want = (a.rows + kRows - 1) / kRows;
     int64_t grid = want;
-    if constexpr (walks(VPT, TPR)) {
+    if constexpr (walks(VPT * VE, TPR)) {
         static std::atomic<int> known[64];  // asked for once per kernel and device
         const int d = current_device() & 63;
         int most = known[d].load(std::memory_order_relaxed);
@@ -371,9 +393,9 @@ cudaError_t norm_row(const NormArgs& a, bool pvec, cudaStream_t s) {
     return norm_row_go<T, VE, VPT, TPR, true>(a, pvec, wide, s);
 }
 
-// Threads and packs per row by the width: the fewest threads that leave a thread 32 elements at most, and
-// with packs of one or two elements 8 up to 4,096 columns (more loads to a row than a warp should queue:
-// 5003x771 fp32 takes 19 us with 32).
+// Threads and packs per row by the width: 16 elements a thread up to 4,096 columns and 32 above; with packs
+// of one or two elements 8 up to 4,096 columns (more loads to a row than a warp should queue:
+// 5003x771 fp32 took 19 us with 32).
 template <typename T, int VE>
 cudaError_t norm_width(const NormArgs& a, bool pvec, cudaStream_t s) {
     if constexpr (VE > 2) {
@@ -382,9 +404,9 @@ cudaError_t norm_width(const NormArgs& a, bool pvec, cudaStream_t s) {
         if (a.d <= 32 * VE) return norm_row<T, VE, 1, 32>(a, pvec, s);
         if (a.d <= 64 * VE) return norm_row<T, VE, 2, 32>(a, pvec, s);
         if (a.d <= 512) return norm_row<T, VE, kV / 2, 32>(a, pvec, s);
-        if (a.d <= 1024) return norm_row<T, VE, kV, 32>(a, pvec, s);
+        if (a.d <= 1024) return norm_row<T, VE, kV / 2, 64>(a, pvec, s);
         if (a.d <= 2048) return norm_row<T, VE, kV / 2, 128>(a, pvec, s);
-        if (a.d <= 4096) return norm_row<T, VE, kV, 128>(a, pvec, s);
+        if (a.d <= 4096) return norm_row<T, VE, kV / 2, 256>(a, pvec, s);
         if (a.d <= 8192) return norm_row<T, VE, kV, 256>(a, pvec, s);
         return norm_row<T, VE, kV, 512>(a, pvec, s);
     } else {

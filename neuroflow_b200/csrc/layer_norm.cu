@@ -481,9 +481,11 @@ __device__ __forceinline__ float2 row_sum2(float a, float b, float2 (*red)[32], 
 }
 
 constexpr int grad_block(int tpr) { return tpr > 256 ? tpr : 256; }
+// blocks per SM that the registers are cut for, with e elements a thread
+constexpr int grad_blocks(int e, int tpr) { return tpr > 256 ? 1 : (e > 8 ? 2 : (e > 4 ? 3 : 4)); }
 
 template <typename T, int VE, int VPT, int TPR>
-__global__ void __launch_bounds__(grad_block(TPR), TPR > 256 ? 1 : (VE * VPT > 8 ? 2 : 4))
+__global__ void __launch_bounds__(grad_block(TPR), grad_blocks(VE * VPT, TPR))
 norm_grad_row_kernel(NormGradArgs a, bool pvec) {
     constexpr int kThreads = grad_block(TPR), kRows = kThreads / TPR;
     constexpr bool kShared = TPR == 1024;
@@ -639,23 +641,32 @@ norm_grad_row_kernel(NormGradArgs a, bool pvec) {
     }
 }
 
+// Launches as many blocks as are resident, at most a.parts, and leaves their number there.
 template <typename T, int VE, int VPT, int TPR>
-cudaError_t norm_grad_row(const NormGradArgs& a, bool pvec, cudaStream_t s) {
+cudaError_t norm_grad_row(NormGradArgs& a, bool pvec, cudaStream_t s) {
     auto kern = norm_grad_row_kernel<T, VE, VPT, TPR>;
     const int smem = a.part && (TPR == 1024 || grad_block(TPR) > TPR) ? 2 * VPT * VE * TPR * 4 : 0;
     cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), smem);
     if (e != cudaSuccess) return e;
+    const int resident = grad_blocks(VE * VPT, TPR) * device_sm_count();
+    if (a.parts > resident) a.parts = resident;
     kern<<<a.parts, grad_block(TPR), smem, s>>>(a, pvec);
     return cudaGetLastError();
 }
 
-// Eight elements a thread up to 1,024 columns (four blocks an SM), sixteen above (two; one over 4,096).
+// Eight elements a thread up to 1,024 columns, three blocks an SM (four blocks' registers spilled: 5003x771
+// fp32 17.3 us, 12.9 with three); sixteen and two blocks above, and for 16-bit packs from 257 columns on
+// (65536x512 bf16: 39.6 us, 42.5 with eight).
 template <typename T, int VE>
-cudaError_t norm_grad_width(const NormGradArgs& a, bool pvec, cudaStream_t s) {
+cudaError_t norm_grad_width(NormGradArgs& a, bool pvec, cudaStream_t s) {
     if constexpr (VE == 4) {
         if (a.d <= 128) return norm_grad_row<T, VE, 1, 32>(a, pvec, s);
     }
     if (a.d <= 256) return norm_grad_row<T, VE, 8 / VE, 32>(a, pvec, s);
+    if constexpr (VE == 8) {
+        if (a.d <= 512) return norm_grad_row<T, VE, 2, 32>(a, pvec, s);
+        if (a.d <= 1024) return norm_grad_row<T, VE, 2, 64>(a, pvec, s);
+    }
     if (a.d <= 512) return norm_grad_row<T, VE, 8 / VE, 64>(a, pvec, s);
     if (a.d <= 1024) return norm_grad_row<T, VE, 8 / VE, 128>(a, pvec, s);
     if (a.d <= 2048) return norm_grad_row<T, VE, 16 / VE, 128>(a, pvec, s);
@@ -665,7 +676,7 @@ cudaError_t norm_grad_width(const NormGradArgs& a, bool pvec, cudaStream_t s) {
 }
 
 template <typename T>
-cudaError_t norm_grad_t(const NormGradArgs& a, cudaStream_t s) {
+cudaError_t norm_grad_t(NormGradArgs& a, cudaStream_t s) {
     if (a.rows == 0) return cudaSuccess;
     if (a.d <= 16384) {
         constexpr int VE = 16 / sizeof(T);
@@ -690,8 +701,8 @@ cudaError_t layer_norm_launch(const NormArgs& a, int xtype, cudaStream_t s) {
     return norm_t<__half>(a, s);
 }
 
-// Blocks of the backward kernels, each with its own partial sums: enough to fill the SMs at the
-// kernels' occupancy, few enough that the partial sums stay small against the rows.
+// The most blocks that the backward kernels launch, each with its own partial sums: enough to fill the
+// SMs at the kernels' occupancy, few enough that the partial sums stay small against the rows.
 int layer_norm_parts(int64_t rows, int64_t d) {
     const int64_t per_block = d <= 256 ? 8 : (d <= 512 ? 4 : (d <= 2048 ? 2 : 1));  // rows at a time
     const int64_t cap = (d <= 1024 ? 4ll : (d <= 4096 ? 2ll : 1ll)) * device_sm_count();
@@ -714,7 +725,8 @@ cudaError_t column_reduce_launch(const float* part, int parts, int64_t n, void* 
     return cudaLaunchKernelEx(&cfg, cols == 8 ? column_reduce_kernel<8> : column_reduce_kernel<32>, part, parts, n, out0, out1, otype);
 }
 
-cudaError_t layer_norm_backward_launch(const NormGradArgs& a, int xtype, cudaStream_t s) {
+cudaError_t layer_norm_backward_launch(const NormGradArgs& args, int xtype, cudaStream_t s) {
+    NormGradArgs a = args;
     cudaError_t e = xtype == kF32    ? norm_grad_t<float>(a, s)
                     : xtype == kBF16 ? norm_grad_t<__nv_bfloat16>(a, s)
                                      : norm_grad_t<__half>(a, s);

@@ -244,9 +244,14 @@ constexpr int row_block(int tpr) { return tpr > 128 ? tpr : 128; }
 // -> 13.2 us, 65536x512 31.9 -> 26.5, 131072x128 fp32 30.6 -> 26.9.  Wider rows keep 32 elements a thread and a
 // block each (4096x8192 bf16: 34 us, 39 walking).
 constexpr bool walks(int n, int tpr) { return n <= 16 && tpr <= 512; }
+// Blocks per SM that the registers are cut for: 768 threads walking (16384x4096 bf16 56 -> 50 us against no
+// bound; 1,024 threads spill, 58 us), 1,024 with wide rows (4096x16001 bf16 162 us, 236 with 512).
+constexpr int row_blocks(int vpt, int ve, int tpr) {
+    return walks(vpt * ve, tpr) ? (row_block(tpr) > 384 ? 1 : 768 / row_block(tpr)) : (tpr >= 512 ? 2 : 1);
+}
 
 template <typename T, int VE, int VPT, int TPR, bool FP8>
-__global__ void __launch_bounds__(row_block(TPR), TPR >= 512 ? 2 : 1) norm_row_kernel(NormArgs a, bool pvec, bool wide) {
+__global__ void __launch_bounds__(row_block(TPR), row_blocks(VPT, VE, TPR)) norm_row_kernel(NormArgs a, bool pvec, bool wide) {
     __shared__ float2 red[2][row_block(TPR) / 32];
     constexpr int kRows = row_block(TPR) / TPR, N = VPT * VE;
     constexpr bool kWalk = walks(N, TPR);

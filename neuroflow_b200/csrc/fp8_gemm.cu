@@ -17,7 +17,7 @@
 //                             bias and GELU.  A block of K takes 745 cycles where its MMAs take 512:
 //                             without the sums 670, without TMEM reads too 650 (barrier hand-over)
 //   4096x4096x8192 to fp32    about 195 us with column scales (a second multiply per element)
-//   1x4096x4096               6.4 us, of which 4.9 are the start and the join (1x1024x1024 takes that)
+//   1x4096x4096               6.2 us, of which 4.5 are the start and the join (1x1024x1024 takes that)
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -818,33 +818,35 @@ cudaError_t launch_narrow(const Fp8GemmArgs& p, int split, cudaStream_t stream) 
     return cudaLaunchKernelEx(&cfg, kern, tmW, tmX, p, split);
 }
 
-// Which kernel, and how it is cut.  Both need about half a microsecond a block of K and CTA (pair: 256 x
-// 256 per two SMs, narrow: 128 x NT per CTA), so the time goes by rounds of CTAs times blocks: in blocks,
-//   pair    rounds * (KB + 5) + 10       (a tile's epilogue is worth 5 blocks, the start 10)
-//   narrow  rounds * (KB / split + 5) + 5
-// e.g. 512x4096x4096: narrow 19.6 us, pair 21.2; 1000x4096x1024: 16.8 and 10.5; 1024x1024x16384: 34.6
-// and 63; 2048x2048x2048 only the pair fits one round (14.7 us).
-// NT is the smallest width that holds M (at most 128), narrower still while even the largest split leaves
-// half the SMs without a CTA (64x1024x1024: 6.7 us with NT = 64, 5.5 with 16).  The split doubles while all
-// CTAs fit one round and each keeps two blocks or more (1x4096x4096: 10.7, 8.1, 6.4 us with 1, 2, 4; 7.7
-// with 8, which takes two rounds).
+// Which kernel, and how it is cut: the cheapest by a model fitted to measurements (us, graphs of launches;
+// KB blocks of K, each within 8 % of what was measured over the shapes below).
+//   narrow, NT columns, K over `split` CTAs   4.3 + rounds ceil(KB / split) c(NT) + 2.5 a further round, + join(NT)
+//       c: 0.20, 0.24, 0.32, 0.42 for NT = 16, 32, 64, 128;  join (partials through the cluster): 0.7, 1.0, 1.5, 2.5
+//   pair                                      6.5 + rounds KB 0.41 (0.65 with column scales) + 2.2 a further round
+// E.g. 256x2048x2048: 7.9 with 32/1, 8.4 with 64/2, 8.8 with 128/4; 300x700x6000: 9.9 with 64/4, 11.9 with
+// 128/4; 512x4096x4096: 18.2 with 128/1, 19.6 pair; 1000x4096x1024: 15.9 with 128/1, 9.8 pair; 1x4096x4096: 9.7,
+// 7.4, 6.2, 7.6 with a split of 1, 2, 4, 8.  Clusters of four and eight do not fill the SMs of every
+// processor cluster, hence 128 CTAs at a time there (300x700x6000 with 128/8, 144 CTAs: 16.6).
 template <int CT>
 cudaError_t dispatch(const Fp8GemmArgs& p, cudaStream_t stream) {
-    const int64_t sms = device_sm_count(), KB = (p.K + kBK - 1) / kBK;
-    const int64_t tn = (static_cast<int64_t>(p.N) + 127) / 128;
-    const auto tiles = [&](int nt) { return tn * ((static_cast<int64_t>(p.M) + nt - 1) / nt); };
-    const auto rounds = [](int64_t n, int64_t at_once) { return (n + at_once - 1) / at_once; };
-    int nt = p.M <= 16 ? 16 : (p.M <= 32 ? 32 : (p.M <= 64 ? 64 : 128));
-    int most = 1;
-    while (most < 8 && most * 4 <= KB) most *= 2;
-    while (nt > 16 && tiles(nt) * most * 2 <= sms) nt /= 2;
-    int split = 1;
-    while (split < most && tiles(nt) * split * 2 <= sms) split *= 2;
-    const int64_t wide = ((static_cast<int64_t>(p.M) + 255) / 256) * ((static_cast<int64_t>(p.N) + 255) / 256);
-    const int64_t pair = rounds(wide, sms / 2) * (KB + 5) + 10;
-    const int64_t narrow = rounds(tiles(nt) * split, nt > 64 ? sms : 2 * sms) * ((KB + split - 1) / split + 5) + 5;
-    if (nt == 128 && pair < narrow) return launch_pair<CT>(p, stream);
-    const bool deep = tiles(nt) * split <= sms;
+    const int64_t sms = device_sm_count(), KB = (p.K + kBK - 1) / kBK, M = p.M, N = p.N;
+    const auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+    constexpr int kCost[4] = {20, 24, 32, 42}, kJoin[4] = {70, 100, 150, 250};  // hundredths of a microsecond
+    int nt = 16, split = 1;
+    int64_t best = -1;
+    for (int i = 0; i < 4; ++i) {
+        const int w = 16 << i;
+        if (i > 0 && w / 2 >= M) break;
+        for (int s = 1; s <= 8 && (s == 1 || 2 * s <= KB); s *= 2) {
+            const int64_t ctas = up(N, 128) * up(M, w) * s;
+            const int64_t rounds = up(ctas, s >= 4 ? sms * 7 / 8 : sms);
+            const int64_t cost = 430 + rounds * up(KB, s) * kCost[i] + (rounds - 1) * 250 + (s > 1 ? kJoin[i] : 0);
+            if (best < 0 || cost < best) best = cost, nt = w, split = s;
+        }
+    }
+    const int64_t rounds = up(up(M, 256) * up(N, 256), sms / 2);
+    if (650 + rounds * KB * (p.b_tile ? 41 : 65) + (rounds - 1) * 220 < best) return launch_pair<CT>(p, stream);
+    const bool deep = up(N, 128) * up(M, nt) * split <= sms;
     if (nt == 16) return deep ? launch_narrow<16, CT, true>(p, split, stream) : launch_narrow<16, CT, false>(p, split, stream);
     if (nt == 32) return deep ? launch_narrow<32, CT, true>(p, split, stream) : launch_narrow<32, CT, false>(p, split, stream);
     if (nt == 64) return deep ? launch_narrow<64, CT, true>(p, split, stream) : launch_narrow<64, CT, false>(p, split, stream);

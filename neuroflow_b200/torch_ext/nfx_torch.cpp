@@ -345,7 +345,13 @@ Tensor fp8_linear(const Tensor& x, const Tensor& w, const OptTensor& b) {
     same_device(fn, x, "weight", w);
     int t = 0;
     vector_of(fn, "bias", b, w.size(0), x, &t);
-    return Fp8LinearFn::apply(x, w, b);
+    if (at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad() || (b && b->requires_grad())))
+        return Fp8LinearFn::apply(x, w, b);
+    // no gradient is asked for: no transposed operands
+    const Quantised xq = fp8_quantise(x, false, false, false), wq = fp8_quantise(w, true, false, false);
+    auto sizes = x.sizes().vec();
+    sizes.back() = w.size(0);
+    return fp8_gemm(xq.q.codes, xq.q.scales, false, wq.q.codes, wq.q.scales, true, b, 0, x.scalar_type(), std::nullopt).view(sizes);
 }
 
 py::object or_none(const Tensor& t) { return t.defined() ? py::cast(t) : py::none(); }
@@ -372,6 +378,8 @@ PYBIND11_MODULE(_nfx_torch, m) {
     m.def("fp8_linear", &fp8_linear);
     m.def("layer_norm_autograd", [](const Tensor& x, const OptTensor& g, const OptTensor& b, double eps) {
         norm_of("layer_norm_autograd", x, g, b);
-        return LayerNormFn::apply(x, g, b, eps);
+        const bool grad = x.requires_grad() || (g && g->requires_grad()) || (b && b->requires_grad());
+        if (!grad || !at::GradMode::is_enabled()) return layer_norm(x, g, b, eps, std::nullopt, false).y;
+        return Tensor(LayerNormFn::apply(x, g, b, eps));
     });
 }

@@ -464,3 +464,32 @@ def test_linear_gradients_that_are_not_needed():
             assert (p.grad is None) if not need >> i & 1 else torch.equal(p.grad, f.grad)
     y = ops.fp8_linear(x, w)
     assert not y.requires_grad and torch.equal(y, ops.fp8_linear(x, w, b))
+
+
+@gpu
+def test_without_gradients():
+    """Under no_grad the differentiable forms give the same outputs and record nothing."""
+    torch, ops = _torch()
+    x, w, b = _case(33, 200, torch.float32, 3), _case(70, 200, torch.float32, 4), torch.randn(70, device="cuda")
+    g = torch.ones(200, device="cuda", requires_grad=True)
+    for t in (x, w, b):
+        t.requires_grad_()
+    y, n = ops.fp8_linear(x, w, b), ops.layer_norm_autograd(x, g)
+    assert y.requires_grad and n.requires_grad
+    with torch.no_grad():
+        y2, n2 = ops.fp8_linear(x, w, b), ops.layer_norm_autograd(x, g)
+    assert not y2.requires_grad and not n2.requires_grad
+    assert torch.equal(y, y2) and torch.equal(n, n2)
+    assert torch.equal(n2, ops.layer_norm(x.detach(), g.detach()))
+
+
+@gpu
+def test_refusals_under_autograd():
+    torch, ops = _torch()
+    from neuroflow_b200 import _nfx
+    x = _case(8, 64, torch.float32, 1).requires_grad_()
+    for f in (lambda: ops.fp8_linear(x, torch.zeros(4, 63, device="cuda")), lambda: ops.fp8_linear(x.t(), torch.zeros(4, 8, device="cuda")),
+              lambda: ops.layer_norm_autograd(x, torch.ones(63, device="cuda"))):
+        with pytest.raises(_nfx.NfxError) as ei:
+            f()
+        assert ei.value.code == 1

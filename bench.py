@@ -614,7 +614,11 @@ def main():
         n = os.cpu_count() or 1
         x = inputs(100, max(1, n))
         from oracle.cpu import Reference
-        ref = Reference()
+        try:
+            ref = Reference()
+        except FileNotFoundError:
+            print(json.dumps({"impl": "reference", "unavailable": "oracle/_ref is not built"}), flush=True)
+            return
         for _ in range(args.warmup):
             ref.bench(path, x[:1], CFG["out_channels"], 1, 1)
         t = 0.0
@@ -647,13 +651,16 @@ def main():
                                              (32, 64, 128, 256))
         if ws == 1 and not args.no_cpu_baseline:
             n = os.cpu_count() or 1
-            v, nthr, reps, t1 = cpu_reference(path, x_host, n)
-            result["cpu_baseline"] = {
-                "value": round(v, 3), "unit": UNIT, "cores": nthr, "kind": "reference",
-                "sample": f"{nthr * reps} samples ({nthr} threads x {reps}) of the same "
-                          "workload through the reference InferenceRuntime::Run (fake-quant "
-                          "fp32 FNO2d; the reference has no INT8 FNO2d); single-thread "
-                          f"{t1:.2f} s/sample"}
+            try:
+                v, nthr, reps, t1 = cpu_reference(path, x_host, n)
+                result["cpu_baseline"] = {
+                    "value": round(v, 3), "unit": UNIT, "cores": nthr, "kind": "reference",
+                    "sample": f"{nthr * reps} samples ({nthr} threads x {reps}) of the same "
+                              "workload through the reference InferenceRuntime::Run (fake-quant "
+                              "fp32 FNO2d; the reference has no INT8 FNO2d); single-thread "
+                              f"{t1:.2f} s/sample"}
+            except FileNotFoundError:  # the reference's sources were not there to compile
+                result["cpu_baseline"] = {"unavailable": "oracle/_ref is not built"}
         print(json.dumps(result), flush=True)
     if ws > 1:
         import torch.distributed as dist

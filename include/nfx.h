@@ -356,7 +356,7 @@ int nfx_fp8_e4m3_selfcheck(unsigned long long* mismatches);
  * NFX_INVALID_ARG and a message in nfx_last_error(). */
 enum { NFX_F32 = 0, NFX_BF16 = 1, NFX_F16 = 2 };
 
-/* Layer norm over the last dimension of x (rows, d):
+/* Layer norm over the last dimension of x (rows, d), 1 <= d < 2^31 - 256:
  *   y = (x - mean) rstd gamma + beta,  rstd = 1 / sqrt(var + eps), var the biased variance.
  * y has x's type; gamma and beta (d,) have param_type, NULL: ones and zeros.  mean and rstd
  * (rows,) are written where not NULL (the backward pass reads them).  Statistics in fp32. */

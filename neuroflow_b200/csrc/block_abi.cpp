@@ -33,7 +33,8 @@ const char* norm_check(int x_type, int param_type, int64_t rows, int64_t d, int6
     if (!type_ok(x_type)) return "x_type must be NFX_F32, NFX_BF16 or NFX_F16";
     if (!type_ok(param_type)) return "param_type must be NFX_F32, NFX_BF16 or NFX_F16";
     if (rows < 0 || d < 1) return "rows must be >= 0 and d >= 1";
-    if (d > kIntMax) return "d must be below 2^31";
+    // the kernels for any width add 256 to a 32-bit column index before they compare it with d
+    if (d > kIntMax - 256) return "d must be below 2^31 - 256";
     if (rows > 1 && ldx < d) return "a row stride is smaller than d";
     if (rows > 0 && !x) return "null pointer";
     return nullptr;

@@ -103,3 +103,14 @@ def test_front_end_refuses_cpu_tensors():
             f()
         assert ei.value.code == 1
     assert isinstance(_nfx.NfxError(1, "x"), RuntimeError) and C.sizeof(C.c_int64) == 8
+
+
+def test_layer_norm_widths_that_a_column_index_cannot_step_over():
+    """The kernels for any width step through a row by 256 columns with 32-bit indices: the widest row
+    leaves room for one step beyond its end."""
+    for d in ((1 << 31) - 256, (1 << 31) - 1):
+        _bad(L.nfx_layer_norm(P, 1, d, None, None, 0, 1, d, 1e-5, P, d, None, None, None), "2^31 - 256")
+        _bad(L.nfx_layer_norm_fp8(P, 1, d, None, None, 0, 1, d, 1e-5, P, d, P, 1, 1, None, None, None), "2^31 - 256")
+        _bad(L.nfx_layer_norm_backward(P, d, P, d, 1, P, P, None, 0, 1, d, P, d, None, None, None, 0, None), "2^31 - 256")
+    d = (1 << 31) - 257  # (no rows: nothing is launched)
+    assert L.nfx_layer_norm(None, 1, d, None, None, 0, 0, d, 1e-5, None, d, None, None, None) == 0

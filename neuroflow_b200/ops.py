@@ -11,9 +11,14 @@ quantiser and the FP8 block-scaled product, forward and backward.
 
 Every call runs the kernels of libnfx.so (the C-ABI of include/nfx.h, reached through the compiled
 front-end torch_ext/nfx_torch.cpp) on the current torch stream of the tensors' device, or on `stream`
-(a torch.cuda.Stream or raw handle), without synchronising; outputs are allocated for that stream.  There is no CPU fallback.  Refused
-arguments raise NfxError with code 1 (InvalidArg).  torch.float32, bfloat16 and float16 are
-accepted where a tensor is not FP8; the last dimension has to be contiguous.
+(a torch.cuda.Stream or raw handle), without synchronising; outputs are allocated for that stream.  There is
+no CPU fallback.  Refused arguments raise NfxError with code 1 (InvalidArg).  torch.float32, bfloat16 and
+float16 are accepted where a tensor is not FP8; the last dimension has to be contiguous.
+
+With `stream` the caller orders it behind the work that made the inputs, and other streams behind it where
+they read the outputs (torch.cuda.Stream.wait_stream).  The tensors of the call are recorded on a
+torch.cuda.Stream, so they may be released at once; a raw handle's life is not known to torch, so there the
+caller keeps them until the work is done.
 """
 from __future__ import annotations
 
@@ -55,15 +60,21 @@ def _refuse(fn, what):
 
 
 @contextlib.contextmanager
-def _on(t, stream):
+def _on(stream, t, *others):
     """`stream` (a torch.cuda.Stream or raw handle on t's device) made current, so that what a call
-    allocates belongs to it."""
+    allocates belongs to it; the tensors of the call (t, and the others that are not None) are recorded
+    on a torch.cuda.Stream, so that their memory is not handed out again before it is done with them."""
     if not t.is_cuda:
         _refuse("stream", "the tensors of a call must be CUDA tensors")
-    if not isinstance(stream, torch.cuda.Stream):
+    known = isinstance(stream, torch.cuda.Stream)
+    if not known:
         stream = torch.cuda.ExternalStream(int(stream), device=t.device)
     with torch.cuda.stream(stream):
         yield
+    if known:
+        for u in (t, *others):
+            if u is not None:
+                u.record_stream(stream)
 
 
 def layer_norm(x, gamma=None, beta=None, eps=1e-5, out=None, stats=False, stream=None):
@@ -71,7 +82,7 @@ def layer_norm(x, gamma=None, beta=None, eps=1e-5, out=None, stats=False, stream
     zeros.  y in x's type (in `out` if given); with `stats` also the fp32 mean and 1/std of each
     row, which layer_norm_backward takes: (y, mean, rstd)."""
     if stream is not None:
-        with _on(x, stream):
+        with _on(stream, x, gamma, beta, out):
             return _ext.layer_norm(x, gamma, beta, eps, out, stats)
     return _ext.layer_norm(x, gamma, beta, eps, out, stats)
 
@@ -80,7 +91,7 @@ def layer_norm_fp8(x, gamma=None, beta=None, eps=1e-5, stats=False, stream=None)
     """layer_norm(x) in FP8 groups of 128 (Fp8Blocks over the flattened rows): what fp8_quantise
     makes of an fp32 y, which is never written.  With `stats`: (blocks, mean, rstd)."""
     if stream is not None:
-        with _on(x, stream):
+        with _on(stream, x, gamma, beta):
             return layer_norm_fp8(x, gamma, beta, eps, stats)
     got = _ext.layer_norm_fp8(x, gamma, beta, eps, stats)
     q = Fp8Blocks(got[0], got[1])
@@ -92,7 +103,7 @@ def layer_norm_backward(dy, x, mean, rstd, gamma=None, param_grads=True, stream=
     (dx, dgamma, dbeta), the last two in gamma's type (fp32 without gamma), or None without
     `param_grads`."""
     if stream is not None:
-        with _on(x, stream):
+        with _on(stream, x, dy, mean, rstd, gamma):
             return _ext.layer_norm_backward(dy, x, mean, rstd, gamma, param_grads)
     return _ext.layer_norm_backward(dy, x, mean, rstd, gamma, param_grads)
 
@@ -104,7 +115,7 @@ def fp8_quantise(x, tile=False, transposed=False, col_sums=False, stream=None):
     `col_sums` (without `tile`) also the fp32 sums of x's columns.  Returns Fp8Blocks, or a tuple of
     it and what was asked for, in that order."""
     if stream is not None:
-        with _on(x, stream):
+        with _on(stream, x):
             return fp8_quantise(x, tile, transposed, col_sums)
     codes, scales, other, sums = _ext.fp8_quantise(x, tile, transposed, col_sums)
     q = Fp8Blocks(codes, scales, tile)
@@ -119,7 +130,7 @@ def fp8_gemm(a, b, bias=None, act=0, out_dtype=torch.bfloat16, out=None, stream=
     if not (isinstance(a, Fp8Blocks) and isinstance(b, Fp8Blocks)):
         _refuse("fp8_gemm", "a and b must be Fp8Blocks")
     if stream is not None:
-        with _on(a.codes, stream):
+        with _on(stream, *a[:2], *b[:2], bias, out):
             return _ext.fp8_gemm(*a, *b, bias, act, out_dtype, out)
     return _ext.fp8_gemm(*a, *b, bias, act, out_dtype, out)
 

@@ -69,6 +69,8 @@ def _on(stream, t, *others):
     known = isinstance(stream, torch.cuda.Stream)
     if not known:
         stream = torch.cuda.ExternalStream(int(stream), device=t.device)
+    elif stream.device != t.device:
+        _refuse("stream", f"the stream is on {stream.device}, the tensors are on {t.device}")
     with torch.cuda.stream(stream):
         yield
     if known:

@@ -61,6 +61,15 @@ def test_tensors_of_a_call_are_recorded_on_its_stream(ops):
         assert all(t.on == [st] for t in used)
 
 
+def test_a_stream_of_another_device_is_refused(ops):
+    """It would be made current on its own device, and the call would run on another stream."""
+    from neuroflow_b200 import _nfx
+    for call, used in _calls(ops, Held):
+        with pytest.raises(_nfx.NfxError) as ei:
+            call(Stream("cuda:1"))
+        assert ei.value.code == 1 and "cuda:1" in str(ei.value)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("which", ["layer_norm", "layer_norm_fp8", "layer_norm_backward", "fp8_quantise", "fp8_gemm"])
 def test_inputs_released_while_the_stream_is_busy_keep_their_memory(which):

@@ -24,8 +24,11 @@ namespace {
 
 constexpr int kAnyThreads = 256;
 
+// v, or zero where it is negative; a NaN stays one.
+__device__ __forceinline__ float not_negative(float v) { return v < 0.0f ? 0.0f : v; }
+
 // s / d with d's reciprocal at hand: the product, and one correction by the exact remainder (Markstein's
-// step), which gives back a constant row's value exactly.
+// step), which gives back a constant row's value exactly where the sum s is exact.
 __device__ __forceinline__ float mean_of(float s, float fd, float inv_d) {
     const float q = s * inv_d;
     return fmaf(fmaf(-q, fd, s), inv_d, q);
@@ -336,7 +339,8 @@ __global__ void __launch_bounds__(row_block(TPR), row_blocks(VPT, VE, TPR)) norm
         // the centred values' own mean is what the first sum's rounding left over
         const float2 t = row_sums<TPR>(s1, s, red[1]);
         const float rest = t.x * inv_d, mu = mu0 + rest;
-        const float rs = __frsqrt_rn(fmaf(-rest, rest, t.y * inv_d) + a.eps), off = -rest * rs;
+        // (a constant row of rounded sums can leave this difference below zero)
+        const float rs = __frsqrt_rn(not_negative(fmaf(-rest, rest, t.y * inv_d)) + a.eps), off = -rest * rs;
         if (live && sub == 0) {
             if (a.mean) a.mean[r] = mu;
             if (a.rstd) a.rstd[r] = rs;

@@ -34,14 +34,14 @@ __device__ __forceinline__ float mean_of(float s, float fd, float inv_d) {
     return fmaf(fmaf(-q, fd, s), inv_d, q);
 }
 
-// Sum of v over the block, the same value in every thread.  `red` holds one float per warp.
-__device__ __forceinline__ float block_sum(float v, float* red) {
-    v = warp_sum(v);
-    __syncthreads();  // the previous sum has been read
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+// Sums of (a, b) over the block, the same bits in every thread.  `red` holds one pair per warp.
+__device__ __forceinline__ float2 block_sums(float a, float b, float2* red) {
+    a = warp_sum(a), b = warp_sum(b);
+    __syncthreads();  // the previous sums have been read
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = make_float2(a, b);
     __syncthreads();
-    float t = 0.0f;
-    for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) t += red[w];
+    float2 t = make_float2(0.0f, 0.0f);
+    for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) t.x += red[w].x, t.y += red[w].y;
     return t;
 }
 
@@ -49,26 +49,30 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
 // after the first).
 template <typename T>
 __global__ void __launch_bounds__(kAnyThreads) norm_any_kernel(NormArgs a) {
-    __shared__ float red[kAnyThreads / 32];
+    __shared__ float2 red[kAnyThreads / 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const float fd = static_cast<float>(a.d);
     for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const T* x = static_cast<const T*>(a.x) + r * a.ldx;
         float s = 0.0f;
         for (int i = threadIdx.x; i < a.d; i += kAnyThreads) s += to_f32(x[i]);
-        const float mu = __fdiv_rn(block_sum(s, red), fd);
+        const float mu0 = __fdiv_rn(block_sums(s, 0.0f, red).x, fd);
+        float s1 = 0.0f;
         s = 0.0f;
         for (int i = threadIdx.x; i < a.d; i += kAnyThreads) {
-            const float c = to_f32(x[i]) - mu;
+            const float c = to_f32(x[i]) - mu0;
+            s1 += c;
             s = fmaf(c, c, s);
         }
-        const float rs = __frsqrt_rn(__fdiv_rn(block_sum(s, red), fd) + a.eps);
+        const float2 t = block_sums(s1, s, red);
+        const float rest = __fdiv_rn(t.x, fd);
+        const float rs = __frsqrt_rn(not_negative(fmaf(-rest, rest, __fdiv_rn(t.y, fd))) + a.eps), off = -rest * rs;
         if (threadIdx.x == 0) {
-            if (a.mean) a.mean[r] = mu;
+            if (a.mean) a.mean[r] = mu0 + rest;
             if (a.rstd) a.rstd[r] = rs;
         }
         auto out = [&](int i) {
-            const float xh = (to_f32(x[i]) - mu) * rs;
+            const float xh = fmaf(to_f32(x[i]) - mu0, rs, off);
             const float g = a.gamma ? load_any(a.gamma, a.ptype, i) : 1.0f;
             return fmaf(xh, g, a.beta ? load_any(a.beta, a.ptype, i) : 0.0f);
         };
@@ -101,7 +105,7 @@ __global__ void __launch_bounds__(kAnyThreads) norm_any_kernel(NormArgs a) {
 // in their order, to its own two rows of partial sums (each column always by one thread).
 template <typename T>
 __global__ void __launch_bounds__(kAnyThreads) norm_grad_any_kernel(NormGradArgs a) {
-    __shared__ float red[kAnyThreads / 32];
+    __shared__ float2 red[kAnyThreads / 32];
     const float fd = static_cast<float>(a.d);
     float* pg = a.part + static_cast<int64_t>(blockIdx.x) * a.d;
     float* pb = a.part + (static_cast<int64_t>(a.parts) + blockIdx.x) * a.d;
@@ -122,8 +126,8 @@ __global__ void __launch_bounds__(kAnyThreads) norm_grad_any_kernel(NormGradArgs
                 pb[i] = g + (first ? 0.0f : pb[i]);
             }
         }
-        s1 = __fdiv_rn(block_sum(s1, red), fd);
-        s2 = __fdiv_rn(block_sum(s2, red), fd);
+        const float2 t = block_sums(s1, s2, red);
+        s1 = __fdiv_rn(t.x, fd), s2 = __fdiv_rn(t.y, fd);
         for (int i = threadIdx.x; i < a.d; i += kAnyThreads) {
             const float xh = (to_f32(x[i]) - mu) * rs, g = to_f32(dy[i]);
             const float ga = a.gamma ? g * load_any(a.gamma, a.ptype, i) : g;

@@ -36,8 +36,8 @@ constexpr int kOutBytes = 32 * 128;  // one staging buffer
 
 // GELU as z * sigmoid(2u) (the tanh form's identity), the exponential by ex2.approx.  Two values
 // share a reciprocal, 1 / a = b / (a b) (the special-function unit bounds this epilogue); the
-// exponents are held under 2^60 so that the product stays finite, where z 2^-60 stands for a result
-// that is smaller still.
+// exponents are held under 2^60 so that the product stays finite.  Where that bites, z < -7 or so, the
+// result is under 2^-57 in size and is returned as zero; a NaN stays one and leaves its neighbour alone.
 __device__ __forceinline__ float2 gelu_sig2(float2 z) {
     const float c2 = -2.0f * 0.7978845608028654f * 1.4426950408889634f;
     float2 e;
@@ -45,7 +45,7 @@ __device__ __forceinline__ float2 gelu_sig2(float2 z) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(fminf(ux, 60.0f)));
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(fminf(uy, 60.0f)));
     const float a = 1.0f + e.x, b = 1.0f + e.y, r = __fdividef(1.0f, a * b);
-    return make_float2(z.x * (r * b), z.y * (r * a));
+    return make_float2((ux > 60.0f ? -0.0f : z.x) * (r * b), (uy > 60.0f ? -0.0f : z.y) * (r * a));
 }
 template <int R>
 __device__ __forceinline__ void reg_inc() {

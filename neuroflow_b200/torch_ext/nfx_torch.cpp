@@ -280,6 +280,23 @@ Tensor fp8_gemm(const Tensor& ac, const Tensor& as, bool a_tile, const Tensor& b
 // ---- autograd -----------------------------------------------------------------------------------
 OptTensor defined(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
 
+// The gradients are made by the kernels, without a graph of their own.  Under create_graph a gradient `g`
+// is handed on with this node: differentiating it raises, where without the node the terms that it
+// contributes to a second derivative would just be missing.
+struct OnceFn : torch::autograd::Function<OnceFn> {
+    static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& g, const Tensor& /* requires grad */, const std::string& fn) {
+        ctx->saved_data["fn"] = fn;
+        return g.variable_data();  // (ours alone, and no view: in-place changes of the gradient stay allowed)
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, const torch::autograd::variable_list&) {
+        refuse(ctx->saved_data["fn"].toStringRef().c_str(), "second derivatives are not available");
+    }
+};
+Tensor once(const char* fn, const Tensor& g) {
+    if (!g.defined() || !at::GradMode::is_enabled()) return g;
+    return OnceFn::apply(g, at::empty({0}, at::kFloat).requires_grad_(), std::string(fn));
+}
+
 struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
     static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const OptTensor& gamma, const OptTensor& beta,
                           double eps) {
@@ -296,7 +313,8 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
         const int64_t bt = ctx->saved_data["beta"].toInt();
         Tensor db = g.dbeta;
         if (db.defined() && bt >= 0) db = db.to(static_cast<at::ScalarType>(bt));
-        return {g.dx, saved[1].defined() ? g.dgamma : Tensor(), bt >= 0 ? db : Tensor(), Tensor()};
+        const char* fn = "layer_norm_autograd";
+        return {once(fn, g.dx), saved[1].defined() ? once(fn, g.dgamma) : Tensor(), bt >= 0 ? once(fn, db) : Tensor(), Tensor()};
     }
 };
 
@@ -332,7 +350,8 @@ struct Fp8LinearFn : torch::autograd::Function<Fp8LinearFn> {
         if (need_dx)
             dx = fp8_gemm(q.q.codes, q.q.scales, false, saved[2], saved[3], true, std::nullopt, 0,
                           static_cast<at::ScalarType>(types[0]), std::nullopt).view(ctx->saved_data["x"].toIntVector());
-        return {dx, dw, q.sums};
+        const char* fn = "fp8_linear";
+        return {once(fn, dx), once(fn, dw), once(fn, q.sums)};
     }
 };
 

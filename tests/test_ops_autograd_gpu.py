@@ -1,0 +1,54 @@
+"""What the differentiable operators do beyond a first backward pass: they refuse what they cannot do,
+instead of leaving terms out."""
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+def _inputs():
+    import torch
+    from neuroflow_b200 import ops
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    rnd = lambda *s: torch.randn(*s, generator=gen, device="cuda")
+    x, w, b, g = rnd(24, 160), rnd(48, 160) / 12, rnd(48), 1 + 0.1 * rnd(160)
+    return torch, ops, x, w, b, g
+
+
+def _forms(ops, w, b, g):
+    return [lambda x: ops.fp8_linear(x, w, b), lambda x: ops.layer_norm_autograd(x, g, g)]
+
+
+def test_second_derivatives_are_refused():
+    """A gradient made under create_graph has no graph of its own: differentiating it is an error, and not a
+    missing term.  What does not differentiate it works."""
+    torch, ops, x, w, b, g = _inputs()
+    from neuroflow_b200 import _nfx
+    for t in (x, w, b, g):
+        t.requires_grad_()
+    for f, params in zip(_forms(ops, w, b, g), ((x, w, b), (x, g))):
+        first = torch.autograd.grad((f(x) ** 2).sum(), params)
+        for i in range(len(params)):
+            y = f(x)
+            grads = torch.autograd.grad((y ** 2).sum(), params, create_graph=True)
+            assert all(torch.equal(p.detach(), q) for p, q in zip(grads, first))
+            with pytest.raises(_nfx.NfxError) as ei:
+                (y.sum() + (grads[i] ** 2).sum()).backward()
+            assert ei.value.code == 1 and "second" in str(ei.value)
+        y = f(x)
+        torch.autograd.grad(y.sum(), params, create_graph=True)
+        y.sum().backward()
+        assert x.grad is not None
+        x.grad = None
+
+
+def test_gradients_made_under_create_graph_can_be_changed_in_place():
+    torch, ops, x, w, b, g = _inputs()
+    for t in (x, w, b, g):
+        t.requires_grad_()
+    for f, params in zip(_forms(ops, w, b, g), ((x, w, b), (x, g))):
+        f(x).sum().backward(create_graph=True)
+        for p in params:
+            with torch.no_grad():
+                p.grad.mul_(0.5)
+                p.grad.zero_()
+            p.grad = None

@@ -140,7 +140,7 @@ def fp8_gemm(a, b, bias=None, act=0, out_dtype=torch.bfloat16, out=None, stream=
 # ---- under autograd -------------------------------------------------------------------------
 def layer_norm_autograd(x, gamma=None, beta=None, eps=1e-5):
     """layer_norm as a differentiable function of x, gamma and beta (once: differentiating a gradient made
-    under create_graph raises)."""
+    under create_graph raises, as does a tangent of forward mode)."""
     return _ext.layer_norm_autograd(x, gamma, beta, eps)
 
 
@@ -149,5 +149,5 @@ def fp8_linear(x, weight, bias=None):
     128 along K, weight (N, K) in 128 x 128 tiles; the gradient dy in groups along N for dx and, with x,
     in groups along the tokens for the weight gradient.  Gradients pass through the rounding to FP8
     unchanged; they come in the types of x, weight and bias, the output in x's.  Differentiable once:
-    differentiating a gradient made under create_graph raises."""
+    differentiating a gradient made under create_graph raises, as does a tangent of forward mode."""
     return _ext.fp8_linear(x, weight, bias)

@@ -280,6 +280,14 @@ Tensor fp8_gemm(const Tensor& ac, const Tensor& as, bool a_tile, const Tensor& b
 // ---- autograd -----------------------------------------------------------------------------------
 OptTensor defined(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
 
+// A tangent of forward mode (a tensor has one whether or not it requires grad) would be dropped.
+void no_tangent(const char* fn, const Tensor& t) {
+    if (t._fw_grad(/*level=*/0).defined()) refuse(fn, "forward-mode differentiation is not available");
+}
+void no_tangent(const char* fn, const OptTensor& t) {
+    if (t) no_tangent(fn, *t);
+}
+
 // The gradients are made by the kernels, without a graph of their own.  Under create_graph a gradient `g`
 // is handed on with this node: differentiating it raises, where without the node the terms that it
 // contributes to a second derivative would just be missing.
@@ -364,6 +372,7 @@ Tensor fp8_linear(const Tensor& x, const Tensor& w, const OptTensor& b) {
     same_device(fn, x, "weight", w);
     int t = 0;
     vector_of(fn, "bias", b, w.size(0), x, &t);
+    no_tangent(fn, x), no_tangent(fn, w), no_tangent(fn, b);
     if (at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad() || (b && b->requires_grad())))
         return Fp8LinearFn::apply(x, w, b);
     // no gradient is asked for: no transposed operands
@@ -396,7 +405,9 @@ PYBIND11_MODULE(_nfx_torch, m) {
     m.def("fp8_gemm", &fp8_gemm);
     m.def("fp8_linear", &fp8_linear);
     m.def("layer_norm_autograd", [](const Tensor& x, const OptTensor& g, const OptTensor& b, double eps) {
-        norm_of("layer_norm_autograd", x, g, b);
+        const char* fn = "layer_norm_autograd";
+        norm_of(fn, x, g, b);
+        no_tangent(fn, x), no_tangent(fn, g), no_tangent(fn, b);
         const bool grad = x.requires_grad() || (g && g->requires_grad()) || (b && b->requires_grad());
         if (!grad || !at::GradMode::is_enabled()) return layer_norm(x, g, b, eps, std::nullopt, false).y;
         return Tensor(LayerNormFn::apply(x, g, b, eps));

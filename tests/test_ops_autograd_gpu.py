@@ -52,3 +52,25 @@ def test_gradients_made_under_create_graph_can_be_changed_in_place():
                 p.grad.mul_(0.5)
                 p.grad.zero_()
             p.grad = None
+
+
+def test_forward_mode_is_refused():
+    """A tangent would be dropped without a word; also where no gradient is asked for."""
+    torch, ops, x, w, b, g = _inputs()
+    from neuroflow_b200 import _nfx
+    import torch.autograd.forward_ad as fw
+    with fw.dual_level():
+        dual = lambda t: fw.make_dual(t, torch.ones_like(t))
+        calls = [lambda: ops.fp8_linear(dual(x), w, b), lambda: ops.fp8_linear(x, dual(w), b),
+                 lambda: ops.fp8_linear(x, w, dual(b)), lambda: ops.layer_norm_autograd(dual(x), g),
+                 lambda: ops.layer_norm_autograd(x, dual(g)), lambda: ops.layer_norm_autograd(x, g, dual(g))]
+        for needs in (False, True):
+            w.requires_grad_(needs), g.requires_grad_(needs)
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad):
+                    for i, call in enumerate(calls):
+                        with pytest.raises(_nfx.NfxError) as ei:
+                            call()
+                        assert ei.value.code == 1 and "forward-mode" in str(ei.value), i
+    w.requires_grad_(False)
+    assert ops.fp8_linear(x, w, b).shape == (24, 48)

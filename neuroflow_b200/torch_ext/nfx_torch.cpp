@@ -94,6 +94,11 @@ Tensor empty(at::IntArrayRef sizes, at::ScalarType t, const Tensor& like) {
 }
 void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
 
+// A call has written into its `out`: a backward pass that saved the buffer finds out by its version.
+void written(const OptTensor& out) {
+    if (out && !out->is_inference()) out->unsafeGetTensorImpl()->bump_version();
+}
+
 // Codes whose rows start on 16-byte boundaries, and scales with the block index outermost (the order in
 // which the product reads them).
 struct Fp8 {
@@ -155,6 +160,7 @@ NormOut layer_norm(const Tensor& x, const OptTensor& gamma, const OptTensor& bet
     if (stats) st = stats_of(x);
     check(nfx_layer_norm(x.const_data_ptr(), n.xt, n.x.ld, n.g, n.b, n.pt, n.x.rows, n.x.cols, static_cast<float>(eps),
                          y.data_ptr(), ldy, ptr(st.first), ptr(st.second), stream_of(x)));
+    written(out);
     return {y, st.first, st.second};
 }
 
@@ -274,6 +280,7 @@ Tensor fp8_gemm(const Tensor& ac, const Tensor& as, bool a_tile, const Tensor& b
     if (!out) c = empty({a.rows, b.rows}, out_dtype, ac);
     check(nfx_fp8_gemm(a.codes, a.ld, a.scales, a.srs, a.sbs, a_tile, b.codes, b.ld, b.scales, b.srs, b.sbs, b_tile, a.rows, b.rows,
                        a.k, bp, bt, static_cast<int>(act), c.data_ptr(), type_of(c.scalar_type()), ldc, stream_of(ac)));
+    written(out);
     return c;
 }
 

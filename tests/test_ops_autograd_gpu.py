@@ -74,3 +74,26 @@ def test_forward_mode_is_refused():
                         assert ei.value.code == 1 and "forward-mode" in str(ei.value), i
     w.requires_grad_(False)
     assert ops.fp8_linear(x, w, b).shape == (24, 48)
+
+
+def _outs(ops, x, w, g):
+    a, q = ops.fp8_quantise(x), ops.fp8_quantise(w, tile=True)
+    return [((24, 160), lambda out: ops.layer_norm(x, g, out=out)), ((24, 48), lambda out: ops.fp8_gemm(a, q, out=out))]
+
+
+def test_writing_into_out_is_seen_by_autograd():
+    """A buffer that a backward pass has saved is changed: the backward pass says so."""
+    torch, ops, x, w, b, g = _inputs()
+    p = torch.ones((), device="cuda", requires_grad=True)
+    for shape, call in _outs(ops, x, w, g):
+        buf = torch.ones(shape, device="cuda")
+        h = (buf * p).sum()
+        version = buf._version
+        assert call(buf) is buf
+        assert buf._version > version
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            h.backward()
+        with torch.inference_mode():
+            call(torch.ones(shape, device="cuda"))
+            inside = torch.ones(shape, device="cuda")
+        call(inside)

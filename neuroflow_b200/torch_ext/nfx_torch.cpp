@@ -94,6 +94,10 @@ Tensor empty(at::IntArrayRef sizes, at::ScalarType t, const Tensor& like) {
 }
 void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
 
+// `out` is written by the kernels, which autograd does not see.
+void no_grad_out(const char* fn, const OptTensor& out) {
+    if (out && out->requires_grad() && at::GradMode::is_enabled()) refuse(fn, "out must not be a tensor that requires grad");
+}
 // A call has written into its `out`: a backward pass that saved the buffer finds out by its version.
 void written(const OptTensor& out) {
     if (out && !out->is_inference()) out->unsafeGetTensorImpl()->bump_version();
@@ -153,6 +157,7 @@ NormOut layer_norm(const Tensor& x, const OptTensor& gamma, const OptTensor& bet
         if (y.sizes() != x.sizes() || y.scalar_type() != x.scalar_type() || y.device() != x.device())
             refuse(fn, "out must have x's shape, type and device");
         ldy = rows_of(fn, "out", y).ld;
+        no_grad_out(fn, out);
     } else {
         y = empty(x.sizes(), x.scalar_type(), x);
     }
@@ -273,6 +278,7 @@ Tensor fp8_gemm(const Tensor& ac, const Tensor& as, bool a_tile, const Tensor& b
         if (c.dim() != 2 || c.size(0) != a.rows || c.size(1) != b.rows)
             refuse(fn, "out must be (" + std::to_string(a.rows) + ", " + std::to_string(b.rows) + ")");
         ldc = rows_of(fn, "out", c).ld;
+        no_grad_out(fn, out);
     } else if (type_of(out_dtype) < 0) {
         refuse(fn, std::string("out_dtype must be float32, bfloat16 or float16, not ") + c10::toString(out_dtype));
     }

@@ -97,3 +97,18 @@ def test_writing_into_out_is_seen_by_autograd():
             call(torch.ones(shape, device="cuda"))
             inside = torch.ones(shape, device="cuda")
         call(inside)
+
+
+def test_out_that_requires_grad_is_refused():
+    torch, ops, x, w, b, g = _inputs()
+    from neuroflow_b200 import _nfx
+    for shape, call in _outs(ops, x, w, g):
+        buf = torch.zeros(shape, device="cuda", requires_grad=True)
+        with pytest.raises(_nfx.NfxError) as ei:
+            call(buf)
+        assert ei.value.code == 1 and "requires grad" in str(ei.value)
+        torch.cuda.synchronize()
+        assert not buf.detach().any()
+        with torch.no_grad():
+            call(buf)
+        assert buf.detach().any()

@@ -267,6 +267,7 @@ Tensor fp8_gemm(const Tensor& ac, const Tensor& as, bool a_tile, const Tensor& b
     const Operand a = operand_of(fn, "a", ac, as, a_tile), b = operand_of(fn, "b", bc, bs, b_tile);
     if (a.k != b.k) refuse(fn, "a has " + std::to_string(a.k) + " columns and b " + std::to_string(b.k));
     same_device(fn, ac, "b", bc);
+    if (act < 0 || act > 2) refuse(fn, "act must be 0, 1 or 2");
     int bt = NFX_F32;
     const void* bp = vector_of(fn, "bias", bias, b.rows, ac, &bt);
     Tensor c;

@@ -112,3 +112,13 @@ def test_out_that_requires_grad_is_refused():
         with torch.no_grad():
             call(buf)
         assert buf.detach().any()
+
+
+def test_activation_numbers_are_not_cut_to_32_bits():
+    torch, ops, x, w, b, g = _inputs()
+    from neuroflow_b200 import _nfx
+    a, q = ops.fp8_quantise(x), ops.fp8_quantise(w, tile=True)
+    for act in (1 << 32, (1 << 32) + 1, -1, 3):
+        with pytest.raises(_nfx.NfxError) as ei:
+            ops.fp8_gemm(a, q, act=act)
+        assert ei.value.code == 1

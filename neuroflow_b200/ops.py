@@ -81,7 +81,7 @@ def _on(stream, t, *others):
 
 def layer_norm(x, gamma=None, beta=None, eps=1e-5, out=None, stats=False, stream=None):
     """Layer norm over the last dimension of x (..., d); gamma and beta (d,), None for ones and
-    zeros.  y in x's type (in `out` if given); with `stats` also the fp32 mean and 1/std of each
+    zeros.  y in x's type (in `out` if given, which may be x); with `stats` also the fp32 mean and 1/std of each
     row, which layer_norm_backward takes: (y, mean, rstd)."""
     if stream is not None:
         with _on(stream, x, gamma, beta, out):

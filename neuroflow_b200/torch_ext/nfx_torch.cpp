@@ -6,6 +6,7 @@
 // Refused arguments raise neuroflow_b200._nfx.NfxError with status 1 (InvalidArg) before anything is
 // launched; errors of the C-ABI raise it with theirs.
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -157,6 +158,8 @@ NormOut layer_norm(const Tensor& x, const OptTensor& gamma, const OptTensor& bet
         if (y.sizes() != x.sizes() || y.scalar_type() != x.scalar_type() || y.device() != x.device())
             refuse(fn, "out must have x's shape, type and device");
         ldy = rows_of(fn, "out", y).ld;
+        // (rows are read and written by different blocks; x itself is fine, its rows are read before they are written)
+        if (at::get_overlap_status(x, y) == at::MemOverlapStatus::Partial) refuse(fn, "out shares a part of x's memory");
         no_grad_out(fn, out);
     } else {
         y = empty(x.sizes(), x.scalar_type(), x);

@@ -122,3 +122,20 @@ def test_activation_numbers_are_not_cut_to_32_bits():
         with pytest.raises(_nfx.NfxError) as ei:
             ops.fp8_gemm(a, q, act=act)
         assert ei.value.code == 1
+
+
+def test_out_may_be_x_but_not_a_part_of_its_memory():
+    torch, ops, x, w, b, g = _inputs()
+    from neuroflow_b200 import _nfx
+    want = ops.layer_norm(x, g)
+    hold = torch.empty(x.numel() + 160, device="cuda")
+    xs, shifted = hold[:x.numel()].view_as(x), hold[160:].view_as(x)
+    xs.copy_(x)
+    with pytest.raises(_nfx.NfxError) as ei:
+        ops.layer_norm(xs, g, out=shifted)
+    assert ei.value.code == 1
+    assert torch.equal(ops.layer_norm(xs, g, out=xs), want) and torch.equal(xs, want)
+    # side by side in wider rows: no element is shared
+    wide = torch.empty(24, 320, device="cuda")
+    wide[:, :160] = x
+    assert torch.equal(ops.layer_norm(wide[:, :160], g, out=wide[:, 160:]), want)

@@ -14,6 +14,7 @@ import concurrent.futures as cf
 import os
 import subprocess
 import sys
+from importlib import metadata
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -76,7 +77,13 @@ TORCH_EXT = os.path.join(PKG, "_nfx_torch.so")
 
 def _build_torch() -> None:
     """The compiled torch front-end of neuroflow_b200.ops (a Python module next to libnfx.so), with the
-    headers and libraries of the installed torch."""
+    headers and libraries of the installed torch; left out where torch is not installed (libnfx.so does not
+    need it)."""
+    try:
+        metadata.version("torch")
+    except metadata.PackageNotFoundError:
+        print("torch is not installed: without _nfx_torch.so (neuroflow_b200.ops)", file=sys.stderr)
+        return
     hdr = os.path.join(ROOT, "include", "nfx.h")
     if os.path.exists(TORCH_EXT) and os.path.getmtime(TORCH_EXT) >= max(os.path.getmtime(TORCH_SRC), os.path.getmtime(hdr)):
         return

@@ -1,0 +1,41 @@
+"""When the torch front-end (_nfx_torch.so) is built, with a stand-in for the compiler."""
+import os
+import subprocess
+
+import pytest
+
+
+@pytest.fixture
+def front(monkeypatch, tmp_path):
+    """(the build module, the list of compiler calls) with outputs under tmp_path."""
+    from neuroflow_b200 import build as nb
+    calls = []
+
+    def run(cmd, **kw):
+        calls.append(cmd)
+        with open(cmd[cmd.index("-o") + 1], "w") as f:
+            f.write("built")
+        return subprocess.CompletedProcess(cmd, 0, "", "")
+
+    monkeypatch.setattr(nb, "TORCH_EXT", str(tmp_path / "_nfx_torch.so"))
+    monkeypatch.setattr(nb.subprocess, "run", run)
+    monkeypatch.setattr(nb, "TORCH_STAMP", str(tmp_path / "stamp"), raising=False)
+    return nb, calls
+
+
+def test_no_torch_no_front_end(front, monkeypatch, capsys):
+    """libnfx.so and the command line do not need torch, and neither does their build."""
+    import importlib.metadata as md
+    nb, calls = front
+    version = md.version
+
+    def none(name):
+        if name == "torch":
+            raise md.PackageNotFoundError(name)
+        return version(name)
+
+    monkeypatch.setattr(md, "version", none)
+    monkeypatch.setitem(__import__("sys").modules, "torch", None)
+    nb._build_torch()
+    assert not calls and not os.path.exists(nb.TORCH_EXT)
+    assert "torch" in capsys.readouterr().err

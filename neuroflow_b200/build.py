@@ -73,6 +73,7 @@ def build(verbose: bool = False) -> str:
 
 TORCH_SRC = os.path.join(PKG, "torch_ext", "nfx_torch.cpp")
 TORCH_EXT = os.path.join(PKG, "_nfx_torch.so")
+TORCH_STAMP = os.path.join(OBJ, "_nfx_torch.made_for")  # the torch and Python that TORCH_EXT was built with
 
 
 def _build_torch() -> None:
@@ -80,12 +81,13 @@ def _build_torch() -> None:
     headers and libraries of the installed torch; left out where torch is not installed (libnfx.so does not
     need it)."""
     try:
-        metadata.version("torch")
+        made_for = f"torch {metadata.version('torch')} {sys.implementation.cache_tag}"
     except metadata.PackageNotFoundError:
         print("torch is not installed: without _nfx_torch.so (neuroflow_b200.ops)", file=sys.stderr)
         return
     hdr = os.path.join(ROOT, "include", "nfx.h")
-    if os.path.exists(TORCH_EXT) and os.path.getmtime(TORCH_EXT) >= max(os.path.getmtime(TORCH_SRC), os.path.getmtime(hdr)):
+    if (os.path.exists(TORCH_EXT) and os.path.getmtime(TORCH_EXT) >= max(os.path.getmtime(TORCH_SRC), os.path.getmtime(hdr))
+            and os.path.exists(TORCH_STAMP) and open(TORCH_STAMP).read() == made_for):
         return
     import sysconfig
 
@@ -101,6 +103,8 @@ def _build_torch() -> None:
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"torch front-end build failed:\n{r.stdout}\n{r.stderr}")
+    with open(TORCH_STAMP, "w") as f:
+        f.write(made_for)
 
 
 CLI_SRC = os.path.join(PKG, "cli", "nflow_infer.cpp")

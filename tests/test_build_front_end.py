@@ -39,3 +39,20 @@ def test_no_torch_no_front_end(front, monkeypatch, capsys):
     nb._build_torch()
     assert not calls and not os.path.exists(nb.TORCH_EXT)
     assert "torch" in capsys.readouterr().err
+
+
+def test_another_torch_builds_it_again(front, monkeypatch):
+    """The binary is made for one version of torch's C++ interface."""
+    import importlib.metadata as md
+    nb, calls = front
+    version, torch_is = md.version, ["2.11.0"]
+    monkeypatch.setattr(md, "version", lambda n: torch_is[0] if n == "torch" else version(n))
+    nb._build_torch()
+    assert len(calls) == 1
+    nb._build_torch()
+    assert len(calls) == 1
+    torch_is[0] = "2.12.0"
+    nb._build_torch()
+    assert len(calls) == 2
+    nb._build_torch()
+    assert len(calls) == 2

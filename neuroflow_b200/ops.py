@@ -28,7 +28,12 @@ from typing import NamedTuple
 import torch
 
 from . import _nfx  # the library itself, with a clear message where it has not been built
-from . import _nfx_torch as _ext
+
+try:
+    from . import _nfx_torch as _ext
+except ImportError as e:
+    raise ImportError("the torch front-end _nfx_torch.so is missing or was built for another torch: build it "
+                      "(python -m neuroflow_b200.build, or __graft_entry__.build())") from e
 
 E4M3 = torch.float8_e4m3fn
 GROUP = 128

@@ -56,3 +56,15 @@ def test_another_torch_builds_it_again(front, monkeypatch):
     assert len(calls) == 2
     nb._build_torch()
     assert len(calls) == 2
+
+
+def test_ops_without_the_front_end_says_what_to_do(monkeypatch):
+    import importlib
+    import sys
+    import neuroflow_b200
+    import neuroflow_b200.ops  # noqa: F401
+    monkeypatch.setitem(sys.modules, "neuroflow_b200._nfx_torch", None)
+    monkeypatch.delattr(neuroflow_b200, "_nfx_torch", raising=False)
+    monkeypatch.delitem(sys.modules, "neuroflow_b200.ops")
+    with pytest.raises(ImportError, match="neuroflow_b200.build"):
+        importlib.import_module("neuroflow_b200.ops")

@@ -171,6 +171,20 @@ def cpu_reference(path: str, x: np.ndarray, nthreads: int, target_s: float = 8.0
     return n * reps / wall, n, reps, t1
 
 
+def cpu_baseline(path: str, x: np.ndarray):
+    """The line's "cpu_baseline" entry; without the compiled reference (its sources were not there to
+    compile) the entry says so."""
+    from oracle import cpu
+    if not os.path.exists(cpu.REF_SO):
+        return {"unavailable": "oracle/_ref is not built"}
+    v, nthr, reps, t1 = cpu_reference(path, x, os.cpu_count() or 1)
+    return {"value": round(v, 3), "unit": UNIT, "cores": nthr, "kind": "reference",
+            "sample": f"{nthr * reps} samples ({nthr} threads x {reps}) of the same "
+                      "workload through the reference InferenceRuntime::Run (fake-quant "
+                      "fp32 FNO2d; the reference has no INT8 FNO2d); single-thread "
+                      f"{t1:.2f} s/sample"}
+
+
 def gemm_rows(device, Ms, Ks):
     """configs[1] GEMM cases: achieved GB/s of nfx_int8_gemm (bias and bias + GELU).
     Each case rotates over enough distinct A / C buffers that every launch reads and
@@ -650,17 +664,7 @@ def main():
             result["gemm_sweep"] = gemm_rows(torch.device("cuda", local), (65536, 1 << 20),
                                              (32, 64, 128, 256))
         if ws == 1 and not args.no_cpu_baseline:
-            n = os.cpu_count() or 1
-            try:
-                v, nthr, reps, t1 = cpu_reference(path, x_host, n)
-                result["cpu_baseline"] = {
-                    "value": round(v, 3), "unit": UNIT, "cores": nthr, "kind": "reference",
-                    "sample": f"{nthr * reps} samples ({nthr} threads x {reps}) of the same "
-                              "workload through the reference InferenceRuntime::Run (fake-quant "
-                              "fp32 FNO2d; the reference has no INT8 FNO2d); single-thread "
-                              f"{t1:.2f} s/sample"}
-            except FileNotFoundError:  # the reference's sources were not there to compile
-                result["cpu_baseline"] = {"unavailable": "oracle/_ref is not built"}
+            result["cpu_baseline"] = cpu_baseline(path, x_host)
         print(json.dumps(result), flush=True)
     if ws > 1:
         import torch.distributed as dist

@@ -250,18 +250,18 @@ constexpr int row_block(int tpr) { return tpr > 128 ? tpr : 128; }
 // parameters 8191x2048 took 10.4 us against 15.9) and the next row is fetched ahead.  8191x2048 bf16 15.9
 // -> 13.2 us, 65536x512 31.9 -> 26.5, 131072x128 fp32 30.6 -> 26.9.  Wider rows keep 32 elements a thread and a
 // block each (4096x8192 bf16: 34 us, 39 walking).
-constexpr bool walks(int n, int tpr) { return n <= 16 && tpr <= 512; }
+constexpr bool walks(int n) { return n <= 16; }
 // Blocks per SM that the registers are cut for: 768 threads walking (16384x4096 bf16 56 -> 50 us against no
 // bound; 1,024 threads spill, 58 us), 1,024 with wide rows (4096x16001 bf16 162 us, 236 with 512).
 constexpr int row_blocks(int vpt, int ve, int tpr) {
-    return walks(vpt * ve, tpr) ? (row_block(tpr) > 384 ? 1 : 768 / row_block(tpr)) : (tpr >= 512 ? 2 : 1);
+    return walks(vpt * ve) ? (row_block(tpr) > 384 ? 1 : 768 / row_block(tpr)) : (tpr >= 512 ? 2 : 1);
 }
 
 template <typename T, int VE, int VPT, int TPR, bool FP8>
 __global__ void __launch_bounds__(row_block(TPR), row_blocks(VPT, VE, TPR)) norm_row_kernel(NormArgs a, bool pvec, bool wide) {
     __shared__ float2 red[2][row_block(TPR) / 32];
     constexpr int kRows = row_block(TPR) / TPR, N = VPT * VE;
-    constexpr bool kWalk = walks(N, TPR);
+    constexpr bool kWalk = walks(N);
     const int lane = threadIdx.x & 31, sub = threadIdx.x % TPR;
     // pack j of this thread is first + j * 32 (a row of fewer than 32 threads has one pack a thread)
     const int first = TPR < 32 ? sub : (sub >> 5) * VPT * 32 + lane;
@@ -392,7 +392,7 @@ cudaError_t norm_row_go(const NormArgs& a, bool pvec, bool wide, cudaStream_t s)
     auto kern = norm_row_kernel<T, VE, VPT, TPR, FP8>;
     const int64_t want = (a.rows + kRows - 1) / kRows;
     int64_t grid = want;
-    if constexpr (walks(VPT * VE, TPR)) {
+    if constexpr (walks(VPT * VE)) {
         static std::atomic<int> known[64];  // asked for once per kernel and device
         const int d = current_device() & 63;
         int most = known[d].load(std::memory_order_relaxed);
@@ -425,7 +425,9 @@ cudaError_t norm_width(const NormArgs& a, bool pvec, cudaStream_t s) {
         if (a.d <= 16 * VE) return norm_row<T, VE, 1, 16>(a, pvec, s);
         if (a.d <= 32 * VE) return norm_row<T, VE, 1, 32>(a, pvec, s);
         if (a.d <= 64 * VE) return norm_row<T, VE, 2, 32>(a, pvec, s);
-        if (a.d <= 512) return norm_row<T, VE, kV / 2, 32>(a, pvec, s);
+        if constexpr (VE == 4) {  // (packs of eight are there with two of them)
+            if (a.d <= 512) return norm_row<T, VE, 4, 32>(a, pvec, s);
+        }
         if (a.d <= 1024) return norm_row<T, VE, kV / 2, 64>(a, pvec, s);
         if (a.d <= 2048) return norm_row<T, VE, kV / 2, 128>(a, pvec, s);
         if (a.d <= 4096) return norm_row<T, VE, kV / 2, 256>(a, pvec, s);
@@ -679,9 +681,10 @@ cudaError_t norm_grad_width(NormGradArgs& a, bool pvec, cudaStream_t s) {
     if constexpr (VE == 8) {
         if (a.d <= 512) return norm_grad_row<T, VE, 2, 32>(a, pvec, s);
         if (a.d <= 1024) return norm_grad_row<T, VE, 2, 64>(a, pvec, s);
+    } else {
+        if (a.d <= 512) return norm_grad_row<T, VE, 8 / VE, 64>(a, pvec, s);
+        if (a.d <= 1024) return norm_grad_row<T, VE, 8 / VE, 128>(a, pvec, s);
     }
-    if (a.d <= 512) return norm_grad_row<T, VE, 8 / VE, 64>(a, pvec, s);
-    if (a.d <= 1024) return norm_grad_row<T, VE, 8 / VE, 128>(a, pvec, s);
     if (a.d <= 2048) return norm_grad_row<T, VE, 16 / VE, 128>(a, pvec, s);
     if (a.d <= 4096) return norm_grad_row<T, VE, 16 / VE, 256>(a, pvec, s);
     if (a.d <= 8192) return norm_grad_row<T, VE, 16 / VE, 512>(a, pvec, s);

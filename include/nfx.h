@@ -415,6 +415,11 @@ int nfx_fp8_gemm(const uint8_t* A, int64_t lda, const float* scale_a, int64_t sc
                  int64_t K, const void* bias, int bias_type, int act, void* C, int c_type, int64_t ldc,
                  void* stream);
 
+/* Test hook: how nfx_fp8_gemm cuts a product on a device of `sms` SMs.  *columns: 0 for the kernel of CTA
+ * pairs (256 x 256 tiles), else the rows of A to a tile of the narrow kernel (16, 32, 64, 128), with *split
+ * CTAs sharing K and *deep set where one CTA takes an SM's shared memory.  Needs no GPU. */
+void nfx_debug_fp8_gemm_plan(int64_t M, int64_t N, int64_t K, int b_tile, int sms, int* columns, int* split, int* deep);
+
 /* Read and clear the device error word of the current device (bit flags of waits
  * that timed out inside kernels).  Synchronises the device. */
 int nfx_device_errors(unsigned* flags_out);

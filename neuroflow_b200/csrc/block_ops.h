@@ -104,6 +104,13 @@ struct Fp8GemmArgs {
     unsigned* err;
     unsigned long long wait_ns;
 };
+// how a product is cut on `sms` SMs: rows of A to a tile of the narrow kernel (0: the kernel of CTA pairs),
+// CTAs that share K, and whether the narrow kernel takes an SM's memory for one CTA's ring
+struct Fp8Plan {
+    int columns, split;
+    bool deep;
+};
+Fp8Plan fp8_gemm_plan(int64_t M, int64_t N, int64_t K, int b_tile, int64_t sms);
 cudaError_t fp8_gemm_launch(const Fp8GemmArgs& a, cudaStream_t s);
 
 #ifdef __CUDACC__

@@ -818,6 +818,21 @@ cudaError_t launch_narrow(const Fp8GemmArgs& p, int split, cudaStream_t stream) 
     return cudaLaunchKernelEx(&cfg, kern, tmW, tmX, p, split);
 }
 
+template <int CT>
+cudaError_t dispatch(const Fp8GemmArgs& p, cudaStream_t stream) {
+    const Fp8Plan c = fp8_gemm_plan(p.M, p.N, p.K, p.b_tile, device_sm_count());
+    if (c.columns == 0) return launch_pair<CT>(p, stream);
+    if (c.columns == 16)
+        return c.deep ? launch_narrow<16, CT, true>(p, c.split, stream) : launch_narrow<16, CT, false>(p, c.split, stream);
+    if (c.columns == 32)
+        return c.deep ? launch_narrow<32, CT, true>(p, c.split, stream) : launch_narrow<32, CT, false>(p, c.split, stream);
+    if (c.columns == 64)
+        return c.deep ? launch_narrow<64, CT, true>(p, c.split, stream) : launch_narrow<64, CT, false>(p, c.split, stream);
+    return launch_narrow<128, CT, true>(p, c.split, stream);
+}
+
+}  // namespace
+
 // Which kernel, and how it is cut: the cheapest by a model fitted to measurements (us, graphs of launches;
 // KB blocks of K, each within 8 % of what was measured over the shapes below).
 //   narrow, NT columns, K over `split` CTAs   4.3 + rounds ceil(KB / split) c(NT) + 2.5 a further round, + join(NT)
@@ -827,10 +842,9 @@ cudaError_t launch_narrow(const Fp8GemmArgs& p, int split, cudaStream_t stream) 
 // 128/4; 512x4096x4096: 18.2 with 128/1, 19.6 pair; 1000x4096x1024: 15.9 with 128/1, 9.8 pair; 1x4096x4096: 9.7,
 // 7.4, 6.2, 7.6 with a split of 1, 2, 4, 8.  Clusters of four and eight do not fill the SMs of every
 // processor cluster, hence 128 CTAs at a time there (300x700x6000 with 128/8, 144 CTAs: 16.6).
-template <int CT>
-cudaError_t dispatch(const Fp8GemmArgs& p, cudaStream_t stream) {
-    const int64_t sms = device_sm_count(), KB = (p.K + kBK - 1) / kBK, M = p.M, N = p.N;
+Fp8Plan fp8_gemm_plan(int64_t M, int64_t N, int64_t K, int b_tile, int64_t sms) {
     const auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+    const int64_t KB = up(K, kBK);
     constexpr int kCost[4] = {20, 24, 32, 42}, kJoin[4] = {70, 100, 150, 250};  // hundredths of a microsecond
     int nt = 16, split = 1;
     int64_t best = -1;
@@ -845,15 +859,9 @@ cudaError_t dispatch(const Fp8GemmArgs& p, cudaStream_t stream) {
         }
     }
     const int64_t rounds = up(up(M, 256) * up(N, 256), sms / 2);
-    if (650 + rounds * KB * (p.b_tile ? 41 : 65) + (rounds - 1) * 220 < best) return launch_pair<CT>(p, stream);
-    const bool deep = up(N, 128) * up(M, nt) * split <= sms;
-    if (nt == 16) return deep ? launch_narrow<16, CT, true>(p, split, stream) : launch_narrow<16, CT, false>(p, split, stream);
-    if (nt == 32) return deep ? launch_narrow<32, CT, true>(p, split, stream) : launch_narrow<32, CT, false>(p, split, stream);
-    if (nt == 64) return deep ? launch_narrow<64, CT, true>(p, split, stream) : launch_narrow<64, CT, false>(p, split, stream);
-    return launch_narrow<128, CT, true>(p, split, stream);
+    if (650 + rounds * KB * (b_tile ? 41 : 65) + (rounds - 1) * 220 < best) return {0, 1, false};
+    return {nt, split, nt == 128 || up(N, 128) * up(M, nt) * split <= sms};
 }
-
-}  // namespace
 
 cudaError_t fp8_gemm_launch(const Fp8GemmArgs& p_in, cudaStream_t stream) {
     Fp8GemmArgs p = p_in;

@@ -853,13 +853,13 @@ Fp8Plan fp8_gemm_plan(int64_t M, int64_t N, int64_t K, int b_tile, int64_t sms) 
         if (i > 0 && w / 2 >= M) break;
         for (int s = 1; s <= 8 && (s == 1 || 2 * s <= KB); s *= 2) {
             const int64_t ctas = up(N, 128) * up(M, w) * s;
-            const int64_t rounds = up(ctas, s >= 4 ? sms * 7 / 8 : sms);
+            const int64_t rounds = up(ctas, s >= 4 && sms > 1 ? sms * 7 / 8 : sms);
             const int64_t cost = 430 + rounds * up(KB, s) * kCost[i] + (rounds - 1) * 250 + (s > 1 ? kJoin[i] : 0);
             if (best < 0 || cost < best) best = cost, nt = w, split = s;
         }
     }
-    const int64_t rounds = up(up(M, 256) * up(N, 256), sms / 2);
-    if (650 + rounds * KB * (b_tile ? 41 : 65) + (rounds - 1) * 220 < best) return {0, 1, false};
+    const int64_t rounds = sms > 1 ? up(up(M, 256) * up(N, 256), sms / 2) : 0;
+    if (sms > 1 && 650 + rounds * KB * (b_tile ? 41 : 65) + (rounds - 1) * 220 < best) return {0, 1, false};
     return {nt, split, nt == 128 || up(N, 128) * up(M, nt) * split <= sms};
 }
 

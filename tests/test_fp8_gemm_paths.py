@@ -44,6 +44,15 @@ def test_each_shape_takes_its_path():
     assert _plan(5, 40, 0, 1)[:2] == (16, 1)  # nothing to sum
 
 
+def test_the_rule_on_devices_of_few_sms():
+    """One SM (also what an unreadable count is taken for) has no pair, and none of them divides by zero."""
+    for sms in (1, 2, 3, 7):
+        for mnk in ((1, 1, 1), (1, 4096, 1 << 20), (2500, 2600, 200), (20000, 20000, 4096)):
+            for b_tile in (0, 1):
+                columns = _plan(*mnk, b_tile, sms)[0]
+                assert columns in (16, 32, 64, 128) if sms == 1 else columns in (0, 16, 32, 64, 128)
+
+
 def test_every_path_of_the_rule_has_a_shape():
     """A sweep over sizes meets no path that is not in the list, save narrow ones that differ in the split
     alone (a split of 8 in more CTAs than SMs)."""

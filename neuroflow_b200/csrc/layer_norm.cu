@@ -8,9 +8,10 @@
 //
 // All statistics and sums are fp32; the variance is the mean of the centred squares (a
 // second sweep), not E[x^2] - mu^2, which cancels when |mu| is large against the spread.
-// That sweep also sums the centred values themselves: their mean is the rounding error of mu,
-// and taking it out leaves y within two or three roundings of the formula (it decides how many
-// FP8 codes fall on the other side of a rounding boundary).  Outputs are rounded once.
+// The rounding error of mu is taken out of the centred values: for fp32 rows that sweep sums them too
+// and their mean is the error, for 16-bit rows it is the division's remainder (sums_centred).  It
+// leaves y within two or three roundings of the formula, which decides how many FP8 codes fall on the
+// other side of a rounding boundary.  Outputs are rounded once.
 #include <atomic>
 
 #include "block_ops.h"
@@ -212,13 +213,13 @@ __device__ __forceinline__ void load_params(const void* p, int type, bool vec, i
     }
 }
 
-// Sums of (a, b) over the TPR threads of a row, the same bits in each of them.
-template <int TPR>
+// Sums of (a, b) over the TPR threads of a row, the same bits in each of them; of a alone without TWO.
+template <int TPR, bool TWO>
 __device__ __forceinline__ float2 row_sums(float a, float b, float2* red) {
 #pragma unroll
     for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1) {
         a += __shfl_xor_sync(0xFFFFFFFFu, a, o);
-        b += __shfl_xor_sync(0xFFFFFFFFu, b, o);
+        if (TWO) b += __shfl_xor_sync(0xFFFFFFFFu, b, o);
     }
     float2 t = make_float2(a, b);
     if constexpr (TPR > 32) {
@@ -229,7 +230,8 @@ __device__ __forceinline__ float2 row_sums(float a, float b, float2* red) {
 #pragma unroll
         for (int k = 1; k < TPR / 32; ++k) {
             const float2 u = red[w0 + k];
-            t.x += u.x, t.y += u.y;
+            t.x += u.x;
+            if (TWO) t.y += u.y;
         }
     }
     return t;
@@ -257,11 +259,24 @@ constexpr int row_blocks(int vpt, int ve, int tpr) {
     return walks(vpt * ve) ? (row_block(tpr) > 384 ? 1 : 768 / row_block(tpr)) : (tpr >= 512 ? 2 : 1);
 }
 
+// Whether the centred values are summed to find the rounding error of the mean (rows of at most `width`).
+// fp32 numbers need it (a constant row of 20,001 times 1000.1 is 0.2 off without).  16-bit ones do not: sums
+// are exact where the numbers are of one size (8 or 11 bits and log2(width) more), and where they are not
+// the spread is as large as the numbers.  There the second sum would only add its own rounding, which is
+// the same way for all numbers of a binade, as they have the same low bits once mu0 is taken off
+// (4096 columns: the mean 1.7e-8 off, and 23 FP8 codes of 12 million on the other side of a boundary against
+// 10 for the formula in plain fp32; 9 without it).
+template <typename T>
+constexpr bool sums_centred(int width) {
+    return sizeof(T) == 4 || (std::is_same<T, __half>::value && width > 8192);
+}
+
 template <typename T, int VE, int VPT, int TPR, bool FP8>
 __global__ void __launch_bounds__(row_block(TPR), row_blocks(VPT, VE, TPR)) norm_row_kernel(NormArgs a, bool pvec, bool wide) {
     __shared__ float2 red[2][row_block(TPR) / 32];
     constexpr int kRows = row_block(TPR) / TPR, N = VPT * VE;
     constexpr bool kWalk = walks(N);
+    constexpr bool kCentred = sums_centred<T>(N * TPR);
     const int lane = threadIdx.x & 31, sub = threadIdx.x % TPR;
     // pack j of this thread is first + j * 32 (a row of fewer than 32 threads has one pack a thread)
     const int first = TPR < 32 ? sub : (sub >> 5) * VPT * 32 + lane;
@@ -312,7 +327,7 @@ __global__ void __launch_bounds__(row_block(TPR), row_blocks(VPT, VE, TPR)) norm
 #pragma unroll
         for (int k = 2; k < N; k += 2) p2 = add2_rn(p2, make_float2(f[k], f[k + 1]));
         s = p2.x + p2.y;
-        const float mu0 = mean_of(row_sums<TPR>(s, 0.0f, red[0]).x, fd, inv_d);
+        const float sum = row_sums<TPR, false>(s, 0.0f, red[0]).x, mu0 = mean_of(sum, fd, inv_d);
         float s1 = 0.0f;
         s = 0.0f;
         if (full) {
@@ -322,7 +337,7 @@ __global__ void __launch_bounds__(row_block(TPR), row_blocks(VPT, VE, TPR)) norm
             for (int k = 0; k < N; k += 2) {
                 const float2 c = add2_rn(make_float2(f[k], f[k + 1]), m2);
                 f[k] = c.x, f[k + 1] = c.y;
-                q1 = add2_rn(q1, c);
+                if (kCentred) q1 = add2_rn(q1, c);
                 q2 = fma2_rn(c, c, q2);
             }
             s1 = q1.x + q1.y;
@@ -334,17 +349,17 @@ __global__ void __launch_bounds__(row_block(TPR), row_blocks(VPT, VE, TPR)) norm
 #pragma unroll
                     for (int i = 0; i < VE; ++i) {
                         v[j][i] -= mu0;
-                        s1 += v[j][i];
+                        if (kCentred) s1 += v[j][i];
                         s = fmaf(v[j][i], v[j][i], s);
                     }
                 }
             }
         }
-        // the centred values' own mean is what the first sum's rounding left over
-        const float2 t = row_sums<TPR>(s1, s, red[1]);
-        const float rest = t.x * inv_d, mu = mu0 + rest;
+        // what the rounding of mu0 left over: of its sum too (the centred values' own mean), or of the division
+        const float2 t = row_sums<TPR, kCentred>(kCentred ? s1 : s, s, red[1]);
+        const float rest = (kCentred ? t.x : fmaf(-mu0, fd, sum)) * inv_d, mu = mu0 + rest;
         // (a constant row of rounded sums can leave this difference below zero)
-        const float rs = __frsqrt_rn(not_negative(fmaf(-rest, rest, t.y * inv_d)) + a.eps), off = -rest * rs;
+        const float rs = __frsqrt_rn(not_negative(fmaf(-rest, rest, (kCentred ? t.y : t.x) * inv_d)) + a.eps), off = -rest * rs;
         if (live && sub == 0) {
             if (a.mean) a.mean[r] = mu;
             if (a.rstd) a.rstd[r] = rs;

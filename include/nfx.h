@@ -314,7 +314,7 @@ int nfx_int8_gemm(const int8_t* A, const float* scale_a, const int32_t* zp_a, fl
 
 /* Failure-path test hook: the budget, in nanoseconds, of the pipeline waits inside the
  * INT8 GEMM kernel (nfx_int8_gemm and the GEMM layers of the FNO1d / TokenMixer2D
- * executors) for launches made after the call; 0 restores the default of 2 s.  With a
+ * executors) and the FP8 product (nfx_fp8_gemm) for launches made after the call; 0 restores the default of 2 s.  With a
  * budget far below the kernel's latency the waits run out: the kernel raises its abort
  * flag, records the timeout in the device error word, waits (with the default budget)
  * for its own loads and MMAs in flight, releases its tensor memory and returns, and the
@@ -350,16 +350,20 @@ int nfx_fp8_e4m3_selfcheck(unsigned long long* mismatches);
  * tensors on the GPU.  No counterpart in the reference (its LayerNorm and Linear exist
  * inside TokenMixer::Forward only, cpp/src/fno.cpp:1418-1438, and its 8-bit forms are
  * per tensor or per channel).  All pointers are DEVICE pointers on the current device,
- * except where NULL is allowed; calls are asynchronous on `stream`, allocate nothing and
- * keep nothing between calls.  Matrices are row-major with a row stride in elements
- * ("ld..."); a matrix of one row has no use for it.  Refused arguments give
+ * except where NULL is allowed; calls are asynchronous on `stream`, allocate nothing (save
+ * the device error word, with the first product on a device: not inside a stream capture)
+ * and keep nothing between calls.  A product whose waits run out records that in the
+ * error word (nfx_device_errors).  Matrices are row-major with a row stride in elements
+ * ("ld..."); a matrix of one row has no use for it.  Outputs share no memory with inputs
+ * except where an entry allows it.  Refused arguments give
  * NFX_INVALID_ARG and a message in nfx_last_error(). */
 enum { NFX_F32 = 0, NFX_BF16 = 1, NFX_F16 = 2 };
 
 /* Layer norm over the last dimension of x (rows, d), 1 <= d < 2^31 - 256:
  *   y = (x - mean) rstd gamma + beta,  rstd = 1 / sqrt(var + eps), var the biased variance.
  * y has x's type; gamma and beta (d,) have param_type, NULL: ones and zeros.  mean and rstd
- * (rows,) are written where not NULL (the backward pass reads them).  Statistics in fp32. */
+ * (rows,) are written where not NULL (the backward pass reads them).  Statistics in fp32.
+ * y may be x (the same pointer and stride). */
 int nfx_layer_norm(const void* x, int x_type, int64_t ldx, const void* gamma, const void* beta, int param_type,
                    int64_t rows, int64_t d, float eps, void* y, int64_t ldy, float* mean, float* rstd,
                    void* stream);
@@ -405,7 +409,7 @@ int nfx_fp8_quantise(const void* x, int x_type, int64_t ldx, int64_t rows, int64
  *   C[m, n] = act(sum_b sa[m, b] sb[n, b] sum_{k in block b} A[m, k] B[n, k] + bias[n])
  * over blocks of 128 along K; with a_tile (b_tile) the scales are per 128 rows.  Each block's
  * sum is formed by the tensor cores, the sum over blocks in fp32.  The product of two scales
- * that meet must be finite in fp32.  The rows of A and B start on 16-byte boundaries (base
+ * that meet must be finite in fp32, and at least 2^-126 to be exact to fp32's precision.  The rows of A and B start on 16-byte boundaries (base
  * and row stride); any M, N, K >= 0.  bias (N,) of bias_type or NULL; act 0 none, 1 GELU
  * (tanh form), 2 ReLU; C of c_type.  The gradients of a linear layer are products of the same
  * kind: dX = dY W is (dY, W^T) with the tiles' transposed codes, dW = dY^T X is (dY^T, X^T). */

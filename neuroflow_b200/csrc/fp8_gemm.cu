@@ -9,15 +9,21 @@
 // fp32 and no product of scales is rounded to fewer bits.
 //
 // Two kernels: pairs of CTAs on 256 x 256 tiles for large results, and a narrow one, with K split
-// over a cluster, for few rows of A or few tiles; dispatch() below chooses.  Both are
+// over a cluster, for few rows of A or few tiles; fp8_gemm_plan() below chooses.  Both are
 // warp-specialised: a TMA producer, an MMA issuer, a scale producer, and the promoting warps.
 //
-// Measured (one B200; HBM 6,457 GB/s, FP8 taken as twice the measured bf16 rate, 3,276 TFLOP/s):
-//   8192x16384x4096 to bf16   507 us, 2,170 TFLOP/s, at the 1,000 W power cap (1.5 GHz); 553 us with
-//                             bias and GELU.  A block of K takes 745 cycles where its MMAs take 512:
-//                             without the sums 670, without TMEM reads too 650 (barrier hand-over)
-//   4096x4096x8192 to fp32    about 195 us with column scales (a second multiply per element)
-//   1x4096x4096               6.2 us, of which 4.5 are the start and the join (1x1024x1024 takes that)
+// Measured (one B200; HBM 6,457 GB/s, FP8 taken as twice the measured bf16 rate, 3,276 TFLOP/s; graphs of
+// launches over operands that do not fit L2 together, a few milliseconds long):
+//   8192x16384x4096 to bf16   481 us, 2,290 TFLOP/s; 535 us with bias and GELU.  In a loop of seconds the
+//                             1,000 W power cap sets the clock: 572 us at 1.43 GHz, 636 us with bias and
+//                             GELU at 1.53 GHz.  A block of K takes 745 cycles where its MMAs take 512
+//                             (without the sums 670, without TMEM reads too 650: barrier hand-over); the
+//                             rest is the tiles' epilogues, of which MMAs of two blocks overlap
+//                             (2304x2048x512, one tile a pair: 8.0 us, 11.1 with bias and GELU)
+//   4096x4096x8192 to fp32    196 us with column scales.  A block of K takes 0.68 us (2304x2048), 0.45 with
+//                             tile scales: four TMEM reads, each waited for, and a second multiply
+//   1x4096x4096               8.5 us, 5.9 with the weights in L2, of which 4.5 are the start and the join
+//                             (1x1024x1024 takes that)
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -833,8 +839,10 @@ cudaError_t dispatch(const Fp8GemmArgs& p, cudaStream_t stream) {
 
 }  // namespace
 
-// Which kernel, and how it is cut: the cheapest by a model fitted to measurements (us, graphs of launches;
-// KB blocks of K, each within 8 % of what was measured over the shapes below).
+// Which kernel, and how it is cut: the cheapest by a model fitted to measurements (us, graphs of launches
+// whose operands stay in L2; with weights from HBM 1x4096x4096 takes 8.5 and not 5.9).  KB blocks of K.  Of the figures
+// below the model is within 8 %, save 1x4096x4096 without (10 %) and with a split of 2 and 8 (11 and 20 %) and
+// 1000x4096x1024 with 128/1 (15 %); of the choices given for a shape, its cheapest is the fastest.
 //   narrow, NT columns, K over `split` CTAs   4.3 + rounds ceil(KB / split) c(NT) + 2.5 a further round, + join(NT)
 //       c: 0.20, 0.24, 0.32, 0.42 for NT = 16, 32, 64, 128;  join (partials through the cluster): 0.7, 1.0, 1.5, 2.5
 //   pair                                      6.5 + rounds KB 0.41 (0.65 with column scales) + 2.2 a further round

@@ -36,17 +36,18 @@ __global__ void __launch_bounds__(128) quant_rows_kernel(QuantArgs a, int64_t ch
     store_codes<VE, VPT, TPR>(v, a.q, r, a.cols, live, first, lane, wide);
 }
 
-// 128 x 128 tiles, one at a time per block.  A thread holds 8 rows x 8
-// columns in registers: lane % 16 counts the columns' eights, 2 * warp + lane / 16 the rows'.  A row's
-// maximum is 8 values and four shuffles, a column's 8 values, a shuffle and eight partial results in
-// shared memory; scales and reciprocals are made by one thread per row and per column.  The
-// transposed codes go through shared memory (16 KB, 8-byte slots XOR-ed with the column's eight, so that
-// neither side has more conflicts than its width) and leave as 128-byte rows.  The tile's bytes are the
-// bound; what keeps them coming for 16-bit types (kAhead) is that the blocks walk over the tiles and a
-// thread copies its part of the next one into shared memory (cp.async, its own slots, so no barrier)
-// while it works on this one: 16384x4096 bf16 both ways with sums 85 us, 147 with a block per tile.  An
-// fp32 tile is twice the bytes for the same work, and there a block per tile is faster (131072x128 to
-// tiles: 17 us, 28 walking).  `VEC`: rows of x start on 16-byte boundaries.
+// 128 x 128 tiles, one at a time per block.  A thread holds 8 rows x 8 columns in registers: lane % 16
+// counts the columns' eights, 2 * warp + lane / 16 the rows'.  A row's maximum is 8 values and four
+// shuffles, a column's 8 values, a shuffle and eight partial results in shared memory; scales and
+// reciprocals are made by one thread per row and per column.  The transposed codes go through shared memory
+// (16 KB, 8-byte slots XOR-ed with the column's eight, so that neither side has more conflicts than its
+// width) and leave as 128-byte rows.  The bytes' latency is the bound, at the quarter of an SM's warps that
+// the registers leave; what keeps them coming for 16-bit types (kAhead) is that the blocks walk over the
+// tiles and a thread copies its part of the next one into shared memory (cp.async, its own slots, so no
+// barrier) while it works on this one: 16384x4096 bf16 both ways with sums 74 us (85, against 147 with a
+// block per tile, while each code was still corrected in the main path).  An fp32 tile is twice the bytes
+// for the same work, and there a block per tile is faster (131072x128 to tiles: 17 us, 28 walking).  `VEC`:
+// rows of x start on 16-byte boundaries.
 constexpr int kTileThreads = 256;
 
 template <typename T, bool VEC>

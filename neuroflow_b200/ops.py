@@ -19,6 +19,14 @@ With `stream` the caller orders it behind the work that made the inputs, and oth
 they read the outputs (torch.cuda.Stream.wait_stream).  The tensors of the call are recorded on a
 torch.cuda.Stream, so they may be released at once; a raw handle's life is not known to torch, so there the
 caller keeps them until the work is done.
+
+Codes are float8_e4m3fn by the library's encoder: as torch's conversion rounds, save that a scaled value
+under 2^-6, the smallest normal number, is at most 7 * 2^-9, the largest subnormal one (torch gives 2^-6 from
+7.5 * 2^-9 on); values beyond +-448 saturate.
+
+Only layer_norm_autograd and fp8_linear are recorded by autograd; the other calls are the operators
+themselves, and write into an `out` as torch's own in-place operations do (its version is raised, it must
+not require grad while gradients are recorded).
 """
 from __future__ import annotations
 

@@ -17,8 +17,8 @@ float16 are accepted where a tensor is not FP8; the last dimension has to be con
 
 With `stream` the caller orders it behind the work that made the inputs, and other streams behind it where
 they read the outputs (torch.cuda.Stream.wait_stream).  The tensors of the call are recorded on a
-torch.cuda.Stream, so they may be released at once; a raw handle's life is not known to torch, so there the
-caller keeps them until the work is done.
+torch.cuda.Stream, so they may be released at once; the life of a raw handle's or ExternalStream's stream is
+not known to torch, so there the caller keeps them until the work is done.
 
 Codes are float8_e4m3fn by the library's encoder: as torch's conversion rounds, save that a scaled value
 under 2^-6, the smallest normal number, is at most 7 * 2^-9, the largest subnormal one (torch gives 2^-6 from
@@ -76,17 +76,17 @@ def _refuse(fn, what):
 def _on(stream, t, *others):
     """`stream` (a torch.cuda.Stream or raw handle on t's device) made current, so that what a call
     allocates belongs to it; the tensors of the call (t, and the others that are not None) are recorded
-    on a torch.cuda.Stream, so that their memory is not handed out again before it is done with them."""
+    on a stream of torch's, so that their memory is not handed out again before it is done with them."""
     if not t.is_cuda:
         _refuse("stream", "the tensors of a call must be CUDA tensors")
-    known = isinstance(stream, torch.cuda.Stream)
-    if not known:
+    ours = isinstance(stream, torch.cuda.Stream) and not isinstance(stream, torch.cuda.ExternalStream)
+    if not isinstance(stream, torch.cuda.Stream):
         stream = torch.cuda.ExternalStream(int(stream), device=t.device)
     elif stream.device != t.device:
         _refuse("stream", f"the stream is on {stream.device}, the tensors are on {t.device}")
     with torch.cuda.stream(stream):
         yield
-    if known:
+    if ours:
         for u in (t, *others):
             if u is not None:
                 u.record_stream(stream)

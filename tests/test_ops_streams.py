@@ -61,6 +61,22 @@ def test_tensors_of_a_call_are_recorded_on_its_stream(ops):
         assert all(t.on == [st] for t in used)
 
 
+def test_streams_that_torch_does_not_own_are_not_recorded(ops, monkeypatch):
+    """Memory recorded on a stream is looked after with an event on it when it is released; a stream of another
+    library, wrapped or as a raw handle, may be gone by then."""
+    class External(Stream):
+        def __init__(self, handle, device=None):
+            super().__init__(device)
+
+    monkeypatch.setattr(ops.torch.cuda, "ExternalStream", External)
+    for call, used in _calls(ops, Held):
+        for st in (1234, External(1234, "cuda:0")):
+            for t in used:
+                t.on.clear()
+            call(st)
+            assert not any(t.on for t in used)
+
+
 def test_a_stream_of_another_device_is_refused(ops):
     """It would be made current on its own device, and the call would run on another stream."""
     from neuroflow_b200 import _nfx

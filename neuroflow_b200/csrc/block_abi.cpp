@@ -221,7 +221,7 @@ int nfx_fp8_gemm(const uint8_t* A, int64_t lda, const float* scale_a, int64_t sc
 }
 
 void nfx_debug_fp8_gemm_plan(int64_t M, int64_t N, int64_t K, int b_tile, int sms, int* columns, int* split, int* deep) {
-    const nfx::Fp8Plan c = nfx::fp8_gemm_plan(M, N, K, b_tile, sms);
+    const nfx::Fp8Plan c = nfx::fp8_gemm_plan(M, N, K, b_tile, sms < 1 ? 1 : sms);
     *columns = c.columns, *split = c.split, *deep = c.deep;
 }
 

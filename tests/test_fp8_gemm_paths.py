@@ -46,6 +46,7 @@ def test_each_shape_takes_its_path():
 
 def test_the_rule_on_devices_of_few_sms():
     """One SM (also what an unreadable count is taken for) has no pair, and none of them divides by zero."""
+    assert _plan(2500, 2600, 200, 1, 0) == _plan(2500, 2600, 200, 1, 1) == _plan(2500, 2600, 200, 1, -5)
     for sms in (1, 2, 3, 7):
         for mnk in ((1, 1, 1), (1, 4096, 1 << 20), (2500, 2600, 200), (20000, 20000, 4096)):
             for b_tile in (0, 1):

@@ -424,6 +424,81 @@ int nfx_fp8_gemm(const uint8_t* A, int64_t lda, const float* scale_a, int64_t sc
  * CTAs sharing K and *deep set where one CTA takes an SM's shared memory.  Needs no GPU. */
 void nfx_debug_fp8_gemm_plan(int64_t M, int64_t N, int64_t K, int b_tile, int sms, int* columns, int* split, int* deep);
 
+/* ---- A pre-norm block in 16 bits: RMS norm with residual, product with epilogue, clipping ----
+ * Beside the FP8 layer above, with the same rules: DEVICE pointers, row strides in elements,
+ * asynchronous on `stream`, nothing allocated (save the device error word, with the first product on
+ * a device) and nothing kept between calls; outputs share no memory with inputs except where an
+ * entry allows it.  No counterpart in the reference. */
+
+/* h = x + residual, rounded to sum_type (x_type or NFX_F32);  y = h rstd gamma,
+ * rstd = 1 / sqrt(mean(h^2) + eps), over the last dimension, 1 <= d < 2^31 - 256.  residual NULL:
+ * h = x (sum_type has no meaning, sum must be NULL).  y has x's type, gamma (d,) param_type (NULL: ones);
+ * sum (rows, d) of sum_type and rstd (rows,) are written where not NULL.  y may be x, sum may be the
+ * residual, either may be the other's input where the types are equal (the same pointer and stride); y
+ * and sum are apart. */
+int nfx_rms_norm(const void* x, int x_type, int64_t ldx, const void* residual, int sum_type, int64_t ld_residual,
+                 const void* gamma, int param_type, int64_t rows, int64_t d, float eps, void* y, int64_t ldy,
+                 void* sum, int64_t ld_sum, float* rstd, void* stream);
+
+/* The same with y in FP8, as nfx_fp8_quantise with tile = 0 would make it from an fp32 y. */
+int nfx_rms_norm_fp8(const void* x, int x_type, int64_t ldx, const void* residual, int sum_type, int64_t ld_residual,
+                     const void* gamma, int param_type, int64_t rows, int64_t d, float eps, uint8_t* codes,
+                     int64_t ld_codes, float* scales, int64_t scale_row_stride, int64_t scale_block_stride,
+                     void* sum, int64_t ld_sum, float* rstd, void* stream);
+
+/* Gradient: with a = gamma dy and xh = h rstd,
+ *   dh = rstd (a - xh mean(a xh)) + dsum,  dgamma = sum over rows of dy xh.
+ * dy and dx have dy_type, h, dsum and dres h_type (dy_type or NFX_F32); dh goes to dx and to dres, the
+ * gradients of x and of the residual, each of which may be NULL, as may dsum (nothing else reaches h)
+ * and dgamma (d,) of param_type.  With dgamma a 16-byte aligned workspace of
+ * nfx_rms_norm_backward_workspace bytes.  dx and dres may be dy, h or dsum of the same type (the same
+ * pointer and stride). */
+int64_t nfx_rms_norm_backward_workspace(int64_t rows, int64_t d);
+int nfx_rms_norm_backward(const void* dy, int dy_type, int64_t lddy, const void* h, int h_type, int64_t ldh,
+                          const float* rstd, const void* gamma, int param_type, const void* dsum, int64_t ld_dsum,
+                          int64_t rows, int64_t d, void* dx, int64_t lddx, void* dres, int64_t ld_dres, void* dgamma,
+                          void* workspace, int64_t workspace_bytes, void* stream);
+
+/* C = act(Z) + residual,  Z = A B^T + bias, for bf16 or fp16 operands (ab_type), sums in fp32.
+ * A is (M, K): element (m, k) at m lda + k, or with a_trans at k lda + m; B is (N, K), the same.  bias
+ * (N,) of bias_type or NULL; act 0 none, 1 GELU (tanh form), 2 ReLU; residual (M, N) of C's type or
+ * NULL; C of ab_type or NFX_F32; Z (M, N), of C's type, is written where not NULL.  Any M, N, K >= 0 and
+ * any alignment; operands whose base or row stride is not a multiple of 16 bytes are first
+ * copied into the workspace (16-byte aligned, nfx_gemm_workspace bytes for these very arguments; 0 where no
+ * copy is needed).  C may be the residual (the same pointer and stride).  Device error word as
+ * nfx_fp8_gemm. */
+int64_t nfx_gemm_workspace(const void* A, int64_t lda, int a_trans, const void* B, int64_t ldb, int b_trans, int64_t M,
+                           int64_t N, int64_t K);
+int nfx_gemm(const void* A, int64_t lda, int a_trans, const void* B, int64_t ldb, int b_trans, int ab_type, int64_t M,
+             int64_t N, int64_t K, const void* bias, int bias_type, int act, const void* residual, int64_t ld_residual,
+             void* C, int c_type, int64_t ldc, void* Z, int64_t ldz, void* workspace, int64_t workspace_bytes,
+             void* stream);
+
+/* Gradient of the activation: dz = dy act'(z), dbias (cols,) = sums of its columns, formed in fp32 before dz
+ * is rounded.  dy, z, dz (rows, cols) of `type`; z is not read with act = 0; dz or dbias may be NULL.
+ * With dbias a 16-byte aligned workspace of nfx_act_backward_workspace bytes.  dz may be dy or z (the
+ * same pointer and stride). */
+int64_t nfx_act_backward_workspace(int64_t rows, int64_t cols);
+int nfx_act_backward(const void* dy, int64_t lddy, const void* z, int64_t ldz, int type, int act, int64_t rows,
+                     int64_t cols, void* dz, int64_t lddz, void* dbias, int bias_type, void* workspace,
+                     int64_t workspace_bytes, void* stream);
+
+/* The 2-norm over all elements of many tensors, and the tensors scaled to a largest norm:
+ *   norm = sqrt(sum g^2),  out = g min(1, max_norm / (norm + eps)).
+ * The four (six) arrays are in HOST memory and read before the call returns: tensor i has counts[i]
+ * elements of types[i] at the DEVICE address grads[i], and goes to out[i] of out_types[i]; out NULL: in
+ * place.  Any alignment, sizes and number of tensors.  Sums of squares are 64-bit numbers; `norm` (one
+ * float on the device) is rounded to fp32.  out[i] may be grads[i] of the same type; beyond that no
+ * output shares memory with another tensor.  A norm of infinity gives zeros, and NaN where an element is
+ * infinite; a NaN gives NaN everywhere.  The workspace is 16-byte aligned, of nfx_grad_norm_workspace
+ * bytes. */
+int64_t nfx_grad_norm_workspace(int64_t tensors);
+int nfx_grad_norm(const void* const* grads, const int64_t* counts, const int* types, int64_t tensors, float* norm,
+                  void* workspace, int64_t workspace_bytes, void* stream);
+int nfx_clip_grad_norm(const void* const* grads, const int64_t* counts, const int* types, void* const* out,
+                       const int* out_types, int64_t tensors, double max_norm, double eps, float* norm,
+                       void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Read and clear the device error word of the current device (bit flags of waits
  * that timed out inside kernels).  Synchronises the device. */
 int nfx_device_errors(unsigned* flags_out);

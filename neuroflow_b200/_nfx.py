@@ -52,6 +52,26 @@ lib.nfx_fp8_gemm.restype = C.c_int
 lib.nfx_fp8_gemm.argtypes = [_vp, _i64, _vp, _i64, _i64, C.c_int, _vp, _i64, _vp, _i64, _i64, C.c_int, _i64,
                              _i64, _i64, _vp, C.c_int, C.c_int, _vp, C.c_int, _i64, _vp]
 
+_int = C.c_int
+_vpp, _intp = C.POINTER(_vp), C.POINTER(_int)
+for _name, _res, _args in [
+        ("nfx_rms_norm", _int, [_vp, _int, _i64, _vp, _int, _i64, _vp, _int, _i64, _i64, C.c_float, _vp, _i64, _vp, _i64, _vp, _vp]),
+        ("nfx_rms_norm_fp8", _int, [_vp, _int, _i64, _vp, _int, _i64, _vp, _int, _i64, _i64, C.c_float, _vp, _i64, _vp, _i64, _i64,
+                                    _vp, _i64, _vp, _vp]),
+        ("nfx_rms_norm_backward_workspace", _i64, [_i64, _i64]),
+        ("nfx_rms_norm_backward", _int, [_vp, _int, _i64, _vp, _int, _i64, _vp, _vp, _int, _vp, _i64, _i64, _i64, _vp, _i64, _vp,
+                                         _i64, _vp, _vp, _i64, _vp]),
+        ("nfx_gemm_workspace", _i64, [_vp, _i64, _int, _vp, _i64, _int, _i64, _i64, _i64]),
+        ("nfx_gemm", _int, [_vp, _i64, _int, _vp, _i64, _int, _int, _i64, _i64, _i64, _vp, _int, _int, _vp, _i64, _vp, _int, _i64,
+                            _vp, _i64, _vp, _i64, _vp]),
+        ("nfx_act_backward_workspace", _i64, [_i64, _i64]),
+        ("nfx_act_backward", _int, [_vp, _i64, _vp, _i64, _int, _int, _i64, _i64, _vp, _i64, _vp, _int, _vp, _i64, _vp]),
+        ("nfx_grad_norm_workspace", _i64, [_i64]),
+        ("nfx_grad_norm", _int, [_vpp, _i64p, _intp, _i64, _vp, _vp, _i64, _vp]),
+        ("nfx_clip_grad_norm", _int, [_vpp, _i64p, _intp, _vpp, _intp, _i64, C.c_double, C.c_double, _vp, _vp, _i64, _vp])]:
+    getattr(lib, _name).restype = _res
+    getattr(lib, _name).argtypes = _args
+
 if hasattr(lib, "nfx_runtime_create"):
     lib.nfx_runtime_create.restype = C.c_int
     lib.nfx_runtime_create.argtypes = [C.c_char_p, C.c_int, C.POINTER(_vp)]

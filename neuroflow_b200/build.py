@@ -72,6 +72,7 @@ def build(verbose: bool = False) -> str:
 
 
 TORCH_SRC = os.path.join(PKG, "torch_ext", "nfx_torch.cpp")
+TORCH_PARTS = [TORCH_SRC, os.path.join(PKG, "torch_ext", "nfx_torch_dense.h"), os.path.join(ROOT, "include", "nfx.h")]
 TORCH_EXT = os.path.join(PKG, "_nfx_torch.so")
 TORCH_STAMP = os.path.join(OBJ, "_nfx_torch.made_for")  # the torch and Python that TORCH_EXT was built with
 
@@ -85,8 +86,7 @@ def _build_torch() -> None:
     except metadata.PackageNotFoundError:
         print("torch is not installed: without _nfx_torch.so (neuroflow_b200.ops)", file=sys.stderr)
         return
-    hdr = os.path.join(ROOT, "include", "nfx.h")
-    if (os.path.exists(TORCH_EXT) and os.path.getmtime(TORCH_EXT) >= max(os.path.getmtime(TORCH_SRC), os.path.getmtime(hdr))
+    if (os.path.exists(TORCH_EXT) and os.path.getmtime(TORCH_EXT) >= max(os.path.getmtime(f) for f in TORCH_PARTS)
             and os.path.exists(TORCH_STAMP) and open(TORCH_STAMP).read() == made_for):
         return
     import sysconfig

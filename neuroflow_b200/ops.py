@@ -1,5 +1,6 @@
-"""Operators of one pre-norm FP8 linear layer on CUDA tensors: layer norm, the FP8 E4M3 block
-quantiser and the FP8 block-scaled product, forward and backward.
+"""Operators of transformer blocks on CUDA tensors, forward and backward: layer norm, the FP8 E4M3 block
+quantiser and the FP8 block-scaled product; RMS norm with the residual's addition, the 16-bit product with
+bias, activation and residual, and gradient clipping.
 
     from neuroflow_b200 import ops
     y, mean, rstd = ops.layer_norm(x, gamma, beta, stats=True)
@@ -8,6 +9,11 @@ quantiser and the FP8 block-scaled product, forward and backward.
     x8 = ops.layer_norm_fp8(x, gamma, beta)              # layer norm straight into FP8
     y = ops.fp8_gemm(x8, w8, bias=b, act=1)              # act(x8 w8^T + b)
     y = ops.fp8_linear(x, w, b); y.backward(dy)          # the same linear layer under autograd
+
+    n, h = ops.rms_norm(x, gamma, residual=h)            # h = x + h, n = its RMS norm; rms_norm_fp8: n in FP8
+    y = ops.gemm(n, w, bias=b, act=1, residual=h)        # act(n w^T + b) + h in bf16 or fp16
+    y = ops.linear(n, w, b, act=1, residual=h)           # the same under autograd
+    norm = ops.clip_grad_norm([p.grad for p in params], 1.0)
 
 Every call runs the kernels of libnfx.so (the C-ABI of include/nfx.h, reached through the compiled
 front-end torch_ext/nfx_torch.cpp) on the current torch stream of the tensors' device, or on `stream`
@@ -24,9 +30,9 @@ Codes are float8_e4m3fn by the library's encoder: as torch's conversion rounds, 
 under 2^-6, the smallest normal number, is at most 7 * 2^-9, the largest subnormal one (torch gives 2^-6 from
 7.5 * 2^-9 on); values beyond +-448 saturate.
 
-Only layer_norm_autograd and fp8_linear are recorded by autograd; the other calls are the operators
-themselves, and write into an `out` as torch's own in-place operations do (its version is raised, it must
-not require grad while gradients are recorded).
+Only layer_norm_autograd, fp8_linear, rms_norm_autograd and linear are recorded by autograd; the other calls
+are the operators themselves, and write into an `out` as torch's own in-place operations do (its version is
+raised, it must not require grad while gradients are recorded).
 """
 from __future__ import annotations
 
@@ -150,6 +156,89 @@ def fp8_gemm(a, b, bias=None, act=0, out_dtype=torch.bfloat16, out=None, stream=
     return _ext.fp8_gemm(*a, *b, bias, act, out_dtype, out)
 
 
+# ---- a block in 16 bits -----------------------------------------------------------------------
+def rms_norm(x, gamma=None, eps=1e-5, residual=None, out=None, sum_out=None, stats=False, stream=None):
+    """RMS norm over the last dimension of x (..., d): y = h gamma / sqrt(mean(h^2) + eps), with h = x, or
+    with a `residual` of x's shape (and type, or float32) h = x + residual in the residual's type; the norm
+    is that of h as it is stored.  gamma (d,), None for ones.  y in x's type.  Returns y; (y, h) with a
+    residual; with `stats` also the fp32 1 / root mean square of each row, which rms_norm_backward takes, as the
+    last one.  `out` receives y and may be x or the residual, `sum_out` receives h and may be the residual or x
+    (the very tensor, of the same type)."""
+    if stream is not None:
+        with _on(stream, x, gamma, residual, out, sum_out):
+            return _ext.rms_norm(x, gamma, eps, residual, out, sum_out, stats)
+    return _ext.rms_norm(x, gamma, eps, residual, out, sum_out, stats)
+
+
+def rms_norm_fp8(x, gamma=None, eps=1e-5, residual=None, sum_out=None, stats=False, stream=None):
+    """rms_norm with y in FP8 groups of 128 (Fp8Blocks over the flattened rows): what fp8_quantise makes of
+    an fp32 y, which is never written.  Returns as rms_norm, with the blocks in y's place."""
+    if stream is not None:
+        with _on(stream, x, gamma, residual, sum_out):
+            return rms_norm_fp8(x, gamma, eps, residual, sum_out, stats)
+    codes, scales, h, rstd = _ext.rms_norm_fp8(x, gamma, eps, residual, sum_out, stats)
+    got = (Fp8Blocks(codes, scales),) + ((h,) if h is not None else ()) + ((rstd,) if stats else ())
+    return got if len(got) > 1 else got[0]
+
+
+def rms_norm_backward(dy, h, rstd, gamma=None, dsum=None, param_grads=True, stream=None):
+    """Gradients of rms_norm from dy (of y's shape and type), the normalised h (rms_norm's sum; x itself where
+    there was no residual) and the saved fp32 rstd; `dsum`, of h's type, is the gradient that reaches h from
+    elsewhere (the residual stream) and is added.  Returns (dx, dresidual, dgamma): dx in dy's type,
+    dresidual in h's (the same tensor where the types are equal: the gradient of x + residual is that of both),
+    dgamma in gamma's type (fp32 without gamma), or None without `param_grads`."""
+    if stream is not None:
+        with _on(stream, h, dy, rstd, gamma, dsum):
+            return _ext.rms_norm_backward(dy, h, rstd, gamma, dsum, param_grads)
+    return _ext.rms_norm_backward(dy, h, rstd, gamma, dsum, param_grads)
+
+
+def gemm(a, b, bias=None, act=0, residual=None, out_dtype=None, out=None, preact=False, stream=None):
+    """act(a b^T + bias) + residual for a (M, K) and b (N, K), both bfloat16 or both float16, sums in fp32: C
+    (M, N) in the operands' type, or in `out_dtype` (that or float32), or in `out` (its type; any row
+    stride; it may be the residual).  Rows or columns of a and of b are contiguous: a.t() and b.t() are taken
+    as they are.  bias (N,) or None; act 0 none, 1 GELU (tanh form), 2 ReLU; residual (M, N) of C's type.  With
+    `preact`: (C, a b^T + bias) of one type, the second for act_backward.  Operands whose base or row
+    stride is no multiple of 16 bytes are copied first."""
+    if stream is not None:
+        with _on(stream, a, b, bias, residual, out):
+            return _ext.gemm(a, b, bias, act, residual, out_dtype, out, preact)
+    return _ext.gemm(a, b, bias, act, residual, out_dtype, out, preact)
+
+
+def act_backward(dy, z, act, bias_dtype=None, stream=None):
+    """Gradient of act(z): (dz, dbias), dz = dy act'(z) in dy's type (dy itself with act = 0, where z may be
+    None); dbias, in `bias_dtype`, the sums of dz over its rows formed in fp32, None without a type."""
+    if stream is not None:
+        with _on(stream, dy, z):
+            return _ext.act_backward(dy, z, act, bias_dtype)
+    return _ext.act_backward(dy, z, act, bias_dtype)
+
+
+def grad_norm(grads, stream=None):
+    """The 2-norm over all elements of the tensors `grads` (one device; float32, bfloat16 and float16 may be
+    mixed; contiguous, or permutations of contiguous tensors): a float32 tensor without dimensions, on the
+    device.  Squares are summed in 64 bits."""
+    grads = list(grads)
+    if stream is not None and grads:
+        with _on(stream, *grads):
+            return _ext.grad_norm(grads)
+    return _ext.grad_norm(grads)
+
+
+def clip_grad_norm(grads, max_norm, eps=1e-6, out=None, stream=None):
+    """Scales `grads` (as in grad_norm) in place by min(1, max_norm / (norm + eps)) and returns norm, their
+    2-norm before, as grad_norm does; nothing is copied to the host.  With `out`, a tensor for each gradient (of
+    its shape and any of the three types; it may be the gradient itself), the gradients are left alone and the
+    scaled ones go there.  No tensor that is written shares memory with another."""
+    grads = list(grads)
+    out = None if out is None else list(out)
+    if stream is not None and grads:
+        with _on(stream, *grads, *(out or ())):
+            return _ext.clip_grad_norm(grads, max_norm, eps, out)
+    return _ext.clip_grad_norm(grads, max_norm, eps, out)
+
+
 # ---- under autograd -------------------------------------------------------------------------
 def layer_norm_autograd(x, gamma=None, beta=None, eps=1e-5):
     """layer_norm as a differentiable function of x, gamma and beta (once: differentiating a gradient made
@@ -164,3 +253,17 @@ def fp8_linear(x, weight, bias=None):
     unchanged; they come in the types of x, weight and bias, the output in x's.  Differentiable once:
     differentiating a gradient made under create_graph raises, as does a tangent of forward mode."""
     return _ext.fp8_linear(x, weight, bias)
+
+
+def rms_norm_autograd(x, gamma=None, eps=1e-5, residual=None):
+    """rms_norm as a differentiable function of x, gamma and the residual: y, or (y, x + residual); once, as
+    layer_norm_autograd."""
+    return _ext.rms_norm_autograd(x, gamma, eps, residual)
+
+
+def linear(x, weight, bias=None, act=0, residual=None):
+    """act(x weight^T + bias) + residual, differentiable: x (..., K) and weight (N, K) both bfloat16 or both
+    float16, bias (N,) of any type, residual and result (..., N) of x's type.  Gradients come in the types of
+    their tensors, sums in fp32; with an activation dz = dy act'(z) is rounded to x's type in between.  Once,
+    as fp8_linear."""
+    return _ext.linear(x, weight, bias, act, residual)

@@ -1,7 +1,8 @@
 // nfx_torch.cpp -- the torch front-end of the transformer-layer operators of libnfx.so (layer norm, FP8
-// block quantiser, FP8 block-scaled product): checks of the tensors, allocation of the outputs on the
-// current stream, and the C-ABI call, in compiled code because a call on one token takes the GPU a few
-// microseconds and the same steps in Python ten or more.  neuroflow_b200/ops.py is the public face.
+// block quantiser, FP8 block-scaled product; in nfx_torch_dense.h those of a block in 16 bits): checks of the
+// tensors, allocation of the outputs on the current stream, and the C-ABI call, in compiled code because a
+// call on one token takes the GPU a few microseconds and the same steps in Python ten or more.
+// neuroflow_b200/ops.py is the public face.
 //
 // Refused arguments raise neuroflow_b200._nfx.NfxError with status 1 (InvalidArg) before anything is
 // launched; errors of the C-ABI raise it with theirs.
@@ -13,8 +14,11 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
+#include <cmath>
 #include <optional>
 #include <string>
+#include <vector>
 
 #include "nfx.h"
 
@@ -399,6 +403,8 @@ Tensor fp8_linear(const Tensor& x, const Tensor& w, const OptTensor& b) {
     return fp8_gemm(xq.q.codes, xq.q.scales, false, wq.q.codes, wq.q.scales, true, b, 0, x.scalar_type(), std::nullopt).view(sizes);
 }
 
+#include "nfx_torch_dense.h"
+
 py::object or_none(const Tensor& t) { return t.defined() ? py::cast(t) : py::none(); }
 
 }  // namespace
@@ -429,4 +435,5 @@ PYBIND11_MODULE(_nfx_torch, m) {
         if (!grad || !at::GradMode::is_enabled()) return layer_norm(x, g, b, eps, std::nullopt, false).y;
         return Tensor(LayerNormFn::apply(x, g, b, eps));
     });
+    dense_defs(m);
 }

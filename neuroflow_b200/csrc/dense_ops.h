@@ -74,6 +74,13 @@ struct GemmDenseArgs {
     unsigned* err;
     unsigned long long wait_ns;
 };
+// how a product is cut on `sms` SMs: rows of A to a tile of the narrow kernel (0: the kernel of CTA pairs),
+// CTAs that share K, and whether the narrow kernel takes an SM's memory for one CTA's ring
+struct DensePlan {
+    int columns, split;
+    bool deep;
+};
+DensePlan gemm_dense_plan(int64_t M, int64_t N, int64_t K, int a_t, int64_t sms);
 int64_t gemm_dense_workspace(const void* A, int64_t lda, int a_t, const void* B, int64_t ldb, int b_t, int64_t M, int64_t N, int64_t K);
 cudaError_t gemm_dense_launch(const GemmDenseArgs& a, cudaStream_t s);
 

@@ -1,13 +1,23 @@
-// gemm_dense.cu -- product of two 16-bit matrices with bias, activation and residual in its epilogue, and the
-// activation's gradient.
+// gemm_dense.cu -- product of two 16-bit matrices with bias, activation and residual in its epilogue, on
+// tcgen05 (kind::f16).
 //
-//   Z = A B^T + bias,  C = act(Z) + R;   dz = dy act'(z),  dbias = sum over rows of dz
+//   Z = A B^T + bias,  C = act(Z) + R
+//
+// A (M, K) and B (N, K) are bf16 or fp16, each with contiguous rows (K-major) or contiguous columns (MN-major:
+// the gradient products dX = dZ W and dW = dZ^T X read the forward pass's matrices as they are).  Sums are
+// fp32.  The tensor core cuts its running sum off instead of rounding it, which drifts over a long K:
+// where C is fp32, pieces of 512 terms are summed in TMEM and joined in registers; where C has 16 bits one
+// piece covers all of K.
+//
+// Two kernels: pairs of CTAs on 256 x 256 tiles for large results, and a narrow one, with K split over a
+// cluster, for few rows of A or few tiles; gemm_dense_plan() below chooses.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
 
 #include "dense_ops.h"
+#include "gemm_parts.cuh"
 #include "nfx_internal.h"
 #include "numerics.cuh"
 #include "sm100.cuh"
@@ -15,110 +25,794 @@
 namespace nfx {
 namespace {
 
-// GELU's tanh form is z s(2u), s the logistic function, u = sqrt(2 / pi) (z + 0.044715 z^3).  -2u, in units
-// of log 2; where it is above kFar the value and the slope are under 2^-90 and are taken as zero.
-constexpr float kFar = 100.0f;
-__device__ __forceinline__ float gelu_exponent(float z) { return -2.302208198f * fmaf(z, (0.044715f * z) * z, z); }
-__device__ __forceinline__ float act_of(float z, int act) {
-    if (act == 1) {
-        const float t = gelu_exponent(z), e = exp2f(fminf(t, kFar));
-        return (t > kFar ? -0.0f : z) * __fdividef(1.0f, 1.0f + e);
-    }
-    return act == 2 ? relu_ref(z) : z;
+constexpr int kBK = 64;          // 128 bytes of K: one swizzled row
+constexpr int kPiece = 512 / kBK;  // blocks of K to a piece where C is fp32
+constexpr int kOutBytes = 32 * 128;
+
+// K-major tiles lie as rows of 128 bytes (64 of K), MN-major ones as 64 rows of K by 64 elements, one such box of
+// 8 KB after the other along MN; both with the 128-byte swizzle.  Their descriptors, and how far a step of
+// 16 along K is in units of 16 bytes.
+__device__ __forceinline__ uint64_t operand_desc(uint32_t addr, int t) {
+    if (!t) return umma_desc(addr, 128);
+    return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(8192 >> 4) << 16) |
+           (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ uint32_t operand_step(int t) { return t ? 16 * 128 / 16 : 32 / 16; }
+
+// kind::f16, fp32 D, M rows of D and n columns
+__device__ __forceinline__ uint32_t idesc_of(int type, int a_t, int b_t, int m, int n) {
+    const uint32_t f = type == kBF16 ? 1u : 0u;
+    return (1u << 4) | (f << 7) | (f << 10) | (static_cast<uint32_t>(a_t) << 15) | (static_cast<uint32_t>(b_t) << 16) |
+           (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
 
-constexpr int kT = 64, kTK = 16;
+__device__ __forceinline__ void mma_f16_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
 
-template <typename T>
-__global__ void __launch_bounds__(256) gemm_simple_kernel(GemmDenseArgs p) {
-    __shared__ float sa[kTK][kT + 1], sb[kTK][kT + 1];
-    const T* A = static_cast<const T*>(p.A);
-    const T* B = static_cast<const T*>(p.B);
-    const int m0 = blockIdx.x * kT, n0 = blockIdx.y * kT, tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    // pieces of 512 terms: one chain of roundings over a long K drifts
-    float acc[4][4] = {}, total[4][4] = {};
-    for (int k0 = 0; k0 < p.K; k0 += kTK) {
-        for (int e = threadIdx.x; e < kT * kTK; e += 256) {
-            const int ra = p.a_t ? e % kT : e / kTK, ka = p.a_t ? e / kT : e % kTK;
-            const int rb = p.b_t ? e % kT : e / kTK, kb = p.b_t ? e / kT : e % kTK;
-            const int64_t ma = m0 + ra, nb = n0 + rb;
-            sa[ka][ra] = ma < p.M && k0 + ka < p.K ? to_f32(A[p.a_t ? (k0 + ka) * p.lda + ma : ma * p.lda + k0 + ka]) : 0.0f;
-            sb[kb][rb] = nb < p.N && k0 + kb < p.K ? to_f32(B[p.b_t ? (k0 + kb) * p.ldb + nb : nb * p.ldb + k0 + kb]) : 0.0f;
+// The 16 bytes at chunk j of a staging row as numbers.
+template <int CT>
+__device__ __forceinline__ void add_chunk(uint4 v, float2 (&acc)[32], int j) {
+    if constexpr (CT == kF32) {
+        acc[2 * j].x += __uint_as_float(v.x), acc[2 * j].y += __uint_as_float(v.y);
+        acc[2 * j + 1].x += __uint_as_float(v.z), acc[2 * j + 1].y += __uint_as_float(v.w);
+    } else {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = unpack_half<CT>(w[i]);
+            acc[4 * j + i].x += f.x, acc[4 * j + i].y += f.y;
         }
-        __syncthreads();
-        for (int k = 0; k < kTK; ++k)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(sa[k][ty * 4 + i], sb[k][tx + 16 * j], acc[i][j]);
-        __syncthreads();
-        if ((k0 + kTK) % 512 == 0 || k0 + kTK >= p.K)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) total[i][j] += acc[i][j], acc[i][j] = 0.0f;
     }
-    for (int i = 0; i < 4; ++i)
+}
+
+// Element i of a matrix that may be written by this very call (an ordinary load).
+template <int CT>
+__device__ __forceinline__ float plain_load(const void* p, int64_t i) {
+    if constexpr (CT == kF32) return static_cast<const float*>(p)[i];
+    else if constexpr (CT == kBF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+    else return __half2float(static_cast<const __half*>(p)[i]);
+}
+
+// What the host finds out about the matrices of the epilogue: whether their rows allow TMA.
+struct Epi {
+    int tma_c, tma_z, tma_r;
+};
+
+// ---------------------------------------------------------------------------------------------------------
+// One tile is 256 x 256, computed by a pair of CTAs with cta_group::2 MMAs: CTA r holds rows 128 r .. of the
+// tile's A and of its B (each operand byte is fetched once per pair, 64 KB for 256 x 256 x 64 products), and rows
+// 128 r .. of the result in its TMEM, in two stages of 256 columns: the next tile's (or piece's) MMAs run
+// while this one's sums are read.  Warps of each CTA:
+//   0-15   epilogue, 32 rows x 64 columns each      16  TMA producer
+//   17     TMEM owner; CTA 0's issues the MMAs      18, 19  none
+// The epilogue's sums move to registers at once (64 a thread), so a TMEM stage is free again before the
+// arithmetic and the stores begin.  Registers: 16 x 32 x 112 + 4 x 32 x 32 = 20 x 32 x 96.
+// Barriers: full (CTA 0's, both CTAs' bytes), empty and accFull (both CTAs', by commit), accEmpty (CTA
+// 0's, arrivals from the epilogue warps of both), rFull (a warp's residual box).
+// ---------------------------------------------------------------------------------------------------------
+constexpr int kPairThreads = 640;
+constexpr int kPairEpi = 16;
+constexpr int kStages = 5;
+constexpr int kStageBytes = 2 * 128 * kBK * 2;
+constexpr int kOffOut = kStages * kStageBytes;
+constexpr int kOffBars = kOffOut + kPairEpi * kOutBytes;
+constexpr int kPairSmem = kOffBars + 8 * (2 * kStages + 2 * 2 + kPairEpi) + 16 + 1024;
+static_assert(kPairSmem <= 227 * 1024, "shared memory budget");
+
+// Rows m0 .., columns n .. (128 bytes of them) between a staging buffer and a matrix whose rows TMA cannot take.
+template <int EL, bool STORE>
+__device__ __forceinline__ void copy_rows(uint8_t* buf, void* mat, int64_t ld, int m0, int n, int rows, int cols, int lane) {
+    for (int r = 0; r < rows; ++r) {
+        uint8_t* g = static_cast<uint8_t*>(mat) + (static_cast<int64_t>(m0 + r) * ld + n) * EL;
+        for (int c = lane; c < cols; c += 32) {
+            uint8_t* s = buf + swz_offset(r * 128 + c * EL, 128);
+            if constexpr (EL == 4) {
+                if (STORE) *reinterpret_cast<uint32_t*>(g + c * 4) = *reinterpret_cast<const uint32_t*>(s);
+                else *reinterpret_cast<uint32_t*>(s) = *reinterpret_cast<const uint32_t*>(g + c * 4);
+            } else {
+                if (STORE) *reinterpret_cast<uint16_t*>(g + c * 2) = *reinterpret_cast<const uint16_t*>(s);
+                else *reinterpret_cast<uint16_t*>(s) = *reinterpret_cast<const uint16_t*>(g + c * 2);
+            }
+        }
+    }
+}
+
+template <int CT>
+struct PairEpilogue {
+    static constexpr int kEl = CT == kF32 ? 4 : 2;
+    static constexpr int kCols = 128 / kEl;  // columns of a box
+    static constexpr int kBoxes = 64 / kCols;
+    const GemmDenseArgs& p;
+    const Epi& e;
+    const CUtensorMap *tmC, *tmZ, *tmR;
+    uint8_t* buf;
+    uint64_t* rbar;
+    int lane;
+    uint32_t rphase;
+
+    // A TMA store clips a box at 16 bytes, not at the element: a last box whose row ends inside 16 bytes goes
+    // out by elements.
+    __device__ __forceinline__ bool whole(int n) const { return n + kCols <= p.N || p.N * kEl % 16 == 0; }
+
+    __device__ __forceinline__ void buffer_free() {
+        if (lane == 0) tma_store_wait_read<0>();
+        __syncwarp();
+    }
+    __device__ __forceinline__ void fetch_residual(int m0, int n) {
+        if (lane == 0) {
+            tma_store_wait_read<0>();
+            mbar_arrive_expect_tx(rbar, kOutBytes);
+            tma_load_2d(buf, tmR, rbar, n, m0);
+        }
+    }
+    __device__ __forceinline__ void put(const float2 (&acc)[32], int b) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<uint4*>(buf + swz_offset(lane * 128 + j * 16, 128)) = pack_chunk<CT, 32>(acc, b * 8 + j);
+    }
+    // the buffer to rows m0 .., columns n ..
+    __device__ __forceinline__ void store(const CUtensorMap* tm, int tma, void* mat, int64_t ld, int m0, int n) {
+        if (tma && whole(n)) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                tma_store_2d(tm, buf, n, m0);
+                tma_store_commit();
+            }
+        } else {
+            __syncwarp();
+            copy_rows<kEl, true>(buf, mat, ld, m0, n, min(32, p.M - m0), min(kCols, p.N - n), lane);
+            fence_proxy_async_smem();  // (a residual may land here next)
+            __syncwarp();
+        }
+    }
+    // Sums of rows m0 + lane, columns n0 .. n0 + 63; `fetched`: the first residual box is on its way.  False when a
+    // residual did not come.
+    __device__ __forceinline__ bool finish(float2 (&acc)[32], int m0, int n0, bool fetched, volatile int* abort, uint64_t budget) {
+        if (p.bias) {
+            float b[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int n = n0 + j * 32 + lane;
+                b[j] = n < p.N ? load_any(p.bias, p.btype, n) : 0.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+                acc[j].x += __shfl_sync(0xFFFFFFFFu, b[j >> 4], (2 * j) & 31);
+                acc[j].y += __shfl_sync(0xFFFFFFFFu, b[j >> 4], (2 * j + 1) & 31);
+            }
+        }
+        if (p.Z) {
+#pragma unroll
+            for (int b = 0; b < kBoxes; ++b) {
+                const int n = n0 + b * kCols;
+                if (n >= p.N) break;
+                buffer_free();
+                put(acc, b);
+                store(tmZ, e.tma_z, p.Z, p.ldz, m0, n);
+            }
+        }
+        if (p.act == 1) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) acc[j] = gelu_sig2(acc[j]);
+        } else if (p.act == 2) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) acc[j] = make_float2(relu_ref(acc[j].x), relu_ref(acc[j].y));
+        }
+#pragma unroll
+        for (int b = 0; b < kBoxes; ++b) {
+            const int n = n0 + b * kCols;
+            if (n >= p.N) break;
+            if (p.res) {
+                if (e.tma_r) {
+                    if (!fetched || b > 0) fetch_residual(m0, n);
+                    if (!mbar_wait(rbar, rphase, abort, budget)) return false;
+                    rphase ^= 1;
+                } else {
+                    buffer_free();
+                    copy_rows<kEl, false>(buf, const_cast<void*>(p.res), p.ldres, m0, n, min(32, p.M - m0), min(kCols, p.N - n), lane);
+                    __syncwarp();
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    add_chunk<CT>(*reinterpret_cast<const uint4*>(buf + swz_offset(lane * 128 + j * 16, 128)), acc, b * 8 + j);
+            } else {
+                buffer_free();
+            }
+            put(acc, b);
+            store(tmC, e.tma_c, p.C, p.ldc, m0, n);
+        }
+        return true;
+    }
+};
+
+template <int CT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmC,
+                 const __grid_constant__ CUtensorMap tmZ, const __grid_constant__ CUtensorMap tmR, const GemmDenseArgs p, const Epi e) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + kOffBars);
+    uint64_t* empty = full + kStages;
+    uint64_t* accFull = empty + kStages;
+    uint64_t* accEmpty = accFull + 2;
+    uint64_t* rFull = accEmpty + 2;
+    uint32_t* sTmem = reinterpret_cast<uint32_t*>(rFull + kPairEpi);
+    volatile int* sAbort = reinterpret_cast<volatile int*>(sTmem + 1);
+
+    const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0);  // (known to be the same in all lanes)
+    const int lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    const int tm = (p.M + 255) / 256, tn = (p.N + 255) / 256;
+    const int tiles = tm * tn;
+    const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
+    const int KB = (p.K + kBK - 1) / kBK;
+    const int piece = CT == kF32 ? kPiece : KB;  // blocks of K that one TMEM stage sums
+    const int pieces = KB == 0 ? 0 : (KB + piece - 1) / piece;
+    const uint64_t budget = p.wait_ns ? p.wait_ns : kWaitNs;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&accFull[s], 1);
+            mbar_init(&accEmpty[s], 2 * kPairEpi);
+        }
+        for (int s = 0; s < kPairEpi; ++s) mbar_init(&rFull[s], 1);
+        *sAbort = 0;
+        fence_mbar_init();
+    }
+    if (warp == kPairEpi + 1) tmem_alloc_pair(sTmem, 512);
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();  // both CTAs' barriers are ready
+    tc_fence_after();
+    const uint32_t tmem_base = *sTmem;
+
+    // the register split stands inside the roles' branches: where they met again, the compiler would
+    // have to assume the smaller count
+    if (warp >= kPairEpi) {
+        reg_dec<32>();
+        if (warp == kPairEpi) {
+            // ---------------- TMA producer
+            if (elect_one()) {
+                int it = 0;
+                bool ok = true;
+                for (int t = first; ok && t < tiles; t += step) {
+                    int mt, nt;
+                    tile_at(t, tm, tn, mt, nt);
+                    const int m = mt * 256 + rank * 128, n = nt * 256 + rank * 128;
+                    for (int kb = 0; kb < KB; ++kb, ++it) {
+                        const int s = it % kStages;
+                        if (!mbar_wait(&empty[s], ((it / kStages) & 1) ^ 1, sAbort, budget)) {
+                            *sAbort = 1;
+                            atomicOr(p.err, kErrWaitSlotFree);
+                            ok = false;
+                            break;
+                        }
+                        if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * kStageBytes);
+                        const uint32_t bar = map_rank(smem_u32(&full[s]), 0);
+                        uint8_t* st = smem + s * kStageBytes;
+                        if (p.a_t) {
+                            tma_load_2d_pair(st, &tmA, bar, m, kb * kBK);
+                            tma_load_2d_pair(st + 8192, &tmA, bar, m + 64, kb * kBK);
+                        } else {
+                            tma_load_2d_pair(st, &tmA, bar, kb * kBK, m);
+                        }
+                        if (p.b_t) {
+                            tma_load_2d_pair(st + 16384, &tmB, bar, n, kb * kBK);
+                            tma_load_2d_pair(st + 24576, &tmB, bar, n + 64, kb * kBK);
+                        } else {
+                            tma_load_2d_pair(st + 16384, &tmB, bar, kb * kBK, n);
+                        }
+                    }
+                }
+                // every load that was issued has landed and been read before the CTA exits
+                for (int j = it > kStages ? it - kStages : 0; j < it; ++j)
+                    if (!mbar_wait_drain(&empty[j % kStages], (j / kStages) & 1)) {
+                        atomicOr(p.err, kErrWaitDrain);
+                        break;
+                    }
+            }
+            __syncwarp();
+        } else if (warp == kPairEpi + 1) {
+            // ---------------- MMA issuer
+            if (rank == 0 && elect_one()) {
+                const uint32_t idesc = idesc_of(p.abtype, p.a_t, p.b_t, 256, 256);
+                const uint32_t astep = operand_step(p.a_t), bstep = operand_step(p.b_t);
+                int it = 0, acc = 0;  // blocks of K, TMEM stages handed over
+                bool ok = true;
+                for (int t = first; ok && t < tiles; t += step) {
+                    for (int kb = 0; kb < KB; ++kb, ++it) {
+                        const int s = it % kStages, in = kb % piece;
+                        const bool free = in > 0 || mbar_wait(&accEmpty[acc & 1], ((acc >> 1) & 1) ^ 1, sAbort, budget);
+                        if (!free || !mbar_wait(&full[s], (it / kStages) & 1, sAbort, budget)) {
+                            *sAbort = 1;
+                            atomicOr(p.err, free ? kErrWaitTmaFull : kErrWaitAccFree);
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint32_t ab = smem_u32(smem + s * kStageBytes);
+                        const uint64_t ad = operand_desc(ab, p.a_t), bd = operand_desc(ab + 16384, p.b_t);
+#pragma unroll
+                        for (int k = 0; k < kBK / 16; ++k)
+                            mma_f16_pair(tmem_base + (acc & 1) * 256, ad + k * astep, bd + k * bstep, idesc, in > 0 || k > 0 ? 1u : 0u);
+                        mma_commit_pair(&empty[s]);
+                        if (in == piece - 1 || kb == KB - 1) {
+                            mma_commit_pair(&accFull[acc & 1]);
+                            ++acc;
+                        }
+                    }
+                }
+                // the last commit completes before TMEM is released: the last block's stage is empty
+                if (it > 0 && !mbar_wait_drain(&empty[(it - 1) % kStages], ((it - 1) / kStages) & 1)) atomicOr(p.err, kErrWaitDrain);
+            }
+            __syncwarp();
+        }
+    } else {
+        // ---------------- epilogue
+        reg_inc<112>();
+        const uint32_t accEmpty0 = map_rank(smem_u32(accEmpty), 0);
+        const uint32_t tmem0 = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16) + (warp >> 2) * 64;
+        PairEpilogue<CT> epi{p, e, &tmC, &tmZ, &tmR, smem + kOffOut + warp * kOutBytes, &rFull[warp], lane, 0};
+        int acc_i = 0;
+        bool ok = true;
+        for (int t = first; ok && t < tiles; t += step) {
+            int mt, nt;
+            tile_at(t, tm, tn, mt, nt);
+            const int m0 = mt * 256 + rank * 128 + (warp & 3) * 32, n0 = nt * 256 + (warp >> 2) * 64;
+            const bool live = m0 < p.M && n0 < p.N;
+            const bool fetched = p.res && e.tma_r && !p.Z && live;
+            if (fetched) epi.fetch_residual(m0, n0);  // it comes while the tile's sums are formed
+            float2 acc[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) acc[j] = make_float2(0.0f, 0.0f);
+            for (int i = 0; i < pieces; ++i, ++acc_i) {
+                const int st = acc_i & 1;
+                if (!mbar_wait(&accFull[st], (acc_i >> 1) & 1, sAbort, budget)) {
+                    *sAbort = 1;
+                    atomicOr(p.err, kErrWaitAccFull);
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t r[32];
+                    tmem_read(tmem0 + st * 256 + c * 32, r);
+                    if (c == 1) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_cluster(accEmpty0 + st * 8);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const float2 v = make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
+                        if constexpr (CT == kF32) acc[c * 16 + j] = add2_rn(acc[c * 16 + j], v);
+                        else acc[c * 16 + j] = v;
+                    }
+                }
+            }
+            bool coming = fetched;  // a residual box that has not been waited for
+            if (ok && live) {
+                coming = !epi.finish(acc, m0, n0, fetched, sAbort, budget);
+                if (coming) {
+                    *sAbort = 1;
+                    atomicOr(p.err, kErrWaitTmaFull);
+                    ok = false;
+                }
+            }
+            if (coming && lane == 0 && !mbar_wait_drain(&rFull[warp], epi.rphase)) atomicOr(p.err, kErrWaitDrain);
+        }
+        if (lane == 0) tma_store_wait_all<0>();
+        __syncwarp();
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();  // neither CTA leaves while the other may still reach its shared memory
+    if (warp == kPairEpi + 1) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem_base, 512);
+    }
+}
+
+CUtensorMapDataType map_type(int t) {
+    return t == kF32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : t == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+}
+// Boxes of an operand: `rows` x 64 of K, or 64 of K by 64 along MN.
+bool operand_map(CUtensorMap* tm, int type, const void* base, int t, int64_t mn, int64_t k, int64_t ld, int rows) {
+    if (t) return encode_2d(tm, map_type(type), base, mn, k, ld * 2, 64, kBK, 128);
+    return encode_2d(tm, map_type(type), base, k, mn, ld * 2, kBK, rows, 128);
+}
+bool tma_rows(const void* p, int64_t ld, int type) {
+    return p && reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * type_bytes(type) % 16 == 0;
+}
+
+template <int CT>
+cudaError_t launch_pair(const GemmDenseArgs& p, cudaStream_t stream) {
+    CUtensorMap tmA{}, tmB{}, tmC{}, tmZ{}, tmR{};
+    if (p.K > 0 && (!operand_map(&tmA, p.abtype, p.A, p.a_t, p.M, p.K, p.lda, 128) || !operand_map(&tmB, p.abtype, p.B, p.b_t, p.N, p.K, p.ldb, 128)))
+        return cudaErrorInvalidValue;
+    constexpr int kEl = CT == kF32 ? 4 : 2;
+    // (a matrix of one row has no row stride to speak of)
+    const auto pitch = [&](int64_t ld) { return p.M == 1 ? (static_cast<int64_t>(p.N) + 7) / 8 * 8 : ld; };
+    Epi e{};
+    const auto map = [&](CUtensorMap* tm, const void* m, int64_t ld, int* on) {
+        *on = tma_rows(m, pitch(ld), CT);
+        return !*on || encode_2d(tm, map_type(CT), m, p.N, p.M, pitch(ld) * kEl, 128 / kEl, 32, 128);
+    };
+    if (!map(&tmC, p.C, p.ldc, &e.tma_c) || !map(&tmZ, p.Z, p.ldz, &e.tma_z) || !map(&tmR, p.res, p.ldres, &e.tma_r)) return cudaErrorInvalidValue;
+    auto kern = gemm_pair_kernel<CT>;
+    const cudaError_t err = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), kPairSmem);
+    if (err != cudaSuccess) return err;
+    const int64_t tiles = static_cast<int64_t>((p.M + 255) / 256) * ((p.N + 255) / 256);
+    const int pairs = device_sm_count() / 2;
+    kern<<<2 * static_cast<int>(tiles < pairs ? tiles : pairs), kPairThreads, kPairSmem, stream>>>(tmA, tmB, tmC, tmZ, tmR, p, e);
+    return cudaGetLastError();
+}
+
+// ---------------------------------------------------------------------------------------------------------
+// The narrow kernel, for few rows of A (a token to a few hundred): rows of B (weights) on the 128 lanes of the
+// MMA and NT rows of A as its columns, and K split over the CTAs of a cluster so that all SMs read weights.  Each
+// CTA sums its share of K, puts the partial tile into its shared memory, and after a cluster barrier every
+// CTA adds the partials of its columns in the order of the ranks (deterministic; no atomics, no
+// workspace), applies the epilogue and stores.  Up to NT = 64 two CTAs fit an SM; a grid that has no more CTAs
+// than SMs takes the memory of both for its own ring instead (DEEP).  Warps: four of epilogue for each 32
+// columns, then one TMA producer, one TMEM owner and MMA issuer.
+// ---------------------------------------------------------------------------------------------------------
+template <int NT, bool DEEP>
+struct NarrowCfg {
+    static constexpr int kPart = NT < 32 ? NT : 32;  // columns of an epilogue warp
+    static constexpr int kEpi = 4 * (NT / kPart);
+    static constexpr int kThreads = 32 * (kEpi + 2);
+    static constexpr int kPerSm = DEEP || NT > 64 ? 1 : 2;
+    static constexpr int kWBytes = 128 * kBK * 2;
+    static constexpr int kStageBytes = kWBytes + NT * kBK * 2;
+    static constexpr int kStages = (NT > 64 ? 196608 : (DEEP ? 204800 : 98304)) / kStageBytes;
+    static constexpr int kTmem = NT * 2 < 32 ? 32 : NT * 2;
+    static constexpr int kOffBars = kStages * kStageBytes;
+    static constexpr int kSmemBytes = kOffBars + 8 * (2 * kStages + 4) + 16 + 1024;
+    static_assert(kPerSm * (kSmemBytes + 1024) <= 228 * 1024, "CTAs per SM");
+    static_assert(128 * NT * 4 <= kStages * kStageBytes, "the partial tile takes the place of the stages");
+};
+
+template <int NT, int CT, bool DEEP>
+__global__ void __launch_bounds__(NarrowCfg<NT, DEEP>::kThreads, NarrowCfg<NT, DEEP>::kPerSm)
+gemm_narrow_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const GemmDenseArgs p, const int split) {
+    using C = NarrowCfg<NT, DEEP>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kOffBars);
+    uint64_t* empty = full + C::kStages;
+    uint64_t* accFull = empty + C::kStages;
+    uint64_t* accEmpty = accFull + 2;
+    uint32_t* sTmem = reinterpret_cast<uint32_t*>(accEmpty + 2);
+    volatile int* sAbort = reinterpret_cast<volatile int*>(sTmem + 1);
+
+    const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0);  // (known to be the same in all lanes)
+    const int lane = threadIdx.x & 31;
+    const int rank = blockIdx.x % split, tile = blockIdx.x / split;  // a cluster is `split` blocks in a row
+    const int tx = (p.M + NT - 1) / NT;
+    const int n0 = tile / tx * 128, m0 = tile % tx * NT;
+    const int KB = (p.K + kBK - 1) / kBK;
+    const int kb0 = static_cast<int>(static_cast<int64_t>(KB) * rank / split);
+    const int count = static_cast<int>(static_cast<int64_t>(KB) * (rank + 1) / split) - kb0;
+    const int piece = CT == kF32 ? kPiece : count;
+    const uint64_t budget = p.wait_ns ? p.wait_ns : kWaitNs;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::kStages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&accFull[s], 1);
+            mbar_init(&accEmpty[s], C::kEpi);
+        }
+        *sAbort = 0;
+        fence_mbar_init();
+    }
+    if (warp == C::kEpi + 1) tmem_alloc(sTmem, C::kTmem);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *sTmem;
+    float* part = reinterpret_cast<float*>(smem);  // (NT, 128) partial sums, after the last block
+
+    if (warp == C::kEpi) {
+        // ---------------- TMA producer
+        if (elect_one()) {
+            int it = 0;
+            for (; it < count; ++it) {
+                const int s = it % C::kStages, k = (kb0 + it) * kBK;
+                if (!mbar_wait(&empty[s], ((it / C::kStages) & 1) ^ 1, sAbort, budget)) {
+                    *sAbort = 1;
+                    atomicOr(p.err, kErrWaitSlotFree);
+                    break;
+                }
+                mbar_arrive_expect_tx(&full[s], C::kStageBytes);
+                uint8_t* st = smem + s * C::kStageBytes;
+                if (p.b_t) {
+                    tma_load_2d(st, &tmW, &full[s], n0, k);
+                    tma_load_2d(st + 8192, &tmW, &full[s], n0 + 64, k);
+                } else {
+                    tma_load_2d(st, &tmW, &full[s], k, n0);
+                }
+                if (NT >= 64 && p.a_t) {
+#pragma unroll
+                    for (int j = 0; j < NT / 64; ++j) tma_load_2d(st + C::kWBytes + j * 8192, &tmX, &full[s], m0 + j * 64, k);
+                } else {
+                    tma_load_2d(st + C::kWBytes, &tmX, &full[s], k, m0);
+                }
+            }
+            // every load that was issued lands before the CTA exits
+            for (int j = it > C::kStages ? it - C::kStages : 0; j < it; ++j)
+                if (!mbar_wait_drain(&full[j % C::kStages], (j / C::kStages) & 1)) {
+                    atomicOr(p.err, kErrWaitDrain);
+                    break;
+                }
+        }
+        __syncwarp();
+    } else if (warp == C::kEpi + 1) {
+        // ---------------- MMA issuer
+        if (elect_one()) {
+            const uint32_t idesc = idesc_of(p.abtype, p.b_t, p.a_t, 128, NT);
+            const uint32_t wstep = operand_step(p.b_t), xstep = operand_step(p.a_t);
+            int it = 0, acc = 0;
+            for (; it < count; ++it) {
+                const int s = it % C::kStages, in = it % piece;
+                const bool free = in > 0 || mbar_wait(&accEmpty[acc & 1], ((acc >> 1) & 1) ^ 1, sAbort, budget);
+                if (!free || !mbar_wait(&full[s], (it / C::kStages) & 1, sAbort, budget)) {
+                    *sAbort = 1;
+                    atomicOr(p.err, free ? kErrWaitTmaFull : kErrWaitAccFree);
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t wb = smem_u32(smem + s * C::kStageBytes);
+                const uint64_t wd = operand_desc(wb, p.b_t), xd = operand_desc(wb + C::kWBytes, p.a_t);
+#pragma unroll
+                for (int k = 0; k < kBK / 16; ++k)
+                    mma_f16(tmem_base + (acc & 1) * NT, wd + k * wstep, xd + k * xstep, idesc, in > 0 || k > 0 ? 1u : 0u);
+                mma_commit(&empty[s]);
+                if (in == piece - 1 || it == count - 1) {
+                    mma_commit(&accFull[acc & 1]);
+                    ++acc;
+                }
+            }
+            // the last commit completes before TMEM is released
+            if (it > 0 && !mbar_wait_drain(&empty[(it - 1) % C::kStages], ((it - 1) / C::kStages) & 1)) atomicOr(p.err, kErrWaitDrain);
+        }
+        __syncwarp();
+    } else {
+        // ---------------- the sums to registers, then to shared memory
+        constexpr int W = C::kPart;
+        const int quad = warp & 3, col0 = (warp >> 2) * W;
+        float2 acc[W / 2];
+#pragma unroll
+        for (int j = 0; j < W / 2; ++j) acc[j] = make_float2(0.0f, 0.0f);
+        bool ok = true;
+        for (int i = 0, done = 0; done < count; ++i, done += piece) {
+            if (!mbar_wait(&accFull[i & 1], (i >> 1) & 1, sAbort, budget)) {
+                *sAbort = 1;
+                atomicOr(p.err, kErrWaitAccFull);
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            uint32_t r[W];
+            tmem_read(tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + (i & 1) * NT + col0, r);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&accEmpty[i & 1]);
+#pragma unroll
+            for (int j = 0; j < W / 2; ++j)
+                acc[j] = add2_rn(acc[j], make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])));
+        }
+        // the last block's MMAs have read every stage: the partial tile goes in their place
+        if (ok) {
+#pragma unroll
+            for (int j = 0; j < W / 2; ++j) {
+                part[(col0 + 2 * j) * 128 + quad * 32 + lane] = acc[j].x;
+                part[(col0 + 2 * j + 1) * 128 + quad * 32 + lane] = acc[j].y;
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (split > 1) cluster_sync();  // the partial tiles of all ranks are there
+
+    // ---------------- join: this CTA's columns (rows of C), a warp per column, four rows of B a lane
+    const bool failed = *sAbort != 0;
+    const int cols = (NT + split - 1) / split;
+    constexpr int kEl = CT == kF32 ? 4 : 2;
+    const auto vec_of = [&](const void* m, int64_t ld) { return reinterpret_cast<uintptr_t>(m) % (4 * kEl) == 0 && (p.M == 1 || ld % 4 == 0); };
+    const bool vec_c = vec_of(p.C, p.ldc), vec_z = vec_of(p.Z, p.ldz), vec_r = vec_of(p.res, p.ldres);
+    const auto store4 = [&](void* mat, int64_t at, bool vec, int n, const float (&o)[4]) {
+        if (vec && n + 4 <= p.N) {
+            if constexpr (CT == kF32) {
+                *reinterpret_cast<float4*>(static_cast<float*>(mat) + at) = make_float4(o[0], o[1], o[2], o[3]);
+            } else {
+                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(mat) + at) =
+                    make_uint2(pack_half<CT>(make_float2(o[0], o[1])), pack_half<CT>(make_float2(o[2], o[3])));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (n + i < p.N) store_any(mat, CT, at + i, o[i]);
+        }
+    };
+    for (int c = rank * cols + warp; c < min(NT, (rank + 1) * cols) && !failed; c += C::kThreads / 32) {
+        const int m = m0 + c, n = n0 + lane * 4;
+        if (m >= p.M || n >= p.N) continue;
+        float4 v;
+        if (split == 1) {
+            v = *reinterpret_cast<const float4*>(part + c * 128 + lane * 4);
+        } else {
+            const uint32_t at = smem_u32(part + c * 128 + lane * 4);
+            v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            float4 w[8];
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+                if (r < split) w[r] = ld_cluster4(map_rank(at, r));
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+                if (r < split) v.x += w[r].x, v.y += w[r].y, v.z += w[r].z, v.w += w[r].w;
+        }
+        float o[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (p.bias && n + i < p.N) o[i] += load_any(p.bias, p.btype, n + i);
+        if (p.Z) store4(p.Z, static_cast<int64_t>(m) * p.ldz + n, vec_z, n, o);
+        if (p.act == 1) {
+            const float2 g0 = gelu_sig2(make_float2(o[0], o[1])), g1 = gelu_sig2(make_float2(o[2], o[3]));
+            o[0] = g0.x, o[1] = g0.y, o[2] = g1.x, o[3] = g1.y;
+        } else if (p.act == 2) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = relu_ref(o[i]);
+        }
+        if (p.res) {
+            const int64_t at = static_cast<int64_t>(m) * p.ldres + n;
+            if (vec_r && n + 4 <= p.N) {
+                if constexpr (CT == kF32) {
+                    const float4 r = *reinterpret_cast<const float4*>(static_cast<const float*>(p.res) + at);
+                    o[0] += r.x, o[1] += r.y, o[2] += r.z, o[3] += r.w;
+                } else {
+                    const uint2 r = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.res) + at);
+                    const float2 f0 = unpack_half<CT>(r.x), f1 = unpack_half<CT>(r.y);
+                    o[0] += f0.x, o[1] += f0.y, o[2] += f1.x, o[3] += f1.y;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (n + i < p.N) o[i] += plain_load<CT>(p.res, at + i);
+            }
+        }
+        store4(p.C, static_cast<int64_t>(m) * p.ldc + n, vec_c, n, o);
+    }
+
+    if (warp == C::kEpi + 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, C::kTmem);
+    }
+    if (split > 1) cluster_sync();  // no CTA leaves while another may still read its partial tile
+}
+
+template <int NT, int CT, bool DEEP>
+cudaError_t launch_narrow(const GemmDenseArgs& p, int split, cudaStream_t stream) {
+    using C = NarrowCfg<NT, DEEP>;
+    CUtensorMap tmW{}, tmX{};
+    if (p.K > 0 && (!operand_map(&tmW, p.abtype, p.B, p.b_t, p.N, p.K, p.ldb, 128) || !operand_map(&tmX, p.abtype, p.A, p.a_t, p.M, p.K, p.lda, NT)))
+        return cudaErrorInvalidValue;
+    auto kern = gemm_narrow_kernel<NT, CT, DEEP>;
+    const cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), C::kSmemBytes);
+    if (e != cudaSuccess) return e;
+    const int64_t tiles = static_cast<int64_t>((p.N + 127) / 128) * ((p.M + NT - 1) / NT);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(tiles * split));
+    cfg.blockDim = dim3(C::kThreads);
+    cfg.dynamicSmemBytes = C::kSmemBytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = static_cast<unsigned>(split);
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, tmW, tmX, p, split);
+}
+
+template <int CT>
+cudaError_t dispatch(const GemmDenseArgs& p, cudaStream_t stream) {
+    const DensePlan c = gemm_dense_plan(p.M, p.N, p.K, p.a_t, device_sm_count());
+    if (c.columns == 0) return launch_pair<CT>(p, stream);
+    if (c.columns == 16) return c.deep ? launch_narrow<16, CT, true>(p, c.split, stream) : launch_narrow<16, CT, false>(p, c.split, stream);
+    if (c.columns == 32) return c.deep ? launch_narrow<32, CT, true>(p, c.split, stream) : launch_narrow<32, CT, false>(p, c.split, stream);
+    if (c.columns == 64) return c.deep ? launch_narrow<64, CT, true>(p, c.split, stream) : launch_narrow<64, CT, false>(p, c.split, stream);
+    return launch_narrow<128, CT, true>(p, c.split, stream);
+}
+
+// ---------------------------------------------------------------------------------------------------------
+// Operands that TMA cannot read (base or row stride no multiple of 16 bytes) are copied first, rows on 16-byte
+// boundaries.
+// ---------------------------------------------------------------------------------------------------------
+__global__ void __launch_bounds__(256) align_rows_kernel(const uint16_t* src, int64_t ld, int64_t rows, int64_t cols, uint16_t* dst, int64_t ldd) {
+    const int64_t packs = ldd / 8, all = rows * packs;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < all; i += static_cast<int64_t>(gridDim.x) * 256) {
+        const int64_t r = i / packs, c = i % packs * 8;
+        const uint16_t* s = src + r * ld + c;
+        uint32_t w[4];
+#pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int64_t m = m0 + ty * 4 + i, n = n0 + tx + 16 * j;
-            if (m >= p.M || n >= p.N) continue;
-            float z = total[i][j];
-            if (p.bias) z += load_any(p.bias, p.btype, n);
-            if (p.Z) store_any(p.Z, p.ctype, m * p.ldz + n, z);
-            z = act_of(z, p.act);
-            if (p.res) z += load_any(p.res, p.ctype, m * p.ldres + n);
-            store_any(p.C, p.ctype, m * p.ldc + n, z);
+            const uint32_t lo = c + 2 * j < cols ? s[2 * j] : 0, hi = c + 2 * j + 1 < cols ? s[2 * j + 1] : 0;
+            w[j] = lo | hi << 16;
         }
-}
-
-// The slope of the activation.  GELU's is s + z s (1 - s) (2u)', with 1 - s as e s, e = e^(-2u) (the
-// difference would lose the digits that z (2u)' multiplies); beyond |z| = 30 it is 0 or 1.
-__device__ __forceinline__ float slope_of(float z, int act) {
-    if (act == 2) return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
-    if (act != 1) return 1.0f;
-    const float c = fminf(fmaxf(z, -30.0f), 30.0f), t = gelu_exponent(c), e = exp2f(fminf(t, kFar)), s = __fdividef(1.0f, 1.0f + e);
-    const float v = fmaf(c * s * (e * s), 1.5957691216057308f * fmaf(0.134145f * c, c, 1.0f), s);
-    return z != z ? z : (t > kFar ? 0.0f : v);
-}
-
-// A block takes 256 columns of a share of the rows, one column a thread: the column's sum stays in a register.
-template <typename T>
-__global__ void __launch_bounds__(256) act_grad_kernel(ActGradArgs a) {
-    const int64_t c = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    const int64_t r0 = a.rows * blockIdx.y / gridDim.y, r1 = a.rows * (blockIdx.y + 1) / gridDim.y;
-    if (c >= a.cols) return;
-    float s = 0.0f;
-    for (int64_t r = r0; r < r1; ++r) {
-        float v = to_f32(static_cast<const T*>(a.dy)[r * a.lddy + c]);
-        if (a.act) v *= slope_of(to_f32(static_cast<const T*>(a.z)[r * a.ldz + c]), a.act);
-        s += v;
-        if (a.dz) static_cast<T*>(a.dz)[r * a.lddz + c] = from_f32<T>(v);
+        *reinterpret_cast<uint4*>(dst + r * ldd + c) = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    if (a.part) a.part[blockIdx.y * a.cols + c] = s;
 }
+
+bool tma_operand(const void* p, int64_t ld, int64_t rows) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (rows <= 1 || ld % 8 == 0); }
+int64_t up8(int64_t v) { return (v + 7) / 8 * 8; }
 
 }  // namespace
 
-int64_t gemm_dense_workspace(const void*, int64_t, int, const void*, int64_t, int, int64_t, int64_t, int64_t) { return 0; }
-
-cudaError_t gemm_dense_launch(const GemmDenseArgs& p, cudaStream_t s) {
-    const dim3 grid((p.M + kT - 1) / kT, (p.N + kT - 1) / kT);
-    if (p.abtype == kBF16) gemm_simple_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(p);
-    else gemm_simple_kernel<__half><<<grid, 256, 0, s>>>(p);
-    return cudaGetLastError();
+// Which kernel, and how it is cut (see the figures in the body).
+DensePlan gemm_dense_plan(int64_t M, int64_t N, int64_t K, int a_t, int64_t sms) {
+    const auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+    const int64_t KB = up(K, kBK);
+    constexpr int kCost[4] = {20, 24, 32, 42}, kJoin[4] = {70, 100, 150, 250};  // hundredths of a microsecond
+    int nt = a_t ? 64 : 16, split = 1;
+    int64_t best = -1;
+    for (int i = a_t ? 2 : 0; i < 4; ++i) {
+        const int w = 16 << i;
+        if (w > nt && w / 2 >= M) break;
+        for (int s = 1; s <= 8 && (s == 1 || 2 * s <= KB); s *= 2) {
+            const int64_t ctas = up(N, 128) * up(M, w) * s;
+            const int64_t rounds = up(ctas, s >= 4 && sms > 1 ? sms * 7 / 8 : sms);
+            const int64_t cost = 430 + rounds * up(KB, s) * kCost[i] + (rounds - 1) * 250 + (s > 1 ? kJoin[i] : 0);
+            if (best < 0 || cost < best) best = cost, nt = w, split = s;
+        }
+    }
+    const int64_t rounds = sms > 1 ? up(up(M, 256) * up(N, 256), sms / 2) : 0;
+    if (sms > 1 && 650 + rounds * KB * 41 + (rounds - 1) * 220 < best) return {0, 1, false};
+    return {nt, split, nt == 128 || up(N, 128) * up(M, nt) * split <= sms};
 }
 
-int act_grad_parts(int64_t rows, int64_t cols) {
-    const int64_t want = (rows + 31) / 32;
-    return static_cast<int>(want < 256 ? want : 256);
+int64_t gemm_dense_workspace(const void* A, int64_t lda, int a_t, const void* B, int64_t ldb, int b_t, int64_t M, int64_t N, int64_t K) {
+    const int64_t ra = a_t ? K : M, ca = a_t ? M : K, rb = b_t ? K : N, cb = b_t ? N : K;
+    return (tma_operand(A, lda, ra) ? 0 : 2 * ra * up8(ca)) + (tma_operand(B, ldb, rb) ? 0 : 2 * rb * up8(cb));
 }
 
-cudaError_t act_grad_launch(const ActGradArgs& a, int type, cudaStream_t s) {
-    const dim3 grid(static_cast<unsigned>((a.cols + 255) / 256), a.parts);
-    if (type == kF32) act_grad_kernel<float><<<grid, 256, 0, s>>>(a);
-    else if (type == kBF16) act_grad_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(a);
-    else act_grad_kernel<__half><<<grid, 256, 0, s>>>(a);
-    return cudaGetLastError();
+cudaError_t gemm_dense_launch(const GemmDenseArgs& args, cudaStream_t stream) {
+    GemmDenseArgs p = args;
+    p.wait_ns = debug_wait_budget_ns();
+    uint16_t* room = static_cast<uint16_t*>(p.ws);
+    const auto align = [&](const void*& base, int64_t& ld, int64_t rows, int64_t cols) {
+        if (p.K == 0) return cudaSuccess;
+        if (tma_operand(base, ld, rows)) {
+            if (rows <= 1) ld = up8(cols);
+            return cudaSuccess;
+        }
+        const int64_t ldd = up8(cols), blocks = (rows * ldd / 8 + 255) / 256, most = 16ll * device_sm_count();
+        align_rows_kernel<<<static_cast<unsigned>(blocks < most ? blocks : most), 256, 0, stream>>>(static_cast<const uint16_t*>(base), ld, rows,
+                                                                                                   cols, room, ldd);
+        base = room, ld = ldd, room += rows * ldd;
+        return cudaGetLastError();
+    };
+    cudaError_t e = align(p.A, p.lda, p.a_t ? p.K : p.M, p.a_t ? p.M : p.K);
+    if (e == cudaSuccess) e = align(p.B, p.ldb, p.b_t ? p.K : p.N, p.b_t ? p.N : p.K);
+    if (e != cudaSuccess) return e;
+    if (p.ctype == kF32) return dispatch<kF32>(p, stream);
+    return p.ctype == kBF16 ? dispatch<kBF16>(p, stream) : dispatch<kF16>(p, stream);
 }
 
 }  // namespace nfx

@@ -182,37 +182,6 @@ __global__ void __launch_bounds__(1024) column_reduce_kernel(const float* part, 
 // the 128 elements of an FP8 group lie in one warp: half a warp's pack (16-bit types), one pack (fp32)
 // or four (VE = 1), and its maximum is a few shuffles.
 // ---------------------------------------------------------------------------
-// VE parameters (of x's type or fp32) from element i; `vec` when they are 16-byte aligned.
-template <typename T, int VE>
-__device__ __forceinline__ void load_params(const void* p, int type, bool vec, int i, float none, float (&o)[VE]) {
-    if (!p) {
-#pragma unroll
-        for (int k = 0; k < VE; ++k) o[k] = none;
-    } else if (VE > 2 && vec && type == kF32) {
-#pragma unroll
-        for (int k = 0; k < VE; k += 4) {
-            const float4 f = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + i + k));
-            o[k] = f.x, o[k + 1] = f.y, o[k + 2] = f.z, o[k + 3] = f.w;
-        }
-    } else if (VE == 8 && vec) {
-        const uint4 u = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i));
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int k = 0; k < VE; k += 2) {
-            float2 f;
-            if (type == kBF16) f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[k / 2]));
-            else f = __half22float2(*reinterpret_cast<const __half2*>(&w[k / 2]));
-            o[k] = f.x, o[k + 1] = f.y;
-        }
-    } else if (type == kF32) {
-#pragma unroll
-        for (int k = 0; k < VE; ++k) o[k] = __ldg(static_cast<const float*>(p) + i + k);
-    } else {
-#pragma unroll
-        for (int k = 0; k < VE; ++k) o[k] = load_any(p, type, i + k);
-    }
-}
-
 // Sums of (a, b) over the TPR threads of a row, the same bits in each of them; of a alone without TWO.
 template <int TPR, bool TWO>
 __device__ __forceinline__ float2 row_sums(float a, float b, float2* red) {

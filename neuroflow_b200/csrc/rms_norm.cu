@@ -1,17 +1,17 @@
 // rms_norm.cu -- root-mean-square norm over the last dimension of (rows, d) with the residual's addition,
-// forward (into the input's type, or straight into FP8 groups of 128) and backward.
+// into the input's type or straight into FP8 groups of 128.
 //
 //   h = x + res, rounded to the residual's type;  r = 1 / sqrt(sum h^2 / d + eps)
 //   y = h r gamma
-//   a = gamma dy,  xh = h r,  dh = r (a - xh mean(a xh)) + dsum
-//   dgamma = sum over rows of dy xh
 //
 // The norm is that of the sum as it is stored, so the backward pass, which reads the stored sum, is the
 // gradient of exactly what was computed.  All sums are fp32.
+#include <atomic>
+
 #include "dense_ops.h"
 #include "nfx_internal.h"
 #include "numerics.cuh"
-#include "row_pack.cuh"
+#include "rms_parts.cuh"
 #include "sm100.cuh"
 
 namespace nfx {
@@ -85,46 +85,262 @@ __global__ void __launch_bounds__(kAnyThreads) rms_any_kernel(RmsArgs a) {
     }
 }
 
-// Any width: a block takes every gridDim.x-th row and adds its rows' parameter gradients, in their order,
-// to its own row of partial sums (each column always by one thread).
-template <typename T, typename H>
-__global__ void __launch_bounds__(kAnyThreads) rms_grad_any_kernel(RmsGradArgs a) {
-    __shared__ float red[kAnyThreads / 32];
-    float* pg = a.part + static_cast<int64_t>(blockIdx.x) * a.d;
-    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-        const T* dy = static_cast<const T*>(a.dy) + r * a.lddy;
-        const H* h = static_cast<const H*>(a.h) + r * a.ldh;
-        const H* ds = a.dsum ? static_cast<const H*>(a.dsum) + r * a.lddsum : nullptr;
-        const float rs = a.rstd[r];
-        float s = 0.0f;
-        for (int i = threadIdx.x; i < a.d; i += kAnyThreads) {
-            const float xh = to_f32(h[i]) * rs, g = to_f32(dy[i]);
-            s = fmaf(a.gamma ? g * load_any(a.gamma, a.ptype, i) : g, xh, s);
-            if (a.part) pg[i] = fmaf(g, xh, r == blockIdx.x ? 0.0f : pg[i]);
+// ---------------------------------------------------------------------------------------------------------
+// The row in registers: read once, written from there.  TPR threads per row, each holding VPT packs of VE
+// elements (16 bytes of x); pack j of lane l of warp w is (w VPT + j) 32 + l of the row, so the 128
+// elements of an FP8 group lie in one warp.  Resident blocks walk over the rows: the next row is
+// fetched while this one is worked on, and gamma stays where it is, in registers, or in shared memory for rows
+// over 4,096 columns.  EDGE: rows start and end anywhere (rms_parts.cuh); then an FP8 row goes through
+// shared memory to reach its groups.
+// ---------------------------------------------------------------------------------------------------------
+constexpr int row_block(int tpr) { return tpr > 128 ? tpr : 128; }
+constexpr int row_blocks(int tpr, int regs) { return tpr >= 512 ? (regs <= 32 ? 2 : 1) : 768 / row_block(tpr); }
+// registers of a row that is on its way: x and the residual
+constexpr int row_regs(int n, int xb, int hb) { return n * (xb + hb) / 4; }
+
+template <typename T, typename H, int VE, int VPT, int TPR, bool FP8, bool EDGE>
+__global__ void __launch_bounds__(row_block(TPR), row_blocks(TPR, row_regs(VE * VPT, sizeof(T), sizeof(H)) + VE * VPT))
+rms_row_kernel(RmsArgs a, Shift sh, bool gvec, bool wide) {
+    __shared__ float red[2][row_block(TPR) / 32];
+    extern __shared__ __align__(16) float room[];  // gamma (rows over 4,096 columns), then rows on their way to FP8
+    constexpr int kRows = row_block(TPR) / TPR, N = VPT * VE, kPacks = TPR * VPT;
+    constexpr bool kGammaShared = TPR >= 512;
+    const int lane = threadIdx.x & 31, sub = threadIdx.x % TPR, mine = threadIdx.x / TPR;
+    const int first = TPR < 32 ? sub : (sub >> 5) * VPT * 32 + lane;
+    const float inv_d = __frcp_rn(static_cast<float>(a.d));
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
+    // (the launcher makes `step` rows a whole number of boundaries: s is the same in all rows of a thread)
+    const int s = EDGE ? static_cast<int>((sh.base + (static_cast<int64_t>(blockIdx.x) * kRows + mine) * sh.step) % VE) : 0;
+    const auto column = [&](int j) { return (first + j * 32) * VE - s; };
+    const auto inside = [&](int c) { return EDGE ? c >= 0 && c + VE <= a.d : c < a.d; };  // without EDGE a row is whole packs
+    const auto touches = [&](int c) { return c < a.d && c + VE > 0; };
+
+    Elems<T, VE> rx[VPT];
+    Elems<H, VE> rr[VPT];
+    const auto fetch = [&](int64_t r) {
+        const T* x = static_cast<const T*>(a.x) + r * a.ldx;
+        const H* res = static_cast<const H*>(a.res) + r * a.ldres;
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            const int c = column(j);
+            if (r < a.rows && inside(c)) {
+                rx[j].load(x + c);
+                if (a.res) rr[j].load(res + c);
+            } else if (EDGE && VE > 1 && r < a.rows && touches(c)) {
+                rx[j].load_part(x, c, a.d);
+                if (a.res) rr[j].load_part(res, c, a.d);
+            } else {
+                rx[j].zero();
+                rr[j].zero();
+            }
         }
-        s = __fdiv_rn(block_sum(s, red), static_cast<float>(a.d));
-        for (int i = threadIdx.x; i < a.d; i += kAnyThreads) {
-            const float xh = to_f32(h[i]) * rs, g = to_f32(dy[i]);
-            float o = rs * fmaf(-xh, s, a.gamma ? g * load_any(a.gamma, a.ptype, i) : g);
-            if (ds) o += to_f32(ds[i]);
-            if (a.dx) static_cast<T*>(a.dx)[r * a.lddx + i] = from_f32<T>(o);
-            if (a.dres) static_cast<H*>(a.dres)[r * a.lddres + i] = from_f32<H>(o);
+    };
+    fetch(static_cast<int64_t>(blockIdx.x) * kRows + mine);
+    float gam[kGammaShared ? 1 : VPT][VE];
+    if constexpr (kGammaShared) {
+        for (int i = threadIdx.x; i < kPacks * VE; i += TPR)
+            room[i] = a.gamma && i - s >= 0 && i - s < a.d ? load_any(a.gamma, a.ptype, i - s) : 1.0f;
+        __syncthreads();
+    } else {
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            const int c = column(j);
+            if (!EDGE && c < a.d) {
+                load_params<T, VE>(a.gamma, a.ptype, gvec, c, 1.0f, gam[j]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < VE; ++i) gam[j][i] = EDGE && a.gamma && c + i >= 0 && c + i < a.d ? load_any(a.gamma, a.ptype, c + i) : 1.0f;
+            }
+        }
+    }
+    int buf = 0;
+    for (int64_t base = static_cast<int64_t>(blockIdx.x) * kRows; base < a.rows; base += step, buf ^= 1) {
+        const int64_t r = base + mine;
+        const bool live = r < a.rows;
+        float v[VPT][VE];
+        float2 q2 = make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            rx[j].get(v[j]);
+            if (a.res) {
+                float h[VE];
+                rr[j].get(h);
+#pragma unroll
+                for (int i = 0; i < VE; ++i) v[j][i] += h[i];
+                Elems<H, VE> o;
+                o.set(v[j]);  // the norm is that of the sum as it is stored
+                o.get(v[j]);
+                if (a.sum && live) {
+                    H* sum = static_cast<H*>(a.sum) + r * a.ldsum;
+                    const int c = column(j);
+                    if (inside(c)) o.store(sum + c);
+                    else if (EDGE && VE > 1 && touches(c)) o.store_part(sum, c, a.d);
+                }
+            }
+            if constexpr (VE == 1) {
+                q2.x = fmaf(v[j][0], v[j][0], q2.x);
+            } else {
+#pragma unroll
+                for (int i = 0; i < VE; i += 2) {
+                    const float2 f = make_float2(v[j][i], v[j][i + 1]);
+                    q2 = fma2_rn(f, f, q2);
+                }
+            }
+        }
+        fetch(r + step);  // the next row comes while this one is worked on
+        const float rs = __frsqrt_rn(row_sum<TPR>(q2.x + q2.y, red[buf]) * inv_d + a.eps);
+        if (live && sub == 0 && a.rstd) a.rstd[r] = rs;
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            const int c = column(j);
+            float g[VE];
+            if constexpr (kGammaShared && VE > 1) {
+#pragma unroll
+                for (int i = 0; i < VE; i += 4) {
+                    const float4 f = *reinterpret_cast<const float4*>(room + (first + j * 32) * VE + i);
+                    g[i] = f.x, g[i + 1] = f.y, g[i + 2] = f.z, g[i + 3] = f.w;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < VE; ++i) g[i] = kGammaShared ? room[(first + j * 32) * VE + i] : gam[j][i];
+            }
+            if constexpr (VE == 1) {
+                v[j][0] = (v[j][0] * rs) * g[0];
+            } else {
+#pragma unroll
+                for (int i = 0; i < VE; i += 2) {
+                    const float2 y = mul2_rn(mul2_rn(make_float2(v[j][i], v[j][i + 1]), make_float2(rs, rs)), make_float2(g[i], g[i + 1]));
+                    v[j][i] = y.x, v[j][i + 1] = y.y;
+                }
+            }
+            if constexpr (!FP8) {
+                if (live) {
+                    T* y = static_cast<T*>(a.y) + r * a.ldy;
+                    Elems<T, VE> o;
+                    o.set(v[j]);
+                    if (inside(c)) o.store(y + c);
+                    else if (EDGE && VE > 1 && touches(c)) o.store_part(y, c, a.d);
+                }
+            }
+        }
+        if constexpr (FP8 && !EDGE) {
+            store_codes<VE, VPT, TPR>(v, a.q, r, a.d, live, first, lane, wide);
+        } else if constexpr (FP8) {
+            // through shared memory to groups of 128 columns, a warp each, four columns a lane
+            const int padded = (a.d + kGroup - 1) / kGroup * kGroup;
+            float* row = room + (kGammaShared ? kPacks * VE : 0) + mine * padded;
+#pragma unroll
+            for (int j = 0; j < VPT; ++j)
+#pragma unroll
+                for (int i = 0; i < VE; ++i)
+                    if (const int c = column(j) + i; c >= 0 && c < a.d) row[c] = v[j][i];
+            if constexpr (TPR > 32) __syncthreads();
+            else __syncwarp();
+            constexpr int kWarps = TPR < 32 ? 1 : TPR / 32;
+            for (int b = TPR < 32 ? 0 : sub >> 5; b < padded / kGroup; b += kWarps) {
+                const int c = b * kGroup + lane * 4;
+                float o[4], top = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    o[i] = c + i < a.d ? row[c + i] : 0.0f;
+                    top = fmaxf(top, finite_abs(o[i]));
+                }
+                const float sc = group_scale(warp_max(top)), inv = __frcp_rn(sc);
+                uint32_t odd = 0, w = scaled_codes<false>(o[0], o[1], o[2], o[3], inv, odd);
+                if (odd) w = scaled_codes<true>(o[0], o[1], o[2], o[3], inv, odd);
+                if (!live || c >= a.d) continue;
+                if (lane == 0) a.q.scales[r * a.q.srs + b * a.q.sbs] = sc;
+                uint8_t* dst = a.q.codes + r * a.q.ld + c;
+                if (wide && c + 4 <= a.d) {
+                    *reinterpret_cast<uint32_t*>(dst) = w;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (c + i < a.d) dst[i] = static_cast<uint8_t>(w >> (8 * i));
+                }
+            }
+            if constexpr (TPR <= 32) __syncwarp();  // (with more warps the next row's sum has a barrier)
         }
     }
 }
 
-template <typename T, typename H>
-cudaError_t rms_t(const RmsArgs& a, cudaStream_t s) {
+template <typename T, typename H, int VE, int VPT, int TPR, bool FP8, bool EDGE>
+cudaError_t rms_row_go(const RmsArgs& a, cudaStream_t s) {
+    constexpr int kThreads = row_block(TPR), kRows = kThreads / TPR;
+    auto kern = rms_row_kernel<T, H, VE, VPT, TPR, FP8, EDGE>;
+    const int gamma = TPR >= 512 ? TPR * VPT * VE * 4 : 0;
+    const int rows = FP8 && EDGE ? kRows * ((a.d + kGroup - 1) / kGroup * kGroup) * 4 : 0;
+    // the most that any width of this kernel asks for decides how many blocks an SM holds
+    constexpr int kMost = (TPR >= 512 ? TPR * VPT * VE * 4 : 0) + (FP8 && EDGE ? kRows * (TPR * VPT * VE + kGroup) * 4 : 0);
+    const cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), kMost);
+    if (e != cudaSuccess) return e;
+    static std::atomic<int> known[64];  // asked for once per kernel and device
+    const int d = current_device() & 63;
+    int most = known[d].load(std::memory_order_relaxed);
+    if (most == 0) {
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&most, kern, kThreads, kMost) != cudaSuccess || most < 1) most = 1;
+        most *= device_sm_count();
+        known[d].store(most, std::memory_order_relaxed);
+    }
+    const int64_t want = (a.rows + kRows - 1) / kRows;
+    int64_t grid = want < most ? want : most;
+    if (EDGE && VE > 1 && grid < want) grid = grid >= VE ? grid / VE * VE : VE;  // steps of whole boundaries
+    const Shift sh = shift_of(a.x, a.ldx, sizeof(T), VE);
+    const bool gvec = aligned16(a.gamma) && (a.ptype == kF32 || VE == 8);
+    const bool wide = FP8 && reinterpret_cast<uintptr_t>(a.q.codes) % 8 == 0 && (a.rows == 1 || a.q.ld % 8 == 0);
+    kern<<<static_cast<unsigned>(grid), kThreads, gamma + rows, s>>>(a, sh, gvec, wide);
+    return cudaGetLastError();
+}
+
+// 16 elements a thread up to 8,192 columns and 32 above; whole packs have a kernel for each width, rows with
+// edges one for every second.
+template <typename T, typename H, int VE, bool FP8>
+cudaError_t rms_whole(const RmsArgs& a, cudaStream_t s) {
+    constexpr int k16 = 16 / VE;
+    if (a.d <= 32 * VE) return rms_row_go<T, H, VE, 1, 32, FP8, false>(a, s);
+    if (a.d <= 512) return rms_row_go<T, H, VE, k16, 32, FP8, false>(a, s);
+    if (a.d <= 1024) return rms_row_go<T, H, VE, k16, 64, FP8, false>(a, s);
+    if (a.d <= 2048) return rms_row_go<T, H, VE, k16, 128, FP8, false>(a, s);
+    if (a.d <= 4096) return rms_row_go<T, H, VE, k16, 256, FP8, false>(a, s);
+    if (a.d <= 8192) return rms_row_go<T, H, VE, k16, 512, FP8, false>(a, s);
+    return rms_row_go<T, H, VE, 2 * k16, 512, FP8, false>(a, s);
+}
+template <typename T, typename H, int VE, bool FP8>
+cudaError_t rms_edge(const RmsArgs& a, cudaStream_t s) {
+    constexpr int k16 = 16 / VE;
+    const int d = a.d + VE - 1;  // the first pack may begin before the row
+    if (d <= 512) return rms_row_go<T, H, VE, k16, 32, FP8, true>(a, s);
+    if (d <= 1024) return rms_row_go<T, H, VE, k16, 64, FP8, true>(a, s);
+    if (d <= 2048) return rms_row_go<T, H, VE, k16, 128, FP8, true>(a, s);
+    if (d <= 4096) return rms_row_go<T, H, VE, k16, 256, FP8, true>(a, s);
+    return rms_row_go<T, H, VE, 2 * k16, 512, FP8, true>(a, s);
+}
+template <typename T, typename H, bool FP8>
+cudaError_t rms_single(const RmsArgs& a, cudaStream_t s) {
+    if (a.d <= 1024) return rms_row_go<T, H, 1, 8, 128, FP8, true>(a, s);
+    if (a.d <= 4096) return rms_row_go<T, H, 1, 16, 256, FP8, true>(a, s);
+    return rms_row_go<T, H, 1, 32, 512, FP8, true>(a, s);
+}
+
+template <typename T, typename H, bool FP8>
+cudaError_t rms_form(const RmsArgs& a, cudaStream_t s) {
+    constexpr int VE = 16 / sizeof(T);
+    if (a.d <= 16384 - VE + 1 || (a.d <= 16384 && a.d % VE == 0)) {
+        const Shift sx = shift_of(a.x, a.ldx, sizeof(T), VE);
+        const auto like = [&](const void* p, int64_t ld, int64_t el) { return !p || same_shift(sx, shift_of(p, ld, el, VE), a.rows); };
+        if (like(a.res, a.ldres, sizeof(H)) && like(a.sum, a.ldsum, sizeof(H)) && (FP8 || like(a.y, a.ldy, sizeof(T)))) {
+            if (sx.base == 0 && (a.rows == 1 || sx.step == 0) && a.d % VE == 0) return rms_whole<T, H, VE, FP8>(a, s);
+            if (a.d <= 16384 - VE + 1) return rms_edge<T, H, VE, FP8>(a, s);
+        }
+    }
+    if (a.d <= 16384) return rms_single<T, H, FP8>(a, s);
     const int64_t cap = 8ll * device_sm_count();
     rms_any_kernel<T, H><<<static_cast<int>(a.rows < cap ? a.rows : cap), kAnyThreads, 0, s>>>(a);
     return cudaGetLastError();
 }
-
 template <typename T, typename H>
-cudaError_t rms_grad_t(RmsGradArgs& a, cudaStream_t s) {
-    if (a.rows == 0) return cudaSuccess;
-    rms_grad_any_kernel<T, H><<<a.parts, kAnyThreads, 0, s>>>(a);
-    return cudaGetLastError();
+cudaError_t rms_t(const RmsArgs& a, cudaStream_t s) {
+    return a.y ? rms_form<T, H, false>(a, s) : rms_form<T, H, true>(a, s);
 }
 
 }  // namespace
@@ -133,21 +349,6 @@ cudaError_t rms_norm_launch(const RmsArgs& a, int xtype, int htype, cudaStream_t
     if (xtype == kF32) return rms_t<float, float>(a, s);
     if (xtype == kBF16) return htype == kF32 ? rms_t<__nv_bfloat16, float>(a, s) : rms_t<__nv_bfloat16, __nv_bfloat16>(a, s);
     return htype == kF32 ? rms_t<__half, float>(a, s) : rms_t<__half, __half>(a, s);
-}
-
-int rms_norm_parts(int64_t rows, int64_t d) {
-    const int64_t cap = 4ll * device_sm_count();
-    return static_cast<int>(rows < cap ? rows : cap);
-}
-
-cudaError_t rms_norm_backward_launch(const RmsGradArgs& args, int dytype, int htype, cudaStream_t s) {
-    RmsGradArgs a = args;
-    cudaError_t e;
-    if (dytype == kF32) e = rms_grad_t<float, float>(a, s);
-    else if (dytype == kBF16) e = htype == kF32 ? rms_grad_t<__nv_bfloat16, float>(a, s) : rms_grad_t<__nv_bfloat16, __nv_bfloat16>(a, s);
-    else e = htype == kF32 ? rms_grad_t<__half, float>(a, s) : rms_grad_t<__half, __half>(a, s);
-    if (e == cudaSuccess && a.dgamma) e = column_reduce_launch(a.part, a.parts, a.d, a.dgamma, nullptr, a.ptype, s);
-    return e;
 }
 
 }  // namespace nfx

@@ -1,0 +1,118 @@
+// rms_parts.cuh -- what the RMS norm's forward and backward kernels share: packs of a row whose first element
+// may lie anywhere, and sums over a row's threads.
+//
+// Rows that do not start on 16-byte boundaries (an odd width) are read by 16-byte words all the same: with
+// s the number of elements from the last boundary to the row's start, pack q holds columns q VE - s ..
+// q VE - s + VE - 1, and only a row's first and last pack go by elements.  That asks for tensors whose rows
+// start at the same distance from a boundary, counted in elements (tensors of one shape, contiguous, do);
+// elsewhere packs are single elements.
+#pragma once
+
+#include "block_ops.h"
+#include "row_pack.cuh"
+
+namespace nfx {
+
+// VE elements as they were read.
+template <typename T, int VE>
+struct Elems {
+    static constexpr int kWords = (static_cast<int>(sizeof(T)) * VE + 3) / 4;
+    uint32_t w[kWords];
+
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) w[i] = 0;
+    }
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (kWords >= 4) {
+#pragma unroll
+            for (int i = 0; i < kWords; i += 4) {
+                const uint4 u = __ldg(reinterpret_cast<const uint4*>(p) + i / 4);
+                w[i] = u.x, w[i + 1] = u.y, w[i + 2] = u.z, w[i + 3] = u.w;
+            }
+        } else if constexpr (sizeof(T) == 4) {
+            w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+        } else {
+            w[0] = __ldg(reinterpret_cast<const uint16_t*>(p));
+        }
+    }
+    // columns c .. of row p that are inside [0, d), zeros beside them
+    __device__ __forceinline__ void load_part(const T* p, int c, int d) {
+        zero();
+#pragma unroll
+        for (int i = 0; i < VE; ++i) {
+            if (c + i < 0 || c + i >= d) continue;
+            if constexpr (sizeof(T) == 4) w[i] = __ldg(reinterpret_cast<const uint32_t*>(p) + c + i);
+            else w[i / 2] |= static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t*>(p) + c + i)) << (16 * (i & 1));
+        }
+    }
+    __device__ __forceinline__ float at(int i) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+        else if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float((i & 1) ? (w[i / 2] & 0xFFFF0000u) : (w[i / 2] << 16));
+        else return __half2float(__ushort_as_half(static_cast<unsigned short>((i & 1) ? w[i / 2] >> 16 : w[i / 2] & 0xFFFFu)));
+    }
+    __device__ __forceinline__ void get(float (&o)[VE]) const {
+#pragma unroll
+        for (int i = 0; i < VE; ++i) o[i] = at(i);
+    }
+    // rounds and packs
+    __device__ __forceinline__ void set(const float (&o)[VE]) {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < VE; ++i) w[i] = __float_as_uint(o[i]);
+        } else if constexpr (VE == 1) {
+            const T t = from_f32<T>(o[0]);
+            w[0] = *reinterpret_cast<const uint16_t*>(&t);
+        } else {
+#pragma unroll
+            for (int i = 0; i < VE; i += 2) w[i / 2] = pack2<T>(o[i], o[i + 1]);
+        }
+    }
+    __device__ __forceinline__ void store(T* p) const {
+        if constexpr (kWords >= 4) {
+#pragma unroll
+            for (int i = 0; i < kWords; i += 4) reinterpret_cast<uint4*>(p)[i / 4] = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+        } else if constexpr (sizeof(T) == 4) {
+            *reinterpret_cast<uint32_t*>(p) = w[0];
+        } else {
+            *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(w[0]);
+        }
+    }
+    __device__ __forceinline__ void store_part(T* p, int c, int d) const {
+#pragma unroll
+        for (int i = 0; i < VE; ++i) {
+            if (c + i < 0 || c + i >= d) continue;
+            if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(p)[c + i] = w[i];
+            else reinterpret_cast<uint16_t*>(p)[c + i] = static_cast<uint16_t>(w[i / 2] >> (16 * (i & 1)));
+        }
+    }
+};
+
+// The sum of `a` over the TPR threads of a row, the same bits in each of them.  `red` alternates between two
+// buffers, so that one barrier separates a call's reads from the next but one's writes.
+template <int TPR>
+__device__ __forceinline__ float row_sum(float a, float* red) {
+#pragma unroll
+    for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1) a += __shfl_xor_sync(0xFFFFFFFFu, a, o);
+    if constexpr (TPR > 32) {
+        constexpr int kW = TPR / 32;
+        const int w = threadIdx.x >> 5, w0 = w / kW * kW;  // the row's first warp
+        if ((threadIdx.x & 31) == 0) red[w] = a;
+        __syncthreads();
+        a = red[w0];
+#pragma unroll
+        for (int k = 1; k < kW; ++k) a += red[w0 + k];
+    }
+    return a;
+}
+
+// The distance in elements from the last VE-element boundary to a matrix' first element, and how a row moves it.
+struct Shift {
+    int base, step;
+};
+inline Shift shift_of(const void* p, int64_t ld, int64_t el, int ve) {
+    return {static_cast<int>(reinterpret_cast<uintptr_t>(p) / static_cast<uintptr_t>(el) % static_cast<uintptr_t>(ve)), static_cast<int>(ld % ve)};
+}
+inline bool same_shift(const Shift& a, const Shift& b, int64_t rows) { return a.base == b.base && (rows <= 1 || a.step == b.step); }
+
+}  // namespace nfx

@@ -1,5 +1,5 @@
 // row_pack.cuh -- rows of a matrix in the registers of a warp, by packs of 16 bytes (pairs of elements or
-// single ones where rows are not aligned to more), and their FP8 form: shared by the layer norm and the
+// single ones where rows are not aligned to more), and their FP8 form: shared by the norms and the
 // quantiser.
 #pragma once
 
@@ -68,6 +68,37 @@ __device__ __forceinline__ void store_pack(T* p, const float (&o)[VE]) {
             make_uint4(pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3]), pack2<T>(o[4], o[5]), pack2<T>(o[6], o[7]));
     }
 }
+// VE parameters (of x's type or fp32) from element i; `vec` when they are 16-byte aligned.
+template <typename T, int VE>
+__device__ __forceinline__ void load_params(const void* p, int type, bool vec, int i, float none, float (&o)[VE]) {
+    if (!p) {
+#pragma unroll
+        for (int k = 0; k < VE; ++k) o[k] = none;
+    } else if (VE > 2 && vec && type == kF32) {
+#pragma unroll
+        for (int k = 0; k < VE; k += 4) {
+            const float4 f = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + i + k));
+            o[k] = f.x, o[k + 1] = f.y, o[k + 2] = f.z, o[k + 3] = f.w;
+        }
+    } else if (VE == 8 && vec) {
+        const uint4 u = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i));
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int k = 0; k < VE; k += 2) {
+            float2 f;
+            if (type == kBF16) f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[k / 2]));
+            else f = __half22float2(*reinterpret_cast<const __half2*>(&w[k / 2]));
+            o[k] = f.x, o[k + 1] = f.y;
+        }
+    } else if (type == kF32) {
+#pragma unroll
+        for (int k = 0; k < VE; ++k) o[k] = __ldg(static_cast<const float*>(p) + i + k);
+    } else {
+#pragma unroll
+        for (int k = 0; k < VE; ++k) o[k] = load_any(p, type, i + k);
+    }
+}
+
 // The codes of four values times `inv` (two products to an instruction, each rounded by itself): plain
 // conversions that note in `odd` where they may differ from the encoder, or, with MEND, its codes.
 template <bool MEND>

@@ -86,27 +86,27 @@ __global__ void __launch_bounds__(kAnyThreads) rms_any_kernel(RmsArgs a) {
 }
 
 // ---------------------------------------------------------------------------------------------------------
-// The row in registers: read once, written from there.  TPR threads per row, each holding VPT packs of VE
-// elements (16 bytes of x); pack j of lane l of warp w is (w VPT + j) 32 + l of the row, so the 128
-// elements of an FP8 group lie in one warp.  Resident blocks walk over the rows: the next row is
-// fetched while this one is worked on, and gamma stays where it is, in registers, or in shared memory for rows
-// over 4,096 columns.  EDGE: rows start and end anywhere (rms_parts.cuh); then an FP8 row goes through
-// shared memory to reach its groups.
+// The row in registers: read once, written from there.  A row is a warp's (ONE, four rows to a block) or a whole
+// block's, of as many warps as it takes; a thread holds VPT packs of VE elements (16 bytes of x), pack j of
+// lane l of warp w being (w VPT + j) 32 + l of the row, so the 128 elements of an FP8 group lie in one warp.
+// Resident blocks walk over the rows: the next row is fetched while this one is worked on, and gamma stays where
+// it is, in registers, or in shared memory for rows over 4,096 columns.  EDGE: rows start and end anywhere
+// (rms_parts.cuh); then an FP8 row goes through shared memory to reach its groups.
 // ---------------------------------------------------------------------------------------------------------
-constexpr int row_block(int tpr) { return tpr > 128 ? tpr : 128; }
-constexpr int row_blocks(int tpr, int regs) { return tpr >= 512 ? (regs <= 32 ? 2 : 1) : 768 / row_block(tpr); }
-// registers of a row that is on its way: x and the residual
-constexpr int row_regs(int n, int xb, int hb) { return n * (xb + hb) / 4; }
+// Blocks per SM that the registers are cut for: 768 threads where a row on its way takes 16 registers, 512 where it
+// takes more.
+constexpr int row_blocks(int most, int coming) { return most >= 512 ? 1 : (coming <= 16 ? 768 : 512) / most; }
 
-template <typename T, typename H, int VE, int VPT, int TPR, bool FP8, bool EDGE>
-__global__ void __launch_bounds__(row_block(TPR), row_blocks(TPR, row_regs(VE * VPT, sizeof(T), sizeof(H)) + VE * VPT))
+template <typename T, typename H, int VE, int VPT, int MOST, bool ONE, bool FP8, bool EDGE>
+__global__ void __launch_bounds__(MOST, row_blocks(MOST, VE * VPT * static_cast<int>(sizeof(T) + sizeof(H)) / 4))
 rms_row_kernel(RmsArgs a, Shift sh, bool gvec, bool wide) {
-    __shared__ float red[2][row_block(TPR) / 32];
+    __shared__ float red[2][MOST / 32];
     extern __shared__ __align__(16) float room[];  // gamma (rows over 4,096 columns), then rows on their way to FP8
-    constexpr int kRows = row_block(TPR) / TPR, N = VPT * VE, kPacks = TPR * VPT;
-    constexpr bool kGammaShared = TPR >= 512;
-    const int lane = threadIdx.x & 31, sub = threadIdx.x % TPR, mine = threadIdx.x / TPR;
-    const int first = TPR < 32 ? sub : (sub >> 5) * VPT * 32 + lane;
+    constexpr int kRows = ONE ? MOST / 32 : 1;
+    constexpr bool kGammaShared = !ONE && MOST >= 512;
+    const int lane = threadIdx.x & 31, warps = ONE ? 1 : blockDim.x >> 5;
+    const int sub = ONE ? lane : threadIdx.x, mine = ONE ? threadIdx.x >> 5 : 0;
+    const int first = (sub >> 5) * VPT * 32 + lane, elems = warps * 32 * VPT * VE;
     const float inv_d = __frcp_rn(static_cast<float>(a.d));
     const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
     // (the launcher makes `step` rows a whole number of boundaries: s is the same in all rows of a thread)
@@ -138,7 +138,7 @@ rms_row_kernel(RmsArgs a, Shift sh, bool gvec, bool wide) {
     fetch(static_cast<int64_t>(blockIdx.x) * kRows + mine);
     float gam[kGammaShared ? 1 : VPT][VE];
     if constexpr (kGammaShared) {
-        for (int i = threadIdx.x; i < kPacks * VE; i += TPR)
+        for (int i = threadIdx.x; i < elems; i += blockDim.x)
             room[i] = a.gamma && i - s >= 0 && i - s < a.d ? load_any(a.gamma, a.ptype, i - s) : 1.0f;
         __syncthreads();
     } else {
@@ -188,7 +188,7 @@ rms_row_kernel(RmsArgs a, Shift sh, bool gvec, bool wide) {
             }
         }
         fetch(r + step);  // the next row comes while this one is worked on
-        const float rs = __frsqrt_rn(row_sum<TPR>(q2.x + q2.y, red[buf]) * inv_d + a.eps);
+        const float rs = __frsqrt_rn(row_sum<ONE>(q2.x + q2.y, red[buf], warps) * inv_d + a.eps);
         if (live && sub == 0 && a.rstd) a.rstd[r] = rs;
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
@@ -224,20 +224,19 @@ rms_row_kernel(RmsArgs a, Shift sh, bool gvec, bool wide) {
             }
         }
         if constexpr (FP8 && !EDGE) {
-            store_codes<VE, VPT, TPR>(v, a.q, r, a.d, live, first, lane, wide);
+            store_codes<VE, VPT, 32>(v, a.q, r, a.d, live, first, lane, wide);
         } else if constexpr (FP8) {
             // through shared memory to groups of 128 columns, a warp each, four columns a lane
             const int padded = (a.d + kGroup - 1) / kGroup * kGroup;
-            float* row = room + (kGammaShared ? kPacks * VE : 0) + mine * padded;
+            float* row = room + (kGammaShared ? elems : 0) + mine * padded;
 #pragma unroll
             for (int j = 0; j < VPT; ++j)
 #pragma unroll
                 for (int i = 0; i < VE; ++i)
                     if (const int c = column(j) + i; c >= 0 && c < a.d) row[c] = v[j][i];
-            if constexpr (TPR > 32) __syncthreads();
-            else __syncwarp();
-            constexpr int kWarps = TPR < 32 ? 1 : TPR / 32;
-            for (int b = TPR < 32 ? 0 : sub >> 5; b < padded / kGroup; b += kWarps) {
+            if constexpr (ONE) __syncwarp();
+            else __syncthreads();
+            for (int b = sub >> 5; b < padded / kGroup; b += warps) {
                 const int c = b * kGroup + lane * 4;
                 float o[4], top = 0.0f;
 #pragma unroll
@@ -259,67 +258,59 @@ rms_row_kernel(RmsArgs a, Shift sh, bool gvec, bool wide) {
                         if (c + i < a.d) dst[i] = static_cast<uint8_t>(w >> (8 * i));
                 }
             }
-            if constexpr (TPR <= 32) __syncwarp();  // (with more warps the next row's sum has a barrier)
+            if constexpr (ONE) __syncwarp();  // (with more warps the next row's sum has a barrier)
         }
     }
 }
 
-template <typename T, typename H, int VE, int VPT, int TPR, bool FP8, bool EDGE>
+template <typename T, typename H, int VE, int VPT, int MOST, bool ONE, bool FP8, bool EDGE>
 cudaError_t rms_row_go(const RmsArgs& a, cudaStream_t s) {
-    constexpr int kThreads = row_block(TPR), kRows = kThreads / TPR;
-    auto kern = rms_row_kernel<T, H, VE, VPT, TPR, FP8, EDGE>;
-    const int gamma = TPR >= 512 ? TPR * VPT * VE * 4 : 0;
-    const int rows = FP8 && EDGE ? kRows * ((a.d + kGroup - 1) / kGroup * kGroup) * 4 : 0;
-    // the most that any width of this kernel asks for decides how many blocks an SM holds
-    constexpr int kMost = (TPR >= 512 ? TPR * VPT * VE * 4 : 0) + (FP8 && EDGE ? kRows * (TPR * VPT * VE + kGroup) * 4 : 0);
+    auto kern = rms_row_kernel<T, H, VE, VPT, MOST, ONE, FP8, EDGE>;
+    const int span = a.d + (EDGE ? VE - 1 : 0);  // the first pack may begin before the row
+    const int threads = ONE ? MOST : (span + 32 * VPT * VE - 1) / (32 * VPT * VE) * 32, rows = ONE ? MOST / 32 : 1;
+    const int smem = (!ONE && MOST >= 512 ? threads * VPT * VE * 4 : 0) + (FP8 && EDGE ? rows * ((a.d + kGroup - 1) / kGroup * kGroup) * 4 : 0);
+    // the most that any width of this kernel asks for
+    constexpr int kMost = (!ONE && MOST >= 512 ? MOST * VPT * VE * 4 : 0) +
+                          (FP8 && EDGE ? (ONE ? MOST / 32 * (32 * VPT * VE + kGroup) : MOST * VPT * VE + kGroup) * 4 : 0);
     const cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), kMost);
     if (e != cudaSuccess) return e;
-    static std::atomic<int> known[64];  // asked for once per kernel and device
-    const int d = current_device() & 63;
-    int most = known[d].load(std::memory_order_relaxed);
+    static std::atomic<int> known[64][MOST / 32];  // asked for once per kernel, device and size of block
+    std::atomic<int>& at = known[current_device() & 63][threads / 32 - 1];
+    int most = at.load(std::memory_order_relaxed);
     if (most == 0) {
-        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&most, kern, kThreads, kMost) != cudaSuccess || most < 1) most = 1;
+        const int room = (!ONE && MOST >= 512 ? threads * VPT * VE * 4 : 0) + (FP8 && EDGE ? rows * (threads / (ONE ? rows : 1) * VPT * VE + kGroup) * 4 : 0);
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&most, kern, threads, room) != cudaSuccess || most < 1) most = 1;
         most *= device_sm_count();
-        known[d].store(most, std::memory_order_relaxed);
+        at.store(most, std::memory_order_relaxed);
     }
-    const int64_t want = (a.rows + kRows - 1) / kRows;
+    const int64_t want = (a.rows + rows - 1) / rows;
     int64_t grid = want < most ? want : most;
     if (EDGE && VE > 1 && grid < want) grid = grid >= VE ? grid / VE * VE : VE;  // steps of whole boundaries
     const Shift sh = shift_of(a.x, a.ldx, sizeof(T), VE);
     const bool gvec = aligned16(a.gamma) && (a.ptype == kF32 || VE == 8);
     const bool wide = FP8 && reinterpret_cast<uintptr_t>(a.q.codes) % 8 == 0 && (a.rows == 1 || a.q.ld % 8 == 0);
-    kern<<<static_cast<unsigned>(grid), kThreads, gamma + rows, s>>>(a, sh, gvec, wide);
+    kern<<<static_cast<unsigned>(grid), threads, smem, s>>>(a, sh, gvec, wide);
     return cudaGetLastError();
 }
 
-// 16 elements a thread up to 8,192 columns and 32 above; whole packs have a kernel for each width, rows with
-// edges one for every second.
-template <typename T, typename H, int VE, bool FP8>
-cudaError_t rms_whole(const RmsArgs& a, cudaStream_t s) {
+// 16 elements a thread up to 8,192 columns and 32 above.
+template <typename T, typename H, int VE, bool FP8, bool EDGE>
+cudaError_t rms_width(const RmsArgs& a, cudaStream_t s) {
     constexpr int k16 = 16 / VE;
-    if (a.d <= 32 * VE) return rms_row_go<T, H, VE, 1, 32, FP8, false>(a, s);
-    if (a.d <= 512) return rms_row_go<T, H, VE, k16, 32, FP8, false>(a, s);
-    if (a.d <= 1024) return rms_row_go<T, H, VE, k16, 64, FP8, false>(a, s);
-    if (a.d <= 2048) return rms_row_go<T, H, VE, k16, 128, FP8, false>(a, s);
-    if (a.d <= 4096) return rms_row_go<T, H, VE, k16, 256, FP8, false>(a, s);
-    if (a.d <= 8192) return rms_row_go<T, H, VE, k16, 512, FP8, false>(a, s);
-    return rms_row_go<T, H, VE, 2 * k16, 512, FP8, false>(a, s);
-}
-template <typename T, typename H, int VE, bool FP8>
-cudaError_t rms_edge(const RmsArgs& a, cudaStream_t s) {
-    constexpr int k16 = 16 / VE;
-    const int d = a.d + VE - 1;  // the first pack may begin before the row
-    if (d <= 512) return rms_row_go<T, H, VE, k16, 32, FP8, true>(a, s);
-    if (d <= 1024) return rms_row_go<T, H, VE, k16, 64, FP8, true>(a, s);
-    if (d <= 2048) return rms_row_go<T, H, VE, k16, 128, FP8, true>(a, s);
-    if (d <= 4096) return rms_row_go<T, H, VE, k16, 256, FP8, true>(a, s);
-    return rms_row_go<T, H, VE, 2 * k16, 512, FP8, true>(a, s);
-}
-template <typename T, typename H, bool FP8>
-cudaError_t rms_single(const RmsArgs& a, cudaStream_t s) {
-    if (a.d <= 1024) return rms_row_go<T, H, 1, 8, 128, FP8, true>(a, s);
-    if (a.d <= 4096) return rms_row_go<T, H, 1, 16, 256, FP8, true>(a, s);
-    return rms_row_go<T, H, 1, 32, 512, FP8, true>(a, s);
+    const int d = a.d + (EDGE ? VE - 1 : 0);
+    if constexpr (VE == 1) {  // (more loads to a row than a warp should queue)
+        if (d <= 2048) return rms_row_go<T, H, 1, 8, 256, false, FP8, true>(a, s);
+        if (d <= 8192) return rms_row_go<T, H, 1, 16, 512, false, FP8, true>(a, s);
+        return rms_row_go<T, H, 1, 32, 512, false, FP8, true>(a, s);
+    } else {
+        if constexpr (!EDGE) {
+            if (d <= 32 * VE) return rms_row_go<T, H, VE, 1, 128, true, FP8, false>(a, s);
+        }
+        if (d <= 512) return rms_row_go<T, H, VE, k16, 128, true, FP8, EDGE>(a, s);
+        if (d <= 4096) return rms_row_go<T, H, VE, k16, 256, false, FP8, EDGE>(a, s);
+        if (d <= 8192) return rms_row_go<T, H, VE, k16, 512, false, FP8, EDGE>(a, s);
+        return rms_row_go<T, H, VE, 2 * k16, 512, false, FP8, EDGE>(a, s);
+    }
 }
 
 template <typename T, typename H, bool FP8>
@@ -329,11 +320,11 @@ cudaError_t rms_form(const RmsArgs& a, cudaStream_t s) {
         const Shift sx = shift_of(a.x, a.ldx, sizeof(T), VE);
         const auto like = [&](const void* p, int64_t ld, int64_t el) { return !p || same_shift(sx, shift_of(p, ld, el, VE), a.rows); };
         if (like(a.res, a.ldres, sizeof(H)) && like(a.sum, a.ldsum, sizeof(H)) && (FP8 || like(a.y, a.ldy, sizeof(T)))) {
-            if (sx.base == 0 && (a.rows == 1 || sx.step == 0) && a.d % VE == 0) return rms_whole<T, H, VE, FP8>(a, s);
-            if (a.d <= 16384 - VE + 1) return rms_edge<T, H, VE, FP8>(a, s);
+            if (sx.base == 0 && (a.rows == 1 || sx.step == 0) && a.d % VE == 0) return rms_width<T, H, VE, FP8, false>(a, s);
+            if (a.d <= 16384 - VE + 1) return rms_width<T, H, VE, FP8, true>(a, s);
         }
     }
-    if (a.d <= 16384) return rms_single<T, H, FP8>(a, s);
+    if (a.d <= 16384) return rms_width<T, H, 1, FP8, true>(a, s);
     const int64_t cap = 8ll * device_sm_count();
     rms_any_kernel<T, H><<<static_cast<int>(a.rows < cap ? a.rows : cap), kAnyThreads, 0, s>>>(a);
     return cudaGetLastError();

@@ -88,20 +88,17 @@ struct Elems {
     }
 };
 
-// The sum of `a` over the TPR threads of a row, the same bits in each of them.  `red` alternates between two
-// buffers, so that one barrier separates a call's reads from the next but one's writes.
-template <int TPR>
-__device__ __forceinline__ float row_sum(float a, float* red) {
-#pragma unroll
-    for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1) a += __shfl_xor_sync(0xFFFFFFFFu, a, o);
-    if constexpr (TPR > 32) {
-        constexpr int kW = TPR / 32;
-        const int w = threadIdx.x >> 5, w0 = w / kW * kW;  // the row's first warp
-        if ((threadIdx.x & 31) == 0) red[w] = a;
+// The sum of `a` over a row's threads, the same bits in each of them: a warp (ONE), or all `warps` of the block.
+// `red` alternates between two buffers, so that one barrier separates a call's reads from the next but one's
+// writes.
+template <bool ONE>
+__device__ __forceinline__ float row_sum(float a, float* red, int warps) {
+    a = warp_sum(a);
+    if constexpr (!ONE) {
+        if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = a;
         __syncthreads();
-        a = red[w0];
-#pragma unroll
-        for (int k = 1; k < kW; ++k) a += red[w0 + k];
+        a = red[0];
+        for (int k = 1; k < warps; ++k) a += red[k];
     }
     return a;
 }

@@ -3,21 +3,26 @@
 //   n = sqrt(sum g^2),  s = min(1, max_norm / (n + eps)),  out = g s
 //
 // The tensors' addresses and sizes are kernel parameters, so nothing is copied to the device and a call can be
-// captured.  Each block leaves its share of the sum of squares as a 64-bit number in the workspace; the
-// scaling kernel's blocks add them in a fixed order, so the result does not change from run to run.
+// captured.  Squares are added in fp32 over the 32 (16 of fp32) elements that a thread has at a time and in 64
+// bits from there; where such a sum leaves the range in which fp32 squares are exact enough, its elements are
+// squared in 64 bits instead.  Each block leaves its share in the workspace, and whoever needs the norm adds the
+// shares in a fixed order, so the result does not change from run to run.
 #include <cuda_runtime.h>
 
 #include <cstdint>
 
 #include "dense_ops.h"
 #include "nfx_internal.h"
+#include "rms_parts.cuh"
+#include "sm100.cuh"
 
 namespace nfx {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kChunk = 16384;  // elements that a block takes at a time
-constexpr int kPartBlocks = 592;
+constexpr int kGroupPacks = 4;                                // packs of 16 bytes that a thread has in flight
+constexpr int kFewThreads = 512, kFewCluster = 8;
+constexpr int kPartBlocks = 8 * 148;                          // shares that one launch leaves, at most
 
 struct Entry {
     const void* src;
@@ -32,9 +37,11 @@ struct Table {
     int count;
     int64_t chunks;
 };
-constexpr int kCap = 900;
+// Kernel parameters hold 32,764 bytes; a launch copies all of them, so short lists have a table of their own.
+constexpr int kCap = 900, kCapFew = 48;
+static_assert(sizeof(Table<kCap>) + 64 <= 32764, "kernel parameters");
 
-// The tensor that chunk c belongs to (tensors without elements have no chunk).
+// The tensor that chunk c belongs to (tensors without elements have no entry).
 template <int CAP>
 __device__ __forceinline__ int tensor_of(const Table<CAP>& t, int64_t c) {
     int lo = 0, hi = t.count - 1;
@@ -46,65 +53,243 @@ __device__ __forceinline__ int tensor_of(const Table<CAP>& t, int64_t c) {
     return lo;
 }
 
+template <int THREADS>
 __device__ __forceinline__ double block_sum(double v, double* red) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    __syncthreads();  // the previous sums have been read
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
     __syncthreads();
     double s = 0.0;
-    for (int w = 0; w < kThreads / 32; ++w) s += red[w];
+    for (int w = 0; w < THREADS / 32; ++w) s += red[w];
     return s;
+}
+
+// The sum of squares of chunk elements [i0, i1) of a tensor, `i` counted from the last 16-byte boundary before its
+// first element (`shift` elements in front of it); this thread's share.
+template <typename T, int THREADS>
+__device__ __forceinline__ double squares_of(const T* src, int64_t n, int shift, int64_t i0, int64_t i1) {
+    constexpr int VE = 16 / sizeof(T);
+    double sum = 0.0;
+    for (int64_t b = i0 + threadIdx.x * VE; b < i1; b += static_cast<int64_t>(THREADS) * VE * kGroupPacks) {
+        Elems<T, VE> v[kGroupPacks];
+#pragma unroll
+        for (int k = 0; k < kGroupPacks; ++k) {
+            const int64_t c = b + static_cast<int64_t>(k) * THREADS * VE - shift;  // the pack's first element
+            if (c + shift < i1 && c >= 0 && c + VE <= n) {
+                v[k].load(src + c);
+            } else {
+                v[k].zero();
+                if (c + shift < i1) {
+                    // (an edge of the tensor: the pack's elements that it has)
+#pragma unroll
+                    for (int i = 0; i < VE; ++i) {
+                        if (c + i < 0 || c + i >= n) continue;
+                        if constexpr (sizeof(T) == 4) v[k].w[i] = __ldg(reinterpret_cast<const uint32_t*>(src) + c + i);
+                        else v[k].w[i / 2] |= static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t*>(src) + c + i)) << (16 * (i & 1));
+                    }
+                }
+            }
+        }
+        float s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kGroupPacks; ++k)
+#pragma unroll
+            for (int i = 0; i < VE; ++i) s = fmaf(v[k].at(i), v[k].at(i), s);
+        if (s > 0x1p-80f && s < 0x1p100f) {
+            sum += static_cast<double>(s);
+        } else {
+            uint32_t any = 0;
+#pragma unroll
+            for (int k = 0; k < kGroupPacks; ++k)
+#pragma unroll
+                for (int i = 0; i < Elems<T, VE>::kWords; ++i) any |= v[k].w[i] & (sizeof(T) == 4 ? 0x7FFFFFFFu : 0x7FFF7FFFu);
+            if (any) {
+#pragma unroll
+                for (int k = 0; k < kGroupPacks; ++k)
+#pragma unroll
+                    for (int i = 0; i < VE; ++i) {
+                        const double g = static_cast<double>(v[k].at(i));
+                        sum = fma(g, g, sum);
+                    }
+            }
+        }
+    }
+    return sum;
+}
+
+// A chunk is this many elements, counted from a 16-byte boundary: finding its tensor takes a few hundred cycles.
+__host__ __device__ constexpr int64_t chunk_of(int threads) { return threads == kThreads ? 32768 : 16384; }
+__host__ __device__ __forceinline__ int shift_el(const void* p, int type) {
+    return static_cast<int>(reinterpret_cast<uintptr_t>(p) % 16 / (type == kF32 ? 4 : 2));
+}
+
+template <int CAP, int THREADS>
+__device__ __forceinline__ double chunk_squares(const Table<CAP>& t, int64_t c) {
+    const int k = tensor_of(t, c);
+    const int64_t n = t.e[k].n;
+    const int type = t.src_type[k], shift = shift_el(t.e[k].src, type);
+    const int64_t i0 = (c - t.e[k].first) * chunk_of(THREADS), i1 = min(n + shift, i0 + chunk_of(THREADS));
+    if (type == kF32) return squares_of<float, THREADS>(static_cast<const float*>(t.e[k].src), n, shift, i0, i1);
+    if (type == kBF16) return squares_of<__nv_bfloat16, THREADS>(static_cast<const __nv_bfloat16*>(t.e[k].src), n, shift, i0, i1);
+    return squares_of<__half, THREADS>(static_cast<const __half*>(t.e[k].src), n, shift, i0, i1);
+}
+
+// Eight elements from `src` on, which lies `q` elements behind a 16-byte boundary: the words that hold them, moved
+// into place.
+template <typename T>
+__device__ __forceinline__ void load_moved(const T* src, int q, float (&o)[8]) {
+    constexpr int kWords = sizeof(T) == 4 ? 12 : 8;
+    uint32_t w[kWords];
+    const uint4* p = reinterpret_cast<const uint4*>(src - q);
+#pragma unroll
+    for (int i = 0; i < kWords / 4; ++i) {
+        uint4 u = make_uint4(0, 0, 0, 0);
+        if (i < (sizeof(T) == 4 ? 2 : 1) || q > 0) u = __ldcs(p + i);
+        w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
+    }
+    const int words = sizeof(T) == 4 ? q : q >> 1;
+    if (words & 2) {
+#pragma unroll
+        for (int i = 0; i + 2 < kWords; ++i) w[i] = w[i + 2];
+    }
+    if (words & 1) {
+#pragma unroll
+        for (int i = 0; i + 1 < kWords; ++i) w[i] = w[i + 1];
+    }
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = __uint_as_float(w[i]);
+    } else {
+        if (q & 1) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 16);
+        }
+        Elems<T, 8> e;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e.w[i] = w[i];
+        e.get(o);
+    }
+}
+
+// out = src s for the chunk's elements, by packs of eight that start on a 16-byte boundary of `dst`.
+template <typename T, typename D, int THREADS>
+__device__ __forceinline__ void scale_chunk(const T* src, D* dst, int64_t n, int shift, int64_t i0, int64_t i1, float s) {
+    for (int64_t b = i0 + threadIdx.x * 8; b < i1; b += THREADS * 8) {
+        const int64_t c = b - shift;
+        // the words that hold the eight elements lie inside the tensor
+        const int q = static_cast<int>(reinterpret_cast<uintptr_t>(src + c) % 16 / sizeof(T));
+        if (c - q >= 0 && c - q + (q > 0 ? 8 + 16 / static_cast<int>(sizeof(T)) : 8) <= n) {
+            float v[8];
+            load_moved(src + c, q, v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] *= s;
+            Elems<D, 8> o;
+            o.set(v);
+#pragma unroll
+            for (int i = 0; i < Elems<D, 8>::kWords; i += 4)
+                __stcs(reinterpret_cast<uint4*>(dst + c) + i / 4, make_uint4(o.w[i], o.w[i + 1], o.w[i + 2], o.w[i + 3]));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (c + i >= 0 && c + i < n) dst[c + i] = from_f32<D>(to_f32(src[c + i]) * s);
+        }
+    }
+}
+
+template <int CAP, int THREADS>
+__device__ __forceinline__ void chunk_scale(const Table<CAP>& t, int64_t c, float s) {
+    const int k = tensor_of(t, c);
+    const Entry& e = t.e[k];
+    if (s == 1.0f && e.dst == e.src) return;  // every element times one
+    // chunks are counted by the source's boundaries, packs by the destination's: a chunk's packs are those that
+    // begin in it
+    const int64_t n = e.n, at = (c - e.first) * chunk_of(THREADS) - shift_el(e.src, t.src_type[k]), end = at + chunk_of(THREADS);
+    const int dt = t.dst_type[k], st = t.src_type[k];
+    const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(e.dst) % 16 / (dt == kF32 ? 4 : 2));
+    const auto pack_from = [&](int64_t i) { return i <= -shift ? static_cast<int64_t>(0) : (i + shift + 7) / 8 * 8; };
+    const int64_t i0 = at <= 0 ? 0 : pack_from(at), i1 = end >= n ? n + shift : pack_from(end);
+    const auto go = [&](auto* src) {
+        if (dt == kF32) scale_chunk<std::remove_const_t<std::remove_pointer_t<decltype(src)>>, float, THREADS>(src, static_cast<float*>(e.dst), n, shift, i0, i1, s);
+        else if (dt == kBF16) scale_chunk<std::remove_const_t<std::remove_pointer_t<decltype(src)>>, __nv_bfloat16, THREADS>(src, static_cast<__nv_bfloat16*>(e.dst), n, shift, i0, i1, s);
+        else scale_chunk<std::remove_const_t<std::remove_pointer_t<decltype(src)>>, __half, THREADS>(src, static_cast<__half*>(e.dst), n, shift, i0, i1, s);
+    };
+    if (st == kF32) go(static_cast<const float*>(e.src));
+    else if (st == kBF16) go(static_cast<const __nv_bfloat16*>(e.src));
+    else go(static_cast<const __half*>(e.src));
+}
+
+// (a NaN stays one; a norm of zero leaves the zeros as they are, also with max_norm and eps of zero)
+__device__ __forceinline__ float scale_for(double n, double max_norm, double eps) {
+    const double q = n == 0.0 ? 1.0 : max_norm / (n + eps);
+    return q >= 1.0 ? 1.0f : static_cast<float>(q);
 }
 
 template <int CAP>
 __global__ void __launch_bounds__(kThreads) grad_squares_kernel(const __grid_constant__ Table<CAP> t, double* part) {
     __shared__ double red[kThreads / 32];
     double s = 0.0;
-    for (int64_t c = blockIdx.x; c < t.chunks; c += gridDim.x) {
-        const int k = tensor_of(t, c);
-        const int64_t i0 = (c - t.e[k].first) * kChunk, i1 = min(t.e[k].n, i0 + kChunk);
-        for (int64_t i = i0 + threadIdx.x; i < i1; i += kThreads) {
-            const double g = load_any(t.e[k].src, t.src_type[k], i);
-            s += g * g;
-        }
-    }
-    s = block_sum(s, red);
+    for (int64_t c = blockIdx.x; c < t.chunks; c += gridDim.x) s += chunk_squares<CAP, kThreads>(t, c);
+    grid_dep_launch();  // the kernel that needs the norm may be placed
+    s = block_sum<kThreads>(s, red);
     if (threadIdx.x == 0) part[blockIdx.x] = s;
 }
 
 __device__ __forceinline__ double joined_norm(const double* part, int64_t parts, double* red) {
     double s = 0.0;
     for (int64_t i = threadIdx.x; i < parts; i += kThreads) s += part[i];
-    return sqrt(block_sum(s, red));
+    return sqrt(block_sum<kThreads>(s, red));
 }
 
 __global__ void __launch_bounds__(kThreads) grad_norm_kernel(const double* part, int64_t parts, float* norm) {
     __shared__ double red[kThreads / 32];
+    grid_dep_wait();
     const double n = joined_norm(part, parts, red);
     if (threadIdx.x == 0) *norm = static_cast<float>(n);
 }
 
+// The chunks in the other order than the squares were summed in: what was read last is still in L2.
 template <int CAP>
 __global__ void __launch_bounds__(kThreads)
 grad_scale_kernel(const __grid_constant__ Table<CAP> t, const double* part, int64_t parts, double max_norm, double eps, float* norm) {
     __shared__ double red[kThreads / 32];
+    grid_dep_wait();
     const double n = joined_norm(part, parts, red);
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = static_cast<float>(n);
-    // (a NaN stays one; a norm of zero leaves the zeros as they are, also with max_norm and eps of zero)
-    const double q = n == 0.0 ? 1.0 : max_norm / (n + eps);
-    const float s = q >= 1.0 ? 1.0f : static_cast<float>(q);
-    for (int64_t c = blockIdx.x; c < t.chunks; c += gridDim.x) {
-        const int k = tensor_of(t, c);
-        if (s == 1.0f && t.e[k].dst == t.e[k].src) continue;
-        const int64_t i0 = (c - t.e[k].first) * kChunk, i1 = min(t.e[k].n, i0 + kChunk);
-        for (int64_t i = i0 + threadIdx.x; i < i1; i += kThreads)
-            store_any(t.e[k].dst, t.dst_type[k], i, load_any(t.e[k].src, t.src_type[k], i) * s);
+    const float s = scale_for(n, max_norm, eps);
+    for (int64_t c = t.chunks - 1 - blockIdx.x; c >= 0; c -= gridDim.x) chunk_scale<CAP, kThreads>(t, c, s);
+}
+
+// A few tensors of few elements: one cluster sums, joins through its shared memory and scales, in one launch.
+template <bool SCALE>
+__global__ void __cluster_dims__(kFewCluster, 1, 1) __launch_bounds__(kFewThreads)
+grad_few_kernel(const __grid_constant__ Table<kCapFew> t, double max_norm, double eps, float* norm) {
+    __shared__ double red[kFewThreads / 32];
+    __shared__ double mine;
+    const uint32_t rank = cluster_ctarank();
+    double s = 0.0;
+    for (int64_t c = rank; c < t.chunks; c += kFewCluster) s += chunk_squares<kCapFew, kFewThreads>(t, c);
+    s = block_sum<kFewThreads>(s, red);
+    if (threadIdx.x == 0) mine = s;
+    cluster_sync();
+    double n = 0.0;
+    for (int r = 0; r < kFewCluster; ++r) {
+        double v;
+        asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(map_rank(smem_u32(&mine), r)) : "memory");
+        n += v;
+    }
+    cluster_sync();  // no CTA leaves while another may still read its share
+    n = sqrt(n);
+    if (rank == 0 && threadIdx.x == 0) *norm = static_cast<float>(n);
+    if constexpr (SCALE) {
+        const float f = scale_for(n, max_norm, eps);
+        for (int64_t c = rank; c < t.chunks; c += kFewCluster) chunk_scale<kCapFew, kFewThreads>(t, c, f);
     }
 }
 
 // The next tensors of the list, as many as the table holds; their number.
 template <int CAP>
-int64_t fill(Table<CAP>& t, const GradTensor* g, int64_t tensors) {
+int64_t fill(Table<CAP>& t, const GradTensor* g, int64_t tensors, int threads) {
     t.count = 0, t.chunks = 0;
     int64_t i = 0;
     for (; i < tensors && t.count < CAP; ++i) {
@@ -112,26 +297,75 @@ int64_t fill(Table<CAP>& t, const GradTensor* g, int64_t tensors) {
         t.e[t.count] = {g[i].src, g[i].dst, g[i].n, t.chunks};
         t.src_type[t.count] = static_cast<uint8_t>(g[i].src_type);
         t.dst_type[t.count] = static_cast<uint8_t>(g[i].dst_type);
-        t.chunks += (g[i].n + kChunk - 1) / kChunk;
+        t.chunks += (g[i].n + shift_el(g[i].src, g[i].src_type) + chunk_of(threads) - 1) / chunk_of(threads);
         ++t.count;
     }
     return i;
 }
-int grid_of(int64_t chunks) { return static_cast<int>(chunks < 1 ? 1 : (chunks < kPartBlocks ? chunks : kPartBlocks)); }
+int grid_of(int64_t chunks) {
+    const int64_t most = 8ll * device_sm_count() < kPartBlocks ? 8ll * device_sm_count() : kPartBlocks;
+    return static_cast<int>(chunks < 1 ? 1 : (chunks < most ? chunks : most));
+}
 
-cudaError_t squares(const GradTensor* g, int64_t tensors, double* part, int64_t* parts, cudaStream_t s) {
+// Launches behind the kernel that leaves the shares, which it may overlap with until it waits for it.
+template <typename... P, typename... A>
+cudaError_t launch_behind(void (*kern)(P...), int grid, cudaStream_t s, A... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(grid));
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = s;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...);
+}
+
+template <int CAP>
+cudaError_t squares(Table<CAP>& t, const GradTensor* g, int64_t tensors, double* part, int64_t* parts, cudaStream_t s) {
     *parts = 0;
-    static thread_local Table<kCap> t;
     while (tensors > 0) {
-        const int64_t took = fill(t, g, tensors);
+        const int64_t took = fill(t, g, tensors, kThreads);
         g += took, tensors -= took;
         if (t.count == 0) continue;
         const int grid = grid_of(t.chunks);
-        grad_squares_kernel<kCap><<<grid, kThreads, 0, s>>>(t, part + *parts);
+        grad_squares_kernel<CAP><<<grid, kThreads, 0, s>>>(t, part + *parts);
         if (const cudaError_t e = cudaGetLastError()) return e;
         *parts += grid;
     }
     return cudaSuccess;
+}
+
+template <int CAP>
+cudaError_t clip(const GradTensor* g, int64_t tensors, double* part, double max_norm, double eps, float* norm, cudaStream_t s) {
+    static thread_local Table<CAP> t;
+    int64_t parts = 0;
+    if (const cudaError_t e = squares(t, g, tensors, part, &parts, s)) return e;
+    const bool whole = tensors <= CAP;  // the table holds all of them, as it was filled
+    bool told = false;
+    while (tensors > 0 || !told) {
+        const int64_t took = whole ? tensors : fill(t, g, tensors, kThreads);
+        g += took, tensors -= took;
+        if (t.count == 0 && told) continue;
+        if (const cudaError_t e = launch_behind(grad_scale_kernel<CAP>, grid_of(t.chunks), s, t, part, parts, max_norm, eps,
+                                                told ? static_cast<float*>(nullptr) : norm))
+            return e;
+        told = true;
+    }
+    return cudaSuccess;
+}
+
+// The cluster reads some 1 TB/s, and a second launch costs 2 us on the device and more on the host.
+constexpr int64_t kFewBytes = 1 << 20;
+bool few(const GradTensor* g, int64_t tensors) {
+    if (tensors > kCapFew) return false;
+    int64_t bytes = 0;
+    for (int64_t i = 0; i < tensors; ++i) {
+        if (g[i].n > kFewBytes) return false;
+        bytes += g[i].n * type_bytes(g[i].src_type);
+    }
+    return bytes <= kFewBytes;
 }
 
 }  // namespace
@@ -139,27 +373,35 @@ cudaError_t squares(const GradTensor* g, int64_t tensors, double* part, int64_t*
 int64_t grad_norm_partials(int64_t tensors) { return ((tensors + kCap - 1) / kCap + 1) * kPartBlocks; }
 
 cudaError_t grad_norm_launch(const GradTensor* g, int64_t tensors, double* part, float* norm, cudaStream_t s) {
+    if (few(g, tensors)) {
+        static thread_local Table<kCapFew> t;
+        fill(t, g, tensors, kFewThreads);
+        grad_few_kernel<false><<<kFewCluster, kFewThreads, 0, s>>>(t, 0.0, 0.0, norm);
+        return cudaGetLastError();
+    }
     int64_t parts = 0;
-    if (const cudaError_t e = squares(g, tensors, part, &parts, s)) return e;
-    grad_norm_kernel<<<1, kThreads, 0, s>>>(part, parts, norm);
-    return cudaGetLastError();
+    cudaError_t e;
+    if (tensors <= kCapFew) {
+        static thread_local Table<kCapFew> t;
+        e = squares(t, g, tensors, part, &parts, s);
+    } else {
+        static thread_local Table<kCap> t;
+        e = squares(t, g, tensors, part, &parts, s);
+    }
+    if (e != cudaSuccess) return e;
+    return launch_behind(grad_norm_kernel, 1, s, part, parts, norm);
 }
 
 cudaError_t grad_clip_launch(const GradTensor* g, int64_t tensors, double* part, double max_norm, double eps, float* norm,
                              cudaStream_t s) {
-    int64_t parts = 0;
-    if (const cudaError_t e = squares(g, tensors, part, &parts, s)) return e;
-    static thread_local Table<kCap> t;
-    bool told = false;
-    while (tensors > 0 || !told) {
-        const int64_t took = fill(t, g, tensors);
-        g += took, tensors -= took;
-        if (t.count == 0 && told) continue;
-        grad_scale_kernel<kCap><<<grid_of(t.chunks), kThreads, 0, s>>>(t, part, parts, max_norm, eps, told ? nullptr : norm);
-        if (const cudaError_t e = cudaGetLastError()) return e;
-        told = true;
+    if (few(g, tensors)) {
+        static thread_local Table<kCapFew> t;
+        fill(t, g, tensors, kFewThreads);
+        grad_few_kernel<true><<<kFewCluster, kFewThreads, 0, s>>>(t, max_norm, eps, norm);
+        return cudaGetLastError();
     }
-    return cudaSuccess;
+    if (tensors <= kCapFew) return clip<kCapFew>(g, tensors, part, max_norm, eps, norm, s);
+    return clip<kCap>(g, tensors, part, max_norm, eps, norm, s);
 }
 
 }  // namespace nfx

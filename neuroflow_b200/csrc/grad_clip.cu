@@ -135,66 +135,88 @@ __device__ __forceinline__ double chunk_squares(const Table<CAP>& t, int64_t c) 
     return squares_of<__half, THREADS>(static_cast<const __half*>(t.e[k].src), n, shift, i0, i1);
 }
 
-// Eight elements from `src` on, which lies `q` elements behind a 16-byte boundary: the words that hold them, moved
-// into place.
-template <typename T>
-__device__ __forceinline__ void load_moved(const T* src, int q, float (&o)[8]) {
-    constexpr int kWords = sizeof(T) == 4 ? 12 : 8;
-    uint32_t w[kWords];
-    const uint4* p = reinterpret_cast<const uint4*>(src - q);
+// Eight elements that lie `q` elements behind a 16-byte boundary: the words that hold them, and how they are moved
+// into place.  MOVED: q > 0.
+template <typename T, bool MOVED>
+struct Moved {
+    static constexpr int kQuads = (sizeof(T) == 4 ? 2 : 1) + (MOVED ? 1 : 0);
+    uint32_t w[4 * kQuads];
+    __device__ __forceinline__ void load(const T* boundary) {
 #pragma unroll
-    for (int i = 0; i < kWords / 4; ++i) {
-        uint4 u = make_uint4(0, 0, 0, 0);
-        if (i < (sizeof(T) == 4 ? 2 : 1) || q > 0) u = __ldcs(p + i);
-        w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
+        for (int i = 0; i < kQuads; ++i) {
+            const uint4 u = __ldcs(reinterpret_cast<const uint4*>(boundary) + i);
+            w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
+        }
     }
-    const int words = sizeof(T) == 4 ? q : q >> 1;
-    if (words & 2) {
+    __device__ __forceinline__ void get(int q, float (&o)[8]) {
+        if constexpr (MOVED) {
+            const int words = sizeof(T) == 4 ? q : q >> 1;
+            if (words & 2) {
 #pragma unroll
-        for (int i = 0; i + 2 < kWords; ++i) w[i] = w[i + 2];
-    }
-    if (words & 1) {
+                for (int i = 0; i + 2 < 4 * kQuads; ++i) w[i] = w[i + 2];
+            }
+            if (words & 1) {
 #pragma unroll
-        for (int i = 0; i + 1 < kWords; ++i) w[i] = w[i + 1];
-    }
-    if constexpr (sizeof(T) == 4) {
+                for (int i = 0; i + 1 < 4 * kQuads; ++i) w[i] = w[i + 1];
+            }
+            if (sizeof(T) == 2 && (q & 1)) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = __uint_as_float(w[i]);
-    } else {
-        if (q & 1) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 16);
+                for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 16);
+            }
         }
         Elems<T, 8> e;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) e.w[i] = w[i];
+        for (int i = 0; i < Elems<T, 8>::kWords; ++i) e.w[i] = w[i];
         e.get(o);
     }
-}
+};
 
-// out = src s for the chunk's elements, by packs of eight that start on a 16-byte boundary of `dst`.
-template <typename T, typename D, int THREADS>
-__device__ __forceinline__ void scale_chunk(const T* src, D* dst, int64_t n, int shift, int64_t i0, int64_t i1, float s) {
-    for (int64_t b = i0 + threadIdx.x * 8; b < i1; b += THREADS * 8) {
+// out = src s for packs of eight that start on a 16-byte boundary of `dst`, [i0, i1) counted from the last one
+// before its first element.
+template <typename T, typename D, int THREADS, bool MOVED>
+__device__ __forceinline__ void scale_packs(const T* src, D* dst, int64_t n, int shift, int q, int64_t i0, int64_t i1, float s) {
+    constexpr int kSpan = MOVED ? 8 + 16 / static_cast<int>(sizeof(T)) : 8;  // elements of the words that are read
+    const auto put = [&](int64_t c, Moved<T, MOVED>& m) {
+        float v[8];
+        m.get(q, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] *= s;
+        Elems<D, 8> o;
+        o.set(v);
+#pragma unroll
+        for (int i = 0; i < Elems<D, 8>::kWords; i += 4)
+            __stcs(reinterpret_cast<uint4*>(dst + c) + i / 4, make_uint4(o.w[i], o.w[i + 1], o.w[i + 2], o.w[i + 3]));
+    };
+    constexpr int kStep = THREADS * 8;
+    for (int64_t b = i0 + threadIdx.x * 8; b < i1; b += kStep * kGroupPacks) {
         const int64_t c = b - shift;
-        // the words that hold the eight elements lie inside the tensor
-        const int q = static_cast<int>(reinterpret_cast<uintptr_t>(src + c) % 16 / sizeof(T));
-        if (c - q >= 0 && c - q + (q > 0 ? 8 + 16 / static_cast<int>(sizeof(T)) : 8) <= n) {
-            float v[8];
-            load_moved(src + c, q, v);
+        Moved<T, MOVED> m[kGroupPacks];
+        // the words of all packs lie inside the tensor
+        if (c - q >= 0 && b + (kGroupPacks - 1) * kStep < i1 && c - q + (kGroupPacks - 1) * kStep + kSpan <= n) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] *= s;
-            Elems<D, 8> o;
-            o.set(v);
+            for (int k = 0; k < kGroupPacks; ++k) m[k].load(src + c + k * kStep - q);
 #pragma unroll
-            for (int i = 0; i < Elems<D, 8>::kWords; i += 4)
-                __stcs(reinterpret_cast<uint4*>(dst + c) + i / 4, make_uint4(o.w[i], o.w[i + 1], o.w[i + 2], o.w[i + 3]));
-        } else {
+            for (int k = 0; k < kGroupPacks; ++k) put(c + k * kStep, m[k]);
+            continue;
+        }
+        for (int k = 0; k < kGroupPacks && b + k * kStep < i1; ++k) {
+            const int64_t at = c + k * kStep;
+            if (at - q >= 0 && at - q + kSpan <= n) {
+                m[0].load(src + at - q);
+                put(at, m[0]);
+            } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (c + i >= 0 && c + i < n) dst[c + i] = from_f32<D>(to_f32(src[c + i]) * s);
+                for (int i = 0; i < 8; ++i)
+                    if (at + i >= 0 && at + i < n) dst[at + i] = from_f32<D>(to_f32(src[at + i]) * s);
+            }
         }
     }
+}
+template <typename T, typename D, int THREADS>
+__device__ __forceinline__ void scale_chunk(const T* src, D* dst, int64_t n, int shift, int64_t i0, int64_t i1, float s) {
+    const int q = static_cast<int>((reinterpret_cast<uintptr_t>(src) - shift * sizeof(T)) % 16 / sizeof(T));
+    if (q == 0) scale_packs<T, D, THREADS, false>(src, dst, n, shift, q, i0, i1, s);
+    else scale_packs<T, D, THREADS, true>(src, dst, n, shift, q, i0, i1, s);
 }
 
 template <int CAP, int THREADS>

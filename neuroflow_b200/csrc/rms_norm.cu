@@ -97,13 +97,15 @@ __global__ void __launch_bounds__(kAnyThreads) rms_any_kernel(RmsArgs a) {
 // takes more.
 constexpr int row_blocks(int most, int coming) { return most >= 512 ? 1 : (coming <= 16 ? 768 : 512) / most; }
 
+constexpr int kFp8Row = kGroup + kGroup / 32;  // words of a group of a row on its way to FP8
+
 template <typename T, typename H, int VE, int VPT, int MOST, bool ONE, bool FP8, bool EDGE>
 __global__ void __launch_bounds__(MOST, row_blocks(MOST, VE * VPT * static_cast<int>(sizeof(T) + sizeof(H)) / 4))
 rms_row_kernel(RmsArgs a, Shift sh, bool gvec, bool wide) {
     __shared__ float red[2][MOST / 32];
     extern __shared__ __align__(16) float room[];  // gamma (rows over 4,096 columns), then rows on their way to FP8
     constexpr int kRows = ONE ? MOST / 32 : 1;
-    constexpr bool kGammaShared = !ONE && MOST >= 512;
+    constexpr bool kGammaShared = !ONE && MOST >= 512, kEdges = EDGE && VE > 1;
     const int lane = threadIdx.x & 31, warps = ONE ? 1 : blockDim.x >> 5;
     const int sub = ONE ? lane : threadIdx.x, mine = ONE ? threadIdx.x >> 5 : 0;
     const int first = (sub >> 5) * VPT * 32 + lane, elems = warps * 32 * VPT * VE;
@@ -111,35 +113,39 @@ rms_row_kernel(RmsArgs a, Shift sh, bool gvec, bool wide) {
     const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
     // (the launcher makes `step` rows a whole number of boundaries: s is the same in all rows of a thread)
     const int s = EDGE ? static_cast<int>((sh.base + (static_cast<int64_t>(blockIdx.x) * kRows + mine) * sh.step) % VE) : 0;
-    const auto column = [&](int j) { return (first + j * 32) * VE - s; };
-    const auto inside = [&](int c) { return EDGE ? c >= 0 && c + VE <= a.d : c < a.d; };  // without EDGE a row is whole packs
-    const auto touches = [&](int c) { return c < a.d && c + VE > 0; };
+    const Split<VE> sp(a.d, s, sub);
+    const auto column = [&](int j) { return (EDGE ? sp.head : 0) + (first + j * 32) * VE; };
+    const auto inside = [&](int j) { return EDGE ? first + j * 32 < sp.packs : (first + j * 32) * VE < a.d; };
 
     Elems<T, VE> rx[VPT];
     Elems<H, VE> rr[VPT];
+    Elems<T, 1> ex;  // the edge element
+    Elems<H, 1> er;
+    ex.zero(), er.zero();
     const auto fetch = [&](int64_t r) {
         const T* x = static_cast<const T*>(a.x) + r * a.ldx;
         const H* res = static_cast<const H*>(a.res) + r * a.ldres;
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
             const int c = column(j);
-            if (r < a.rows && inside(c)) {
+            if (r < a.rows && inside(j)) {
                 rx[j].load(x + c);
                 if (a.res) rr[j].load(res + c);
-            } else if (EDGE && VE > 1 && r < a.rows && touches(c)) {
-                rx[j].load_part(x, c, a.d);
-                if (a.res) rr[j].load_part(res, c, a.d);
             } else {
                 rx[j].zero();
                 rr[j].zero();
             }
+        }
+        if (kEdges && sp.edge >= 0 && r < a.rows) {
+            ex.load(x + sp.edge);
+            if (a.res) er.load(res + sp.edge);
         }
     };
     fetch(static_cast<int64_t>(blockIdx.x) * kRows + mine);
     float gam[kGammaShared ? 1 : VPT][VE];
     if constexpr (kGammaShared) {
         for (int i = threadIdx.x; i < elems; i += blockDim.x)
-            room[i] = a.gamma && i - s >= 0 && i - s < a.d ? load_any(a.gamma, a.ptype, i - s) : 1.0f;
+            room[i] = a.gamma && column(0) - first * VE + i < a.d ? load_any(a.gamma, a.ptype, column(0) - first * VE + i) : 1.0f;
         __syncthreads();
     } else {
 #pragma unroll
@@ -149,10 +155,11 @@ rms_row_kernel(RmsArgs a, Shift sh, bool gvec, bool wide) {
                 load_params<T, VE>(a.gamma, a.ptype, gvec, c, 1.0f, gam[j]);
             } else {
 #pragma unroll
-                for (int i = 0; i < VE; ++i) gam[j][i] = EDGE && a.gamma && c + i >= 0 && c + i < a.d ? load_any(a.gamma, a.ptype, c + i) : 1.0f;
+                for (int i = 0; i < VE; ++i) gam[j][i] = EDGE && a.gamma && c + i < a.d ? load_any(a.gamma, a.ptype, c + i) : 1.0f;
             }
         }
     }
+    const float egam = kEdges && a.gamma && sp.edge >= 0 ? load_any(a.gamma, a.ptype, sp.edge) : 1.0f;
     int buf = 0;
     for (int64_t base = static_cast<int64_t>(blockIdx.x) * kRows; base < a.rows; base += step, buf ^= 1) {
         const int64_t r = base + mine;
@@ -172,9 +179,7 @@ rms_row_kernel(RmsArgs a, Shift sh, bool gvec, bool wide) {
                 o.get(v[j]);
                 if (a.sum && live) {
                     H* sum = static_cast<H*>(a.sum) + r * a.ldsum;
-                    const int c = column(j);
-                    if (inside(c)) o.store(sum + c);
-                    else if (EDGE && VE > 1 && touches(c)) o.store_part(sum, c, a.d);
+                    if (inside(j)) o.store(sum + column(j));
                 }
             }
             if constexpr (VE == 1) {
@@ -187,12 +192,23 @@ rms_row_kernel(RmsArgs a, Shift sh, bool gvec, bool wide) {
                 }
             }
         }
+        float ev = 0.0f;
+        if (kEdges && sp.edge >= 0) {
+            ev = ex.at(0);
+            if (a.res) {
+                const float f[1] = {ev + er.at(0)};
+                Elems<H, 1> o;
+                o.set(f);
+                ev = o.at(0);
+                if (a.sum && live) o.store(static_cast<H*>(a.sum) + r * a.ldsum + sp.edge);
+            }
+            q2.x = fmaf(ev, ev, q2.x);
+        }
         fetch(r + step);  // the next row comes while this one is worked on
         const float rs = __frsqrt_rn(row_sum<ONE>(q2.x + q2.y, red[buf], warps) * inv_d + a.eps);
         if (live && sub == 0 && a.rstd) a.rstd[r] = rs;
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
-            const int c = column(j);
             float g[VE];
             if constexpr (kGammaShared && VE > 1) {
 #pragma unroll
@@ -214,34 +230,38 @@ rms_row_kernel(RmsArgs a, Shift sh, bool gvec, bool wide) {
                 }
             }
             if constexpr (!FP8) {
-                if (live) {
-                    T* y = static_cast<T*>(a.y) + r * a.ldy;
-                    Elems<T, VE> o;
-                    o.set(v[j]);
-                    if (inside(c)) o.store(y + c);
-                    else if (EDGE && VE > 1 && touches(c)) o.store_part(y, c, a.d);
-                }
+                Elems<T, VE> o;
+                o.set(v[j]);
+                if (live && inside(j)) o.store(static_cast<T*>(a.y) + r * a.ldy + column(j));
             }
+        }
+        if (kEdges && sp.edge >= 0) {
+            ev = (ev * rs) * egam;
+            if (!FP8 && live) static_cast<T*>(a.y)[r * a.ldy + sp.edge] = from_f32<T>(ev);
         }
         if constexpr (FP8 && !EDGE) {
             store_codes<VE, VPT, 32>(v, a.q, r, a.d, live, first, lane, wide);
         } else if constexpr (FP8) {
-            // through shared memory to groups of 128 columns, a warp each, four columns a lane
-            const int padded = (a.d + kGroup - 1) / kGroup * kGroup;
-            float* row = room + (kGammaShared ? elems : 0) + mine * padded;
+            // through shared memory to groups of 128 columns, a warp each, four columns a lane; a word in 33 is left
+            // out, so that lanes eight (and four) columns apart meet different banks
+            const int blocks = (a.d + kGroup - 1) / kGroup;
+            float* row = room + (kGammaShared ? elems : 0) + mine * blocks * kFp8Row;
+            const auto at = [&](int c) -> float& { return row[c + (c >> 5)]; };
 #pragma unroll
-            for (int j = 0; j < VPT; ++j)
+            for (int j = 0; j < VPT; ++j) {
+                if (!inside(j)) continue;
 #pragma unroll
-                for (int i = 0; i < VE; ++i)
-                    if (const int c = column(j) + i; c >= 0 && c < a.d) row[c] = v[j][i];
+                for (int i = 0; i < VE; ++i) at(column(j) + i) = v[j][i];
+            }
+            if (kEdges && sp.edge >= 0) at(sp.edge) = ev;
             if constexpr (ONE) __syncwarp();
             else __syncthreads();
-            for (int b = sub >> 5; b < padded / kGroup; b += warps) {
+            for (int b = sub >> 5; b < blocks; b += warps) {
                 const int c = b * kGroup + lane * 4;
                 float o[4], top = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    o[i] = c + i < a.d ? row[c + i] : 0.0f;
+                    o[i] = c + i < a.d ? at(c + i) : 0.0f;
                     top = fmaxf(top, finite_abs(o[i]));
                 }
                 const float sc = group_scale(warp_max(top)), inv = __frcp_rn(sc);
@@ -266,20 +286,19 @@ rms_row_kernel(RmsArgs a, Shift sh, bool gvec, bool wide) {
 template <typename T, typename H, int VE, int VPT, int MOST, bool ONE, bool FP8, bool EDGE>
 cudaError_t rms_row_go(const RmsArgs& a, cudaStream_t s) {
     auto kern = rms_row_kernel<T, H, VE, VPT, MOST, ONE, FP8, EDGE>;
-    const int span = a.d + (EDGE ? VE - 1 : 0);  // the first pack may begin before the row
-    const int threads = ONE ? MOST : (span + 32 * VPT * VE - 1) / (32 * VPT * VE) * 32, rows = ONE ? MOST / 32 : 1;
-    const int smem = (!ONE && MOST >= 512 ? threads * VPT * VE * 4 : 0) + (FP8 && EDGE ? rows * ((a.d + kGroup - 1) / kGroup * kGroup) * 4 : 0);
-    // the most that any width of this kernel asks for
-    constexpr int kMost = (!ONE && MOST >= 512 ? MOST * VPT * VE * 4 : 0) +
-                          (FP8 && EDGE ? (ONE ? MOST / 32 * (32 * VPT * VE + kGroup) : MOST * VPT * VE + kGroup) * 4 : 0);
-    const cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), kMost);
+    // (a row's packs are d / VE at most, its edges go beside them)
+    const int threads = ONE || a.d < 32 * VPT * VE ? (ONE ? MOST : 32) : (a.d + 32 * VPT * VE - 1) / (32 * VPT * VE) * 32, rows = ONE ? MOST / 32 : 1;
+    constexpr int kGammaBytes = !ONE && MOST >= 512 ? VPT * VE * 4 : 0;  // a thread
+    const auto smem_of = [&](int n, int d) { return n * kGammaBytes + (FP8 && EDGE ? rows * ((d + kGroup - 1) / kGroup) * kFp8Row * 4 : 0); };
+    // a block of `threads` holds rows of up to `room` columns: what they ask for decides how many blocks an SM has
+    const int room = (ONE ? 32 : threads) * VPT * VE + VE;
+    const cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), smem_of(MOST, (ONE ? 32 : MOST) * VPT * VE + VE));
     if (e != cudaSuccess) return e;
     static std::atomic<int> known[64][MOST / 32];  // asked for once per kernel, device and size of block
     std::atomic<int>& at = known[current_device() & 63][threads / 32 - 1];
     int most = at.load(std::memory_order_relaxed);
     if (most == 0) {
-        const int room = (!ONE && MOST >= 512 ? threads * VPT * VE * 4 : 0) + (FP8 && EDGE ? rows * (threads / (ONE ? rows : 1) * VPT * VE + kGroup) * 4 : 0);
-        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&most, kern, threads, room) != cudaSuccess || most < 1) most = 1;
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&most, kern, threads, smem_of(threads, room)) != cudaSuccess || most < 1) most = 1;
         most *= device_sm_count();
         at.store(most, std::memory_order_relaxed);
     }
@@ -289,7 +308,7 @@ cudaError_t rms_row_go(const RmsArgs& a, cudaStream_t s) {
     const Shift sh = shift_of(a.x, a.ldx, sizeof(T), VE);
     const bool gvec = aligned16(a.gamma) && (a.ptype == kF32 || VE == 8);
     const bool wide = FP8 && reinterpret_cast<uintptr_t>(a.q.codes) % 8 == 0 && (a.rows == 1 || a.q.ld % 8 == 0);
-    kern<<<static_cast<unsigned>(grid), threads, smem, s>>>(a, sh, gvec, wide);
+    kern<<<static_cast<unsigned>(grid), threads, smem_of(threads, a.d), s>>>(a, sh, gvec, wide);
     return cudaGetLastError();
 }
 
@@ -297,7 +316,7 @@ cudaError_t rms_row_go(const RmsArgs& a, cudaStream_t s) {
 template <typename T, typename H, int VE, bool FP8, bool EDGE>
 cudaError_t rms_width(const RmsArgs& a, cudaStream_t s) {
     constexpr int k16 = 16 / VE;
-    const int d = a.d + (EDGE ? VE - 1 : 0);
+    const int d = a.d;
     if constexpr (VE == 1) {  // (more loads to a row than a warp should queue)
         if (d <= 2048) return rms_row_go<T, H, 1, 8, 256, false, FP8, true>(a, s);
         if (d <= 8192) return rms_row_go<T, H, 1, 16, 512, false, FP8, true>(a, s);
@@ -316,12 +335,12 @@ cudaError_t rms_width(const RmsArgs& a, cudaStream_t s) {
 template <typename T, typename H, bool FP8>
 cudaError_t rms_form(const RmsArgs& a, cudaStream_t s) {
     constexpr int VE = 16 / sizeof(T);
-    if (a.d <= 16384 - VE + 1 || (a.d <= 16384 && a.d % VE == 0)) {
+    if (a.d <= 16384) {
         const Shift sx = shift_of(a.x, a.ldx, sizeof(T), VE);
         const auto like = [&](const void* p, int64_t ld, int64_t el) { return !p || same_shift(sx, shift_of(p, ld, el, VE), a.rows); };
         if (like(a.res, a.ldres, sizeof(H)) && like(a.sum, a.ldsum, sizeof(H)) && (FP8 || like(a.y, a.ldy, sizeof(T)))) {
             if (sx.base == 0 && (a.rows == 1 || sx.step == 0) && a.d % VE == 0) return rms_width<T, H, VE, FP8, false>(a, s);
-            if (a.d <= 16384 - VE + 1) return rms_width<T, H, VE, FP8, true>(a, s);
+            return rms_width<T, H, VE, FP8, true>(a, s);
         }
     }
     if (a.d <= 16384) return rms_width<T, H, 1, FP8, true>(a, s);

@@ -67,7 +67,7 @@ constexpr int grad_blocks(int most) { return most >= 512 ? 1 : 512 / most; }
 template <typename T, typename H, int VE, int VPT, int MOST, bool ONE, bool EDGE>
 __global__ void __launch_bounds__(MOST, grad_blocks(MOST)) rms_grad_row_kernel(RmsGradArgs a, Shift sh, bool gvec) {
     __shared__ float red[2][MOST / 32];
-    constexpr bool kShared = MOST == 1024;
+    constexpr bool kShared = MOST == 1024, kEdges = EDGE && VE > 1;
     constexpr int kRows = ONE ? MOST / 32 : 1, E = VPT * VE;
     // ONE: element e of lane l at e 32 + l, to join the rows' sums; kShared: the sums, element e of thread t at e
     // threads + t (no bank conflicts), then gamma in the same way
@@ -78,12 +78,15 @@ __global__ void __launch_bounds__(MOST, grad_blocks(MOST)) rms_grad_row_kernel(R
     const float inv_d = __frcp_rn(static_cast<float>(a.d));
     const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
     const int s = EDGE ? static_cast<int>((sh.base + (static_cast<int64_t>(blockIdx.x) * kRows + mine) * sh.step) % VE) : 0;
-    const auto column = [&](int j) { return (first + j * 32) * VE - s; };
-    const auto inside = [&](int c) { return EDGE ? c >= 0 && c + VE <= a.d : c < a.d; };
-    const auto touches = [&](int c) { return c < a.d && c + VE > 0; };
+    const Split<VE> sp(a.d, s, sub);
+    const auto column = [&](int j) { return (EDGE ? sp.head : 0) + (first + j * 32) * VE; };
+    const auto inside = [&](int j) { return EDGE ? first + j * 32 < sp.packs : (first + j * 32) * VE < a.d; };
 
     Elems<T, VE> ny[VPT];
     Elems<H, VE> nh[VPT], ns[VPT];
+    Elems<T, 1> ey;  // the edge element
+    Elems<H, 1> eh, es;
+    ey.zero(), eh.zero(), es.zero();
     float next_rs = 0.0f;
     const auto fetch = [&](int64_t r) {
         const T* dy = static_cast<const T*>(a.dy) + r * a.lddy;
@@ -93,16 +96,21 @@ __global__ void __launch_bounds__(MOST, grad_blocks(MOST)) rms_grad_row_kernel(R
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
             const int c = column(j);
-            if (r < a.rows && inside(c)) {
+            if (r < a.rows && inside(j)) {
                 ny[j].load(dy + c);
                 nh[j].load(h + c);
                 if (a.dsum) ns[j].load(ds + c);
-            } else if (EDGE && VE > 1 && r < a.rows && touches(c)) {
-                ny[j].load_part(dy, c, a.d);
-                nh[j].load_part(h, c, a.d);
-                if (a.dsum) ns[j].load_part(ds, c, a.d);
             } else {
                 ny[j].zero(), nh[j].zero(), ns[j].zero();
+            }
+        }
+        if (kEdges && sp.edge >= 0) {
+            if (r < a.rows) {
+                ey.load(dy + sp.edge);
+                eh.load(h + sp.edge);
+                if (a.dsum) es.load(ds + sp.edge);
+            } else {
+                ey.zero(), eh.zero();
             }
         }
     };
@@ -117,7 +125,7 @@ __global__ void __launch_bounds__(MOST, grad_blocks(MOST)) rms_grad_row_kernel(R
             load_params<T, VE>(a.gamma, a.ptype, gvec, c, 1.0f, g);
         } else {
 #pragma unroll
-            for (int i = 0; i < VE; ++i) g[i] = EDGE && a.gamma && c + i >= 0 && c + i < a.d ? load_any(a.gamma, a.ptype, c + i) : 1.0f;
+            for (int i = 0; i < VE; ++i) g[i] = EDGE && a.gamma && c + i < a.d ? load_any(a.gamma, a.ptype, c + i) : 1.0f;
         }
 #pragma unroll
         for (int i = 0; i < VE; ++i) {
@@ -125,6 +133,8 @@ __global__ void __launch_bounds__(MOST, grad_blocks(MOST)) rms_grad_row_kernel(R
             else gam[j][i] = g[i], pg[j][i] = 0.0f;
         }
     }
+    const float egam = kEdges && a.gamma && sp.edge >= 0 ? load_any(a.gamma, a.ptype, sp.edge) : 1.0f;
+    float epg = 0.0f;
     int buf = 0;
     if (!kShared) fetch(static_cast<int64_t>(blockIdx.x) * kRows + mine);
     for (int64_t base = static_cast<int64_t>(blockIdx.x) * kRows; base < a.rows; base += step, buf ^= 1) {
@@ -135,9 +145,14 @@ __global__ void __launch_bounds__(MOST, grad_blocks(MOST)) rms_grad_row_kernel(R
         Elems<H, VE> h[VPT], ds[VPT];
 #pragma unroll
         for (int j = 0; j < VPT; ++j) y[j] = ny[j], h[j] = nh[j], ds[j] = ns[j];
-        const float rs = next_rs;
+        const float rs = next_rs, fy = ey.at(0), fh = eh.at(0), fs = es.at(0);
         if (!kShared) fetch(r + step);
         float t = 0.0f;
+        if (kEdges) {
+            const float dyx = fy * (fh * rs);
+            t = egam * dyx;
+            epg += dyx;
+        }
 #pragma unroll
         for (int j = 0; j < VPT; ++j)
 #pragma unroll
@@ -156,8 +171,8 @@ __global__ void __launch_bounds__(MOST, grad_blocks(MOST)) rms_grad_row_kernel(R
         if (!live) continue;
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
+            if (!inside(j)) continue;
             const int c = column(j);
-            if (!touches(c)) continue;
             float o[VE];
 #pragma unroll
             for (int i = 0; i < VE; ++i) {
@@ -169,16 +184,20 @@ __global__ void __launch_bounds__(MOST, grad_blocks(MOST)) rms_grad_row_kernel(R
                 T* dx = static_cast<T*>(a.dx) + r * a.lddx;
                 Elems<T, VE> w;
                 w.set(o);
-                if (inside(c)) w.store(dx + c);
-                else w.store_part(dx, c, a.d);
+                w.store(dx + c);
             }
             if (a.dres) {
                 H* dr = static_cast<H*>(a.dres) + r * a.lddres;
                 Elems<H, VE> w;
                 w.set(o);
-                if (inside(c)) w.store(dr + c);
-                else w.store_part(dr, c, a.d);
+                w.store(dr + c);
             }
+        }
+        if (kEdges && sp.edge >= 0) {
+            float o = rs * fmaf(-fh, m, fy * egam);
+            if (a.dsum) o += fs;
+            if (a.dx) static_cast<T*>(a.dx)[r * a.lddx + sp.edge] = from_f32<T>(o);
+            if (a.dres) static_cast<H*>(a.dres)[r * a.lddres + sp.edge] = from_f32<H>(o);
         }
     }
     if (!a.part) return;
@@ -186,13 +205,14 @@ __global__ void __launch_bounds__(MOST, grad_blocks(MOST)) rms_grad_row_kernel(R
     if constexpr (ONE) {
         // the block's rows join their sums, one warp after the other (with EDGE each warp's columns are its own: by column)
         if constexpr (EDGE) {
-            for (int i = threadIdx.x; i < 32 * E; i += threads) room[i] = 0.0f;
+            for (int i = threadIdx.x; i < a.d; i += threads) room[i] = 0.0f;
             __syncthreads();
             for (int k = 0; k < kRows; ++k) {
                 if (mine == k) {
 #pragma unroll
                     for (int e = 0; e < E; ++e)
-                        if (const int c = column(e / VE) + e % VE; c >= 0 && c < a.d) room[c] += pg[e / VE][e % VE];
+                        if (inside(e / VE)) room[column(e / VE) + e % VE] += pg[e / VE][e % VE];
+                    if (kEdges && sp.edge >= 0) room[sp.edge] += epg;
                 }
                 __syncthreads();
             }
@@ -221,16 +241,16 @@ __global__ void __launch_bounds__(MOST, grad_blocks(MOST)) rms_grad_row_kernel(R
         float o[VE];
 #pragma unroll
         for (int i = 0; i < VE; ++i) o[i] = kShared ? sums[(j * VE + i) * threads + sub] : pg[j][i];
+        if (!inside(j)) continue;
         if constexpr (!EDGE) {  // (d is a multiple of VE, the workspace 16-byte aligned)
-            if (c >= a.d) continue;
 #pragma unroll
             for (int i = 0; i < VE; i += 4) *reinterpret_cast<float4*>(out + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
         } else {
 #pragma unroll
-            for (int i = 0; i < VE; ++i)
-                if (c + i >= 0 && c + i < a.d) out[c + i] = o[i];
+            for (int i = 0; i < VE; ++i) out[c + i] = o[i];
         }
     }
+    if (kEdges && sp.edge >= 0) out[sp.edge] = epg;
 }
 
 // Launches as many blocks as are resident, at most a.parts, and leaves their number there.
@@ -238,9 +258,9 @@ template <typename T, typename H, int VE, int VPT, int MOST, bool ONE, bool EDGE
 cudaError_t rms_grad_go(RmsGradArgs& a, cudaStream_t s) {
     auto kern = rms_grad_row_kernel<T, H, VE, VPT, MOST, ONE, EDGE>;
     constexpr int E = VPT * VE;
-    const int span = a.d + (EDGE ? VE - 1 : 0);
-    const int threads = ONE ? MOST : (span + 32 * E - 1) / (32 * E) * 32, rows = ONE ? MOST / 32 : 1;
-    const int smem = MOST == 1024 ? 2 * E * threads * 4 : (ONE ? E * 32 * 4 : 0);
+    // (a row's packs are d / VE at most, its edges go beside them)
+    const int threads = ONE ? MOST : (a.d + 32 * E - 1) / (32 * E) * 32, rows = ONE ? MOST / 32 : 1;
+    const int smem = MOST == 1024 ? 2 * E * threads * 4 : (ONE ? (E * 32 + VE) * 4 : 0);
     const cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), MOST == 1024 ? 2 * E * 1024 * 4 : smem);
     if (e != cudaSuccess) return e;
     static std::atomic<int> known[64][MOST / 32];  // asked for once per kernel, device and size of block
@@ -263,7 +283,7 @@ cudaError_t rms_grad_go(RmsGradArgs& a, cudaStream_t s) {
 // Sixteen elements a thread where a row's three numbers have 16 bits, eight where some have 32.
 template <typename T, typename H, int VE, bool EDGE>
 cudaError_t rms_grad_width(RmsGradArgs& a, cudaStream_t s) {
-    const int d = a.d + (EDGE ? VE - 1 : 0);
+    const int d = a.d;
     if constexpr (sizeof(H) == 2 && VE > 1) {
         if (d <= 512) return rms_grad_go<T, H, VE, 16 / VE, 256, true, EDGE>(a, s);
         if (d <= 4096) return rms_grad_go<T, H, VE, 16 / VE, 256, false, EDGE>(a, s);
@@ -286,7 +306,7 @@ cudaError_t rms_grad_t(RmsGradArgs& a, cudaStream_t s) {
     const auto like = [&](const void* p, int64_t ld, int64_t el) { return !p || same_shift(sy, shift_of(p, ld, el, VE), a.rows); };
     if (like(a.h, a.ldh, sizeof(H)) && like(a.dsum, a.lddsum, sizeof(H)) && like(a.dx, a.lddx, sizeof(T)) && like(a.dres, a.lddres, sizeof(H))) {
         if (a.d <= 16384 && sy.base == 0 && (a.rows == 1 || sy.step == 0) && a.d % VE == 0) return rms_grad_width<T, H, VE, false>(a, s);
-        if (a.d <= 16384 - VE + 1) return rms_grad_width<T, H, VE, true>(a, s);
+        if (a.d <= 16384) return rms_grad_width<T, H, VE, true>(a, s);
     }
     if (a.d <= 16384) return rms_grad_width<T, H, 1, true>(a, s);
     rms_grad_any_kernel<T, H><<<a.parts, kAnyThreads, 0, s>>>(a);

@@ -1,11 +1,11 @@
 // rms_parts.cuh -- what the RMS norm's forward and backward kernels share: packs of a row whose first element
 // may lie anywhere, and sums over a row's threads.
 //
-// Rows that do not start on 16-byte boundaries (an odd width) are read by 16-byte words all the same: with
-// s the number of elements from the last boundary to the row's start, pack q holds columns q VE - s ..
-// q VE - s + VE - 1, and only a row's first and last pack go by elements.  That asks for tensors whose rows
-// start at the same distance from a boundary, counted in elements (tensors of one shape, contiguous, do);
-// elsewhere packs are single elements.
+// Rows that do not start on 16-byte boundaries (an odd width) are read by 16-byte words all the same: up to VE - 1
+// elements in front of the first boundary and behind the last one are the row's edges, an element each for the
+// first lanes of its first warp, and what lies between them is whole packs.  That asks for tensors whose rows start
+// at the same distance from a boundary, counted in elements (tensors of one shape, contiguous, do); elsewhere
+// packs are single elements.
 #pragma once
 
 #include "block_ops.h"
@@ -34,16 +34,6 @@ struct Elems {
             w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
         } else {
             w[0] = __ldg(reinterpret_cast<const uint16_t*>(p));
-        }
-    }
-    // columns c .. of row p that are inside [0, d), zeros beside them
-    __device__ __forceinline__ void load_part(const T* p, int c, int d) {
-        zero();
-#pragma unroll
-        for (int i = 0; i < VE; ++i) {
-            if (c + i < 0 || c + i >= d) continue;
-            if constexpr (sizeof(T) == 4) w[i] = __ldg(reinterpret_cast<const uint32_t*>(p) + c + i);
-            else w[i / 2] |= static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t*>(p) + c + i)) << (16 * (i & 1));
         }
     }
     __device__ __forceinline__ float at(int i) const {
@@ -78,14 +68,6 @@ struct Elems {
             *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(w[0]);
         }
     }
-    __device__ __forceinline__ void store_part(T* p, int c, int d) const {
-#pragma unroll
-        for (int i = 0; i < VE; ++i) {
-            if (c + i < 0 || c + i >= d) continue;
-            if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(p)[c + i] = w[i];
-            else reinterpret_cast<uint16_t*>(p)[c + i] = static_cast<uint16_t>(w[i / 2] >> (16 * (i & 1)));
-        }
-    }
 };
 
 // The sum of `a` over a row's threads, the same bits in each of them: a warp (ONE), or all `warps` of the block.
@@ -102,6 +84,19 @@ __device__ __forceinline__ float row_sum(float a, float* red, int warps) {
     }
     return a;
 }
+
+// How a row of d elements that starts s elements behind a boundary falls into edges and packs, and the edge element
+// that a thread takes (its column, or -1).
+template <int VE>
+struct Split {
+    int head, packs, edge;
+    __device__ __forceinline__ Split(int d, int s, int sub) {
+        head = min((VE - s) % VE, d);
+        packs = (d - head) / VE;
+        const int tail = head + packs * VE;
+        edge = sub < head ? sub : (sub >= VE && tail + sub - VE < d && sub < 2 * VE ? tail + sub - VE : -1);
+    }
+};
 
 // The distance in elements from the last VE-element boundary to a matrix' first element, and how a row moves it.
 struct Shift {

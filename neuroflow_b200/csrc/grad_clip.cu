@@ -22,7 +22,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kGroupPacks = 4;                                // packs of 16 bytes that a thread has in flight
 constexpr int kFewThreads = 512, kFewCluster = 8;
-constexpr int kPartBlocks = 8 * 148;                          // shares that one launch leaves, at most
+constexpr int kPartBlocks = 4 * 148;                          // shares that one launch leaves, at most
 
 struct Entry {
     const void* src;
@@ -68,10 +68,10 @@ __device__ __forceinline__ double block_sum(double v, double* red) {
 // The sum of squares of chunk elements [i0, i1) of a tensor, `i` counted from the last 16-byte boundary before its
 // first element (`shift` elements in front of it); this thread's share.
 template <typename T, int THREADS>
-__device__ __forceinline__ double squares_of(const T* src, int64_t n, int shift, int64_t i0, int64_t i1) {
+__device__ __forceinline__ double squares_of(const T* src, int64_t n, int shift, int64_t i0, int64_t i1, int tid) {
     constexpr int VE = 16 / sizeof(T);
     double sum = 0.0;
-    for (int64_t b = i0 + threadIdx.x * VE; b < i1; b += static_cast<int64_t>(THREADS) * VE * kGroupPacks) {
+    for (int64_t b = i0 + tid * VE; b < i1; b += static_cast<int64_t>(THREADS) * VE * kGroupPacks) {
         Elems<T, VE> v[kGroupPacks];
 #pragma unroll
         for (int k = 0; k < kGroupPacks; ++k) {
@@ -119,108 +119,116 @@ __device__ __forceinline__ double squares_of(const T* src, int64_t n, int shift,
 }
 
 // A chunk is this many elements, counted from a 16-byte boundary: finding its tensor takes a few hundred cycles.
-__host__ __device__ constexpr int64_t chunk_of(int threads) { return threads == kThreads ? 32768 : 16384; }
+// A warp takes as much as it can have in flight.
+__host__ __device__ constexpr int64_t chunk_of(int threads) { return threads == kThreads ? 32768 : 1024; }
 __host__ __device__ __forceinline__ int shift_el(const void* p, int type) {
     return static_cast<int>(reinterpret_cast<uintptr_t>(p) % 16 / (type == kF32 ? 4 : 2));
 }
 
 template <int CAP, int THREADS>
-__device__ __forceinline__ double chunk_squares(const Table<CAP>& t, int64_t c) {
+__device__ __forceinline__ double chunk_squares(const Table<CAP>& t, int64_t c, int tid) {
     const int k = tensor_of(t, c);
     const int64_t n = t.e[k].n;
     const int type = t.src_type[k], shift = shift_el(t.e[k].src, type);
     const int64_t i0 = (c - t.e[k].first) * chunk_of(THREADS), i1 = min(n + shift, i0 + chunk_of(THREADS));
-    if (type == kF32) return squares_of<float, THREADS>(static_cast<const float*>(t.e[k].src), n, shift, i0, i1);
-    if (type == kBF16) return squares_of<__nv_bfloat16, THREADS>(static_cast<const __nv_bfloat16*>(t.e[k].src), n, shift, i0, i1);
-    return squares_of<__half, THREADS>(static_cast<const __half*>(t.e[k].src), n, shift, i0, i1);
+    if (type == kF32) return squares_of<float, THREADS>(static_cast<const float*>(t.e[k].src), n, shift, i0, i1, tid);
+    if (type == kBF16) return squares_of<__nv_bfloat16, THREADS>(static_cast<const __nv_bfloat16*>(t.e[k].src), n, shift, i0, i1, tid);
+    return squares_of<__half, THREADS>(static_cast<const __half*>(t.e[k].src), n, shift, i0, i1, tid);
 }
 
-// Eight elements that lie `q` elements behind a 16-byte boundary: the words that hold them, and how they are moved
-// into place.  MOVED: q > 0.
-template <typename T, bool MOVED>
+// N elements that lie `q` elements behind a boundary: the words that hold them, and how they are moved into place.
+// Boundaries are of 16 bytes, or of what N elements take where that is less.  MOVED: q > 0.
+template <typename T, int N, bool MOVED>
 struct Moved {
-    static constexpr int kQuads = (sizeof(T) == 4 ? 2 : 1) + (MOVED ? 1 : 0);
-    uint32_t w[4 * kQuads];
+    static constexpr int kUnit = N * static_cast<int>(sizeof(T)) < 16 ? N * static_cast<int>(sizeof(T)) : 16;  // bytes
+    static constexpr int kUnits = N * static_cast<int>(sizeof(T)) / kUnit + (MOVED ? 1 : 0);
+    static constexpr int kWords = kUnits * kUnit / 4;
+    static constexpr int kSpan = kUnits * kUnit / static_cast<int>(sizeof(T));  // elements that are read
+    uint32_t w[kWords];
     __device__ __forceinline__ void load(const T* boundary) {
 #pragma unroll
-        for (int i = 0; i < kQuads; ++i) {
-            const uint4 u = __ldcs(reinterpret_cast<const uint4*>(boundary) + i);
-            w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
+        for (int i = 0; i < kUnits; ++i) {
+            if constexpr (kUnit == 16) {
+                const uint4 u = __ldcs(reinterpret_cast<const uint4*>(boundary) + i);
+                w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
+            } else {
+                const uint2 u = __ldcs(reinterpret_cast<const uint2*>(boundary) + i);
+                w[2 * i] = u.x, w[2 * i + 1] = u.y;
+            }
         }
     }
-    __device__ __forceinline__ void get(int q, float (&o)[8]) {
+    __device__ __forceinline__ void get(int q, float (&o)[N]) {
         if constexpr (MOVED) {
             const int words = sizeof(T) == 4 ? q : q >> 1;
             if (words & 2) {
 #pragma unroll
-                for (int i = 0; i + 2 < 4 * kQuads; ++i) w[i] = w[i + 2];
+                for (int i = 0; i + 2 < kWords; ++i) w[i] = w[i + 2];
             }
             if (words & 1) {
 #pragma unroll
-                for (int i = 0; i + 1 < 4 * kQuads; ++i) w[i] = w[i + 1];
+                for (int i = 0; i + 1 < kWords; ++i) w[i] = w[i + 1];
             }
             if (sizeof(T) == 2 && (q & 1)) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 16);
+                for (int i = 0; i < N / 2; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 16);
             }
         }
-        Elems<T, 8> e;
+        Elems<T, N> e;
 #pragma unroll
-        for (int i = 0; i < Elems<T, 8>::kWords; ++i) e.w[i] = w[i];
+        for (int i = 0; i < Elems<T, N>::kWords; ++i) e.w[i] = w[i];
         e.get(o);
     }
 };
 
-// out = src s for packs of eight that start on a 16-byte boundary of `dst`, [i0, i1) counted from the last one
-// before its first element.
+// out = src s for packs of 16 bytes of `dst`, elements [i0, i1) counted from the last 16-byte boundary before its
+// first element.
 template <typename T, typename D, int THREADS, bool MOVED>
-__device__ __forceinline__ void scale_packs(const T* src, D* dst, int64_t n, int shift, int q, int64_t i0, int64_t i1, float s) {
-    constexpr int kSpan = MOVED ? 8 + 16 / static_cast<int>(sizeof(T)) : 8;  // elements of the words that are read
-    const auto put = [&](int64_t c, Moved<T, MOVED>& m) {
-        float v[8];
+__device__ __forceinline__ void scale_packs(const T* src, D* dst, int64_t n, int shift, int q, int64_t i0, int64_t i1, float s, int tid) {
+    constexpr int N = 16 / sizeof(D), kSpan = Moved<T, N, MOVED>::kSpan, kStep = THREADS * N;
+    constexpr int kPacks = sizeof(T) == 2 && sizeof(D) == 4 ? 2 * kGroupPacks : kGroupPacks;
+    const auto put = [&](int64_t c, Moved<T, N, MOVED>& m) {
+        float v[N];
         m.get(q, v);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] *= s;
-        Elems<D, 8> o;
+        for (int i = 0; i < N; ++i) v[i] *= s;
+        Elems<D, N> o;
         o.set(v);
-#pragma unroll
-        for (int i = 0; i < Elems<D, 8>::kWords; i += 4)
-            __stcs(reinterpret_cast<uint4*>(dst + c) + i / 4, make_uint4(o.w[i], o.w[i + 1], o.w[i + 2], o.w[i + 3]));
+        __stcs(reinterpret_cast<uint4*>(dst + c), make_uint4(o.w[0], o.w[1], o.w[2], o.w[3]));
     };
-    constexpr int kStep = THREADS * 8;
-    for (int64_t b = i0 + threadIdx.x * 8; b < i1; b += kStep * kGroupPacks) {
+    for (int64_t b = i0 + tid * N; b < i1; b += kStep * kPacks) {
         const int64_t c = b - shift;
-        Moved<T, MOVED> m[kGroupPacks];
+        Moved<T, N, MOVED> m[kPacks];
         // the words of all packs lie inside the tensor
-        if (c - q >= 0 && b + (kGroupPacks - 1) * kStep < i1 && c - q + (kGroupPacks - 1) * kStep + kSpan <= n) {
+        if (c - q >= 0 && b + (kPacks - 1) * kStep < i1 && c - q + (kPacks - 1) * kStep + kSpan <= n) {
 #pragma unroll
-            for (int k = 0; k < kGroupPacks; ++k) m[k].load(src + c + k * kStep - q);
+            for (int k = 0; k < kPacks; ++k) m[k].load(src + c + k * kStep - q);
 #pragma unroll
-            for (int k = 0; k < kGroupPacks; ++k) put(c + k * kStep, m[k]);
+            for (int k = 0; k < kPacks; ++k) put(c + k * kStep, m[k]);
             continue;
         }
-        for (int k = 0; k < kGroupPacks && b + k * kStep < i1; ++k) {
+        for (int k = 0; k < kPacks && b + k * kStep < i1; ++k) {
             const int64_t at = c + k * kStep;
             if (at - q >= 0 && at - q + kSpan <= n) {
                 m[0].load(src + at - q);
                 put(at, m[0]);
             } else {
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
+                for (int i = 0; i < N; ++i)
                     if (at + i >= 0 && at + i < n) dst[at + i] = from_f32<D>(to_f32(src[at + i]) * s);
             }
         }
     }
 }
 template <typename T, typename D, int THREADS>
-__device__ __forceinline__ void scale_chunk(const T* src, D* dst, int64_t n, int shift, int64_t i0, int64_t i1, float s) {
-    const int q = static_cast<int>((reinterpret_cast<uintptr_t>(src) - shift * sizeof(T)) % 16 / sizeof(T));
-    if (q == 0) scale_packs<T, D, THREADS, false>(src, dst, n, shift, q, i0, i1, s);
-    else scale_packs<T, D, THREADS, true>(src, dst, n, shift, q, i0, i1, s);
+__device__ __forceinline__ void scale_chunk(const T* src, D* dst, int64_t n, int shift, int64_t i0, int64_t i1, float s, int tid) {
+    constexpr int kUnit = Moved<T, 16 / sizeof(D), false>::kUnit;
+    const int q = static_cast<int>((reinterpret_cast<uintptr_t>(src) - shift * sizeof(T)) % kUnit / sizeof(T));
+    if (q == 0) scale_packs<T, D, THREADS, false>(src, dst, n, shift, q, i0, i1, s, tid);
+    else scale_packs<T, D, THREADS, true>(src, dst, n, shift, q, i0, i1, s, tid);
 }
 
 template <int CAP, int THREADS>
-__device__ __forceinline__ void chunk_scale(const Table<CAP>& t, int64_t c, float s) {
+__device__ __forceinline__ void chunk_scale(const Table<CAP>& t, int64_t c, float s, int tid) {
     const int k = tensor_of(t, c);
     const Entry& e = t.e[k];
     if (s == 1.0f && e.dst == e.src) return;  // every element times one
@@ -228,13 +236,13 @@ __device__ __forceinline__ void chunk_scale(const Table<CAP>& t, int64_t c, floa
     // begin in it
     const int64_t n = e.n, at = (c - e.first) * chunk_of(THREADS) - shift_el(e.src, t.src_type[k]), end = at + chunk_of(THREADS);
     const int dt = t.dst_type[k], st = t.src_type[k];
-    const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(e.dst) % 16 / (dt == kF32 ? 4 : 2));
-    const auto pack_from = [&](int64_t i) { return i <= -shift ? static_cast<int64_t>(0) : (i + shift + 7) / 8 * 8; };
+    const int shift = shift_el(e.dst, dt), pack = dt == kF32 ? 4 : 8;
+    const auto pack_from = [&](int64_t i) { return i <= -shift ? static_cast<int64_t>(0) : (i + shift + pack - 1) / pack * pack; };
     const int64_t i0 = at <= 0 ? 0 : pack_from(at), i1 = end >= n ? n + shift : pack_from(end);
     const auto go = [&](auto* src) {
-        if (dt == kF32) scale_chunk<std::remove_const_t<std::remove_pointer_t<decltype(src)>>, float, THREADS>(src, static_cast<float*>(e.dst), n, shift, i0, i1, s);
-        else if (dt == kBF16) scale_chunk<std::remove_const_t<std::remove_pointer_t<decltype(src)>>, __nv_bfloat16, THREADS>(src, static_cast<__nv_bfloat16*>(e.dst), n, shift, i0, i1, s);
-        else scale_chunk<std::remove_const_t<std::remove_pointer_t<decltype(src)>>, __half, THREADS>(src, static_cast<__half*>(e.dst), n, shift, i0, i1, s);
+        if (dt == kF32) scale_chunk<std::remove_const_t<std::remove_pointer_t<decltype(src)>>, float, THREADS>(src, static_cast<float*>(e.dst), n, shift, i0, i1, s, tid);
+        else if (dt == kBF16) scale_chunk<std::remove_const_t<std::remove_pointer_t<decltype(src)>>, __nv_bfloat16, THREADS>(src, static_cast<__nv_bfloat16*>(e.dst), n, shift, i0, i1, s, tid);
+        else scale_chunk<std::remove_const_t<std::remove_pointer_t<decltype(src)>>, __half, THREADS>(src, static_cast<__half*>(e.dst), n, shift, i0, i1, s, tid);
     };
     if (st == kF32) go(static_cast<const float*>(e.src));
     else if (st == kBF16) go(static_cast<const __nv_bfloat16*>(e.src));
@@ -251,7 +259,7 @@ template <int CAP>
 __global__ void __launch_bounds__(kThreads) grad_squares_kernel(const __grid_constant__ Table<CAP> t, double* part) {
     __shared__ double red[kThreads / 32];
     double s = 0.0;
-    for (int64_t c = blockIdx.x; c < t.chunks; c += gridDim.x) s += chunk_squares<CAP, kThreads>(t, c);
+    for (int64_t c = blockIdx.x; c < t.chunks; c += gridDim.x) s += chunk_squares<CAP, kThreads>(t, c, threadIdx.x);
     grid_dep_launch();  // the kernel that needs the norm may be placed
     s = block_sum<kThreads>(s, red);
     if (threadIdx.x == 0) part[blockIdx.x] = s;
@@ -279,18 +287,21 @@ grad_scale_kernel(const __grid_constant__ Table<CAP> t, const double* part, int6
     const double n = joined_norm(part, parts, red);
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = static_cast<float>(n);
     const float s = scale_for(n, max_norm, eps);
-    for (int64_t c = t.chunks - 1 - blockIdx.x; c >= 0; c -= gridDim.x) chunk_scale<CAP, kThreads>(t, c, s);
+    for (int64_t c = t.chunks - 1 - blockIdx.x; c >= 0; c -= gridDim.x) chunk_scale<CAP, kThreads>(t, c, s, threadIdx.x);
 }
 
-// A few tensors of few elements: one cluster sums, joins through its shared memory and scales, in one launch.
+// A few tensors of few elements: one cluster sums, joins through its shared memory and scales, in one launch; a chunk
+// is a warp's.
 template <bool SCALE>
 __global__ void __cluster_dims__(kFewCluster, 1, 1) __launch_bounds__(kFewThreads)
 grad_few_kernel(const __grid_constant__ Table<kCapFew> t, double max_norm, double eps, float* norm) {
     __shared__ double red[kFewThreads / 32];
     __shared__ double mine;
     const uint32_t rank = cluster_ctarank();
+    const int lane = threadIdx.x & 31, first = static_cast<int>(rank) + kFewCluster * static_cast<int>(threadIdx.x >> 5);
+    constexpr int kStep = kFewCluster * kFewThreads / 32;
     double s = 0.0;
-    for (int64_t c = rank; c < t.chunks; c += kFewCluster) s += chunk_squares<kCapFew, kFewThreads>(t, c);
+    for (int64_t c = first; c < t.chunks; c += kStep) s += chunk_squares<kCapFew, 32>(t, c, lane);
     s = block_sum<kFewThreads>(s, red);
     if (threadIdx.x == 0) mine = s;
     cluster_sync();
@@ -300,13 +311,15 @@ grad_few_kernel(const __grid_constant__ Table<kCapFew> t, double max_norm, doubl
         asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(map_rank(smem_u32(&mine), r)) : "memory");
         n += v;
     }
-    cluster_sync();  // no CTA leaves while another may still read its share
+    asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
     n = sqrt(n);
     if (rank == 0 && threadIdx.x == 0) *norm = static_cast<float>(n);
     if constexpr (SCALE) {
         const float f = scale_for(n, max_norm, eps);
-        for (int64_t c = rank; c < t.chunks; c += kFewCluster) chunk_scale<kCapFew, kFewThreads>(t, c, f);
+        for (int64_t c = first; c < t.chunks; c += kStep) chunk_scale<kCapFew, 32>(t, c, f, lane);
+        __syncwarp();
     }
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // no CTA leaves while another may still read its share
 }
 
 // The next tensors of the list, as many as the table holds; their number.
@@ -324,8 +337,8 @@ int64_t fill(Table<CAP>& t, const GradTensor* g, int64_t tensors, int threads) {
     }
     return i;
 }
-int grid_of(int64_t chunks) {
-    const int64_t most = 8ll * device_sm_count() < kPartBlocks ? 8ll * device_sm_count() : kPartBlocks;
+int grid_of(int64_t chunks, int per_sm) {
+    const int64_t all = static_cast<int64_t>(per_sm) * device_sm_count(), most = all < kPartBlocks ? all : kPartBlocks;
     return static_cast<int>(chunks < 1 ? 1 : (chunks < most ? chunks : most));
 }
 
@@ -351,7 +364,7 @@ cudaError_t squares(Table<CAP>& t, const GradTensor* g, int64_t tensors, double*
         const int64_t took = fill(t, g, tensors, kThreads);
         g += took, tensors -= took;
         if (t.count == 0) continue;
-        const int grid = grid_of(t.chunks);
+        const int grid = grid_of(t.chunks, 4);
         grad_squares_kernel<CAP><<<grid, kThreads, 0, s>>>(t, part + *parts);
         if (const cudaError_t e = cudaGetLastError()) return e;
         *parts += grid;
@@ -370,7 +383,7 @@ cudaError_t clip(const GradTensor* g, int64_t tensors, double* part, double max_
         const int64_t took = whole ? tensors : fill(t, g, tensors, kThreads);
         g += took, tensors -= took;
         if (t.count == 0 && told) continue;
-        if (const cudaError_t e = launch_behind(grad_scale_kernel<CAP>, grid_of(t.chunks), s, t, part, parts, max_norm, eps,
+        if (const cudaError_t e = launch_behind(grad_scale_kernel<CAP>, grid_of(t.chunks, 4), s, t, part, parts, max_norm, eps,
                                                 told ? static_cast<float*>(nullptr) : norm))
             return e;
         told = true;
@@ -397,7 +410,7 @@ int64_t grad_norm_partials(int64_t tensors) { return ((tensors + kCap - 1) / kCa
 cudaError_t grad_norm_launch(const GradTensor* g, int64_t tensors, double* part, float* norm, cudaStream_t s) {
     if (few(g, tensors)) {
         static thread_local Table<kCapFew> t;
-        fill(t, g, tensors, kFewThreads);
+        fill(t, g, tensors, 32);
         grad_few_kernel<false><<<kFewCluster, kFewThreads, 0, s>>>(t, 0.0, 0.0, norm);
         return cudaGetLastError();
     }
@@ -418,7 +431,7 @@ cudaError_t grad_clip_launch(const GradTensor* g, int64_t tensors, double* part,
                              cudaStream_t s) {
     if (few(g, tensors)) {
         static thread_local Table<kCapFew> t;
-        fill(t, g, tensors, kFewThreads);
+        fill(t, g, tensors, 32);
         grad_few_kernel<true><<<kFewCluster, kFewThreads, 0, s>>>(t, max_norm, eps, norm);
         return cudaGetLastError();
     }

@@ -74,6 +74,10 @@ struct GemmDenseArgs {
     unsigned* err;
     unsigned long long wait_ns;
 };
+// the kernel for products of at most few_rows rows, K shared by `split` CTAs of a cluster
+inline int few_rows(int a_t, int b_t) { return a_t ? 0 : (b_t ? 16 : 32); }
+int gemm_few_split(int64_t M, int64_t N, int64_t K, int b_t, int64_t sms);
+cudaError_t gemm_few_launch(const GemmDenseArgs& a, int split, cudaStream_t s);
 // how a product is cut on `sms` SMs: rows of A to a tile of the narrow kernel (0: the kernel of CTA pairs),
 // CTAs that share K, and whether the narrow kernel takes an SM's memory for one CTA's ring
 struct DensePlan {

@@ -71,14 +71,6 @@ __device__ __forceinline__ void add_chunk(uint4 v, float2 (&acc)[32], int j) {
     }
 }
 
-// Element i of a matrix that may be written by this very call (an ordinary load).
-template <int CT>
-__device__ __forceinline__ float plain_load(const void* p, int64_t i) {
-    if constexpr (CT == kF32) return static_cast<const float*>(p)[i];
-    else if constexpr (CT == kBF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-    else return __half2float(static_cast<const __half*>(p)[i]);
-}
-
 // What the host finds out about the matrices of the epilogue: whether their rows allow TMA.
 struct Epi {
     int tma_c, tma_z, tma_r;
@@ -787,7 +779,17 @@ DensePlan gemm_dense_plan(int64_t M, int64_t N, int64_t K, int a_t, int64_t sms)
     return {nt, split, nt == 128 || up(N, 128) * up(M, nt) * split <= sms};
 }
 
+// The kernel for few rows (gemm_few.cu): CTAs of a cluster that share K, as many as the SMs hold two of, each with a
+// step for every warp at least.
+int gemm_few_split(int64_t M, int64_t N, int64_t K, int b_t, int64_t sms) {
+    const int64_t cols = b_t ? 64 : (M <= 8 ? 16 : 32), tiles = (N + cols - 1) / cols;
+    int split = 1;
+    while (split < 8 && tiles * split <= sms && K >= 512 * split) split *= 2;
+    return split;
+}
+
 int64_t gemm_dense_workspace(const void* A, int64_t lda, int a_t, const void* B, int64_t ldb, int b_t, int64_t M, int64_t N, int64_t K) {
+    if (M <= few_rows(a_t, b_t)) return 0;  // read as they lie
     const int64_t ra = a_t ? K : M, ca = a_t ? M : K, rb = b_t ? K : N, cb = b_t ? N : K;
     return (tma_operand(A, lda, ra) ? 0 : 2 * ra * up8(ca)) + (tma_operand(B, ldb, rb) ? 0 : 2 * rb * up8(cb));
 }
@@ -795,6 +797,7 @@ int64_t gemm_dense_workspace(const void* A, int64_t lda, int a_t, const void* B,
 cudaError_t gemm_dense_launch(const GemmDenseArgs& args, cudaStream_t stream) {
     GemmDenseArgs p = args;
     p.wait_ns = debug_wait_budget_ns();
+    if (p.M <= few_rows(p.a_t, p.b_t)) return gemm_few_launch(p, gemm_few_split(p.M, p.N, p.K, p.b_t, device_sm_count()), stream);
     uint16_t* room = static_cast<uint16_t*>(p.ws);
     const auto align = [&](const void*& base, int64_t& ld, int64_t rows, int64_t cols) {
         if (p.K == 0) return cudaSuccess;

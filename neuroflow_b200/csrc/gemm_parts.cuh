@@ -94,6 +94,19 @@ __device__ __forceinline__ void tmem_read(uint32_t taddr, uint32_t (&r)[32]) {
         : "memory");
 }
 
+// Element i of a matrix that may be written by this very call (an ordinary load).
+template <int CT>
+__device__ __forceinline__ float plain_load(const void* p, int64_t i) {
+    if constexpr (CT == kF32) return static_cast<const float*>(p)[i];
+    else if constexpr (CT == kBF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+    else return __half2float(static_cast<const __half*>(p)[i]);
+}
+
+__device__ __forceinline__ float ld_cluster(uint32_t cluster_addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
+    return v;
+}
 __device__ __forceinline__ float4 ld_cluster4(uint32_t cluster_addr) {
     float4 v;
     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"

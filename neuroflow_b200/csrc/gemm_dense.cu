@@ -225,7 +225,7 @@ struct PairEpilogue {
 };
 
 template <int CT>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+__global__ void __launch_bounds__(kPairThreads, 1)
 gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmC,
                  const __grid_constant__ CUtensorMap tmZ, const __grid_constant__ CUtensorMap tmR, const GemmDenseArgs p, const Epi e) {
     extern __shared__ uint8_t smem_raw[];
@@ -263,11 +263,14 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         fence_mbar_init();
     }
     if (warp == kPairEpi + 1) tmem_alloc_pair(sTmem, 512);
+    if (warp == kPairEpi && lane == 0) prefetch_tmap(&tmA), prefetch_tmap(&tmB);
     tc_fence_before();
     __syncthreads();
     cluster_sync();  // both CTAs' barriers are ready
     tc_fence_after();
     const uint32_t tmem_base = *sTmem;
+    grid_dep_launch();
+    grid_dep_wait();  // what the kernel before this one wrote may be read from here on
 
     // the register split stands inside the roles' branches: where they met again, the compiler would
     // have to assume the smaller count
@@ -449,8 +452,7 @@ cudaError_t launch_pair(const GemmDenseArgs& p, cudaStream_t stream) {
     if (err != cudaSuccess) return err;
     const int64_t tiles = static_cast<int64_t>((p.M + 255) / 256) * ((p.N + 255) / 256);
     const int pairs = device_sm_count() / 2;
-    kern<<<2 * static_cast<int>(tiles < pairs ? tiles : pairs), kPairThreads, kPairSmem, stream>>>(tmA, tmB, tmC, tmZ, tmR, p, e);
-    return cudaGetLastError();
+    return launch_early(kern, 2 * static_cast<int>(tiles < pairs ? tiles : pairs), kPairThreads, kPairSmem, 2, stream, tmA, tmB, tmC, tmZ, tmR, p, e);
 }
 
 // ---------------------------------------------------------------------------------------------------------
@@ -515,10 +517,13 @@ gemm_narrow_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
         fence_mbar_init();
     }
     if (warp == C::kEpi + 1) tmem_alloc(sTmem, C::kTmem);
+    if (warp == C::kEpi && lane == 0) prefetch_tmap(&tmW), prefetch_tmap(&tmX);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *sTmem;
+    grid_dep_launch();
+    grid_dep_wait();  // what the kernel before this one wrote may be read from here on
     float* part = reinterpret_cast<float*>(smem);  // (NT, 128) partial sums, after the last block
 
     if (warp == C::kEpi) {
@@ -709,18 +714,7 @@ cudaError_t launch_narrow(const GemmDenseArgs& p, int split, cudaStream_t stream
     const cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), C::kSmemBytes);
     if (e != cudaSuccess) return e;
     const int64_t tiles = static_cast<int64_t>((p.N + 127) / 128) * ((p.M + NT - 1) / NT);
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(tiles * split));
-    cfg.blockDim = dim3(C::kThreads);
-    cfg.dynamicSmemBytes = C::kSmemBytes;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = static_cast<unsigned>(split);
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kern, tmW, tmX, p, split);
+    return launch_early(kern, static_cast<int>(tiles * split), C::kThreads, C::kSmemBytes, split, stream, tmW, tmX, p, split);
 }
 
 template <int CT>

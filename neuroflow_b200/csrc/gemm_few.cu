@@ -103,6 +103,9 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_few_kernel(const GemmDenseAr
     const bool by_elements = which == 0 ? p.K % kStep != 0 : (!VEC && which < 3 && steps >= which);
     const int64_t arow = p.lda;
 
+    grid_dep_launch();
+    grid_dep_wait();  // what the kernel before this one wrote may be read from here on
+
     // rows beyond the matrices' ends read the last one: what comes of them is not stored
     if constexpr (KMAJOR) {
         float c[kMT][NT][4];
@@ -263,18 +266,7 @@ cudaError_t few_go(const GemmDenseArgs& p, int split, cudaStream_t s) {
     const cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), kSmem);
     if (e != cudaSuccess) return e;
     constexpr int kCols = Few<KMAJOR, VEC, NT>::kCols;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>((p.N + kCols - 1) / kCols * split));
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = kSmem;
-    cfg.stream = s;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = static_cast<unsigned>(split);
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = split > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kern, p, split);
+    return launch_early(kern, (p.N + kCols - 1) / kCols * split, kThreads, kSmem, split, s, p, split);
 }
 template <typename T, int CT, bool KMAJOR, bool VEC>
 cudaError_t few_width(const GemmDenseArgs& p, int split, cudaStream_t s) {

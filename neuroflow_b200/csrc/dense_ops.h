@@ -74,8 +74,17 @@ struct GemmDenseArgs {
     unsigned* err;
     unsigned long long wait_ns;
 };
-// the kernel for products of at most few_rows rows, K shared by `split` CTAs of a cluster
-inline int few_rows(int a_t, int b_t) { return a_t ? 0 : (b_t ? 16 : 32); }
+// whether TMA reads a matrix of 16-bit elements: `rows` contiguous runs, `ld` from one to the next
+inline bool tma_operand(const void* p, int64_t ld, int64_t rows) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (rows <= 1 || ld % 8 == 0);
+}
+// Whether a product is the kernel's for few rows (gemm_few.cu): up to 16 of them (16x4096x4096: 10.0 us, 10.6 with the
+// narrow kernel; 32x4096x4096: 13.7, 10.8), and up to 32 with rows of B that TMA cannot read, which would be copied
+// first (32x1023x1023: 6.9, 7.3).
+inline bool few_rows(const void* A, int64_t lda, int a_t, const void* B, int64_t ldb, int b_t, int64_t M, int64_t N, int64_t K) {
+    if (a_t || M > 32) return false;
+    return M <= 16 || (!b_t && !(tma_operand(A, lda, M) && tma_operand(B, ldb, N)));
+}
 int gemm_few_split(int64_t M, int64_t N, int64_t K, int b_t, int64_t sms);
 cudaError_t gemm_few_launch(const GemmDenseArgs& a, int split, cudaStream_t s);
 // how a product is cut on `sms` SMs: rows of A to a tile of the narrow kernel (0: the kernel of CTA pairs),

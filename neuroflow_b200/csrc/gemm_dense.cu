@@ -224,6 +224,23 @@ struct PairEpilogue {
     }
 };
 
+// One block of K of a CTA's 128 rows of A and of B into a stage; its bytes count on the barrier `bar`.
+__device__ __forceinline__ void load_stage(const GemmDenseArgs& p, const CUtensorMap& tmA, const CUtensorMap& tmB, uint8_t* st, uint32_t bar,
+                                           int m, int n, int k) {
+    if (p.a_t) {
+        tma_load_2d_pair(st, &tmA, bar, m, k);
+        tma_load_2d_pair(st + 8192, &tmA, bar, m + 64, k);
+    } else {
+        tma_load_2d_pair(st, &tmA, bar, k, m);
+    }
+    if (p.b_t) {
+        tma_load_2d_pair(st + 16384, &tmB, bar, n, k);
+        tma_load_2d_pair(st + 24576, &tmB, bar, n + 64, k);
+    } else {
+        tma_load_2d_pair(st + 16384, &tmB, bar, k, n);
+    }
+}
+
 template <int CT>
 __global__ void __launch_bounds__(kPairThreads, 1)
 gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmC,
@@ -296,18 +313,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
                         if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * kStageBytes);
                         const uint32_t bar = map_rank(smem_u32(&full[s]), 0);
                         uint8_t* st = smem + s * kStageBytes;
-                        if (p.a_t) {
-                            tma_load_2d_pair(st, &tmA, bar, m, kb * kBK);
-                            tma_load_2d_pair(st + 8192, &tmA, bar, m + 64, kb * kBK);
-                        } else {
-                            tma_load_2d_pair(st, &tmA, bar, kb * kBK, m);
-                        }
-                        if (p.b_t) {
-                            tma_load_2d_pair(st + 16384, &tmB, bar, n, kb * kBK);
-                            tma_load_2d_pair(st + 24576, &tmB, bar, n + 64, kb * kBK);
-                        } else {
-                            tma_load_2d_pair(st + 16384, &tmB, bar, kb * kBK, n);
-                        }
+                        load_stage(p, tmA, tmB, st, bar, m, n, kb * kBK);
                     }
                 }
                 // every load that was issued has landed and been read before the CTA exits
@@ -453,6 +459,268 @@ cudaError_t launch_pair(const GemmDenseArgs& p, cudaStream_t stream) {
     const int64_t tiles = static_cast<int64_t>((p.M + 255) / 256) * ((p.N + 255) / 256);
     const int pairs = device_sm_count() / 2;
     return launch_early(kern, 2 * static_cast<int>(tiles < pairs ? tiles : pairs), kPairThreads, kPairSmem, 2, stream, tmA, tmB, tmC, tmZ, tmR, p, e);
+}
+
+// ---------------------------------------------------------------------------------------------------------
+// Few tiles and a long K: a cluster of 2 S CTAs for one 256 x 256 tile, each of its S pairs summing a share of K.
+// A CTA puts its 128 x 256 partial sums where the operands were, and after a cluster barrier every CTA adds the
+// partials of its 256 / S columns in the order of the pairs, applies the epilogue and stores, each lane a
+// row.  Warps as in the kernel of pairs, without the idle ones.
+// ---------------------------------------------------------------------------------------------------------
+constexpr int kSplitThreads = 32 * (kPairEpi + 2);
+constexpr int kSplitSmem = kOffOut + 8 * (2 * kStages + 2 * 2) + 16 + 1024;
+static_assert(128 * 256 * 4 <= kOffOut, "the partial sums take the place of the operands");
+
+// W columns of a row, from column n on: acc += or = what lies in `mat`, or the other way round.
+template <int CT, int W>
+__device__ __forceinline__ void row_store(void* mat, int64_t at, bool vec, int n, int N, const float (&v)[W]) {
+    constexpr int kEl = CT == kF32 ? 4 : 2, kVec = 16 / kEl;
+    if (vec && n + W <= N) {
+#pragma unroll
+        for (int j = 0; j < W; j += kVec) {
+            uint4 u;
+            if constexpr (CT == kF32) {
+                u = make_uint4(__float_as_uint(v[j]), __float_as_uint(v[j + 1]), __float_as_uint(v[j + 2]), __float_as_uint(v[j + 3]));
+            } else {
+                uint32_t w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = pack_half<CT>(make_float2(v[j + 2 * i], v[j + 2 * i + 1]));
+                u = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            *reinterpret_cast<uint4*>(static_cast<uint8_t*>(mat) + (at + j) * kEl) = u;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < W; ++j)
+            if (n + j < N) store_any(mat, CT, at + j, v[j]);
+    }
+}
+template <int CT, int W>
+__device__ __forceinline__ void row_add(const void* mat, int64_t at, bool vec, int n, int N, float (&v)[W]) {
+    constexpr int kEl = CT == kF32 ? 4 : 2, kVec = 16 / kEl;
+    if (vec && n + W <= N) {
+#pragma unroll
+        for (int j = 0; j < W; j += kVec) {
+            const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(mat) + (at + j) * kEl);
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (CT == kF32) {
+                    v[j + i] += __uint_as_float(w[i]);
+                } else {
+                    const float2 f = unpack_half<CT>(w[i]);
+                    v[j + 2 * i] += f.x, v[j + 2 * i + 1] += f.y;
+                }
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < W; ++j)
+            if (n + j < N) v[j] += plain_load<CT>(mat, at + j);
+    }
+}
+
+template <int CT, int S>
+__global__ void __launch_bounds__(kSplitThreads, 1)
+gemm_split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const GemmDenseArgs p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + kOffOut);
+    uint64_t* empty = full + kStages;
+    uint64_t* accFull = empty + kStages;
+    uint64_t* accEmpty = accFull + 2;
+    uint32_t* sTmem = reinterpret_cast<uint32_t*>(accEmpty + 2);
+    volatile int* sAbort = reinterpret_cast<volatile int*>(sTmem + 1);
+
+    const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0);  // (known to be the same in all lanes)
+    const int lane = threadIdx.x & 31;
+    const uint32_t crank = cluster_ctarank(), rank = crank & 1, lead = crank & ~1u;
+    const int pair = static_cast<int>(crank >> 1), tn = (p.N + 255) / 256, tile = blockIdx.x / (2 * S);
+    const int mt = tile / tn, nt = tile % tn;
+    const int KB = (p.K + kBK - 1) / kBK;
+    const int kb0 = static_cast<int>(static_cast<int64_t>(KB) * pair / S), count = static_cast<int>(static_cast<int64_t>(KB) * (pair + 1) / S) - kb0;
+    const int piece = CT == kF32 ? kPiece : count;
+    const uint64_t budget = p.wait_ns ? p.wait_ns : kWaitNs;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&accFull[s], 1);
+            mbar_init(&accEmpty[s], 2 * kPairEpi);
+        }
+        *sAbort = 0;
+        fence_mbar_init();
+    }
+    if (warp == kPairEpi + 1) tmem_alloc_pair(sTmem, 512);
+    if (warp == kPairEpi && lane == 0) prefetch_tmap(&tmA), prefetch_tmap(&tmB);
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();  // the barriers of all CTAs are ready
+    tc_fence_after();
+    const uint32_t tmem_base = *sTmem;
+    float* part = reinterpret_cast<float*>(smem);  // four columns, 128 rows of them, and so on
+    grid_dep_launch();
+    grid_dep_wait();  // what the kernel before this one wrote may be read from here on
+
+    if (warp == kPairEpi) {
+        // ---------------- TMA producer
+        if (elect_one()) {
+            const int m = mt * 256 + rank * 128, n = nt * 256 + rank * 128;
+            int it = 0;
+            for (; it < count; ++it) {
+                const int s = it % kStages, k = (kb0 + it) * kBK;
+                if (!mbar_wait(&empty[s], ((it / kStages) & 1) ^ 1, sAbort, budget)) {
+                    *sAbort = 1;
+                    atomicOr(p.err, kErrWaitSlotFree);
+                    break;
+                }
+                if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * kStageBytes);
+                load_stage(p, tmA, tmB, smem + s * kStageBytes, map_rank(smem_u32(&full[s]), lead), m, n, k);
+            }
+            // every load that was issued has landed and been read before the partial sums take its place
+            for (int j = it > kStages ? it - kStages : 0; j < it; ++j)
+                if (!mbar_wait_drain(&empty[j % kStages], (j / kStages) & 1)) {
+                    *sAbort = 1;
+                    atomicOr(p.err, kErrWaitDrain);
+                    break;
+                }
+        }
+        __syncwarp();
+    } else if (warp == kPairEpi + 1) {
+        // ---------------- MMA issuer
+        if (rank == 0 && elect_one()) {
+            const uint32_t idesc = idesc_of(p.abtype, p.a_t, p.b_t, 256, 256);
+            const uint32_t astep = operand_step(p.a_t), bstep = operand_step(p.b_t);
+            int it = 0, acc = 0;
+            for (; it < count; ++it) {
+                const int s = it % kStages, in = it % piece;
+                const bool free = in > 0 || mbar_wait(&accEmpty[acc & 1], ((acc >> 1) & 1) ^ 1, sAbort, budget);
+                if (!free || !mbar_wait(&full[s], (it / kStages) & 1, sAbort, budget)) {
+                    *sAbort = 1;
+                    atomicOr(p.err, free ? kErrWaitTmaFull : kErrWaitAccFree);
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t ab = smem_u32(smem + s * kStageBytes);
+                const uint64_t ad = operand_desc(ab, p.a_t), bd = operand_desc(ab + 16384, p.b_t);
+#pragma unroll
+                for (int k = 0; k < kBK / 16; ++k)
+                    mma_f16_pair(tmem_base + (acc & 1) * 256, ad + k * astep, bd + k * bstep, idesc, in > 0 || k > 0 ? 1u : 0u);
+                mma_commit_pair(&empty[s], 3u << lead);
+                if (in == piece - 1 || it == count - 1) {
+                    mma_commit_pair(&accFull[acc & 1], 3u << lead);
+                    ++acc;
+                }
+            }
+            // the last commit completes before TMEM is released
+            if (it > 0 && !mbar_wait_drain(&empty[(it - 1) % kStages], ((it - 1) / kStages) & 1)) atomicOr(p.err, kErrWaitDrain);
+        }
+        __syncwarp();
+    } else {
+        // ---------------- the sums to registers, then to shared memory
+        const uint32_t accEmpty0 = map_rank(smem_u32(accEmpty), lead);
+        const uint32_t tmem0 = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16) + (warp >> 2) * 64;
+        float2 acc[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) acc[j] = make_float2(0.0f, 0.0f);
+        bool ok = true;
+        for (int i = 0, done = 0; done < count; ++i, done += piece) {
+            if (!mbar_wait(&accFull[i & 1], (i >> 1) & 1, sAbort, budget)) {
+                *sAbort = 1;
+                atomicOr(p.err, kErrWaitAccFull);
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                uint32_t r[32];
+                tmem_read(tmem0 + (i & 1) * 256 + c * 32, r);
+                if (c == 1) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(accEmpty0 + (i & 1) * 8);
+                }
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    acc[c * 16 + j] = add2_rn(acc[c * 16 + j], make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])));
+            }
+        }
+        // the last block's MMAs have read every stage of both CTAs
+        if (ok) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                *reinterpret_cast<float4*>(part + (((warp >> 2) * 16 + j) * 128 + (warp & 3) * 32 + lane) * 4) =
+                    make_float4(acc[2 * j].x, acc[2 * j].y, acc[2 * j + 1].x, acc[2 * j + 1].y);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();  // the partial sums of all pairs are there
+
+    // ---------------- join: 256 / S columns of this CTA's rows, 64 / S of them and 32 rows a warp
+    if (warp < kPairEpi && *sAbort == 0) {
+        constexpr int W = 64 / S;
+        const int r = (warp & 3) * 32 + lane, c0 = pair * (256 / S) + (warp >> 2) * W;
+        const int m = mt * 256 + rank * 128 + r, n = nt * 256 + c0;
+        float v[W];
+        float4 u[S][W / 4];
+#pragma unroll
+        for (int q = 0; q < S; ++q)
+#pragma unroll
+            for (int j = 0; j < W / 4; ++j) u[q][j] = ld_cluster4(map_rank(smem_u32(part + ((c0 / 4 + j) * 128 + r) * 4), 2 * q + rank));
+#pragma unroll
+        for (int j = 0; j < W / 4; ++j) {
+            float4 t = u[0][j];
+#pragma unroll
+            for (int q = 1; q < S; ++q) t.x += u[q][j].x, t.y += u[q][j].y, t.z += u[q][j].z, t.w += u[q][j].w;
+            v[4 * j] = t.x, v[4 * j + 1] = t.y, v[4 * j + 2] = t.z, v[4 * j + 3] = t.w;
+        }
+        if (p.bias) {
+            const float b = n + (lane % W) < p.N ? load_any(p.bias, p.btype, n + (lane % W)) : 0.0f;
+#pragma unroll
+            for (int j = 0; j < W; ++j) v[j] += __shfl_sync(0xFFFFFFFFu, b, j);
+        }
+        if (m < p.M && n < p.N) {
+            const auto vec_of = [&](const void* q, int64_t ld) { return reinterpret_cast<uintptr_t>(q) % 16 == 0 && (p.M == 1 || ld * (CT == kF32 ? 4 : 2) % 16 == 0); };
+            if (p.Z) row_store<CT, W>(p.Z, static_cast<int64_t>(m) * p.ldz + n, vec_of(p.Z, p.ldz), n, p.N, v);
+            if (p.act == 1) {
+#pragma unroll
+                for (int j = 0; j < W; j += 2) {
+                    const float2 g = gelu_sig2(make_float2(v[j], v[j + 1]));
+                    v[j] = g.x, v[j + 1] = g.y;
+                }
+            } else if (p.act == 2) {
+#pragma unroll
+                for (int j = 0; j < W; ++j) v[j] = relu_ref(v[j]);
+            }
+            if (p.res) row_add<CT, W>(p.res, static_cast<int64_t>(m) * p.ldres + n, vec_of(p.res, p.ldres), n, p.N, v);
+            row_store<CT, W>(p.C, static_cast<int64_t>(m) * p.ldc + n, vec_of(p.C, p.ldc), n, p.N, v);
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();  // no CTA leaves while another may still reach its shared memory
+    if (warp == kPairEpi + 1) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem_base, 512);
+    }
+}
+
+template <int CT, int S>
+cudaError_t launch_split(const GemmDenseArgs& p, cudaStream_t stream) {
+    CUtensorMap tmA{}, tmB{};
+    if (!operand_map(&tmA, p.abtype, p.A, p.a_t, p.M, p.K, p.lda, 128) || !operand_map(&tmB, p.abtype, p.B, p.b_t, p.N, p.K, p.ldb, 128))
+        return cudaErrorInvalidValue;
+    auto kern = gemm_split_kernel<CT, S>;
+    const cudaError_t err = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), kSplitSmem);
+    if (err != cudaSuccess) return err;
+    const int64_t tiles = static_cast<int64_t>((p.M + 255) / 256) * ((p.N + 255) / 256);
+    return launch_early(kern, tiles * 2 * S, kSplitThreads, kSplitSmem, 2 * S, stream, tmA, tmB, p);
 }
 
 // ---------------------------------------------------------------------------------------------------------
@@ -720,7 +988,7 @@ cudaError_t launch_narrow(const GemmDenseArgs& p, int split, cudaStream_t stream
 template <int CT>
 cudaError_t dispatch(const GemmDenseArgs& p, cudaStream_t stream) {
     const DensePlan c = gemm_dense_plan(p.M, p.N, p.K, p.a_t, device_sm_count());
-    if (c.columns == 0) return launch_pair<CT>(p, stream);
+    if (c.columns == 0) return c.split == 1 ? launch_pair<CT>(p, stream) : (c.split == 2 ? launch_split<CT, 2>(p, stream) : launch_split<CT, 4>(p, stream));
     if (c.columns == 16) return c.deep ? launch_narrow<16, CT, true>(p, c.split, stream) : launch_narrow<16, CT, false>(p, c.split, stream);
     if (c.columns == 32) return c.deep ? launch_narrow<32, CT, true>(p, c.split, stream) : launch_narrow<32, CT, false>(p, c.split, stream);
     if (c.columns == 64) return c.deep ? launch_narrow<64, CT, true>(p, c.split, stream) : launch_narrow<64, CT, false>(p, c.split, stream);
@@ -746,44 +1014,61 @@ __global__ void __launch_bounds__(256) align_rows_kernel(const uint16_t* src, in
     }
 }
 
-bool tma_operand(const void* p, int64_t ld, int64_t rows) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (rows <= 1 || ld % 8 == 0); }
 int64_t up8(int64_t v) { return (v + 7) / 8 * 8; }
 
 }  // namespace
 
-// Which kernel, and how it is cut (see the figures in the body).
+// Which kernel, and how it is cut: the cheapest by a model fitted to 590 measurements (us, graphs of launches over
+// operands that do not fit L2 together); KB blocks of 64 along K, rounds of the CTAs (pairs) that run at a time.
+//   narrow, NT columns, split s   base + rounds ceil(KB / s) c + further per further round + join (s > 1)
+//       NT = 16, 32, 64, 128: base 3.3, 4.6, 5.4, 6.0; c 0.22, 0.22, 0.24, 0.27, where two CTAs share an SM 0.30, 0.34,
+//       0.35; further 3.7, 4.2, 5.2, 7.4; join 1.0, 0.6, 0.7, 0.8
+//   pairs, split s                5.6 + rounds ceil(KB / s) 0.32 + 1.4 per further round + 0, 1.9, 3.5 (s = 1, 2, 4)
+// Clusters do not fill every processor cluster's SMs: 132 CTAs at a time in fours, 112 in eights, 70 and 56 pairs.  Over
+// the 61 measured shapes the choice takes 1.9 % longer than the best one.  E.g. 512x4096x4096: 19.5 with pairs and a
+// split of 2, 22.7 with 128/1, 25.7 with pairs alone; 355x3616x7136: 26.6, 36.0, 40.6; 64x1024x1024: 5.2 with 16/4,
+// 5.5 with 64/8, 8.5 with 64/1; 1024x1024x1024: 9.4 with 64/1, 9.8 with 128/2, 10.6 pairs.
 DensePlan gemm_dense_plan(int64_t M, int64_t N, int64_t K, int a_t, int64_t sms) {
     const auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
     const int64_t KB = up(K, kBK);
-    constexpr int kCost[4] = {20, 24, 32, 42}, kJoin[4] = {70, 100, 150, 250};  // hundredths of a microsecond
-    int nt = a_t ? 64 : 16, split = 1;
+    constexpr int kBase[4] = {327, 459, 537, 603}, kCost[4] = {22, 22, 24, 27}, kShared[4] = {30, 34, 35, 0};  // hundredths of a microsecond
+    constexpr int kFurther[4] = {366, 424, 520, 735}, kJoin[4] = {100, 60, 73, 75};
+    DensePlan plan{a_t ? 64 : 16, 1, false};
     int64_t best = -1;
-    for (int i = a_t ? 2 : 0; i < 4; ++i) {
+    for (int i = a_t ? 2 : 0; i < 4; ++i) {  // (boxes of an MN-major A are 64 wide)
         const int w = 16 << i;
-        if (w > nt && w / 2 >= M) break;
+        if (w > plan.columns && best >= 0 && w / 2 >= M) break;
         for (int s = 1; s <= 8 && (s == 1 || 2 * s <= KB); s *= 2) {
-            const int64_t ctas = up(N, 128) * up(M, w) * s;
-            const int64_t rounds = up(ctas, s >= 4 && sms > 1 ? sms * 7 / 8 : sms);
-            const int64_t cost = 430 + rounds * up(KB, s) * kCost[i] + (rounds - 1) * 250 + (s > 1 ? kJoin[i] : 0);
-            if (best < 0 || cost < best) best = cost, nt = w, split = s;
+            const int64_t ctas = up(N, 128) * up(M, w) * s, cap = s == 8 ? up(sms * 3, 4) : (s == 4 ? up(sms * 7, 8) : sms);
+            const bool shared = w <= 64 && ctas > sms;
+            const int64_t rounds = up(ctas, shared ? 2 * cap : cap);
+            const int64_t cost = kBase[i] + rounds * up(KB, s) * (shared ? kShared[i] : kCost[i]) + (rounds - 1) * kFurther[i] + (s > 1 ? kJoin[i] : 0);
+            if (best < 0 || cost < best) best = cost, plan = {w, s, w == 128 || ctas <= sms};
         }
     }
-    const int64_t rounds = sms > 1 ? up(up(M, 256) * up(N, 256), sms / 2) : 0;
-    if (sms > 1 && 650 + rounds * KB * 41 + (rounds - 1) * 220 < best) return {0, 1, false};
-    return {nt, split, nt == 128 || up(N, 128) * up(M, nt) * split <= sms};
+    const int64_t tiles = up(M, 256) * up(N, 256), pairs = sms / 2;
+    for (int s = 1; s <= 4 && pairs > 0 && (s == 1 || 2 * s <= KB); s *= 2) {
+        const int64_t at_a_time = s == 1 ? pairs : (s == 2 ? pairs * 19 / 20 : pairs * 3 / 4);
+        if (s > 1 && tiles * s > at_a_time) break;
+        const int64_t rounds = up(tiles * s, at_a_time), cost = 560 + rounds * up(KB, s) * 32 + (rounds - 1) * 143 + (s == 1 ? 0 : (s == 2 ? 187 : 351));
+        if (cost < best) best = cost, plan = {0, s, false};
+    }
+    return plan;
 }
 
-// The kernel for few rows (gemm_few.cu): CTAs of a cluster that share K, as many as the SMs hold two of, each with a
-// step for every warp at least.
+// The kernel for few rows (gemm_few.cu): CTAs of a cluster share K until each warp has no more steps than it keeps in
+// flight, as far as the SMs hold them, two each (1x1024x1024: 2.4 us with one CTA for K, 2.9 with 2, 3.1 with 4;
+// 16x4096x4096: 13.4, 10.0, 13.9).
 int gemm_few_split(int64_t M, int64_t N, int64_t K, int b_t, int64_t sms) {
     const int64_t cols = b_t ? 64 : (M <= 8 ? 16 : 32), tiles = (N + cols - 1) / cols;
+    const int64_t share = b_t ? 384 : (M <= 8 ? 2048 : (M <= 16 ? 768 : 256));
     int split = 1;
-    while (split < 8 && tiles * split <= sms && K >= 512 * split) split *= 2;
+    while (split < 8 && K > share * split && tiles * split * 2 <= 2 * sms) split *= 2;
     return split;
 }
 
 int64_t gemm_dense_workspace(const void* A, int64_t lda, int a_t, const void* B, int64_t ldb, int b_t, int64_t M, int64_t N, int64_t K) {
-    if (M <= few_rows(a_t, b_t)) return 0;  // read as they lie
+    if (few_rows(A, lda, a_t, B, ldb, b_t, M, N, K)) return 0;  // read as they lie
     const int64_t ra = a_t ? K : M, ca = a_t ? M : K, rb = b_t ? K : N, cb = b_t ? N : K;
     return (tma_operand(A, lda, ra) ? 0 : 2 * ra * up8(ca)) + (tma_operand(B, ldb, rb) ? 0 : 2 * rb * up8(cb));
 }
@@ -791,7 +1076,7 @@ int64_t gemm_dense_workspace(const void* A, int64_t lda, int a_t, const void* B,
 cudaError_t gemm_dense_launch(const GemmDenseArgs& args, cudaStream_t stream) {
     GemmDenseArgs p = args;
     p.wait_ns = debug_wait_budget_ns();
-    if (p.M <= few_rows(p.a_t, p.b_t)) return gemm_few_launch(p, gemm_few_split(p.M, p.N, p.K, p.b_t, device_sm_count()), stream);
+    if (few_rows(p.A, p.lda, p.a_t, p.B, p.ldb, p.b_t, p.M, p.N, p.K)) return gemm_few_launch(p, gemm_few_split(p.M, p.N, p.K, p.b_t, device_sm_count()), stream);
     uint16_t* room = static_cast<uint16_t*>(p.ws);
     const auto align = [&](const void*& base, int64_t& ld, int64_t rows, int64_t cols) {
         if (p.K == 0) return cudaSuccess;

@@ -1,4 +1,4 @@
-// gemm_few.cu -- the 16-bit product for at most 32 rows of A, contiguous ones: a few tokens against a weight, where reading B is
+// gemm_few.cu -- the 16-bit product for few rows of A (few_rows in dense_ops.h), contiguous ones: a few tokens against a weight, where reading B is
 // what has to be done.
 //
 //   Z = A B^T + bias,  C = act(Z) + R
@@ -272,13 +272,12 @@ template <typename T, int CT, bool KMAJOR, bool VEC>
 cudaError_t few_width(const GemmDenseArgs& p, int split, cudaStream_t s) {
     if constexpr (!KMAJOR) return few_go<T, CT, false, VEC, 2>(p, split, s);
     if (p.M <= 8) return few_go<T, CT, true, VEC, 1>(p, split, s);
-    if (p.M <= 16) return few_go<T, CT, true, VEC, 2>(p, split, s);
-    return few_go<T, CT, true, VEC, 4>(p, split, s);
+    if (VEC || p.M <= 16) return few_go<T, CT, true, VEC, 2>(p, split, s);
+    return few_go<T, CT, true, false, 4>(p, split, s);
 }
 template <typename T, int CT>
 cudaError_t few_form(const GemmDenseArgs& p, int split, cudaStream_t s) {
-    const auto on16 = [](const void* q, int64_t ld, int64_t rows) { return reinterpret_cast<uintptr_t>(q) % 16 == 0 && (rows <= 1 || ld % 8 == 0); };
-    const bool vec = on16(p.A, p.lda, p.M) && on16(p.B, p.ldb, p.b_t ? p.K : p.N);
+    const bool vec = tma_operand(p.A, p.lda, p.M) && tma_operand(p.B, p.ldb, p.b_t ? p.K : p.N);
     if (!p.b_t) return vec ? few_width<T, CT, true, true>(p, split, s) : few_width<T, CT, true, false>(p, split, s);
     return vec ? few_width<T, CT, false, true>(p, split, s) : few_width<T, CT, false, false>(p, split, s);
 }

@@ -409,12 +409,13 @@ __device__ __forceinline__ void mma_f8_pair(uint32_t d_tmem, uint64_t adesc, uin
         "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-// Arrive on the barrier at this offset in both CTAs once this thread's earlier MMAs are complete.
-__device__ __forceinline__ void mma_commit_pair(uint64_t* bar) {
+// Arrive on the barrier at this offset in both CTAs of the pair (`mask`: their ranks in the cluster) once this
+// thread's earlier MMAs are complete.
+__device__ __forceinline__ void mma_commit_pair(uint64_t* bar, uint32_t mask = 3) {
     asm volatile(
         "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
             smem_u32(bar)),
-        "h"(static_cast<unsigned short>(3))
+        "h"(static_cast<unsigned short>(mask))
         : "memory");
 }
 // kind::f8f6f4, E4M3 operands, fp32 D, both K-major, M = 256 over a CTA pair.

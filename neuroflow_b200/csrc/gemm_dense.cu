@@ -71,6 +71,10 @@ __device__ __forceinline__ void add_chunk(uint4 v, float2 (&acc)[32], int j) {
     }
 }
 
+// Rows of the boxes that each CTA of a pair loads (0: none, the matrix ends before them).
+struct PairRows {
+    int a[2], b[2];
+};
 // What the host finds out about the matrices of the epilogue: whether their rows allow TMA.
 struct Epi {
     int tma_c, tma_z, tma_r;
@@ -225,26 +229,25 @@ struct PairEpilogue {
 };
 
 // One block of K of a CTA's 128 rows of A and of B into a stage; its bytes count on the barrier `bar`.
+__device__ __forceinline__ void load_half(const CUtensorMap& tm, uint8_t* st, uint32_t bar, int t, int mn, int rows, int k) {
+    if (t) {
+        if (rows > 0) tma_load_2d_pair(st, &tm, bar, mn, k);
+        if (rows > 64) tma_load_2d_pair(st + 8192, &tm, bar, mn + 64, k);
+    } else if (rows > 0) {
+        tma_load_2d_pair(st, &tm, bar, k, mn);
+    }
+}
 __device__ __forceinline__ void load_stage(const GemmDenseArgs& p, const CUtensorMap& tmA, const CUtensorMap& tmB, uint8_t* st, uint32_t bar,
-                                           int m, int n, int k) {
-    if (p.a_t) {
-        tma_load_2d_pair(st, &tmA, bar, m, k);
-        tma_load_2d_pair(st + 8192, &tmA, bar, m + 64, k);
-    } else {
-        tma_load_2d_pair(st, &tmA, bar, k, m);
-    }
-    if (p.b_t) {
-        tma_load_2d_pair(st + 16384, &tmB, bar, n, k);
-        tma_load_2d_pair(st + 24576, &tmB, bar, n + 64, k);
-    } else {
-        tma_load_2d_pair(st + 16384, &tmB, bar, k, n);
-    }
+                                           int m, int n, int k, const PairRows& r, uint32_t rank) {
+    load_half(tmA, st, bar, p.a_t, m, r.a[rank], k);
+    load_half(tmB, st + 16384, bar, p.b_t, n, r.b[rank], k);
 }
 
 template <int CT>
 __global__ void __launch_bounds__(kPairThreads, 1)
 gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmC,
-                 const __grid_constant__ CUtensorMap tmZ, const __grid_constant__ CUtensorMap tmR, const GemmDenseArgs p, const Epi e) {
+                 const __grid_constant__ CUtensorMap tmZ, const __grid_constant__ CUtensorMap tmR, const GemmDenseArgs p, const Epi e,
+                 const PairRows rows) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + kOffBars);
@@ -310,10 +313,10 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
                             ok = false;
                             break;
                         }
-                        if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * kStageBytes);
+                        if (rank == 0) mbar_arrive_expect_tx(&full[s], (rows.a[0] + rows.a[1] + rows.b[0] + rows.b[1]) * kBK * 2);
                         const uint32_t bar = map_rank(smem_u32(&full[s]), 0);
                         uint8_t* st = smem + s * kStageBytes;
-                        load_stage(p, tmA, tmB, st, bar, m, n, kb * kBK);
+                        load_stage(p, tmA, tmB, st, bar, m, n, kb * kBK, rows, rank);
                     }
                 }
                 // every load that was issued has landed and been read before the CTA exits
@@ -430,10 +433,18 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
 CUtensorMapDataType map_type(int t) {
     return t == kF32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : t == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
 }
+// Rows of an operand's box, of which `most` would be a tile's: fewer where the whole matrix has fewer (rows that the
+// copy engine fills with zeros are as slow as ones that it reads).  Of MN-major operands whole boxes of 64 are left out.
+int box_rows(int t, int64_t mn, int most) { return static_cast<int>(mn >= most ? most : (t ? (mn + 63) / 64 * 64 : (mn + 7) / 8 * 8)); }
 // Boxes of an operand: `rows` x 64 of K, or 64 of K by 64 along MN.
 bool operand_map(CUtensorMap* tm, int type, const void* base, int t, int64_t mn, int64_t k, int64_t ld, int rows) {
     if (t) return encode_2d(tm, map_type(type), base, mn, k, ld * 2, 64, kBK, 128);
     return encode_2d(tm, map_type(type), base, k, mn, ld * 2, kBK, rows, 128);
+}
+PairRows pair_rows(const GemmDenseArgs& p) {
+    // (a matrix of at most 128 rows has none for the second CTA; of more, the boxes are whole)
+    const int a = box_rows(p.a_t, p.M, 128), b = box_rows(p.b_t, p.N, 128);
+    return {{a, p.M > 128 ? a : 0}, {b, p.N > 128 ? b : 0}};
 }
 bool tma_rows(const void* p, int64_t ld, int type) {
     return p && reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * type_bytes(type) % 16 == 0;
@@ -442,7 +453,8 @@ bool tma_rows(const void* p, int64_t ld, int type) {
 template <int CT>
 cudaError_t launch_pair(const GemmDenseArgs& p, cudaStream_t stream) {
     CUtensorMap tmA{}, tmB{}, tmC{}, tmZ{}, tmR{};
-    if (p.K > 0 && (!operand_map(&tmA, p.abtype, p.A, p.a_t, p.M, p.K, p.lda, 128) || !operand_map(&tmB, p.abtype, p.B, p.b_t, p.N, p.K, p.ldb, 128)))
+    const PairRows rows = pair_rows(p);
+    if (p.K > 0 && (!operand_map(&tmA, p.abtype, p.A, p.a_t, p.M, p.K, p.lda, rows.a[0]) || !operand_map(&tmB, p.abtype, p.B, p.b_t, p.N, p.K, p.ldb, rows.b[0])))
         return cudaErrorInvalidValue;
     constexpr int kEl = CT == kF32 ? 4 : 2;
     // (a matrix of one row has no row stride to speak of)
@@ -458,7 +470,7 @@ cudaError_t launch_pair(const GemmDenseArgs& p, cudaStream_t stream) {
     if (err != cudaSuccess) return err;
     const int64_t tiles = static_cast<int64_t>((p.M + 255) / 256) * ((p.N + 255) / 256);
     const int pairs = device_sm_count() / 2;
-    return launch_early(kern, 2 * static_cast<int>(tiles < pairs ? tiles : pairs), kPairThreads, kPairSmem, 2, stream, tmA, tmB, tmC, tmZ, tmR, p, e);
+    return launch_early(kern, 2 * static_cast<int>(tiles < pairs ? tiles : pairs), kPairThreads, kPairSmem, 2, stream, tmA, tmB, tmC, tmZ, tmR, p, e, rows);
 }
 
 // ---------------------------------------------------------------------------------------------------------
@@ -522,7 +534,7 @@ __device__ __forceinline__ void row_add(const void* mat, int64_t at, bool vec, i
 
 template <int CT, int S>
 __global__ void __launch_bounds__(kSplitThreads, 1)
-gemm_split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const GemmDenseArgs p) {
+gemm_split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const GemmDenseArgs p, const PairRows rows) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + kOffOut);
@@ -577,8 +589,8 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
                     atomicOr(p.err, kErrWaitSlotFree);
                     break;
                 }
-                if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * kStageBytes);
-                load_stage(p, tmA, tmB, smem + s * kStageBytes, map_rank(smem_u32(&full[s]), lead), m, n, k);
+                if (rank == 0) mbar_arrive_expect_tx(&full[s], (rows.a[0] + rows.a[1] + rows.b[0] + rows.b[1]) * kBK * 2);
+                load_stage(p, tmA, tmB, smem + s * kStageBytes, map_rank(smem_u32(&full[s]), lead), m, n, k, rows, rank);
             }
             // every load that was issued has landed and been read before the partial sums take its place
             for (int j = it > kStages ? it - kStages : 0; j < it; ++j)
@@ -714,13 +726,14 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
 template <int CT, int S>
 cudaError_t launch_split(const GemmDenseArgs& p, cudaStream_t stream) {
     CUtensorMap tmA{}, tmB{};
-    if (!operand_map(&tmA, p.abtype, p.A, p.a_t, p.M, p.K, p.lda, 128) || !operand_map(&tmB, p.abtype, p.B, p.b_t, p.N, p.K, p.ldb, 128))
+    const PairRows rows = pair_rows(p);
+    if (!operand_map(&tmA, p.abtype, p.A, p.a_t, p.M, p.K, p.lda, rows.a[0]) || !operand_map(&tmB, p.abtype, p.B, p.b_t, p.N, p.K, p.ldb, rows.b[0]))
         return cudaErrorInvalidValue;
     auto kern = gemm_split_kernel<CT, S>;
     const cudaError_t err = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), kSplitSmem);
     if (err != cudaSuccess) return err;
     const int64_t tiles = static_cast<int64_t>((p.M + 255) / 256) * ((p.N + 255) / 256);
-    return launch_early(kern, tiles * 2 * S, kSplitThreads, kSplitSmem, 2 * S, stream, tmA, tmB, p);
+    return launch_early(kern, tiles * 2 * S, kSplitThreads, kSplitSmem, 2 * S, stream, tmA, tmB, p, rows);
 }
 
 // ---------------------------------------------------------------------------------------------------------
@@ -750,7 +763,8 @@ struct NarrowCfg {
 
 template <int NT, int CT, bool DEEP>
 __global__ void __launch_bounds__(NarrowCfg<NT, DEEP>::kThreads, NarrowCfg<NT, DEEP>::kPerSm)
-gemm_narrow_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const GemmDenseArgs p, const int split) {
+gemm_narrow_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const GemmDenseArgs p, const int split,
+                   const int wrows, const int xrows) {
     using C = NarrowCfg<NT, DEEP>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -805,17 +819,18 @@ gemm_narrow_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
                     atomicOr(p.err, kErrWaitSlotFree);
                     break;
                 }
-                mbar_arrive_expect_tx(&full[s], C::kStageBytes);
+                mbar_arrive_expect_tx(&full[s], (wrows + xrows) * kBK * 2);
                 uint8_t* st = smem + s * C::kStageBytes;
                 if (p.b_t) {
                     tma_load_2d(st, &tmW, &full[s], n0, k);
-                    tma_load_2d(st + 8192, &tmW, &full[s], n0 + 64, k);
+                    if (wrows > 64) tma_load_2d(st + 8192, &tmW, &full[s], n0 + 64, k);
                 } else {
                     tma_load_2d(st, &tmW, &full[s], k, n0);
                 }
                 if (NT >= 64 && p.a_t) {
 #pragma unroll
-                    for (int j = 0; j < NT / 64; ++j) tma_load_2d(st + C::kWBytes + j * 8192, &tmX, &full[s], m0 + j * 64, k);
+                    for (int j = 0; j < NT / 64; ++j)
+                        if (j * 64 < xrows) tma_load_2d(st + C::kWBytes + j * 8192, &tmX, &full[s], m0 + j * 64, k);
                 } else {
                     tma_load_2d(st + C::kWBytes, &tmX, &full[s], k, m0);
                 }
@@ -976,13 +991,14 @@ template <int NT, int CT, bool DEEP>
 cudaError_t launch_narrow(const GemmDenseArgs& p, int split, cudaStream_t stream) {
     using C = NarrowCfg<NT, DEEP>;
     CUtensorMap tmW{}, tmX{};
-    if (p.K > 0 && (!operand_map(&tmW, p.abtype, p.B, p.b_t, p.N, p.K, p.ldb, 128) || !operand_map(&tmX, p.abtype, p.A, p.a_t, p.M, p.K, p.lda, NT)))
+    const int wrows = box_rows(p.b_t, p.N, 128), xrows = box_rows(p.a_t, p.M, NT);
+    if (p.K > 0 && (!operand_map(&tmW, p.abtype, p.B, p.b_t, p.N, p.K, p.ldb, wrows) || !operand_map(&tmX, p.abtype, p.A, p.a_t, p.M, p.K, p.lda, xrows)))
         return cudaErrorInvalidValue;
     auto kern = gemm_narrow_kernel<NT, CT, DEEP>;
     const cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), C::kSmemBytes);
     if (e != cudaSuccess) return e;
     const int64_t tiles = static_cast<int64_t>((p.N + 127) / 128) * ((p.M + NT - 1) / NT);
-    return launch_early(kern, static_cast<int>(tiles * split), C::kThreads, C::kSmemBytes, split, stream, tmW, tmX, p, split);
+    return launch_early(kern, static_cast<int>(tiles * split), C::kThreads, C::kSmemBytes, split, stream, tmW, tmX, p, split, wrows, xrows);
 }
 
 template <int CT>
@@ -999,18 +1015,37 @@ cudaError_t dispatch(const GemmDenseArgs& p, cudaStream_t stream) {
 // Operands that TMA cannot read (base or row stride no multiple of 16 bytes) are copied first, rows on 16-byte
 // boundaries.
 // ---------------------------------------------------------------------------------------------------------
-__global__ void __launch_bounds__(256) align_rows_kernel(const uint16_t* src, int64_t ld, int64_t rows, int64_t cols, uint16_t* dst, int64_t ldd) {
-    const int64_t packs = ldd / 8, all = rows * packs;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < all; i += static_cast<int64_t>(gridDim.x) * 256) {
-        const int64_t r = i / packs, c = i % packs * 8;
-        const uint16_t* s = src + r * ld + c;
-        uint32_t w[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t lo = c + 2 * j < cols ? s[2 * j] : 0, hi = c + 2 * j + 1 < cols ? s[2 * j + 1] : 0;
-            w[j] = lo | hi << 16;
+struct AlignJob {
+    const uint16_t* src;
+    int64_t ld, rows, cols;
+    uint16_t* dst;
+    int64_t ldd, packs;  // packs: of eight elements, rows ldd / 8
+};
+
+// Eight elements of the result a thread, from the two 16-byte words that hold them where both lie inside the matrix.
+__global__ void __launch_bounds__(256) align_rows_kernel(const AlignJob a, const AlignJob b) {
+    grid_dep_launch();
+    grid_dep_wait();
+    for (int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; e < a.packs + b.packs; e += static_cast<int64_t>(gridDim.x) * 256) {
+        const bool second = e >= a.packs;
+        const AlignJob& j = second ? b : a;
+        const int64_t i = second ? e - a.packs : e, per = j.ldd / 8;
+        int64_t r, c;
+        if (j.packs < (1ll << 31)) {
+            const uint32_t q = static_cast<uint32_t>(i) / static_cast<uint32_t>(per);
+            r = q, c = (static_cast<uint32_t>(i) - q * static_cast<uint32_t>(per)) * 8;
+        } else {
+            r = i / per, c = i % per * 8;
         }
-        *reinterpret_cast<uint4*>(dst + r * ldd + c) = make_uint4(w[0], w[1], w[2], w[3]);
+        const uint16_t* p = j.src + r * j.ld + c;
+        const int q = static_cast<int>(reinterpret_cast<uintptr_t>(p) >> 1) & 7;
+        uint32_t w[4];
+        if (c + 8 <= j.cols && p - q >= j.src && p - q + 16 <= j.src + (j.rows - 1) * j.ld + j.cols) {
+            load8<false>(p, w);
+        } else {
+            load_single<8>(p, 0, static_cast<int>(j.cols - c < 8 ? j.cols - c : 8), w);
+        }
+        *reinterpret_cast<uint4*>(j.dst + r * j.ldd + c) = make_uint4(w[0], w[1], w[2], w[3]);
     }
 }
 
@@ -1021,8 +1056,8 @@ int64_t up8(int64_t v) { return (v + 7) / 8 * 8; }
 // Which kernel, and how it is cut: the cheapest by a model fitted to 590 measurements (us, graphs of launches over
 // operands that do not fit L2 together); KB blocks of 64 along K, rounds of the CTAs (pairs) that run at a time.
 //   narrow, NT columns, split s   base + rounds ceil(KB / s) c + further per further round + join (s > 1)
-//       NT = 16, 32, 64, 128: base 3.3, 4.6, 5.4, 6.0; c 0.22, 0.22, 0.24, 0.27, where two CTAs share an SM 0.30, 0.34,
-//       0.35; further 3.7, 4.2, 5.2, 7.4; join 1.0, 0.6, 0.7, 0.8
+//       NT = 16, 32, 64, 128: base 3.3, 4.6, 5.4, 6.0; c 0.22, 0.22, 0.24, 0.27, where two CTAs share an SM 0.32, 0.36,
+//       0.40; further 3.7, 4.2, 5.2, 7.4; join 1.0, 0.6, 0.7, 0.8
 //   pairs, split s                5.6 + rounds ceil(KB / s) 0.32 + 1.4 per further round + 0, 1.9, 3.5 (s = 1, 2, 4)
 // Clusters do not fill every processor cluster's SMs: 132 CTAs at a time in fours, 112 in eights, 70 and 56 pairs.  Over
 // the 61 measured shapes the choice takes 1.9 % longer than the best one.  E.g. 512x4096x4096: 19.5 with pairs and a
@@ -1031,7 +1066,7 @@ int64_t up8(int64_t v) { return (v + 7) / 8 * 8; }
 DensePlan gemm_dense_plan(int64_t M, int64_t N, int64_t K, int a_t, int64_t sms) {
     const auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
     const int64_t KB = up(K, kBK);
-    constexpr int kBase[4] = {327, 459, 537, 603}, kCost[4] = {22, 22, 24, 27}, kShared[4] = {30, 34, 35, 0};  // hundredths of a microsecond
+    constexpr int kBase[4] = {327, 459, 537, 603}, kCost[4] = {22, 22, 24, 27}, kShared[4] = {32, 36, 40, 0};  // hundredths of a microsecond
     constexpr int kFurther[4] = {366, 424, 520, 735}, kJoin[4] = {100, 60, 73, 75};
     DensePlan plan{a_t ? 64 : 16, 1, false};
     int64_t best = -1;
@@ -1078,21 +1113,24 @@ cudaError_t gemm_dense_launch(const GemmDenseArgs& args, cudaStream_t stream) {
     p.wait_ns = debug_wait_budget_ns();
     if (few_rows(p.A, p.lda, p.a_t, p.B, p.ldb, p.b_t, p.M, p.N, p.K)) return gemm_few_launch(p, gemm_few_split(p.M, p.N, p.K, p.b_t, device_sm_count()), stream);
     uint16_t* room = static_cast<uint16_t*>(p.ws);
-    const auto align = [&](const void*& base, int64_t& ld, int64_t rows, int64_t cols) {
-        if (p.K == 0) return cudaSuccess;
+    AlignJob job[2]{};
+    const auto align = [&](const void*& base, int64_t& ld, int64_t rows, int64_t cols, AlignJob& j) {
+        if (p.K == 0) return;
         if (tma_operand(base, ld, rows)) {
             if (rows <= 1) ld = up8(cols);
-            return cudaSuccess;
+            return;
         }
-        const int64_t ldd = up8(cols), blocks = (rows * ldd / 8 + 255) / 256, most = 16ll * device_sm_count();
-        align_rows_kernel<<<static_cast<unsigned>(blocks < most ? blocks : most), 256, 0, stream>>>(static_cast<const uint16_t*>(base), ld, rows,
-                                                                                                   cols, room, ldd);
+        const int64_t ldd = up8(cols);
+        j = {static_cast<const uint16_t*>(base), ld, rows, cols, room, ldd, rows * ldd / 8};
         base = room, ld = ldd, room += rows * ldd;
-        return cudaGetLastError();
     };
-    cudaError_t e = align(p.A, p.lda, p.a_t ? p.K : p.M, p.a_t ? p.M : p.K);
-    if (e == cudaSuccess) e = align(p.B, p.ldb, p.b_t ? p.K : p.N, p.b_t ? p.N : p.K);
-    if (e != cudaSuccess) return e;
+    align(p.A, p.lda, p.a_t ? p.K : p.M, p.a_t ? p.M : p.K, job[0]);
+    align(p.B, p.ldb, p.b_t ? p.K : p.N, p.b_t ? p.N : p.K, job[1]);
+    if (const int64_t blocks = (job[0].packs + job[1].packs + 255) / 256; blocks > 0) {
+        const int64_t most = 16ll * device_sm_count();
+        const cudaError_t e = launch_early(align_rows_kernel, blocks < most ? blocks : most, 256, 0, 1, stream, job[0], job[1]);
+        if (e != cudaSuccess) return e;
+    }
     if (p.ctype == kF32) return dispatch<kF32>(p, stream);
     return p.ctype == kBF16 ? dispatch<kBF16>(p, stream) : dispatch<kF16>(p, stream);
 }

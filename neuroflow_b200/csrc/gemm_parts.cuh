@@ -117,6 +117,36 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t cluster_addr) {
 }
 
 
+// Elements [i, i + N) of a row; those from `end` on are zeros.
+template <int N>
+__device__ __forceinline__ void load_single(const uint16_t* p, int i, int end, uint32_t (&w)[N / 2]) {
+#pragma unroll
+    for (int j = 0; j < N / 2; ++j) {
+        const uint32_t lo = i + 2 * j < end ? __ldg(p + i + 2 * j) : 0, hi = i + 2 * j + 1 < end ? __ldg(p + i + 2 * j + 1) : 0;
+        w[j] = lo | hi << 16;
+    }
+}
+// Eight elements from p on, which lies on a 16-byte boundary (VEC) or anywhere: then the two words that hold them are
+// read, up to 14 bytes in front of p and behind its eight elements, and moved into place.
+template <bool VEC>
+__device__ __forceinline__ void load8(const uint16_t* p, uint32_t (&w)[4]) {
+    if constexpr (VEC) {
+        const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+        w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+    } else {
+        const int q = static_cast<int>(reinterpret_cast<uintptr_t>(p) >> 1) & 7;
+        const uint4* b = reinterpret_cast<const uint4*>(p - q);
+        const uint4 u = __ldg(b), v = __ldg(b + (q ? 1 : 0));
+        uint32_t m[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 6; ++i) m[i] = q & 4 ? m[i + 2] : m[i];
+#pragma unroll
+        for (int i = 0; i < 5; ++i) m[i] = q & 2 ? m[i + 1] : m[i];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = q & 1 ? __funnelshift_r(m[i], m[i + 1], 16) : m[i];
+    }
+}
+
 // A launch in clusters of `cluster` blocks that may begin while the kernel before it in the stream still runs: up to
 // grid_dep_wait() the kernel touches nothing that another one writes.
 template <typename... P, typename... A>

@@ -474,6 +474,13 @@ int nfx_gemm(const void* A, int64_t lda, int a_trans, const void* B, int64_t ldb
              void* C, int c_type, int64_t ldc, void* Z, int64_t ldz, void* workspace, int64_t workspace_bytes,
              void* stream);
 
+/* Test hook: how nfx_gemm cuts a product on a device of `sms` SMs (`aligned`: operands' bases and row strides are
+ * multiples of 16 bytes).  *columns: 0 for the kernels of CTA pairs (256 x 256 tiles), -1 for the one for few
+ * rows, else the rows of A to a tile of the narrow kernel (16, 32, 64, 128), with *split CTAs (pairs) sharing K and
+ * *deep set where one CTA takes an SM's shared memory.  Needs no GPU. */
+void nfx_debug_gemm_plan(int64_t M, int64_t N, int64_t K, int a_trans, int b_trans, int aligned, int sms, int* columns, int* split,
+                         int* deep);
+
 /* Gradient of the activation: dz = dy act'(z), dbias (cols,) = sums of its columns, formed in fp32 before dz
  * is rounded.  dy, z, dz (rows, cols) of `type`; z is not read with act = 0; dz or dbias may be NULL.
  * With dbias a 16-byte aligned workspace of nfx_act_backward_workspace bytes.  dz may be dy or z (the

@@ -12,6 +12,7 @@
 #include <cstdint>
 
 #include "dense_ops.h"
+#include "launch.cuh"
 #include "nfx_internal.h"
 #include "rms_parts.cuh"
 #include "sm100.cuh"
@@ -258,6 +259,7 @@ __device__ __forceinline__ float scale_for(double n, double max_norm, double eps
 template <int CAP>
 __global__ void __launch_bounds__(kThreads) grad_squares_kernel(const __grid_constant__ Table<CAP> t, double* part) {
     __shared__ double red[kThreads / 32];
+    grid_dep_wait();
     double s = 0.0;
     for (int64_t c = blockIdx.x; c < t.chunks; c += gridDim.x) s += chunk_squares<CAP, kThreads>(t, c, threadIdx.x);
     grid_dep_launch();  // the kernel that needs the norm may be placed
@@ -284,6 +286,7 @@ __global__ void __launch_bounds__(kThreads)
 grad_scale_kernel(const __grid_constant__ Table<CAP> t, const double* part, int64_t parts, double max_norm, double eps, float* norm) {
     __shared__ double red[kThreads / 32];
     grid_dep_wait();
+    grid_dep_launch();
     const double n = joined_norm(part, parts, red);
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = static_cast<float>(n);
     const float s = scale_for(n, max_norm, eps);
@@ -293,11 +296,13 @@ grad_scale_kernel(const __grid_constant__ Table<CAP> t, const double* part, int6
 // A few tensors of few elements: one cluster sums, joins through its shared memory and scales, in one launch; a chunk
 // is a warp's.
 template <bool SCALE>
-__global__ void __cluster_dims__(kFewCluster, 1, 1) __launch_bounds__(kFewThreads)
+__global__ void __launch_bounds__(kFewThreads)
 grad_few_kernel(const __grid_constant__ Table<kCapFew> t, double max_norm, double eps, float* norm) {
     __shared__ double red[kFewThreads / 32];
     __shared__ double mine;
     const uint32_t rank = cluster_ctarank();
+    grid_dep_launch();
+    grid_dep_wait();
     const int lane = threadIdx.x & 31, first = static_cast<int>(rank) + kFewCluster * static_cast<int>(threadIdx.x >> 5);
     constexpr int kStep = kFewCluster * kFewThreads / 32;
     double s = 0.0;
@@ -342,21 +347,6 @@ int grid_of(int64_t chunks, int per_sm) {
     return static_cast<int>(chunks < 1 ? 1 : (chunks < most ? chunks : most));
 }
 
-// Launches behind the kernel that leaves the shares, which it may overlap with until it waits for it.
-template <typename... P, typename... A>
-cudaError_t launch_behind(void (*kern)(P...), int grid, cudaStream_t s, A... args) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(grid));
-    cfg.blockDim = dim3(kThreads);
-    cfg.stream = s;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...);
-}
-
 template <int CAP>
 cudaError_t squares(Table<CAP>& t, const GradTensor* g, int64_t tensors, double* part, int64_t* parts, cudaStream_t s) {
     *parts = 0;
@@ -365,8 +355,7 @@ cudaError_t squares(Table<CAP>& t, const GradTensor* g, int64_t tensors, double*
         g += took, tensors -= took;
         if (t.count == 0) continue;
         const int grid = grid_of(t.chunks, 4);
-        grad_squares_kernel<CAP><<<grid, kThreads, 0, s>>>(t, part + *parts);
-        if (const cudaError_t e = cudaGetLastError()) return e;
+        if (const cudaError_t e = launch_early(grad_squares_kernel<CAP>, grid, kThreads, 0, 1, s, t, part + *parts)) return e;
         *parts += grid;
     }
     return cudaSuccess;
@@ -383,8 +372,8 @@ cudaError_t clip(const GradTensor* g, int64_t tensors, double* part, double max_
         const int64_t took = whole ? tensors : fill(t, g, tensors, kThreads);
         g += took, tensors -= took;
         if (t.count == 0 && told) continue;
-        if (const cudaError_t e = launch_behind(grad_scale_kernel<CAP>, grid_of(t.chunks, 4), s, t, part, parts, max_norm, eps,
-                                                told ? static_cast<float*>(nullptr) : norm))
+        if (const cudaError_t e = launch_early(grad_scale_kernel<CAP>, grid_of(t.chunks, 4), kThreads, 0, 1, s, t, part, parts, max_norm, eps,
+                                               told ? static_cast<float*>(nullptr) : norm))
             return e;
         told = true;
     }
@@ -411,8 +400,7 @@ cudaError_t grad_norm_launch(const GradTensor* g, int64_t tensors, double* part,
     if (few(g, tensors)) {
         static thread_local Table<kCapFew> t;
         fill(t, g, tensors, 32);
-        grad_few_kernel<false><<<kFewCluster, kFewThreads, 0, s>>>(t, 0.0, 0.0, norm);
-        return cudaGetLastError();
+        return launch_early(grad_few_kernel<false>, kFewCluster, kFewThreads, 0, kFewCluster, s, t, 0.0, 0.0, norm);
     }
     int64_t parts = 0;
     cudaError_t e;
@@ -424,7 +412,7 @@ cudaError_t grad_norm_launch(const GradTensor* g, int64_t tensors, double* part,
         e = squares(t, g, tensors, part, &parts, s);
     }
     if (e != cudaSuccess) return e;
-    return launch_behind(grad_norm_kernel, 1, s, part, parts, norm);
+    return launch_early(grad_norm_kernel, 1, kThreads, 0, 1, s, part, parts, norm);
 }
 
 cudaError_t grad_clip_launch(const GradTensor* g, int64_t tensors, double* part, double max_norm, double eps, float* norm,
@@ -432,8 +420,7 @@ cudaError_t grad_clip_launch(const GradTensor* g, int64_t tensors, double* part,
     if (few(g, tensors)) {
         static thread_local Table<kCapFew> t;
         fill(t, g, tensors, 32);
-        grad_few_kernel<true><<<kFewCluster, kFewThreads, 0, s>>>(t, max_norm, eps, norm);
-        return cudaGetLastError();
+        return launch_early(grad_few_kernel<true>, kFewCluster, kFewThreads, 0, kFewCluster, s, t, max_norm, eps, norm);
     }
     if (tensors <= kCapFew) return clip<kCapFew>(g, tensors, part, max_norm, eps, norm, s);
     return clip<kCap>(g, tensors, part, max_norm, eps, norm, s);

@@ -9,6 +9,7 @@
 #include <atomic>
 
 #include "dense_ops.h"
+#include "launch.cuh"
 #include "nfx_internal.h"
 #include "numerics.cuh"
 #include "rms_parts.cuh"
@@ -141,6 +142,8 @@ rms_row_kernel(RmsArgs a, Shift sh, bool gvec, bool wide) {
             if (a.res) er.load(res + sp.edge);
         }
     };
+    grid_dep_launch();
+    grid_dep_wait();  // what the kernel before this one wrote may be read from here on
     fetch(static_cast<int64_t>(blockIdx.x) * kRows + mine);
     float gam[kGammaShared ? 1 : VPT][VE];
     if constexpr (kGammaShared) {
@@ -308,8 +311,7 @@ cudaError_t rms_row_go(const RmsArgs& a, cudaStream_t s) {
     const Shift sh = shift_of(a.x, a.ldx, sizeof(T), VE);
     const bool gvec = aligned16(a.gamma) && (a.ptype == kF32 || VE == 8);
     const bool wide = FP8 && reinterpret_cast<uintptr_t>(a.q.codes) % 8 == 0 && (a.rows == 1 || a.q.ld % 8 == 0);
-    kern<<<static_cast<unsigned>(grid), threads, smem_of(threads, a.d), s>>>(a, sh, gvec, wide);
-    return cudaGetLastError();
+    return launch_early(kern, grid, threads, smem_of(threads, a.d), 1, s, a, sh, gvec, wide);
 }
 
 // 16 elements a thread up to 8,192 columns and 32 above.

@@ -7,6 +7,7 @@
 #include <atomic>
 
 #include "dense_ops.h"
+#include "launch.cuh"
 #include "nfx_internal.h"
 #include "numerics.cuh"
 #include "rms_parts.cuh"
@@ -114,6 +115,7 @@ __global__ void __launch_bounds__(MOST, grad_blocks(MOST)) rms_grad_row_kernel(R
             }
         }
     };
+    grid_dep_wait();  // what the kernel before this one wrote may be read from here on
     float gam[kShared ? 1 : VPT][VE], pg[kShared ? 1 : VPT][VE];
     float* const sums = room;
     float* const gams = room + E * threads;
@@ -276,8 +278,7 @@ cudaError_t rms_grad_go(RmsGradArgs& a, cudaStream_t s) {
     if (grid > a.parts) grid = a.parts;
     if (EDGE && VE > 1 && grid < want) grid = grid / VE * VE;  // steps of whole boundaries (a.parts is VE at least)
     a.parts = static_cast<int>(grid);
-    kern<<<static_cast<unsigned>(grid), threads, smem, s>>>(a, shift_of(a.dy, a.lddy, sizeof(T), VE), aligned16(a.gamma) && (a.ptype == kF32 || VE == 8));
-    return cudaGetLastError();
+    return launch_early(kern, grid, threads, smem, 1, s, a, shift_of(a.dy, a.lddy, sizeof(T), VE), aligned16(a.gamma) && (a.ptype == kF32 || VE == 8));
 }
 
 // Sixteen elements a thread where a row's three numbers have 16 bits, eight where some have 32.

@@ -19,12 +19,16 @@ constexpr float kFar = 100.0f;
 __device__ __forceinline__ float gelu_exponent(float z) { return -2.302208198f * fmaf(z, (0.044715f * z) * z, z); }
 
 // The slope of the activation.  GELU's is s + z s (1 - s) (2u)', with 1 - s as e s, e = e^(-2u) (the
-// difference would lose the digits that z (2u)' multiplies); beyond |z| = 30 it is 0 or 1.
+// difference would lose the digits that z (2u)' multiplies); beyond |z| = 30 it is 0 or 1.  The hardware's
+// exponential and reciprocal are a few 2^-22 off.
 __device__ __forceinline__ float slope_of(float z, int act) {
     if (act == 2) return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
     if (act != 1) return 1.0f;
-    const float c = fminf(fmaxf(z, -30.0f), 30.0f), t = gelu_exponent(c), e = exp2f(fminf(t, kFar)), s = __fdividef(1.0f, 1.0f + e);
-    const float v = fmaf(c * s * (e * s), 1.5957691216057308f * fmaf(0.134145f * c, c, 1.0f), s);
+    const float c = fminf(fmaxf(z, -30.0f), 30.0f), t = gelu_exponent(c);
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fminf(t, kFar)));
+    const float s = __fdividef(1.0f, 1.0f + e);
+    const float v = fmaf(c * s * (e * s), fmaf(1.5957691216057308f * 0.134145f * c, c, 1.5957691216057308f), s);
     return z != z ? z : (t > kFar ? 0.0f : v);
 }
 
@@ -34,7 +38,7 @@ __device__ __forceinline__ float slope_of(float z, int act) {
 constexpr int kWarps = 8;
 
 template <typename T, int VE, int VPT>
-__global__ void __launch_bounds__(32 * kWarps) act_grad_kernel(ActGradArgs a) {
+__global__ void __launch_bounds__(32 * kWarps, 4) act_grad_kernel(ActGradArgs a) {
     constexpr int E = VE * VPT, kU = 2;
     __shared__ float joined[kWarps][32 * E];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -120,7 +124,7 @@ cudaError_t act_grad_t(const ActGradArgs& a, cudaStream_t s) {
 
 // Shares of the rows: enough to fill the SMs, each of 32 rows at least.
 int act_grad_parts(int64_t rows, int64_t cols) {
-    const int64_t across = (cols + 255) / 256, all = (8ll * device_sm_count() + across - 1) / across, want = (rows + 31) / 32;
+    const int64_t across = (cols + 255) / 256, all = (4ll * device_sm_count() + across - 1) / across, want = (rows + 31) / 32;
     const int64_t n = want < all ? want : all;
     return static_cast<int>(n < 1 ? 1 : n);
 }

@@ -7,39 +7,44 @@
 
 #include "dense_ops.h"
 #include "nfx_internal.h"
+#include "numerics.cuh"
 #include "rms_parts.cuh"
 #include "sm100.cuh"
 
 namespace nfx {
 namespace {
 
-// GELU's tanh form is z s(2u), s the logistic function, u = sqrt(2 / pi) (z + 0.044715 z^3).  -2u, in units
-// of log 2; where it is above kFar the value and the slope are under 2^-90 and are taken as zero.
-constexpr float kFar = 100.0f;
-__device__ __forceinline__ float gelu_exponent(float z) { return -2.302208198f * fmaf(z, (0.044715f * z) * z, z); }
-
-// The slope of the activation.  GELU's is s + z s (1 - s) (2u)', with 1 - s as e s, e = e^(-2u) (the
-// difference would lose the digits that z (2u)' multiplies); beyond |z| = 30 it is 0 or 1.  The hardware's
-// exponential and reciprocal are a few 2^-22 off.
-__device__ __forceinline__ float slope_of(float z, int act) {
-    if (act == 2) return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
-    if (act != 1) return 1.0f;
-    const float c = fminf(fmaxf(z, -30.0f), 30.0f), t = gelu_exponent(c);
-    float e;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fminf(t, kFar)));
-    const float s = __fdividef(1.0f, 1.0f + e);
-    const float v = fmaf(c * s * (e * s), fmaf(1.5957691216057308f * 0.134145f * c, c, 1.5957691216057308f), s);
-    return z != z ? z : (t > kFar ? 0.0f : v);
+// The activation's slope at two numbers.  GELU's tanh form is z s(2u), s the logistic function, u = sqrt(2 / pi) (z +
+// 0.044715 z^3), and its slope s + z s (1 - s) (2u)', with 1 - s as e s, e = e^(-2u) (the difference would lose the
+// digits that z (2u)' multiplies).  Beyond |z| = 30, and where e is over 2^60, it is 0 or 1 to 2^-50.  Two numbers
+// share a reciprocal and the packed products; the hardware's exponential and reciprocal are a few 2^-22 off.
+constexpr float kFar = 60.0f;
+__device__ __forceinline__ float2 slope2(float2 z, int act) {
+    if (act == 2) return make_float2(z.x > 0.0f ? 1.0f : (z.x != z.x ? z.x : 0.0f), z.y > 0.0f ? 1.0f : (z.y != z.y ? z.y : 0.0f));
+    const auto both = [](float v) { return make_float2(v, v); };
+    const float2 c = make_float2(fminf(fmaxf(z.x, -30.0f), 30.0f), fminf(fmaxf(z.y, -30.0f), 30.0f)), c2 = mul2_rn(c, c);
+    // -2u in units of log 2, and (2u)'
+    const float2 t = mul2_rn(c, fma2_rn(c2, both(-2.302208198f * 0.044715f), both(-2.302208198f)));
+    const float2 d = fma2_rn(c2, both(1.5957691216057308f * 0.134145f), both(1.5957691216057308f));
+    float2 e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(fminf(t.x, kFar)));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(fminf(t.y, kFar)));
+    const float a = 1.0f + e.x, b = 1.0f + e.y, r = __fdividef(1.0f, a * b);
+    const float2 s = mul2_rn(both(r), make_float2(b, a));
+    const float2 v = fma2_rn(mul2_rn(mul2_rn(c, s), mul2_rn(e, s)), d, s);
+    return make_float2(z.x != z.x ? z.x : (t.x > kFar ? 0.0f : v.x), z.y != z.y ? z.y : (t.y > kFar ? 0.0f : v.y));
 }
 
 // A warp takes 32 VE columns (by 16-byte words; single ones, four a lane, where rows are not aligned to them) of every
-// eighth row of the block's share, two rows at a time; the columns' sums stay in registers and are joined over the
-// block's warps at the end.  4095x2048 bf16 with GELU and the bias gradient: see gemm_dense.cu's training step.
+// eighth row of the block's share, the next row on its way while one is worked on; the columns' sums stay in
+// registers and are joined over the block's warps at the end.  16384x4096 bf16 with GELU and the bias gradient:
+// 70 us, 5.8 TB/s (two rows at a time without a next one 88 us, with one, which spills, 104); 4095x2048: 12.8 us, of
+// which joining the shares takes 2.6.
 constexpr int kWarps = 8;
 
 template <typename T, int VE, int VPT>
 __global__ void __launch_bounds__(32 * kWarps, 4) act_grad_kernel(ActGradArgs a) {
-    constexpr int E = VE * VPT, kU = 2;
+    constexpr int E = VE * VPT;
     __shared__ float joined[kWarps][32 * E];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t c0 = static_cast<int64_t>(blockIdx.x) * 32 * E + lane * VE;
@@ -49,40 +54,49 @@ __global__ void __launch_bounds__(32 * kWarps, 4) act_grad_kernel(ActGradArgs a)
     float s[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) s[e] = 0.0f;
-    for (int64_t r = r0 + warp; r < r1; r += kWarps * kU) {
-        Elems<T, VE> y[kU][VPT], z[kU][VPT];
+    Elems<T, VE> ny[VPT], nz[VPT];
+    const auto fetch = [&](int64_t r) {
 #pragma unroll
-        for (int u = 0; u < kU; ++u)
-#pragma unroll
-            for (int j = 0; j < VPT; ++j) {
-                const int64_t c = c0 + j * 32 * VE, row = r + u * kWarps;
-                if (row < r1 && c < a.cols) {
-                    y[u][j].load(static_cast<const T*>(a.dy) + row * a.lddy + c);
-                    if (a.act) z[u][j].load(static_cast<const T*>(a.z) + row * a.ldz + c);
-                } else {
-                    y[u][j].zero(), z[u][j].zero();
-                }
+        for (int j = 0; j < VPT; ++j) {
+            const int64_t c = c0 + j * 32 * VE;
+            if (r < r1 && c < a.cols) {
+                ny[j].load(static_cast<const T*>(a.dy) + r * a.lddy + c);
+                if (a.act) nz[j].load(static_cast<const T*>(a.z) + r * a.ldz + c);
+            } else {
+                ny[j].zero(), nz[j].zero();
             }
+        }
+    };
+    fetch(r0 + warp);
+    for (int64_t r = r0 + warp; r < r1; r += kWarps) {
+        Elems<T, VE> y[VPT], z[VPT];
 #pragma unroll
-        for (int u = 0; u < kU; ++u)
+        for (int j = 0; j < VPT; ++j) y[j] = ny[j], z[j] = nz[j];
+        fetch(r + kWarps);
+        float v[E];
 #pragma unroll
-            for (int j = 0; j < VPT; ++j) {
-                const int64_t c = c0 + j * 32 * VE, row = r + u * kWarps;
-                if (row >= r1 || c >= a.cols) continue;
-                float v[VE];
-                y[u][j].get(v);
-                if (a.act) {
+        for (int e = 0; e < E; ++e) v[e] = y[e / VE].at(e % VE);
+        if (a.act) {
 #pragma unroll
-                    for (int i = 0; i < VE; ++i) v[i] *= slope_of(z[u][j].at(i), a.act);
-                }
-#pragma unroll
-                for (int i = 0; i < VE; ++i) s[j * VE + i] += v[i];
-                if (a.dz) {
-                    Elems<T, VE> o;
-                    o.set(v);
-                    o.store(static_cast<T*>(a.dz) + row * a.lddz + c);
-                }
+            for (int e = 0; e < E; e += 2) {
+                const float2 w = slope2(make_float2(z[e / VE].at(e % VE), z[(e + 1) / VE].at((e + 1) % VE)), a.act);
+                v[e] *= w.x, v[e + 1] *= w.y;
             }
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) s[e] += v[e];
+        if (!a.dz) continue;
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            const int64_t c = c0 + j * 32 * VE;
+            if (c >= a.cols) continue;
+            float o[VE];
+#pragma unroll
+            for (int i = 0; i < VE; ++i) o[i] = v[j * VE + i];
+            Elems<T, VE> w;
+            w.set(o);
+            w.store(static_cast<T*>(a.dz) + r * a.lddz + c);
+        }
     }
     if (!a.part) return;
 #pragma unroll

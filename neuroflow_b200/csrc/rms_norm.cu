@@ -290,7 +290,7 @@ template <typename T, typename H, int VE, int VPT, int MOST, bool ONE, bool FP8,
 cudaError_t rms_row_go(const RmsArgs& a, cudaStream_t s) {
     auto kern = rms_row_kernel<T, H, VE, VPT, MOST, ONE, FP8, EDGE>;
     // (a row's packs are d / VE at most, its edges go beside them)
-    const int threads = ONE || a.d < 32 * VPT * VE ? (ONE ? MOST : 32) : (a.d + 32 * VPT * VE - 1) / (32 * VPT * VE) * 32, rows = ONE ? MOST / 32 : 1;
+    const int packs = a.d / VE, threads = ONE ? MOST : (packs < 1 ? 1 : (packs + 32 * VPT - 1) / (32 * VPT)) * 32, rows = ONE ? MOST / 32 : 1;
     constexpr int kGammaBytes = !ONE && MOST >= 512 ? VPT * VE * 4 : 0;  // a thread
     const auto smem_of = [&](int n, int d) { return n * kGammaBytes + (FP8 && EDGE ? rows * ((d + kGroup - 1) / kGroup) * kFp8Row * 4 : 0); };
     // a block of `threads` holds rows of up to `room` columns: what they ask for decides how many blocks an SM has
@@ -318,7 +318,7 @@ cudaError_t rms_row_go(const RmsArgs& a, cudaStream_t s) {
 template <typename T, typename H, int VE, bool FP8, bool EDGE>
 cudaError_t rms_width(const RmsArgs& a, cudaStream_t s) {
     constexpr int k16 = 16 / VE;
-    const int d = a.d;
+    const int d = a.d / VE * VE;  // (edges need no packs)
     if constexpr (VE == 1) {  // (more loads to a row than a warp should queue)
         if (d <= 2048) return rms_row_go<T, H, 1, 8, 256, false, FP8, true>(a, s);
         if (d <= 8192) return rms_row_go<T, H, 1, 16, 512, false, FP8, true>(a, s);

@@ -261,7 +261,7 @@ cudaError_t rms_grad_go(RmsGradArgs& a, cudaStream_t s) {
     auto kern = rms_grad_row_kernel<T, H, VE, VPT, MOST, ONE, EDGE>;
     constexpr int E = VPT * VE;
     // (a row's packs are d / VE at most, its edges go beside them)
-    const int threads = ONE ? MOST : (a.d + 32 * E - 1) / (32 * E) * 32, rows = ONE ? MOST / 32 : 1;
+    const int packs = a.d / VE, threads = ONE ? MOST : (packs < 1 ? 1 : (packs + 32 * VPT - 1) / (32 * VPT)) * 32, rows = ONE ? MOST / 32 : 1;
     const int smem = MOST == 1024 ? 2 * E * threads * 4 : (ONE ? (E * 32 + VE) * 4 : 0);
     const cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), MOST == 1024 ? 2 * E * 1024 * 4 : smem);
     if (e != cudaSuccess) return e;
@@ -284,7 +284,7 @@ cudaError_t rms_grad_go(RmsGradArgs& a, cudaStream_t s) {
 // Sixteen elements a thread where a row's three numbers have 16 bits, eight where some have 32.
 template <typename T, typename H, int VE, bool EDGE>
 cudaError_t rms_grad_width(RmsGradArgs& a, cudaStream_t s) {
-    const int d = a.d;
+    const int d = a.d / VE * VE;  // (edges need no packs)
     if constexpr (sizeof(H) == 2 && VE > 1) {
         if (d <= 512) return rms_grad_go<T, H, VE, 16 / VE, 256, true, EDGE>(a, s);
         if (d <= 4096) return rms_grad_go<T, H, VE, 16 / VE, 256, false, EDGE>(a, s);

@@ -18,69 +18,90 @@
 namespace nfx {
 namespace {
 
-constexpr int kAnyThreads = 256;
+// Wider rows than the registers hold: a block of 512 threads takes a row in two sweeps, the second from L2.  An
+// element of a row is the same thread's in both.
+constexpr int kWideThreads = 512;
 
-// The sum of `a` over the block, the same bits in every thread.  `red` holds one number per warp.
-__device__ __forceinline__ float block_sum(float a, float* red) {
-    a = warp_sum(a);
-    __syncthreads();  // the previous sums have been read
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = a;
-    __syncthreads();
-    float t = 0.0f;
-    for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) t += red[w];
-    return t;
-}
-
-// Any width: one block per row, the row read twice (from L2 the second time).
-template <typename T, typename H>
-__global__ void __launch_bounds__(kAnyThreads) rms_any_kernel(RmsArgs a) {
-    __shared__ float red[kAnyThreads / 32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+template <typename T, typename H, int VE, bool FP8>
+__global__ void __launch_bounds__(kWideThreads, 2) rms_wide_kernel(RmsArgs a, Shift sh, bool wide) {
+    __shared__ float red[2][kWideThreads / 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tid = threadIdx.x;
+    grid_dep_launch();
+    grid_dep_wait();  // what the kernel before this one wrote may be read from here on
+    int buf = 0;
+    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x, buf ^= 1) {
+        const Split<VE> sp(a.d, static_cast<int>((sh.base + r * sh.step) % VE), tid);
         const T* x = static_cast<const T*>(a.x) + r * a.ldx;
         const H* res = a.res ? static_cast<const H*>(a.res) + r * a.ldres : nullptr;
         H* sum = a.sum ? static_cast<H*>(a.sum) + r * a.ldsum : nullptr;
-        // (the sum may be written over x or the residual: the second sweep reads it, by the same threads)
-        float s = 0.0f;
-        for (int i = threadIdx.x; i < a.d; i += kAnyThreads) {
-            float h = to_f32(x[i]);
-            if (res) {
-                const H hr = from_f32<H>(h + to_f32(res[i]));
-                h = to_f32(hr);
-                if (sum) sum[i] = hr;
+        // x + res as it is stored; plain loads where the first sweep has written
+        const auto pack = [&](int c, bool again, float (&v)[VE]) {
+            if (again && sum) {
+                Elems<H, VE> e;
+                e.load_plain(sum + c);
+                e.get(v);
+                return;
             }
-            s = fmaf(h, h, s);
-        }
-        const float rs = __frsqrt_rn(__fdiv_rn(block_sum(s, red), static_cast<float>(a.d)) + a.eps);
-        if (threadIdx.x == 0 && a.rstd) a.rstd[r] = rs;
-        auto out = [&](int i) {
-            float h;
-            if (sum) h = to_f32(sum[i]);
-            else if (res) h = to_f32(from_f32<H>(to_f32(x[i]) + to_f32(res[i])));
-            else h = to_f32(x[i]);
-            return (h * rs) * (a.gamma ? load_any(a.gamma, a.ptype, i) : 1.0f);
+            Elems<T, VE> e;
+            e.load(x + c);
+            e.get(v);
+            if (!res) return;
+            Elems<H, VE> f;
+            f.load(res + c);
+#pragma unroll
+            for (int i = 0; i < VE; ++i) v[i] += f.at(i);
+            f.set(v);
+            f.get(v);
+            if (!again && sum) f.store(sum + c);
         };
-        if (a.y) {
+        const auto single = [&](int c, bool again) {
+            if (again && sum) return to_f32(sum[c]);
+            const float v = to_f32(x[c]);
+            if (!res) return v;
+            const H h = from_f32<H>(v + to_f32(res[c]));
+            if (!again && sum) sum[c] = h;
+            return to_f32(h);
+        };
+        float q = 0.0f;
+        for (int k = tid; k < sp.packs; k += kWideThreads) {
+            float v[VE];
+            pack(sp.head + k * VE, false, v);
+#pragma unroll
+            for (int i = 0; i < VE; ++i) q = fmaf(v[i], v[i], q);
+        }
+        if (VE > 1 && sp.edge >= 0) {
+            const float v = single(sp.edge, false);
+            q = fmaf(v, v, q);
+        }
+        const float rs = __frsqrt_rn(__fdiv_rn(row_sum<false>(q, red[buf], kWideThreads / 32), static_cast<float>(a.d)) + a.eps);
+        if (tid == 0 && a.rstd) a.rstd[r] = rs;
+        const auto gamma = [&](int c) { return a.gamma ? load_any(a.gamma, a.ptype, c) : 1.0f; };
+        if constexpr (!FP8) {
             T* y = static_cast<T*>(a.y) + r * a.ldy;
-            for (int i = threadIdx.x; i < a.d; i += kAnyThreads) y[i] = from_f32<T>(out(i));
+            for (int k = tid; k < sp.packs; k += kWideThreads) {
+                const int c = sp.head + k * VE;
+                float v[VE];
+                pack(c, true, v);
+#pragma unroll
+                for (int i = 0; i < VE; ++i) v[i] = (v[i] * rs) * gamma(c + i);
+                Elems<T, VE> o;
+                o.set(v);
+                o.store(y + c);
+            }
+            if (VE > 1 && sp.edge >= 0) y[sp.edge] = from_f32<T>((single(sp.edge, true) * rs) * gamma(sp.edge));
         } else {
             if (sum) __syncthreads();  // the groups below are read by other threads than wrote the sum
             const int blocks = (a.d + kGroup - 1) / kGroup;
-            for (int b = warp; b < blocks; b += kAnyThreads / 32) {
-                float v[kGroup / 32], am = 0.0f;
+            for (int b = warp; b < blocks; b += kWideThreads / 32) {
+                const int c = b * kGroup + lane * 4;
+                float o[4], top = 0.0f;
 #pragma unroll
-                for (int j = 0; j < kGroup / 32; ++j) {
-                    const int i = b * kGroup + j * 32 + lane;
-                    v[j] = i < a.d ? out(i) : 0.0f;
-                    am = fmaxf(am, finite_abs(v[j]));
+                for (int i = 0; i < 4; ++i) {
+                    o[i] = c + i < a.d ? (single(c + i, true) * rs) * gamma(c + i) : 0.0f;
+                    top = fmaxf(top, finite_abs(o[i]));
                 }
-                const float sc = group_scale(warp_max(am)), inv = __frcp_rn(sc);
-#pragma unroll
-                for (int j = 0; j < kGroup / 32; ++j) {
-                    const int i = b * kGroup + j * 32 + lane;
-                    if (i < a.d) a.q.codes[r * a.q.ld + i] = static_cast<uint8_t>(e4m3_code(v[j], inv));
-                }
-                if (lane == 0) a.q.scales[r * a.q.srs + b * a.q.sbs] = sc;
+                const float sc = group_scale(warp_max(top));
+                if (c < a.d) store_codes4(a.q, r, b, c, a.d, lane, wide, o, sc, __frcp_rn(sc));
             }
         }
     }
@@ -268,18 +289,7 @@ rms_row_kernel(RmsArgs a, Shift sh, bool gvec, bool wide) {
                     top = fmaxf(top, finite_abs(o[i]));
                 }
                 const float sc = group_scale(warp_max(top)), inv = __frcp_rn(sc);
-                uint32_t odd = 0, w = scaled_codes<false>(o[0], o[1], o[2], o[3], inv, odd);
-                if (odd) w = scaled_codes<true>(o[0], o[1], o[2], o[3], inv, odd);
-                if (!live || c >= a.d) continue;
-                if (lane == 0) a.q.scales[r * a.q.srs + b * a.q.sbs] = sc;
-                uint8_t* dst = a.q.codes + r * a.q.ld + c;
-                if (wide && c + 4 <= a.d) {
-                    *reinterpret_cast<uint32_t*>(dst) = w;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (c + i < a.d) dst[i] = static_cast<uint8_t>(w >> (8 * i));
-                }
+                if (live && c < a.d) store_codes4(a.q, r, b, c, a.d, lane, wide, o, sc, inv);
             }
             if constexpr (ONE) __syncwarp();  // (with more warps the next row's sum has a barrier)
         }
@@ -334,21 +344,29 @@ cudaError_t rms_width(const RmsArgs& a, cudaStream_t s) {
     }
 }
 
+template <typename T, typename H, int VE, bool FP8>
+cudaError_t rms_wide_go(const RmsArgs& a, cudaStream_t s) {
+    const int64_t most = 2ll * device_sm_count();
+    const bool wide = FP8 && reinterpret_cast<uintptr_t>(a.q.codes) % 8 == 0 && (a.rows == 1 || a.q.ld % 8 == 0);
+    return launch_early(rms_wide_kernel<T, H, VE, FP8>, a.rows < most ? a.rows : most, kWideThreads, 0, 1, s, a, shift_of(a.x, a.ldx, sizeof(T), VE),
+                        wide);
+}
+
 template <typename T, typename H, bool FP8>
 cudaError_t rms_form(const RmsArgs& a, cudaStream_t s) {
     constexpr int VE = 16 / sizeof(T);
+    const Shift sx = shift_of(a.x, a.ldx, sizeof(T), VE);
+    const auto like = [&](const void* p, int64_t ld, int64_t el) { return !p || same_shift(sx, shift_of(p, ld, el, VE), a.rows); };
+    const bool alike = like(a.res, a.ldres, sizeof(H)) && like(a.sum, a.ldsum, sizeof(H)) && (FP8 || like(a.y, a.ldy, sizeof(T)));
+    if (alike && a.d > 16384) return rms_wide_go<T, H, VE, FP8>(a, s);
     if (a.d <= 16384) {
-        const Shift sx = shift_of(a.x, a.ldx, sizeof(T), VE);
-        const auto like = [&](const void* p, int64_t ld, int64_t el) { return !p || same_shift(sx, shift_of(p, ld, el, VE), a.rows); };
-        if (like(a.res, a.ldres, sizeof(H)) && like(a.sum, a.ldsum, sizeof(H)) && (FP8 || like(a.y, a.ldy, sizeof(T)))) {
+        if (alike) {
             if (sx.base == 0 && (a.rows == 1 || sx.step == 0) && a.d % VE == 0) return rms_width<T, H, VE, FP8, false>(a, s);
             return rms_width<T, H, VE, FP8, true>(a, s);
         }
     }
     if (a.d <= 16384) return rms_width<T, H, 1, FP8, true>(a, s);
-    const int64_t cap = 8ll * device_sm_count();
-    rms_any_kernel<T, H><<<static_cast<int>(a.rows < cap ? a.rows : cap), kAnyThreads, 0, s>>>(a);
-    return cudaGetLastError();
+    return rms_wide_go<T, H, 1, FP8>(a, s);
 }
 template <typename T, typename H>
 cudaError_t rms_t(const RmsArgs& a, cudaStream_t s) {

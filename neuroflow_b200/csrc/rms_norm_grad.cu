@@ -16,45 +16,79 @@
 namespace nfx {
 namespace {
 
-constexpr int kAnyThreads = 256;
+// Wider rows than the registers hold: a block of 512 threads takes every gridDim.x-th row in two sweeps, the second from
+// L2, and adds its rows' parameter gradients, in their order, to its own row of partial sums (each column always by one
+// thread: the launcher makes gridDim.x rows a whole number of boundaries).
+constexpr int kWideThreads = 512;
 
-// The sum of `a` over the block, the same bits in every thread.  `red` holds one number per warp.
-__device__ __forceinline__ float block_sum(float a, float* red) {
-    a = warp_sum(a);
-    __syncthreads();  // the previous sums have been read
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = a;
-    __syncthreads();
-    float t = 0.0f;
-    for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) t += red[w];
-    return t;
-}
-
-// Any width: a block takes every gridDim.x-th row and adds its rows' parameter gradients, in their order,
-// to its own row of partial sums (each column always by one thread).
-template <typename T, typename H>
-__global__ void __launch_bounds__(kAnyThreads) rms_grad_any_kernel(RmsGradArgs a) {
-    __shared__ float red[kAnyThreads / 32];
+template <typename T, typename H, int VE>
+__global__ void __launch_bounds__(kWideThreads, 2) rms_grad_wide_kernel(RmsGradArgs a, Shift sh) {
+    __shared__ float red[2][kWideThreads / 32];
+    const int tid = threadIdx.x;
     float* pg = a.part + static_cast<int64_t>(blockIdx.x) * a.d;
-    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    const Split<VE> sp(a.d, static_cast<int>((sh.base + static_cast<int64_t>(blockIdx.x) * sh.step) % VE), tid);
+    const auto gamma = [&](int c) { return a.gamma ? load_any(a.gamma, a.ptype, c) : 1.0f; };
+    grid_dep_wait();  // what the kernel before this one wrote may be read from here on
+    int buf = 0;
+    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x, buf ^= 1) {
         const T* dy = static_cast<const T*>(a.dy) + r * a.lddy;
         const H* h = static_cast<const H*>(a.h) + r * a.ldh;
-        const H* ds = a.dsum ? static_cast<const H*>(a.dsum) + r * a.lddsum : nullptr;
+        const H* ds = static_cast<const H*>(a.dsum) + r * a.lddsum;
         const float rs = a.rstd[r];
-        float s = 0.0f;
-        for (int i = threadIdx.x; i < a.d; i += kAnyThreads) {
-            const float xh = to_f32(h[i]) * rs, g = to_f32(dy[i]);
-            s = fmaf(a.gamma ? g * load_any(a.gamma, a.ptype, i) : g, xh, s);
-            if (a.part) pg[i] = fmaf(g, xh, r == blockIdx.x ? 0.0f : pg[i]);
+        const bool begin = r == blockIdx.x;
+        float t = 0.0f;
+        const auto term = [&](int c, float g, float hv) {
+            const float dyx = g * (hv * rs);
+            t = fmaf(gamma(c), dyx, t);
+            return dyx;
+        };
+        for (int k = tid; k < sp.packs; k += kWideThreads) {
+            const int c = sp.head + k * VE;
+            Elems<T, VE> y;
+            Elems<H, VE> x;
+            y.load(dy + c), x.load(h + c);
+#pragma unroll
+            for (int i = 0; i < VE; ++i) {
+                const float p = term(c + i, y.at(i), x.at(i));
+                if (a.part) pg[c + i] = p + (begin ? 0.0f : pg[c + i]);
+            }
         }
-        s = __fdiv_rn(block_sum(s, red), static_cast<float>(a.d));
-        for (int i = threadIdx.x; i < a.d; i += kAnyThreads) {
-            const float xh = to_f32(h[i]) * rs, g = to_f32(dy[i]);
-            float o = rs * fmaf(-xh, s, a.gamma ? g * load_any(a.gamma, a.ptype, i) : g);
-            if (ds) o += to_f32(ds[i]);
-            if (a.dx) static_cast<T*>(a.dx)[r * a.lddx + i] = from_f32<T>(o);
-            if (a.dres) static_cast<H*>(a.dres)[r * a.lddres + i] = from_f32<H>(o);
+        if (VE > 1 && sp.edge >= 0) {
+            const float p = term(sp.edge, to_f32(dy[sp.edge]), to_f32(h[sp.edge]));
+            if (a.part) pg[sp.edge] = p + (begin ? 0.0f : pg[sp.edge]);
+        }
+        const float m = __fdiv_rn(row_sum<false>(t, red[buf], kWideThreads / 32), static_cast<float>(a.d)) * rs;
+        T* dx = static_cast<T*>(a.dx) + r * a.lddx;
+        H* dr = static_cast<H*>(a.dres) + r * a.lddres;
+        for (int k = tid; k < sp.packs; k += kWideThreads) {
+            const int c = sp.head + k * VE;
+            Elems<T, VE> y;
+            Elems<H, VE> x, s;
+            y.load(dy + c), x.load(h + c);
+            if (a.dsum) s.load(ds + c);
+            float o[VE];
+#pragma unroll
+            for (int i = 0; i < VE; ++i) {
+                o[i] = rs * fmaf(-x.at(i), m, y.at(i) * gamma(c + i));
+                if (a.dsum) o[i] += s.at(i);
+            }
+            if (a.dx) y.set(o), y.store(dx + c);
+            if (a.dres) x.set(o), x.store(dr + c);
+        }
+        if (VE > 1 && sp.edge >= 0) {
+            const int c = sp.edge;
+            float o = rs * fmaf(-to_f32(h[c]), m, to_f32(dy[c]) * gamma(c));
+            if (a.dsum) o += to_f32(ds[c]);
+            if (a.dx) dx[c] = from_f32<T>(o);
+            if (a.dres) dr[c] = from_f32<H>(o);
         }
     }
+}
+
+template <typename T, typename H, int VE>
+cudaError_t rms_grad_wide_go(RmsGradArgs& a, cudaStream_t s) {
+    if (VE > 1 && a.parts < a.rows) a.parts = a.parts / VE * VE;  // steps of whole boundaries (a.parts is VE at least)
+    return launch_early(rms_grad_wide_kernel<T, H, VE>, a.parts, kWideThreads, 0, 1, s, a, shift_of(a.dy, a.lddy, sizeof(T), VE));
 }
 
 // ---------------------------------------------------------------------------------------------------------
@@ -307,11 +341,10 @@ cudaError_t rms_grad_t(RmsGradArgs& a, cudaStream_t s) {
     const auto like = [&](const void* p, int64_t ld, int64_t el) { return !p || same_shift(sy, shift_of(p, ld, el, VE), a.rows); };
     if (like(a.h, a.ldh, sizeof(H)) && like(a.dsum, a.lddsum, sizeof(H)) && like(a.dx, a.lddx, sizeof(T)) && like(a.dres, a.lddres, sizeof(H))) {
         if (a.d <= 16384 && sy.base == 0 && (a.rows == 1 || sy.step == 0) && a.d % VE == 0) return rms_grad_width<T, H, VE, false>(a, s);
-        if (a.d <= 16384) return rms_grad_width<T, H, VE, true>(a, s);
+        return a.d <= 16384 ? rms_grad_width<T, H, VE, true>(a, s) : rms_grad_wide_go<T, H, VE>(a, s);
     }
     if (a.d <= 16384) return rms_grad_width<T, H, 1, true>(a, s);
-    rms_grad_any_kernel<T, H><<<a.parts, kAnyThreads, 0, s>>>(a);
-    return cudaGetLastError();
+    return rms_grad_wide_go<T, H, 1>(a, s);
 }
 
 }  // namespace

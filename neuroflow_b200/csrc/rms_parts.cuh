@@ -36,6 +36,20 @@ struct Elems {
             w[0] = __ldg(reinterpret_cast<const uint16_t*>(p));
         }
     }
+    // by an ordinary load, of what this kernel has written
+    __device__ __forceinline__ void load_plain(const T* p) {
+        if constexpr (kWords >= 4) {
+#pragma unroll
+            for (int i = 0; i < kWords; i += 4) {
+                const uint4 u = reinterpret_cast<const uint4*>(p)[i / 4];
+                w[i] = u.x, w[i + 1] = u.y, w[i + 2] = u.z, w[i + 3] = u.w;
+            }
+        } else if constexpr (sizeof(T) == 4) {
+            w[0] = *reinterpret_cast<const uint32_t*>(p);
+        } else {
+            w[0] = *reinterpret_cast<const uint16_t*>(p);
+        }
+    }
     __device__ __forceinline__ float at(int i) const {
         if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
         else if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float((i & 1) ? (w[i / 2] & 0xFFFF0000u) : (w[i / 2] << 16));
@@ -97,6 +111,22 @@ struct Split {
         edge = sub < head ? sub : (sub >= VE && tail + sub - VE < d && sub < 2 * VE ? tail + sub - VE : -1);
     }
 };
+
+// Four columns' codes, and by the group's first lane its scale: group b of row r, columns c .. c + 3.
+__device__ __forceinline__ void store_codes4(const Fp8Out& q, int64_t r, int b, int c, int d, int lane, bool wide, const float (&o)[4], float sc,
+                                             float inv) {
+    uint32_t odd = 0, w = scaled_codes<false>(o[0], o[1], o[2], o[3], inv, odd);
+    if (odd) w = scaled_codes<true>(o[0], o[1], o[2], o[3], inv, odd);
+    if (lane == 0) q.scales[r * q.srs + b * q.sbs] = sc;
+    uint8_t* dst = q.codes + r * q.ld + c;
+    if (wide && c + 4 <= d) {
+        *reinterpret_cast<uint32_t*>(dst) = w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (c + i < d) dst[i] = static_cast<uint8_t>(w >> (8 * i));
+    }
+}
 
 // The distance in elements from the last VE-element boundary to a matrix' first element, and how a row moves it.
 struct Shift {

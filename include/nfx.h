@@ -463,9 +463,9 @@ int nfx_rms_norm_backward(const void* dy, int dy_type, int64_t lddy, const void*
  * A is (M, K): element (m, k) at m lda + k, or with a_trans at k lda + m; B is (N, K), the same.  bias
  * (N,) of bias_type or NULL; act 0 none, 1 GELU (tanh form), 2 ReLU; residual (M, N) of C's type or
  * NULL; C of ab_type or NFX_F32; Z (M, N), of C's type, is written where not NULL.  Any M, N, K >= 0 and
- * any alignment; operands whose base or row stride is not a multiple of 16 bytes are first
- * copied into the workspace (16-byte aligned, nfx_gemm_workspace bytes for these very arguments; 0 where no
- * copy is needed).  C may be the residual (the same pointer and stride).  Device error word as
+ * any alignment.  The workspace (16-byte aligned, nfx_gemm_workspace bytes for these very arguments on
+ * this device, often 0) takes copies of operands whose base or row stride is not a multiple of 16 bytes, and
+ * partial sums of a long K.  C may be the residual (the same pointer and stride).  Device error word as
  * nfx_fp8_gemm. */
 int64_t nfx_gemm_workspace(const void* A, int64_t lda, int a_trans, const void* B, int64_t ldb, int b_trans, int64_t M,
                            int64_t N, int64_t K);
@@ -477,9 +477,9 @@ int nfx_gemm(const void* A, int64_t lda, int a_trans, const void* B, int64_t ldb
 /* Test hook: how nfx_gemm cuts a product on a device of `sms` SMs (`aligned`: operands' bases and row strides are
  * multiples of 16 bytes).  *columns: 0 for the kernels of CTA pairs (256 x 256 tiles), -1 for the one for few
  * rows, else the rows of A to a tile of the narrow kernel (16, 32, 64, 128), with *split CTAs (pairs) sharing K and
- * *deep set where one CTA takes an SM's shared memory.  Needs no GPU. */
+ * *deep set where one CTA takes an SM's shared memory, and *runs of K joined by a second kernel.  Needs no GPU. */
 void nfx_debug_gemm_plan(int64_t M, int64_t N, int64_t K, int a_trans, int b_trans, int aligned, int sms, int* columns, int* split,
-                         int* deep);
+                         int* deep, int* runs);
 
 /* Gradient of the activation: dz = dy act'(z), dbias (cols,) = sums of its columns, formed in fp32 before dz
  * is rounded.  dy, z, dz (rows, cols) of `type`; z is not read with act = 0; dz or dbias may be NULL.

@@ -206,15 +206,15 @@ int nfx_gemm(const void* A, int64_t lda, int a_trans, const void* B, int64_t ldb
 }
 
 void nfx_debug_gemm_plan(int64_t M, int64_t N, int64_t K, int a_trans, int b_trans, int aligned, int sms, int* columns, int* split,
-                         int* deep) {
+                         int* deep, int* runs) {
     const void* at = reinterpret_cast<const void*>(static_cast<uintptr_t>(aligned ? 16 : 2));
     const int64_t n = sms < 1 ? 1 : sms;
     if (nfx::few_rows(at, 8, a_trans, at, 8, b_trans, M, N, K)) {
-        *columns = -1, *split = nfx::gemm_few_split(M, N, K, b_trans, n), *deep = 0;
+        *columns = -1, *split = nfx::gemm_few_split(M, N, K, b_trans, n), *deep = 0, *runs = 1;
         return;
     }
     const nfx::DensePlan c = nfx::gemm_dense_plan(M, N, K, a_trans, n);
-    *columns = c.columns, *split = c.split, *deep = c.deep;
+    *columns = c.columns, *split = c.split, *deep = c.deep, *runs = c.runs;
 }
 
 int64_t nfx_act_backward_workspace(int64_t rows, int64_t cols) {

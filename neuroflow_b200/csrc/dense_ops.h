@@ -70,7 +70,8 @@ struct GemmDenseArgs {
     int64_t ldc;
     void* Z;  // what the activation is taken of, of C's type, or nullptr
     int64_t ldz;
-    void* ws;  // room for operands that TMA cannot read, gemm_dense_workspace bytes
+    void* ws;  // room for operands that TMA cannot read and for sums of runs of K, gemm_dense_workspace bytes
+    int runs;  // set by the launcher
     unsigned* err;
     unsigned long long wait_ns;
 };
@@ -88,10 +89,12 @@ inline bool few_rows(const void* A, int64_t lda, int a_t, const void* B, int64_t
 int gemm_few_split(int64_t M, int64_t N, int64_t K, int b_t, int64_t sms);
 cudaError_t gemm_few_launch(const GemmDenseArgs& a, int split, cudaStream_t s);
 // how a product is cut on `sms` SMs: rows of A to a tile of the narrow kernel (0: the kernel of CTA pairs),
-// CTAs that share K, and whether the narrow kernel takes an SM's memory for one CTA's ring
+// CTAs that share K, whether the narrow kernel takes an SM's memory for one CTA's ring, and runs of K that are joined
+// by a second kernel
 struct DensePlan {
     int columns, split;
     bool deep;
+    int runs;
 };
 DensePlan gemm_dense_plan(int64_t M, int64_t N, int64_t K, int a_t, int64_t sms);
 int64_t gemm_dense_workspace(const void* A, int64_t lda, int a_t, const void* B, int64_t ldb, int b_t, int64_t M, int64_t N, int64_t K);

@@ -14,6 +14,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 
 #include "dense_ops.h"
@@ -777,12 +778,13 @@ gemm_narrow_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
 
     const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0);  // (known to be the same in all lanes)
     const int lane = threadIdx.x & 31;
-    const int rank = blockIdx.x % split, tile = blockIdx.x / split;  // a cluster is `split` blocks in a row
-    const int tx = (p.M + NT - 1) / NT;
+    const int rank = blockIdx.x % split, all = blockIdx.x / split;  // a cluster is `split` blocks in a row
+    const int tx = (p.M + NT - 1) / NT, tiles = tx * ((p.N + 127) / 128);
+    const int tile = all % tiles, run = all / tiles;  // run: of K, one of p.runs, each with a C of its own
     const int n0 = tile / tx * 128, m0 = tile % tx * NT;
-    const int KB = (p.K + kBK - 1) / kBK;
-    const int kb0 = static_cast<int>(static_cast<int64_t>(KB) * rank / split);
-    const int count = static_cast<int>(static_cast<int64_t>(KB) * (rank + 1) / split) - kb0;
+    const int KB = (p.K + kBK - 1) / kBK, parts = split * p.runs, part_i = run * split + rank;
+    const int kb0 = static_cast<int>(static_cast<int64_t>(KB) * part_i / parts);
+    const int count = static_cast<int>(static_cast<int64_t>(KB) * (part_i + 1) / parts) - kb0;
     const int piece = CT == kF32 ? kPiece : count;
     const uint64_t budget = p.wait_ns ? p.wait_ns : kWaitNs;
 
@@ -977,7 +979,7 @@ gemm_narrow_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
                     if (n + i < p.N) o[i] += plain_load<CT>(p.res, at + i);
             }
         }
-        store4(p.C, static_cast<int64_t>(m) * p.ldc + n, vec_c, n, o);
+        store4(p.C, (static_cast<int64_t>(run) * p.M + m) * p.ldc + n, vec_c, n, o);
     }
 
     if (warp == C::kEpi + 1) {
@@ -998,17 +1000,62 @@ cudaError_t launch_narrow(const GemmDenseArgs& p, int split, cudaStream_t stream
     const cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), C::kSmemBytes);
     if (e != cudaSuccess) return e;
     const int64_t tiles = static_cast<int64_t>((p.N + 127) / 128) * ((p.M + NT - 1) / NT);
-    return launch_early(kern, static_cast<int>(tiles * split), C::kThreads, C::kSmemBytes, split, stream, tmW, tmX, p, split, wrows, xrows);
+    return launch_early(kern, tiles * split * p.runs, C::kThreads, C::kSmemBytes, split, stream, tmW, tmX, p, split, wrows, xrows);
 }
 
 template <int CT>
-cudaError_t dispatch(const GemmDenseArgs& p, cudaStream_t stream) {
-    const DensePlan c = gemm_dense_plan(p.M, p.N, p.K, p.a_t, device_sm_count());
-    if (c.columns == 0) return c.split == 1 ? launch_pair<CT>(p, stream) : (c.split == 2 ? launch_split<CT, 2>(p, stream) : launch_split<CT, 4>(p, stream));
+cudaError_t narrow(const GemmDenseArgs& p, const DensePlan& c, cudaStream_t stream) {
     if (c.columns == 16) return c.deep ? launch_narrow<16, CT, true>(p, c.split, stream) : launch_narrow<16, CT, false>(p, c.split, stream);
     if (c.columns == 32) return c.deep ? launch_narrow<32, CT, true>(p, c.split, stream) : launch_narrow<32, CT, false>(p, c.split, stream);
     if (c.columns == 64) return c.deep ? launch_narrow<64, CT, true>(p, c.split, stream) : launch_narrow<64, CT, false>(p, c.split, stream);
     return launch_narrow<128, CT, true>(p, c.split, stream);
+}
+
+// Joins the sums of the runs of K, in their order, and applies the epilogue; four columns a thread.
+template <int CT>
+__global__ void __launch_bounds__(256) gemm_join_kernel(const GemmDenseArgs p, const float* sums, int runs, bool vec) {
+    grid_dep_launch();
+    grid_dep_wait();
+    const int64_t per = (p.N + 3) / 4, all = per * p.M, plane = static_cast<int64_t>(p.M) * p.N;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < all; i += static_cast<int64_t>(gridDim.x) * 256) {
+        const int64_t m = i / per;
+        const int n = static_cast<int>(i % per) * 4, cols = min(4, p.N - n);
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const float* at = sums + m * p.N + n;
+        if (vec) {
+            for (int r = 0; r < runs; ++r, at += plane) {
+                const float4 f = *reinterpret_cast<const float4*>(at);
+                v[0] += f.x, v[1] += f.y, v[2] += f.z, v[3] += f.w;
+            }
+        } else {
+            for (int r = 0; r < runs; ++r, at += plane)
+                for (int c = 0; c < cols; ++c) v[c] += at[c];
+        }
+        for (int c = 0; c < cols; ++c) {
+            float z = v[c];
+            if (p.bias) z += load_any(p.bias, p.btype, n + c);
+            if (p.Z) store_any(p.Z, CT, m * p.ldz + n + c, z);
+            if (p.act == 1) z = gelu_sig2(make_float2(z, 0.0f)).x;
+            else if (p.act == 2) z = relu_ref(z);
+            if (p.res) z += plain_load<CT>(p.res, m * p.ldres + n + c);
+            store_any(p.C, CT, m * p.ldc + n + c, z);
+        }
+    }
+}
+
+template <int CT>
+cudaError_t dispatch(const GemmDenseArgs& p, float* sums, cudaStream_t stream) {
+    const DensePlan c = gemm_dense_plan(p.M, p.N, p.K, p.a_t, device_sm_count());
+    if (c.runs > 1) {
+        GemmDenseArgs q = p;
+        q.runs = c.runs, q.C = sums, q.ctype = kF32, q.ldc = p.N, q.bias = nullptr, q.act = 0, q.res = nullptr, q.Z = nullptr;
+        const cudaError_t e = narrow<kF32>(q, c, stream);
+        if (e != cudaSuccess) return e;
+        const int64_t blocks = ((p.N + 3ll) / 4 * p.M + 255) / 256, most = 4ll * device_sm_count();
+        return launch_early(gemm_join_kernel<CT>, blocks < most ? blocks : most, 256, 0, 1, stream, p, static_cast<const float*>(sums), c.runs, p.N % 4 == 0);
+    }
+    if (c.columns == 0) return c.split == 1 ? launch_pair<CT>(p, stream) : (c.split == 2 ? launch_split<CT, 2>(p, stream) : launch_split<CT, 4>(p, stream));
+    return narrow<CT>(p, c, stream);
 }
 
 // ---------------------------------------------------------------------------------------------------------
@@ -1068,7 +1115,7 @@ DensePlan gemm_dense_plan(int64_t M, int64_t N, int64_t K, int a_t, int64_t sms)
     const int64_t KB = up(K, kBK);
     constexpr int kBase[4] = {327, 459, 537, 603}, kCost[4] = {22, 22, 24, 27}, kShared[4] = {32, 36, 40, 0};  // hundredths of a microsecond
     constexpr int kFurther[4] = {366, 424, 520, 735}, kJoin[4] = {100, 60, 73, 75};
-    DensePlan plan{a_t ? 64 : 16, 1, false};
+    DensePlan plan{a_t ? 64 : 16, 1, false, 1};
     int64_t best = -1;
     for (int i = a_t ? 2 : 0; i < 4; ++i) {  // (boxes of an MN-major A are 64 wide)
         const int w = 16 << i;
@@ -1078,15 +1125,25 @@ DensePlan gemm_dense_plan(int64_t M, int64_t N, int64_t K, int a_t, int64_t sms)
             const bool shared = w <= 64 && ctas > sms;
             const int64_t rounds = up(ctas, shared ? 2 * cap : cap);
             const int64_t cost = kBase[i] + rounds * up(KB, s) * (shared ? kShared[i] : kCost[i]) + (rounds - 1) * kFurther[i] + (s > 1 ? kJoin[i] : 0);
-            if (best < 0 || cost < best) best = cost, plan = {w, s, w == 128 || ctas <= sms};
+            if (best < 0 || cost < best) best = cost, plan = {w, s, w == 128 || ctas <= sms, 1};
         }
+    }
+    // a long K for a result of a few tiles: runs of K for as many clusters of eight as there are, joined by a second kernel
+    // (2.5 us, and some 4 MB of sums a microsecond); 64x64x65536: 34.6 us in one run
+    for (int i = a_t ? 2 : 0; i < 4; ++i) {
+        const int w = 16 << i;
+        if (w > 16 && w / 2 >= M && w > (a_t ? 64 : 16)) break;
+        const int64_t ctas = up(N, 128) * up(M, w) * 8, runs = std::min(up(sms * 3, 4) / ctas, KB / 32);
+        if (runs < 2) continue;
+        const int64_t cost = kBase[i] + up(KB, 8 * runs) * kCost[i] + kJoin[i] + 250 + M * N * runs / 10000;
+        if (cost < best) best = cost, plan = {w, 8, true, static_cast<int>(runs)};
     }
     const int64_t tiles = up(M, 256) * up(N, 256), pairs = sms / 2;
     for (int s = 1; s <= 4 && pairs > 0 && (s == 1 || 2 * s <= KB); s *= 2) {
         const int64_t at_a_time = s == 1 ? pairs : (s == 2 ? pairs * 19 / 20 : pairs * 3 / 4);
         if (s > 1 && tiles * s > at_a_time) break;
         const int64_t rounds = up(tiles * s, at_a_time), cost = 560 + rounds * up(KB, s) * 32 + (rounds - 1) * 143 + (s == 1 ? 0 : (s == 2 ? 187 : 351));
-        if (cost < best) best = cost, plan = {0, s, false};
+        if (cost < best) best = cost, plan = {0, s, false, 1};
     }
     return plan;
 }
@@ -1105,7 +1162,8 @@ int gemm_few_split(int64_t M, int64_t N, int64_t K, int b_t, int64_t sms) {
 int64_t gemm_dense_workspace(const void* A, int64_t lda, int a_t, const void* B, int64_t ldb, int b_t, int64_t M, int64_t N, int64_t K) {
     if (few_rows(A, lda, a_t, B, ldb, b_t, M, N, K)) return 0;  // read as they lie
     const int64_t ra = a_t ? K : M, ca = a_t ? M : K, rb = b_t ? K : N, cb = b_t ? N : K;
-    return (tma_operand(A, lda, ra) ? 0 : 2 * ra * up8(ca)) + (tma_operand(B, ldb, rb) ? 0 : 2 * rb * up8(cb));
+    const int64_t runs = gemm_dense_plan(M, N, K, a_t, device_sm_count()).runs;
+    return (tma_operand(A, lda, ra) ? 0 : 2 * ra * up8(ca)) + (tma_operand(B, ldb, rb) ? 0 : 2 * rb * up8(cb)) + (runs > 1 ? runs * M * N * 4 : 0);
 }
 
 cudaError_t gemm_dense_launch(const GemmDenseArgs& args, cudaStream_t stream) {
@@ -1131,8 +1189,10 @@ cudaError_t gemm_dense_launch(const GemmDenseArgs& args, cudaStream_t stream) {
         const cudaError_t e = launch_early(align_rows_kernel, blocks < most ? blocks : most, 256, 0, 1, stream, job[0], job[1]);
         if (e != cudaSuccess) return e;
     }
-    if (p.ctype == kF32) return dispatch<kF32>(p, stream);
-    return p.ctype == kBF16 ? dispatch<kBF16>(p, stream) : dispatch<kF16>(p, stream);
+    p.runs = 1;
+    float* sums = reinterpret_cast<float*>(room);  // (rows of eight elements: on a 16-byte boundary)
+    if (p.ctype == kF32) return dispatch<kF32>(p, sums, stream);
+    return p.ctype == kBF16 ? dispatch<kBF16>(p, sums, stream) : dispatch<kF16>(p, sums, stream);
 }
 
 }  // namespace nfx

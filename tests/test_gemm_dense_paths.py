@@ -27,6 +27,9 @@ PATHS = {
 MORE = [((16, 1, 0), (4355, 72, 130, 0)), ((64, 1, 0), (9000, 130, 40, 1)), ((0, 1, 0), (3100, 3000, 200, 0)), ((0, 2, 0), (512, 4096, 4097, 0)),
         ((0, 4, 0), (700, 700, 5000, 0)), ((128, 1, 1), (120, 16101, 1030, 0)), ((0, 1, 0), (12000, 72, 130, 0)), ((0, 1, 0), (19000, 130, 40, 1)),
         ((0, 1, 0), (120, 19101, 300, 0)), ((0, 1, 0), (12000, 72, 130, 1))]
+# a long K in several runs, joined by a second kernel: (columns, split, deep, runs)
+MORE += [((16, 8, 1, 2), (47, 214, 11781, 0)), ((16, 8, 1, 5), (17, 39, 10849, 0)), ((32, 8, 1, 3), (97, 10, 11997, 0)),
+         ((64, 8, 1, 3), (194, 9, 8196, 1)), ((64, 8, 1, 13), (64, 64, 65536, 1)), ((128, 8, 1, 3), (202, 129, 11506, 0))]
 # (split, B transposed, aligned): (M, N, K) of the kernel for few rows
 FEW = {
     (1, 0, 0): [(2, 38, 70), (15, 37, 75), (32, 39, 76)], (1, 0, 1): [(2, 37, 70), (11, 38, 80), (1, 300, 9), (16, 41, 31)],
@@ -44,10 +47,10 @@ def _plan(m, n, k, a_t=0, b_t=0, aligned=1, sms=B200_SMS):
     from neuroflow_b200 import _nfx
     f = _nfx.lib.nfx_debug_gemm_plan
     f.restype = None
-    f.argtypes = [C.c_int64] * 3 + [C.c_int] * 4 + [C.POINTER(C.c_int)] * 3
-    got = [C.c_int() for _ in range(3)]
+    f.argtypes = [C.c_int64] * 3 + [C.c_int] * 4 + [C.POINTER(C.c_int)] * 4
+    got = [C.c_int() for _ in range(4)]
     f(m, n, k, a_t, b_t, aligned, sms, *got)
-    return tuple(v.value for v in got)
+    return tuple(v.value for v in got[:3 if got[3].value == 1 else 4])  # (the runs of K where there are more)
 
 
 def test_each_shape_takes_its_path():
@@ -67,7 +70,7 @@ def test_the_rule_on_devices_of_few_sms():
     for sms in (1, 2, 3, 7):
         for mnk in ((1, 1, 1), (40, 1, 1), (33, 4096, 1 << 20), (2500, 2600, 200), (20000, 20000, 4096)):
             for t in (0, 1):
-                columns, split, _ = _plan(*mnk, t, sms=sms)
+                columns, split = _plan(*mnk, t, sms=sms)[:2]
                 assert columns in ((-1, 16, 32, 64, 128) if sms == 1 else (-1, 0, 16, 32, 64, 128)) and split in (1, 2, 4, 8)
 
 
@@ -78,7 +81,7 @@ def test_every_path_of_the_rule_has_a_shape():
     for _ in range(20000):
         a_t = r.randrange(2)
         path = _plan(size(20000), size(30000), size(30000), a_t)
-        assert path in PATHS or path[0] == -1, path
+        assert path in PATHS or path[0] == -1 or (len(path) == 4 and path[1:3] == (8, 1) and path[0] in (16, 32, 64, 128)), path
 
 
 def _held(rows, cols, fill, aligned=True, extra=0):
@@ -157,7 +160,8 @@ def test_paths_against_64_bits(path, out):
 
 
 @gpu
-@pytest.mark.parametrize("shape", [PATHS[(0, 1, 0)], PATHS[(0, 2, 0)], PATHS[(0, 4, 0)], PATHS[(16, 2, 1)], PATHS[(128, 2, 1)], (12, 300, 500, 0)])
+@pytest.mark.parametrize("shape", [PATHS[(0, 1, 0)], PATHS[(0, 2, 0)], PATHS[(0, 4, 0)], PATHS[(16, 2, 1)], PATHS[(128, 2, 1)], (12, 300, 500, 0),
+                                   (47, 214, 11781, 0)])
 @pytest.mark.parametrize("out", ["bfloat16", "float32"])
 def test_results_of_any_pitch(shape, out):
     """Rows of C and of the residual that allow copies of whole boxes, and ones that do not; rows that end inside 16
@@ -180,7 +184,8 @@ def test_results_of_any_pitch(shape, out):
 
 
 @gpu
-@pytest.mark.parametrize("shape", [PATHS[(0, 1, 0)], PATHS[(0, 2, 0)], PATHS[(16, 2, 1)], PATHS[(64, 8, 1)], (12, 300, 500, 0), (5, 70, 33, 0)])
+@pytest.mark.parametrize("shape", [PATHS[(0, 1, 0)], PATHS[(0, 2, 0)], PATHS[(16, 2, 1)], PATHS[(64, 8, 1)], (12, 300, 500, 0), (5, 70, 33, 0),
+                                   (47, 214, 11781, 0)])
 def test_bad_values_stay_in_their_row_and_column(shape):
     torch, ops = _torch()
     m, n, k, a_t = shape
@@ -205,7 +210,7 @@ def budget():
 
 
 @gpu
-@pytest.mark.parametrize("m,n,k", [(2048, 2304, 4096), (512, 4096, 4096), (64, 1024, 8192), (300, 700, 3000)])
+@pytest.mark.parametrize("m,n,k", [(2048, 2304, 4096), (512, 4096, 4096), (64, 1024, 8192), (300, 700, 3000), (64, 64, 20000)])
 def test_waits_that_run_out_are_reported(budget, m, n, k):
     """With a budget of 1 ns the pipeline waits give up, the kernel records it in the device error word, waits for its own
     copies and MMAs with the normal limit, releases its tensor memory and returns; with the normal budget the same

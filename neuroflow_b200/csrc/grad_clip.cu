@@ -36,7 +36,7 @@ struct Table {
     Entry e[CAP];
     uint8_t src_type[CAP], dst_type[CAP];
     int count;
-    int64_t chunks;
+    int64_t chunks, chunk;
 };
 // Kernel parameters hold 32,764 bytes; a launch copies all of them, so short lists have a table of their own.
 constexpr int kCap = 900, kCapFew = 48;
@@ -119,9 +119,10 @@ __device__ __forceinline__ double squares_of(const T* src, int64_t n, int shift,
     return sum;
 }
 
-// A chunk is this many elements, counted from a 16-byte boundary: finding its tensor takes a few hundred cycles.
-// A warp takes as much as it can have in flight.
-__host__ __device__ constexpr int64_t chunk_of(int threads) { return threads == kThreads ? 32768 : 1024; }
+// Elements of a chunk, counted from a 16-byte boundary.  Finding a chunk's tensor takes a few hundred cycles, so chunks
+// are large where there are enough of them (120M bf16 into bf16: 121 us with 16,384, 126 with 8,192, 123 with 32,768;
+// 605,000 fp32: 7.7, 5.7, 11.3).  A warp of the cluster's kernel takes as much as it can have in flight.
+constexpr int64_t kChunk = 16384, kChunkSmall = 8192, kChunkWarp = 1024;
 __host__ __device__ __forceinline__ int shift_el(const void* p, int type) {
     return static_cast<int>(reinterpret_cast<uintptr_t>(p) % 16 / (type == kF32 ? 4 : 2));
 }
@@ -131,7 +132,7 @@ __device__ __forceinline__ double chunk_squares(const Table<CAP>& t, int64_t c, 
     const int k = tensor_of(t, c);
     const int64_t n = t.e[k].n;
     const int type = t.src_type[k], shift = shift_el(t.e[k].src, type);
-    const int64_t i0 = (c - t.e[k].first) * chunk_of(THREADS), i1 = min(n + shift, i0 + chunk_of(THREADS));
+    const int64_t i0 = (c - t.e[k].first) * t.chunk, i1 = min(n + shift, i0 + t.chunk);
     if (type == kF32) return squares_of<float, THREADS>(static_cast<const float*>(t.e[k].src), n, shift, i0, i1, tid);
     if (type == kBF16) return squares_of<__nv_bfloat16, THREADS>(static_cast<const __nv_bfloat16*>(t.e[k].src), n, shift, i0, i1, tid);
     return squares_of<__half, THREADS>(static_cast<const __half*>(t.e[k].src), n, shift, i0, i1, tid);
@@ -235,7 +236,7 @@ __device__ __forceinline__ void chunk_scale(const Table<CAP>& t, int64_t c, floa
     if (s == 1.0f && e.dst == e.src) return;  // every element times one
     // chunks are counted by the source's boundaries, packs by the destination's: a chunk's packs are those that
     // begin in it
-    const int64_t n = e.n, at = (c - e.first) * chunk_of(THREADS) - shift_el(e.src, t.src_type[k]), end = at + chunk_of(THREADS);
+    const int64_t n = e.n, at = (c - e.first) * t.chunk - shift_el(e.src, t.src_type[k]), end = at + t.chunk;
     const int dt = t.dst_type[k], st = t.src_type[k];
     const int shift = shift_el(e.dst, dt), pack = dt == kF32 ? 4 : 8;
     const auto pack_from = [&](int64_t i) { return i <= -shift ? static_cast<int64_t>(0) : (i + shift + pack - 1) / pack * pack; };
@@ -329,18 +330,23 @@ grad_few_kernel(const __grid_constant__ Table<kCapFew> t, double max_norm, doubl
 
 // The next tensors of the list, as many as the table holds; their number.
 template <int CAP>
-int64_t fill(Table<CAP>& t, const GradTensor* g, int64_t tensors, int threads) {
-    t.count = 0, t.chunks = 0;
+int64_t fill(Table<CAP>& t, const GradTensor* g, int64_t tensors, int64_t chunk) {
+    t.count = 0, t.chunks = 0, t.chunk = chunk;
     int64_t i = 0;
     for (; i < tensors && t.count < CAP; ++i) {
         if (g[i].n == 0) continue;
         t.e[t.count] = {g[i].src, g[i].dst, g[i].n, t.chunks};
         t.src_type[t.count] = static_cast<uint8_t>(g[i].src_type);
         t.dst_type[t.count] = static_cast<uint8_t>(g[i].dst_type);
-        t.chunks += (g[i].n + shift_el(g[i].src, g[i].src_type) + chunk_of(threads) - 1) / chunk_of(threads);
+        t.chunks += (g[i].n + shift_el(g[i].src, g[i].src_type) + chunk - 1) / chunk;
         ++t.count;
     }
     return i;
+}
+int64_t chunk_for(const GradTensor* g, int64_t tensors) {
+    int64_t n = 0;
+    for (int64_t i = 0; i < tensors; ++i) n += g[i].n;
+    return n < 4 * kPartBlocks * kChunk ? kChunkSmall : kChunk;
 }
 int grid_of(int64_t chunks, int per_sm) {
     const int64_t all = static_cast<int64_t>(per_sm) * device_sm_count(), most = all < kPartBlocks ? all : kPartBlocks;
@@ -350,8 +356,9 @@ int grid_of(int64_t chunks, int per_sm) {
 template <int CAP>
 cudaError_t squares(Table<CAP>& t, const GradTensor* g, int64_t tensors, double* part, int64_t* parts, cudaStream_t s) {
     *parts = 0;
+    const int64_t chunk = chunk_for(g, tensors);
     while (tensors > 0) {
-        const int64_t took = fill(t, g, tensors, kThreads);
+        const int64_t took = fill(t, g, tensors, chunk);
         g += took, tensors -= took;
         if (t.count == 0) continue;
         const int grid = grid_of(t.chunks, 4);
@@ -366,10 +373,11 @@ cudaError_t clip(const GradTensor* g, int64_t tensors, double* part, double max_
     static thread_local Table<CAP> t;
     int64_t parts = 0;
     if (const cudaError_t e = squares(t, g, tensors, part, &parts, s)) return e;
+    const int64_t chunk = chunk_for(g, tensors);
     const bool whole = tensors <= CAP;  // the table holds all of them, as it was filled
     bool told = false;
     while (tensors > 0 || !told) {
-        const int64_t took = whole ? tensors : fill(t, g, tensors, kThreads);
+        const int64_t took = whole ? tensors : fill(t, g, tensors, chunk);
         g += took, tensors -= took;
         if (t.count == 0 && told) continue;
         if (const cudaError_t e = launch_early(grad_scale_kernel<CAP>, grid_of(t.chunks, 4), kThreads, 0, 1, s, t, part, parts, max_norm, eps,
@@ -380,8 +388,9 @@ cudaError_t clip(const GradTensor* g, int64_t tensors, double* part, double max_
     return cudaSuccess;
 }
 
-// The cluster reads some 1 TB/s, and a second launch costs 2 us on the device and more on the host.
-constexpr int64_t kFewBytes = 1 << 20;
+// One launch of a cluster: 5.4 us for 65,000 fp32 numbers, 9.4 for 245,000, where two launches over all SMs take 5.7
+// for 605,000 (and a launch more on the host).
+constexpr int64_t kFewBytes = 384 << 10;
 bool few(const GradTensor* g, int64_t tensors) {
     if (tensors > kCapFew) return false;
     int64_t bytes = 0;
@@ -399,7 +408,7 @@ int64_t grad_norm_partials(int64_t tensors) { return ((tensors + kCap - 1) / kCa
 cudaError_t grad_norm_launch(const GradTensor* g, int64_t tensors, double* part, float* norm, cudaStream_t s) {
     if (few(g, tensors)) {
         static thread_local Table<kCapFew> t;
-        fill(t, g, tensors, 32);
+        fill(t, g, tensors, kChunkWarp);
         return launch_early(grad_few_kernel<false>, kFewCluster, kFewThreads, 0, kFewCluster, s, t, 0.0, 0.0, norm);
     }
     int64_t parts = 0;
@@ -419,7 +428,7 @@ cudaError_t grad_clip_launch(const GradTensor* g, int64_t tensors, double* part,
                              cudaStream_t s) {
     if (few(g, tensors)) {
         static thread_local Table<kCapFew> t;
-        fill(t, g, tensors, 32);
+        fill(t, g, tensors, kChunkWarp);
         return launch_early(grad_few_kernel<true>, kFewCluster, kFewThreads, 0, kFewCluster, s, t, max_norm, eps, norm);
     }
     if (tensors <= kCapFew) return clip<kCapFew>(g, tensors, part, max_norm, eps, norm, s);

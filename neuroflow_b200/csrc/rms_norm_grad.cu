@@ -310,7 +310,7 @@ cudaError_t rms_grad_go(RmsGradArgs& a, cudaStream_t s) {
     const int64_t want = (a.rows + rows - 1) / rows;
     int64_t grid = want < most ? want : most;
     if (grid > a.parts) grid = a.parts;
-    if (EDGE && VE > 1 && grid < want) grid = grid / VE * VE;  // steps of whole boundaries (a.parts is VE at least)
+    if (EDGE && VE > 1 && grid < want) grid = grid >= VE ? grid / VE * VE : VE;  // steps of whole boundaries (a.parts is VE at least)
     a.parts = static_cast<int>(grid);
     return launch_early(kern, grid, threads, smem, 1, s, a, shift_of(a.dy, a.lddy, sizeof(T), VE), aligned16(a.gamma) && (a.ptype == kF32 || VE == 8));
 }

@@ -295,3 +295,102 @@ def test_backward_pass_in_a_graph():
         kept = [t.clone() for t in got]
         want = torch.autograd.grad(_block(ops, p, x, h), leaves, c)
         assert all(torch.equal(a, b) for a, b in zip(kept, want))
+
+
+def test_rows_and_tensors_beyond_32_bit_offsets():
+    """Rows 2^30 elements apart: the third one begins at element 2^31."""
+    torch, ops = _torch()
+    gen = torch.Generator(device="cuda").manual_seed(12)
+    pitch = 1 << 30
+    hold = torch.zeros(2 * pitch + 4096, device="cuda", dtype=torch.bfloat16)
+
+    def far(cols, at):
+        v = hold.as_strided((3, cols), (pitch, 1), at)
+        v.copy_(torch.randn(3, cols, generator=gen, device="cuda"))
+        return v
+
+    for cols in (300, 301):
+        x, h, y, s = far(cols, 0), far(cols, 512), hold.as_strided((3, cols), (pitch, 1), 1024), hold.as_strided((3, cols), (pitch, 1), 1536)
+        g = 1 + 0.1 * torch.randn(cols, generator=gen, device="cuda")
+        n, t, r = ops.rms_norm(x.contiguous(), g, residual=h.contiguous(), stats=True)
+        a, b, q = ops.rms_norm(x, g, residual=h, out=y, sum_out=s, stats=True)
+        assert torch.equal(a, n) and torch.equal(b, t) and torch.equal(q, r)
+        u, v = ops.rms_norm_backward(x, s, q, g, dsum=h), ops.rms_norm_backward(x.contiguous(), t, q, g, dsum=h.contiguous())
+        # dgamma: rows that lie otherwise go through another kernel, and each is within (rows + 4) 2^-24 sum |dy xh| of the
+        # exact sum; dx's terms are rounded alike
+        mag = (x.double() * s.double() * q.double()[:, None]).abs().sum(0)
+        assert torch.equal(u[0], v[0]) and ((u[2].double() - v[2].double()).abs() <= 2 * 7 * 2.0 ** -24 * mag).all()
+        c, e = ops.act_backward(x, h, 1, torch.float32), ops.act_backward(x.contiguous(), h.contiguous(), 1, torch.float32)
+        assert torch.equal(c[0], e[0]) and torch.equal(c[1], e[1])
+        # whole numbers, so that the sums are exact whichever kernel forms them
+        for v in (x, h):
+            v.copy_(torch.randint(-3, 4, (3, cols), generator=gen, device="cuda"))
+        w = torch.randint(-3, 4, (200, cols), generator=gen, device="cuda").bfloat16()
+        want = x.double() @ w.double().t()
+        out = hold.as_strided((3, 200), (pitch, 1), 2048)
+        assert torch.equal(ops.gemm(x, w, residual=h[:, :200], out=out), (want + h[:, :200].double()).bfloat16())
+        assert torch.equal(ops.gemm(w, x, out_dtype=torch.float32).double(), want.t())
+        assert torch.equal(ops.gemm(x.t(), x.t(), out_dtype=torch.float32).double(), x.double().t() @ x.double())
+
+
+def test_operands_of_one_row_or_column_with_strides():
+    torch, ops = _torch()
+    gen = torch.Generator(device="cuda").manual_seed(13)
+    ints = lambda *s: torch.randint(-3, 4, s, generator=gen, device="cuda").bfloat16()
+    for k in (1, 8, 70, 1000, 5000):
+        for pitch in (1, 3, 8, 64):
+            wide = ints(k, pitch)
+            one = wide[:, :1].t()  # (1, k), k elements `pitch` apart
+            other = ints(40, k)
+            for a, b in ((one, other), (other, one), (one, one), (one, ints(k, 40).t()), (ints(k, 300).t(), one)):
+                want = a.double() @ b.double().t()
+                assert torch.equal(ops.gemm(a, b, out_dtype=torch.float32).double(), want), (k, pitch)
+    a, b = ints(300, 1), ints(200, 1)
+    assert torch.equal(ops.gemm(a, b, out_dtype=torch.float32).double(), a.double() @ b.double().t())
+
+
+def test_linear_of_a_vector_and_of_no_tokens():
+    torch, ops = _torch()
+    p, rnd = _params(64, 96, 14, torch.bfloat16)
+    w, b = p["w1"].requires_grad_(), p["b1"].requires_grad_()
+    x = rnd(64).bfloat16().requires_grad_()
+    for act in (0, 1, 2):
+        y = ops.linear(x, w, b, act=act)
+        assert y.shape == (96,) and torch.equal(y, ops.linear(x[None], w, b, act=act)[0])
+        dx, dw, db = torch.autograd.grad(y, (x, w, b), torch.ones_like(y))
+        ex, ew, eb = torch.autograd.grad(ops.linear(x[None], w, b, act=act), (x, w, b), torch.ones_like(y)[None])
+        assert torch.equal(dx, ex) and torch.equal(dw, ew) and torch.equal(db, eb)
+        none = torch.zeros(0, 64, device="cuda", dtype=torch.bfloat16).requires_grad_()
+        y = ops.linear(none, w, b, act=act, residual=torch.zeros(0, 96, device="cuda", dtype=torch.bfloat16))
+        dx, dw, db = torch.autograd.grad(y, (none, w, b), torch.zeros_like(y))
+        assert dx.shape == (0, 64) and not dw.any() and not db.any()
+    y, h = ops.rms_norm_autograd(none, p["g1"].requires_grad_(), residual=none.detach())
+    dg, = torch.autograd.grad(y, p["g1"], torch.zeros_like(y))
+    assert y.shape == (0, 64) and not dg.any()
+
+
+def test_two_streams_at_once():
+    """The same calls on two streams, without order between them: nothing is shared but the error word."""
+    torch, ops = _torch()
+    p, rnd = _params(256, 1000, 15, torch.bfloat16)
+    xs = [rnd(700, 256).bfloat16() for _ in range(2)]
+    odd = [rnd(33, 4001).bfloat16() for _ in range(2)]
+    grads = [[rnd(n) for n in (5, 70001, 300)] for _ in range(2)]
+
+    def work(i):
+        n, h = ops.rms_norm(xs[i], p["g1"], residual=xs[1 - i])
+        y = ops.gemm(ops.gemm(n, p["w1"], bias=p["b1"], act=1), p["w2"], residual=h)
+        return [n, h, y, ops.gemm(odd[i], odd[1 - i]), ops.gemm(n.t(), y.t(), out_dtype=torch.float32),
+                ops.rms_norm_backward(y, h, torch.ones(700, device="cuda"), p["g1"])[2], ops.grad_norm(grads[i])]
+
+    want = [[t.clone() for t in work(i)] for i in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(3):
+        got = [None, None]
+        for _ in range(5):
+            for i, s in enumerate(streams):
+                with torch.cuda.stream(s):
+                    got[i] = work(i)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for i in range(2) for a, b in zip(got[i], want[i]))

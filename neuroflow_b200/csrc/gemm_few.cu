@@ -14,6 +14,10 @@
 //     8 g + j as its column g.
 // The eight warps of a block share K by turns, blocks of a cluster by parts; partial sums are joined in a fixed
 // order through shared memory.
+//
+// Measured (one B200, weights from HBM): 1x4096x4096 8.1 to 8.4 us, 4.1 TB/s (narrow kernel 10.0), 1x4096x16384 23 us, 5.8 TB/s,
+// 16x4096x4096 9.8 us, 1x1024x1024 2.4 us (4.3), 1x64x64 1.6 us.  Small ones are bound by the launch and one trip to
+// memory, large ones by HBM.
 #include <cuda_runtime.h>
 
 #include <cstdint>

@@ -3,7 +3,11 @@
 //   a = gamma dy,  xh = h r,  dh = r (a - xh mean(a xh)) + dsum
 //   dgamma = sum over rows of dy xh
 //
-// All sums are fp32.
+// All sums are fp32; dgamma's are joined in a fixed order by a second kernel (3 us).
+//
+// Bound by HBM.  Measured (one B200; GPU time, both kernels): 16384x4096 bf16 with dsum 85.6 us, 6.3 TB/s; bf16 with an fp32
+// stream 169 us, 6.3 TB/s; 65536x512 bf16 44 us, 6.1 TB/s; 8192x2048 bf16 27.4 us, 4.9 TB/s, 8192x2047 35.2 us; 5003x1031
+// fp16 17.8 us; 4096x16384 bf16 137 us, 3.9 TB/s; 2048x20000 256 us.
 #include <atomic>
 
 #include "dense_ops.h"

@@ -9,11 +9,11 @@
 // shares in a fixed order, so the result does not change from run to run.
 //
 // Bound by HBM: the elements are read twice, as more of them than L2 holds are seldom there the second time.  Measured (one
-// B200, GPU time): 120M bf16 in 300 tensors, norm alone 41 us, 5.8 TB/s; in place or into bf16 121 us, into unaligned fp32
-// 180 us (4.0 TB/s of the bytes that one reading would take); 120M fp32 244 us; 6 tensors of 65,000 fp32 in one launch
-// 5.4 us.
+// B200, GPU time): 120M bf16 in 300 tensors, norm alone 42 us, 5.7 TB/s; into bf16 132 us, into unaligned fp32 166 us
+// (4.4 TB/s of the bytes that one reading would take); 120M fp32 249 us; 6 tensors of 66,000 fp32 in one launch 5.0 us.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 
 #include "dense_ops.h"
@@ -29,6 +29,10 @@ constexpr int kThreads = 256;
 constexpr int kGroupPacks = 4;                                // packs of 16 bytes that a thread has in flight
 constexpr int kFewThreads = 512, kFewCluster = 8;
 constexpr int kPartBlocks = 4 * 148;                          // shares that one launch leaves, at most
+// Blocks of the scaling kernel at most: far more than are resident, so that one which ends early is followed by another
+// (134M bf16 into fp32: 200 us with 4 * 148, 193 with 8, 187 with 16, 184 with 32, 188 with one for each chunk).  The
+// kernel of the squares leaves a share for each block; there 4 are best (45 us; 53 with 16).
+constexpr int kScaleBlocks = 32 * 148;
 
 struct Entry {
     const void* src;
@@ -192,7 +196,6 @@ struct Moved {
 template <typename T, typename D, int THREADS, bool MOVED>
 __device__ __forceinline__ void scale_packs(const T* src, D* dst, int64_t n, int shift, int q, int64_t i0, int64_t i1, float s, int tid) {
     constexpr int N = 16 / sizeof(D), kSpan = Moved<T, N, MOVED>::kSpan, kStep = THREADS * N;
-    constexpr int kPacks = sizeof(T) == 2 && sizeof(D) == 4 ? 2 * kGroupPacks : kGroupPacks;
     const auto put = [&](int64_t c, Moved<T, N, MOVED>& m) {
         float v[N];
         m.get(q, v);
@@ -202,18 +205,18 @@ __device__ __forceinline__ void scale_packs(const T* src, D* dst, int64_t n, int
         o.set(v);
         __stcs(reinterpret_cast<uint4*>(dst + c), make_uint4(o.w[0], o.w[1], o.w[2], o.w[3]));
     };
-    for (int64_t b = i0 + tid * N; b < i1; b += kStep * kPacks) {
+    for (int64_t b = i0 + tid * N; b < i1; b += kStep * kGroupPacks) {
         const int64_t c = b - shift;
-        Moved<T, N, MOVED> m[kPacks];
+        Moved<T, N, MOVED> m[kGroupPacks];
         // the words of all packs lie inside the tensor
-        if (c - q >= 0 && b + (kPacks - 1) * kStep < i1 && c - q + (kPacks - 1) * kStep + kSpan <= n) {
+        if (c - q >= 0 && b + (kGroupPacks - 1) * kStep < i1 && c - q + (kGroupPacks - 1) * kStep + kSpan <= n) {
 #pragma unroll
-            for (int k = 0; k < kPacks; ++k) m[k].load(src + c + k * kStep - q);
+            for (int k = 0; k < kGroupPacks; ++k) m[k].load(src + c + k * kStep - q);
 #pragma unroll
-            for (int k = 0; k < kPacks; ++k) put(c + k * kStep, m[k]);
+            for (int k = 0; k < kGroupPacks; ++k) put(c + k * kStep, m[k]);
             continue;
         }
-        for (int k = 0; k < kPacks && b + k * kStep < i1; ++k) {
+        for (int k = 0; k < kGroupPacks && b + k * kStep < i1; ++k) {
             const int64_t at = c + k * kStep;
             if (at - q >= 0 && at - q + kSpan <= n) {
                 m[0].load(src + at - q);
@@ -353,10 +356,7 @@ int64_t chunk_for(const GradTensor* g, int64_t tensors) {
     for (int64_t i = 0; i < tensors; ++i) n += g[i].n;
     return n < 4 * kPartBlocks * kChunk ? kChunkSmall : kChunk;
 }
-int grid_of(int64_t chunks, int per_sm) {
-    const int64_t all = static_cast<int64_t>(per_sm) * device_sm_count(), most = all < kPartBlocks ? all : kPartBlocks;
-    return static_cast<int>(chunks < 1 ? 1 : (chunks < most ? chunks : most));
-}
+int grid_of(int64_t chunks, int64_t most) { return static_cast<int>(chunks < 1 ? 1 : (chunks < most ? chunks : most)); }
 
 template <int CAP>
 cudaError_t squares(Table<CAP>& t, const GradTensor* g, int64_t tensors, double* part, int64_t* parts, cudaStream_t s) {
@@ -366,7 +366,7 @@ cudaError_t squares(Table<CAP>& t, const GradTensor* g, int64_t tensors, double*
         const int64_t took = fill(t, g, tensors, chunk);
         g += took, tensors -= took;
         if (t.count == 0) continue;
-        const int grid = grid_of(t.chunks, 4);
+        const int grid = grid_of(t.chunks, std::min<int64_t>(4 * device_sm_count(), kPartBlocks));
         if (const cudaError_t e = launch_early(grad_squares_kernel<CAP>, grid, kThreads, 0, 1, s, t, part + *parts)) return e;
         *parts += grid;
     }
@@ -385,7 +385,7 @@ cudaError_t clip(const GradTensor* g, int64_t tensors, double* part, double max_
         const int64_t took = whole ? tensors : fill(t, g, tensors, chunk);
         g += took, tensors -= took;
         if (t.count == 0 && told) continue;
-        if (const cudaError_t e = launch_early(grad_scale_kernel<CAP>, grid_of(t.chunks, 4), kThreads, 0, 1, s, t, part, parts, max_norm, eps,
+        if (const cudaError_t e = launch_early(grad_scale_kernel<CAP>, grid_of(t.chunks, kScaleBlocks), kThreads, 0, 1, s, t, part, parts, max_norm, eps,
                                                told ? static_cast<float*>(nullptr) : norm))
             return e;
         told = true;

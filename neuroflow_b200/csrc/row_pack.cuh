@@ -99,13 +99,17 @@ __device__ __forceinline__ void load_params(const void* p, int type, bool vec, i
     }
 }
 
-// The codes of four values times `inv` (two products to an instruction, each rounded by itself): plain
+// The codes of four values times `i`, `j` (two products to an instruction, each rounded by itself): plain
 // conversions that note in `odd` where they may differ from the encoder, or, with MEND, its codes.
 template <bool MEND>
-__device__ __forceinline__ uint32_t scaled_codes(float a, float b, float c, float d, float inv, uint32_t& odd) {
-    const float2 p = mul2_rn(make_float2(a, b), make_float2(inv, inv)), q = mul2_rn(make_float2(c, d), make_float2(inv, inv));
+__device__ __forceinline__ uint32_t scaled_codes(float a, float b, float c, float d, float2 i, float2 j, uint32_t& odd) {
+    const float2 p = mul2_rn(make_float2(a, b), i), q = mul2_rn(make_float2(c, d), j);
     const uint32_t w = e4m3_convert4(p.x, p.y, q.x, q.y, odd);
     return MEND ? e4m3_mend4(w, p.x, p.y, q.x, q.y) : w;
+}
+template <bool MEND>
+__device__ __forceinline__ uint32_t scaled_codes(float a, float b, float c, float d, float inv, uint32_t& odd) {
+    return scaled_codes<MEND>(a, b, c, d, make_float2(inv, inv), make_float2(inv, inv), odd);
 }
 
 // FP8 codes of a lane's VPT packs (values v, zero beyond column d): pack j holds columns (first_pack +

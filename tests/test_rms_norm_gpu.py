@@ -225,6 +225,47 @@ def test_in_place(d):
     assert hs is r and torch.equal(r, h) and torch.equal(q.codes.view(torch.uint8), w.codes.view(torch.uint8))
 
 
+@pytest.mark.parametrize("x,h", [("float32", "float32"), ("bfloat16", "bfloat16"), ("bfloat16", "float32"), ("float16", None)])
+@pytest.mark.parametrize("d", [5, 8, 13, 35, 127, 128, 131, 250, 264, 500, 519, 1000, 1031, 2047, 4099, 6001, 8200, 16384, 16390])
+def test_fp8_exactly_wherever_rows_start(d, x, h):
+    """Two products, each rounded by itself, and the quantiser's codes: the same bits as torch's products with the rstd
+    that was returned, then fp8_quantise.  Inputs and codes start anywhere, large values sit beside the groups' ends, and
+    what lies between the rows of codes is not written."""
+    torch, ops = _torch()
+    from neuroflow_b200._nfx import lib
+    rows, types = 9, {"float32": 0, "bfloat16": 1, "float16": 2}
+    gen = torch.Generator(device="cuda").manual_seed(d)
+    for shift, pitch, code_shift, code_pitch in ((0, d, 0, d), (1, d, 3, d + 1), (3, d + 1, 0, d + 7), (6, d + 2, 5, d), (7, d + 3, 1, d + 3),
+                                                 (2, -(-d // 8) * 8, 4, -(-d // 16) * 16), (5, -(-d // 8) * 8 + 8, 6, d + 5)):
+        def held(t):
+            v = torch.zeros(rows * pitch + 16, device="cuda", dtype=t.dtype)[shift:shift + rows * pitch].view(rows, pitch)[:, :d]
+            return v.copy_(t)
+        X = torch.randn(rows, d, generator=gen, device="cuda")
+        for i, c in enumerate((0, 6, 7, 120, 121, 127, 128, 129, 255, 256, d - 1)):
+            if c < d:
+                X[i % rows, c] = 1000.0 + i
+        X[rows - 1, d // 2:] = 0
+        X = held(X.to(getattr(torch, x)))
+        R = None if h is None else held(torch.randn(rows, d, generator=gen, device="cuda").to(getattr(torch, h)))
+        S = None if R is None else held(R)
+        G = 1 + 0.2 * torch.randn(d, generator=gen, device="cuda")
+        groups = -(-d // 128)
+        buf = torch.full((rows * code_pitch + 16,), 0x55, device="cuda", dtype=torch.uint8)
+        scales, rstd = torch.empty(rows, groups, device="cuda"), torch.empty(rows, device="cuda")
+        ptr = lambda t: None if t is None else t.data_ptr()
+        assert lib.nfx_rms_norm_fp8(ptr(X), types[x], pitch, ptr(R), 0 if h is None else types[h], pitch, ptr(G), 0, rows, d, EPS,
+                                    ptr(buf) + code_shift, code_pitch, ptr(scales), groups, 1, ptr(S), pitch, ptr(rstd),
+                                    torch.cuda.current_stream().cuda_stream) == 0
+        want, H, _ = _plain(X, R, G)
+        assert S is None or torch.equal(S, H)
+        q = ops.fp8_quantise((H.float() * rstd[:, None]) * G)
+        codes = buf[code_shift:code_shift + rows * code_pitch].view(rows, code_pitch)[:, :d]
+        assert torch.equal(codes, q.codes.view(torch.uint8)), (shift, pitch, code_shift, code_pitch)
+        assert torch.equal(scales, q.scales)
+        buf[code_shift:code_shift + rows * code_pitch].view(rows, code_pitch)[:, :d] = 0x55
+        assert bool((buf == 0x55).all())
+
+
 def test_empty_and_leading_dimensions():
     torch, ops = _torch()
     X, R, G = _case(12, 200, "float32", "float32", "float32", 1)

@@ -47,8 +47,9 @@ struct Table {
     int count;
     int64_t chunks, chunk;
 };
-// Kernel parameters hold 32,764 bytes; a launch copies all of them, so short lists have a table of their own.
-constexpr int kCap = 900, kCapFew = 48;
+// Kernel parameters hold 32,764 bytes; a launch copies all of them (two launches with 900 entries take 6.5 us longer on
+// the host than with 48), so short lists have tables of their own.
+constexpr int kCap = 900, kCapMid = 240, kCapFew = 48;
 static_assert(sizeof(Table<kCap>) + 64 <= 32764, "kernel parameters");
 
 // The tensor that chunk c belongs to (tensors without elements have no entry).
@@ -421,6 +422,9 @@ cudaError_t grad_norm_launch(const GradTensor* g, int64_t tensors, double* part,
     if (tensors <= kCapFew) {
         static thread_local Table<kCapFew> t;
         e = squares(t, g, tensors, part, &parts, s);
+    } else if (tensors <= kCapMid) {
+        static thread_local Table<kCapMid> t;
+        e = squares(t, g, tensors, part, &parts, s);
     } else {
         static thread_local Table<kCap> t;
         e = squares(t, g, tensors, part, &parts, s);
@@ -437,6 +441,7 @@ cudaError_t grad_clip_launch(const GradTensor* g, int64_t tensors, double* part,
         return launch_early(grad_few_kernel<true>, kFewCluster, kFewThreads, 0, kFewCluster, s, t, max_norm, eps, norm);
     }
     if (tensors <= kCapFew) return clip<kCapFew>(g, tensors, part, max_norm, eps, norm, s);
+    if (tensors <= kCapMid) return clip<kCapMid>(g, tensors, part, max_norm, eps, norm, s);
     return clip<kCap>(g, tensors, part, max_norm, eps, norm, s);
 }
 

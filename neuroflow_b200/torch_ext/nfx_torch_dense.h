@@ -275,13 +275,33 @@ ActGrad act_backward(const char* fn, const Tensor& dy, const OptTensor& z, int64
 }
 
 // ---- gradient norm --------------------------------------------------------------------------------
+// A Python list of tensors, which are read where they are: a list of hundreds is looked at tensor by tensor while
+// nothing else of the call takes as long.
+class TensorList {
+    py::list held_;
+    std::vector<const Tensor*> t_;
+
+public:
+    TensorList(const char* what, py::list list) : held_(std::move(list)) {
+        const Py_ssize_t n = PyList_GET_SIZE(held_.ptr());
+        t_.reserve(static_cast<size_t>(n));
+        for (Py_ssize_t i = 0; i < n; ++i) {
+            PyObject* const o = PyList_GET_ITEM(held_.ptr(), i);
+            if (!THPVariable_CheckExact(o) && !THPVariable_Check(o)) throw py::type_error(std::string(what) + " must be tensors");
+            t_.push_back(&THPVariable_Unpack(o));
+        }
+    }
+    size_t size() const { return t_.size(); }
+    const Tensor& operator[](size_t i) const { return *t_[i]; }
+};
 struct GradList {
     std::vector<const void*> src;
     std::vector<void*> dst;
     std::vector<int64_t> n;
     std::vector<int> types, dst_types;
 };
-void no_overlap(const char* fn, const GradList& l, const std::vector<Tensor>& g, const std::vector<Tensor>* out) {
+int64_t bytes_of(int type) { return type == NFX_F32 ? 4 : 2; }
+void no_overlap(const char* fn, const GradList& l, bool out) {
     struct Part {
         uintptr_t at, end;
         bool write;
@@ -292,9 +312,9 @@ void no_overlap(const char* fn, const GradList& l, const std::vector<Tensor>& g,
         if (l.n[i] == 0) continue;
         const uintptr_t s = reinterpret_cast<uintptr_t>(l.src[i]);
         const uintptr_t d = out ? reinterpret_cast<uintptr_t>(l.dst[i]) : s;
-        const bool same = d == s && (!out || l.types[i] == l.dst_types[i]);
-        if (!same) p.push_back({s, s + static_cast<uintptr_t>(l.n[i] * g[i].element_size()), false});
-        p.push_back({d, d + static_cast<uintptr_t>(l.n[i] * (out ? (*out)[i] : g[i]).element_size()), true});
+        const int dt = out ? l.dst_types[i] : l.types[i];
+        if (d != s || dt != l.types[i]) p.push_back({s, s + static_cast<uintptr_t>(l.n[i] * bytes_of(l.types[i])), false});
+        p.push_back({d, d + static_cast<uintptr_t>(l.n[i] * bytes_of(dt)), true});
     }
     const auto before = [](const Part& a, const Part& b) { return a.at < b.at; };
     if (!std::is_sorted(p.begin(), p.end(), before)) std::sort(p.begin(), p.end(), before);
@@ -304,11 +324,12 @@ void no_overlap(const char* fn, const GradList& l, const std::vector<Tensor>& g,
         (q.write ? write_end : read_end) = std::max(q.write ? write_end : read_end, q.end);
     }
 }
-GradList grads_of(const char* fn, const std::vector<Tensor>& g, const std::vector<Tensor>* out) {
-    if (g.empty()) refuse(fn, "there are no gradients");
+GradList grads_of(const char* fn, const TensorList& g, const TensorList* out) {
+    if (g.size() == 0) refuse(fn, "there are no gradients");
     if (out && out->size() != g.size()) refuse(fn, "out must have a tensor for each gradient");
     GradList l;
     l.src.reserve(g.size()), l.n.reserve(g.size()), l.types.reserve(g.size());
+    if (out) l.dst.reserve(g.size()), l.dst_types.reserve(g.size());
     for (size_t i = 0; i < g.size(); ++i) {
         const Tensor& t = g[i];
         if (!t.defined() || t.layout() != at::kStrided) refuse(fn, "a gradient must be a dense tensor");
@@ -329,8 +350,9 @@ GradList grads_of(const char* fn, const std::vector<Tensor>& g, const std::vecto
     return l;
 }
 
-Tensor grad_norm(const std::vector<Tensor>& g) {
+Tensor grad_norm(py::list grads) {
     const char* fn = "grad_norm";
+    const TensorList g("gradients", std::move(grads));
     const GradList l = grads_of(fn, g, nullptr);
     c10::cuda::CUDAGuard guard(g[0].device());
     const Tensor norm = empty({}, at::kFloat, g[0]);
@@ -340,23 +362,26 @@ Tensor grad_norm(const std::vector<Tensor>& g) {
     return norm;
 }
 
-Tensor clip_grad_norm(const std::vector<Tensor>& g, double max_norm, double eps, const std::optional<std::vector<Tensor>>& out) {
+Tensor clip_grad_norm(py::list grads, double max_norm, double eps, std::optional<py::list> outs) {
     const char* fn = "clip_grad_norm";
-    const std::vector<Tensor>& to = out ? *out : g;
+    const bool out = outs.has_value();
+    const TensorList g("gradients", std::move(grads)), o("out", out ? std::move(*outs) : py::list());
+    const TensorList& to = out ? o : g;
     if (!(max_norm >= 0)) refuse(fn, "max_norm must be >= 0");
     if (!(eps >= 0) || std::isinf(eps)) refuse(fn, "eps must be >= 0 and finite");
-    const GradList l = grads_of(fn, g, out ? &to : nullptr);
+    const GradList l = grads_of(fn, g, out ? &o : nullptr);
     if (at::GradMode::is_enabled())
-        for (const Tensor& t : to)
-            if (t.requires_grad()) refuse(fn, "a tensor that is written must not require grad");
-    no_overlap(fn, l, g, out ? &to : nullptr);
+        for (size_t i = 0; i < to.size(); ++i)
+            if (to[i].requires_grad()) refuse(fn, "a tensor that is written must not require grad");
+    no_overlap(fn, l, out);
     c10::cuda::CUDAGuard guard(g[0].device());
     const Tensor norm = empty({}, at::kFloat, g[0]);
     const int64_t bytes = nfx_grad_norm_workspace(static_cast<int64_t>(g.size()));
     const Tensor ws = workspace(bytes, g[0]);
     check(nfx_clip_grad_norm(l.src.data(), l.n.data(), l.types.data(), out ? l.dst.data() : nullptr, out ? l.dst_types.data() : nullptr,
                              static_cast<int64_t>(g.size()), max_norm, eps, ptr(norm), raw(ws), bytes, stream_of(g[0])));
-    for (const Tensor& t : to) written(t);
+    for (size_t i = 0; i < to.size(); ++i)
+        if (!to[i].is_inference()) to[i].unsafeGetTensorImpl()->bump_version();
     return norm;
 }
 

@@ -156,3 +156,6 @@ def test_front_end_refuses_cpu_tensors():
         with pytest.raises(_nfx.NfxError) as ei:
             f()
         assert ei.value.code == 1
+    for f in (lambda: ops.grad_norm([None]), lambda: ops.clip_grad_norm([x, 3], 1.0), lambda: ops.clip_grad_norm([x], 1.0, out=["x"])):
+        with pytest.raises(TypeError, match="must be tensors"):
+            f()

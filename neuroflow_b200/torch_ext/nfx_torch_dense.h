@@ -240,6 +240,18 @@ Product gemm(const char* fn, const Tensor& at, const Tensor& bt, const OptTensor
     return o;
 }
 
+Matrix transposed(const Matrix& m) { return {m.cols, m.rows, m.ld, 1 - m.t, m.p}; }
+// a b^T of `type` as a tensor of `sizes`, the product's elements in order.
+Tensor plain_product(const Matrix& a, const Matrix& b, at::ScalarType type, at::IntArrayRef sizes, const Tensor& like) {
+    c10::cuda::CUDAGuard guard(like.device());
+    const Tensor c = empty(sizes, type, like);
+    const int64_t bytes = nfx_gemm_workspace(a.p, a.ld, a.t, b.p, b.ld, b.t, a.rows, b.rows, a.cols);
+    const Tensor ws = workspace(bytes, like);
+    check(nfx_gemm(a.p, a.ld, a.t, b.p, b.ld, b.t, type_of(type), a.rows, b.rows, a.cols, nullptr, NFX_F32, 0, nullptr, 0, c.data_ptr(), type_of(type),
+                   b.rows, nullptr, b.rows, raw(ws), bytes, stream_of(like)));
+    return c;
+}
+
 struct ActGrad {
     Tensor dz, db;
 };
@@ -425,12 +437,11 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
         const bool grad_z = x.requires_grad() || w.requires_grad() || (b && b->requires_grad());
         const Product p = gemm("linear", x2, w, b, act, r2, std::nullopt, std::nullopt, act != 0 && grad_z);
         ctx->save_for_backward({w.requires_grad() ? x : Tensor(), x.requires_grad() ? w : Tensor(), p.z});
-        ctx->saved_data["act"] = act;
-        ctx->saved_data["needs"] = (x.requires_grad() ? 1 : 0) | (w.requires_grad() ? 2 : 0) | (b && b->requires_grad() ? 4 : 0) |
-                                   (residual && residual->requires_grad() ? 8 : 0);
-        ctx->saved_data["bias"] = b ? static_cast<int64_t>(b->scalar_type()) : static_cast<int64_t>(-1);
-        ctx->saved_data["x"] = x.sizes().vec();
-        ctx->saved_data["n"] = w.size(0);
+        // which gradients are wanted, the activation and the bias' type
+        const int64_t needs = (x.requires_grad() ? 1 : 0) | (w.requires_grad() ? 2 : 0) | (b && b->requires_grad() ? 4 : 0) |
+                              (residual && residual->requires_grad() ? 8 : 0);
+        ctx->saved_data["what"] = needs | act << 4 | static_cast<int64_t>(b ? b->scalar_type() : at::kFloat) << 8;
+        if (x.dim() == 2) return p.c;
         auto sizes = x.sizes().vec();
         sizes.back() = w.size(0);
         return p.c.view(sizes);
@@ -438,21 +449,27 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
         const char* fn = "linear";
         const auto saved = ctx->get_saved_variables();
-        const int64_t needs = ctx->saved_data["needs"].toInt(), act = ctx->saved_data["act"].toInt(), n = ctx->saved_data["n"].toInt();
-        const auto xs = ctx->saved_data["x"].toIntVector();
+        const int64_t what = ctx->saved_data["what"].toInt(), needs = what & 15, act = what >> 4 & 15;
+        const Tensor dy = grads[0].contiguous();
+        const at::ScalarType type = dy.scalar_type();
         int64_t rows = 1;
-        for (size_t i = 0; i + 1 < xs.size(); ++i) rows *= xs[i];
-        const Tensor dy = grads[0].contiguous(), dy2 = dy.view({rows, n});
+        for (int64_t i = 0; i + 1 < dy.dim(); ++i) rows *= dy.size(i);
+        const auto flat = [&](const Tensor& t) { return t.dim() == 2 ? t : t.reshape({rows, t.size(-1)}); };
         Tensor dx, dw, db;
         if (needs & 7) {
-            const ActGrad g = act_backward(fn, dy2, defined(saved[2]), act, (needs & 3) != 0,
-                                           needs & 4 ? std::optional<at::ScalarType>(static_cast<at::ScalarType>(ctx->saved_data["bias"].toInt()))
-                                                     : std::nullopt);
+            const ActGrad g = act_backward(fn, flat(dy), defined(saved[2]), act, (needs & 3) != 0,
+                                           needs & 4 ? std::optional<at::ScalarType>(static_cast<at::ScalarType>(what >> 8)) : std::nullopt);
             db = g.db;
-            if (needs & 2)
-                dw = gemm(fn, g.dz.t(), saved[0].reshape({rows, xs.back()}).t(), std::nullopt, 0, std::nullopt, std::nullopt, std::nullopt, false).c;
-            if (needs & 1)
-                dx = gemm(fn, g.dz, saved[1].t(), std::nullopt, 0, std::nullopt, std::nullopt, std::nullopt, false).c.view(xs);
+            if (needs & 2) {
+                const Tensor x = flat(saved[0]);
+                const int64_t sizes[2] = {dy.size(-1), x.size(1)};
+                dw = plain_product(transposed(matrix_of(fn, "dy", g.dz, type)), transposed(matrix_of(fn, "x", x, type)), type, sizes, dy);
+            }
+            if (needs & 1) {
+                auto sizes = dy.sizes().vec();
+                sizes.back() = saved[1].size(1);
+                dx = plain_product(matrix_of(fn, "dy", g.dz, type), transposed(matrix_of(fn, "weight", saved[1], type)), type, sizes, dy);
+            }
         }
         return {once(fn, dx), once(fn, dw), once(fn, db), Tensor(), needs & 8 ? once(fn, grads[0]) : Tensor(), Tensor()};
     }

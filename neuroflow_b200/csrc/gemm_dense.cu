@@ -1120,7 +1120,8 @@ int64_t copy_stride(int64_t cols) { return cols > 256 ? (cols + 63) / 64 * 64 : 
 //       NT = 16, 32, 64, 128: base 3.3, 4.6, 5.4, 6.0; c 0.22, 0.22, 0.24, 0.27, where two CTAs share an SM 0.32, 0.36,
 //       0.40; further 3.7, 4.2, 5.2, 7.4; join 1.0, 0.6, 0.7, 0.8
 //   pairs, split s                5.6 + rounds ceil(KB / s) 0.32 + 1.4 per further round + 0, 1.9, 3.5 (s = 1, 2, 4)
-// Clusters do not fill every processor cluster's SMs: 132 CTAs at a time in fours, 112 in eights, 70 and 56 pairs.  Over
+// Clusters do not fill every processor cluster's SMs: 132 CTAs at a time in fours, 112 in eights, 66 and 56 pairs
+// (440x4304x11248 as 34 tiles of two pairs each: 79 us, twice what one round takes).  Over
 // the 61 measured shapes the choice takes 1.9 % longer than the best one.  E.g. 512x4096x4096: 19.5 with pairs and a
 // split of 2, 22.7 with 128/1, 25.7 with pairs alone; 355x3616x7136: 26.6, 36.0, 40.6; 64x1024x1024: 5.2 with 16/4,
 // 5.5 with 64/8, 8.5 with 64/1; 1024x1024x1024: 9.4 with 64/1, 9.8 with 128/2, 10.6 pairs.
@@ -1154,7 +1155,7 @@ DensePlan gemm_dense_plan(int64_t M, int64_t N, int64_t K, int a_t, int64_t sms)
     }
     const int64_t tiles = up(M, 256) * up(N, 256), pairs = sms / 2;
     for (int s = 1; s <= 4 && pairs > 0 && (s == 1 || 2 * s <= KB); s *= 2) {
-        const int64_t at_a_time = s == 1 ? pairs : (s == 2 ? pairs * 19 / 20 : pairs * 3 / 4);
+        const int64_t at_a_time = s == 1 ? pairs : (s == 2 ? pairs * 9 / 10 : pairs * 3 / 4);
         if (s > 1 && tiles * s > at_a_time) break;
         const int64_t rounds = up(tiles * s, at_a_time), cost = 560 + rounds * up(KB, s) * 32 + (rounds - 1) * 143 + (s == 1 ? 0 : (s == 2 ? 187 : 351));
         if (cost < best) best = cost, plan = {0, s, false, 1};

@@ -139,6 +139,21 @@ def test_a_sum_beyond_fp32_is_scaled_all_the_same():
     assert ((g[0].double() - 0.1).abs() <= 0.1 * SCALE).all()
 
 
+@pytest.mark.parametrize("count", [47, 48, 49, 239, 240, 241, 899, 900, 901, 1805])
+def test_lists_as_long_as_the_tables(count):
+    """Lists that just fit a table of the kernels' parameters or just do not, some tensors without elements among them,
+    in place and into unaligned parts of one buffer."""
+    torch, ops = _torch()
+    g = _grads([(37 * i) % 900 * (i % 7 != 3) + 2000 * (i % 50 == 0) for i in range(count)], ALL, count)
+    before = [t.clone() for t in g]
+    assert abs(float(ops.grad_norm(g)) - _norm(g)) <= NORM * _norm(g)
+    flat = torch.full((sum(t.numel() for t in g) + 3,), 7.0, device="cuda")
+    out = list(flat[1:-2].split([t.numel() for t in g]))
+    _check(out, before, ops.clip_grad_norm(g, 2.0, out=out), 2.0)
+    assert all(torch.equal(p, q) for p, q in zip(g, before)) and flat[0] == 7 and (flat[-2:] == 7).all()
+    _check(g, before, ops.clip_grad_norm(g, 2.0), 2.0)
+
+
 def test_permuted_and_large():
     torch, ops = _torch()
     a = _grads([64 * 48], ("float32",), 4)[0].view(64, 48)

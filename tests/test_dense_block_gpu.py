@@ -369,6 +369,32 @@ def test_linear_of_a_vector_and_of_no_tokens():
     assert y.shape == (0, 64) and not dg.any()
 
 
+@pytest.mark.parametrize("act", [0, 1, 2])
+@pytest.mark.parametrize("shape", [(3, 5, 64), (1, 64), (2, 1, 65), (4, 2, 3, 24)])
+def test_linear_makes_the_gradients_that_are_asked_for(shape, act):
+    """Any of the four gradients alone or together: the same bits, and those of the calls that the layer is made of."""
+    torch, ops = _torch()
+    gen = torch.Generator(device="cuda").manual_seed(act)
+    rnd = lambda *s: torch.randn(*s, generator=gen, device="cuda").bfloat16()
+    k, n = shape[-1], 40
+    ts = [rnd(*shape), rnd(n, k + 3)[:, :k], rnd(n), rnd(*shape[:-1], n)]
+    dy = rnd(n, *shape[:-1]).movedim(0, -1)  # (not contiguous)
+    x2, dy2 = ts[0].view(-1, k), dy.reshape(-1, n).contiguous()
+    y, z = ops.gemm(x2, ts[1], bias=ts[2], act=act, residual=ts[3].reshape(-1, n), preact=True)
+    dz, db = ops.act_backward(dy2, z, act, torch.bfloat16)
+    want = [ops.gemm(dz, ts[1].t()).view(shape), ops.gemm(dz.t(), x2.t()), db, dy]
+    for mask in range(1, 16):
+        leaves = [t.detach().requires_grad_(bool(mask >> i & 1)) for i, t in enumerate(ts)]
+        got = ops.linear(leaves[0], leaves[1], leaves[2], act=act, residual=leaves[3])
+        assert torch.equal(got.detach().view(-1, n), y)
+        asked = [i for i in range(4) if mask >> i & 1]
+        for i, g in zip(asked, torch.autograd.grad(got, [leaves[i] for i in asked], dy)):
+            w = want[i]
+            assert g.shape == ts[i].shape
+            # (dz of one row may be taken as a row or a column: the same products, maybe added in another order)
+            assert torch.equal(g, w) or (g.double() - w.double()).abs().max() <= 2.0 ** -8 * w.double().abs().max(), (mask, i)
+
+
 def test_two_streams_at_once():
     """The same calls on two streams, without order between them: nothing is shared but the error word."""
     torch, ops = _torch()

@@ -928,7 +928,9 @@ gemm_narrow_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
     const bool failed = *sAbort != 0;
     const int cols = (NT + split - 1) / split;
     constexpr int kEl = CT == kF32 ? 4 : 2;
-    const auto vec_of = [&](const void* m, int64_t ld) { return reinterpret_cast<uintptr_t>(m) % (4 * kEl) == 0 && (p.M == 1 || ld % 4 == 0); };
+    // (a matrix of one row has no row stride to speak of, a run's C has: it is one of p.runs, M rows apart)
+    const bool one_row = p.M == 1 && p.runs == 1;
+    const auto vec_of = [&](const void* m, int64_t ld) { return reinterpret_cast<uintptr_t>(m) % (4 * kEl) == 0 && (one_row || ld % 4 == 0); };
     const bool vec_c = vec_of(p.C, p.ldc), vec_z = vec_of(p.Z, p.ldz), vec_r = vec_of(p.res, p.ldres);
     const auto store4 = [&](void* mat, int64_t at, bool vec, int n, const float (&o)[4]) {
         if (vec && n + 4 <= p.N) {

@@ -52,7 +52,7 @@ constexpr const char* kStride = "a row stride is smaller than its row";
 const char* rms_check(int64_t rows, int64_t d, int x_type, int h_type, int param_type, bool with_h) {
     if (!type_ok(x_type) || !type_ok(param_type) || (with_h && !type_ok(h_type))) return kTypes;
     if (rows < 0 || d < 1) return "rows must be >= 0 and d >= 1";
-    // the kernels for any width add 256 to a 32-bit column index before they compare it with d
+    // columns are 32-bit numbers, also when rounded up to a whole FP8 group; loops that step by more count without a sign
     if (d > kIntMax - 256) return "d must be below 2^31 - 256";
     if (with_h && h_type != x_type && h_type != NFX_F32) return "the residual must have x's type or be NFX_F32";
     return nullptr;

@@ -39,6 +39,7 @@ __global__ void __launch_bounds__(kWideThreads, 2) rms_wide_kernel(RmsArgs a, Sh
     int buf = 0;
     for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x, buf ^= 1) {
         const Split<VE> sp(a.d, static_cast<int>((sh.base + r * sh.step) % VE), tid);
+        const uint32_t packs = sp.packs;  // (up to 2^31: the number of the next one has no sign)
         const T* x = static_cast<const T*>(a.x) + r * a.ldx;
         const H* res = a.res ? static_cast<const H*>(a.res) + r * a.ldres : nullptr;
         H* sum = a.sum ? static_cast<H*>(a.sum) + r * a.ldsum : nullptr;
@@ -71,9 +72,9 @@ __global__ void __launch_bounds__(kWideThreads, 2) rms_wide_kernel(RmsArgs a, Sh
             return to_f32(h);
         };
         float q = 0.0f;
-        for (int k = tid; k < sp.packs; k += kWideThreads) {
+        for (uint32_t k = tid; k < packs; k += kWideThreads) {
             float v[VE];
-            pack(sp.head + k * VE, false, v);
+            pack(sp.head + static_cast<int>(k) * VE, false, v);
 #pragma unroll
             for (int i = 0; i < VE; ++i) q = fmaf(v[i], v[i], q);
         }
@@ -86,8 +87,8 @@ __global__ void __launch_bounds__(kWideThreads, 2) rms_wide_kernel(RmsArgs a, Sh
         const auto gamma = [&](int c) { return a.gamma ? load_any(a.gamma, a.ptype, c) : 1.0f; };
         if constexpr (!FP8) {
             T* y = static_cast<T*>(a.y) + r * a.ldy;
-            for (int k = tid; k < sp.packs; k += kWideThreads) {
-                const int c = sp.head + k * VE;
+            for (uint32_t k = tid; k < packs; k += kWideThreads) {
+                const int c = sp.head + static_cast<int>(k) * VE;
                 float v[VE];
                 pack(c, true, v);
 #pragma unroll

@@ -31,6 +31,7 @@ __global__ void __launch_bounds__(kWideThreads, 2) rms_grad_wide_kernel(RmsGradA
     const int tid = threadIdx.x;
     float* pg = a.part + static_cast<int64_t>(blockIdx.x) * a.d;
     const Split<VE> sp(a.d, static_cast<int>((sh.base + static_cast<int64_t>(blockIdx.x) * sh.step) % VE), tid);
+    const uint32_t packs = sp.packs;  // (up to 2^31: the number of the next one has no sign)
     const auto gamma = [&](int c) { return a.gamma ? load_any(a.gamma, a.ptype, c) : 1.0f; };
     grid_dep_wait();  // what the kernel before this one wrote may be read from here on
     int buf = 0;
@@ -46,8 +47,8 @@ __global__ void __launch_bounds__(kWideThreads, 2) rms_grad_wide_kernel(RmsGradA
             t = fmaf(gamma(c), dyx, t);
             return dyx;
         };
-        for (int k = tid; k < sp.packs; k += kWideThreads) {
-            const int c = sp.head + k * VE;
+        for (uint32_t k = tid; k < packs; k += kWideThreads) {
+            const int c = sp.head + static_cast<int>(k) * VE;
             Elems<T, VE> y;
             Elems<H, VE> x;
             y.load(dy + c), x.load(h + c);
@@ -64,8 +65,8 @@ __global__ void __launch_bounds__(kWideThreads, 2) rms_grad_wide_kernel(RmsGradA
         const float m = __fdiv_rn(row_sum<false>(t, red[buf], kWideThreads / 32), static_cast<float>(a.d)) * rs;
         T* dx = static_cast<T*>(a.dx) + r * a.lddx;
         H* dr = static_cast<H*>(a.dres) + r * a.lddres;
-        for (int k = tid; k < sp.packs; k += kWideThreads) {
-            const int c = sp.head + k * VE;
+        for (uint32_t k = tid; k < packs; k += kWideThreads) {
+            const int c = sp.head + static_cast<int>(k) * VE;
             Elems<T, VE> y;
             Elems<H, VE> x, s;
             y.load(dy + c), x.load(h + c);

@@ -5,9 +5,8 @@
 //
 // A (M, K) and B (N, K) are bf16 or fp16, each with contiguous rows (K-major) or contiguous columns (MN-major:
 // the gradient products dX = dZ W and dW = dZ^T X read the forward pass's matrices as they are).  Sums are
-// fp32.  The tensor core cuts its running sum off instead of rounding it, which drifts over a long K:
-// where C is fp32, pieces of 512 terms are summed in TMEM and joined in registers; where C has 16 bits one
-// piece covers all of K.
+// fp32.  The tensor core cuts its running sum off instead of rounding it, which drifts over a long K, so pieces
+// of 512 terms (4,096 where C has 16 bits) are summed in TMEM and joined in registers (piece_terms()).
 //
 // Three kernels: pairs of CTAs on 256 x 256 tiles for large results; the same with K split over the pairs of a cluster
 // where such tiles are few; and a narrow one, with K split over a cluster, for few rows of A or few tiles.
@@ -38,7 +37,8 @@ namespace nfx {
 namespace {
 
 constexpr int kBK = 64;          // 128 bytes of K: one swizzled row
-constexpr int kPiece = 512 / kBK;  // blocks of K to a piece where C is fp32
+template <int CT>
+constexpr int kPiece = piece_terms(CT) / kBK;  // blocks of K that one TMEM stage sums
 constexpr int kOutBytes = 32 * 128;
 
 // K-major tiles lie as rows of 128 bytes (64 of K), MN-major ones as 64 rows of K by 64 elements, one such box of
@@ -277,8 +277,8 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     const int tiles = tm * tn;
     const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
     const int KB = (p.K + kBK - 1) / kBK;
-    const int piece = CT == kF32 ? kPiece : KB;  // blocks of K that one TMEM stage sums
-    const int pieces = KB == 0 ? 0 : (KB + piece - 1) / piece;
+    constexpr int piece = kPiece<CT>;
+    const int pieces = (KB + piece - 1) / piece;
     const uint64_t budget = p.wait_ns ? p.wait_ns : kWaitNs;
 
     if (threadIdx.x == 0) {
@@ -410,11 +410,13 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
                         __syncwarp();
                         if (lane == 0) mbar_arrive_cluster(accEmpty0 + st * 8);
                     }
+                    if (CT != kF32 && i == 0) {  // (most often the only one)
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const float2 v = make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
-                        if constexpr (CT == kF32) acc[c * 16 + j] = add2_rn(acc[c * 16 + j], v);
-                        else acc[c * 16 + j] = v;
+                        for (int j = 0; j < 16; ++j) acc[c * 16 + j] = make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            acc[c * 16 + j] = add2_rn(acc[c * 16 + j], make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])));
                     }
                 }
             }
@@ -563,7 +565,7 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
     const int mt = tile / tn, nt = tile % tn;
     const int KB = (p.K + kBK - 1) / kBK;
     const int kb0 = static_cast<int>(static_cast<int64_t>(KB) * pair / S), count = static_cast<int>(static_cast<int64_t>(KB) * (pair + 1) / S) - kb0;
-    const int piece = CT == kF32 ? kPiece : count;
+    constexpr int piece = kPiece<CT>;
     const uint64_t budget = p.wait_ns ? p.wait_ns : kWaitNs;
 
     if (threadIdx.x == 0) {
@@ -796,7 +798,7 @@ gemm_narrow_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
     const int KB = (p.K + kBK - 1) / kBK, parts = split * p.runs, part_i = run * split + rank;
     const int kb0 = static_cast<int>(static_cast<int64_t>(KB) * part_i / parts);
     const int count = static_cast<int>(static_cast<int64_t>(KB) * (part_i + 1) / parts) - kb0;
-    const int piece = CT == kF32 ? kPiece : count;
+    constexpr int piece = kPiece<CT>;
     const uint64_t budget = p.wait_ns ? p.wait_ns : kWaitNs;
 
     if (threadIdx.x == 0) {

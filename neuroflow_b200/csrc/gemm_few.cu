@@ -13,10 +13,10 @@
 //     rows k0 + 4 t .. + 3; pairs of rows are joined by byte permutations, and instruction j takes column
 //     8 g + j as its column g.
 // The eight warps of a block share K by turns, blocks of a cluster by parts; partial sums are joined in a fixed
-// order through shared memory.
+// order through shared memory, where a warp also adds up the pieces of a long K (piece_terms()).
 //
 // Measured (one B200, weights from HBM): 1x4096x4096 8.1 to 8.4 us, 4.1 TB/s (narrow kernel 10.0), 1x4096x16384 23 us, 5.8 TB/s,
-// 16x4096x4096 9.8 us, 1x1024x1024 2.4 us (4.3), 1x64x64 1.6 us.  Small ones are bound by the launch and one trip to
+// 16x4096x4096 9.8 us, 1x1024x1024 2.3 us (4.3), 1x64x64 1.7 us.  Small ones are bound by the launch and one trip to
 // memory, large ones by HBM.
 #include <cuda_runtime.h>
 
@@ -54,13 +54,18 @@ struct Few {
     static constexpr int kCols = KMAJOR ? 16 * kMT : 64;
     static constexpr int kU = KMAJOR ? (NT == 1 ? (VEC ? 8 : 4) : (NT == 2 && VEC ? 3 : 2)) : 3;
     static constexpr int kOut = kRows * kCols;
-    static constexpr int kSmem = (kWarps + 1) * kOut * 4;
+    static constexpr int kPart = KMAJOR ? kOut : kRows * 66;  // a warp's sums
+    static constexpr int kSmem = (kWarps * kPart + kOut) * 4;
+    // where the sum of row m of A and row n of B is among a warp's: a warp's lanes, and 32 columns, lie in unlike banks
+    __device__ static constexpr int place(int m, int n) {
+        return KMAJOR ? m * kCols + (kCols > 16 ? n ^ ((m & 6) << 2) : n) : m * 66 + n + (n >> 5);
+    }
 };
 
 template <typename T, int CT, bool KMAJOR, bool VEC, int NT>
 __global__ void __launch_bounds__(kThreads, 2) gemm_few_kernel(const GemmDenseArgs p, const int split) {
     using F = Few<KMAJOR, VEC, NT>;
-    constexpr int kCols = F::kCols, kOut = F::kOut, kU = F::kU, kMT = F::kMT;
+    constexpr int kCols = F::kCols, kOut = F::kOut, kPart = F::kPart, kU = F::kU, kMT = F::kMT;
     extern __shared__ float part[];  // (warp, row of A, row of B) sums, then the block's
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int rank = blockIdx.x % split, n0 = blockIdx.x / split * kCols;
@@ -76,6 +81,8 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_few_kernel(const GemmDenseAr
     const int which = rank == split - 1 ? kWarps - 1 - warp : 3;
     const bool by_elements = which == 0 ? p.K % kStep != 0 : (!VEC && which < 3 && steps >= which);
     const int64_t arow = p.lda;
+    constexpr int kTurns = piece_terms(CT) / (kStep * kU);  // turns of a warp's loop to a piece of K
+    float* mine = part + warp * kPart;
 
     grid_dep_launch();
     grid_dep_wait();  // what the kernel before this one wrote may be read from here on
@@ -102,21 +109,42 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_few_kernel(const GemmDenseAr
                     mma16<T>(c[i][j], wb[2 * i][2], wb[2 * i + 1][2], wb[2 * i][3], wb[2 * i + 1][3], wa[j][2], wa[j][3]);
                 }
         };
-        for (int s = s0 + warp; s < s1; s += kWarps * kU) {
-            uint32_t wb[kU][2 * kMT][4], wa[kU][NT][4];
+        const auto put = [&](auto add) {  // to this lane's places
 #pragma unroll
-            for (int u = 0; u < kU; ++u) {
-                if (s + u * kWarps < s1) {
-                    const int k = (s + u * kWarps) * kStep + t * 8;
+            for (int i = 0; i < kMT; ++i)
 #pragma unroll
-                    for (int i = 0; i < 2 * kMT; ++i) load8<VEC>(br[i] + k, wb[u][i]);
+                for (int j = 0; j < NT; ++j)
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) load8<VEC>(ar[j] + k, wa[u][j]);
+                    for (int e = 0; e < 4; ++e) {
+                        float& m = mine[F::place(j * 8 + 2 * t + (e & 1), i * 16 + g + 8 * (e >> 1))];
+                        m = add ? m + c[i][j][e] : c[i][j][e];
+                        c[i][j][e] = 0.0f;
+                    }
+        };
+        int s = s0 + warp;
+        bool first = true;
+        for (;;) {
+            const int end = min(s1, s + kWarps * kU * kTurns);
+            for (; s < end; s += kWarps * kU) {
+                uint32_t wb[kU][2 * kMT][4], wa[kU][NT][4];
+#pragma unroll
+                for (int u = 0; u < kU; ++u) {
+                    if (s + u * kWarps < s1) {
+                        const int k = (s + u * kWarps) * kStep + t * 8;
+#pragma unroll
+                        for (int i = 0; i < 2 * kMT; ++i) load8<VEC>(br[i] + k, wb[u][i]);
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) load8<VEC>(ar[j] + k, wa[u][j]);
+                    }
                 }
-            }
 #pragma unroll
-            for (int u = 0; u < kU; ++u)
-                if (s + u * kWarps < s1) step(wb[u], wa[u]);
+                for (int u = 0; u < kU; ++u)
+                    if (s + u * kWarps < s1) step(wb[u], wa[u]);
+            }
+            if (s >= s1) [[likely]] break;
+            if (first) put(std::false_type{});
+            else put(std::true_type{});
+            first = false;
         }
         if (by_elements) {
             uint32_t wb[2 * kMT][4], wa[NT][4];
@@ -127,13 +155,8 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_few_kernel(const GemmDenseAr
             for (int j = 0; j < NT; ++j) load_single<8>(ar[j], k, p.K, wa[j]);
             step(wb, wa);
         }
-        float* mine = part + warp * kOut;
-#pragma unroll
-        for (int i = 0; i < kMT; ++i)
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) mine[(j * 8 + 2 * t + (e & 1)) * kCols + i * 16 + g + 8 * (e >> 1)] = c[i][j][e];
+        if (first) [[likely]] put(std::false_type{});
+        else put(std::true_type{});
     } else {
         float c[8][4];
 #pragma unroll
@@ -153,28 +176,47 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_few_kernel(const GemmDenseAr
                 mma16<T>(c[j], wa[0][0], wa[1][0], wa[0][1], wa[1][1], lo, hi);
             }
         };
-        for (int s = s0 + warp; s < s1; s += kWarps * kU) {
-            uint32_t wb[kU][4][4], wa[kU][2][2];
+        const auto put = [&](auto add) {
 #pragma unroll
-            for (int u = 0; u < kU; ++u) {
-                if (s + u * kWarps < s1) {
-                    const int k = (s + u * kWarps) * kStep + t * 4;
+            for (int j = 0; j < 8; ++j)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) row(k + r, wb[u][r]);
+                for (int i = 0; i < 4; ++i) {
+                    float& m = mine[F::place(g + 8 * (i >> 1), (2 * t + (i & 1)) * 8 + j)];
+                    m = add ? m + c[j][i] : c[j][i];
+                    c[j][i] = 0.0f;
+                }
+        };
+        int s = s0 + warp;
+        bool first = true;
+        for (;;) {
+            const int end = min(s1, s + kWarps * kU * kTurns);
+            for (; s < end; s += kWarps * kU) {
+                uint32_t wb[kU][4][4], wa[kU][2][2];
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if constexpr (VEC) {
-                            const uint2 v = __ldg(reinterpret_cast<const uint2*>(ar[h] + k));
-                            wa[u][h][0] = v.x, wa[u][h][1] = v.y;
-                        } else {
-                            load_single<4>(ar[h], k, p.K, wa[u][h]);
+                for (int u = 0; u < kU; ++u) {
+                    if (s + u * kWarps < s1) {
+                        const int k = (s + u * kWarps) * kStep + t * 4;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) row(k + r, wb[u][r]);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            if constexpr (VEC) {
+                                const uint2 v = __ldg(reinterpret_cast<const uint2*>(ar[h] + k));
+                                wa[u][h][0] = v.x, wa[u][h][1] = v.y;
+                            } else {
+                                load_single<4>(ar[h], k, p.K, wa[u][h]);
+                            }
                         }
                     }
                 }
-            }
 #pragma unroll
-            for (int u = 0; u < kU; ++u)
-                if (s + u * kWarps < s1) step(wb[u], wa[u]);
+                for (int u = 0; u < kU; ++u)
+                    if (s + u * kWarps < s1) step(wb[u], wa[u]);
+            }
+            if (s >= s1) [[likely]] break;
+            if (first) put(std::false_type{});
+            else put(std::true_type{});
+            first = false;
         }
         if (by_elements) {
             uint32_t wb[4][4], wa[2][2];
@@ -188,18 +230,15 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_few_kernel(const GemmDenseAr
             for (int h = 0; h < 2; ++h) load_single<4>(ar[h], k, p.K, wa[h]);
             step(wb, wa);
         }
-        float* mine = part + warp * kOut;
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) mine[(g + 8 * (i >> 1)) * kCols + (2 * t + (i & 1)) * 8 + j] = c[j][i];
+        if (first) [[likely]] put(std::false_type{});
+        else put(std::true_type{});
     }
     __syncthreads();
-    float* sum = part + kWarps * kOut;
+    float* sum = part + kWarps * kPart;
     const auto joined = [&](int e) {
         float v = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) v += part[w * kOut + e];
+        for (int w = 0; w < kWarps; ++w) v += part[w * kPart + F::place(e / kCols, e % kCols)];
         return v;
     };
     if (split > 1) {

@@ -26,6 +26,12 @@ __device__ __forceinline__ float2 gelu_sig2(float2 z) {
     const float a = 1.0f + e.x, b = 1.0f + e.y, r = __fdividef(1.0f, a * b);
     return make_float2((ux > 60.0f ? -0.0f : z.x) * (r * b), (uy > 60.0f ? -0.0f : z.y) * (r * a));
 }
+// Terms that a tensor core sums by itself before the sum is joined with others in fp32.  It cuts its running sum off instead
+// of rounding it, so a sum of numbers of one sign comes out low, the more the longer it is: by 3e-6 of itself after 512
+// terms, where fp32 results stop, by 2.4e-5 after 4,096, a twentieth of an fp16 result's own rounding, where 16-bit
+// results do, and by 3.9e-4 after 65,536.
+constexpr int piece_terms(int ct) { return ct == kF32 ? 512 : 4096; }
+
 template <int R>
 __device__ __forceinline__ void reg_inc() {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R));

@@ -497,7 +497,7 @@ int nfx_act_backward(const void* dy, int64_t lddy, const void* z, int64_t ldz, i
  * place.  Any alignment, sizes and number of tensors.  Sums of squares are 64-bit numbers; `norm` (one
  * float on the device) is rounded to fp32.  out[i] may be grads[i] of the same type; beyond that no
  * output shares memory with another tensor.  A norm of infinity gives zeros, and NaN where an element is
- * infinite; a NaN gives NaN everywhere.  The workspace is 16-byte aligned, of nfx_grad_norm_workspace
+ * infinite, but with a max_norm of infinity nothing is scaled; a NaN gives NaN everywhere.  The workspace is 16-byte aligned, of nfx_grad_norm_workspace
  * bytes. */
 int64_t nfx_grad_norm_workspace(int64_t tensors);
 int nfx_grad_norm(const void* const* grads, const int64_t* counts, const int* types, int64_t tensors, float* norm,

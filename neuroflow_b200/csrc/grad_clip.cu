@@ -260,9 +260,10 @@ __device__ __forceinline__ void chunk_scale(const Table<CAP>& t, int64_t c, floa
     else go(static_cast<const __half*>(e.src));
 }
 
-// (a NaN stays one; a norm of zero leaves the zeros as they are, also with max_norm and eps of zero)
+// (a NaN stays one; a norm of zero leaves the zeros as they are, also with max_norm and eps of zero, and a max_norm of
+// infinity leaves everything, also with an infinite norm)
 __device__ __forceinline__ float scale_for(double n, double max_norm, double eps) {
-    const double q = n == 0.0 ? 1.0 : max_norm / (n + eps);
+    const double q = n == 0.0 || (isinf(max_norm) && !isnan(n)) ? 1.0 : max_norm / (n + eps);
     return q >= 1.0 ? 1.0f : static_cast<float>(q);
 }
 

@@ -228,7 +228,8 @@ def grad_norm(grads, stream=None):
 
 def clip_grad_norm(grads, max_norm, eps=1e-6, out=None, stream=None):
     """Scales `grads` (as in grad_norm) in place by min(1, max_norm / (norm + eps)) and returns norm, their
-    2-norm before, as grad_norm does; nothing is copied to the host.  With `out`, a tensor for each gradient (of
+    2-norm before, as grad_norm does; nothing is copied to the host.  A norm of infinity makes zeros of finite elements
+    and NaN of infinite ones, a max_norm of infinity scales nothing, and a NaN makes NaN of everything.  With `out`, a tensor for each gradient (of
     its shape and any of the three types; it may be the gradient itself), the gradients are left alone and the
     scaled ones go there.  No tensor that is written shares memory with another."""
     grads = list(grads)

@@ -204,3 +204,19 @@ def test_capture_in_graphs_that_share_memory():
         _check(oa, a, na.clone(), 1.0)
         gb.replay()
         _check(ob, b, nb.clone(), 2.0)
+
+
+@pytest.mark.parametrize("count", [2, 60, 250, 901])
+@pytest.mark.parametrize("n", [50, 40000])
+def test_a_largest_norm_of_infinity_with_an_infinite_element(count, n):
+    """Nothing is scaled, in place or into other tensors; a NaN makes NaN of everything all the same."""
+    torch, ops = _torch()
+    inf = float("inf")
+    g = _grads([n] + [5] * (count - 1), ALL, 1)
+    g[0][7], g[1][2] = inf, -inf
+    before = [t.clone() for t in g]
+    out = [torch.zeros(t.shape, device="cuda") for t in g]
+    assert ops.clip_grad_norm(g, inf, out=out) == inf and all(torch.equal(o, t.float()) for o, t in zip(out, before))
+    assert ops.clip_grad_norm(g, inf) == inf and all(torch.equal(t, b) for t, b in zip(g, before))
+    g[1][3] = float("nan")
+    assert ops.clip_grad_norm(g, inf).isnan() and all(t.isnan().all() for t in g)

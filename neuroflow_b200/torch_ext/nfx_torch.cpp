@@ -326,6 +326,12 @@ Tensor once(const char* fn, const Tensor& g) {
     if (!g.defined() || !at::GradMode::is_enabled()) return g;
     return OnceFn::apply(g, at::empty({0}, at::kFloat).requires_grad_(), std::string(fn));
 }
+// The same for a gradient whose memory is another one's too, the caller's or a second gradient: under create_graph a copy,
+// as in-place changes of what OnceFn hands on raise no other tensor's version.
+Tensor once_shared(const char* fn, const Tensor& g) {
+    if (!g.defined() || !at::GradMode::is_enabled()) return g;
+    return once(fn, g.detach().clone());
+}
 
 struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
     static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const OptTensor& gamma, const OptTensor& beta,

@@ -416,7 +416,7 @@ struct RmsNormFn : torch::autograd::Function<RmsNormFn> {
         const int64_t needs = ctx->saved_data["needs"].toInt();
         const Tensor dy = grads[0], ds = grads.size() > 1 ? grads[1] : Tensor();
         if (!dy.defined()) {  // only the sum is used: its gradient is that of both terms
-            const auto as = [&](bool need, at::ScalarType t) { return need && ds.defined() ? once(fn, ds.to(t)) : Tensor(); };
+            const auto as = [&](bool need, at::ScalarType t) { return need && ds.defined() ? once_shared(fn, ds.to(t)) : Tensor(); };
             return {as(needs & 1, static_cast<at::ScalarType>(ctx->saved_data["xtype"].toInt())), Tensor(), Tensor(),
                     as(needs & 4, ds.defined() ? ds.scalar_type() : at::kFloat)};
         }
@@ -424,7 +424,7 @@ struct RmsNormFn : torch::autograd::Function<RmsNormFn> {
                                       ds.defined() ? OptTensor(ds.contiguous()) : std::nullopt, (needs & 2) != 0, (needs & 1) != 0,
                                       (needs & 4) != 0);
         return {needs & 1 ? once(fn, g.dx) : Tensor(), needs & 2 ? once(fn, g.dgamma) : Tensor(), Tensor(),
-                needs & 4 ? once(fn, g.dres) : Tensor()};
+                needs & 4 ? ((needs & 1) && g.dres.is_same(g.dx) ? once_shared(fn, g.dres) : once(fn, g.dres)) : Tensor()};
     }
 };
 
@@ -471,7 +471,7 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
                 dx = plain_product(matrix_of(fn, "dy", g.dz, type), transposed(matrix_of(fn, "weight", saved[1], type)), type, sizes, dy);
             }
         }
-        return {once(fn, dx), once(fn, dw), once(fn, db), Tensor(), needs & 8 ? once(fn, grads[0]) : Tensor(), Tensor()};
+        return {once(fn, dx), once(fn, dw), once(fn, db), Tensor(), needs & 8 ? once_shared(fn, grads[0]) : Tensor(), Tensor()};
     }
 };
 

@@ -300,6 +300,11 @@ Tensor fp8_gemm(const Tensor& ac, const Tensor& as, bool a_tile, const Tensor& b
 }
 
 // ---- autograd -----------------------------------------------------------------------------------
+// A result in other sizes, no view to autograd: it may be changed in place.
+Tensor in_sizes(const Tensor& t, at::IntArrayRef sizes) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return t.view(sizes);
+}
 OptTensor defined(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
 
 // A tangent of forward mode (a tensor has one whether or not it requires grad) would be dropped.
@@ -369,7 +374,7 @@ struct Fp8LinearFn : torch::autograd::Function<Fp8LinearFn> {
                                                         b ? static_cast<int64_t>(b->scalar_type()) : 0};
         auto sizes = x.sizes().vec();
         sizes.back() = w.size(0);
-        return fp8_gemm(xq.q.codes, xq.q.scales, false, wq.q.codes, wq.q.scales, true, b, 0, x.scalar_type(), std::nullopt).view(sizes);
+        return in_sizes(fp8_gemm(xq.q.codes, xq.q.scales, false, wq.q.codes, wq.q.scales, true, b, 0, x.scalar_type(), std::nullopt), sizes);
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
         const auto saved = ctx->get_saved_variables();
@@ -407,7 +412,7 @@ Tensor fp8_linear(const Tensor& x, const Tensor& w, const OptTensor& b) {
     const Quantised xq = fp8_quantise(x, false, false, false), wq = fp8_quantise(w, true, false, false);
     auto sizes = x.sizes().vec();
     sizes.back() = w.size(0);
-    return fp8_gemm(xq.q.codes, xq.q.scales, false, wq.q.codes, wq.q.scales, true, b, 0, x.scalar_type(), std::nullopt).view(sizes);
+    return in_sizes(fp8_gemm(xq.q.codes, xq.q.scales, false, wq.q.codes, wq.q.scales, true, b, 0, x.scalar_type(), std::nullopt), sizes);
 }
 
 #include "nfx_torch_dense.h"

@@ -444,7 +444,7 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
         if (x.dim() == 2) return p.c;
         auto sizes = x.sizes().vec();
         sizes.back() = w.size(0);
-        return p.c.view(sizes);
+        return in_sizes(p.c, sizes);
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
         const char* fn = "linear";
@@ -496,9 +496,8 @@ Tensor linear(const Tensor& x, const Tensor& w, const OptTensor& b, int64_t act,
     if (at::GradMode::is_enabled() &&
         (x.requires_grad() || w.requires_grad() || (b && b->requires_grad()) || (residual && residual->requires_grad())))
         return LinearFn::apply(x, w, b, act, residual, flat(x, w.size(1)));
-    return gemm(fn, flat(x, w.size(1)), w, b, act, residual ? OptTensor(flat(*residual, w.size(0))) : std::nullopt, std::nullopt, std::nullopt,
-                false)
-        .c.view(sizes);
+    const OptTensor r2 = residual ? OptTensor(flat(*residual, w.size(0))) : std::nullopt;
+    return in_sizes(gemm(fn, flat(x, w.size(1)), w, b, act, r2, std::nullopt, std::nullopt, false).c, sizes);
 }
 
 void dense_defs(py::module_& m) {

@@ -494,11 +494,12 @@ int nfx_act_backward(const void* dy, int64_t lddy, const void* z, int64_t ldz, i
  *   norm = sqrt(sum g^2),  out = g min(1, max_norm / (norm + eps)).
  * The four (six) arrays are in HOST memory and read before the call returns: tensor i has counts[i]
  * elements of types[i] at the DEVICE address grads[i], and goes to out[i] of out_types[i]; out NULL: in
- * place.  Any alignment, sizes and number of tensors.  Sums of squares are 64-bit numbers; `norm` (one
- * float on the device) is rounded to fp32.  out[i] may be grads[i] of the same type; beyond that no
- * output shares memory with another tensor.  A norm of infinity gives zeros, and NaN where an element is
- * infinite, but with a max_norm of infinity nothing is scaled; a NaN gives NaN everywhere.  The workspace is 16-byte aligned, of nfx_grad_norm_workspace
- * bytes. */
+ * place.  Any alignment, sizes and number of tensors.  Groups of up to 32 squares (16 of fp32 elements) are
+ * added in fp32, or in 64 bits where that would over- or underflow, and the groups in 64 bits; `norm` (one
+ * float on the device) is rounded to fp32.  out[i] may be grads[i] of the same type; beyond that no output
+ * shares memory with another tensor.  A norm of infinity gives zeros, and NaN where an element is infinite,
+ * but with a max_norm of infinity nothing is scaled; a NaN gives NaN everywhere.  The workspace is 16-byte
+ * aligned, of nfx_grad_norm_workspace bytes. */
 int64_t nfx_grad_norm_workspace(int64_t tensors);
 int nfx_grad_norm(const void* const* grads, const int64_t* counts, const int* types, int64_t tensors, float* norm,
                   void* workspace, int64_t workspace_bytes, void* stream);

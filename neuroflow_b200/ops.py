@@ -218,7 +218,8 @@ def act_backward(dy, z, act, bias_dtype=None, stream=None):
 def grad_norm(grads, stream=None):
     """The 2-norm over all elements of the tensors `grads` (one device; float32, bfloat16 and float16 may be
     mixed; contiguous, or permutations of contiguous tensors): a float32 tensor without dimensions, on the
-    device.  Squares are summed in 64 bits."""
+    device.  Groups of up to 32 squares (16 of float32 elements) are added in fp32, or in 64 bits where that would
+    over- or underflow, and the groups in 64 bits."""
     grads = list(grads)
     if stream is not None and grads:
         with _on(stream, *grads):

@@ -220,3 +220,15 @@ def test_a_largest_norm_of_infinity_with_an_infinite_element(count, n):
     assert ops.clip_grad_norm(g, inf) == inf and all(torch.equal(t, b) for t, b in zip(g, before))
     g[1][3] = float("nan")
     assert ops.clip_grad_norm(g, inf).isnan() and all(t.isnan().all() for t in g)
+
+
+@pytest.mark.parametrize("dtype,group", [("float32", 16), ("bfloat16", 32), ("float16", 32)])
+@pytest.mark.parametrize("sizes", [[33], [5000] * 7, [1 << 20, 3]])
+def test_norm_within_what_a_group_of_squares_loses(sizes, dtype, group):
+    """A group's additions are off by 2^-24 of its sum each at most; the groups, positive all of them, are added in 64 bits, so
+    the sum of squares is off by group 2^-24 of itself, the norm by half of that and its rounding to fp32."""
+    torch, ops = _torch()
+    for size in (1.0, 1e-3, 300.0):
+        g = _grads(sizes, (dtype,), group, size)
+        want = _norm(g)
+        assert abs(float(ops.grad_norm(g)) - want) <= (group / 2 + 1) * 2.0 ** -24 * want

@@ -38,8 +38,8 @@ __device__ __forceinline__ float2 slope2(float2 z, int act) {
 // A warp takes 32 VE columns (by 16-byte words; single ones, four a lane, where rows are not aligned to them) of every
 // eighth row of the block's share, the next row on its way while one is worked on; the columns' sums stay in
 // registers and are joined over the block's warps at the end.  16384x4096 bf16 with GELU and the bias gradient:
-// 70 us, 5.8 TB/s (two rows at a time without a next one 88 us, with one, which spills, 104); 4095x2048: 12.8 us, of
-// which joining the shares takes 2.6.
+// 70 us, 5.8 TB/s (two rows at a time without a next one 88 us, with one, which spills, 104); 16384x4095, by single
+// elements, 103 us; 4095x2048: 12.8 us, of which joining the shares takes 2.6.
 constexpr int kWarps = 8;
 
 template <typename T, int VE, int VPT>

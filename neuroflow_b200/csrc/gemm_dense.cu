@@ -14,13 +14,15 @@
 //
 // Measured (one B200, 1,644 TFLOP/s for a library product of 8192^3 in a burst, 1,355 over seconds; graphs of launches over
 // operands that do not fit L2, a few milliseconds long):
-//   8192x16384x4096 bf16, bias and GELU   704 us, 1,562 TFLOP/s; in a loop of seconds the 1,000 W power cap sets the clock:
-//                                         830 to 866 us, 1,270 to 1,330 TFLOP/s.  A block of K takes some 670 cycles where
-//                                         its MMAs take 512: 32 KB a block are 49 bytes a cycle and SM from L2
-//   4096x2048x8192 to fp32                101 us, 1,362 TFLOP/s: 128 tiles on 74 pairs; both operands MN-major
-//   4096x4096x4096                        98 us, 1,409 TFLOP/s;   2048x2048x2048   16.8 us, 1,020 TFLOP/s
-//   512x4096x4096                         19.7 us (K split over two pairs; 22.7 narrow, 25.7 pairs alone)
-//   64x4096x4096                          11.7 us, 2.9 TB/s of weights;   1024x1024x1024   9.4 to 9.8 us
+//   8192x16384x4096 bf16, bias and GELU   705 to 730 us, 1,510 to 1,560 TFLOP/s; call after call for seconds, as the 1,000 W
+//                                         power cap sets the clock, 830 us, 1,325 TFLOP/s.  A block of K takes some 670 cycles
+//                                         where its MMAs take 512: 32 KB a block are 49 bytes a cycle and SM from L2
+//   4096x2048x8192 to fp32                101 us, 1,362 TFLOP/s; call after call 117 us, 1,174 TFLOP/s: 128 tiles on 74 pairs;
+//                                         both operands MN-major
+//   4096x4096x4096                        98 us, 1,405 TFLOP/s;   2048x2048x2048   17.1 us, 1,005 TFLOP/s
+//   512x4096x4096                         19.9 us (K split over two pairs; 22.7 narrow, 25.7 pairs alone)
+//   17, 64, 128, 256 x4096x4096           11.0, 11.8, 12.7, 16.1 us, 3.1 to 2.3 TB/s: 5 us before the first block of K
+//   1024x1024x1024                        9.8 us
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -497,7 +499,8 @@ constexpr int kSplitThreads = 32 * (kPairEpi + 2);
 constexpr int kSplitSmem = kOffOut + 8 * (2 * kStages + 2 * 2) + 16 + 1024;
 static_assert(128 * 256 * 4 <= kOffOut, "the partial sums take the place of the operands");
 
-// W columns of a row, from column n on: acc += or = what lies in `mat`, or the other way round.
+// W columns of a row, from column n on, element `at` of `mat` being the first: stored there (row_store) or added to v
+// (row_add).  `vec`: rows start on 16-byte boundaries.
 template <int CT, int W>
 __device__ __forceinline__ void row_store(void* mat, int64_t at, bool vec, int n, int N, const float (&v)[W]) {
     constexpr int kEl = CT == kF32 ? 4 : 2, kVec = 16 / kEl;
@@ -1074,8 +1077,8 @@ cudaError_t dispatch(const GemmDenseArgs& p, float* sums, cudaStream_t stream) {
 }
 
 // ---------------------------------------------------------------------------------------------------------
-// Operands that TMA cannot read (base or row stride no multiple of 16 bytes) are copied first, rows on 16-byte
-// boundaries.
+// Operands that TMA cannot read (base or row stride no multiple of 16 bytes) are copied first, rows on the boundaries
+// that copy_stride() gives.
 // ---------------------------------------------------------------------------------------------------------
 struct AlignJob {
     const uint16_t* src;

@@ -266,6 +266,7 @@ def rms_norm_autograd(x, gamma=None, eps=1e-5, residual=None):
 def linear(x, weight, bias=None, act=0, residual=None):
     """act(x weight^T + bias) + residual, differentiable: x (..., K) and weight (N, K) both bfloat16 or both
     float16, bias (N,) of any type, residual and result (..., N) of x's type.  Gradients come in the types of
-    their tensors, sums in fp32; with an activation dz = dy act'(z) is rounded to x's type in between.  Once,
-    as fp8_linear."""
+    their tensors, sums in fp32; with an activation dz = dy act'(z) is rounded to x's type in between, as is the z
+    that is kept for it (gemm with preact and out_dtype float32, and act_backward, keep both in fp32).  Once, as
+    fp8_linear."""
     return _ext.linear(x, weight, bias, act, residual)

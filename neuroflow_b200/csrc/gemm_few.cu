@@ -16,7 +16,7 @@
 // order through shared memory, where a warp also adds up the pieces of a long K (piece_terms()).
 //
 // Measured (one B200, weights from HBM): 1x4096x4096 8.1 to 8.4 us, 4.1 TB/s (narrow kernel 10.0), 1x4096x16384 23 us, 5.8 TB/s,
-// 16x4096x4096 9.8 us, 1x1024x1024 2.3 us (4.3), 1x64x64 1.7 us.  Small ones are bound by the launch and one trip to
+// 16x4096x4096 9.8 us, 1x1024x1024 2.4 us (4.3), 1x64x64 1.6 us.  Small ones are bound by the launch and one trip to
 // memory, large ones by HBM.
 #include <cuda_runtime.h>
 
@@ -56,13 +56,18 @@ struct Few {
     static constexpr int kOut = kRows * kCols;
     static constexpr int kPart = KMAJOR ? kOut : kRows * 66;  // a warp's sums
     static constexpr int kSmem = (kWarps * kPart + kOut) * 4;
+    // turns of a warp's loop to a piece of K
+    template <int CT>
+    __host__ __device__ static constexpr int turns() { return piece_terms(CT) / ((KMAJOR ? 32 : 16) * kU); }
     // where the sum of row m of A and row n of B is among a warp's: a warp's lanes, and 32 columns, lie in unlike banks
     __device__ static constexpr int place(int m, int n) {
-        return KMAJOR ? m * kCols + (kCols > 16 ? n ^ ((m & 6) << 2) : n) : m * 66 + n + (n >> 5);
+        return KMAJOR ? m * kCols + (NT > 1 ? n ^ ((m & 6) << 2) : n) : m * 66 + n + (n >> 5);
     }
 };
 
-template <typename T, int CT, bool KMAJOR, bool VEC, int NT>
+// LONG: a warp may have more than one piece of K.  Ordinary lengths go without the loop and the sums for that (1x64x64: 1.6 us,
+// 1.75 with them; 8x1023x1023 3.8, 4.1), save for the widest form, where that makes no difference.
+template <typename T, int CT, bool KMAJOR, bool VEC, int NT, bool LONG>
 __global__ void __launch_bounds__(kThreads, 2) gemm_few_kernel(const GemmDenseArgs p, const int split) {
     using F = Few<KMAJOR, VEC, NT>;
     constexpr int kCols = F::kCols, kOut = F::kOut, kPart = F::kPart, kU = F::kU, kMT = F::kMT;
@@ -81,8 +86,7 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_few_kernel(const GemmDenseAr
     const int which = rank == split - 1 ? kWarps - 1 - warp : 3;
     const bool by_elements = which == 0 ? p.K % kStep != 0 : (!VEC && which < 3 && steps >= which);
     const int64_t arow = p.lda;
-    constexpr int kTurns = piece_terms(CT) / (kStep * kU);  // turns of a warp's loop to a piece of K
-    float* mine = part + warp * kPart;
+    constexpr int kTurns = F::template turns<CT>();
 
     grid_dep_launch();
     grid_dep_wait();  // what the kernel before this one wrote may be read from here on
@@ -110,6 +114,7 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_few_kernel(const GemmDenseAr
                 }
         };
         const auto put = [&](auto add) {  // to this lane's places
+            float* mine = part + warp * kPart;
 #pragma unroll
             for (int i = 0; i < kMT; ++i)
 #pragma unroll
@@ -118,13 +123,13 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_few_kernel(const GemmDenseAr
                     for (int e = 0; e < 4; ++e) {
                         float& m = mine[F::place(j * 8 + 2 * t + (e & 1), i * 16 + g + 8 * (e >> 1))];
                         m = add ? m + c[i][j][e] : c[i][j][e];
-                        c[i][j][e] = 0.0f;
+                        if (LONG) c[i][j][e] = 0.0f;
                     }
         };
         int s = s0 + warp;
         bool first = true;
         for (;;) {
-            const int end = min(s1, s + kWarps * kU * kTurns);
+            const int end = LONG ? min(s1, s + kWarps * kU * kTurns) : s1;
             for (; s < end; s += kWarps * kU) {
                 uint32_t wb[kU][2 * kMT][4], wa[kU][NT][4];
 #pragma unroll
@@ -141,7 +146,7 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_few_kernel(const GemmDenseAr
                 for (int u = 0; u < kU; ++u)
                     if (s + u * kWarps < s1) step(wb[u], wa[u]);
             }
-            if (s >= s1) [[likely]] break;
+            if (!LONG || s >= s1) [[likely]] break;
             if (first) put(std::false_type{});
             else put(std::true_type{});
             first = false;
@@ -155,7 +160,7 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_few_kernel(const GemmDenseAr
             for (int j = 0; j < NT; ++j) load_single<8>(ar[j], k, p.K, wa[j]);
             step(wb, wa);
         }
-        if (first) [[likely]] put(std::false_type{});
+        if (!LONG || first) [[likely]] put(std::false_type{});
         else put(std::true_type{});
     } else {
         float c[8][4];
@@ -177,19 +182,20 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_few_kernel(const GemmDenseAr
             }
         };
         const auto put = [&](auto add) {
+            float* mine = part + warp * kPart;
 #pragma unroll
             for (int j = 0; j < 8; ++j)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     float& m = mine[F::place(g + 8 * (i >> 1), (2 * t + (i & 1)) * 8 + j)];
                     m = add ? m + c[j][i] : c[j][i];
-                    c[j][i] = 0.0f;
+                    if (LONG) c[j][i] = 0.0f;
                 }
         };
         int s = s0 + warp;
         bool first = true;
         for (;;) {
-            const int end = min(s1, s + kWarps * kU * kTurns);
+            const int end = LONG ? min(s1, s + kWarps * kU * kTurns) : s1;
             for (; s < end; s += kWarps * kU) {
                 uint32_t wb[kU][4][4], wa[kU][2][2];
 #pragma unroll
@@ -213,7 +219,7 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_few_kernel(const GemmDenseAr
                 for (int u = 0; u < kU; ++u)
                     if (s + u * kWarps < s1) step(wb[u], wa[u]);
             }
-            if (s >= s1) [[likely]] break;
+            if (!LONG || s >= s1) [[likely]] break;
             if (first) put(std::false_type{});
             else put(std::true_type{});
             first = false;
@@ -230,7 +236,7 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_few_kernel(const GemmDenseAr
             for (int h = 0; h < 2; ++h) load_single<4>(ar[h], k, p.K, wa[h]);
             step(wb, wa);
         }
-        if (first) [[likely]] put(std::false_type{});
+        if (!LONG || first) [[likely]] put(std::false_type{});
         else put(std::true_type{});
     }
     __syncthreads();
@@ -274,7 +280,10 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_few_kernel(const GemmDenseAr
 
 template <typename T, int CT, bool KMAJOR, bool VEC, int NT>
 cudaError_t few_go(const GemmDenseArgs& p, int split, cudaStream_t s) {
-    auto kern = gemm_few_kernel<T, CT, KMAJOR, VEC, NT>;
+    using F = Few<KMAJOR, VEC, NT>;
+    // (a block has at most one step more than this, a warp then at most turns() turns)
+    const bool more = NT == 4 || p.K / (KMAJOR ? 32 : 16) / split >= kWarps * F::kU * F::template turns<CT>();
+    auto kern = more ? gemm_few_kernel<T, CT, KMAJOR, VEC, NT, true> : gemm_few_kernel<T, CT, KMAJOR, VEC, NT, NT == 4>;
     constexpr int kSmem = Few<KMAJOR, VEC, NT>::kSmem;
     const cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), kSmem);
     if (e != cudaSuccess) return e;

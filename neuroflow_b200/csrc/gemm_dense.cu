@@ -257,7 +257,8 @@ __device__ __forceinline__ void load_stage(const GemmDenseArgs& p, const CUtenso
     load_half(tmB, st + 16384, bar, p.b_t, n, r.b[rank], k);
 }
 
-template <int CT>
+// LONG: K has more than one piece (5765x1016x192 with GELU: 13.4 us, 13.9 where the epilogue may have to add).
+template <int CT, bool LONG>
 __global__ void __launch_bounds__(kPairThreads, 1)
 gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmC,
                  const __grid_constant__ CUtensorMap tmZ, const __grid_constant__ CUtensorMap tmR, const GemmDenseArgs p, const Epi e,
@@ -279,8 +280,8 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     const int tiles = tm * tn;
     const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
     const int KB = (p.K + kBK - 1) / kBK;
-    constexpr int piece = kPiece<CT>;
-    const int pieces = (KB + piece - 1) / piece;
+    const int piece = LONG ? kPiece<CT> : KB;
+    const int pieces = LONG ? (KB + piece - 1) / piece : min(KB, 1);
     const uint64_t budget = p.wait_ns ? p.wait_ns : kWaitNs;
 
     if (threadIdx.x == 0) {
@@ -412,7 +413,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
                         __syncwarp();
                         if (lane == 0) mbar_arrive_cluster(accEmpty0 + st * 8);
                     }
-                    if (CT != kF32 && i == 0) {  // (most often the only one)
+                    if (!LONG || (CT != kF32 && i == 0)) {
 #pragma unroll
                         for (int j = 0; j < 16; ++j) acc[c * 16 + j] = make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
                     } else {
@@ -481,7 +482,7 @@ cudaError_t launch_pair(const GemmDenseArgs& p, cudaStream_t stream) {
         return !*on || encode_2d(tm, map_type(CT), m, p.N, p.M, pitch(ld) * kEl, 128 / kEl, 32, 128);
     };
     if (!map(&tmC, p.C, p.ldc, &e.tma_c) || !map(&tmZ, p.Z, p.ldz, &e.tma_z) || !map(&tmR, p.res, p.ldres, &e.tma_r)) return cudaErrorInvalidValue;
-    auto kern = gemm_pair_kernel<CT>;
+    auto kern = CT == kF32 || p.K > piece_terms(CT) ? gemm_pair_kernel<CT, true> : gemm_pair_kernel<CT, CT == kF32>;
     const cudaError_t err = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), kPairSmem);
     if (err != cudaSuccess) return err;
     const int64_t tiles = static_cast<int64_t>((p.M + 255) / 256) * ((p.N + 255) / 256);
